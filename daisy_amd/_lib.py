@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
+from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 from typing import Optional
 
 import torch
@@ -16,9 +16,11 @@ import torch
 _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "csrc", "libdaisy_hip.so")
 _lib: Optional[ctypes.CDLL] = None
 
-ABI_VERSION = 5
+ABI_VERSION = 6
 LINEAR_MAX_ROWS = 8
 STATUS_POSITION_PAST_TABLES = 1
+STATUS_LENGTH_PAST_PAGES = 2
+STATUS_PAGE_OUT_OF_RANGE = 4
 DECODE_STATIC_SCRATCH_BYTES = 4 << 20
 
 _I64P = POINTER(c_int64)
@@ -152,6 +154,28 @@ SIGNATURES = {
         c_void_p, c_void_p, c_void_p, c_int, c_void_p,          # cos, sin, pos0 (device int32), table_rows, status
         c_void_p, _I64P, c_void_p, _I64P, c_void_p, _I64P,         # q_out, k_out, v_out (+ strides)
         c_int, c_int, c_int, c_int, c_float, c_void_p]),        # B, T, H, D, eps, stream
+    "daisy_paged_append_fwd": (c_int, [
+        c_void_p, _I64P, c_void_p, _I64P, c_void_p, _I64P, c_int,  # q, k, v (+ strides), inputs are fp16
+        c_void_p, _I64P, c_void_p,                              # ve, ve strides, gate
+        c_void_p, c_void_p, c_int,                              # cos, sin, table_rows
+        c_void_p, _I64P, c_void_p, _I64P, c_int,                # k_pages, v_pages (+ strides), cache is fp16
+        c_void_p, c_int64, c_int, c_int, c_int, c_int,          # page_table (+ row stride), n_seq, max_pages, num_pages, page_size
+        c_void_p, c_void_p,                                     # positions, rows
+        c_void_p, _I64P, c_void_p, _I64P, c_void_p, _I64P, c_int,  # q_out, k_out, v_out (+ strides), zero_skipped
+        c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p]),  # N, Hq, H, D, eps, status, stream
+    "daisy_paged_attn_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
+    "daisy_paged_attn_fwd": (c_int, [
+        c_void_p, _I64P, c_void_p, _I64P, c_void_p, _I64P, c_int,  # q, k_pages, v_pages (+ strides), cache is fp16
+        c_void_p, c_int64, c_int, c_int, c_int, c_void_p,       # page_table (+ row stride), max_pages, num_pages, page_size, lens
+        c_void_p, _I64P,                                        # o (+ strides)
+        c_int, c_int, c_int, c_int, c_int, c_float, c_void_p,   # B, Hq, H, D, window, scale, status
+        c_void_p, c_size_t, c_void_p]),                         # workspace, bytes, stream
+    "daisy_logits_process_fwd": (c_int, [
+        c_void_p, c_int64, c_void_p, c_int64, c_int,            # x, y (+ row strides), type
+        c_void_p, c_int64, c_int, c_void_p, c_int, c_int,       # history (+ row stride), is int64, history_lens, T, lookback
+        c_void_p, c_double, c_void_p, c_float, c_void_p, c_float, c_float, c_float,  # repetition, presence, frequency (rows, number), half_life, cap
+        c_void_p, c_int64, c_void_p, c_int64,                   # bias, allowed (+ row strides)
+        c_int, c_int, c_void_p]),                               # B, V, stream
 }
 
 

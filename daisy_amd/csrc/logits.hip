@@ -1,0 +1,192 @@
+// Penalties for repeated tokens, biases and grammar masks on the logits of a batch (gfx950), in one pass.
+//
+// Row b with logits x[V], the last `lookback` tokens h of its history (age 1 is the newest), for every token v:
+//   n = #{j: h_j = v},  w = sum over those j of 2^(-age_j / half_life)  (of 1 without a half life),  s = r^min(w, cap)
+//   y = (x > 0 ? x / s : x s) - f n - p [n > 0] + bias[v],  and -inf where the mask's bit of v is clear.
+// Fp32 throughout, rounded once.  r, f and p are numbers or one per row.
+//
+// A workgroup takes a slice of one row's vocabulary, a word of 64 bits of the LDS for each of its tokens: it reads the history, adds one to
+// the count (17 bits) and the weight to the sum (17 + 30 bits) of every token of its slice in one integer atomic, so that the result
+// does not depend on the order, and then goes over the logits, which it has asked for before.
+#include "common.h"
+
+#include <math.h>
+
+namespace daisy {
+
+enum LogitsType { kLogitsF32 = 0, kLogitsBf16 = 1, kLogitsF16 = 2 };
+constexpr int kWeightBits = 30, kCountShift = 47;      // a weight of one is 2^30; 2^17 - 1 of them stay below the count
+constexpr int kMostHistory = (1 << 17) - 1;
+constexpr int kPerThread = 8;
+
+struct RowSetting { float value; const float* rows; };
+__device__ __forceinline__ float setting(const RowSetting& s, int b) { return s.rows != nullptr ? s.rows[b] : s.value; }
+
+struct LogitsParams {
+  const void* x; int64_t x_st;
+  void* y; int64_t y_st;
+  const void* history; int64_t h_st; const int32_t* lens; int T, lookback;
+  RowSetting repetition, presence, frequency;      // (the number `repetition` as its logarithm to base 2)
+  float inv_half_life, cap;
+  const float* bias; int64_t bias_st;
+  const uint32_t* allowed; int64_t allowed_st;
+  int V, slice;
+};
+
+// Four values of a row from element v on, where nothing but the elements' own alignment is known; `full`: all four are there.
+typedef float f32x4_near __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint16_t u16x4_near __attribute__((ext_vector_type(4), aligned(2)));
+template <int E> __device__ __forceinline__ float widen(uint16_t u) {
+  if constexpr (E == kLogitsBf16) return bf16lo_to_f32(u);
+  else return (float)__builtin_bit_cast(_Float16, u);
+}
+template <int E> __device__ __forceinline__ uint16_t narrow(float f) {
+  if constexpr (E == kLogitsBf16) return (uint16_t)(pack_bf16x2(f, 0.f) & 0xffffu);
+  else return __builtin_bit_cast(uint16_t, (_Float16)f);
+}
+template <int E> __device__ __forceinline__ f32x4 load4(const void* row, int v, int left) {
+  f32x4 f = {0.f, 0.f, 0.f, 0.f};
+  if constexpr (E == kLogitsF32) {
+    const float* at = (const float*)row + v;
+    if (left >= 4) return __builtin_nontemporal_load((const f32x4_near*)at);
+    for (int i = 0; i < left; ++i) f[i] = at[i];
+  } else {
+    const uint16_t* at = (const uint16_t*)row + v;
+    if (left >= 4) {
+      const u16x4_near u = __builtin_nontemporal_load((const u16x4_near*)at);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = widen<E>(u[i]);
+      return f;
+    }
+    for (int i = 0; i < left; ++i) f[i] = widen<E>(at[i]);
+  }
+  return f;
+}
+template <int E> __device__ __forceinline__ void store4(void* row, int v, int left, const f32x4& f) {
+  if constexpr (E == kLogitsF32) {
+    float* at = (float*)row + v;
+    if (left >= 4) __builtin_nontemporal_store((f32x4_near)f, (f32x4_near*)at);
+    else for (int i = 0; i < left; ++i) at[i] = f[i];
+  } else {
+    uint16_t* at = (uint16_t*)row + v;
+    if (left >= 4) {
+      u16x4_near u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) u[i] = narrow<E>(f[i]);
+      __builtin_nontemporal_store(u, (u16x4_near*)at);
+    } else {
+      for (int i = 0; i < left; ++i) at[i] = narrow<E>(f[i]);
+    }
+  }
+}
+
+template <int E, bool HISTORY, typename TOKEN>
+__global__ __launch_bounds__(1024) void logits_kernel(LogitsParams p) {
+  extern __shared__ uint64_t seen[];      // [slice]
+  const int b = blockIdx.y, tid = threadIdx.x, threads = blockDim.x;
+  const int v0 = blockIdx.x * p.slice, v1 = min(v0 + p.slice, p.V);
+  constexpr int ROUNDS = kPerThread / 4;
+  const char* x_row = (const char*)p.x + b * p.x_st * (E == kLogitsF32 ? 4 : 2);
+  char* y_row = (char*)p.y + b * p.y_st * (E == kLogitsF32 ? 4 : 2);
+  f32x4 x[ROUNDS];
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r) {
+    const int v = v0 + 4 * (tid + r * threads);
+    x[r] = load4<E>(x_row, v, v1 - v);
+  }
+  float lg = 0.f, presence = 0.f, frequency = 0.f;
+  if constexpr (HISTORY) {
+    for (int i = tid; i < p.slice; i += threads) seen[i] = 0;
+    lg = p.repetition.rows != nullptr ? log2f(p.repetition.rows[b]) : p.repetition.value;
+    presence = setting(p.presence, b);
+    frequency = setting(p.frequency, b);
+    const int n = p.lens != nullptr ? min(max(p.lens[b], 0), p.T) : p.T;
+    const TOKEN* history = (const TOKEN*)p.history + b * p.h_st;
+    __syncthreads();
+    for (int j = max(n - p.lookback, 0) + tid; j < n; j += threads) {
+      const TOKEN token = history[j];
+      if (token < (TOKEN)v0 || token >= (TOKEN)v1) continue;      // another slice's, or no token at all
+      const float weight = fast_exp2((float)(j - n) * p.inv_half_life);
+      const uint64_t add = ((uint64_t)1 << kCountShift) + (uint32_t)(weight * (float)(1u << kWeightBits) + 0.5f);
+      __hip_atomic_fetch_add(&seen[(int)token - v0], add, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r) {
+    const int v = v0 + 4 * (tid + r * threads), left = v1 - v;
+    if (left <= 0) break;
+    if constexpr (HISTORY) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint64_t s = seen[v - v0 + i];
+        if (s == 0) continue;
+        const float w = (float)(s & (((uint64_t)1 << kCountShift) - 1)) * (1.f / (float)(1u << kWeightBits));
+        const float power = fminf(w, p.cap) * lg;
+        x[r][i] *= fast_exp2(x[r][i] > 0.f ? -power : power);
+        x[r][i] -= fmaf(frequency, (float)(uint32_t)(s >> kCountShift), presence);
+      }
+    }
+    if (p.bias != nullptr) {
+      const float* at = p.bias + b * p.bias_st + v;
+      if (left >= 4) x[r] += *(const f32x4_near*)at;
+      else for (int i = 0; i < left; ++i) x[r][i] += at[i];
+    }
+    if (p.allowed != nullptr) {
+      const uint32_t bits = p.allowed[b * p.allowed_st + (v >> 5)] >> (v & 31);      // (v is a multiple of 4)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[r][i] = (bits >> i) & 1 ? x[r][i] : -__builtin_inff();
+    }
+    store4<E>(y_row, v, left, x[r]);
+  }
+}
+
+template <int E> static void logits_launch(const LogitsParams& p, bool tokens64, dim3 grid, int threads, hipStream_t s) {
+  const size_t lds = p.history ? (size_t)p.slice * sizeof(uint64_t) : 0;
+  if (!p.history) hipLaunchKernelGGL((logits_kernel<E, false, int32_t>), grid, dim3(threads), 0, s, p);
+  else if (tokens64) hipLaunchKernelGGL((logits_kernel<E, true, int64_t>), grid, dim3(threads), lds, s, p);
+  else hipLaunchKernelGGL((logits_kernel<E, true, int32_t>), grid, dim3(threads), lds, s, p);
+}
+
+}  // namespace daisy
+
+using namespace daisy;
+
+extern "C" int daisy_logits_process_fwd(const void* x, int64_t x_stride, void* y, int64_t y_stride, int type,
+                                        const void* history, int64_t history_stride, int history_is_int64, const int32_t* history_lens, int T, int lookback,
+                                        const float* repetition_rows, double repetition, const float* presence_rows, float presence,
+                                        const float* frequency_rows, float frequency, float half_life, float cap,
+                                        const float* bias, int64_t bias_stride, const int32_t* allowed, int64_t allowed_stride,
+                                        int B, int V, void* stream) {
+  DAISY_CHECK_ARG(x && y && B > 0 && V > 0 && B <= 65535 && V < (1 << 30), "logits_process: x and y must be non-NULL, B=%d (at most 65535), V=%d positive", B, V);
+  DAISY_CHECK_SUPPORTED(type >= 0 && type <= 2, "logits_process: type %d not supported (0 fp32, 1 bf16, 2 fp16)", type);
+  DAISY_CHECK_ARG(x_stride >= 0 && y_stride >= V * (B > 1), "logits_process: rows of y must not overlap");
+  DAISY_CHECK_ARG(!history || (T >= 0 && lookback >= 0), "logits_process: T=%d, lookback=%d must not be negative", T, lookback);
+  DAISY_CHECK_ARG(repetition_rows || repetition > 0.0, "logits_process: repetition must be positive");
+  DAISY_CHECK_ARG(half_life >= 0.f && cap >= 0.f, "logits_process: half_life and cap must not be negative");
+  if (history && (T == 0 || lookback == 0)) history = nullptr;
+  if (lookback > T) lookback = T;
+  DAISY_CHECK_SUPPORTED(!history || lookback <= kMostHistory, "logits_process: a history of %d tokens is too long (at most %d are counted)", lookback, kMostHistory);
+  const int elem = type == kLogitsF32 ? 4 : 2;
+  DAISY_CHECK_ARG((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) % elem == 0 && (reinterpret_cast<uintptr_t>(bias) & 3) == 0,
+                  "logits_process: tensors must be aligned to their elements");
+  LogitsParams p = {};
+  p.x = x; p.x_st = x_stride; p.y = y; p.y_st = y_stride;
+  p.history = history; p.h_st = history_stride; p.lens = history_lens; p.T = T; p.lookback = lookback;
+  // (from the caller's 64 bits: rounded to 32 first, a number near one is off by 2^-24 / (r - 1) of its logarithm, and that many times over
+  // where nothing caps the power)
+  p.repetition = {repetition_rows ? 0.f : (float)log2(repetition), repetition_rows}; p.presence = {presence, presence_rows}; p.frequency = {frequency, frequency_rows};
+  p.inv_half_life = half_life > 0.f ? 1.f / half_life : 0.f; p.cap = cap;
+  p.bias = bias; p.bias_st = bias_stride; p.allowed = (const uint32_t*)allowed; p.allowed_st = allowed_stride;
+  p.V = V;
+  int slice = 8192;
+  while (slice > 1024 && (int64_t)B * ((V + slice - 1) / slice) < 512) slice /= 2;
+  p.slice = slice;
+  const dim3 grid((unsigned)((V + slice - 1) / slice), (unsigned)B);
+  hipStream_t s = (hipStream_t)stream;
+  if (type == kLogitsF32) logits_launch<kLogitsF32>(p, history_is_int64, grid, slice / kPerThread, s);
+  else if (type == kLogitsBf16) logits_launch<kLogitsBf16>(p, history_is_int64, grid, slice / kPerThread, s);
+  else logits_launch<kLogitsF16>(p, history_is_int64, grid, slice / kPerThread, s);
+  DAISY_CHECK_LAUNCH("logits_kernel");
+  return DAISY_OK;
+}

@@ -1,0 +1,678 @@
+// A paged key-value cache: appending to it, and the attention of one new token per sequence over it (gfx950).
+//
+// The cache is a pool of pages, k and v [pages, H, page_size, D]; a page holds page_size consecutive positions of one
+// sequence, and row s of the page table names the pages of sequence s in order.  Sequences have lengths of their own, so
+// everything that depends on a length or a position is read from device memory when the kernels run: a launch can be recorded
+// once and replayed while sequences grow, come and go.
+#include "common.h"
+
+namespace daisy {
+
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+template <bool F16> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (F16) {
+    const f16x2 h = {(_Float16)a, (_Float16)b};
+    return __builtin_bit_cast(uint32_t, h);
+  } else {
+    return pack_bf16x2(a, b);
+  }
+}
+template <bool F16> __device__ __forceinline__ void unpack8_as(const u32x4& r, float* f) {
+  if constexpr (F16) {
+    const f16x8 h = __builtin_bit_cast(f16x8, r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = (float)h[i];
+  } else {
+    unpack8(r, f);
+  }
+}
+template <bool F16> __device__ __forceinline__ u32x4 pack8_as(const float* f) {
+  return u32x4{pack2<F16>(f[0], f[1]), pack2<F16>(f[2], f[3]), pack2<F16>(f[4], f[5]), pack2<F16>(f[6], f[7])};
+}
+
+__device__ __forceinline__ void raise_status(int32_t* status, int bit) {
+  if (status != nullptr) __hip_atomic_fetch_or(status, bit, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Append
+// ---------------------------------------------------------------------------------------------------------------
+// Per token and head:  x' = x rsqrt(mean(x^2) + eps) for q, k and v where a norm is wanted;
+//   q, k: y1 = x1 cos + x2 sin, y2 = x2 cos - x1 sin on the pairs (i, i + D/2), row `position` of the tables;  v = g v + (1 - g) ve.
+// All of it in fp32, rounded once as it is stored: pages and q in the cache's type, copies in the inputs'.
+struct AppendParams {
+  const uint16_t* in[3]; int64_t in_st[3], in_sh[3];     // q, k, v [N, heads, D]
+  const uint16_t* ve; int64_t e_st, e_sh; const float* gate;
+  const float* cos; const float* sin; int table_rows;
+  uint16_t* pages[2]; int64_t sp[2], sh[2], ss[2];       // k, v [pages, H, page_size, D]
+  const int32_t* table; int64_t table_st; int seqs, max_pages, num_pages, page_size;
+  const int32_t* positions; const int32_t* rows;
+  uint16_t* q_out; int64_t qo_st, qo_sh;
+  uint16_t* copy[2]; int64_t c_st[2], c_sh[2];           // k, v [N, H, D] or null
+  int N, Hq, H, zero_skipped; float eps;                 // eps < 0: no norm
+  int32_t* status;
+};
+
+// A row of D channels is shared by D / 16 lanes; lane c holds channels [8c, 8c + 8) and their partners of the rotation.
+template <int D, bool IN16, bool CACHE16>
+__global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
+  constexpr int LPR = D / 16, HALF = D / 2;
+  const int rows_per_token = p.Hq + 2 * p.H;
+  const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPR;
+  const int c = threadIdx.x % LPR;
+  const int64_t token64 = item / rows_per_token;
+  if (token64 >= p.N) return;            // (whole groups of lanes: the sums below stay among lanes of one row)
+  const int token = (int)token64;
+  int h = (int)(item - token64 * rows_per_token);
+  const int kind = h < p.Hq ? 0 : h < p.Hq + p.H ? 1 : 2;
+  h -= kind == 0 ? 0 : kind == 1 ? p.Hq : p.Hq + p.H;
+
+  const int pos = p.positions[token];
+  const int seq = p.rows != nullptr ? p.rows[token] : token;
+  // A negative position: no token.  Everything else that does not lead to a page of the pool is an error of the caller's that
+  // only the device can see: nothing is written to the cache, q and the copies become NaN, the status word says so.
+  const bool skipped = pos < 0;
+  int bits = 0, page = 0;
+  if (!skipped) {
+    if (p.cos != nullptr && pos >= p.table_rows) bits |= DAISY_STATUS_POSITION_PAST_TABLES;
+    const int at = pos / p.page_size;
+    if (seq < 0 || seq >= p.seqs || at >= p.max_pages) {
+      bits |= DAISY_STATUS_LENGTH_PAST_PAGES;
+    } else {
+      page = p.table[seq * p.table_st + at];
+      if (page < 0 || page >= p.num_pages) bits |= DAISY_STATUS_PAGE_OUT_OF_RANGE;
+    }
+    if (bits && c == 0 && kind == 1 && h == 0) raise_status(p.status, bits);
+  }
+
+  float lo[8], hi[8];
+  {
+    const uint16_t* src = p.in[kind] + token * p.in_st[kind] + h * p.in_sh[kind] + 8 * c;
+    unpack8_as<IN16>(__builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src)), lo);
+    unpack8_as<IN16>(__builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + HALF)), hi);
+  }
+  if (p.eps >= 0.f) {
+    float sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum += lo[e] * lo[e] + hi[e] * hi[e];
+    sum = group_sum<LPR>(sum);
+    const float rstd = rsqrtf(sum / (float)D + p.eps);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) { lo[e] *= rstd; hi[e] *= rstd; }
+  }
+  if (kind < 2 && p.cos != nullptr) {
+    const int64_t off = (int64_t)(skipped || bits ? 0 : pos) * HALF + 8 * c;
+    const f32x4 c0 = *reinterpret_cast<const f32x4*>(p.cos + off), c1 = *reinterpret_cast<const f32x4*>(p.cos + off + 4);
+    const f32x4 s0 = *reinterpret_cast<const f32x4*>(p.sin + off), s1 = *reinterpret_cast<const f32x4*>(p.sin + off + 4);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x1 = lo[e], x2 = hi[e], cc = e < 4 ? c0[e & 3] : c1[e & 3], sn = e < 4 ? s0[e & 3] : s1[e & 3];
+      lo[e] = fmaf(x1, cc, x2 * sn);
+      hi[e] = fmaf(x2, cc, -(x1 * sn));
+    }
+  }
+  if (kind == 2 && p.ve != nullptr) {
+    const uint16_t* src = p.ve + token * p.e_st + h * p.e_sh + 8 * c;
+    float el[8], eh[8];
+    unpack8_as<IN16>(__builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src)), el);
+    unpack8_as<IN16>(__builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + HALF)), eh);
+    const float g = *p.gate, og = 1.f - g;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) { lo[e] = fmaf(g, lo[e], og * el[e]); hi[e] = fmaf(g, hi[e], og * eh[e]); }
+  }
+
+  if (skipped || bits) {
+    const float fill = skipped ? 0.f : __builtin_nanf("");
+#pragma unroll
+    for (int e = 0; e < 8; ++e) lo[e] = hi[e] = fill;
+  }
+  const bool leave = skipped && !p.zero_skipped;
+  if (kind == 0) {
+    if (leave) return;
+    uint16_t* dst = p.q_out + token * p.qo_st + h * p.qo_sh + 8 * c;
+    *reinterpret_cast<u32x4*>(dst) = pack8_as<CACHE16>(lo);
+    *reinterpret_cast<u32x4*>(dst + HALF) = pack8_as<CACHE16>(hi);
+    return;
+  }
+  const int w = kind - 1;
+  if (!skipped && !bits) {
+    uint16_t* dst = p.pages[w] + page * p.sp[w] + h * p.sh[w] + (int64_t)(pos % p.page_size) * p.ss[w] + 8 * c;
+    *reinterpret_cast<u32x4*>(dst) = pack8_as<CACHE16>(lo);
+    *reinterpret_cast<u32x4*>(dst + HALF) = pack8_as<CACHE16>(hi);
+  }
+  if (p.copy[w] != nullptr && !skipped) {
+    uint16_t* dst = p.copy[w] + token * p.c_st[w] + h * p.c_sh[w] + 8 * c;
+    *reinterpret_cast<u32x4*>(dst) = pack8_as<IN16>(lo);
+    *reinterpret_cast<u32x4*>(dst + HALF) = pack8_as<IN16>(hi);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Attention
+// ---------------------------------------------------------------------------------------------------------------
+// o[b, h] = sum_t softmax_t(scale q[b, h] . k_t) v_t over the positions max(0, len - window) <= t < len of sequence b, G = Hq / H query heads
+// to a key head; zero where there is no position.
+//
+// The work is tiles of 32 positions.  A unit is a (sequence, key head, up to 16 of its query heads); all tiles of all units, one
+// behind the other, are dealt to the wavefronts in equal runs, whatever the lengths: every wavefront reads the lengths, sums
+// them up and finds where its run begins.  A run that covers a whole unit writes the result; the others leave their partial sums,
+// at most two of a wavefront, which a second kernel joins.
+//
+// Both products run on 16x16x32 matrix instructions with nothing between memory and registers: S^T = K Q^T puts 16 query heads in
+// the columns (one head uses one column of 16: the products are 1/16 of use then and still far from bounding anything), so that
+// a lane holds 4 + 4 keys of one head, and those are, as they are, the B operand of O^T = V^T P^T: rows 4c + r and 16 + 4c + r of a tile for
+// the lanes of group c.  V's rows arrive 16 bytes a lane, and v_perm pairs the keys of neighbouring rows.
+struct PagedParams {
+  const uint16_t* q; int64_t q_sb, q_sh;
+  const uint16_t* k; int64_t k_sp, k_sh, k_ss;
+  const uint16_t* v; int64_t v_sp, v_sh, v_ss;
+  const int32_t* table; int64_t table_st; int max_pages, num_pages, blocks_per_page, capacity;
+  const int32_t* lens;
+  uint16_t* o; int64_t o_sb, o_sh;
+  float* part; float2* stat;      // [2 * wavefronts][heads of a unit][D], [..][..]: unnormalised sums; reference and sum of exponentials
+  int B, H, G, head_tiles, heads, window, waves, min_share;      // heads: of a unit, min(G, 16)
+  float scale_log2e;
+  int32_t* status;
+};
+
+constexpr int kTile = 32;       // positions
+constexpr int kBlock = 16;      // positions: pages are multiples of it, so that half a tile lies in one page
+
+template <int CTRL, int ROWS> __device__ __forceinline__ int dpp_int(int x) {
+  return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, true);
+}
+// Sums of the lanes up to each lane.
+__device__ __forceinline__ int wave_scan(int x) {
+  x += dpp_int<0x111, 0xf>(x);      // row_shr 1, 2, 4, 8
+  x += dpp_int<0x112, 0xf>(x);
+  x += dpp_int<0x114, 0xf>(x);
+  x += dpp_int<0x118, 0xf>(x);
+  x += dpp_int<0x142, 0xa>(x);      // row_bcast 15 into rows 1 and 3
+  x += dpp_int<0x143, 0xc>(x);      // row_bcast 31 into rows 2 and 3
+  return x;
+}
+__device__ __forceinline__ float wave_max(float x) {
+  x = fmaxf(x, dpp_move<0xB1>(x));
+  x = fmaxf(x, dpp_move<0x4E>(x));
+  x = fmaxf(x, dpp_move<0x141>(x));
+  x = fmaxf(x, dpp_move<0x128>(x));
+  const LanePair r = row_pair(x);
+  const LanePair t = half_pair(fmaxf(r.x, r.y));
+  return fmaxf(t.x, t.y);
+}
+
+// The positions that a sequence's new token sees, [lo, hi), and the tiles they lie in.
+struct Extent { int lo, hi, first, tiles; bool past; };
+__device__ __forceinline__ Extent extent(const PagedParams& p, int len) {
+  Extent e;
+  e.past = len > p.capacity;
+  e.hi = min(max(len, 0), p.capacity);
+  e.lo = p.window > 0 ? max(e.hi - p.window, 0) : 0;
+  e.first = e.lo / kTile;
+  e.tiles = e.hi > e.lo ? (e.hi + kTile - 1) / kTile - e.first : 0;
+  return e;
+}
+__device__ __forceinline__ int len_of(const PagedParams& p, int b) { return b < p.B ? p.lens[b] : 0; }
+
+// Tiles of all sequences (of one unit each), and how many of a unit's tiles a wavefront takes.
+__device__ __forceinline__ int total_tiles(const PagedParams& p, int lane) {
+  int sum = 0;
+  for (int base = 0; base < p.B; base += 64) sum += extent(p, len_of(p, base + lane)).tiles;
+  return __builtin_amdgcn_readlane(wave_scan(sum), 63);
+}
+__device__ __forceinline__ int share_of(const PagedParams& p, int total) { return max((total + p.waves - 1) / p.waves, p.min_share); }
+
+template <bool F16> __device__ __forceinline__ f32x4 mfma(const u32x4& a, const u32x4& b, const f32x4& c) {
+  if constexpr (F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// The wavefronts of a SIMD that the registers of a head width leave room for.
+constexpr int paged_waves_per_simd(int D) { return D <= 64 ? 4 : D <= 128 ? 3 : 2; }
+
+template <int D, bool F16>
+__global__ __launch_bounds__(256, paged_waves_per_simd(D)) void paged_attn_kernel(PagedParams p) {
+  constexpr int KS = D / 32;                     // steps of the first product
+  constexpr int J = D / 16;                      // 16-row pieces of the second product's result
+  constexpr int W = D == 64 ? 4 : 8;             // channels of a V row that a lane has beside each other
+  constexpr int P = D / 16 / W;                  // such pieces of a row
+  constexpr int VD = J / 2;                      // dwords of a V row that a lane holds
+  // The reference of the exponentials stays kHead below the largest score that set it and moves when a score is kLimit above it, so that
+  // fp16 probabilities use the type's range on both sides of one.
+  constexpr float kHead = F16 ? 9.f : 0.f, kLimit = F16 ? 15.f : 8.f;
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+  const int n = lane & 15, c = lane >> 4;
+  const int units = p.H * p.head_tiles;
+  const int total = total_tiles(p, lane) * units;
+  const int share = share_of(p, total);
+  int64_t x64 = (int64_t)wave * share;
+  if (x64 >= total) return;
+  int x = (int)x64;
+  const int x_end = (int)min(x64 + share, (int64_t)total);
+
+  const uint32_t k_off = (uint32_t)(n * p.k_ss + 8 * c) * 2, v_off = (uint32_t)(4 * c * p.v_ss + W * n) * 2;
+  int base = 0, before = 0, len = 0, tiles = 0, upto = 0, chunk = -1;      // 64 sequences from `base` on, one a lane
+  while (x < x_end) {
+    // ---- the unit that x lies in
+    while (chunk < 0 || x >= (before + chunk) * units) {
+      if (chunk >= 0) { before += chunk; base += 64; }
+      len = len_of(p, base + lane);
+      tiles = extent(p, len).tiles;
+      upto = wave_scan(tiles);
+      chunk = __builtin_amdgcn_readlane(upto, 63);
+    }
+    const uint64_t here = __ballot(tiles > 0 && (before + upto - tiles) * units <= x);
+    const int bl = 63 - __builtin_clzll(here);
+    const int b = base + bl, n_tiles = __builtin_amdgcn_readlane(tiles, bl);
+    const Extent e = extent(p, __builtin_amdgcn_readlane(len, bl));
+    const int rel = x - (before + __builtin_amdgcn_readlane(upto, bl) - n_tiles) * units;
+    const int unit = rel / n_tiles, off = rel - unit * n_tiles;
+    const int count = min(n_tiles - off, x_end - x);
+    const int h = unit / p.head_tiles, head0 = (unit - h * p.head_tiles) * 16;
+
+    // ---- its query heads: columns past the last one repeat it
+    u32x4 qf[KS];
+    {
+      const uint16_t* src = p.q + b * p.q_sb + (int64_t)(h * p.G + min(head0 + n, p.G - 1)) * p.q_sh + 8 * c;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const u32x4*>(src + 32 * s);
+    }
+    f32x4 acc[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = -__builtin_inff(), l = 0.f;
+
+    // ---- pages: lane i has that of the run's block i, for 32 tiles at a time
+    const int32_t* row = p.table + b * p.table_st;
+    const int blk_lo = e.lo / kBlock, blk_hi = (e.hi - 1) / kBlock;
+    bool bad = e.past;
+    int id = 0, in = 0;
+    auto pages_from = [&](int block) {
+      const int blk = min(max(block + lane, blk_lo), blk_hi);      // (blocks outside the range: read, but not used)
+      const int at = (unsigned)blk / (unsigned)p.blocks_per_page;
+      in = blk - at * p.blocks_per_page;
+      id = row[at];
+      const bool out = (unsigned)id >= (unsigned)p.num_pages;
+      bad |= out;
+      id = out ? 0 : id;
+    };
+    const char* kh = reinterpret_cast<const char*>(p.k + h * p.k_sh);
+    const char* vh = reinterpret_cast<const char*>(p.v + h * p.v_sh);
+    u32x4 kr[2][KS];
+    uint32_t vr[8][VD];
+    auto load_k = [&](int i) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int64_t pg = __builtin_amdgcn_readlane(id, 2 * i + half), slot = __builtin_amdgcn_readlane(in, 2 * i + half) * kBlock;
+        const char* src = kh + (pg * p.k_sp + slot * p.k_ss) * 2;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) kr[half][s] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + k_off + 64 * s));
+      }
+    };
+    auto load_v = [&](int i) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int64_t pg = __builtin_amdgcn_readlane(id, 2 * i + half), slot = __builtin_amdgcn_readlane(in, 2 * i + half) * kBlock;
+        const char* src = vh + (pg * p.v_sp + slot * p.v_ss) * 2;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const char* at = src + r * p.v_ss * 2;
+#pragma unroll
+          for (int t = 0; t < P; ++t) {
+            if constexpr (W == 8) {
+              const u32x4 d = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at + v_off + 256 * t));
+#pragma unroll
+              for (int i4 = 0; i4 < 4; ++i4) vr[4 * half + r][4 * t + i4] = d[i4];
+            } else {
+              const u32x2 d = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(at + v_off));
+              vr[4 * half + r][0] = d[0];
+              vr[4 * half + r][1] = d[1];
+            }
+          }
+        }
+      }
+    };
+
+    const int tile0 = e.first + off;
+    pages_from(2 * tile0);
+    load_k(0);
+    load_v(0);
+    for (int i = 0; i < count; ++i) {
+      const int key0 = (tile0 + i) * kTile + 4 * c;
+      const bool edge = (tile0 + i) * kTile < e.lo || (tile0 + i + 1) * kTile > e.hi;
+      const bool more = i + 1 < count;
+      // ---- scores
+      f32x4 sa = {0.f, 0.f, 0.f, 0.f}, sb = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        sa = mfma<F16>(kr[0][s], qf[s], sa);
+        sb = mfma<F16>(kr[1][s], qf[s], sb);
+      }
+      if (more) {
+        if (((i + 1) & 31) == 0) pages_from(2 * (tile0 + i + 1));
+        load_k((i + 1) & 31);
+      }
+      // ---- probabilities
+      float s[8];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) { s[r] = sa[r] * p.scale_log2e; s[4 + r] = sb[r] * p.scale_log2e; }
+      if (edge) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const int key = key0 + (r & 3) + (r & 4) * 4;
+          const bool seen = key >= e.lo && key < e.hi;
+          s[r] = seen ? s[r] : -__builtin_inff();
+#pragma unroll
+          for (int d = 0; d < VD; ++d) vr[r][d] = seen ? vr[r][d] : 0;      // what lies there may be anything
+        }
+      }
+      float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+      {
+        const LanePair r = row_pair(top);
+        const LanePair t = half_pair(fmaxf(r.x, r.y));
+        top = fmaxf(t.x, t.y);
+      }
+      if (__any(top > m + kLimit)) {
+        const float moved = top > m + kLimit ? top - kHead : m;
+        const float f = moved > m ? fast_exp2(m - moved) : 1.f;
+        m = moved;
+        l *= f;
+#pragma unroll
+        for (int j = 0; j < J; ++j) acc[j] *= f;
+      }
+#pragma unroll
+      for (int r = 0; r < 8; ++r) s[r] = fast_exp2(s[r] - m);
+      l += ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+      const u32x4 pf = pack8_as<F16>(s);
+      // ---- O^T += V^T P^T
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const int d = (j / W) * (W / 2) + (j % W) / 2;
+        u32x4 vf;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) vf[t] = __builtin_amdgcn_perm(vr[2 * t + 1][d], vr[2 * t][d], (j & 1) ? 0x07060302u : 0x05040100u);
+        acc[j] = mfma<F16>(vf, pf, acc[j]);
+      }
+      if (more) load_v((i + 1) & 31);
+    }
+
+    // ---- the four groups of lanes have summed their own keys
+    {
+      const LanePair r = row_pair(l);
+      const LanePair t = half_pair(r.x + r.y);
+      l = t.x + t.y;
+    }
+    if (__any(bad)) {
+      l = __builtin_nanf("");
+      if (lane == 0) raise_status(p.status, e.past ? DAISY_STATUS_LENGTH_PAST_PAGES : DAISY_STATUS_PAGE_OUT_OF_RANGE);
+    }
+    const int head = head0 + n;
+    if (head < p.G) {
+      if (off == 0 && count == n_tiles) {
+        const float inv = 1.f / l;
+        uint16_t* dst = p.o + b * p.o_sb + (int64_t)(h * p.G + head) * p.o_sh + 4 * W * c;
+#pragma unroll
+        for (int t = 0; t < P; ++t)
+#pragma unroll
+          for (int i8 = 0; i8 < W / 2; ++i8) {
+            float f[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = acc[t * W + (8 * i8 + i) % W][(8 * i8 + i) / W] * inv;
+            *reinterpret_cast<u32x4*>(dst + 128 * t + 8 * i8) = pack8_as<F16>(f);
+          }
+      } else {
+        const int64_t slot = (int64_t)(2 * wave + (off == 0 ? 1 : 0)) * p.heads + n;
+        float* dst = p.part + slot * D + 4 * W * c;
+#pragma unroll
+        for (int t = 0; t < P; ++t)
+#pragma unroll
+          for (int i4 = 0; i4 < W; ++i4) {
+            f32x4 f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = acc[t * W + (4 * i4 + i) % W][(4 * i4 + i) / W];
+            *reinterpret_cast<f32x4*>(dst + 128 * t + 4 * i4) = f;
+          }
+        if (c == 0) p.stat[slot] = float2{m, l};
+      }
+    }
+    x += count;
+  }
+}
+
+// One workgroup per (sequence, query head): joins the partial sums of a unit that was split, writes zeros for a sequence without positions.
+template <int D, bool F16>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
+  constexpr int LPR = D / 4, GROUPS = 256 / LPR;      // lanes of a row of partial sums, rows at a time
+  __shared__ float4 sums[256];
+  const int lane = threadIdx.x & 63;
+  const int q_head = blockIdx.x, b = blockIdx.y;
+  const int h = q_head / p.G, g = q_head - h * p.G, head_tile = g >> 4, n = g & 15;
+  const int units = p.H * p.head_tiles;
+  int sum = 0, first = 0;
+  for (int base = 0; base < p.B; base += 64) {
+    const int t = extent(p, len_of(p, base + lane)).tiles;
+    sum += t;
+    first += base + lane < b ? t : 0;
+  }
+  const int total = __builtin_amdgcn_readlane(wave_scan(sum), 63) * units;
+  first = __builtin_amdgcn_readlane(wave_scan(first), 63) * units;
+  const int n_tiles = extent(p, p.lens[b]).tiles;
+  uint16_t* dst = p.o + b * p.o_sb + q_head * p.o_sh;
+  if (n_tiles == 0) {
+    if (threadIdx.x < D / 8) *reinterpret_cast<u32x4*>(dst + 8 * threadIdx.x) = u32x4{0, 0, 0, 0};
+    return;
+  }
+  const int share = share_of(p, total);
+  first += (h * p.head_tiles + head_tile) * n_tiles;
+  const int w0 = first / share, w1 = (first + n_tiles - 1) / share;
+  if (w0 == w1) return;
+  // the wavefront that the unit begins in has it in its second slot, where it begins with the unit too; the others in their first
+  const int parts = w1 - w0 + 1;
+  auto slot = [&](int i) { return (int64_t)(2 * (w0 + i) + (i == 0 ? 1 : 0)) * p.heads + n; };
+  float top = -__builtin_inff();
+  for (int i = lane; i < parts; i += 64) top = fmaxf(top, p.stat[slot(i)].x);
+  top = wave_max(top);
+  const int r = threadIdx.x / LPR, at = threadIdx.x % LPR;
+  float l = 0.f;
+  f32x4 a = {0.f, 0.f, 0.f, 0.f};
+  for (int i = r; i < parts; i += GROUPS) {
+    const int64_t s = slot(i);
+    const float2 st = p.stat[s];
+    const float f = fast_exp2(st.x - top);
+    l += f * st.y;
+    a += f * *reinterpret_cast<const f32x4*>(p.part + s * D + 4 * at);
+  }
+  sums[threadIdx.x] = float4{a[0], a[1], a[2], a[3]};
+  __shared__ float ls[GROUPS];
+  if (at == 0) ls[r] = l;
+  __syncthreads();
+  if (threadIdx.x >= LPR) return;
+  l = 0.f;
+  a = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < GROUPS; ++i) {
+    l += ls[i];
+    const float4 t = sums[i * LPR + at];
+    a += f32x4{t.x, t.y, t.z, t.w};
+  }
+  a *= 1.f / l;
+  *reinterpret_cast<u32x2*>(dst + 4 * at) = u32x2{pack2<F16>(a[0], a[1]), pack2<F16>(a[2], a[3])};
+}
+
+// How many wavefronts share the work, and the least number of tiles that one takes.  At least 4 tiles, and more where a unit has many
+// query heads, whose partial sums (D + 2 floats each, written and read) would otherwise outweigh the tiles (64 D bytes of K and V each).
+struct PagedSplit { int waves, min_share, heads, head_tiles; };
+static PagedSplit paged_split(int B, int H, int G, int D, int64_t capacity) {
+  PagedSplit s;
+  s.head_tiles = (G + 15) / 16;
+  s.heads = G < 16 ? G : 16;
+  s.min_share = s.heads <= 6 ? 4 : (2 * s.heads + 2) / 3;
+  const int64_t tiles = ((capacity + kTile - 1) / kTile) * B * H * s.head_tiles;
+  const int64_t waves = (tiles + s.min_share - 1) / s.min_share;
+  const int64_t most = 256 * 4 * paged_waves_per_simd(D);
+  s.waves = (int)(waves < most ? waves : most);
+  return s;
+}
+
+template <bool F16> static void paged_launch(const PagedParams& p, int D, dim3 grid, dim3 join, hipStream_t s) {
+  switch (D) {
+    case 64:
+      hipLaunchKernelGGL((paged_attn_kernel<64, F16>), grid, dim3(256), 0, s, p);
+      hipLaunchKernelGGL((paged_join_kernel<64, F16>), join, dim3(256), 0, s, p);
+      break;
+    case 128:
+      hipLaunchKernelGGL((paged_attn_kernel<128, F16>), grid, dim3(256), 0, s, p);
+      hipLaunchKernelGGL((paged_join_kernel<128, F16>), join, dim3(256), 0, s, p);
+      break;
+    default:
+      hipLaunchKernelGGL((paged_attn_kernel<256, F16>), grid, dim3(256), 0, s, p);
+      hipLaunchKernelGGL((paged_join_kernel<256, F16>), join, dim3(256), 0, s, p);
+  }
+}
+
+template <int D> static void append_launch(const AppendParams& p, bool in16, bool cache16, hipStream_t s) {
+  const int64_t lanes = (int64_t)p.N * (p.Hq + 2 * p.H) * (D / 16);
+  const dim3 grid((unsigned)((lanes + 255) / 256));
+  if (in16) {
+    if (cache16) hipLaunchKernelGGL((paged_append_kernel<D, true, true>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((paged_append_kernel<D, true, false>), grid, dim3(256), 0, s, p);
+  } else {
+    if (cache16) hipLaunchKernelGGL((paged_append_kernel<D, false, true>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((paged_append_kernel<D, false, false>), grid, dim3(256), 0, s, p);
+  }
+}
+
+static bool al16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0; }
+static bool rows_of_16(const int64_t* strides, int n) {
+  for (int i = 0; i < n; ++i)
+    if (strides[i] % 8 != 0 || strides[i] < 0) return false;
+  return true;
+}
+// A page's rows are reached with 32-bit byte offsets from where it begins.
+static bool page_rows_fit(const int64_t* strides) { return strides[2] <= ((int64_t)1 << 24); }
+
+}  // namespace daisy
+
+using namespace daisy;
+
+#define DAISY_CHECK_HEAD_DIM(what, D) \
+  DAISY_CHECK_SUPPORTED((D) == 64 || (D) == 128 || (D) == 256, what ": head_dim %d not supported (64, 128 or 256)", (D))
+#define DAISY_CHECK_PAGES(what)                                                                                                           \
+  DAISY_CHECK_ARG(k_pages && v_pages && k_pages_strides && v_pages_strides, what ": the pages and their strides must be non-NULL");       \
+  DAISY_CHECK_ARG(page_table, what ": the page table must be non-NULL");                                                                  \
+  DAISY_CHECK_ARG(num_pages > 0 && max_pages > 0 && table_stride >= 0, what ": num_pages=%d, max_pages=%d must be positive", num_pages,   \
+                  max_pages);                                                                                                             \
+  DAISY_CHECK_SUPPORTED(page_size > 0 && page_size % 16 == 0, what ": page_size %d not supported (a multiple of 16)", page_size);         \
+  DAISY_CHECK_ARG((int64_t)max_pages * page_size < ((int64_t)1 << 31), what ": a sequence of %lld positions is too long",                  \
+                  (long long)max_pages * page_size);                                                                                      \
+  DAISY_CHECK_ARG(al16(k_pages) && al16(v_pages) && rows_of_16(k_pages_strides, 3) && rows_of_16(v_pages_strides, 3) &&                    \
+                      page_rows_fit(k_pages_strides) && page_rows_fit(v_pages_strides),                                                   \
+                  what ": pages must be 16-byte aligned, their strides multiples of 8 elements, a row's at most 2^24")
+
+extern "C" int daisy_paged_append_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                                      const void* v, const int64_t* v_strides, int in_is_f16,
+                                      const void* ve, const int64_t* ve_strides, const float* gate,
+                                      const float* cos, const float* sin, int table_rows,
+                                      void* k_pages, const int64_t* k_pages_strides, void* v_pages, const int64_t* v_pages_strides,
+                                      int cache_is_f16, const int32_t* page_table, int64_t table_stride, int n_seq, int max_pages,
+                                      int num_pages, int page_size, const int32_t* positions, const int32_t* rows,
+                                      void* q_out, const int64_t* q_out_strides, void* k_out, const int64_t* k_out_strides,
+                                      void* v_out, const int64_t* v_out_strides, int zero_skipped,
+                                      int N, int Hq, int H, int D, float eps, int32_t* status, void* stream) {
+  DAISY_CHECK_ARG(k && v && k_strides && v_strides && positions, "paged_append: k, v and the positions must be non-NULL");
+  DAISY_CHECK_ARG((q == nullptr) == (q_out == nullptr) && (q == nullptr) == (Hq == 0), "paged_append: q, q_out and Hq=%d go together", Hq);
+  DAISY_CHECK_ARG(!q || (q_strides && q_out_strides), "paged_append: q and q_out need strides");
+  DAISY_CHECK_ARG(N > 0 && Hq >= 0 && H > 0 && n_seq > 0, "paged_append: N=%d, H=%d, n_seq=%d must be positive", N, H, n_seq);
+  DAISY_CHECK_ARG((cos == nullptr) == (sin == nullptr) && (!cos || table_rows > 0), "paged_append: cos and sin must both be given or both NULL");
+  DAISY_CHECK_ARG((ve == nullptr) == (gate == nullptr) && (!ve || ve_strides), "paged_append: ve, its strides and gate go together");
+  DAISY_CHECK_ARG((!k_out || k_out_strides) && (!v_out || v_out_strides), "paged_append: k_out and v_out need strides");
+  DAISY_CHECK_ARG(rows || N <= n_seq, "paged_append: without rows, token i belongs to sequence i: %d tokens, %d sequences", N, n_seq);
+  DAISY_CHECK_HEAD_DIM("paged_append", D);
+  DAISY_CHECK_PAGES("paged_append");
+  DAISY_CHECK_ARG(al16(q) && al16(k) && al16(v) && al16(ve) && al16(cos) && al16(sin) && al16(q_out) && al16(k_out) && al16(v_out),
+                  "paged_append: tensors must be 16-byte aligned");
+  DAISY_CHECK_ARG((!q || (rows_of_16(q_strides, 2) && rows_of_16(q_out_strides, 2))) && rows_of_16(k_strides, 2) && rows_of_16(v_strides, 2) &&
+                      (!ve || rows_of_16(ve_strides, 2)) && (!k_out || rows_of_16(k_out_strides, 2)) && (!v_out || rows_of_16(v_out_strides, 2)),
+                  "paged_append: strides must be multiples of 8 elements");
+  DAISY_CHECK_ARG((int64_t)N * ((int64_t)Hq + 2 * (int64_t)H) * (D / 16) <= (int64_t)255 << 31, "paged_append: too many rows (%d tokens)", N);
+  AppendParams p = {};
+  const void* in[3] = {q, k, v};
+  const int64_t* in_strides[3] = {q_strides, k_strides, v_strides};
+  for (int i = q ? 0 : 1; i < 3; ++i) {
+    p.in[i] = (const uint16_t*)in[i];
+    p.in_st[i] = in_strides[i][0]; p.in_sh[i] = in_strides[i][1];
+  }
+  if (ve) { p.ve = (const uint16_t*)ve; p.e_st = ve_strides[0]; p.e_sh = ve_strides[1]; p.gate = gate; }
+  p.cos = cos; p.sin = sin; p.table_rows = table_rows;
+  const int64_t* page_strides[2] = {k_pages_strides, v_pages_strides};
+  const int64_t* copy_strides[2] = {k_out_strides, v_out_strides};
+  p.pages[0] = (uint16_t*)k_pages; p.pages[1] = (uint16_t*)v_pages;
+  p.copy[0] = (uint16_t*)k_out; p.copy[1] = (uint16_t*)v_out;
+  for (int i = 0; i < 2; ++i) {
+    p.sp[i] = page_strides[i][0]; p.sh[i] = page_strides[i][1]; p.ss[i] = page_strides[i][2];
+    if (p.copy[i]) { p.c_st[i] = copy_strides[i][0]; p.c_sh[i] = copy_strides[i][1]; }
+  }
+  p.table = page_table; p.table_st = table_stride; p.seqs = n_seq; p.max_pages = max_pages; p.num_pages = num_pages; p.page_size = page_size;
+  p.positions = positions; p.rows = rows;
+  p.q_out = (uint16_t*)q_out;
+  if (q_out) { p.qo_st = q_out_strides[0]; p.qo_sh = q_out_strides[1]; }
+  p.N = N; p.Hq = Hq; p.H = H; p.zero_skipped = zero_skipped; p.eps = eps; p.status = status;
+  hipStream_t s = (hipStream_t)stream;
+  if (D == 64) append_launch<64>(p, in_is_f16, cache_is_f16, s);
+  else if (D == 128) append_launch<128>(p, in_is_f16, cache_is_f16, s);
+  else append_launch<256>(p, in_is_f16, cache_is_f16, s);
+  DAISY_CHECK_LAUNCH("paged_append_kernel");
+  return DAISY_OK;
+}
+
+static bool paged_shape_ok(int B, int Hq, int H, int D, int max_pages, int page_size) {
+  return B > 0 && H > 0 && Hq > 0 && Hq % H == 0 && (D == 64 || D == 128 || D == 256) && max_pages > 0 && page_size > 0 &&
+         (int64_t)max_pages * page_size < ((int64_t)1 << 31);
+}
+
+extern "C" size_t daisy_paged_attn_workspace_bytes(int B, int Hq, int H, int D, int max_pages, int page_size) {
+  if (!paged_shape_ok(B, Hq, H, D, max_pages, page_size)) return 0;
+  const PagedSplit sp = paged_split(B, H, Hq / H, D, (int64_t)max_pages * page_size);
+  return (size_t)2 * sp.waves * sp.heads * (D + 2) * sizeof(float);
+}
+
+extern "C" int daisy_paged_attn_fwd(const void* q, const int64_t* q_strides,
+                                    const void* k_pages, const int64_t* k_pages_strides, const void* v_pages, const int64_t* v_pages_strides,
+                                    int cache_is_f16, const int32_t* page_table, int64_t table_stride, int max_pages, int num_pages, int page_size,
+                                    const int32_t* lens, void* o, const int64_t* o_strides, int B, int Hq, int H, int D, int window, float scale,
+                                    int32_t* status, void* workspace, size_t workspace_bytes, void* stream) {
+  DAISY_CHECK_ARG(q && q_strides && o && o_strides && lens, "paged_attn: q, o, their strides and the lengths must be non-NULL");
+  DAISY_CHECK_ARG(B > 0 && H > 0 && Hq > 0 && Hq % H == 0, "paged_attn: B=%d, H=%d must be positive, Hq=%d a multiple of H", B, H, Hq);
+  DAISY_CHECK_HEAD_DIM("paged_attn", D);
+  DAISY_CHECK_PAGES("paged_attn");
+  DAISY_CHECK_ARG(al16(q) && al16(o) && rows_of_16(q_strides, 2) && rows_of_16(o_strides, 2),
+                  "paged_attn: q and o must be 16-byte aligned, their strides multiples of 8 elements");
+  const int64_t capacity = (int64_t)max_pages * page_size;
+  const PagedSplit sp = paged_split(B, H, Hq / H, D, capacity);
+  DAISY_CHECK_ARG((capacity / kTile + 1) * B * H * sp.head_tiles < ((int64_t)1 << 31) && B <= 65535, "paged_attn: %d sequences of up to %lld positions are too many",
+                  B, (long long)capacity);
+  const size_t need = daisy_paged_attn_workspace_bytes(B, Hq, H, D, max_pages, page_size);
+  if (workspace == nullptr || workspace_bytes < need || !al16(workspace)) {
+    set_error("paged_attn: workspace of %zu bytes, %zu needed on a 16-byte boundary", workspace_bytes, need);
+    return DAISY_ERR_WORKSPACE;
+  }
+  PagedParams p = {};
+  p.q = (const uint16_t*)q; p.q_sb = q_strides[0]; p.q_sh = q_strides[1];
+  p.k = (const uint16_t*)k_pages; p.k_sp = k_pages_strides[0]; p.k_sh = k_pages_strides[1]; p.k_ss = k_pages_strides[2];
+  p.v = (const uint16_t*)v_pages; p.v_sp = v_pages_strides[0]; p.v_sh = v_pages_strides[1]; p.v_ss = v_pages_strides[2];
+  p.table = page_table; p.table_st = table_stride; p.max_pages = max_pages; p.num_pages = num_pages;
+  p.blocks_per_page = page_size / kBlock; p.capacity = (int)capacity;
+  p.lens = lens;
+  p.o = (uint16_t*)o; p.o_sb = o_strides[0]; p.o_sh = o_strides[1];
+  p.part = (float*)workspace;
+  p.stat = (float2*)(p.part + (size_t)2 * sp.waves * sp.heads * D);
+  p.B = B; p.H = H; p.G = Hq / H; p.head_tiles = sp.head_tiles; p.heads = sp.heads; p.window = window; p.waves = sp.waves; p.min_share = sp.min_share;
+  p.scale_log2e = scale * kLog2e; p.status = status;
+  const dim3 grid((unsigned)((sp.waves + 3) / 4)), join((unsigned)Hq, (unsigned)B);
+  if (cache_is_f16) paged_launch<true>(p, D, grid, join, (hipStream_t)stream);
+  else paged_launch<false>(p, D, grid, join, (hipStream_t)stream);
+  DAISY_CHECK_LAUNCH("paged_attn_kernel");
+  return DAISY_OK;
+}

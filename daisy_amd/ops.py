@@ -420,6 +420,10 @@ def raise_for_status(status: torch.Tensor) -> None:
     if bits & _lib.STATUS_POSITION_PAST_TABLES:
         raise RuntimeError("a decode step ran at a position past the rotary tables (Rotary buffers too small); "
                            "its outputs are NaN")
+    if bits & _lib.STATUS_LENGTH_PAST_PAGES:
+        raise RuntimeError("a length or position of a paged call lies past what the page table has room for; its outputs are NaN")
+    if bits & _lib.STATUS_PAGE_OUT_OF_RANGE:
+        raise RuntimeError("a paged call needed a page table entry that names no page of the pool; its outputs are NaN")
 
 
 def kda_workspace_bytes(B: int, T: int, H: int, Dk: int, Dv: int, chunk: int = 64) -> int:
@@ -768,3 +772,282 @@ def gated_rmsnorm(x: torch.Tensor, gate: torch.Tensor, weight: torch.Tensor, eps
                                          xc.numel() // D, D, float(eps), _lib.current_stream(dev))
     _lib.check(rc, "daisy_gated_rmsnorm_fwd")
     return out
+
+
+# ----------------------------------------------------------------------------------------------
+# sequences of unequal length: a paged cache, and the logits of a batch of requests
+# ----------------------------------------------------------------------------------------------
+_HALF_TYPES = (torch.bfloat16, torch.float16)
+
+
+def _no_autograd(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} has no backward: call it under torch.no_grad() or with tensors that need no gradient")
+
+
+def _check_rows(name: str, t: torch.Tensor, ndim: int, dtypes) -> None:
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} must be {' or '.join(str(d)[6:] for d in dtypes)}, got {t.dtype}")
+    if t.dim() != ndim:
+        raise ValueError(f"{name} must have {ndim} dims, got shape {tuple(t.shape)}")
+    if t.stride(-1) != 1:
+        raise ValueError(f"{name} must be contiguous in its last dim")
+
+
+def _check_index(name: str, t: torch.Tensor, n: int) -> None:
+    if t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 [{n}] tensor, got {tuple(t.shape)} {t.dtype}")
+
+
+def _check_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor) -> Tuple[int, int, int, int]:
+    """Validates what the host can see of a paged cache; returns (pages, H, page size, D)."""
+    _check_rows("k_pages", k_pages, 4, _HALF_TYPES)
+    _check_rows("v_pages", v_pages, 4, (k_pages.dtype,))
+    if v_pages.shape != k_pages.shape or 0 in k_pages.shape:
+        raise ValueError(f"k_pages, v_pages must be [pages, H, page_size, D], got {tuple(k_pages.shape)}, {tuple(v_pages.shape)}")
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[1] == 0 or page_table.stride(1) != 1:
+        raise ValueError(f"page_table must be an int32 [sequences, pages] tensor, contiguous in its last dim, got {tuple(page_table.shape)} {page_table.dtype}")
+    return tuple(k_pages.shape)
+
+
+def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                 positions: torch.Tensor, *, rows: Optional[torch.Tensor] = None, q: Optional[torch.Tensor] = None,
+                 cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None, eps: Optional[float] = None,
+                 ve: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None,
+                 k_out: Optional[torch.Tensor] = None, v_out: Optional[torch.Tensor] = None,
+                 status: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Appends keys and values to a paged cache, preparing them (and the queries) on the way, in one launch.
+
+    ``k``, ``v`` ``[N, H, D]`` and ``q [N, Hq, D]``: rows of the QKV projection for N tokens, bf16 or fp16, any token and head
+    strides; ``positions`` int32 ``[N]``: each token's position in its sequence, ``rows`` int32 ``[N]``: its sequence, a row of
+    ``page_table`` (``None``: token i belongs to sequence i, a decode step).  ``k_pages``, ``v_pages`` ``[pages, H, page_size, D]``, bf16 or fp16;
+    position t of sequence s is row ``t % page_size`` of page ``page_table[s, t // page_size]`` (int32).  Page size: a multiple of 16;
+    D: 64, 128 or 256.
+
+    ``eps``: RMS norm of q, k and v first (``None``: none).  ``cos``/``sin`` (fp32 ``[rows, D/2]``) rotate q and k at the token's position.
+    ``ve [N, H, D]`` and ``gate`` (one fp32): v becomes ``gate * v + (1 - gate) * ve``.  Fp32 throughout, one rounding.
+
+    Returns the prepared queries in the cache's dtype (``q_out`` if given), ``None`` without ``q``.  ``k_out``, ``v_out``: ``[N, H, D]`` in k's
+    dtype, receive k and v too (for the attention over a prompt).  A token at a negative position is skipped: the cache and rows of buffers
+    that the caller gave stay as they are, a query row of a tensor made here is zero.  Two tokens of one call must not share a place.
+
+    The device reads positions, rows and table when the kernel runs.  One that leads to no page or past the rotary tables writes nothing to
+    the cache, gives NaN elsewhere, and raises a bit in ``status`` (one-element int32, see ``raise_for_status``).
+    """
+    dev = _lib.require_gpu(k, v, k_pages, v_pages, page_table, positions, rows, q, cos, sin, ve, gate, q_out, k_out, v_out, status)
+    _no_autograd("paged_append", k, v, q, ve, gate)
+    _check_status(status)
+    P, H, size, D = _check_pages(k_pages, v_pages, page_table)
+    _check_rows("k", k, 3, _HALF_TYPES)
+    _check_rows("v", v, 3, (k.dtype,))
+    N = k.shape[0]
+    if k.shape != (N, H, D) or v.shape != k.shape:
+        raise ValueError(f"k, v must be [N, {H}, {D}] to fit the pages, got {tuple(k.shape)}, {tuple(v.shape)}")
+    _check_index("positions", positions, N)
+    if rows is not None:
+        _check_index("rows", rows, N)
+    elif N > page_table.shape[0]:
+        raise ValueError(f"without rows, token i belongs to sequence i: {N} tokens, {page_table.shape[0]} sequences")
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin must be given together")
+    if cos is not None:
+        for name, t in (("cos", cos), ("sin", sin)):
+            if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != D // 2 or not t.is_contiguous() or t.shape != cos.shape:
+                raise ValueError(f"{name} must be a contiguous fp32 [rows, {D // 2}] table, got {tuple(t.shape)} {t.dtype}")
+    if eps is not None and not eps >= 0.0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    if (ve is None) != (gate is None):
+        raise ValueError("ve and gate must be given together")
+    if ve is not None:
+        _check_rows("ve", ve, 3, (k.dtype,))
+        if ve.shape != k.shape or gate.dtype != torch.float32 or gate.numel() != 1:
+            raise ValueError(f"ve must be [N, {H}, {D}] and gate a one-element fp32 tensor")
+    Hq, zero_skipped = 0, False
+    if q is not None:
+        _check_rows("q", q, 3, (k.dtype,))
+        Hq = q.shape[1]
+        if q.shape != (N, Hq, D) or Hq == 0:
+            raise ValueError(f"q must be [{N}, Hq, {D}], got {tuple(q.shape)}")
+        if q_out is None:
+            q_out, zero_skipped = torch.empty((N, Hq, D), dtype=k_pages.dtype, device=dev), True
+        _check_rows("q_out", q_out, 3, (k_pages.dtype,))
+        if q_out.shape != q.shape:
+            raise ValueError(f"q_out must be {tuple(q.shape)}, got {tuple(q_out.shape)}")
+    elif q_out is not None:
+        raise ValueError("q_out is only produced when q is given")
+    for name, t in (("k_out", k_out), ("v_out", v_out)):
+        if t is not None:
+            _check_rows(name, t, 3, (k.dtype,))
+            if t.shape != k.shape:
+                raise ValueError(f"{name} must be {tuple(k.shape)}, got {tuple(t.shape)}")
+    if N == 0:
+        return q_out
+    d2, d3 = (0, 1), (0, 1, 2)
+    st = lambda t: None if t is None else _lib.strides(t, d2)      # noqa: E731
+    lib = _lib.load()
+    with _lib.on_device(dev):
+        rc = lib.daisy_paged_append_fwd(
+            _lib.ptr(q), st(q), k.data_ptr(), st(k), v.data_ptr(), st(v), 1 if k.dtype == torch.float16 else 0, _lib.ptr(ve), st(ve), _lib.ptr(gate),
+            _lib.ptr(cos), _lib.ptr(sin), 0 if cos is None else int(cos.shape[0]),
+            k_pages.data_ptr(), _lib.strides(k_pages, d3), v_pages.data_ptr(), _lib.strides(v_pages, d3), 1 if k_pages.dtype == torch.float16 else 0,
+            page_table.data_ptr(), page_table.stride(0), page_table.shape[0], page_table.shape[1], P, size, positions.data_ptr(), _lib.ptr(rows),
+            _lib.ptr(q_out), st(q_out), _lib.ptr(k_out), st(k_out), _lib.ptr(v_out), st(v_out), 1 if zero_skipped else 0,
+            N, Hq, H, D, -1.0 if eps is None else float(eps), _lib.ptr(status), _lib.current_stream(dev))
+    _lib.check(rc, "daisy_paged_append_fwd")
+    return q_out
+
+
+def paged_attention_workspace_bytes(B: int, Hq: int, H: int, D: int, max_pages: int, page_size: int) -> int:
+    return int(_lib.load().daisy_paged_attn_workspace_bytes(B, Hq, H, D, max_pages, page_size))
+
+
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor, *,
+                    window: Optional[int] = None, scale: float = ATTN_SCALE, out: Optional[torch.Tensor] = None,
+                    workspace: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The attention of one new token per sequence over a paged cache that holds its key and value already (``paged_append``).
+
+    ``q [B, Hq, D]`` in the cache's dtype (bf16 or fp16), any batch and head strides; ``k_pages``, ``v_pages``, ``page_table`` as for ``paged_append``, row b of
+    the table for sequence b; Hq a multiple of the cache's H, ``Hq // H`` query heads to a key head.  ``lens`` int32 ``[B]``: the number of
+    positions of each sequence, the new token's among them; the last ``window`` of them are seen (``None``: all).  A sequence of length zero gives
+    zeros.  Returns ``o [B, Hq, D]`` in q's dtype.
+
+    Lengths and table are read when the kernels run, and the work is split over the lengths that are found there: nothing but shapes is fixed by a
+    recording.  A length beyond the table's room, or a page that is none, gives NaN for the heads of that sequence and raises a bit in ``status``.
+    """
+    dev = _lib.require_gpu(q, k_pages, v_pages, page_table, lens, out, workspace, status)
+    _no_autograd("paged_attention", q, k_pages, v_pages)
+    _check_status(status)
+    P, H, size, D = _check_pages(k_pages, v_pages, page_table)
+    _check_rows("q", q, 3, (k_pages.dtype,))
+    B, Hq = q.shape[:2]
+    if q.shape[2] != D or Hq == 0 or Hq % H != 0:
+        raise ValueError(f"q must be [B, a multiple of {H}, {D}] to fit the pages, got {tuple(q.shape)}")
+    if page_table.shape[0] < B:
+        raise ValueError(f"page_table has {page_table.shape[0]} rows for {B} sequences")
+    _check_index("lens", lens, B)
+    if window is not None and window <= 0:
+        raise ValueError(f"window must be positive or None, got {window}")
+    if out is None:
+        out = torch.empty((B, Hq, D), dtype=q.dtype, device=dev)
+    else:
+        _check_rows("out", out, 3, (q.dtype,))
+        if out.shape != q.shape:
+            raise ValueError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
+    if B == 0:
+        return out
+    lib = _lib.load()
+    max_pages = page_table.shape[1]
+    need = int(lib.daisy_paged_attn_workspace_bytes(B, Hq, H, D, max_pages, size))
+    if workspace is None or workspace.numel() * workspace.element_size() < need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    elif not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
+    with _lib.on_device(dev):
+        rc = lib.daisy_paged_attn_fwd(
+            q.data_ptr(), _lib.strides(q, (0, 1)), k_pages.data_ptr(), _lib.strides(k_pages, (0, 1, 2)),
+            v_pages.data_ptr(), _lib.strides(v_pages, (0, 1, 2)), 1 if q.dtype == torch.float16 else 0,
+            page_table.data_ptr(), page_table.stride(0), max_pages, P, size, lens.data_ptr(), out.data_ptr(), _lib.strides(out, (0, 1)),
+            B, Hq, H, D, min(int(window), 2 ** 31 - 1) if window is not None else 0, float(scale), _lib.ptr(status),
+            workspace.data_ptr(), workspace.numel() * workspace.element_size(), _lib.current_stream(dev))
+    _lib.check(rc, "daisy_paged_attn_fwd")
+    return out
+
+
+_LOGITS_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+MAX_HISTORY = 131071      # tokens of a row's history that process_logits can count
+
+
+def process_logits(logits: torch.Tensor, history: Optional[torch.Tensor] = None, history_lens: Optional[torch.Tensor] = None, *,
+                   repetition: Union[float, torch.Tensor] = 1.0, half_life: Optional[float] = None, cap: Optional[float] = None,
+                   presence: Union[float, torch.Tensor] = 0.0, frequency: Union[float, torch.Tensor] = 0.0, lookback: Optional[int] = None,
+                   bias: Optional[torch.Tensor] = None, allowed: Optional[torch.Tensor] = None,
+                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Penalties for repeated tokens, biases and grammar masks on ``logits [B, V]`` (or ``[V]``; fp32, bf16 or fp16) in one launch.
+
+    ``history [B, T]`` (int64 or int32 token ids, ``history_lens`` int32 ``[B]`` of them; ``None``: all T): of the last ``lookback`` (``None``: all, at most
+    ``MAX_HISTORY``), a token that was seen n times, at ages (1 = the newest) that add up to ``w = sum 2 ** (-age / half_life)`` (``None``: w = n),
+    has its logit divided by ``repetition ** min(w, cap)`` where positive and multiplied by it otherwise; ``frequency * n`` and, for n > 0, ``presence``
+    are subtracted.  ``cap=1`` without a half life is the usual penalty; ``half_life=140, cap=3, lookback=128`` is the generator's
+    (``penalise_repeats``).  Ids outside the vocabulary count for nothing.  ``repetition``, ``presence``, ``frequency``: a number, or fp32 ``[B]`` on the GPU.
+
+    ``bias`` (fp32 ``[V]`` or ``[B, V]``) is added.  ``allowed`` (int32 ``[ceil(V / 32)]`` or ``[B, ceil(V / 32)]``, see ``pack_allowed``): tokens whose bit
+    (``v % 32`` of word ``v // 32``) is clear become -inf, whatever they were; a row without a set bit is -inf throughout.
+
+    Returns a new tensor in the dtype of ``logits``, or ``out`` (which may be ``logits`` itself).  The result does not depend on any order of
+    summation.
+    """
+    settings = [t for t in (repetition, presence, frequency) if isinstance(t, torch.Tensor)]
+    dev = _lib.require_gpu(logits, history, history_lens, bias, allowed, out, *settings)
+    _no_autograd("process_logits", logits, bias, *settings)
+    if logits.dtype not in _LOGITS_TYPES:
+        raise TypeError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")
+    if logits.dim() not in (1, 2) or logits.stride(-1) != 1 and logits.shape[-1] > 1:
+        raise ValueError(f"logits must be [B, V] or [V], contiguous in the last dim, got {tuple(logits.shape)}")
+    x = logits.unsqueeze(0) if logits.dim() == 1 else logits
+    B, V = x.shape
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    elif out.dtype != logits.dtype or out.shape != logits.shape or (V > 1 and out.stride(-1) != 1):
+        raise ValueError(f"out must be {tuple(logits.shape)} {logits.dtype}, contiguous in the last dim")
+    T = 0
+    if history is not None:
+        if history.dim() == 1 and logits.dim() == 1:
+            history = history.unsqueeze(0)
+        if history.dtype not in (torch.int64, torch.int32) or history.dim() != 2 or history.shape[0] != B or (history.shape[1] > 1 and history.stride(1) != 1):
+            raise ValueError(f"history must be int64 or int32 [{B}, T], contiguous in the last dim, got {tuple(history.shape)} {history.dtype}")
+        T = history.shape[1]
+        if history_lens is not None:
+            _check_index("history_lens", history_lens, B)
+    elif history_lens is not None:
+        raise ValueError("history_lens needs a history")
+    if lookback is not None and lookback < 0:
+        raise ValueError(f"lookback must not be negative, got {lookback}")
+    lookback = T if lookback is None else min(int(lookback), T)
+    if lookback > MAX_HISTORY:
+        raise ValueError(f"a history of {lookback} tokens is too long: give a lookback of at most {MAX_HISTORY}")
+    if half_life is not None and not half_life > 0.0:
+        raise ValueError(f"half_life must be positive, got {half_life}")
+    if cap is not None and not cap >= 0.0:
+        raise ValueError(f"cap must not be negative, got {cap}")
+    numbers = []
+    for name, t in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
+        if isinstance(t, torch.Tensor):
+            if t.dtype != torch.float32 or t.shape != (B,) or not t.is_contiguous():
+                raise ValueError(f"{name} must be a number or a contiguous fp32 [{B}] tensor, got {tuple(t.shape)} {t.dtype}")
+            numbers += [t.data_ptr(), 0.0]
+        else:
+            numbers += [None, float(t)]
+    if not isinstance(repetition, torch.Tensor) and not repetition > 0.0:
+        raise ValueError(f"repetition must be positive, got {repetition}")
+    strides = []
+    for name, t, width, dtype in (("bias", bias, V, torch.float32), ("allowed", allowed, (V + 31) // 32, torch.int32)):
+        if t is None:
+            strides.append(0)
+            continue
+        if t.dtype != dtype or t.shape not in ((width,), (B, width)) or (width > 1 and t.stride(-1) != 1):
+            raise ValueError(f"{name} must be {str(dtype)[6:]} [{width}] or [{B}, {width}], contiguous in the last dim, got {tuple(t.shape)} {t.dtype}")
+        strides.append(t.stride(0) if t.dim() == 2 else 0)
+    if B == 0 or V == 0:
+        return out
+    y = out.unsqueeze(0) if out.dim() == 1 else out
+    lib = _lib.load()
+    with _lib.on_device(dev):
+        rc = lib.daisy_logits_process_fwd(
+            x.data_ptr(), x.stride(0), y.data_ptr(), y.stride(0), _LOGITS_TYPES[logits.dtype], _lib.ptr(history),
+            0 if history is None else history.stride(0), 0 if history is None or history.dtype == torch.int32 else 1, _lib.ptr(history_lens),
+            T, lookback, *numbers, 0.0 if half_life is None else float(half_life), float("inf") if cap is None else float(cap),
+            _lib.ptr(bias), strides[0], _lib.ptr(allowed), strides[1], B, V, _lib.current_stream(dev))
+    _lib.check(rc, "daisy_logits_process_fwd")
+    return out
+
+
+def pack_allowed(mask: torch.Tensor) -> torch.Tensor:
+    """The bits that ``process_logits`` takes as ``allowed``: bool ``[..., V]`` -> int32 ``[..., ceil(V / 32)]`` on the same device."""
+    if mask.dtype != torch.bool or mask.dim() == 0:
+        raise TypeError(f"mask must be a bool [..., V] tensor, got {tuple(mask.shape)} {mask.dtype}")
+    V = mask.shape[-1]
+    words = torch.zeros(*mask.shape[:-1], (V + 31) // 32 * 32, dtype=torch.bool, device=mask.device)
+    words[..., :V] = mask
+    bits = words.view(*mask.shape[:-1], -1, 32).to(torch.int64) << torch.arange(32, device=mask.device)
+    total = bits.sum(dim=-1)
+    return (total - ((total >> 31) << 32)).to(torch.int32)

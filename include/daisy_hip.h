@@ -36,6 +36,8 @@ extern "C" {
 /* Bits a kernel raises in a caller-supplied status word (int32 in device memory, never cleared by
  * the library) when it meets a condition that only the device can see. */
 #define DAISY_STATUS_POSITION_PAST_TABLES 1   /* a position read from device memory lies past the rotation tables */
+#define DAISY_STATUS_LENGTH_PAST_PAGES 2      /* a length or position lies past the pages that the page table has room for, or names a row it does not have */
+#define DAISY_STATUS_PAGE_OUT_OF_RANGE 4      /* a page table entry that was needed names no page of the pool */
 
 /* Text of the last error raised on this thread ("" if none). */
 const char* daisy_last_error(void);
@@ -453,6 +455,89 @@ int daisy_short_conv_varlen_fwd(const void* x, int64_t x_row_stride, const void*
  */
 int daisy_gated_rmsnorm_fwd(const void* x, const void* gate, const void* weight, void* out,
                             int64_t rows, int D, float eps, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * A paged key-value cache: decode steps over sequences of unequal length.  The reference's cache
+ * (inference/kv_cache.py:4-68) has one position for the whole batch; these entry points take the
+ * same steps (attention.py:116-139, :181-202) with a position per token and a length per sequence.
+ *
+ * The cache is a pool of pages, k_pages and v_pages [num_pages, H, page_size, D], bf16 or fp16
+ * (cache_is_f16), strides = {page, head, row}.  page_table: int32 [n_seq, max_pages] with a row stride;
+ * position t of sequence s lies in page page_table[s][t / page_size], row t % page_size.  Entries
+ * that a call does not need are not read as pages and may hold anything (-1 by convention).
+ * page_size: a multiple of 16.  D: 64, 128 or 256.  Strides in elements, multiples of 8; pointers
+ * 16-byte aligned.  Positions, lengths, rows and the table are read when the kernels run, so that launches
+ * can be recorded in a HIP graph and replayed while they change.  What only the device can see is
+ * reported in *status (int32 or NULL): DAISY_STATUS_POSITION_PAST_TABLES, DAISY_STATUS_LENGTH_PAST_PAGES,
+ * DAISY_STATUS_PAGE_OUT_OF_RANGE; results that depend on it are NaN, and no memory outside the
+ * tensors is touched.
+ *
+ * daisy_paged_append_fwd: for token i of N at position positions[i] of sequence rows[i] (rows NULL:
+ * sequence i),
+ *   x' = x * rsqrt(mean(x^2) + eps) for q, k and v (eps < 0: x' = x),
+ *   q, k rotated with row positions[i] of cos, sin (fp32 [table_rows, D/2], or both NULL),
+ *   v = gate * v' + (1 - gate) * ve (ve and gate, one fp32, both or neither),
+ * in fp32, rounded once: k and v into the pages, q into q_out (the cache's type), and k and v into k_out and
+ * v_out (the inputs' type) where those are given.  A token at a negative position is skipped: nothing of it
+ * is written, except that its row of q_out becomes zero where zero_skipped is set.
+ * q, k, v, ve: bf16 or fp16 (in_is_f16) [N, Hq], [N, H] heads of D with {token, head} strides; q and
+ * q_out may be NULL (Hq = 0).  Two tokens of one call at the same place of the cache: either may be the one that
+ * stays, or parts of both.
+ */
+int daisy_paged_append_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                           const void* v, const int64_t* v_strides, int in_is_f16,
+                           const void* ve, const int64_t* ve_strides, const float* gate,
+                           const float* cos, const float* sin, int table_rows,
+                           void* k_pages, const int64_t* k_pages_strides,
+                           void* v_pages, const int64_t* v_pages_strides, int cache_is_f16,
+                           const int32_t* page_table, int64_t table_stride, int n_seq, int max_pages,
+                           int num_pages, int page_size,
+                           const int32_t* positions, const int32_t* rows,
+                           void* q_out, const int64_t* q_out_strides, void* k_out, const int64_t* k_out_strides,
+                           void* v_out, const int64_t* v_out_strides, int zero_skipped,
+                           int N, int Hq, int H, int D, float eps, int32_t* status, void* stream);
+
+/* daisy_paged_attn_fwd: the attention of one new token per sequence, whose key and value are in the cache already:
+ *   o[b, h] = sum_t softmax_t(scale <q[b, h], k_t>) v_t,  max(0, lens[b] - window) <= t < lens[b]
+ * (window <= 0: all positions), the key head of query head h being h / (Hq / H); a length of zero or less gives
+ * zeros.  q, o: the cache's type, [B, Hq, D] with {batch, head} strides.  The work is split over the lengths
+ * as they are when the kernel runs.  workspace: daisy_paged_attn_workspace_bytes(...) bytes, 16-byte aligned,
+ * of no other call that may run at the same time.
+ */
+size_t daisy_paged_attn_workspace_bytes(int B, int Hq, int H, int D, int max_pages, int page_size);
+int daisy_paged_attn_fwd(const void* q, const int64_t* q_strides,
+                         const void* k_pages, const int64_t* k_pages_strides,
+                         const void* v_pages, const int64_t* v_pages_strides, int cache_is_f16,
+                         const int32_t* page_table, int64_t table_stride, int max_pages, int num_pages, int page_size,
+                         const int32_t* lens, void* o, const int64_t* o_strides,
+                         int B, int Hq, int H, int D, int window, float scale, int32_t* status,
+                         void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Penalties for repeated tokens, biases and grammar masks on the logits of a batch, in one pass: the
+ * repetition penalty of the reference's generator (inference/generate.py:47-58) and what
+ * serving asks for beside it.  Per row b and token v, with h the last `lookback` of the row's
+ * history_lens[b] (NULL: T) tokens, age 1 the newest:
+ *   n = #{j : h_j = v};  w = sum over those j of 2^(-age_j / half_life)  (half_life 0: of 1);
+ *   s = repetition^min(w, cap);  y = (x > 0 ? x / s : x * s) - frequency * n - presence * [n > 0]
+ *   y += bias[v];  y = -inf where bit v % 32 of allowed[v / 32] is clear
+ * in fp32, rounded once to the type of x.
+ * x, y        : [B, V], type 0 = fp32, 1 = bf16, 2 = fp16, row strides; y may be x, and must not overlap it otherwise.
+ * history     : int32 or int64 (history_is_int64) [B, T] with a row stride, or NULL; ids outside 0 .. V - 1 count
+ *               for nothing.  At most 131071 tokens of a row are looked at (min(T, lookback)).
+ * repetition, presence, frequency: a number, or, where the pointer before it is given, fp32 [B].
+ * bias        : fp32 [V] (bias_stride 0) or [B, V], or NULL.
+ * allowed     : int32 [ceil(V / 32)] (allowed_stride 0) or [B, ceil(V / 32)], or NULL.
+ * Counts and weights are summed in integers: the result does not depend on any order.
+ */
+int daisy_logits_process_fwd(const void* x, int64_t x_stride, void* y, int64_t y_stride, int type,
+                             const void* history, int64_t history_stride, int history_is_int64,
+                             const int32_t* history_lens, int T, int lookback,
+                             const float* repetition_rows, double repetition,
+                             const float* presence_rows, float presence,
+                             const float* frequency_rows, float frequency, float half_life, float cap,
+                             const float* bias, int64_t bias_stride, const int32_t* allowed, int64_t allowed_stride,
+                             int B, int V, void* stream);
 
 #ifdef __cplusplus
 }
