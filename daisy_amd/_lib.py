@@ -161,7 +161,7 @@ SIGNATURES = {
         c_void_p, _I64P, c_void_p, _I64P, c_int,                # k_pages, v_pages (+ strides), cache is fp16
         c_void_p, c_int64, c_int, c_int, c_int, c_int,          # page_table (+ row stride), n_seq, max_pages, num_pages, page_size
         c_void_p, c_void_p,                                     # positions, rows
-        c_void_p, _I64P, c_void_p, _I64P, c_void_p, _I64P, c_int,  # q_out, k_out, v_out (+ strides), zero_skipped
+        c_void_p, _I64P, c_int, c_void_p, _I64P, c_void_p, _I64P, c_int,  # q_out (+ strides), is fp16, k_out, v_out (+ strides), zero_skipped
         c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p]),  # N, Hq, H, D, eps, status, stream
     "daisy_paged_attn_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
     "daisy_paged_attn_fwd": (c_int, [

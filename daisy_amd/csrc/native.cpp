@@ -711,6 +711,163 @@ PyObject* py_kda_layer(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- sequences of unequal length --------------------------------------------------------------------------------------
+// bf16 or fp16, `dims` dimensions, the last one contiguous
+bool rows_half(const Tensor& t, int64_t dims, int dev) {
+  return on_gpu(t, dev) && (bf16(t) || t.scalar_type() == at::kHalf) && t.dim() == dims && t.stride(-1) == 1;
+}
+bool same_type(const Tensor& a, const Tensor& b) { return a.scalar_type() == b.scalar_type(); }
+bool one_of(const Tensor& t, at::ScalarType type, int dev) { return on_gpu(t, dev) && t.scalar_type() == type && t.numel() == 1; }
+int is_f16(const Tensor& t) { return t.scalar_type() == at::kHalf; }
+
+// Pages [pages, H, page size, D] and the table of sequences.
+bool paged_cache(const Tensor& k, const Tensor& v, const Tensor& table, int dev) {
+  return rows_half(k, 4, dev) && rows_half(v, 4, dev) && same_type(k, v) && k.sizes() == v.sizes() && k.numel() > 0 && on_gpu(table, dev) &&
+         table.scalar_type() == at::kInt && table.dim() == 2 && table.size(1) > 0 && table.stride(1) == 1 && k.size(0) <= INT32_MAX && table.size(0) <= INT32_MAX;
+}
+bool int32_row(const Tensor& t, int64_t n, int dev) { return int32_vector(t, n, dev) && t.dim() == 1; }
+
+// paged_append(k, v, k_pages, v_pages, page_table, positions, rows, q, cos, sin, eps (< 0: none), ve, gate, q_out, k_out, v_out, status) -> q_out, or True without q
+PyObject* py_paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (intercepted() || n != 17) return none();
+  for (int i = 0; i < 6; ++i)
+    if (!is_tensor(a[i])) return none();
+  for (int i : {6, 7, 8, 9, 11, 12, 13, 14, 15, 16})
+    if (!tensor_or_none(a[i])) return none();
+  const Tensor &k = THPVariable_Unpack(a[0]), &v = THPVariable_Unpack(a[1]), &kp = THPVariable_Unpack(a[2]), &vp = THPVariable_Unpack(a[3]);
+  const Tensor &table = THPVariable_Unpack(a[4]), &pos = THPVariable_Unpack(a[5]);
+  const Tensor *rows = opt_tensor(a[6]), *q = opt_tensor(a[7]), *cos = opt_tensor(a[8]), *sin = opt_tensor(a[9]), *ve = opt_tensor(a[11]), *gate = opt_tensor(a[12]);
+  const Tensor *q_out = opt_tensor(a[13]), *k_out = opt_tensor(a[14]), *v_out = opt_tensor(a[15]), *status = opt_tensor(a[16]);
+  const float eps = (float)PyFloat_AsDouble(a[10]);
+  if (PyErr_Occurred()) { PyErr_Clear(); return none(); }
+  const int dev = gpu_of(k);
+  if (dev < 0 || !paged_cache(kp, vp, table, dev) || !rows_half(k, 3, dev) || !rows_half(v, 3, dev) || !same_type(k, v) || k.sizes() != v.sizes()) return none();
+  const int64_t N = k.size(0), H = kp.size(1), D = kp.size(3);
+  if (N < 1 || N > INT32_MAX || k.size(1) != H || k.size(2) != D || !int32_row(pos, N, dev) || (rows && !int32_row(*rows, N, dev))) return none();
+  if ((cos == nullptr) != (sin == nullptr) || (ve == nullptr) != (gate == nullptr) || (!q && q_out)) return none();
+  if (cos && !(rotary_table(*cos, 1, D / 2, dev) && rotary_table(*sin, 1, D / 2, dev) && cos->size(0) == sin->size(0) && cos->size(0) <= INT32_MAX)) return none();
+  if (ve && !(rows_half(*ve, 3, dev) && same_type(*ve, k) && ve->sizes() == k.sizes() && one_of(*gate, at::kFloat, dev))) return none();
+  if (q && !(rows_half(*q, 3, dev) && same_type(*q, k) && q->size(0) == N && q->size(1) > 0 && q->size(2) == D)) return none();
+  if (q_out && !(rows_half(*q_out, 3, dev) && (same_type(*q_out, kp) || same_type(*q_out, k)) && q_out->sizes() == q->sizes())) return none();
+  for (const Tensor* t : {k_out, v_out})
+    if (t && !(rows_half(*t, 3, dev) && same_type(*t, k) && t->sizes() == k.sizes())) return none();
+  if ((status && !one_of(*status, at::kInt, dev)) || needs_autograd({&k, &v, q, ve, gate})) return none();
+  Unlocked unlocked;
+  Tensor qo;
+  if (q) qo = q_out ? *q_out : empty(q->sizes(), kp.scalar_type(), k);
+  auto st = [](const Tensor* t) { return t ? Strides2(*t) : Strides2(); };
+  const Strides2 qs = st(q), ks(k), vs(v), es = st(ve), qos = qo.defined() ? Strides2(qo) : Strides2(), kos = st(k_out), vos = st(v_out);
+  const Strides3 kps(kp), vps(vp);
+  const int rc = daisy_paged_append_fwd(ptr(q), qs.s, ptr(k), ks.s, ptr(v), vs.s, is_f16(k), ptr(ve), es.s, (const float*)ptr(gate), (const float*)ptr(cos),
+                                        (const float*)ptr(sin), cos ? (int)cos->size(0) : 0, ptr(kp), kps.s, ptr(vp), vps.s, is_f16(kp),
+                                        (const int32_t*)ptr(table), table.stride(0), (int)table.size(0), (int)std::min<int64_t>(table.size(1), INT32_MAX),
+                                        (int)kp.size(0), (int)std::min<int64_t>(kp.size(2), INT32_MAX), (const int32_t*)ptr(pos), (const int32_t*)ptr(rows),
+                                        q ? ptr(qo) : nullptr, qos.s, q ? is_f16(qo) : 0, ptr(k_out), kos.s, ptr(v_out), vos.s, q && !q_out,
+                                        (int)N, q ? (int)q->size(1) : 0, (int)H, (int)D, eps, (int32_t*)ptr(status), stream_of(dev));
+  if (rc != DAISY_OK) return none();
+  unlocked.end();
+  if (q) return wrap(qo);
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_attention(q, k_pages, v_pages, page_table, lens, window (0: all), scale, out, workspace, status) -> out
+PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (intercepted() || n != 10) return none();
+  for (int i = 0; i < 5; ++i)
+    if (!is_tensor(a[i])) return none();
+  for (int i : {7, 8, 9})
+    if (!tensor_or_none(a[i])) return none();
+  const Tensor &q = THPVariable_Unpack(a[0]), &kp = THPVariable_Unpack(a[1]), &vp = THPVariable_Unpack(a[2]), &table = THPVariable_Unpack(a[3]), &lens = THPVariable_Unpack(a[4]);
+  const Tensor *out = opt_tensor(a[7]), *ws = opt_tensor(a[8]), *status = opt_tensor(a[9]);
+  const long window = PyLong_AsLong(a[5]);
+  const float scale = (float)PyFloat_AsDouble(a[6]);
+  if (PyErr_Occurred()) { PyErr_Clear(); return none(); }
+  const int dev = gpu_of(q);
+  if (dev < 0 || window < 0 || !paged_cache(kp, vp, table, dev) || !rows_half(q, 3, dev) || !same_type(q, kp)) return none();
+  const int64_t B = q.size(0), Hq = q.size(1), H = kp.size(1), D = kp.size(3);
+  if (B < 1 || B > INT32_MAX || Hq < 1 || Hq > INT32_MAX || Hq % H != 0 || q.size(2) != D || table.size(0) < B || !int32_row(lens, B, dev)) return none();
+  if (out && !(rows_half(*out, 3, dev) && same_type(*out, q) && out->sizes() == q.sizes())) return none();
+  if ((status && !one_of(*status, at::kInt, dev)) || (ws && !(on_gpu(*ws, dev) && ws->is_contiguous())) || needs_autograd({&q, &kp, &vp})) return none();
+  const int max_pages = (int)std::min<int64_t>(table.size(1), INT32_MAX), size = (int)std::min<int64_t>(kp.size(2), INT32_MAX);
+  const size_t need = daisy_paged_attn_workspace_bytes((int)B, (int)Hq, (int)H, (int)D, max_pages, size);
+  if (need == 0) return none();
+  Unlocked unlocked;
+  Tensor o = out ? *out : empty(q.sizes(), q.scalar_type(), q);
+  Tensor w = ws && (size_t)(ws->numel() * ws->element_size()) >= need ? *ws : empty({(int64_t)need}, at::kByte, q);
+  const Strides2 qs(q), os(o);
+  const Strides3 ks(kp), vs(vp);
+  const int rc = daisy_paged_attn_fwd(ptr(q), qs.s, ptr(kp), ks.s, ptr(vp), vs.s, is_f16(kp), (const int32_t*)ptr(table), table.stride(0), max_pages, (int)kp.size(0), size,
+                                      (const int32_t*)ptr(lens), ptr(o), os.s, (int)B, (int)Hq, (int)H, (int)D, (int)std::min<long>(window, INT32_MAX), scale,
+                                      (int32_t*)ptr(status), ptr(w), (size_t)(w.numel() * w.element_size()), stream_of(dev));
+  if (rc != DAISY_OK) return none();
+  unlocked.end();
+  return wrap(o);
+  END_HANDLE_TH_ERRORS
+}
+
+// process_logits(logits, history, history_lens, repetition, half_life (0: none), cap, presence, frequency, lookback (-1: all), bias, allowed, out) -> out
+// repetition, presence, frequency: a float or a tensor.
+PyObject* py_process_logits(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (intercepted() || n != 12 || !is_tensor(a[0])) return none();
+  for (int i : {1, 2, 9, 10, 11})
+    if (!tensor_or_none(a[i])) return none();
+  const Tensor& x = THPVariable_Unpack(a[0]);
+  const Tensor *history = opt_tensor(a[1]), *lens = opt_tensor(a[2]), *bias = opt_tensor(a[9]), *allowed = opt_tensor(a[10]), *out = opt_tensor(a[11]);
+  const int dev = gpu_of(x);
+  const at::ScalarType type = x.scalar_type();
+  if (dev < 0 || x.dim() < 1 || x.dim() > 2 || x.numel() == 0 || !(type == at::kFloat || type == at::kBFloat16 || type == at::kHalf)) return none();
+  const int64_t B = x.dim() == 2 ? x.size(0) : 1, V = x.size(-1);
+  auto last_dense = [](const Tensor& t) { return t.size(-1) <= 1 || t.stride(-1) == 1; };
+  auto row = [](const Tensor& t) { return t.dim() == 2 ? t.stride(0) : 0; };
+  if (B > INT32_MAX || V > INT32_MAX || !last_dense(x)) return none();
+  if (out && !(on_gpu(*out, dev) && out->scalar_type() == type && out->sizes() == x.sizes() && last_dense(*out))) return none();
+  int64_t T = 0;
+  if (history) {
+    if (!on_gpu(*history, dev) || !(history->scalar_type() == at::kLong || history->scalar_type() == at::kInt)) return none();
+    if (!(history->dim() == 2 ? history->size(0) == B : history->dim() == 1 && x.dim() == 1) || !last_dense(*history)) return none();
+    T = history->size(-1);
+  }
+  if (lens && !(history && int32_row(*lens, B, dev))) return none();
+  double number[3];
+  const float* rows[3] = {nullptr, nullptr, nullptr};
+  const Tensor* settings[3] = {nullptr, nullptr, nullptr};
+  const int at_setting[3] = {3, 6, 7};
+  for (int i = 0; i < 3; ++i) {
+    PyObject* o = a[at_setting[i]];
+    if (is_tensor(o)) {
+      const Tensor& t = THPVariable_Unpack(o);
+      if (!on_gpu(t, dev) || !f32(t) || t.dim() != 1 || t.size(0) != B || !t.is_contiguous()) return none();
+      settings[i] = &t;
+      rows[i] = (const float*)ptr(t);
+      number[i] = 0.0;
+    } else {
+      number[i] = PyFloat_AsDouble(o);
+    }
+  }
+  const double half_life = PyFloat_AsDouble(a[4]), cap = PyFloat_AsDouble(a[5]);
+  const long asked = PyLong_AsLong(a[8]);
+  if (PyErr_Occurred()) { PyErr_Clear(); return none(); }
+  const int64_t lookback = asked < 0 ? T : std::min<int64_t>(asked, T);
+  if (T > INT32_MAX || (bias && !(on_gpu(*bias, dev) && f32(*bias) && bias->size(-1) == V && last_dense(*bias) && (bias->dim() == 1 || (bias->dim() == 2 && bias->size(0) == B))))) return none();
+  if (allowed && !(on_gpu(*allowed, dev) && allowed->scalar_type() == at::kInt && allowed->size(-1) == (V + 31) / 32 && last_dense(*allowed) &&
+                   (allowed->dim() == 1 || (allowed->dim() == 2 && allowed->size(0) == B)))) return none();
+  if (needs_autograd({&x, bias, settings[0], settings[1], settings[2]})) return none();
+  Unlocked unlocked;
+  Tensor y = out ? *out : empty(x.sizes(), type, x);
+  const int rc = daisy_logits_process_fwd(ptr(x), row(x), ptr(y), row(y), type == at::kFloat ? 0 : type == at::kBFloat16 ? 1 : 2, ptr(history), history ? row(*history) : 0,
+                                          history && history->scalar_type() == at::kLong, (const int32_t*)ptr(lens), (int)T, (int)lookback, rows[0], number[0], rows[1],
+                                          (float)number[1], rows[2], (float)number[2], (float)half_life, (float)cap, (const float*)ptr(bias), bias ? row(*bias) : 0,
+                                          (const int32_t*)ptr(allowed), allowed ? row(*allowed) : 0, (int)B, (int)V, stream_of(dev));
+  if (rc != DAISY_OK) return none();
+  unlocked.end();
+  return wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
 template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
 PyObject* call(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   PyObject* r = F(self, a, n);
@@ -719,6 +876,7 @@ PyObject* call(PyObject* self, PyObject* const* a, Py_ssize_t n) {
 }
 #define FAST(name) {#name, (PyCFunction)(void (*)(void))call<py_##name>, METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {FAST(linear), FAST(norm), FAST(linears), FAST(prefill_attention), FAST(layer_prefill), FAST(layer_step), FAST(kda_chunk), FAST(kda_layer),
+                          FAST(paged_append), FAST(paged_attention), FAST(process_logits),
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

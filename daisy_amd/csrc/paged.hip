@@ -41,7 +41,7 @@ __device__ __forceinline__ void raise_status(int32_t* status, int bit) {
 // ---------------------------------------------------------------------------------------------------------------
 // Per token and head:  x' = x rsqrt(mean(x^2) + eps) for q, k and v where a norm is wanted;
 //   q, k: y1 = x1 cos + x2 sin, y2 = x2 cos - x1 sin on the pairs (i, i + D/2), row `position` of the tables;  v = g v + (1 - g) ve.
-// All of it in fp32, rounded once as it is stored: pages and q in the cache's type, copies in the inputs'.
+// All of it in fp32, rounded once as it is stored: pages in the cache's type, copies in the inputs', q in either.
 struct AppendParams {
   const uint16_t* in[3]; int64_t in_st[3], in_sh[3];     // q, k, v [N, heads, D]
   const uint16_t* ve; int64_t e_st, e_sh; const float* gate;
@@ -51,7 +51,7 @@ struct AppendParams {
   const int32_t* positions; const int32_t* rows;
   uint16_t* q_out; int64_t qo_st, qo_sh;
   uint16_t* copy[2]; int64_t c_st[2], c_sh[2];           // k, v [N, H, D] or null
-  int N, Hq, H, zero_skipped; float eps;                 // eps < 0: no norm
+  int N, Hq, H, zero_skipped, q_f16; float eps;                 // eps < 0: no norm
   int32_t* status;
 };
 
@@ -132,8 +132,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
   if (kind == 0) {
     if (leave) return;
     uint16_t* dst = p.q_out + token * p.qo_st + h * p.qo_sh + 8 * c;
-    *reinterpret_cast<u32x4*>(dst) = pack8_as<CACHE16>(lo);
-    *reinterpret_cast<u32x4*>(dst + HALF) = pack8_as<CACHE16>(hi);
+    *reinterpret_cast<u32x4*>(dst) = p.q_f16 ? pack8_as<true>(lo) : pack8_as<false>(lo);
+    *reinterpret_cast<u32x4*>(dst + HALF) = p.q_f16 ? pack8_as<true>(hi) : pack8_as<false>(hi);
     return;
   }
   const int w = kind - 1;
@@ -578,8 +578,8 @@ extern "C" int daisy_paged_append_fwd(const void* q, const int64_t* q_strides, c
                                       void* k_pages, const int64_t* k_pages_strides, void* v_pages, const int64_t* v_pages_strides,
                                       int cache_is_f16, const int32_t* page_table, int64_t table_stride, int n_seq, int max_pages,
                                       int num_pages, int page_size, const int32_t* positions, const int32_t* rows,
-                                      void* q_out, const int64_t* q_out_strides, void* k_out, const int64_t* k_out_strides,
-                                      void* v_out, const int64_t* v_out_strides, int zero_skipped,
+                                      void* q_out, const int64_t* q_out_strides, int q_out_is_f16,
+                                      void* k_out, const int64_t* k_out_strides, void* v_out, const int64_t* v_out_strides, int zero_skipped,
                                       int N, int Hq, int H, int D, float eps, int32_t* status, void* stream) {
   DAISY_CHECK_ARG(k && v && k_strides && v_strides && positions, "paged_append: k, v and the positions must be non-NULL");
   DAISY_CHECK_ARG((q == nullptr) == (q_out == nullptr) && (q == nullptr) == (Hq == 0), "paged_append: q, q_out and Hq=%d go together", Hq);
@@ -618,7 +618,7 @@ extern "C" int daisy_paged_append_fwd(const void* q, const int64_t* q_strides, c
   p.positions = positions; p.rows = rows;
   p.q_out = (uint16_t*)q_out;
   if (q_out) { p.qo_st = q_out_strides[0]; p.qo_sh = q_out_strides[1]; }
-  p.N = N; p.Hq = Hq; p.H = H; p.zero_skipped = zero_skipped; p.eps = eps; p.status = status;
+  p.N = N; p.Hq = Hq; p.H = H; p.zero_skipped = zero_skipped; p.q_f16 = q_out_is_f16; p.eps = eps; p.status = status;
   hipStream_t s = (hipStream_t)stream;
   if (D == 64) append_launch<64>(p, in_is_f16, cache_is_f16, s);
   else if (D == 128) append_launch<128>(p, in_is_f16, cache_is_f16, s);

@@ -827,13 +827,18 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     ``eps``: RMS norm of q, k and v first (``None``: none).  ``cos``/``sin`` (fp32 ``[rows, D/2]``) rotate q and k at the token's position.
     ``ve [N, H, D]`` and ``gate`` (one fp32): v becomes ``gate * v + (1 - gate) * ve``.  Fp32 throughout, one rounding.
 
-    Returns the prepared queries in the cache's dtype (``q_out`` if given), ``None`` without ``q``.  ``k_out``, ``v_out``: ``[N, H, D]`` in k's
+    Returns the prepared queries in the cache's dtype, or ``q_out`` (the cache's dtype or k's); ``None`` without ``q``.  ``k_out``, ``v_out``: ``[N, H, D]`` in k's
     dtype, receive k and v too (for the attention over a prompt).  A token at a negative position is skipped: the cache and rows of buffers
     that the caller gave stay as they are, a query row of a tensor made here is zero.  Two tokens of one call must not share a place.
 
     The device reads positions, rows and table when the kernel runs.  One that leads to no page or past the rotary tables writes nothing to
     the cache, gives NaN elsewhere, and raises a bit in ``status`` (one-element int32, see ``raise_for_status``).
     """
+    if eps is not None and not eps >= 0.0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    fast = _lib.native().paged_append(k, v, k_pages, v_pages, page_table, positions, rows, q, cos, sin, -1.0 if eps is None else eps, ve, gate, q_out, k_out, v_out, status)
+    if fast is not None:
+        return fast if fast is not True else None
     dev = _lib.require_gpu(k, v, k_pages, v_pages, page_table, positions, rows, q, cos, sin, ve, gate, q_out, k_out, v_out, status)
     _no_autograd("paged_append", k, v, q, ve, gate)
     _check_status(status)
@@ -854,8 +859,6 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
         for name, t in (("cos", cos), ("sin", sin)):
             if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != D // 2 or not t.is_contiguous() or t.shape != cos.shape:
                 raise ValueError(f"{name} must be a contiguous fp32 [rows, {D // 2}] table, got {tuple(t.shape)} {t.dtype}")
-    if eps is not None and not eps >= 0.0:
-        raise ValueError(f"eps must not be negative, got {eps}")
     if (ve is None) != (gate is None):
         raise ValueError("ve and gate must be given together")
     if ve is not None:
@@ -870,7 +873,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
             raise ValueError(f"q must be [{N}, Hq, {D}], got {tuple(q.shape)}")
         if q_out is None:
             q_out, zero_skipped = torch.empty((N, Hq, D), dtype=k_pages.dtype, device=dev), True
-        _check_rows("q_out", q_out, 3, (k_pages.dtype,))
+        _check_rows("q_out", q_out, 3, tuple({k_pages.dtype, k.dtype}))
         if q_out.shape != q.shape:
             raise ValueError(f"q_out must be {tuple(q.shape)}, got {tuple(q_out.shape)}")
     elif q_out is not None:
@@ -891,7 +894,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
             _lib.ptr(cos), _lib.ptr(sin), 0 if cos is None else int(cos.shape[0]),
             k_pages.data_ptr(), _lib.strides(k_pages, d3), v_pages.data_ptr(), _lib.strides(v_pages, d3), 1 if k_pages.dtype == torch.float16 else 0,
             page_table.data_ptr(), page_table.stride(0), page_table.shape[0], page_table.shape[1], P, size, positions.data_ptr(), _lib.ptr(rows),
-            _lib.ptr(q_out), st(q_out), _lib.ptr(k_out), st(k_out), _lib.ptr(v_out), st(v_out), 1 if zero_skipped else 0,
+            _lib.ptr(q_out), st(q_out), 1 if q_out is not None and q_out.dtype == torch.float16 else 0, _lib.ptr(k_out), st(k_out), _lib.ptr(v_out), st(v_out), 1 if zero_skipped else 0,
             N, Hq, H, D, -1.0 if eps is None else float(eps), _lib.ptr(status), _lib.current_stream(dev))
     _lib.check(rc, "daisy_paged_append_fwd")
     return q_out
@@ -914,6 +917,11 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     Lengths and table are read when the kernels run, and the work is split over the lengths that are found there: nothing but shapes is fixed by a
     recording.  A length beyond the table's room, or a page that is none, gives NaN for the heads of that sequence and raises a bit in ``status``.
     """
+    if window is not None and window <= 0:
+        raise ValueError(f"window must be positive or None, got {window}")
+    fast = _lib.native().paged_attention(q, k_pages, v_pages, page_table, lens, 0 if window is None else window, scale, out, workspace, status)
+    if fast is not None:
+        return fast
     dev = _lib.require_gpu(q, k_pages, v_pages, page_table, lens, out, workspace, status)
     _no_autograd("paged_attention", q, k_pages, v_pages)
     _check_status(status)
@@ -925,8 +933,6 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if page_table.shape[0] < B:
         raise ValueError(f"page_table has {page_table.shape[0]} rows for {B} sequences")
     _check_index("lens", lens, B)
-    if window is not None and window <= 0:
-        raise ValueError(f"window must be positive or None, got {window}")
     if out is None:
         out = torch.empty((B, Hq, D), dtype=q.dtype, device=dev)
     else:
@@ -976,6 +982,12 @@ def process_logits(logits: torch.Tensor, history: Optional[torch.Tensor] = None,
     Returns a new tensor in the dtype of ``logits``, or ``out`` (which may be ``logits`` itself).  The result does not depend on any order of
     summation.
     """
+    if lookback is not None and lookback < 0:
+        raise ValueError(f"lookback must not be negative, got {lookback}")
+    fast = _lib.native().process_logits(logits, history, history_lens, repetition, 0.0 if half_life is None else half_life or -1.0, float("inf") if cap is None else cap,
+                                        presence, frequency, -1 if lookback is None else lookback, bias, allowed, out)
+    if fast is not None:
+        return fast
     settings = [t for t in (repetition, presence, frequency) if isinstance(t, torch.Tensor)]
     dev = _lib.require_gpu(logits, history, history_lens, bias, allowed, out, *settings)
     _no_autograd("process_logits", logits, bias, *settings)
@@ -1000,8 +1012,6 @@ def process_logits(logits: torch.Tensor, history: Optional[torch.Tensor] = None,
             _check_index("history_lens", history_lens, B)
     elif history_lens is not None:
         raise ValueError("history_lens needs a history")
-    if lookback is not None and lookback < 0:
-        raise ValueError(f"lookback must not be negative, got {lookback}")
     lookback = T if lookback is None else min(int(lookback), T)
     if lookback > MAX_HISTORY:
         raise ValueError(f"a history of {lookback} tokens is too long: give a lookback of at most {MAX_HISTORY}")

@@ -477,8 +477,8 @@ int daisy_gated_rmsnorm_fwd(const void* x, const void* gate, const void* weight,
  *   x' = x * rsqrt(mean(x^2) + eps) for q, k and v (eps < 0: x' = x),
  *   q, k rotated with row positions[i] of cos, sin (fp32 [table_rows, D/2], or both NULL),
  *   v = gate * v' + (1 - gate) * ve (ve and gate, one fp32, both or neither),
- * in fp32, rounded once: k and v into the pages, q into q_out (the cache's type), and k and v into k_out and
- * v_out (the inputs' type) where those are given.  A token at a negative position is skipped: nothing of it
+ * in fp32, rounded once: k and v into the pages, q into q_out (bf16 or fp16: q_out_is_f16), and k and v into k_out
+ * and v_out (the inputs' type) where those are given.  A token at a negative position is skipped: nothing of it
  * is written, except that its row of q_out becomes zero where zero_skipped is set.
  * q, k, v, ve: bf16 or fp16 (in_is_f16) [N, Hq], [N, H] heads of D with {token, head} strides; q and
  * q_out may be NULL (Hq = 0).  Two tokens of one call at the same place of the cache: either may be the one that
@@ -493,8 +493,8 @@ int daisy_paged_append_fwd(const void* q, const int64_t* q_strides, const void* 
                            const int32_t* page_table, int64_t table_stride, int n_seq, int max_pages,
                            int num_pages, int page_size,
                            const int32_t* positions, const int32_t* rows,
-                           void* q_out, const int64_t* q_out_strides, void* k_out, const int64_t* k_out_strides,
-                           void* v_out, const int64_t* v_out_strides, int zero_skipped,
+                           void* q_out, const int64_t* q_out_strides, int q_out_is_f16,
+                           void* k_out, const int64_t* k_out_strides, void* v_out, const int64_t* v_out_strides, int zero_skipped,
                            int N, int Hq, int H, int D, float eps, int32_t* status, void* stream);
 
 /* daisy_paged_attn_fwd: the attention of one new token per sequence, whose key and value are in the cache already:

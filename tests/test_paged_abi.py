@@ -22,7 +22,7 @@ def attend(q=P, qs=S2, k=P, ks=S3, v=P, table=P, stride=4, max_pages=4, num_page
 def append(q=P, k=P, v=P, table=P, stride=4, n_seq=1, max_pages=4, num_pages=8, page=16, positions=P, rows=None, q_out=P, N=1, Hq=2, H=2, D=128, ve=None, gate=None,
            cos=None, sin=None, table_rows=0, k_out=None, k_out_strides=None, ss=S2):
     return _lib.load().daisy_paged_append_fwd(q, S2, k, ss, v, S2, 0, ve, S2, gate, cos, sin, table_rows, P, S3, P, S3, 0, table, stride, n_seq, max_pages, num_pages, page,
-                                              positions, rows, q_out, S2, k_out, k_out_strides, None, None, 0, N, Hq, H, D, 1e-6, None, None)
+                                              positions, rows, q_out, S2, 0, k_out, k_out_strides, None, None, 0, N, Hq, H, D, 1e-6, None, None)
 
 
 @pytest.mark.parametrize("kw,rc,text", [

@@ -307,6 +307,8 @@ def test_append_of_packed_prompts(source, cache, D, Hq, H, page, norm, rotate, m
                            k_out=k_out, v_out=v_out, status=status)
     live = pos >= 0
     if Hq:
+        other = ops.paged_append(k, v, k_pages, v_pages, table, pos, rows=rows, q=q, cos=cos, sin=sin, eps=eps, ve=ve, gate=gate, q_out=torch.empty(N, Hq, D, dtype=source, device=DEV))
+        near(other[live], *(t[live] for t in prepared(q, pos, cos, sin, eps)), "q in the inputs' type")
         assert got.dtype == cache and bool((got[~live] == 0).all())
         want, size = prepared(q, pos, cos, sin, eps)
         near(got[live], want[live], size[live], "q")
