@@ -157,13 +157,21 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
 //
 // The work is tiles of 32 positions.  A unit is a (sequence, key head, up to 16 of its query heads); all tiles of all units, one
 // behind the other, are dealt to the wavefronts in equal runs, whatever the lengths: every wavefront reads the lengths, sums
-// them up and finds where its run begins.  A run that covers a whole unit writes the result; the others leave their partial sums,
-// at most two of a wavefront, which a second kernel joins.
+// them up and finds where its run begins.  A run that covers a whole unit writes the result; of the others partial sums stay, at most two
+// of a wavefront, which meet in the workgroup's LDS.  What of them goes on beyond the workgroup, at most one at each end, a second kernel joins.
 //
 // Both products run on 16x16x32 matrix instructions with nothing between memory and registers: S^T = K Q^T puts 16 query heads in
 // the columns (one head uses one column of 16: the products are 1/16 of use then and still far from bounding anything), so that
 // a lane holds 4 + 4 keys of one head, and those are, as they are, the B operand of O^T = V^T P^T: rows 4c + r and 16 + 4c + r of a tile for
 // the lanes of group c.  V's rows arrive 16 bytes a lane, and v_perm pairs the keys of neighbouring rows.
+// What a wavefront's run leaves open: whether it begins inside a unit, whether that goes on beyond it, whether it ends inside another one; the
+// query heads of the two, and where the second one's results belong.
+enum { kBeginsInside = 1, kGoesThrough = 2, kEndsInside = 4 };
+struct OpenUnits { int flags, heads0, heads1; int64_t out; };
+// A unit that goes on beyond a workgroup's run: the workgroups that have a part of it (first, last; -1: there is no such unit), its query heads, where
+// its results belong.
+struct SplitUnit { int first, last, heads, unused; int64_t out, unused2; };
+
 struct PagedParams {
   const uint16_t* q; int64_t q_sb, q_sh;
   const uint16_t* k; int64_t k_sp, k_sh, k_ss;
@@ -171,8 +179,9 @@ struct PagedParams {
   const int32_t* table; int64_t table_st; int max_pages, num_pages, blocks_per_page, capacity;
   const int32_t* lens;
   uint16_t* o; int64_t o_sb, o_sh;
-  float* part; float2* stat;      // [2 * wavefronts][heads of a unit][D], [..][..]: unnormalised sums; reference and sum of exponentials
-  int B, H, G, head_tiles, heads, window, waves, min_share;      // heads: of a unit, min(G, 16)
+  SplitUnit* split;               // [workgroups]
+  float* part; float2* stat;      // [2 * workgroups][heads of a unit][D], [..][..]: unnormalised sums; reference and sum of exponentials
+  int B, H, G, head_tiles, heads, window, groups;      // heads: of a unit, min(G, 16); groups: workgroups
   float scale_log2e;
   int32_t* status;
 };
@@ -193,16 +202,6 @@ __device__ __forceinline__ int wave_scan(int x) {
   x += dpp_int<0x143, 0xc>(x);      // row_bcast 31 into rows 2 and 3
   return x;
 }
-__device__ __forceinline__ float wave_max(float x) {
-  x = fmaxf(x, dpp_move<0xB1>(x));
-  x = fmaxf(x, dpp_move<0x4E>(x));
-  x = fmaxf(x, dpp_move<0x141>(x));
-  x = fmaxf(x, dpp_move<0x128>(x));
-  const LanePair r = row_pair(x);
-  const LanePair t = half_pair(fmaxf(r.x, r.y));
-  return fmaxf(t.x, t.y);
-}
-
 // The positions that a sequence's new token sees, [lo, hi), and the tiles they lie in.
 struct Extent { int lo, hi, first, tiles; bool past; };
 __device__ __forceinline__ Extent extent(const PagedParams& p, int len) {
@@ -216,13 +215,14 @@ __device__ __forceinline__ Extent extent(const PagedParams& p, int len) {
 }
 __device__ __forceinline__ int len_of(const PagedParams& p, int b) { return b < p.B ? p.lens[b] : 0; }
 
-// Tiles of all sequences (of one unit each), and how many of a unit's tiles a wavefront takes.
+// Tiles of all sequences (of one unit each).
 __device__ __forceinline__ int total_tiles(const PagedParams& p, int lane) {
   int sum = 0;
   for (int base = 0; base < p.B; base += 64) sum += extent(p, len_of(p, base + lane)).tiles;
   return __builtin_amdgcn_readlane(wave_scan(sum), 63);
 }
-__device__ __forceinline__ int share_of(const PagedParams& p, int total) { return max((total + p.waves - 1) / p.waves, p.min_share); }
+// How many tiles a wavefront takes.
+__device__ __forceinline__ int share_of(const PagedParams& p, int total) { return (total + 4 * p.groups - 1) / (4 * p.groups); }
 
 template <bool F16> __device__ __forceinline__ f32x4 mfma(const u32x4& a, const u32x4& b, const f32x4& c) {
   if constexpr (F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -243,17 +243,20 @@ __global__ __launch_bounds__(256, paged_waves_per_simd(D)) void paged_attn_kerne
   // fp16 probabilities use the type's range on both sides of one.
   constexpr float kHead = F16 ? 9.f : 0.f, kLimit = F16 ? 15.f : 8.f;
 
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+  extern __shared__ float open_sums[];      // [4 wavefronts][2][heads][D]: of the unit that the run begins in the middle of, of the one that it ends in the middle of
+  __shared__ float2 open_stats[4][2][16];
+  __shared__ OpenUnits open_units[4];
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = blockIdx.x * 4 + wv;
   const int n = lane & 15, c = lane >> 4;
   const int units = p.H * p.head_tiles;
   const int total = total_tiles(p, lane) * units;
   const int share = share_of(p, total);
-  int64_t x64 = (int64_t)wave * share;
-  if (x64 >= total) return;
-  int x = (int)x64;
-  const int x_end = (int)min(x64 + share, (int64_t)total);
+  int x = (int)min((int64_t)wave * share, (int64_t)total);
+  const int x_end = (int)min((int64_t)x + share, (int64_t)total);
+  OpenUnits mine = {0, 0, 0, 0};
+  SplitUnit beyond = {-1, 0, 0, 0, 0, 0};
 
-  const uint32_t k_off = (uint32_t)(n * p.k_ss + 8 * c) * 2, v_off = (uint32_t)(4 * c * p.v_ss + W * n) * 2;
+  const uint32_t k_row = (uint32_t)p.k_ss * 2, v_row = (uint32_t)p.v_ss * 2;      // bytes, fewer than 2^24
   int base = 0, before = 0, len = 0, tiles = 0, upto = 0, chunk = -1;      // 64 sequences from `base` on, one a lane
   while (x < x_end) {
     // ---- the unit that x lies in
@@ -303,31 +306,42 @@ __global__ __launch_bounds__(256, paged_waves_per_simd(D)) void paged_attn_kerne
     const char* vh = reinterpret_cast<const char*>(p.v + h * p.v_sh);
     u32x4 kr[2][KS];
     uint32_t vr[8][VD];
+    const int tile0 = e.first + off;
+    auto at_edge = [&](int i) { return (tile0 + i) * kTile < e.lo || (tile0 + i + 1) * kTile > e.hi; };
+    // Half `half` of tile i of the run: where its rows are, in the pages of `base`.
+    auto half_tile = [&](const char* base, int64_t sp, int64_t ss, int i, int half) {
+      const int64_t pg = __builtin_amdgcn_readlane(id, 2 * (i & 31) + half), slot = __builtin_amdgcn_readlane(in, 2 * (i & 31) + half) * kBlock;
+      return base + (pg * sp + slot * ss) * 2;
+    };
+    // A row of it, or where that is outside the range, another one that is read anyhow: nothing is fetched for the rows that a short sequence does not
+    // have, and every tile is asked for by the same instructions in the same order, which the waits for them count.
+    auto row_of = [&](int row, int i, int half) {
+      const int first = (tile0 + i) * kTile + half * kBlock;
+      return min(max(row, min(max(e.lo - first, 0), kBlock - 1)), min(max(e.hi - 1 - first, 0), kBlock - 1));
+    };
     auto load_k = [&](int i) {
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const int64_t pg = __builtin_amdgcn_readlane(id, 2 * i + half), slot = __builtin_amdgcn_readlane(in, 2 * i + half) * kBlock;
-        const char* src = kh + (pg * p.k_sp + slot * p.k_ss) * 2;
+        const char* src = half_tile(kh, p.k_sp, p.k_ss, i, half) + (__umul24(row_of(n, i, half), k_row) + 16 * c);
 #pragma unroll
-        for (int s = 0; s < KS; ++s) kr[half][s] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + k_off + 64 * s));
+        for (int s = 0; s < KS; ++s) kr[half][s] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + 64 * s));
       }
     };
     auto load_v = [&](int i) {
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const int64_t pg = __builtin_amdgcn_readlane(id, 2 * i + half), slot = __builtin_amdgcn_readlane(in, 2 * i + half) * kBlock;
-        const char* src = vh + (pg * p.v_sp + slot * p.v_ss) * 2;
+        const char* src = half_tile(vh, p.v_sp, p.v_ss, i, half);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const char* at = src + r * p.v_ss * 2;
+          const char* at = src + (__umul24(row_of(4 * c + r, i, half), v_row) + 2 * W * n);
 #pragma unroll
           for (int t = 0; t < P; ++t) {
             if constexpr (W == 8) {
-              const u32x4 d = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at + v_off + 256 * t));
+              const u32x4 d = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at + 256 * t));
 #pragma unroll
               for (int i4 = 0; i4 < 4; ++i4) vr[4 * half + r][4 * t + i4] = d[i4];
             } else {
-              const u32x2 d = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(at + v_off));
+              const u32x2 d = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(at));
               vr[4 * half + r][0] = d[0];
               vr[4 * half + r][1] = d[1];
             }
@@ -336,13 +350,11 @@ __global__ __launch_bounds__(256, paged_waves_per_simd(D)) void paged_attn_kerne
       }
     };
 
-    const int tile0 = e.first + off;
     pages_from(2 * tile0);
     load_k(0);
     load_v(0);
     for (int i = 0; i < count; ++i) {
       const int key0 = (tile0 + i) * kTile + 4 * c;
-      const bool edge = (tile0 + i) * kTile < e.lo || (tile0 + i + 1) * kTile > e.hi;
       const bool more = i + 1 < count;
       // ---- scores
       f32x4 sa = {0.f, 0.f, 0.f, 0.f}, sb = {0.f, 0.f, 0.f, 0.f};
@@ -353,13 +365,13 @@ __global__ __launch_bounds__(256, paged_waves_per_simd(D)) void paged_attn_kerne
       }
       if (more) {
         if (((i + 1) & 31) == 0) pages_from(2 * (tile0 + i + 1));
-        load_k((i + 1) & 31);
+        load_k(i + 1);
       }
       // ---- probabilities
       float s[8];
 #pragma unroll
       for (int r = 0; r < 4; ++r) { s[r] = sa[r] * p.scale_log2e; s[4 + r] = sb[r] * p.scale_log2e; }
-      if (edge) {
+      if (at_edge(i)) {
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
           const int key = key0 + (r & 3) + (r & 4) * 4;
@@ -386,7 +398,17 @@ __global__ __launch_bounds__(256, paged_waves_per_simd(D)) void paged_attn_kerne
 #pragma unroll
       for (int r = 0; r < 8; ++r) s[r] = fast_exp2(s[r] - m);
       l += ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+      // In two parts, the second what the rounding of the first has lost: the matrix pipe has time for both, and the result is as if the
+      // probabilities had not been rounded.
       const u32x4 pf = pack8_as<F16>(s);
+      u32x4 pl;
+      {
+        float f[8];
+        unpack8_as<F16>(pf, f);
+#pragma unroll
+        for (int r = 0; r < 8; ++r) f[r] = s[r] - f[r];
+        pl = pack8_as<F16>(f);
+      }
       // ---- O^T += V^T P^T
 #pragma unroll
       for (int j = 0; j < J; ++j) {
@@ -395,8 +417,9 @@ __global__ __launch_bounds__(256, paged_waves_per_simd(D)) void paged_attn_kerne
 #pragma unroll
         for (int t = 0; t < 4; ++t) vf[t] = __builtin_amdgcn_perm(vr[2 * t + 1][d], vr[2 * t][d], (j & 1) ? 0x07060302u : 0x05040100u);
         acc[j] = mfma<F16>(vf, pf, acc[j]);
+        acc[j] = mfma<F16>(vf, pl, acc[j]);
       }
-      if (more) load_v((i + 1) & 31);
+      if (more) load_v(i + 1);
     }
 
     // ---- the four groups of lanes have summed their own keys
@@ -424,8 +447,8 @@ __global__ __launch_bounds__(256, paged_waves_per_simd(D)) void paged_attn_kerne
             *reinterpret_cast<u32x4*>(dst + 128 * t + 8 * i8) = pack8_as<F16>(f);
           }
       } else {
-        const int64_t slot = (int64_t)(2 * wave + (off == 0 ? 1 : 0)) * p.heads + n;
-        float* dst = p.part + slot * D + 4 * W * c;
+        const int which = off == 0 ? 1 : 0;
+        float* dst = open_sums + ((2 * wv + which) * p.heads + n) * D + 4 * W * c;
 #pragma unroll
         for (int t = 0; t < P; ++t)
 #pragma unroll
@@ -435,101 +458,185 @@ __global__ __launch_bounds__(256, paged_waves_per_simd(D)) void paged_attn_kerne
             for (int i = 0; i < 4; ++i) f[i] = acc[t * W + (4 * i4 + i) % W][(4 * i4 + i) / W];
             *reinterpret_cast<f32x4*>(dst + 128 * t + 4 * i4) = f;
           }
-        if (c == 0) p.stat[slot] = float2{m, l};
+        if (c == 0) open_stats[wv][which][n] = float2{m, l};
       }
     }
+    if (off > 0) {
+      mine.flags |= off + count < n_tiles ? kBeginsInside | kGoesThrough : kBeginsInside;
+      mine.heads0 = min(p.G - head0, 16);
+    } else if (count < n_tiles) {
+      mine.flags |= kEndsInside;
+      mine.heads1 = min(p.G - head0, 16);
+      mine.out = b * p.o_sb + (int64_t)(h * p.G + head0) * p.o_sh;
+    }
+    if (off + count < n_tiles && wv == 3)
+      beyond = SplitUnit{(x - off) / (4 * share), (x - off + n_tiles - 1) / (4 * share), min(p.G - head0, 16), 0, b * p.o_sb + (int64_t)(h * p.G + head0) * p.o_sh, 0};
     x += count;
   }
+
+  // ---- what the wavefronts have left open: chains of the same unit, from where one of them broke off (or the workgroup began) on
+  if (lane == 0) open_units[wv] = mine;
+  if (lane == 0 && wv == 3) p.split[blockIdx.x] = beyond;
+  // (sequences without positions: dealt out one by one)
+  for (int b = blockIdx.x; b < p.B; b += p.groups) {
+    if (extent(p, p.lens[b]).tiles > 0) continue;
+    for (int i = threadIdx.x; i < p.H * p.G * (D / 8); i += 256)
+      *reinterpret_cast<u32x4*>(p.o + b * p.o_sb + (i / (D / 8)) * p.o_sh + i % (D / 8) * 8) = u32x4{0, 0, 0, 0};
+  }
+  __syncthreads();
+  for (int w = 0; w < 4; ++w) {
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      const int flags = open_units[w].flags;
+      if (which == 0 ? w > 0 || !(flags & kBeginsInside) : !(flags & kEndsInside)) continue;
+      bool on = which == 1 || (flags & kGoesThrough);
+      int last = w;
+      while (on && last < 3) on = open_units[++last].flags & kGoesThrough;
+      const int heads = which == 0 ? open_units[w].heads0 : open_units[w].heads1;
+      const int64_t slot = (int64_t)(2 * blockIdx.x + which) * p.heads;
+      for (int i = threadIdx.x; i < heads * (D / 4); i += 256) {
+        const int g = i / (D / 4), at = i % (D / 4) * 4;
+        float2 st = open_stats[w][which][g];
+        f32x4 sum = *reinterpret_cast<const f32x4*>(open_sums + ((2 * w + which) * p.heads + g) * D + at);
+        for (int y = w + 1; y <= last; ++y) {
+          const float2 more = open_stats[y][0][g];
+          const float top = fmaxf(st.x, more.x), f = fast_exp2(st.x - top), e = fast_exp2(more.x - top);
+          sum = f * sum + e * *reinterpret_cast<const f32x4*>(open_sums + (2 * y * p.heads + g) * D + at);
+          st = float2{top, f * st.y + e * more.y};
+        }
+        if (which == 1 && !on) {
+          sum *= 1.f / st.y;
+          *reinterpret_cast<u32x2*>(p.o + open_units[w].out + g * p.o_sh + at) = u32x2{pack2<F16>(sum[0], sum[1]), pack2<F16>(sum[2], sum[3])};
+        } else {
+          *reinterpret_cast<f32x4*>(p.part + (slot + g) * D + at) = sum;
+          if (at == 0) p.stat[slot + g] = st;
+        }
+      }
+    }
+  }
 }
 
-// One workgroup per (sequence, query head): joins the partial sums of a unit that was split, writes zeros for a sequence without positions.
+// Joins the partial sums of the units that lie in more than one workgroup's run.  The results of a unit are dealt to as many workgroups as there are
+// ends of runs in it: to those of the runs that it goes on beyond.
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
-  constexpr int LPR = D / 4, GROUPS = 256 / LPR;      // lanes of a row of partial sums, rows at a time
-  __shared__ float4 sums[256];
-  const int lane = threadIdx.x & 63;
-  const int q_head = blockIdx.x, b = blockIdx.y;
-  const int h = q_head / p.G, g = q_head - h * p.G, head_tile = g >> 4, n = g & 15;
-  const int units = p.H * p.head_tiles;
-  int sum = 0, first = 0;
-  for (int base = 0; base < p.B; base += 64) {
-    const int t = extent(p, len_of(p, base + lane)).tiles;
-    sum += t;
-    first += base + lane < b ? t : 0;
-  }
-  const int total = __builtin_amdgcn_readlane(wave_scan(sum), 63) * units;
-  first = __builtin_amdgcn_readlane(wave_scan(first), 63) * units;
-  const int n_tiles = extent(p, p.lens[b]).tiles;
-  uint16_t* dst = p.o + b * p.o_sb + q_head * p.o_sh;
-  if (n_tiles == 0) {
-    if (threadIdx.x < D / 8) *reinterpret_cast<u32x4*>(dst + 8 * threadIdx.x) = u32x4{0, 0, 0, 0};
+  constexpr int kFew = 8;
+  __shared__ float4 sums[4][8];
+  __shared__ float2 stats[4];
+  const SplitUnit u = p.split[blockIdx.x];
+  if (u.first < 0) return;
+  const int parts = u.last - u.first + 1, helpers = parts - 1, me = (int)blockIdx.x - u.first;
+  // the workgroup that the unit begins in has it in its second slot, where it begins with the unit too; the others in their first
+  auto slot = [&](int i, int head) { return (int64_t)(2 * (u.first + i) + (i == 0 ? 1 : 0)) * p.heads + head; };
+  if (parts <= kFew) {
+    // a thread per four channels, every part of which it asks for at once
+    for (int col = me + helpers * (int)threadIdx.x; col < u.heads * (D / 4); col += helpers * 256) {
+      const int head = col / (D / 4), at = col % (D / 4) * 4;
+      float2 st[kFew];
+      f32x4 v[kFew];
+#pragma unroll
+      for (int i = 0; i < kFew; ++i) {
+        const int64_t s = slot(min(i, parts - 1), head);
+        st[i] = p.stat[s];
+        v[i] = *reinterpret_cast<const f32x4*>(p.part + s * D + at);
+      }
+      float top = st[0].x, l = 0.f;
+#pragma unroll
+      for (int i = 1; i < kFew; ++i) top = fmaxf(top, st[i].x);
+      f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < kFew; ++i) {
+        const float f = i < parts ? fast_exp2(st[i].x - top) : 0.f;
+        l = i < parts ? fmaf(f, st[i].y, l) : l;
+        a = i < parts ? a + f * v[i] : a;
+      }
+      a *= 1.f / l;
+      *reinterpret_cast<u32x2*>(p.o + u.out + head * p.o_sh + at) = u32x2{pack2<F16>(a[0], a[1]), pack2<F16>(a[2], a[3])};
+    }
     return;
   }
-  const int share = share_of(p, total);
-  first += (h * p.head_tiles + head_tile) * n_tiles;
-  const int w0 = first / share, w1 = (first + n_tiles - 1) / share;
-  if (w0 == w1) return;
-  // the wavefront that the unit begins in has it in its second slot, where it begins with the unit too; the others in their first
-  const int parts = w1 - w0 + 1;
-  auto slot = [&](int i) { return (int64_t)(2 * (w0 + i) + (i == 0 ? 1 : 0)) * p.heads + n; };
-  float top = -__builtin_inff();
-  for (int i = lane; i < parts; i += 64) top = fmaxf(top, p.stat[slot(i)].x);
-  top = wave_max(top);
-  const int r = threadIdx.x / LPR, at = threadIdx.x % LPR;
-  float l = 0.f;
-  f32x4 a = {0.f, 0.f, 0.f, 0.f};
-  for (int i = r; i < parts; i += GROUPS) {
-    const int64_t s = slot(i);
-    const float2 st = p.stat[s];
-    const float f = fast_exp2(st.x - top);
-    l += f * st.y;
-    a += f * *reinterpret_cast<const f32x4*>(p.part + s * D + 4 * at);
+  // 32 channels at a time: eight lanes for them, 32 parts side by side
+  constexpr int U = 4;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = threadIdx.x / 8, at = threadIdx.x % 8 * 4;
+  for (int chunk = me; chunk < u.heads * (D / 32); chunk += helpers) {
+    const int head = chunk / (D / 32), d0 = chunk % (D / 32) * 32;
+    float m = -__builtin_inff(), l = 0.f;
+    f32x4 a = {0.f, 0.f, 0.f, 0.f};
+    for (int i0 = r; i0 < parts; i0 += 32 * U) {
+      float2 st[U];
+      f32x4 v[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const int64_t s = slot(min(i0 + 32 * i, parts - 1), head);
+        st[i] = p.stat[s];
+        v[i] = *reinterpret_cast<const f32x4*>(p.part + s * D + d0 + at);
+      }
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        if (i0 + 32 * i >= parts) break;
+        const float top = fmaxf(m, st[i].x), f = m > -__builtin_inff() ? fast_exp2(m - top) : 0.f, e = fast_exp2(st[i].x - top);
+        l = f * l + e * st[i].y;
+        a = f * a + e * v[i];
+        m = top;
+      }
+    }
+    // the eight parts of a wavefront (the first of which it has, as parts > 8 x 3 or not), then the wavefronts
+    auto across = [](float x, auto op) {
+      x = op(x, dpp_move<0x128>(x));
+      const LanePair r = row_pair(x);
+      const LanePair t = half_pair(op(r.x, r.y));
+      return op(t.x, t.y);
+    };
+    auto add = [](float x, float y) { return x + y; };
+    const float top = across(m, [](float x, float y) { return fmaxf(x, y); });
+    const float f = m > -__builtin_inff() ? fast_exp2(m - top) : 0.f;
+    l = across(f * l, add);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = across(f * a[i], add);
+    __syncthreads();      // (the chunk before has been read)
+    if (lane < 8) sums[wave][lane] = float4{a[0], a[1], a[2], a[3]};
+    if (lane == 0) stats[wave] = float2{top, l};
+    __syncthreads();
+    if (threadIdx.x < 8) {
+      float best = stats[0].x, all = 0.f;
+#pragma unroll
+      for (int i = 1; i < 4; ++i) best = fmaxf(best, stats[i].x);
+      a = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float w = stats[i].x > -__builtin_inff() ? fast_exp2(stats[i].x - best) : 0.f;
+        const float4 t = sums[i][threadIdx.x];
+        all = fmaf(w, stats[i].y, all);
+        a += w * f32x4{t.x, t.y, t.z, t.w};
+      }
+      a *= 1.f / all;
+      *reinterpret_cast<u32x2*>(p.o + u.out + head * p.o_sh + d0 + at) = u32x2{pack2<F16>(a[0], a[1]), pack2<F16>(a[2], a[3])};
+    }
   }
-  sums[threadIdx.x] = float4{a[0], a[1], a[2], a[3]};
-  __shared__ float ls[GROUPS];
-  if (at == 0) ls[r] = l;
-  __syncthreads();
-  if (threadIdx.x >= LPR) return;
-  l = 0.f;
-  a = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int i = 0; i < GROUPS; ++i) {
-    l += ls[i];
-    const float4 t = sums[i * LPR + at];
-    a += f32x4{t.x, t.y, t.z, t.w};
-  }
-  a *= 1.f / l;
-  *reinterpret_cast<u32x2*>(dst + 4 * at) = u32x2{pack2<F16>(a[0], a[1]), pack2<F16>(a[2], a[3])};
 }
 
-// How many wavefronts share the work, and the least number of tiles that one takes.  At least 4 tiles, and more where a unit has many
-// query heads, whose partial sums (D + 2 floats each, written and read) would otherwise outweigh the tiles (64 D bytes of K and V each).
-struct PagedSplit { int waves, min_share, heads, head_tiles; };
+// How many workgroups share the work: one round of what the chip holds, less where there are fewer tiles.
+struct PagedSplit { int groups, heads, head_tiles; size_t lds; };
 static PagedSplit paged_split(int B, int H, int G, int D, int64_t capacity) {
   PagedSplit s;
   s.head_tiles = (G + 15) / 16;
   s.heads = G < 16 ? G : 16;
-  s.min_share = s.heads <= 6 ? 4 : (2 * s.heads + 2) / 3;
+  s.lds = (size_t)8 * s.heads * D * sizeof(float);
+  const int by_lds = (int)((size_t)156 * 1024 / (s.lds + 2048)), per_cu = by_lds < paged_waves_per_simd(D) ? by_lds : paged_waves_per_simd(D);
   const int64_t tiles = ((capacity + kTile - 1) / kTile) * B * H * s.head_tiles;
-  const int64_t waves = (tiles + s.min_share - 1) / s.min_share;
-  const int64_t most = 256 * 4 * paged_waves_per_simd(D);
-  s.waves = (int)(waves < most ? waves : most);
+  const int64_t groups = (tiles + 3) / 4, most = 256 * per_cu;
+  s.groups = (int)(groups < most ? groups : most);
   return s;
 }
 
-template <bool F16> static void paged_launch(const PagedParams& p, int D, dim3 grid, dim3 join, hipStream_t s) {
-  switch (D) {
-    case 64:
-      hipLaunchKernelGGL((paged_attn_kernel<64, F16>), grid, dim3(256), 0, s, p);
-      hipLaunchKernelGGL((paged_join_kernel<64, F16>), join, dim3(256), 0, s, p);
-      break;
-    case 128:
-      hipLaunchKernelGGL((paged_attn_kernel<128, F16>), grid, dim3(256), 0, s, p);
-      hipLaunchKernelGGL((paged_join_kernel<128, F16>), join, dim3(256), 0, s, p);
-      break;
-    default:
-      hipLaunchKernelGGL((paged_attn_kernel<256, F16>), grid, dim3(256), 0, s, p);
-      hipLaunchKernelGGL((paged_join_kernel<256, F16>), join, dim3(256), 0, s, p);
-  }
+template <int D, bool F16> static void paged_launch(const PagedParams& p, size_t lds, hipStream_t s) {
+  hipLaunchKernelGGL((paged_attn_kernel<D, F16>), dim3((unsigned)p.groups), dim3(256), lds, s, p);
+  hipLaunchKernelGGL((paged_join_kernel<D, F16>), dim3((unsigned)p.groups), dim3(256), 0, s, p);
+}
+template <bool F16> static void paged_launch(const PagedParams& p, int D, size_t lds, hipStream_t s) {
+  if (D == 64) paged_launch<64, F16>(p, lds, s);
+  else if (D == 128) paged_launch<128, F16>(p, lds, s);
+  else paged_launch<256, F16>(p, lds, s);
 }
 
 template <int D> static void append_launch(const AppendParams& p, bool in16, bool cache16, hipStream_t s) {
@@ -550,8 +657,8 @@ static bool rows_of_16(const int64_t* strides, int n) {
     if (strides[i] % 8 != 0 || strides[i] < 0) return false;
   return true;
 }
-// A page's rows are reached with 32-bit byte offsets from where it begins.
-static bool page_rows_fit(const int64_t* strides) { return strides[2] <= ((int64_t)1 << 24); }
+// A page's rows are reached with 24-bit products.
+static bool page_rows_fit(const int64_t* strides) { return strides[2] < ((int64_t)1 << 23); }
 
 }  // namespace daisy
 
@@ -569,7 +676,7 @@ using namespace daisy;
                   (long long)max_pages * page_size);                                                                                      \
   DAISY_CHECK_ARG(al16(k_pages) && al16(v_pages) && rows_of_16(k_pages_strides, 3) && rows_of_16(v_pages_strides, 3) &&                    \
                       page_rows_fit(k_pages_strides) && page_rows_fit(v_pages_strides),                                                   \
-                  what ": pages must be 16-byte aligned, their strides multiples of 8 elements, a row's at most 2^24")
+                  what ": pages must be 16-byte aligned, their strides multiples of 8 elements, a row's less than 2^23")
 
 extern "C" int daisy_paged_append_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
                                       const void* v, const int64_t* v_strides, int in_is_f16,
@@ -635,7 +742,7 @@ static bool paged_shape_ok(int B, int Hq, int H, int D, int max_pages, int page_
 extern "C" size_t daisy_paged_attn_workspace_bytes(int B, int Hq, int H, int D, int max_pages, int page_size) {
   if (!paged_shape_ok(B, Hq, H, D, max_pages, page_size)) return 0;
   const PagedSplit sp = paged_split(B, H, Hq / H, D, (int64_t)max_pages * page_size);
-  return (size_t)2 * sp.waves * sp.heads * (D + 2) * sizeof(float);
+  return (size_t)sp.groups * (sizeof(SplitUnit) + 2 * sp.heads * (D + 2) * sizeof(float));
 }
 
 extern "C" int daisy_paged_attn_fwd(const void* q, const int64_t* q_strides,
@@ -651,7 +758,7 @@ extern "C" int daisy_paged_attn_fwd(const void* q, const int64_t* q_strides,
                   "paged_attn: q and o must be 16-byte aligned, their strides multiples of 8 elements");
   const int64_t capacity = (int64_t)max_pages * page_size;
   const PagedSplit sp = paged_split(B, H, Hq / H, D, capacity);
-  DAISY_CHECK_ARG((capacity / kTile + 1) * B * H * sp.head_tiles < ((int64_t)1 << 31) && B <= 65535, "paged_attn: %d sequences of up to %lld positions are too many",
+  DAISY_CHECK_ARG((capacity / kTile + 1) * B * H * sp.head_tiles < ((int64_t)1 << 31) , "paged_attn: %d sequences of up to %lld positions are too many",
                   B, (long long)capacity);
   const size_t need = daisy_paged_attn_workspace_bytes(B, Hq, H, D, max_pages, page_size);
   if (workspace == nullptr || workspace_bytes < need || !al16(workspace)) {
@@ -666,13 +773,13 @@ extern "C" int daisy_paged_attn_fwd(const void* q, const int64_t* q_strides,
   p.blocks_per_page = page_size / kBlock; p.capacity = (int)capacity;
   p.lens = lens;
   p.o = (uint16_t*)o; p.o_sb = o_strides[0]; p.o_sh = o_strides[1];
-  p.part = (float*)workspace;
-  p.stat = (float2*)(p.part + (size_t)2 * sp.waves * sp.heads * D);
-  p.B = B; p.H = H; p.G = Hq / H; p.head_tiles = sp.head_tiles; p.heads = sp.heads; p.window = window; p.waves = sp.waves; p.min_share = sp.min_share;
+  p.split = (SplitUnit*)workspace;
+  p.part = (float*)(p.split + sp.groups);
+  p.stat = (float2*)(p.part + (size_t)2 * sp.groups * sp.heads * D);
+  p.B = B; p.H = H; p.G = Hq / H; p.head_tiles = sp.head_tiles; p.heads = sp.heads; p.window = window; p.groups = sp.groups;
   p.scale_log2e = scale * kLog2e; p.status = status;
-  const dim3 grid((unsigned)((sp.waves + 3) / 4)), join((unsigned)Hq, (unsigned)B);
-  if (cache_is_f16) paged_launch<true>(p, D, grid, join, (hipStream_t)stream);
-  else paged_launch<false>(p, D, grid, join, (hipStream_t)stream);
+  if (cache_is_f16) paged_launch<true>(p, D, sp.lds, (hipStream_t)stream);
+  else paged_launch<false>(p, D, sp.lds, (hipStream_t)stream);
   DAISY_CHECK_LAUNCH("paged_attn_kernel");
   return DAISY_OK;
 }
