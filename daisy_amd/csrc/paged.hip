@@ -6,6 +6,8 @@
 // once and replayed while sequences grow, come and go.
 #include "common.h"
 
+#include <type_traits>
+
 namespace daisy {
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -352,10 +354,11 @@ __global__ __launch_bounds__(256, paged_waves_per_simd(D)) void paged_attn_kerne
 
     pages_from(2 * tile0);
     load_k(0);
+    __builtin_amdgcn_sched_barrier(0);      // K ahead of V, as in the loop: what waits for a tile's keys does not wait for its values
     load_v(0);
-    for (int i = 0; i < count; ++i) {
+    // (The last tile by itself: a wait counts what was asked for behind what it waits for, which no branch may leave open.)
+    auto step = [&](int i, auto more) {
       const int key0 = (tile0 + i) * kTile + 4 * c;
-      const bool more = i + 1 < count;
       // ---- scores
       f32x4 sa = {0.f, 0.f, 0.f, 0.f}, sb = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -363,7 +366,7 @@ __global__ __launch_bounds__(256, paged_waves_per_simd(D)) void paged_attn_kerne
         sa = mfma<F16>(kr[0][s], qf[s], sa);
         sb = mfma<F16>(kr[1][s], qf[s], sb);
       }
-      if (more) {
+      if constexpr (more.value) {
         if (((i + 1) & 31) == 0) pages_from(2 * (tile0 + i + 1));
         load_k(i + 1);
       }
@@ -419,8 +422,10 @@ __global__ __launch_bounds__(256, paged_waves_per_simd(D)) void paged_attn_kerne
         acc[j] = mfma<F16>(vf, pf, acc[j]);
         acc[j] = mfma<F16>(vf, pl, acc[j]);
       }
-      if (more) load_v(i + 1);
-    }
+      if constexpr (more.value) load_v(i + 1);
+    };
+    for (int i = 0; i + 1 < count; ++i) step(i, std::true_type());
+    step(count - 1, std::false_type());
 
     // ---- the four groups of lanes have summed their own keys
     {
