@@ -27,7 +27,7 @@ from torch import Tensor, nn
 
 from . import _lib, ops
 from .functional import NORM_EPS_BF16, init_linear, norm
-from .kv_cache import RingContext
+from .kv_cache import PagedContext, RingContext
 
 
 @dataclass
@@ -46,11 +46,14 @@ class WindowMask:
     bound will do).  It changes no row; without a ``window`` the attention kernel takes it as one, and orders its
     blocks and tiles by it (T = 32768, 8 heads of 128, rows bounded by 8 and by 4 key blocks of 128: 156 -> 137 and
     95 -> 80 us).
+    ``paged``: the call's tokens are prompts packed behind one another, whose keys and values go into a ``PagedKVCache`` layer at
+    positions of their own (``core.admit`` sets it per layer).
     """
     window: Optional[int]
     doc_start: Optional[Tensor] = None
     kv_out: Optional[Tuple[Tensor, Tensor]] = None
     span: Optional[int] = None
+    paged: Optional[PagedContext] = None
 
 
 def doc_start_from_ids(input_seq: Tensor, eos_token_id: int) -> Tensor:
@@ -349,8 +352,9 @@ def _held(store: dict, module: nn.Module, name: str):
 class CausalSelfAttention(nn.Module):
     """Merged-QKVO sliding-window causal self-attention (models/daisy/attention.py:73-202)."""
 
-    # step() takes a KVCache layer handle (RingContext) in place of chronological k_ctx / v_ctx.
+    # step() takes a KVCache layer handle (RingContext) in place of chronological k_ctx / v_ctx, or a PagedKVCache layer's.
     accepts_ring_context = True
+    accepts_paged_context = True
 
     def __init__(self, dim: int, num_heads: int, head_dim, receives_ve: bool = False,
                  layer_idx: Optional[int] = None, max_seq_len: int = 131072):
@@ -437,6 +441,8 @@ class CausalSelfAttention(nn.Module):
         if mask.doc_start is not None and mask.doc_start.device != x.device:    # e.g. converted from a mask built on the CPU
             mask = replace(mask, doc_start=mask.doc_start.to(x.device))
         window = mask.window or mask.span
+        if mask.paged is not None:
+            return self._attend_paged(x, ve, mask, window)
         dest = kv_out if kv_out is not None else mask.kv_out
         if self._fused_prep_ok():
             rot = _held(self._modules, self, "rotary")
@@ -476,6 +482,44 @@ class CausalSelfAttention(nn.Module):
         q_rot = _apply_rope(q, cos[None, :, None, :], sin[None, :, None, :]) if want_q else None
         return y, q_rot, k_rot.to(dtype).transpose(1, 2), v.transpose(1, 2)
 
+    def _append_paged(self, x: Tensor, ve: Optional[Tensor], ctx: PagedContext, prompt: bool):
+        """QKV projection of the tokens ``x [N, dim]``, norm, rotation at each token's position, value mix and the way into the pages; the
+        prepared queries ``[N, H, D]`` in the cache's dtype, or, for a prompt, q, k and v in bf16."""
+        if not self._fused_prep_ok():
+            raise ValueError("a paged cache needs the fused kernels (bf16 weights, head dim 64 or 128)")
+        N, H, D = x.size(0), self.num_heads, self.head_dim
+        qkv = step_linear(_as_bf16(x), self.qkvo_w[:3].flatten(end_dim=1)).view(N, 3 * H, D)
+        gate = None
+        if self.receives_ve:
+            torch._assert(ve is not None, "ve must be provided when receives_ve=True")
+            ve = _as_bf16(ve).view(N, H, D)
+            gate = torch.sigmoid(self.g_ve.detach()).to(torch.bfloat16).float().reshape(1)
+        else:
+            ve = None
+        out = torch.empty(3, N, H, D, dtype=torch.bfloat16, device=x.device) if prompt else (None, None, None)
+        q = ops.paged_append(qkv[:, H:2 * H], qkv[:, 2 * H:], ctx.k_pages, ctx.v_pages, ctx.page_table, ctx.positions, rows=ctx.rows, q=qkv[:, :H],
+                             cos=self.rotary.cos, sin=self.rotary.sin, eps=NORM_EPS_BF16, ve=ve, gate=gate, q_out=out[0], k_out=out[1], v_out=out[2],
+                             status=ctx.status)
+        return (q, out[1], out[2]) if prompt else q
+
+    def _attend_paged(self, x: Tensor, ve: Optional[Tensor], mask: WindowMask, window: Optional[int]):
+        """``_attend`` for prompts packed behind one another, ``x [1, N, dim]``."""
+        torch._assert(x.size(0) == 1, "packed prompts come as a batch of one")
+        q, k, v = self._append_paged(x[0], None if ve is None else ve[0], mask.paged, True)
+        o, _ = ops.prefill_attention(q[None], k[None], v[None], window=window, scale=self.attn_scale, doc_start=mask.doc_start)
+        y = step_linear(o.view(1, -1, self.m_dim), self.qkvo_w[3])
+        return y, q[None], k[None].transpose(1, 2), v[None].transpose(1, 2)
+
+    def _step_paged(self, x: Tensor, ctx: PagedContext, ve: Optional[Tensor], window: Optional[int]):
+        """One token of every sequence of a paged cache, at the positions that the device holds."""
+        if ctx.window is not None and (window is None or window > ctx.window):
+            raise ValueError(f"the paged cache keeps {ctx.window} positions, a window of {window} was asked for")
+        B = x.size(0)
+        q = self._append_paged(x[:, 0], ve, ctx, False)
+        o = ops.paged_attention(q, ctx.k_pages, ctx.v_pages, ctx.page_table, ctx.lens, window=window, scale=self.attn_scale, status=ctx.status)
+        y = step_linear(_as_bf16(o).reshape(B, 1, self.m_dim), self.qkvo_w[3])
+        return y, None, None
+
     # -- reference interface -----------------------------------------------
     def forward(self, x: Tensor, ve: Optional[Tensor], block_mask=None, attn_mask: MaskLike = None):
         """``block_mask``: a ``WindowMask``, or the ``flex_attention`` ``BlockMask`` the reference's
@@ -502,7 +546,7 @@ class CausalSelfAttention(nn.Module):
             self.last_k = k_rows.clone() if aliased else k_rows
         return y, k, v
 
-    def step(self, x, k_ctx: Union[Tensor, RingContext], v_ctx: Union[Tensor, RingContext], pos: Union[int, Tensor],
+    def step(self, x, k_ctx: Union[Tensor, RingContext, PagedContext], v_ctx: Union[Tensor, RingContext, PagedContext], pos: Union[int, Tensor],
              ve: Optional[Tensor], window: Optional[int]):
         """One token: returns ``y [B, 1, dim]``, ``k [B, 1, H, D]``, ``v [B, 1, H, D]``.
 
@@ -514,9 +558,14 @@ class CausalSelfAttention(nn.Module):
         ``pos`` may be a one-element int32 device tensor (with a ``RingContext`` only): nothing on
         the host then depends on the position, so the step can be recorded in a HIP graph and
         replayed while the tensor counts up.
+
+        With the ``PagedContext`` of a ``PagedKVCache`` layer every sequence is at a position of its own: ``pos`` is not looked at, the new rows
+        go into the pages, and ``None, None`` is returned for them.
         """
         B = x.size(0)
         torch._assert(x.size(1) == 1, "step() requires single position only")
+        if isinstance(k_ctx, PagedContext):
+            return self._step_paged(x, k_ctx, ve, window)
         fused = self._fused_prep_ok()
         ring = k_ctx if isinstance(k_ctx, RingContext) else None
         # the one-launch step streams a bf16 ring, or an fp16 one (the reference generator's default)

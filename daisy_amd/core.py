@@ -11,14 +11,15 @@ model attributes (``embed``, ``blocks``, ``skip_map``, ``skip_weights``, ``ve_mo
 * write each layer's keys and values straight into the ring cache as the layer finishes
   (nothing of size ``L * T`` is ever stacked; a prompt shorter than the ring is written into its
   slots by the pre-attention kernel itself, with no copy at all), and
-* accept a batch of sequences (the cache has a batch dimension; the reference pins B = 1).
+* accept a batch of sequences (the cache has a batch dimension; the reference pins B = 1), or, with a
+  ``PagedKVCache``, sequences of unequal length that come and go (``admit``, then ``step`` for all of them).
 
 They work on the reference's ``DaisyCore`` once its blocks hold this package's
 ``CausalSelfAttention``, and on any module with the same attributes.
 """
 from __future__ import annotations
 
-from typing import Dict, List, Optional, Tuple
+from typing import Dict, List, Optional, Sequence, Tuple, Union
 
 import dataclasses
 
@@ -28,7 +29,7 @@ from torch import Tensor
 
 from .attention import CausalSelfAttention, WindowMask, step_linear, build_window_mask
 from .functional import norm
-from .kv_cache import KVCache
+from .kv_cache import KVCache, PagedKVCache
 
 
 def _value_embeddings(model, ids: Tensor) -> Dict[int, Tensor]:
@@ -110,14 +111,81 @@ def prefill(model, input_seq: Tensor, cache: Optional[KVCache] = None, debug: bo
 
 
 @torch.no_grad()
-def step(model, token_ids: Tensor, cache: KVCache) -> Tensor:
+def admit(model, prompts: Sequence[Tensor], cache: PagedKVCache) -> Tuple[Tensor, List[int]]:
+    """Runs new sequences' prompts (1-D token tensors of any lengths) and puts them into free slots of a paged cache: the logits of
+    their last positions ``[n, V]``, and the slots.
+
+    The prompts run packed behind one another, without padding: one row of all their tokens, each prompt a document of its own (an
+    end-of-sequence token inside a prompt opens another one, as in ``prefill``), each token at its position in its prompt.
+    """
+    torch._assert(len(prompts) > 0 and all(p.ndim == 1 and p.numel() > 0 for p in prompts), "prompts must be token vectors that are not empty")
+    layers = [getattr(blk, "attn", None) for blk in model.blocks]
+    _check_paged(layers)
+    if any(attn is not None and not attn._fused_prep_ok() for attn in layers):
+        raise ValueError("a paged cache needs the fused kernels (bf16 weights, head dim 64 or 128)")
+    rotary = [attn.rotary.cos.shape[0] for attn in layers if attn is not None]
+    lengths = [p.numel() for p in prompts]
+    torch._assert(max(lengths) <= min(rotary, default=max(lengths)), f"Rotary buffers too small {min(rotary, default=0)} < {max(lengths)}")
+    slots = cache.admit(lengths)
+    try:
+        return _walk_prompts(model, prompts, lengths, slots, cache), slots
+    except BaseException:
+        for slot in slots:
+            cache.release(slot)
+        raise
+
+
+def _walk_prompts(model, prompts: Sequence[Tensor], lengths: List[int], slots: List[int], cache: PagedKVCache) -> Tensor:
+    """The layer walk of ``admit``: the logits of the prompts' last positions."""
+    dev = cache.k.device
+    ids = torch.cat([p.to(dev) for p in prompts])[None]
+    n = torch.tensor(lengths, device=dev)
+    start = torch.cumsum(n, 0) - n
+    at = torch.arange(ids.size(1), device=dev)
+    of = torch.repeat_interleave(torch.arange(len(prompts), device=dev), n, output_size=ids.size(1))
+    positions = (at - start[of]).to(torch.int32)
+    rows = torch.tensor(slots, device=dev)[of].to(torch.int32)
+    doc_start = torch.cummax(torch.where((ids[0] == model.eos_token_id) | (positions == 0), at, torch.zeros_like(at)), 0).values.to(torch.int32)
+    window = getattr(model, "window_size", None)
+    x = x0 = norm(model.embed(ids))
+    skip_map, skip_weights = model.skip_map, model.skip_weights
+    ve_map = _value_embeddings(model, ids)
+    skip_connections = []
+    for i, blk in enumerate(model.blocks):
+        if i in skip_map:
+            gate = torch.sigmoid(skip_weights[skip_map[i]])
+            x = x * gate + (1 - gate) * skip_connections[skip_map[i]]
+        mask = WindowMask(window, doc_start, span=max(lengths), paged=cache.context(i, positions, rows))
+        x, _, _ = blk.prefill(x, ve_map.get(i), x0, attn_mask=mask, debug=False)
+        skip_connections.append(x)
+    x = norm(x[0, start + n - 1])
+    return F.linear(x.bfloat16(), model.lm_head_w.bfloat16()).float()
+
+
+def _check_paged(layers) -> None:
+    for attn in layers:
+        if attn is not None and not getattr(attn, "accepts_paged_context", False):
+            raise ValueError(f"a paged cache needs attention layers that take its pages, not {type(attn).__name__}")
+
+
+@torch.no_grad()
+def step(model, token_ids: Tensor, cache: Union[KVCache, PagedKVCache]) -> Tensor:
     """``DaisyCore.step`` (daisy_core.py:294-323) for one new token per sequence, ``token_ids [B]``
     (or a 0-dim tensor when B = 1), at position ``cache.t``.
 
     Each attention layer streams its ring in place and appends the new row itself (bf16 cache and
     this package's attention), or gets the chronological view and the row is written here.
     Advances the cache; returns ``logits [B, V]``.
+
+    With a ``PagedKVCache``, B is the number of its slots and every sequence is at a position of its own; the logits of free
+    slots mean nothing.  What only the device can see is reported by ``cache.check()``.
     """
+    if isinstance(cache, PagedKVCache):
+        _check_paged(getattr(blk, "attn", None) for blk in model.blocks)
+        cache.begin_step()
+        logits = _walk_step(model, token_ids, cache, 0)
+        cache.advance()
+        return logits
     logits = _walk_step(model, token_ids, cache, cache.t)
     cache.advance()
     return logits
@@ -129,12 +197,13 @@ def _walk_step(model, token_ids: Tensor, cache: KVCache, pos, status: Optional[T
     ``status``: the int32 word in which the attention kernels report a device position they cannot use."""
     token_ids = token_ids.reshape(-1, 1)
     B = token_ids.size(0)
-    torch._assert(B == cache.B, "token batch does not match the cache")
+    paged = isinstance(cache, PagedKVCache)
+    torch._assert(B == (cache.sequences if paged else cache.B), "token batch does not match the cache")
     on_device = isinstance(pos, Tensor)
     x = x0 = norm(model.embed(token_ids))
     skip_map, skip_weights = model.skip_map, model.skip_weights
     ve_map = _value_embeddings(model, token_ids)
-    window = getattr(model, "attn_window_size", cache.W)
+    window = getattr(model, "attn_window_size", cache.window if paged else cache.W)
     in_place = cache.dtype in (torch.bfloat16, torch.float16)
     skip_connections = []
     # (A module's children and a list of modules are looked up by name on every access: four lookups of the attention and an index a
@@ -146,6 +215,8 @@ def _walk_step(model, token_ids: Tensor, cache: KVCache, pos, status: Optional[T
         attn = getattr(blk, "attn", None)
         if attn is None or not getattr(attn, "uses_kv_context", True):
             k_ctx = v_ctx = None        # no attention, or one that keeps its own state (KDA layers)
+        elif paged:
+            k_ctx = v_ctx = cache.context(i)
         elif in_place and getattr(attn, "accepts_ring_context", False):
             k_ctx = v_ctx = cache.ring(i)
             k_ctx.status = status
@@ -154,7 +225,7 @@ def _walk_step(model, token_ids: Tensor, cache: KVCache, pos, status: Optional[T
             k_ctx, v_ctx = cache.view(i)
         x, k_new, v_new = blk.step(x, ve_map.get(i), x0, k_ctx, v_ctx, pos, window)
         skip_connections.append(x)
-        if k_new is not None and not cache._staged[i]:
+        if k_new is not None and not paged and not cache._staged[i]:
             torch._assert(not on_device, "a recorded step needs attention layers that write the ring themselves")
             cache.write(i, k_new.to(cache.dtype), v_new.to(cache.dtype))
     x = norm(x)
@@ -263,6 +334,46 @@ class GraphedStep:
         self._graph.replay()
         cache.advance()
         self._pos_host = cache.t
+        return self._logits
+
+
+class GraphedPagedStep:
+    """``step(model, tokens, cache)`` with a ``PagedKVCache`` recorded once as a HIP graph and replayed for every later step, while
+    sequences grow, are admitted and released: the recorded launches read the table, positions and lengths from the cache's tensors, whose addresses
+    do not change.  The returned logits are a buffer that the next call overwrites.
+    """
+
+    def __init__(self, model, cache: PagedKVCache):
+        _check_paged(getattr(blk, "attn", None) for blk in model.blocks)
+        self.model, self.cache = model, cache
+        self.tokens = torch.zeros(cache.sequences, dtype=torch.long, device=cache.k.device)
+        self._graph: Optional[torch.cuda.CUDAGraph] = None
+        self._logits: Optional[Tensor] = None
+
+    def check(self) -> None:
+        self.cache.check()
+
+    def _record(self) -> None:
+        dev = self.cache.k.device
+        # One eager pass on a side stream first; it writes the rows that the first replay writes again.
+        side = torch.cuda.Stream(device=dev)
+        side.wait_stream(torch.cuda.current_stream(dev))
+        with torch.cuda.stream(side):
+            _walk_step(self.model, self.tokens, self.cache, 0)
+        torch.cuda.current_stream(dev).wait_stream(side)
+        self._graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(self._graph):
+            self._logits = _walk_step(self.model, self.tokens, self.cache, 0)
+            self.cache.count_on_device()
+
+    @torch.no_grad()
+    def __call__(self, token_ids: Tensor) -> Tensor:
+        self.cache.begin_step()
+        self.tokens.copy_(token_ids.reshape(-1))
+        if self._graph is None:
+            self._record()
+        self._graph.replay()
+        self.cache.advance(on_device=False)
         return self._logits
 
 

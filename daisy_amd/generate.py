@@ -16,18 +16,21 @@ What is arranged differently here:
 
 Sampling follows the reference's arithmetic (inference/generate.py:13-58): temperature, top-k,
 nucleus filter, Gumbel-max draw, and the distance-decayed repetition penalty over the last 128
-tokens; the random numbers are drawn with the same call, so a seed gives the same tokens.
+tokens; the random numbers are drawn with the same call, so a seed gives the same tokens.  Beyond it: presence and frequency
+penalties, biases and a mask of the tokens that may follow (a grammar's, say), in one launch with the repetition penalty, and
+prompts of unequal length (``generate_ragged``).
 """
 from __future__ import annotations
 
 import time
-from typing import Iterator, List, Optional, Tuple
+from typing import Callable, Dict, Iterator, List, Optional, Sequence, Tuple, Union
 
 import torch
 from torch import Tensor
 
+from . import ops
 from .attention import CausalSelfAttention
-from .kv_cache import KVCache
+from .kv_cache import KVCache, PagedKVCache
 
 _NEG_INF = float("-inf")
 _PENALTY_LOOKBACK = 128      # tokens of history the repetition penalty looks at (generate.py:271)
@@ -98,7 +101,9 @@ def penalise_repeats(logits: Tensor, recent: Tensor, strength: Tensor, _one: Opt
 class Generator:
     def __init__(self, model, window, seed, device=None, dtype=torch.float16, max_seq_len: int = 65536,
                  temperature=1.0, top_k=None, top_p=None, repetition_penalty=1.0, eos_token_id=None,
-                 record_steps: bool = False, direct_prefill: bool = False):
+                 record_steps: bool = False, direct_prefill: bool = False, presence_penalty: float = 0.0, frequency_penalty: float = 0.0,
+                 logit_bias: Union[None, Dict[int, float], Tensor] = None,
+                 allowed_tokens: Optional[Callable[[Tensor, Tensor], Optional[Tensor]]] = None):
         eos = eos_token_id if eos_token_id is not None else getattr(model, "eos_token_id", None)
         if eos is None:
             raise AssertionError("eos_token_id must be given or be an attribute of the model")
@@ -139,6 +144,14 @@ class Generator:
         # generate_batch: one bf16 ring, and one recorded step, per batch size
         self._batch_caches: dict = {}
         self._batch_steps: dict = {}
+        # generate_ragged: the paged cache of the last call and its recorded step
+        self._paged_cache: Optional[PagedKVCache] = None
+        self._paged_step = None
+        # What ops.process_logits adds to the repetition penalty, over the same last tokens: a bias per token ({id: value} or [vocab]), and
+        # allowed_tokens(seen [B, T], lens [B]) -> which tokens may follow, bool [B, vocab] or bits (ops.pack_allowed), or None for all.
+        self.presence_penalty, self.frequency_penalty = float(presence_penalty), float(frequency_penalty)
+        self.allowed_tokens = allowed_tokens
+        self.logit_bias = self._bias_row(logit_bias)
 
         torch.manual_seed(seed)
         self._tokens = torch.empty(256, dtype=torch.long, device=self.device)
@@ -193,6 +206,32 @@ class Generator:
         if self._rep_p_host == 1.0 and self.apply_repetition_penalty is penalise_repeats:
             return logits
         return self.apply_repetition_penalty(logits, recent, self.rep_p_t, self._one)
+
+    def _bias_row(self, bias) -> Optional[Tensor]:
+        if bias is None or isinstance(bias, Tensor):
+            return None if bias is None else bias.to(device=self.device, dtype=torch.float32).reshape(self.vocab_size).contiguous()
+        row = torch.zeros(self.vocab_size, dtype=torch.float32)
+        for token, value in bias.items():
+            if not 0 <= token < self.vocab_size:
+                raise ValueError(f"logit_bias names token {token} of a vocabulary of {self.vocab_size}")
+            row[token] = value
+        return row.to(self.device)
+
+    def _adjusts_logits(self) -> bool:
+        return self.presence_penalty != 0.0 or self.frequency_penalty != 0.0 or self.logit_bias is not None or self.allowed_tokens is not None
+
+    def _adjusted(self, logits: Tensor, seen: Tensor, lens: Tensor) -> Tensor:
+        """Penalties, bias and mask on ``logits [B, V]`` after the tokens ``seen [B, T]``, ``lens [B]`` (int32) of each row, in one launch."""
+        strength = self._rep_p_host
+        if self.apply_repetition_penalty is not penalise_repeats:
+            raise ValueError("a repetition routine of the caller's does not combine with presence and frequency penalties, biases, masks or prompts of unequal length")
+        allowed = None
+        if self.allowed_tokens is not None:
+            allowed = self.allowed_tokens(seen, lens)
+            if allowed is not None and allowed.dtype == torch.bool:
+                allowed = ops.pack_allowed(allowed)
+        return ops.process_logits(logits, seen, lens, repetition=strength, half_life=140.0, cap=3.0, presence=self.presence_penalty,
+                                  frequency=self.frequency_penalty, lookback=_PENALTY_LOOKBACK, bias=self.logit_bias, allowed=allowed)
 
     # -- model calls -----------------------------------------------------------------------
     def _prefill(self, prompt_ids: Tensor) -> Tensor:
@@ -263,7 +302,11 @@ class Generator:
         self._sync()
         t_prompt = time.perf_counter()
         for produced in range(1, max_new_tokens + 1):
-            scores = self._penalised(logits[-1], self.history[-_PENALTY_LOOKBACK:])
+            if self._adjusts_logits():
+                seen = torch.full((1,), self._n_tokens, dtype=torch.int32, device=self.device)
+                scores = self._adjusted(logits[-1:], self.history[None], seen)[0]
+            else:
+                scores = self._penalised(logits[-1], self.history[-_PENALTY_LOOKBACK:])
             token = self.sample(scores, self.temperature, self.top_k, self.top_p)
             if token == self.eos_token_id:
                 break
@@ -312,7 +355,10 @@ class Generator:
         done = torch.zeros(B, dtype=torch.bool, device=self.device)
         for produced in range(1, max_new_tokens + 1):
             scores = self._trim(logits)
-            scores = self._penalised(scores, seen[:, max(n_seen - _PENALTY_LOOKBACK, 0):n_seen])
+            if self._adjusts_logits():
+                scores = self._adjusted(scores, seen[:, :n_seen], torch.full((B,), n_seen, dtype=torch.int32, device=self.device))
+            else:
+                scores = self._penalised(scores, seen[:, max(n_seen - _PENALTY_LOOKBACK, 0):n_seen])
             token = self.sample(scores, self.temperature, self.top_k, self.top_p)
             token = torch.where(done, eos, token)
             done |= token == eos
@@ -321,3 +367,46 @@ class Generator:
             if produced < max_new_tokens:
                 logits = step(token)
         return seen[:, ids.size(1):n_seen].clone()
+
+    @torch.inference_mode()
+    def generate_ragged(self, prompts: Sequence[Tensor], max_new_tokens: int, record_steps: bool = False) -> Tensor:
+        """Prompts of unequal length (1-D token tensors) -> ``[B, max_new_tokens]`` ids, with the same sampling settings as
+        ``generate``; a row that produces the end-of-sequence token keeps emitting it.
+
+        The prompts run packed, without padding, into a bf16 paged cache (``core.admit``), every step runs all sequences at positions of their
+        own (``core.step``; ``record_steps``: recorded once as a HIP graph and replayed).  The model needs what ``generate_batch`` needs.
+        """
+        from . import core
+        assert len(prompts) > 0 and all(p.ndim == 1 and p.numel() > 0 for p in prompts) and max_new_tokens > 0
+        B, lengths = len(prompts), [p.numel() for p in prompts]
+        longest = max(lengths) + max_new_tokens
+        cache, size = self._paged_cache, 64
+        pages = sum(-(-(n + max_new_tokens) // size) for n in lengths)
+        if cache is None or cache.sequences != B or cache.pages < pages or cache.max_len < longest:
+            cache = self._paged_cache = PagedKVCache(L=self.cache.L, sequences=B, H=self.cache.H, D=self.cache.D, pages=pages, device=self.device,
+                                                     dtype=torch.bfloat16, page_size=size, max_len=longest)
+            self._paged_step = None
+        for slot in range(B):
+            if cache.length(slot) is not None:
+                cache.release(slot)
+        if record_steps and self._paged_step is None:
+            self._paged_step = core.GraphedPagedStep(self.model, cache)
+        step = self._paged_step if record_steps else lambda tokens: core.step(self.model, tokens, cache)
+        logits, _ = core.admit(self.model, prompts, cache)      # (all slots are free: sequence i is in slot i)
+        seen = torch.zeros(B, longest, dtype=torch.long, device=self.device)
+        for row, prompt in zip(seen, prompts):
+            row[:prompt.numel()] = prompt
+        lens = torch.tensor(lengths, dtype=torch.int32, device=self.device)
+        first = lens.long()
+        eos = self.eos_token_id.to(torch.long)
+        done = torch.zeros(B, dtype=torch.bool, device=self.device)
+        for produced in range(1, max_new_tokens + 1):
+            scores = self._adjusted(self._trim(logits), seen, lens)
+            token = self.sample(scores, self.temperature, self.top_k, self.top_p)
+            token = torch.where(done, eos, token)
+            done |= token == eos
+            seen.scatter_(1, lens.long()[:, None], token[:, None])
+            lens += 1
+            if produced < max_new_tokens:
+                logits = step(token)
+        return seen.gather(1, first[:, None] + torch.arange(max_new_tokens, device=self.device))

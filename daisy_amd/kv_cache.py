@@ -11,7 +11,7 @@ writes the new row itself, and no chronological copy is ever made.
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Optional, Tuple
+from typing import Dict, List, Optional, Tuple
 
 import torch
 from torch import Tensor
@@ -130,3 +130,163 @@ class KVCache:
         for src, slots in self._prompt_runs(pos):
             self.k[layer][:, :, slots].copy_(k[:, :, src])
             self.v[layer][:, :, slots].copy_(v[:, :, src])
+
+
+# ----------------------------------------------------------------------------------------------
+# sequences of unequal length
+# ----------------------------------------------------------------------------------------------
+@dataclass
+class PagedContext:
+    """Handle to one layer of a ``PagedKVCache`` for one call: ``k_pages``/``v_pages`` ``[pages, H, page_size, D]`` (views), the
+    cache's ``page_table``, the ``positions`` of the call's tokens and, for a prompt, the sequences (``rows``) that they belong to;
+    for a step the sequences' lengths with the new token (``lens``)."""
+    k_pages: Tensor
+    v_pages: Tensor
+    page_table: Tensor
+    positions: Tensor
+    lens: Optional[Tensor]
+    rows: Optional[Tensor]
+    status: Optional[Tensor]
+    window: Optional[int]
+
+
+class PagedKVCache:
+    """A key-value cache for sequences of unequal length that come and go (the reference's cache has one position for the whole
+    batch, inference/kv_cache.py:4-68).
+
+    Storage is a pool of ``pages`` pages, ``k, v [L, pages, H, page_size, D]`` (bf16 or fp16); each of the ``sequences`` slots owns the pages
+    that its row of ``page_table`` names, for up to ``max_len`` positions.  A step runs all slots at once; free ones are
+    skipped.  With ``window``, pages that no step can see any more go back to the pool.
+
+    The host knows every length, so that ``admit`` and ``begin_step`` raise where the pool is empty; the device has the table, the next token's
+    ``positions`` (-1 for a free slot) and the ``lens`` with it, at fixed addresses, for steps recorded in a HIP graph.
+    """
+
+    def __init__(self, L, sequences, H, D, pages, device, dtype, page_size: int = 64, max_len: int = 65536, window: Optional[int] = None):
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError(f"a paged cache holds bfloat16 or float16, got {dtype}")
+        if page_size <= 0 or page_size % 16 != 0:
+            raise ValueError(f"page_size must be a multiple of 16, got {page_size}")
+        if min(L, sequences, H, D, pages, max_len) <= 0 or (window is not None and window <= 0):
+            raise ValueError("a paged cache needs positive sizes")
+        self.L, self.sequences, self.H, self.D, self.pages, self.page_size = L, sequences, H, D, pages, page_size
+        self.max_len, self.window, self.device, self.dtype = max_len, window, device, dtype
+        self.k = torch.empty((L, pages, H, page_size, D), device=device, dtype=dtype)
+        self.v = torch.empty_like(self.k)
+        width = -(-max_len // page_size)
+        self.page_table = torch.full((sequences, width), -1, device=device, dtype=torch.int32)
+        self.positions = torch.full((sequences,), -1, device=device, dtype=torch.int32)
+        self.lens = torch.zeros(sequences, device=device, dtype=torch.int32)
+        self.status = torch.zeros(1, device=device, dtype=torch.int32)      # raised by the kernels, see check()
+        self._live = torch.zeros(sequences, device=device, dtype=torch.int32)
+        self._free = list(range(pages - 1, -1, -1))
+        self._length: List[Optional[int]] = [None] * sequences               # None: a free slot
+        self._owned: List[Dict[int, int]] = [{} for _ in range(sequences)]    # entry of the table -> page
+        self._reach: List[int] = [0] * sequences                             # entries that each slot has taken so far
+        self._changes: Dict[int, int] = {}                                   # flat entry -> page, not on the device yet
+
+    # -- what there is -----------------------------------------------------------------------
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def length(self, slot: int) -> Optional[int]:
+        """Positions of a sequence, ``None`` for a free slot."""
+        return self._length[slot]
+
+    def check(self) -> None:
+        """Raises what the kernels reported (a position past the rotary tables, say).  Synchronises."""
+        from . import ops
+        ops.raise_for_status(self.status)
+
+    # -- slots and pages -----------------------------------------------------------------------
+    def _take(self, wanted: Dict[int, range], left: Dict[int, List[int]]) -> None:
+        """Gives every slot the entries that it wants and takes those that it has left behind, or raises and changes nothing."""
+        count, back = sum(len(e) for e in wanted.values()), sum(len(e) for e in left.values())
+        if count > len(self._free) + back:
+            raise RuntimeError(f"the paged cache is full: {count} pages wanted, {len(self._free) + back} of {self.pages} free")
+        for slot, entries in left.items():
+            for entry in entries:
+                self._set(slot, entry, -1)
+        for slot, entries in wanted.items():
+            for entry in entries:
+                self._set(slot, entry, self._free.pop())
+            self._reach[slot] = entries.stop
+
+    def _set(self, slot: int, entry: int, page: int) -> None:
+        if page < 0:
+            self._free.append(self._owned[slot].pop(entry))
+        else:
+            self._owned[slot][entry] = page
+        self._changes[slot * self.page_table.shape[1] + entry] = page
+
+    def _upload(self) -> None:
+        """The table's changes, in one copy that the host does not wait for."""
+        if not self._changes:
+            return
+        both = torch.tensor([list(self._changes.keys()), list(self._changes.values())], dtype=torch.int64, pin_memory=self.page_table.is_cuda)
+        both = both.to(self.page_table.device, non_blocking=True)
+        self.page_table.view(-1).scatter_(0, both[0], both[1].to(torch.int32))
+        self._changes.clear()
+
+    def admit(self, lengths: List[int]) -> List[int]:
+        """Free slots for new sequences of these many positions each, with pages for them: the slots, in order.  The positions are
+        to be filled (``ops.paged_append``, ``core.admit``) before the next step."""
+        slots = [s for s, n in enumerate(self._length) if n is None][:len(lengths)]
+        if len(slots) < len(lengths):
+            raise RuntimeError(f"the paged cache has {len(slots)} free slots for {len(lengths)} sequences")
+        for n in lengths:
+            if not 0 < n <= self.max_len:
+                raise ValueError(f"a sequence must have 1 to {self.max_len} positions, got {n}")
+        self._take({s: range(-(-n // self.page_size)) for s, n in zip(slots, lengths)}, {})
+        for s, n in zip(slots, lengths):
+            self._length[s] = n
+        self._upload()
+        at = torch.tensor(slots, device=self.page_table.device)
+        self.positions[at] = torch.tensor(lengths, dtype=torch.int32, device=self.page_table.device)
+        self.lens[at] = self.positions[at] + 1
+        self._live[at] = 1
+        return slots
+
+    def release(self, slot: int) -> None:
+        """Ends a sequence: its pages go back, later steps skip the slot."""
+        if self._length[slot] is None:
+            raise ValueError(f"slot {slot} has no sequence")
+        for entry in list(self._owned[slot]):
+            self._set(slot, entry, -1)
+        self._length[slot], self._reach[slot] = None, 0
+        self._upload()
+        self.positions[slot], self.lens[slot], self._live[slot] = -1, 0, 0
+
+    def begin_step(self) -> None:
+        """Makes room for one more position of every sequence, from the pages that a window has left behind and the pool."""
+        wanted, left = {}, {}
+        for slot, n in enumerate(self._length):
+            if n is None:
+                continue
+            if n >= self.max_len:
+                raise RuntimeError(f"the sequence in slot {slot} has reached {self.max_len} positions")
+            if n >= self._reach[slot] * self.page_size:
+                wanted[slot] = range(self._reach[slot], n // self.page_size + 1)
+                if self.window is not None:
+                    left[slot] = [e for e in self._owned[slot] if (e + 1) * self.page_size <= n + 1 - self.window]
+        if wanted:
+            self._take(wanted, left)
+            self._upload()
+
+    def advance(self, on_device: bool = True) -> None:
+        """Every sequence has one position more.  ``on_device=False``: the device has counted already (a recorded step)."""
+        if on_device:
+            self.count_on_device()
+        self._length = [None if n is None else n + 1 for n in self._length]
+
+    def count_on_device(self) -> None:
+        self.positions.add_(self._live)
+        self.lens.add_(self._live)
+
+    # -- handles --------------------------------------------------------------------------------
+    def context(self, layer: int, positions: Optional[Tensor] = None, rows: Optional[Tensor] = None) -> PagedContext:
+        """The layer for a step of all slots, or for a prompt's tokens at ``positions`` of sequences ``rows``."""
+        if positions is None:
+            return PagedContext(self.k[layer], self.v[layer], self.page_table, self.positions, self.lens, None, self.status, self.window)
+        return PagedContext(self.k[layer], self.v[layer], self.page_table, positions, None, rows, self.status, self.window)
