@@ -62,39 +62,45 @@ template <int D, bool IN16, bool CACHE16>
 __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
   constexpr int LPR = D / 16, HALF = D / 2;
   const int rows_per_token = p.Hq + 2 * p.H;
-  const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPR;
+  const uint32_t item = blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
   const int c = threadIdx.x % LPR;
-  const int64_t token64 = item / rows_per_token;
-  if (token64 >= p.N) return;            // (whole groups of lanes: the sums below stay among lanes of one row)
-  const int token = (int)token64;
-  int h = (int)(item - token64 * rows_per_token);
-  const int kind = h < p.Hq ? 0 : h < p.Hq + p.H ? 1 : 2;
-  h -= kind == 0 ? 0 : kind == 1 ? p.Hq : p.Hq + p.H;
+  const int token = (int)(item / (uint32_t)rows_per_token), row = (int)(item - (uint32_t)token * (uint32_t)rows_per_token);
+  if (token >= p.N) return;              // (whole groups of lanes: the sums below stay among lanes of one row)
+  const int kind = row < p.Hq ? 0 : row < p.Hq + p.H ? 1 : 2, h = row - (kind == 0 ? 0 : kind == 1 ? p.Hq : p.Hq + p.H);
 
+  // (the row first: the way to its page is three reads long)
+  const uint16_t* src = p.in[kind] + token * p.in_st[kind] + h * p.in_sh[kind] + 8 * c;
+  const u32x4 raw0 = *reinterpret_cast<const u32x4*>(src), raw1 = *reinterpret_cast<const u32x4*>(src + HALF);
   const int pos = p.positions[token];
   const int seq = p.rows != nullptr ? p.rows[token] : token;
   // A negative position: no token.  Everything else that does not lead to a page of the pool is an error of the caller's that
   // only the device can see: nothing is written to the cache, q and the copies become NaN, the status word says so.
   const bool skipped = pos < 0;
-  int bits = 0, page = 0;
+  int bits = 0, page = 0, slot = 0;
   if (!skipped) {
     if (p.cos != nullptr && pos >= p.table_rows) bits |= DAISY_STATUS_POSITION_PAST_TABLES;
-    const int at = pos / p.page_size;
+    const int at = (int)((unsigned)pos / (unsigned)p.page_size);
+    slot = pos - at * p.page_size;
     if (seq < 0 || seq >= p.seqs || at >= p.max_pages) {
       bits |= DAISY_STATUS_LENGTH_PAST_PAGES;
     } else {
       page = p.table[seq * p.table_st + at];
       if (page < 0 || page >= p.num_pages) bits |= DAISY_STATUS_PAGE_OUT_OF_RANGE;
     }
-    if (bits && c == 0 && kind == 1 && h == 0) raise_status(p.status, bits);
+    if (bits && c == 0 && row == 0) raise_status(p.status, bits);
+  }
+  float cs[8], sn[8];
+  if (p.cos != nullptr && kind < 2) {
+    const int64_t off = (int64_t)(skipped || bits ? 0 : pos) * HALF + 8 * c;
+    const f32x4 c0 = *reinterpret_cast<const f32x4*>(p.cos + off), c1 = *reinterpret_cast<const f32x4*>(p.cos + off + 4);
+    const f32x4 s0 = *reinterpret_cast<const f32x4*>(p.sin + off), s1 = *reinterpret_cast<const f32x4*>(p.sin + off + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { cs[e] = c0[e]; cs[4 + e] = c1[e]; sn[e] = s0[e]; sn[4 + e] = s1[e]; }
   }
 
   float lo[8], hi[8];
-  {
-    const uint16_t* src = p.in[kind] + token * p.in_st[kind] + h * p.in_sh[kind] + 8 * c;
-    unpack8_as<IN16>(__builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src)), lo);
-    unpack8_as<IN16>(__builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + HALF)), hi);
-  }
+  unpack8_as<IN16>(raw0, lo);
+  unpack8_as<IN16>(raw1, hi);
   if (p.eps >= 0.f) {
     float sum = 0.f;
 #pragma unroll
@@ -105,34 +111,29 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
     for (int e = 0; e < 8; ++e) { lo[e] *= rstd; hi[e] *= rstd; }
   }
   if (kind < 2 && p.cos != nullptr) {
-    const int64_t off = (int64_t)(skipped || bits ? 0 : pos) * HALF + 8 * c;
-    const f32x4 c0 = *reinterpret_cast<const f32x4*>(p.cos + off), c1 = *reinterpret_cast<const f32x4*>(p.cos + off + 4);
-    const f32x4 s0 = *reinterpret_cast<const f32x4*>(p.sin + off), s1 = *reinterpret_cast<const f32x4*>(p.sin + off + 4);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float x1 = lo[e], x2 = hi[e], cc = e < 4 ? c0[e & 3] : c1[e & 3], sn = e < 4 ? s0[e & 3] : s1[e & 3];
-      lo[e] = fmaf(x1, cc, x2 * sn);
-      hi[e] = fmaf(x2, cc, -(x1 * sn));
+      const float x1 = lo[e], x2 = hi[e];
+      lo[e] = fmaf(x1, cs[e], x2 * sn[e]);
+      hi[e] = fmaf(x2, cs[e], -(x1 * sn[e]));
     }
   }
   if (kind == 2 && p.ve != nullptr) {
     const uint16_t* src = p.ve + token * p.e_st + h * p.e_sh + 8 * c;
     float el[8], eh[8];
-    unpack8_as<IN16>(__builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src)), el);
-    unpack8_as<IN16>(__builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + HALF)), eh);
+    unpack8_as<IN16>(*reinterpret_cast<const u32x4*>(src), el);
+    unpack8_as<IN16>(*reinterpret_cast<const u32x4*>(src + HALF), eh);
     const float g = *p.gate, og = 1.f - g;
 #pragma unroll
     for (int e = 0; e < 8; ++e) { lo[e] = fmaf(g, lo[e], og * el[e]); hi[e] = fmaf(g, hi[e], og * eh[e]); }
   }
-
   if (skipped || bits) {
     const float fill = skipped ? 0.f : __builtin_nanf("");
 #pragma unroll
     for (int e = 0; e < 8; ++e) lo[e] = hi[e] = fill;
   }
-  const bool leave = skipped && !p.zero_skipped;
   if (kind == 0) {
-    if (leave) return;
+    if (skipped && !p.zero_skipped) return;
     uint16_t* dst = p.q_out + token * p.qo_st + h * p.qo_sh + 8 * c;
     *reinterpret_cast<u32x4*>(dst) = p.q_f16 ? pack8_as<true>(lo) : pack8_as<false>(lo);
     *reinterpret_cast<u32x4*>(dst + HALF) = p.q_f16 ? pack8_as<true>(hi) : pack8_as<false>(hi);
@@ -140,7 +141,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
   }
   const int w = kind - 1;
   if (!skipped && !bits) {
-    uint16_t* dst = p.pages[w] + page * p.sp[w] + h * p.sh[w] + (int64_t)(pos % p.page_size) * p.ss[w] + 8 * c;
+    uint16_t* dst = p.pages[w] + page * p.sp[w] + h * p.sh[w] + slot * p.ss[w] + 8 * c;
     *reinterpret_cast<u32x4*>(dst) = pack8_as<CACHE16>(lo);
     *reinterpret_cast<u32x4*>(dst + HALF) = pack8_as<CACHE16>(hi);
   }
@@ -644,16 +645,13 @@ template <bool F16> static void paged_launch(const PagedParams& p, int D, size_t
   else paged_launch<256, F16>(p, lds, s);
 }
 
-template <int D> static void append_launch(const AppendParams& p, bool in16, bool cache16, hipStream_t s) {
+template <int D, bool IN16, bool CACHE16> static void append_launch(const AppendParams& p, hipStream_t s) {
   const int64_t lanes = (int64_t)p.N * (p.Hq + 2 * p.H) * (D / 16);
-  const dim3 grid((unsigned)((lanes + 255) / 256));
-  if (in16) {
-    if (cache16) hipLaunchKernelGGL((paged_append_kernel<D, true, true>), grid, dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((paged_append_kernel<D, true, false>), grid, dim3(256), 0, s, p);
-  } else {
-    if (cache16) hipLaunchKernelGGL((paged_append_kernel<D, false, true>), grid, dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((paged_append_kernel<D, false, false>), grid, dim3(256), 0, s, p);
-  }
+  hipLaunchKernelGGL((paged_append_kernel<D, IN16, CACHE16>), dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, s, p);
+}
+template <int D> static void append_launch(const AppendParams& p, bool in16, bool cache16, hipStream_t s) {
+  if (in16) cache16 ? append_launch<D, true, true>(p, s) : append_launch<D, true, false>(p, s);
+  else cache16 ? append_launch<D, false, true>(p, s) : append_launch<D, false, false>(p, s);
 }
 
 static bool al16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0; }
@@ -708,7 +706,7 @@ extern "C" int daisy_paged_append_fwd(const void* q, const int64_t* q_strides, c
   DAISY_CHECK_ARG((!q || (rows_of_16(q_strides, 2) && rows_of_16(q_out_strides, 2))) && rows_of_16(k_strides, 2) && rows_of_16(v_strides, 2) &&
                       (!ve || rows_of_16(ve_strides, 2)) && (!k_out || rows_of_16(k_out_strides, 2)) && (!v_out || rows_of_16(v_out_strides, 2)),
                   "paged_append: strides must be multiples of 8 elements");
-  DAISY_CHECK_ARG((int64_t)N * ((int64_t)Hq + 2 * (int64_t)H) * (D / 16) <= (int64_t)255 << 31, "paged_append: too many rows (%d tokens)", N);
+  DAISY_CHECK_ARG((int64_t)N * ((int64_t)Hq + 2 * (int64_t)H) < (int64_t)1 << 31, "paged_append: too many rows (%d tokens)", N);
   AppendParams p = {};
   const void* in[3] = {q, k, v};
   const int64_t* in_strides[3] = {q_strides, k_strides, v_strides};
