@@ -218,12 +218,6 @@ __device__ __forceinline__ Extent extent(const PagedParams& p, int len) {
 }
 __device__ __forceinline__ int len_of(const PagedParams& p, int b) { return b < p.B ? p.lens[b] : 0; }
 
-// Tiles of all sequences (of one unit each).
-__device__ __forceinline__ int total_tiles(const PagedParams& p, int lane) {
-  int sum = 0;
-  for (int base = 0; base < p.B; base += 64) sum += extent(p, len_of(p, base + lane)).tiles;
-  return __builtin_amdgcn_readlane(wave_scan(sum), 63);
-}
 // How many tiles a wavefront takes.
 __device__ __forceinline__ int share_of(const PagedParams& p, int total) { return (total + 4 * p.groups - 1) / (4 * p.groups); }
 
@@ -252,7 +246,17 @@ __global__ __launch_bounds__(256, paged_waves_per_simd(D)) void paged_attn_kerne
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = blockIdx.x * 4 + wv;
   const int n = lane & 15, c = lane >> 4;
   const int units = p.H * p.head_tiles;
-  const int total = total_tiles(p, lane) * units;
+  // Tiles of the sequences (of one unit each): a lane sums up those of its 64th of the sequences, which gives the total and where a run begins.
+  const int per_lane = (p.B + 63) >> 6;
+  int own = 0, n4[4];
+  for (int j = 0; j < per_lane; j += 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) n4[i] = j + i < per_lane ? len_of(p, lane * per_lane + j + i) : 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) own += extent(p, n4[i]).tiles;
+  }
+  const int own_upto = wave_scan(own);
+  const int total = __builtin_amdgcn_readlane(own_upto, 63) * units;
   const int share = share_of(p, total);
   int x = (int)min((int64_t)wave * share, (int64_t)total);
   const int x_end = (int)min((int64_t)x + share, (int64_t)total);
@@ -260,7 +264,13 @@ __global__ __launch_bounds__(256, paged_waves_per_simd(D)) void paged_attn_kerne
   SplitUnit beyond = {-1, 0, 0, 0, 0, 0};
 
   const uint32_t k_row = (uint32_t)p.k_ss * 2, v_row = (uint32_t)p.v_ss * 2;      // bytes, fewer than 2^24
-  int base = 0, before = 0, len = 0, tiles = 0, upto = 0, chunk = -1;      // 64 sequences from `base` on, one a lane
+  // 64 sequences from `base` on, one a lane; up to 64 are all there
+  int base = 0, before = 0, len = n4[0], tiles = own, upto = own_upto, chunk = per_lane == 1 ? __builtin_amdgcn_readlane(own_upto, 63) : -1;
+  if (per_lane > 1 && x < x_end) {
+    const int first = 63 - __builtin_clzll(__ballot(own > 0 && (own_upto - own) * units <= x));
+    base = first * per_lane;
+    before = __builtin_amdgcn_readlane(own_upto - own, first);
+  }
   while (x < x_end) {
     // ---- the unit that x lies in
     while (chunk < 0 || x >= (before + chunk) * units) {
