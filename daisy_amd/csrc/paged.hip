@@ -218,19 +218,38 @@ __device__ __forceinline__ Extent extent(const PagedParams& p, int len) {
 }
 __device__ __forceinline__ int len_of(const PagedParams& p, int b) { return b < p.B ? p.lens[b] : 0; }
 
-// How many tiles a wavefront takes.
-__device__ __forceinline__ int share_of(const PagedParams& p, int total) { return (total + 4 * p.groups - 1) / (4 * p.groups); }
+constexpr int kCus = 256;
+__device__ __forceinline__ int wave_min(int x) {
+  x = min(x, __builtin_amdgcn_update_dpp(x, x, 0x111, 0xf, 0xf, false));      // row_shr 1, 2, 4, 8: lanes without a neighbour keep their own
+  x = min(x, __builtin_amdgcn_update_dpp(x, x, 0x112, 0xf, 0xf, false));
+  x = min(x, __builtin_amdgcn_update_dpp(x, x, 0x114, 0xf, 0xf, false));
+  x = min(x, __builtin_amdgcn_update_dpp(x, x, 0x118, 0xf, 0xf, false));
+  x = min(x, __builtin_amdgcn_update_dpp(x, x, 0x142, 0xa, 0xf, false));      // row_bcast 15, 31
+  x = min(x, __builtin_amdgcn_update_dpp(x, x, 0x143, 0xc, 0xf, false));
+  return __builtin_amdgcn_readlane(x, 63);
+}
+// How many tiles a wavefront takes: no fewer than the workgroups there are can do, and more (a lane tries each number up to twice as many) where that
+// takes a thirty-second or more off the most loaded of the compute units.  32 sequences of 1024, 8 heads: 683 workgroups of 4 x 3 tiles, three of them
+// on most compute units, 31.1 us; 512 of 4 x 4, two on each, 28.6.  With next to nothing to gain, more wavefronts are the better ones:
+// 2 x 131072 positions, 16 heads, 3049 runs of 43 tiles 319.6 us, 2048 of 64 329.9.
+__device__ __forceinline__ int share_of(const PagedParams& p, int total, int lane) {
+  if (total <= 4 * kCus) return 1;
+  const int least = (total + 4 * p.groups - 1) / (4 * p.groups), more = min(lane, least);
+  const int share = least + more, groups = (total + 4 * share - 1) / (4 * share), load = (groups + kCus - 1) / kCus * share;
+  return least + (wave_min((more == 0 ? load - load / 32 : load) * 64 + more) & 63);
+}
 
 template <bool F16> __device__ __forceinline__ f32x4 mfma(const u32x4& a, const u32x4& b, const f32x4& c) {
   if constexpr (F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// The wavefronts of a SIMD that the registers of a head width leave room for.
-constexpr int paged_waves_per_simd(int D) { return D <= 64 ? 4 : D <= 128 ? 3 : 2; }
+// Workgroups per compute unit, a wavefront of each per SIMD: what the registers of a head width leave room for.  (Heads of 256: one, whose tiles of 32 KB
+// keep enough under way; 32 sequences of 1024, 8 heads: 46.6 us, with two 51.9, with two whose registers are held to their half 62.)
+constexpr int paged_groups_per_cu(int D) { return D <= 64 ? 4 : D <= 128 ? 3 : 1; }
 
 template <int D, bool F16>
-__global__ __launch_bounds__(256, paged_waves_per_simd(D)) void paged_attn_kernel(PagedParams p) {
+__global__ __launch_bounds__(256, paged_groups_per_cu(D)) void paged_attn_kernel(PagedParams p) {
   constexpr int KS = D / 32;                     // steps of the first product
   constexpr int J = D / 16;                      // 16-row pieces of the second product's result
   constexpr int W = D == 64 ? 4 : 8;             // channels of a V row that a lane has beside each other
@@ -257,7 +276,7 @@ __global__ __launch_bounds__(256, paged_waves_per_simd(D)) void paged_attn_kerne
   }
   const int own_upto = wave_scan(own);
   const int total = __builtin_amdgcn_readlane(own_upto, 63) * units;
-  const int share = share_of(p, total);
+  const int share = share_of(p, total, lane);
   int x = (int)min((int64_t)wave * share, (int64_t)total);
   const int x_end = (int)min((int64_t)x + share, (int64_t)total);
   OpenUnits mine = {0, 0, 0, 0};
@@ -532,73 +551,42 @@ __global__ __launch_bounds__(256, paged_waves_per_simd(D)) void paged_attn_kerne
   }
 }
 
-// Joins the partial sums of the units that lie in more than one workgroup's run.  The results of a unit are dealt to as many workgroups as there are
-// ends of runs in it: to those of the runs that it goes on beyond.
-template <int D, bool F16>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
-  constexpr int kFew = 8;
-  __shared__ float4 sums[4][8];
-  __shared__ float2 stats[4];
-  const SplitUnit u = p.split[blockIdx.x];
-  if (u.first < 0) return;
-  const int parts = u.last - u.first + 1, helpers = parts - 1, me = (int)blockIdx.x - u.first;
-  // the workgroup that the unit begins in has it in its second slot, where it begins with the unit too; the others in their first
-  auto slot = [&](int i, int head) { return (int64_t)(2 * (u.first + i) + (i == 0 ? 1 : 0)) * p.heads + head; };
-  if (parts <= kFew) {
-    // a thread per four channels, every part of which it asks for at once
-    for (int col = me + helpers * (int)threadIdx.x; col < u.heads * (D / 4); col += helpers * 256) {
-      const int head = col / (D / 4), at = col % (D / 4) * 4;
-      float2 st[kFew];
-      f32x4 v[kFew];
-#pragma unroll
-      for (int i = 0; i < kFew; ++i) {
-        const int64_t s = slot(min(i, parts - 1), head);
-        st[i] = p.stat[s];
-        v[i] = *reinterpret_cast<const f32x4*>(p.part + s * D + at);
-      }
-      float top = st[0].x, l = 0.f;
-#pragma unroll
-      for (int i = 1; i < kFew; ++i) top = fmaxf(top, st[i].x);
-      f32x4 a = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < kFew; ++i) {
-        const float f = i < parts ? fast_exp2(st[i].x - top) : 0.f;
-        l = i < parts ? fmaf(f, st[i].y, l) : l;
-        a = i < parts ? a + f * v[i] : a;
-      }
-      a *= 1.f / l;
-      *reinterpret_cast<u32x2*>(p.o + u.out + head * p.o_sh + at) = u32x2{pack2<F16>(a[0], a[1]), pack2<F16>(a[2], a[3])};
-    }
-    return;
-  }
-  // 32 channels at a time: eight lanes for them, 32 parts side by side
-  constexpr int U = 4;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = threadIdx.x / 8, at = threadIdx.x % 8 * 4;
-  for (int chunk = me; chunk < u.heads * (D / 32); chunk += helpers) {
-    const int head = chunk / (D / 32), d0 = chunk % (D / 32) * 32;
+// Where part i of a unit is: the workgroup that the unit begins in has it in its second slot, where it begins with the unit too, the others in their first.
+__device__ __forceinline__ int64_t part_slot(const PagedParams& p, const SplitUnit& u, int i, int head) {
+  return (int64_t)(2 * (u.first + i) + (i == 0 ? 1 : 0)) * p.heads + head;
+}
+
+// A unit's parts, joined for some of its results: CH channels of a head at a time, CH / 4 lanes for them and 1024 / CH parts side by side.
+template <int D, bool F16, int CH>
+__device__ __forceinline__ void join_parts(const PagedParams& p, const SplitUnit& u, int parts, int helpers, int me, float4 (*sums)[16], float2* stats) {
+  constexpr int LPR = CH / 4, GROUPS = 256 / LPR, U = 4;      // (U parts asked for at once)
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = threadIdx.x / LPR, at = threadIdx.x % LPR * 4;
+  for (int chunk = me; chunk < u.heads * (D / CH); chunk += helpers) {
+    const int head = chunk / (D / CH), d0 = chunk % (D / CH) * CH;
     float m = -__builtin_inff(), l = 0.f;
     f32x4 a = {0.f, 0.f, 0.f, 0.f};
-    for (int i0 = r; i0 < parts; i0 += 32 * U) {
+    for (int i0 = r; i0 < parts; i0 += GROUPS * U) {
       float2 st[U];
       f32x4 v[U];
 #pragma unroll
       for (int i = 0; i < U; ++i) {
-        const int64_t s = slot(min(i0 + 32 * i, parts - 1), head);
+        const int64_t s = part_slot(p, u, min(i0 + GROUPS * i, parts - 1), head);
         st[i] = p.stat[s];
         v[i] = *reinterpret_cast<const f32x4*>(p.part + s * D + d0 + at);
       }
 #pragma unroll
       for (int i = 0; i < U; ++i) {
-        if (i0 + 32 * i >= parts) break;
+        if (i0 + GROUPS * i >= parts) break;
         const float top = fmaxf(m, st[i].x), f = m > -__builtin_inff() ? fast_exp2(m - top) : 0.f, e = fast_exp2(st[i].x - top);
         l = f * l + e * st[i].y;
         a = f * a + e * v[i];
         m = top;
       }
     }
-    // the eight parts of a wavefront (the first of which it has, as parts > 8 x 3 or not), then the wavefronts
+    // the groups of a wavefront, some of which may have had no part, then the wavefronts
     auto across = [](float x, auto op) {
-      x = op(x, dpp_move<0x128>(x));
+      if constexpr (LPR <= 4) x = op(x, dpp_move<0x124>(x));      // row_ror 4, 8
+      if constexpr (LPR <= 8) x = op(x, dpp_move<0x128>(x));
       const LanePair r = row_pair(x);
       const LanePair t = half_pair(op(r.x, r.y));
       return op(t.x, t.y);
@@ -610,10 +598,10 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) a[i] = across(f * a[i], add);
     __syncthreads();      // (the chunk before has been read)
-    if (lane < 8) sums[wave][lane] = float4{a[0], a[1], a[2], a[3]};
+    if (lane < LPR) sums[wave][lane] = float4{a[0], a[1], a[2], a[3]};
     if (lane == 0) stats[wave] = float2{top, l};
     __syncthreads();
-    if (threadIdx.x < 8) {
+    if (threadIdx.x < LPR) {
       float best = stats[0].x, all = 0.f;
 #pragma unroll
       for (int i = 1; i < 4; ++i) best = fmaxf(best, stats[i].x);
@@ -631,6 +619,51 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
   }
 }
 
+// Joins the partial sums of the units that lie in more than one workgroup's run.  The results of a unit are dealt to as many workgroups as there are
+// ends of runs in it: to those of the runs that it goes on beyond.
+template <int D, bool F16>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
+  constexpr int kFew = 8;
+  __shared__ float4 sums[4][16];
+  __shared__ float2 stats[4];
+  const SplitUnit u = p.split[blockIdx.x];
+  if (u.first < 0) return;
+  const int parts = u.last - u.first + 1, helpers = parts - 1, me = (int)blockIdx.x - u.first;
+  if (parts <= kFew) {
+    // a thread per four channels, every part of which it asks for at once
+    for (int col = me + helpers * (int)threadIdx.x; col < u.heads * (D / 4); col += helpers * 256) {
+      const int head = col / (D / 4), at = col % (D / 4) * 4;
+      float2 st[kFew];
+      f32x4 v[kFew];
+#pragma unroll
+      for (int i = 0; i < kFew; ++i) {
+        const int64_t s = part_slot(p, u, min(i, parts - 1), head);
+        st[i] = p.stat[s];
+        v[i] = *reinterpret_cast<const f32x4*>(p.part + s * D + at);
+      }
+      float top = st[0].x, l = 0.f;
+#pragma unroll
+      for (int i = 1; i < kFew; ++i) top = fmaxf(top, st[i].x);
+      f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < kFew; ++i) {
+        const float f = i < parts ? fast_exp2(st[i].x - top) : 0.f;
+        l = i < parts ? fmaf(f, st[i].y, l) : l;
+        a = i < parts ? a + f * v[i] : a;
+      }
+      a *= 1.f / l;
+      *reinterpret_cast<u32x2*>(p.o + u.out + head * p.o_sh + at) = u32x2{pack2<F16>(a[0], a[1]), pack2<F16>(a[2], a[3])};
+    }
+  // as narrow as there are workgroups for the pieces, and as parts ask for a pass of 256, 128, 64
+  } else if (parts > 128 || u.heads * (D / 16) <= helpers) {
+    join_parts<D, F16, 16>(p, u, parts, helpers, me, sums, stats);
+  } else if (parts > 64 || u.heads * (D / 32) <= helpers) {
+    join_parts<D, F16, 32>(p, u, parts, helpers, me, sums, stats);
+  } else {
+    join_parts<D, F16, 64>(p, u, parts, helpers, me, sums, stats);
+  }
+}
+
 // How many workgroups share the work: one round of what the chip holds, less where there are fewer tiles.
 struct PagedSplit { int groups, heads, head_tiles; size_t lds; };
 static PagedSplit paged_split(int B, int H, int G, int D, int64_t capacity) {
@@ -638,9 +671,9 @@ static PagedSplit paged_split(int B, int H, int G, int D, int64_t capacity) {
   s.head_tiles = (G + 15) / 16;
   s.heads = G < 16 ? G : 16;
   s.lds = (size_t)8 * s.heads * D * sizeof(float);
-  const int by_lds = (int)((size_t)156 * 1024 / (s.lds + 2048)), per_cu = by_lds < paged_waves_per_simd(D) ? by_lds : paged_waves_per_simd(D);
+  const int by_lds = (int)((size_t)156 * 1024 / (s.lds + 2048)), per_cu = by_lds < paged_groups_per_cu(D) ? by_lds : paged_groups_per_cu(D);
   const int64_t tiles = ((capacity + kTile - 1) / kTile) * B * H * s.head_tiles;
-  const int64_t groups = (tiles + 3) / 4, most = 256 * per_cu;
+  const int64_t groups = (tiles + 3) / 4, most = kCus * per_cu;
   s.groups = (int)(groups < most ? groups : most);
   return s;
 }
