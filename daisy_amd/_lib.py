@@ -167,7 +167,7 @@ SIGNATURES = {
     "daisy_paged_attn_fwd": (c_int, [
         c_void_p, _I64P, c_void_p, _I64P, c_void_p, _I64P, c_int,  # q, k_pages, v_pages (+ strides), cache is fp16
         c_void_p, c_int64, c_int, c_int, c_int, c_void_p,       # page_table (+ row stride), max_pages, num_pages, page_size, lens
-        c_void_p, _I64P,                                        # o (+ strides)
+        c_void_p, _I64P, c_int,                                 # o (+ strides), is fp16
         c_int, c_int, c_int, c_int, c_int, c_float, c_void_p,   # B, Hq, H, D, window, scale, status
         c_void_p, c_size_t, c_void_p]),                         # workspace, bytes, stream
     "daisy_logits_process_fwd": (c_int, [

@@ -514,10 +514,20 @@ class CausalSelfAttention(nn.Module):
         """One token of every sequence of a paged cache, at the positions that the device holds."""
         if ctx.window is not None and (window is None or window > ctx.window):
             raise ValueError(f"the paged cache keeps {ctx.window} positions, a window of {window} was asked for")
+        if self._fused_prep_ok():
+            rot = _held(self._modules, self, "rotary")
+            x, ve = _as_bf16(x), _as_bf16(ve) if self.receives_ve else None
+            y = _lib.native().paged_layer_step(
+                x, _held(self._parameters, self, "qkvo_w"), ctx.k_pages, ctx.v_pages, ctx.page_table, ctx.positions, ctx.lens, _held(rot._buffers, rot, "cos"),
+                _held(rot._buffers, rot, "sin"), ve, _held(self._parameters, self, "g_ve") if self.receives_ve else None, ctx.status, window or 0,
+                float(self.attn_scale), NORM_EPS_BF16, STEP_ROWS_KERNEL_MAX)
+            if y is not None:
+                return y, None, None
         B = x.size(0)
         q = self._append_paged(x[:, 0], ve, ctx, False)
-        o = ops.paged_attention(q, ctx.k_pages, ctx.v_pages, ctx.page_table, ctx.lens, window=window, scale=self.attn_scale, status=ctx.status)
-        y = step_linear(_as_bf16(o).reshape(B, 1, self.m_dim), self.qkvo_w[3])
+        o = ops.paged_attention(q, ctx.k_pages, ctx.v_pages, ctx.page_table, ctx.lens, window=window, scale=self.attn_scale,
+                                out=torch.empty(q.shape, dtype=torch.bfloat16, device=q.device), status=ctx.status)
+        y = step_linear(o.view(B, 1, self.m_dim), self.qkvo_w[3])
         return y, None, None
 
     # -- reference interface -----------------------------------------------

@@ -789,7 +789,7 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (dev < 0 || window < 0 || !paged_cache(kp, vp, table, dev) || !rows_half(q, 3, dev) || !same_type(q, kp)) return none();
   const int64_t B = q.size(0), Hq = q.size(1), H = kp.size(1), D = kp.size(3);
   if (B < 1 || B > INT32_MAX || Hq < 1 || Hq > INT32_MAX || Hq % H != 0 || q.size(2) != D || table.size(0) < B || !int32_row(lens, B, dev)) return none();
-  if (out && !(rows_half(*out, 3, dev) && same_type(*out, q) && out->sizes() == q.sizes())) return none();
+  if (out && !(rows_half(*out, 3, dev) && (same_type(*out, q) || bf16(*out)) && out->sizes() == q.sizes())) return none();
   if ((status && !one_of(*status, at::kInt, dev)) || (ws && !(on_gpu(*ws, dev) && ws->is_contiguous())) || needs_autograd({&q, &kp, &vp})) return none();
   const int max_pages = (int)std::min<int64_t>(table.size(1), INT32_MAX), size = (int)std::min<int64_t>(kp.size(2), INT32_MAX);
   const size_t need = daisy_paged_attn_workspace_bytes((int)B, (int)Hq, (int)H, (int)D, max_pages, size);
@@ -800,11 +800,77 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const Strides2 qs(q), os(o);
   const Strides3 ks(kp), vs(vp);
   const int rc = daisy_paged_attn_fwd(ptr(q), qs.s, ptr(kp), ks.s, ptr(vp), vs.s, is_f16(kp), (const int32_t*)ptr(table), table.stride(0), max_pages, (int)kp.size(0), size,
-                                      (const int32_t*)ptr(lens), ptr(o), os.s, (int)B, (int)Hq, (int)H, (int)D, (int)std::min<long>(window, INT32_MAX), scale,
+                                      (const int32_t*)ptr(lens), ptr(o), os.s, is_f16(o), (int)B, (int)Hq, (int)H, (int)D, (int)std::min<long>(window, INT32_MAX), scale,
                                       (int32_t*)ptr(status), ptr(w), (size_t)(w.numel() * w.element_size()), stream_of(dev));
   if (rc != DAISY_OK) return none();
   unlocked.end();
   return wrap(o);
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_layer_step(x, qkvo_w, k_pages, v_pages, page_table, positions, lens, cos, sin, ve, g_ve, status, window (0: all), scale, eps, max_rows) -> y [B, 1, dim]
+// CausalSelfAttention.step over a paged cache: QKV projection, append, attention, output projection.  Nothing here is undone by the Python path that
+// a refusal leaves the call to: it writes the same rows to the same places.
+PyObject* py_paged_layer_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (intercepted() || n != 16) return none();
+  for (int i = 0; i < 9; ++i)
+    if (!is_tensor(a[i])) return none();
+  for (int i : {9, 10, 11})
+    if (!tensor_or_none(a[i])) return none();
+  const Tensor &x = THPVariable_Unpack(a[0]), &w = THPVariable_Unpack(a[1]), &kp = THPVariable_Unpack(a[2]), &vp = THPVariable_Unpack(a[3]);
+  const Tensor &table = THPVariable_Unpack(a[4]), &pos = THPVariable_Unpack(a[5]), &lens = THPVariable_Unpack(a[6]), &cos = THPVariable_Unpack(a[7]), &sin = THPVariable_Unpack(a[8]);
+  const Tensor *ve = opt_tensor(a[9]), *g_ve = opt_tensor(a[10]), *status = opt_tensor(a[11]);
+  const long window = PyLong_AsLong(a[12]);
+  const float scale = (float)PyFloat_AsDouble(a[13]), eps = (float)PyFloat_AsDouble(a[14]);
+  const int max_rows = (int)PyLong_AsLong(a[15]);
+  if (PyErr_Occurred()) { PyErr_Clear(); return none(); }
+  const int dev = gpu_of(x);
+  if (dev < 0 || window < 0 || !paged_cache(kp, vp, table, dev)) return none();
+  const int64_t H = kp.size(1), D = kp.size(3), dim = H * D;
+  Rows r;
+  if (x.dim() != 3 || x.size(1) != 1 || !as_rows(x, dev, r) || r.K != dim) return none();
+  const int64_t B = r.M;
+  if (!rows_bf16(w, 3, dev) || !w.is_contiguous() || w.size(0) != 4 || w.size(1) != dim || w.size(2) != dim || (reinterpret_cast<uintptr_t>(ptr(w)) & 15) != 0) return none();
+  if (table.size(0) < B || !int32_row(pos, B, dev) || !int32_row(lens, B, dev)) return none();
+  if (!rotary_table(cos, 1, D / 2, dev) || !rotary_table(sin, 1, D / 2, dev) || cos.size(0) != sin.size(0) || cos.size(0) > INT32_MAX) return none();
+  if ((status && !one_of(*status, at::kInt, dev)) || (ve == nullptr) != (g_ve == nullptr) || needs_autograd({&x, &w, ve, g_ve})) return none();
+  GateSource gate{nullptr, 0};
+  if (ve && !(gate_source(*g_ve, dev, gate) && on_gpu(*ve, dev) && bf16(*ve) && ve->is_contiguous() && ve->numel() == B * dim)) return none();
+  const int max_pages = (int)std::min<int64_t>(table.size(1), INT32_MAX), size = (int)std::min<int64_t>(kp.size(2), INT32_MAX);
+  const size_t need = daisy_paged_attn_workspace_bytes((int)B, (int)H, (int)H, (int)D, max_pages, size);
+  if (need == 0) return none();
+
+  Unlocked unlocked;
+  const hipStream_t s = stream_of(dev);
+  const uint16_t *wp = (const uint16_t*)ptr(w), *wo = wp + 3 * dim * dim;
+  Tensor qkv, y;
+  if (max_rows > 0 && (B <= max_rows || daisy::proj_wanted((int)B, (int)(3 * dim), (int)dim))) {
+    qkv = empty({B, 3 * dim}, at::kBFloat16, x);
+    if (!own_linear(r, wp, dim, (int)(3 * dim), nullptr, (uint16_t*)ptr(qkv), 3 * dim, max_rows, s)) return none();
+  } else {
+    qkv = at::linear(x, w.narrow(0, 0, 3).view({3 * dim, dim}));
+  }
+  const uint16_t* base = (const uint16_t*)ptr(qkv);
+  const int64_t rs[2] = {3 * dim, D}, os[2] = {dim, D};
+  const Strides3 ks(kp), vs(vp);
+  Tensor q = empty({B, dim}, kp.scalar_type(), x), o = empty({B, 1, dim}, at::kBFloat16, x), ws = empty({(int64_t)need}, at::kByte, x);
+  if (daisy::paged_append_launch(base, rs, base + dim, rs, base + 2 * dim, rs, 0, ptr(ve), os, gate, (const float*)ptr(cos), (const float*)ptr(sin), (int)cos.size(0),
+                                 ptr(kp), ks.s, ptr(vp), vs.s, is_f16(kp), (const int32_t*)ptr(table), table.stride(0), (int)table.size(0), max_pages, (int)kp.size(0), size,
+                                 (const int32_t*)ptr(pos), nullptr, ptr(q), os, is_f16(q), nullptr, nullptr, nullptr, nullptr, 1, (int)B, (int)H, (int)H, (int)D, eps,
+                                 (int32_t*)ptr(status), s) != DAISY_OK) return none();
+  if (daisy_paged_attn_fwd(ptr(q), os, ptr(kp), ks.s, ptr(vp), vs.s, is_f16(kp), (const int32_t*)ptr(table), table.stride(0), max_pages, (int)kp.size(0), size,
+                           (const int32_t*)ptr(lens), ptr(o), os, 0, (int)B, (int)H, (int)H, (int)D, (int)std::min<long>(window, INT32_MAX), scale, (int32_t*)ptr(status),
+                           ptr(ws), need, s) != DAISY_OK) return none();
+  const Rows orow{(const uint16_t*)ptr(o), dim, (int)B, (int)dim};
+  if (max_rows > 0 && (B <= max_rows || daisy::proj_wanted((int)B, (int)dim, (int)dim))) {
+    y = empty({B, 1, dim}, at::kBFloat16, x);
+    if (!own_linear(orow, wo, dim, (int)dim, nullptr, (uint16_t*)ptr(y), dim, max_rows, s)) return none();
+  } else {
+    y = at::linear(o, w.select(0, 3));
+  }
+  unlocked.end();
+  return wrap(y);
   END_HANDLE_TH_ERRORS
 }
 
@@ -876,7 +942,7 @@ PyObject* call(PyObject* self, PyObject* const* a, Py_ssize_t n) {
 }
 #define FAST(name) {#name, (PyCFunction)(void (*)(void))call<py_##name>, METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {FAST(linear), FAST(norm), FAST(linears), FAST(prefill_attention), FAST(layer_prefill), FAST(layer_step), FAST(kda_chunk), FAST(kda_layer),
-                          FAST(paged_append), FAST(paged_attention), FAST(process_logits),
+                          FAST(paged_append), FAST(paged_attention), FAST(paged_layer_step), FAST(process_logits),
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

@@ -46,7 +46,7 @@ __device__ __forceinline__ void raise_status(int32_t* status, int bit) {
 // All of it in fp32, rounded once as it is stored: pages in the cache's type, copies in the inputs', q in either.
 struct AppendParams {
   const uint16_t* in[3]; int64_t in_st[3], in_sh[3];     // q, k, v [N, heads, D]
-  const uint16_t* ve; int64_t e_st, e_sh; const float* gate;
+  const uint16_t* ve; int64_t e_st, e_sh; GateSource gate;
   const float* cos; const float* sin; int table_rows;
   uint16_t* pages[2]; int64_t sp[2], sh[2], ss[2];       // k, v [pages, H, page_size, D]
   const int32_t* table; int64_t table_st; int seqs, max_pages, num_pages, page_size;
@@ -123,7 +123,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
     float el[8], eh[8];
     unpack8_as<IN16>(*reinterpret_cast<const u32x4*>(src), el);
     unpack8_as<IN16>(*reinterpret_cast<const u32x4*>(src + HALF), eh);
-    const float g = *p.gate, og = 1.f - g;
+    const float g = gate_value(p.gate), og = 1.f - g;
 #pragma unroll
     for (int e = 0; e < 8; ++e) { lo[e] = fmaf(g, lo[e], og * el[e]); hi[e] = fmaf(g, hi[e], og * eh[e]); }
   }
@@ -181,13 +181,18 @@ struct PagedParams {
   const uint16_t* v; int64_t v_sp, v_sh, v_ss;
   const int32_t* table; int64_t table_st; int max_pages, num_pages, blocks_per_page, capacity;
   const int32_t* lens;
-  uint16_t* o; int64_t o_sb, o_sh;
+  uint16_t* o; int64_t o_sb, o_sh; int o_f16;
   SplitUnit* split;               // [workgroups]
   float* part; float2* stat;      // [2 * workgroups][heads of a unit][D], [..][..]: unnormalised sums; reference and sum of exponentials
   int B, H, G, head_tiles, heads, window, groups;      // heads: of a unit, min(G, 16); groups: workgroups
   float scale_log2e;
   int32_t* status;
 };
+
+// Four results in the type of o: bf16, or an fp16 cache's.
+template <bool F16> __device__ __forceinline__ u32x2 pack_out(const PagedParams& p, const f32x4& f) {
+  return F16 && p.o_f16 ? u32x2{pack2<F16>(f[0], f[1]), pack2<F16>(f[2], f[3])} : u32x2{pack2<false>(f[0], f[1]), pack2<false>(f[2], f[3])};
+}
 
 constexpr int kTile = 32;       // positions
 constexpr int kBlock = 16;      // positions: pages are multiples of it, so that half a tile lies in one page
@@ -479,7 +484,7 @@ __global__ __launch_bounds__(256, paged_groups_per_cu(D)) void paged_attn_kernel
             float f[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) f[i] = acc[t * W + (8 * i8 + i) % W][(8 * i8 + i) / W] * inv;
-            *reinterpret_cast<u32x4*>(dst + 128 * t + 8 * i8) = pack8_as<F16>(f);
+            *reinterpret_cast<u32x4*>(dst + 128 * t + 8 * i8) = F16 && p.o_f16 ? pack8_as<F16>(f) : pack8_as<false>(f);
           }
       } else {
         const int which = off == 0 ? 1 : 0;
@@ -541,7 +546,7 @@ __global__ __launch_bounds__(256, paged_groups_per_cu(D)) void paged_attn_kernel
         }
         if (which == 1 && !on) {
           sum *= 1.f / st.y;
-          *reinterpret_cast<u32x2*>(p.o + open_units[w].out + g * p.o_sh + at) = u32x2{pack2<F16>(sum[0], sum[1]), pack2<F16>(sum[2], sum[3])};
+          *reinterpret_cast<u32x2*>(p.o + open_units[w].out + g * p.o_sh + at) = pack_out<F16>(p, sum);
         } else {
           *reinterpret_cast<f32x4*>(p.part + (slot + g) * D + at) = sum;
           if (at == 0) p.stat[slot + g] = st;
@@ -614,7 +619,7 @@ __device__ __forceinline__ void join_parts(const PagedParams& p, const SplitUnit
         a += w * f32x4{t.x, t.y, t.z, t.w};
       }
       a *= 1.f / all;
-      *reinterpret_cast<u32x2*>(p.o + u.out + head * p.o_sh + d0 + at) = u32x2{pack2<F16>(a[0], a[1]), pack2<F16>(a[2], a[3])};
+      *reinterpret_cast<u32x2*>(p.o + u.out + head * p.o_sh + d0 + at) = pack_out<F16>(p, a);
     }
   }
 }
@@ -652,7 +657,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
         a = i < parts ? a + f * v[i] : a;
       }
       a *= 1.f / l;
-      *reinterpret_cast<u32x2*>(p.o + u.out + head * p.o_sh + at) = u32x2{pack2<F16>(a[0], a[1]), pack2<F16>(a[2], a[3])};
+      *reinterpret_cast<u32x2*>(p.o + u.out + head * p.o_sh + at) = pack_out<F16>(p, a);
     }
   // as narrow as there are workgroups for the pieces, and as parts ask for a pass of 256, 128, 64
   } else if (parts > 128 || u.heads * (D / 16) <= helpers) {
@@ -698,13 +703,13 @@ template <int D> static void append_launch(const AppendParams& p, bool in16, boo
 }
 
 static bool al16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0; }
-static bool rows_of_16(const int64_t* strides, int n) {
-  for (int i = 0; i < n; ++i)
-    if (strides[i] % 8 != 0 || strides[i] < 0) return false;
-  return true;
-}
+// (the stride of a dim of one says nothing)
+static bool step_of_16(int64_t stride, int n) { return n == 1 || (stride % 8 == 0 && stride >= 0); }
+static bool rows_of_16(const int64_t* strides, int n0, int n1) { return step_of_16(strides[0], n0) && step_of_16(strides[1], n1); }
+// Rows that are written: two of them are not the same.
+static bool apart(const int64_t* strides, int n0, int n1) { return (n0 == 1 || strides[0] > 0) && (n1 == 1 || strides[1] > 0); }
 // A page's rows are reached with 24-bit products.
-static bool page_rows_fit(const int64_t* strides) { return strides[2] < ((int64_t)1 << 23); }
+static bool page_rows_fit(const int64_t* strides) { return step_of_16(strides[2], 16) && strides[2] < ((int64_t)1 << 23); }
 
 }  // namespace daisy
 
@@ -720,13 +725,13 @@ using namespace daisy;
   DAISY_CHECK_SUPPORTED(page_size > 0 && page_size % 16 == 0, what ": page_size %d not supported (a multiple of 16)", page_size);         \
   DAISY_CHECK_ARG((int64_t)max_pages * page_size < ((int64_t)1 << 31), what ": a sequence of %lld positions is too long",                  \
                   (long long)max_pages * page_size);                                                                                      \
-  DAISY_CHECK_ARG(al16(k_pages) && al16(v_pages) && rows_of_16(k_pages_strides, 3) && rows_of_16(v_pages_strides, 3) &&                    \
+  DAISY_CHECK_ARG(al16(k_pages) && al16(v_pages) && rows_of_16(k_pages_strides, num_pages, H) && rows_of_16(v_pages_strides, num_pages, H) && \
                       page_rows_fit(k_pages_strides) && page_rows_fit(v_pages_strides),                                                   \
                   what ": pages must be 16-byte aligned, their strides multiples of 8 elements, a row's less than 2^23")
 
-extern "C" int daisy_paged_append_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+int daisy::paged_append_launch(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
                                       const void* v, const int64_t* v_strides, int in_is_f16,
-                                      const void* ve, const int64_t* ve_strides, const float* gate,
+                                      const void* ve, const int64_t* ve_strides, GateSource gate,
                                       const float* cos, const float* sin, int table_rows,
                                       void* k_pages, const int64_t* k_pages_strides, void* v_pages, const int64_t* v_pages_strides,
                                       int cache_is_f16, const int32_t* page_table, int64_t table_stride, int n_seq, int max_pages,
@@ -739,16 +744,19 @@ extern "C" int daisy_paged_append_fwd(const void* q, const int64_t* q_strides, c
   DAISY_CHECK_ARG(!q || (q_strides && q_out_strides), "paged_append: q and q_out need strides");
   DAISY_CHECK_ARG(N > 0 && Hq >= 0 && H > 0 && n_seq > 0, "paged_append: N=%d, H=%d, n_seq=%d must be positive", N, H, n_seq);
   DAISY_CHECK_ARG((cos == nullptr) == (sin == nullptr) && (!cos || table_rows > 0), "paged_append: cos and sin must both be given or both NULL");
-  DAISY_CHECK_ARG((ve == nullptr) == (gate == nullptr) && (!ve || ve_strides), "paged_append: ve, its strides and gate go together");
+  DAISY_CHECK_ARG((ve == nullptr) == (gate.p == nullptr) && (!ve || ve_strides), "paged_append: ve, its strides and gate go together");
   DAISY_CHECK_ARG((!k_out || k_out_strides) && (!v_out || v_out_strides), "paged_append: k_out and v_out need strides");
   DAISY_CHECK_ARG(rows || N <= n_seq, "paged_append: without rows, token i belongs to sequence i: %d tokens, %d sequences", N, n_seq);
   DAISY_CHECK_HEAD_DIM("paged_append", D);
   DAISY_CHECK_PAGES("paged_append");
   DAISY_CHECK_ARG(al16(q) && al16(k) && al16(v) && al16(ve) && al16(cos) && al16(sin) && al16(q_out) && al16(k_out) && al16(v_out),
                   "paged_append: tensors must be 16-byte aligned");
-  DAISY_CHECK_ARG((!q || (rows_of_16(q_strides, 2) && rows_of_16(q_out_strides, 2))) && rows_of_16(k_strides, 2) && rows_of_16(v_strides, 2) &&
-                      (!ve || rows_of_16(ve_strides, 2)) && (!k_out || rows_of_16(k_out_strides, 2)) && (!v_out || rows_of_16(v_out_strides, 2)),
+  DAISY_CHECK_ARG((!q || (rows_of_16(q_strides, N, Hq) && rows_of_16(q_out_strides, N, Hq))) && rows_of_16(k_strides, N, H) && rows_of_16(v_strides, N, H) &&
+                      (!ve || rows_of_16(ve_strides, N, H)) && (!k_out || rows_of_16(k_out_strides, N, H)) && (!v_out || rows_of_16(v_out_strides, N, H)),
                   "paged_append: strides must be multiples of 8 elements");
+  DAISY_CHECK_ARG((!q || apart(q_out_strides, N, Hq)) && (!k_out || apart(k_out_strides, N, H)) && (!v_out || apart(v_out_strides, N, H)) &&
+                      apart(k_pages_strides, num_pages, H) && apart(v_pages_strides, num_pages, H) && k_pages_strides[2] > 0 && v_pages_strides[2] > 0,
+                  "paged_append: rows that are written must not overlap");
   DAISY_CHECK_ARG((int64_t)N * ((int64_t)Hq + 2 * (int64_t)H) < (int64_t)1 << 31, "paged_append: too many rows (%d tokens)", N);
   AppendParams p = {};
   const void* in[3] = {q, k, v};
@@ -780,9 +788,29 @@ extern "C" int daisy_paged_append_fwd(const void* q, const int64_t* q_strides, c
   return DAISY_OK;
 }
 
+extern "C" int daisy_paged_append_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                                      const void* v, const int64_t* v_strides, int in_is_f16,
+                                      const void* ve, const int64_t* ve_strides, const float* gate,
+                                      const float* cos, const float* sin, int table_rows,
+                                      void* k_pages, const int64_t* k_pages_strides, void* v_pages, const int64_t* v_pages_strides,
+                                      int cache_is_f16, const int32_t* page_table, int64_t table_stride, int n_seq, int max_pages,
+                                      int num_pages, int page_size, const int32_t* positions, const int32_t* rows,
+                                      void* q_out, const int64_t* q_out_strides, int q_out_is_f16,
+                                      void* k_out, const int64_t* k_out_strides, void* v_out, const int64_t* v_out_strides, int zero_skipped,
+                                      int N, int Hq, int H, int D, float eps, int32_t* status, void* stream) {
+  return paged_append_launch(q, q_strides, k, k_strides, v, v_strides, in_is_f16, ve, ve_strides, GateSource{gate, GateSource::kValue}, cos, sin, table_rows,
+                             k_pages, k_pages_strides, v_pages, v_pages_strides, cache_is_f16, page_table, table_stride, n_seq, max_pages, num_pages,
+                             page_size, positions, rows, q_out, q_out_strides, q_out_is_f16, k_out, k_out_strides, v_out, v_out_strides, zero_skipped,
+                             N, Hq, H, D, eps, status, stream);
+}
+
+// Tiles are counted in 32 bits, with room for a share's rounding.
+static bool paged_tiles_fit(int B, int Hq, int H, int64_t capacity) {
+  return ((double)capacity / kTile + 1) * B * H * ((Hq / H + 15) / 16) < (double)(1 << 30);
+}
 static bool paged_shape_ok(int B, int Hq, int H, int D, int max_pages, int page_size) {
   return B > 0 && H > 0 && Hq > 0 && Hq % H == 0 && (D == 64 || D == 128 || D == 256) && max_pages > 0 && page_size > 0 &&
-         (int64_t)max_pages * page_size < ((int64_t)1 << 31);
+         (int64_t)max_pages * page_size < ((int64_t)1 << 31) && paged_tiles_fit(B, Hq, H, (int64_t)max_pages * page_size);
 }
 
 extern "C" size_t daisy_paged_attn_workspace_bytes(int B, int Hq, int H, int D, int max_pages, int page_size) {
@@ -794,18 +822,19 @@ extern "C" size_t daisy_paged_attn_workspace_bytes(int B, int Hq, int H, int D, 
 extern "C" int daisy_paged_attn_fwd(const void* q, const int64_t* q_strides,
                                     const void* k_pages, const int64_t* k_pages_strides, const void* v_pages, const int64_t* v_pages_strides,
                                     int cache_is_f16, const int32_t* page_table, int64_t table_stride, int max_pages, int num_pages, int page_size,
-                                    const int32_t* lens, void* o, const int64_t* o_strides, int B, int Hq, int H, int D, int window, float scale,
+                                    const int32_t* lens, void* o, const int64_t* o_strides, int o_is_f16, int B, int Hq, int H, int D, int window, float scale,
                                     int32_t* status, void* workspace, size_t workspace_bytes, void* stream) {
   DAISY_CHECK_ARG(q && q_strides && o && o_strides && lens, "paged_attn: q, o, their strides and the lengths must be non-NULL");
   DAISY_CHECK_ARG(B > 0 && H > 0 && Hq > 0 && Hq % H == 0, "paged_attn: B=%d, H=%d must be positive, Hq=%d a multiple of H", B, H, Hq);
   DAISY_CHECK_HEAD_DIM("paged_attn", D);
   DAISY_CHECK_PAGES("paged_attn");
-  DAISY_CHECK_ARG(al16(q) && al16(o) && rows_of_16(q_strides, 2) && rows_of_16(o_strides, 2),
+  DAISY_CHECK_ARG(al16(q) && al16(o) && rows_of_16(q_strides, B, Hq) && rows_of_16(o_strides, B, Hq),
                   "paged_attn: q and o must be 16-byte aligned, their strides multiples of 8 elements");
   const int64_t capacity = (int64_t)max_pages * page_size;
+  DAISY_CHECK_ARG(paged_tiles_fit(B, Hq, H, capacity), "paged_attn: %d sequences of up to %lld positions, %d key heads, are too many", B, (long long)capacity, H);
+  DAISY_CHECK_SUPPORTED(!o_is_f16 || cache_is_f16, "paged_attn: an fp16 o needs an fp16 cache");
+  DAISY_CHECK_ARG(apart(o_strides, B, Hq), "paged_attn: rows of o must not overlap");
   const PagedSplit sp = paged_split(B, H, Hq / H, D, capacity);
-  DAISY_CHECK_ARG((capacity / kTile + 1) * B * H * sp.head_tiles < ((int64_t)1 << 31) , "paged_attn: %d sequences of up to %lld positions are too many",
-                  B, (long long)capacity);
   const size_t need = daisy_paged_attn_workspace_bytes(B, Hq, H, D, max_pages, page_size);
   if (workspace == nullptr || workspace_bytes < need || !al16(workspace)) {
     set_error("paged_attn: workspace of %zu bytes, %zu needed on a 16-byte boundary", workspace_bytes, need);
@@ -818,7 +847,7 @@ extern "C" int daisy_paged_attn_fwd(const void* q, const int64_t* q_strides,
   p.table = page_table; p.table_st = table_stride; p.max_pages = max_pages; p.num_pages = num_pages;
   p.blocks_per_page = page_size / kBlock; p.capacity = (int)capacity;
   p.lens = lens;
-  p.o = (uint16_t*)o; p.o_sb = o_strides[0]; p.o_sh = o_strides[1];
+  p.o = (uint16_t*)o; p.o_f16 = o_is_f16; p.o_sb = o_strides[0]; p.o_sh = o_strides[1];
   p.split = (SplitUnit*)workspace;
   p.part = (float*)(p.split + sp.groups);
   p.stat = (float2*)(p.part + (size_t)2 * sp.groups * sp.heads * D);

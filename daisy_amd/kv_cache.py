@@ -232,6 +232,8 @@ class PagedKVCache:
     def admit(self, lengths: List[int]) -> List[int]:
         """Free slots for new sequences of these many positions each, with pages for them: the slots, in order.  The positions are
         to be filled (``ops.paged_append``, ``core.admit``) before the next step."""
+        if not lengths:
+            return []
         slots = [s for s, n in enumerate(self._length) if n is None][:len(lengths)]
         if len(slots) < len(lengths):
             raise RuntimeError(f"the paged cache has {len(slots)} free slots for {len(lengths)} sequences")

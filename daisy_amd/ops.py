@@ -912,7 +912,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     ``q [B, Hq, D]`` in the cache's dtype (bf16 or fp16), any batch and head strides; ``k_pages``, ``v_pages``, ``page_table`` as for ``paged_append``, row b of
     the table for sequence b; Hq a multiple of the cache's H, ``Hq // H`` query heads to a key head.  ``lens`` int32 ``[B]``: the number of
     positions of each sequence, the new token's among them; the last ``window`` of them are seen (``None``: all).  A sequence of length zero gives
-    zeros.  Returns ``o [B, Hq, D]`` in q's dtype.
+    zeros.  Returns ``o [B, Hq, D]`` in q's dtype, or ``out``, which may be bf16 with an fp16 cache.
 
     Lengths and table are read when the kernels run, and the work is split over the lengths that are found there: nothing but shapes is fixed by a
     recording.  A length beyond the table's room, or a page that is none, gives NaN for the heads of that sequence and raises a bit in ``status``.
@@ -936,7 +936,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if out is None:
         out = torch.empty((B, Hq, D), dtype=q.dtype, device=dev)
     else:
-        _check_rows("out", out, 3, (q.dtype,))
+        _check_rows("out", out, 3, (torch.bfloat16,) if q.dtype == torch.bfloat16 else _HALF_TYPES)
         if out.shape != q.shape:
             raise ValueError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
     if B == 0:
@@ -953,7 +953,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
             q.data_ptr(), _lib.strides(q, (0, 1)), k_pages.data_ptr(), _lib.strides(k_pages, (0, 1, 2)),
             v_pages.data_ptr(), _lib.strides(v_pages, (0, 1, 2)), 1 if q.dtype == torch.float16 else 0,
             page_table.data_ptr(), page_table.stride(0), max_pages, P, size, lens.data_ptr(), out.data_ptr(), _lib.strides(out, (0, 1)),
-            B, Hq, H, D, min(int(window), 2 ** 31 - 1) if window is not None else 0, float(scale), _lib.ptr(status),
+            1 if out.dtype == torch.float16 else 0, B, Hq, H, D, min(int(window), 2 ** 31 - 1) if window is not None else 0, float(scale), _lib.ptr(status),
             workspace.data_ptr(), workspace.numel() * workspace.element_size(), _lib.current_stream(dev))
     _lib.check(rc, "daisy_paged_attn_fwd")
     return out
@@ -974,7 +974,7 @@ def process_logits(logits: torch.Tensor, history: Optional[torch.Tensor] = None,
     ``MAX_HISTORY``), a token that was seen n times, at ages (1 = the newest) that add up to ``w = sum 2 ** (-age / half_life)`` (``None``: w = n),
     has its logit divided by ``repetition ** min(w, cap)`` where positive and multiplied by it otherwise; ``frequency * n`` and, for n > 0, ``presence``
     are subtracted.  ``cap=1`` without a half life is the usual penalty; ``half_life=140, cap=3, lookback=128`` is the generator's
-    (``penalise_repeats``).  Ids outside the vocabulary count for nothing.  ``repetition``, ``presence``, ``frequency``: a number, or fp32 ``[B]`` on the GPU.
+    (``penalise_repeats``).  Ids outside the vocabulary count for nothing.  ``repetition`` (positive), ``presence``, ``frequency``: a number, or fp32 ``[B]`` on the GPU.
 
     ``bias`` (fp32 ``[V]`` or ``[B, V]``) is added.  ``allowed`` (int32 ``[ceil(V / 32)]`` or ``[B, ceil(V / 32)]``, see ``pack_allowed``): tokens whose bit
     (``v % 32`` of word ``v // 32``) is clear become -inf, whatever they were; a row without a set bit is -inf throughout.

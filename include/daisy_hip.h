@@ -500,7 +500,7 @@ int daisy_paged_append_fwd(const void* q, const int64_t* q_strides, const void* 
 /* daisy_paged_attn_fwd: the attention of one new token per sequence, whose key and value are in the cache already:
  *   o[b, h] = sum_t softmax_t(scale <q[b, h], k_t>) v_t,  max(0, lens[b] - window) <= t < lens[b]
  * (window <= 0: all positions), the key head of query head h being h / (Hq / H); a length of zero or less gives
- * zeros.  q, o: the cache's type, [B, Hq, D] with {batch, head} strides.  The work is split over the lengths
+ * zeros.  q: the cache's type, o: bf16, or fp16 (o_is_f16) with an fp16 cache; [B, Hq, D] with {batch, head} strides.  The work is split over the lengths
  * as they are when the kernel runs.  workspace: daisy_paged_attn_workspace_bytes(...) bytes, 16-byte aligned,
  * of no other call that may run at the same time.
  */
@@ -509,7 +509,7 @@ int daisy_paged_attn_fwd(const void* q, const int64_t* q_strides,
                          const void* k_pages, const int64_t* k_pages_strides,
                          const void* v_pages, const int64_t* v_pages_strides, int cache_is_f16,
                          const int32_t* page_table, int64_t table_stride, int max_pages, int num_pages, int page_size,
-                         const int32_t* lens, void* o, const int64_t* o_strides,
+                         const int32_t* lens, void* o, const int64_t* o_strides, int o_is_f16,
                          int B, int Hq, int H, int D, int window, float scale, int32_t* status,
                          void* workspace, size_t workspace_bytes, void* stream);
 

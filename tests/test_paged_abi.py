@@ -15,8 +15,8 @@ def error():
     return _lib.load().daisy_last_error().decode()
 
 
-def attend(q=P, qs=S2, k=P, ks=S3, v=P, table=P, stride=4, max_pages=4, num_pages=8, page=16, lens=P, o=P, B=1, Hq=2, H=2, D=128, ws=P, ws_bytes=1 << 15):
-    return _lib.load().daisy_paged_attn_fwd(q, qs, k, ks, v, ks, 0, table, stride, max_pages, num_pages, page, lens, o, S2, B, Hq, H, D, 0, 0.12, None, ws, ws_bytes, None)
+def attend(q=P, qs=S2, k=P, ks=S3, v=P, table=P, stride=4, max_pages=4, num_pages=8, page=16, lens=P, o=P, os=S2, B=1, Hq=2, H=2, D=128, ws=P, ws_bytes=1 << 15):
+    return _lib.load().daisy_paged_attn_fwd(q, qs, k, ks, v, ks, 0, table, stride, max_pages, num_pages, page, lens, o, os, 0, B, Hq, H, D, 0, 0.12, None, ws, ws_bytes, None)
 
 
 def append(q=P, k=P, v=P, table=P, stride=4, n_seq=1, max_pages=4, num_pages=8, page=16, positions=P, rows=None, q_out=P, N=1, Hq=2, H=2, D=128, ve=None, gate=None,
@@ -32,7 +32,8 @@ def append(q=P, k=P, v=P, table=P, stride=4, n_seq=1, max_pages=4, num_pages=8, 
     (dict(max_pages=1 << 27, page=16), -1, "too long"), (dict(max_pages=1 << 20, B=1 << 15), -1, "too many"),
     (dict(q=P + 2), -1, "aligned"), (dict(k=P + 8), -1, "aligned"), (dict(ks=(ctypes.c_int64 * 3)(4096, 2048, 129)), -1, "multiples of 8"),
     (dict(ks=(ctypes.c_int64 * 3)(4096, 2048, -128)), -1, "strides"), (dict(ks=(ctypes.c_int64 * 3)(4096, 2048, 1 << 23)), -1, "2^23"),
-    (dict(qs=(ctypes.c_int64 * 2)(4, 128)), -1, "multiples of 8"), (dict(ws=None), -3, "workspace"), (dict(ws_bytes=16), -3, "workspace"), (dict(ws=P + 4), -3, "workspace")])
+    (dict(qs=(ctypes.c_int64 * 2)(128, 4)), -1, "multiples of 8"), (dict(os=(ctypes.c_int64 * 2)(256, 0)), -1, "overlap"), (dict(os=(ctypes.c_int64 * 2)(0, 128), B=2), -1, "overlap"),
+    (dict(B=1 << 30, Hq=1 << 20, H=1 << 20, max_pages=1 << 20), -1, "too many"), (dict(ws=None), -3, "workspace"), (dict(ws_bytes=16), -3, "workspace"), (dict(ws=P + 4), -3, "workspace")])
 def test_attention_argument_errors(kw, rc, text):
     assert attend(**kw) == rc and text in error(), error()
 
@@ -41,8 +42,8 @@ def test_attention_argument_errors(kw, rc, text):
     (dict(k=None), -1, "non-NULL"), (dict(positions=None), -1, "non-NULL"), (dict(q=None), -1, "go together"), (dict(q_out=None), -1, "go together"), (dict(Hq=0), -1, "go together"),
     (dict(N=0), -1, "N=0"), (dict(H=0), -1, "H=0"), (dict(n_seq=0), -1, "n_seq"), (dict(N=2), -1, "token i belongs"), (dict(cos=P), -1, "cos and sin"),
     (dict(cos=P, sin=P), -1, "cos and sin"), (dict(ve=P), -1, "gate"), (dict(gate=P), -1, "gate"), (dict(k_out=P), -1, "strides"), (dict(D=32), -2, "head_dim 32"),
-    (dict(page=17), -2, "page_size"), (dict(k=P + 2), -1, "aligned"), (dict(ss=(ctypes.c_int64 * 2)(12, 128)), -1, "multiples of 8"),
-    (dict(N=1 << 30, rows=P, Hq=1 << 20), -1, "too many rows")])
+    (dict(page=17), -2, "page_size"), (dict(k=P + 2), -1, "aligned"), (dict(ss=(ctypes.c_int64 * 2)(128, 12)), -1, "multiples of 8"),
+    (dict(N=1 << 30, rows=P, Hq=1 << 20), -1, "too many rows"), (dict(k_out=P, k_out_strides=(ctypes.c_int64 * 2)(0, 0)), -1, "overlap")])
 def test_append_argument_errors(kw, rc, text):
     assert append(**kw) == rc and text in error(), error()
 
@@ -66,6 +67,7 @@ def test_workspaces_of_the_paged_attention():
     assert size(1, 12, 12, 128, 128, 64) == (256 * 12 // 4) * (32 + 2 * 130 * 4)
     assert size(1000, 16, 16, 128, 128, 64) == 768 * (32 + 2 * 130 * 4)               # as many workgroups as the chip holds
     assert size(1000, 64, 1, 128, 128, 64) == 512 * (32 + 2 * 16 * 130 * 4)           # at most 16 heads to a unit; their sums fill the LDS
+    assert size(1 << 30, 1 << 20, 1 << 20, 128, 1 << 20, 64) == 0
     assert size(0, 1, 1, 128, 1, 16) == size(1, 3, 2, 128, 1, 16) == size(1, 1, 1, 80, 1, 16) == size(1, 1, 1, 128, 1 << 27, 16) == 0
 
 

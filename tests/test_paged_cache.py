@@ -36,6 +36,7 @@ def test_sequences_come_grow_and_go():
 
 def test_what_does_not_fit_changes_nothing():
     c = cache()
+    assert c.admit([]) == []
     c.admit([33, 33])
     before = c.page_table.clone(), list(c._free)
     with pytest.raises(RuntimeError, match="full"):

@@ -95,6 +95,9 @@ def test_attention_over_every_edge_of_blocks_tiles_and_pages(dtype, D, H, G, pag
     assert bool((o[[0, 15]] == 0).all()), "a sequence without positions gives zeros"
     again = ops.paged_attention(q, k, v, table, lens, scale=0.12)
     assert torch.equal(o, again)
+    if dtype == F16:
+        wide = ops.paged_attention(q, k, v, table, lens, scale=0.12, out=torch.empty(q.shape, dtype=BF16, device=DEV))
+        check_attention(wide, q, rows, 0.12, "bf16 results")
 
 
 @pytest.mark.parametrize("window", [1, 2, 16, 31, 32, 33, 100, 1000])
@@ -193,6 +196,19 @@ def test_strides_of_every_tensor():
     got = ops.paged_attention(q, k2, v2, wide[:3, 3:3 + table.shape[1]], lt, out=out)
     assert got is out and torch.equal(got, base)
     assert bool((room[:, 0] == 5).all() and (room[:, 1, 0] == 5).all() and (room[:, 1, -1] == 5).all())
+
+
+def test_strides_of_dims_of_one_say_nothing():
+    g = gen(15)
+    k, v, table, rows = make_cache([40], 1, 16, 64, BF16, g)
+    odd = lambda t: torch.as_strided(t, t.shape, (3, 5) + t.stride()[2:])      # noqa: E731
+    q = odd(randn(g, 1, 1, 64, dtype=BF16))
+    assert q.stride() == (3, 5, 1)
+    o = ops.paged_attention(q, k, v, table, torch.tensor([40], dtype=torch.int32, device=DEV), out=odd(torch.empty(1, 1, 64, dtype=BF16, device=DEV)))
+    check_attention(o, q, rows, ops.ATTN_SCALE, "one row")
+    x, pos = odd(randn(g, 1, 1, 64, dtype=BF16)), torch.tensor([5], dtype=torch.int32, device=DEV)
+    ops.paged_append(x, x, k, v, table, pos, q=x)
+    assert torch.equal(k[int(table[0, 0]), 0, 5], x[0, 0])
 
 
 def test_rows_of_the_table_behind_the_last_sequence_are_not_read():
@@ -491,7 +507,7 @@ def test_refusals_name_what_is_wrong():
                       (ValueError, dict(q=randn(g, 1, 3, 64, dtype=BF16))), (ValueError, dict(q=randn(g, 2, 2, 64, dtype=BF16))), (ValueError, dict(v=v[:-1])),
                       (ValueError, dict(table=table.long())), (ValueError, dict(table=table[:, :0])), (ValueError, dict(lens=lens.long())),
                       (ValueError, dict(lens=lens.repeat(2))), (ValueError, dict(window=0)), (ValueError, dict(window=-3)), (ValueError, dict(out=q[..., :32])),
-                      (TypeError, dict(out=q.float())), (RuntimeError, dict(lens=lens.cpu())), (ValueError, dict(status=torch.zeros(2, dtype=torch.int32, device=DEV))),
+                      (TypeError, dict(out=q.float())), (TypeError, dict(out=q.half())), (RuntimeError, dict(lens=lens.cpu())), (ValueError, dict(status=torch.zeros(2, dtype=torch.int32, device=DEV))),
                       (RuntimeError, dict(k=k[:, :, :8], v=v[:, :, :8])), (RuntimeError, dict(k=k[..., :32], v=v[..., :32], q=q[..., :32])),
                       (RuntimeError, dict(q=q.clone().requires_grad_()))]:
         with pytest.raises(error):

@@ -49,6 +49,29 @@ def test_unequal_sequences_give_what_each_gives_alone(D, dtype, window, keep):
                 _close(a, b, f"sequence {i}, step {n}")
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_step_in_one_call_and_kernel_by_kernel_are_the_same(dtype, monkeypatch):
+    from daisy_amd import _lib
+    model, prompts, g = model_and_prompts([9, 40, 3])
+    a, b = paged(model, 4, dtype=dtype), paged(model, 4, dtype=dtype)
+    native = _lib.native()
+
+    class WithoutTheCall:
+        def __getattr__(self, name):
+            return (lambda *args: None) if name == "paged_layer_step" else getattr(native, name)
+
+    with torch.inference_mode():
+        for c in (a, b):
+            core.admit(model, prompts, c)
+        for _ in range(4):
+            tokens = torch.randint(2, 96, (4,), generator=g, device=DEV)
+            one = core.step(model, tokens, a)
+            with monkeypatch.context() as m:
+                m.setattr(_lib, "native", lambda: WithoutTheCall())
+                other = core.step(model, tokens, b)
+            assert torch.equal(one[:3], other[:3])
+
+
 def test_sequences_come_and_go_between_recorded_steps():
     """The recorded step follows admissions and releases, bit for bit as the eager one, and slots that are free disturb nobody."""
     model, prompts, g = model_and_prompts([5, 33, 12, 20, 7])
