@@ -103,7 +103,7 @@ __global__ __launch_bounds__(1024) void logits_kernel(LogitsParams p) {
     constexpr int kWords = 16 / sizeof(Word);
     for (int i = tid; i < p.slice / kWords; i += threads) *reinterpret_cast<u32x4*>(seen + kWords * i) = u32x4{0, 0, 0, 0};
     lg = p.repetition.rows != nullptr ? log2f(p.repetition.rows[b]) : p.repetition.value;
-    presence = setting(p.presence, b);
+    presence = lg != lg ? lg : setting(p.presence, b);      // (a row's number below zero or NaN: its seen tokens are NaN)
     frequency = setting(p.frequency, b);
     const int n = p.lens != nullptr ? min(max(p.lens[b], 0), p.T) : p.T;
     const TOKEN* history = (const TOKEN*)p.history + b * p.h_st;
@@ -143,8 +143,12 @@ __global__ __launch_bounds__(1024) void logits_kernel(LogitsParams p) {
         } else {
           w = count = (float)s;
         }
-        const float power = fminf(w, p.cap) * lg;
-        x[r][i] *= fast_exp2(x[r][i] > 0.f ? -power : power);
+        // in two factors, each of them a normal number: what leaves fp32's range on either side leaves it by the product, and 0 stays 0, -inf
+        // stays -inf (a token that came 400 times at 1.3 has a power of 151)
+        float power = fminf(w, p.cap) * lg;
+        power = fminf(fmaxf(x[r][i] > 0.f ? -power : power, -252.f), 254.f);
+        const float half = rintf(0.5f * power);
+        x[r][i] = x[r][i] * fast_exp2(half) * fast_exp2(power - half);
         x[r][i] -= fmaf(frequency, count, presence);
       }
     }
@@ -201,7 +205,8 @@ extern "C" int daisy_logits_process_fwd(const void* x, int64_t x_stride, void* y
   DAISY_CHECK_SUPPORTED(type >= 0 && type <= 2, "logits_process: type %d not supported (0 fp32, 1 bf16, 2 fp16)", type);
   DAISY_CHECK_ARG(x_stride >= 0 && y_stride >= V * (B > 1), "logits_process: rows of y must not overlap");
   DAISY_CHECK_ARG(!history || (T >= 0 && lookback >= 0), "logits_process: T=%d, lookback=%d must not be negative", T, lookback);
-  DAISY_CHECK_ARG(repetition_rows || repetition > 0.0, "logits_process: repetition must be positive");
+  DAISY_CHECK_SUPPORTED(!history || T < (1 << 30), "logits_process: rows of history of %d tokens are too long", T);
+  DAISY_CHECK_ARG(repetition_rows || (repetition > 0.0 && isfinite(repetition)), "logits_process: repetition must be positive and finite");
   DAISY_CHECK_ARG(half_life >= 0.f && cap >= 0.f, "logits_process: half_life and cap must not be negative");
   if (history && (T == 0 || lookback == 0)) history = nullptr;
   if (lookback > T) lookback = T;

@@ -6,6 +6,8 @@
 // once and replayed while sequences grow, come and go.
 #include "common.h"
 
+#include <float.h>
+
 #include <type_traits>
 
 namespace daisy {
@@ -323,7 +325,7 @@ __global__ __launch_bounds__(256, paged_groups_per_cu(D)) void paged_attn_kernel
     f32x4 acc[J];
 #pragma unroll
     for (int j = 0; j < J; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m = -__builtin_inff(), l = 0.f;
+    float m = -FLT_MAX, l = 0.f;      // (finite: a key may score -inf, a whole tile of them too)
 
     // ---- pages: lane i has that of the run's block i, for 32 tiles at a time
     const int32_t* row = p.table + b * p.table_st;

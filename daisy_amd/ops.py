@@ -1027,8 +1027,8 @@ def process_logits(logits: torch.Tensor, history: Optional[torch.Tensor] = None,
             numbers += [t.data_ptr(), 0.0]
         else:
             numbers += [None, float(t)]
-    if not isinstance(repetition, torch.Tensor) and not repetition > 0.0:
-        raise ValueError(f"repetition must be positive, got {repetition}")
+    if not isinstance(repetition, torch.Tensor) and not 0.0 < repetition < float("inf"):
+        raise ValueError(f"repetition must be positive and finite, got {repetition}")
     strides = []
     for name, t, width, dtype in (("bias", bias, V, torch.float32), ("allowed", allowed, (V + 31) // 32, torch.int32)):
         if t is None:

@@ -132,6 +132,24 @@ def test_masked_places_may_hold_anything():
     assert math.isnan(got[0, 4]) and got[0, 5] == math.inf and got[0, 6] == -math.inf and got[0, 7] == -2.0
 
 
+@pytest.mark.parametrize("repetition", [1.3, 0.7, 1.0])
+def test_powers_beyond_the_range_of_32_bits(repetition):
+    """A token that came hundreds of times has a power of hundreds: zero stays zero, -inf stays -inf, the others end at zero or an infinity."""
+    values = torch.tensor([[0.0, -math.inf, math.inf, 5.0, -5.0, 1e-20, -1e-20, 1e30, -1e30]], device=DEV)
+    n = values.shape[1]
+    for times in (100, 300, 400, 1000, 14000):
+        h = torch.arange(n, device=DEV).repeat(times)[None]
+        got = ops.process_logits(values, h, repetition=repetition)[0].tolist()
+        for y, x in zip(got, values[0].tolist()):
+            power = times * math.log2(repetition) * (-1 if x > 0 else 1)
+            want = x if x == 0 or math.isinf(x) else math.copysign(2.0 ** min(max(math.log2(abs(x)) + power, -1000), 1000), x)
+            if abs(want) >= 2.0 ** 128:
+                assert y == math.copysign(math.inf, want), (times, x)
+            else:
+                # (a result below the normal numbers may be zero)
+                assert y == want or abs(y - want) <= 2 ** -21 * (1 + abs(power)) * abs(want) + 2 ** -126, (times, x, y, want)
+
+
 def test_lowest_values_of_a_type():
     for dtype in (F32, BF16, F16):
         low = torch.finfo(dtype).min
@@ -233,7 +251,7 @@ def test_refusals():
     bits = torch.zeros(2, 2, dtype=torch.int32, device=DEV)
     for error, args, kw in [(TypeError, (x.double(),), {}), (ValueError, (x[None],), {}), (ValueError, (x.t(),), {}), (ValueError, (x, h[:1]), {}), (ValueError, (x, h.float()), {}),
                             (ValueError, (x, None, lens), {}), (ValueError, (x, h, lens.long()), {}), (ValueError, (x, h, lens[:1]), {}), (ValueError, (x, h), dict(half_life=0.0)),
-                            (ValueError, (x, h), dict(cap=-1.0)), (ValueError, (x, h), dict(repetition=0.0)), (ValueError, (x, h), dict(repetition=math.nan)),
+                            (ValueError, (x, h), dict(cap=-1.0)), (ValueError, (x, h), dict(repetition=0.0)), (ValueError, (x, h), dict(repetition=math.nan)), (ValueError, (x, h), dict(repetition=math.inf)),
                             (ValueError, (x, h), dict(repetition=lens.float()[:1])), (ValueError, (x, h), dict(presence=lens)), (ValueError, (x, h), dict(lookback=-1)),
                             (ValueError, (x,), dict(bias=x.bfloat16())), (ValueError, (x,), dict(bias=x[:, :32])), (ValueError, (x,), dict(allowed=bits[:, :1])),
                             (ValueError, (x,), dict(allowed=bits.bool())), (ValueError, (x,), dict(out=x[:1])), (ValueError, (x,), dict(out=x.half())), (RuntimeError, (x.cpu(),), {}),

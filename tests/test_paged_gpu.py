@@ -177,6 +177,32 @@ def test_many_small_probabilities_beside_a_large_one():
     assert abs(float(o[0, 0, 0]) - want) <= (2 * half_step(F16) + 1e-4) * want
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("B", [1, 40])
+def test_keys_that_score_minus_infinity_weigh_nothing(dtype, B):
+    """In single places, a whole tile at the beginning, several in a run and parts of a long sequence: as if they were not there.  A sequence of
+    nothing else has no softmax: NaN."""
+    g = gen(5)
+    n, H, page, D = 5000, 2, 64, 128
+    k, v, table, _ = make_cache([n] * B, H, page, D, dtype, g)
+    q = randn(g, B, H, D, dtype=dtype)
+    q[..., 0] = 1.0
+    off = torch.zeros(n, dtype=torch.bool, device=DEV)
+    for a, b in ((0, 70), (100, 101), (500, 1700), (4990, 5000)):
+        off[a:b] = True
+    lens = torch.full((B,), n, dtype=torch.int32, device=DEV)
+    at = torch.arange(n, device=DEV)
+    for b in range(B):
+        k[table[b, at // page].long()[off], :, (at % page)[off], 0] = -math.inf
+    rows = []
+    for b in range(B):
+        pages = table[b, at // page].long()
+        rows.append((k[pages, :, at % page][~off].double(), v[pages, :, at % page][~off].double()))
+    check_attention(ops.paged_attention(q, k, v, table, lens, scale=0.12), q, rows, 0.12, f"{B} sequences")
+    nothing = ops.paged_attention(q, k, v, table, torch.full_like(lens, 65), scale=0.12)
+    assert bool(torch.isnan(nothing).all())
+
+
 def test_strides_of_every_tensor():
     """Views: queries of one projection, pages that lie [page, row, head, D] or between others, a slice of a wider table, a slice of the output."""
     g = gen(5)
