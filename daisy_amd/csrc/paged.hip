@@ -173,9 +173,9 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
 // query heads of the two, and where the second one's results belong.
 enum { kBeginsInside = 1, kGoesThrough = 2, kEndsInside = 4 };
 struct OpenUnits { int flags, heads0, heads1; int64_t out; };
-// A unit that goes on beyond a workgroup's run: the workgroups that have a part of it (first, last; -1: there is no such unit), its query heads, where
-// its results belong.
-struct SplitUnit { int first, last, heads, unused; int64_t out, unused2; };
+// A unit that goes on beyond a workgroup's run: the workgroups that have a part of it (first, last; -1: there is no such unit), its sequence and
+// which one of the sequence's it is.
+struct SplitUnit { int first, last, b, unit; };
 
 struct PagedParams {
   const uint16_t* q; int64_t q_sb, q_sh;
@@ -287,7 +287,7 @@ __global__ __launch_bounds__(256, paged_groups_per_cu(D)) void paged_attn_kernel
   int x = (int)min((int64_t)wave * share, (int64_t)total);
   const int x_end = (int)min((int64_t)x + share, (int64_t)total);
   OpenUnits mine = {0, 0, 0, 0};
-  SplitUnit beyond = {-1, 0, 0, 0, 0, 0};
+  SplitUnit beyond = {-1, 0, 0, 0};
 
   const uint32_t k_row = (uint32_t)p.k_ss * 2, v_row = (uint32_t)p.v_ss * 2;      // bytes, fewer than 2^24
   // 64 sequences from `base` on, one a lane; up to 64 are all there
@@ -512,7 +512,7 @@ __global__ __launch_bounds__(256, paged_groups_per_cu(D)) void paged_attn_kernel
       mine.out = b * p.o_sb + (int64_t)(h * p.G + head0) * p.o_sh;
     }
     if (off + count < n_tiles && wv == 3)
-      beyond = SplitUnit{(x - off) / (4 * share), (x - off + n_tiles - 1) / (4 * share), min(p.G - head0, 16), 0, b * p.o_sb + (int64_t)(h * p.G + head0) * p.o_sh, 0};
+      beyond = SplitUnit{(x - off) / (4 * share), (x - off + n_tiles - 1) / (4 * share), b, unit};
     x += count;
   }
 
@@ -565,10 +565,10 @@ __device__ __forceinline__ int64_t part_slot(const PagedParams& p, const SplitUn
 
 // A unit's parts, joined for some of its results: CH channels of a head at a time, CH / 4 lanes for them and 1024 / CH parts side by side.
 template <int D, bool F16, int CH>
-__device__ __forceinline__ void join_parts(const PagedParams& p, const SplitUnit& u, int parts, int helpers, int me, float4 (*sums)[16], float2* stats) {
+__device__ __forceinline__ void join_parts(const PagedParams& p, const SplitUnit& u, uint16_t* out, int heads, int parts, int helpers, int me, float4 (*sums)[16], float2* stats) {
   constexpr int LPR = CH / 4, GROUPS = 256 / LPR, U = 4;      // (U parts asked for at once)
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = threadIdx.x / LPR, at = threadIdx.x % LPR * 4;
-  for (int chunk = me; chunk < u.heads * (D / CH); chunk += helpers) {
+  for (int chunk = me; chunk < heads * (D / CH); chunk += helpers) {
     const int head = chunk / (D / CH), d0 = chunk % (D / CH) * CH;
     float m = -__builtin_inff(), l = 0.f;
     f32x4 a = {0.f, 0.f, 0.f, 0.f};
@@ -621,7 +621,7 @@ __device__ __forceinline__ void join_parts(const PagedParams& p, const SplitUnit
         a += w * f32x4{t.x, t.y, t.z, t.w};
       }
       a *= 1.f / all;
-      *reinterpret_cast<u32x2*>(p.o + u.out + head * p.o_sh + d0 + at) = pack_out<F16>(p, a);
+      *reinterpret_cast<u32x2*>(out + head * p.o_sh + d0 + at) = pack_out<F16>(p, a);
     }
   }
 }
@@ -634,11 +634,15 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
   __shared__ float4 sums[4][16];
   __shared__ float2 stats[4];
   const SplitUnit u = p.split[blockIdx.x];
-  if (u.first < 0) return;
+  // No such unit; or, where another call has the same workspace at the same time, one that is not this call's: its results are lost, nothing else is.
+  if (u.first < 0 || u.first > (int)blockIdx.x || u.last <= (int)blockIdx.x || u.last >= p.groups) return;
+  if ((unsigned)u.b >= (unsigned)p.B || (unsigned)u.unit >= (unsigned)(p.H * p.head_tiles)) return;
   const int parts = u.last - u.first + 1, helpers = parts - 1, me = (int)blockIdx.x - u.first;
+  const int h = u.unit / p.head_tiles, head0 = (u.unit - h * p.head_tiles) * 16, heads = min(p.G - head0, 16);
+  uint16_t* out = p.o + u.b * p.o_sb + (int64_t)(h * p.G + head0) * p.o_sh;
   if (parts <= kFew) {
     // a thread per four channels, every part of which it asks for at once
-    for (int col = me + helpers * (int)threadIdx.x; col < u.heads * (D / 4); col += helpers * 256) {
+    for (int col = me + helpers * (int)threadIdx.x; col < heads * (D / 4); col += helpers * 256) {
       const int head = col / (D / 4), at = col % (D / 4) * 4;
       float2 st[kFew];
       f32x4 v[kFew];
@@ -659,15 +663,15 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
         a = i < parts ? a + f * v[i] : a;
       }
       a *= 1.f / l;
-      *reinterpret_cast<u32x2*>(p.o + u.out + head * p.o_sh + at) = pack_out<F16>(p, a);
+      *reinterpret_cast<u32x2*>(out + head * p.o_sh + at) = pack_out<F16>(p, a);
     }
   // as narrow as there are workgroups for the pieces, and as parts ask for a pass of 256, 128, 64
-  } else if (parts > 128 || u.heads * (D / 16) <= helpers) {
-    join_parts<D, F16, 16>(p, u, parts, helpers, me, sums, stats);
-  } else if (parts > 64 || u.heads * (D / 32) <= helpers) {
-    join_parts<D, F16, 32>(p, u, parts, helpers, me, sums, stats);
+  } else if (parts > 128 || heads * (D / 16) <= helpers) {
+    join_parts<D, F16, 16>(p, u, out, heads, parts, helpers, me, sums, stats);
+  } else if (parts > 64 || heads * (D / 32) <= helpers) {
+    join_parts<D, F16, 32>(p, u, out, heads, parts, helpers, me, sums, stats);
   } else {
-    join_parts<D, F16, 64>(p, u, parts, helpers, me, sums, stats);
+    join_parts<D, F16, 64>(p, u, out, heads, parts, helpers, me, sums, stats);
   }
 }
 

@@ -915,7 +915,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     zeros.  Returns ``o [B, Hq, D]`` in q's dtype, or ``out``, which may be bf16 with an fp16 cache.
 
     Lengths and table are read when the kernels run, and the work is split over the lengths that are found there: nothing but shapes is fixed by a
-    recording.  A length beyond the table's room, or a page that is none, gives NaN for the heads of that sequence and raises a bit in ``status``.
+    recording.  ``workspace``: at least ``paged_attention_workspace_bytes`` on the GPU, whatever it holds, for one call at a time (two that run at
+    once, recorded ones too, need one each); ``None``: a tensor made for the call.  A length beyond the table's room, or a page that is none, gives NaN for the heads of that sequence and raises a bit in ``status``.
     """
     if window is not None and window <= 0:
         raise ValueError(f"window must be positive or None, got {window}")

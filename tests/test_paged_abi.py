@@ -62,11 +62,11 @@ def test_logits_argument_errors(kw, rc, text):
 
 def test_workspaces_of_the_paged_attention():
     size = ops.paged_attention_workspace_bytes
-    # 32 bytes and two partial results of D + 2 floats for every query head of a unit, for each workgroup of four wavefronts with a tile of 32 positions each
-    assert size(1, 1, 1, 128, 1, 16) == 32 + 2 * 130 * 4
-    assert size(1, 12, 12, 128, 128, 64) == (256 * 12 // 4) * (32 + 2 * 130 * 4)
-    assert size(1000, 16, 16, 128, 128, 64) == 768 * (32 + 2 * 130 * 4)               # as many workgroups as the chip holds
-    assert size(1000, 64, 1, 128, 128, 64) == 512 * (32 + 2 * 16 * 130 * 4)           # at most 16 heads to a unit; their sums fill the LDS
+    # 16 bytes and two partial results of D + 2 floats for every query head of a unit, for each workgroup of four wavefronts with a tile of 32 positions each
+    assert size(1, 1, 1, 128, 1, 16) == 16 + 2 * 130 * 4
+    assert size(1, 12, 12, 128, 128, 64) == (256 * 12 // 4) * (16 + 2 * 130 * 4)
+    assert size(1000, 16, 16, 128, 128, 64) == 768 * (16 + 2 * 130 * 4)               # as many workgroups as the chip holds
+    assert size(1000, 64, 1, 128, 128, 64) == 512 * (16 + 2 * 16 * 130 * 4)           # at most 16 heads to a unit; their sums fill the LDS
     assert size(1 << 30, 1 << 20, 1 << 20, 128, 1 << 20, 64) == 0
     assert size(0, 1, 1, 128, 1, 16) == size(1, 3, 2, 128, 1, 16) == size(1, 1, 1, 80, 1, 16) == size(1, 1, 1, 128, 1 << 27, 16) == 0
 

@@ -124,6 +124,21 @@ def test_work_is_split_over_what_is_there(lens, H, G):
     check_attention(o, q, rows, ops.ATTN_SCALE, "split")
 
 
+@pytest.mark.parametrize("fill", [0, 0x01, 0x7f, 0xff])
+def test_what_a_workspace_held_before_means_nothing(fill):
+    """One workspace for calls of different shapes, with anything in it."""
+    g = gen(17)
+    cases = []
+    for lens, H, G, D in (([5000, 30, 0], 2, 8, 128), ([100] * 70, 1, 1, 64), ([700, 64, 3], 1, 17, 256)):
+        k, v, table, rows = make_cache(lens, H, 32, D, BF16, g)
+        q = randn(g, len(lens), H * G, D, dtype=BF16)
+        cases.append((q, k, v, table, torch.tensor(lens, dtype=torch.int32, device=DEV)))
+    need = max(ops.paged_attention_workspace_bytes(q.shape[0], q.shape[1], k.shape[1], q.shape[2], table.shape[1], 32) for q, k, v, table, _ in cases)
+    space = torch.full((need,), fill, dtype=torch.uint8, device=DEV)
+    for args in cases + cases:
+        assert torch.equal(ops.paged_attention(*args, workspace=space), ops.paged_attention(*args))
+
+
 def test_every_sequence_empty():
     g = gen(1)
     k, v, table, _ = make_cache([0, 0, 0], 2, 16, 128, BF16, g)
