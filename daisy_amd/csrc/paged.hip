@@ -298,8 +298,9 @@ __global__ __launch_bounds__(256, paged_groups_per_cu(D)) void paged_attn_kernel
     before = __builtin_amdgcn_readlane(own_upto - own, first);
   }
   while (x < x_end) {
-    // ---- the unit that x lies in
-    while (chunk < 0 || x >= (before + chunk) * units) {
+    // ---- the unit that x lies in.  (More than 64 lengths are read twice: somebody who changes them meanwhile gets wrong results, but every index below
+    // stays inside the call's tensors and x goes on.)
+    while (chunk < 0 || (x >= (before + chunk) * units && base < p.B)) {
       if (chunk >= 0) { before += chunk; base += 64; }
       len = len_of(p, base + lane);
       tiles = extent(p, len).tiles;
@@ -307,12 +308,12 @@ __global__ __launch_bounds__(256, paged_groups_per_cu(D)) void paged_attn_kernel
       chunk = __builtin_amdgcn_readlane(upto, 63);
     }
     const uint64_t here = __ballot(tiles > 0 && (before + upto - tiles) * units <= x);
-    const int bl = 63 - __builtin_clzll(here);
-    const int b = base + bl, n_tiles = __builtin_amdgcn_readlane(tiles, bl);
+    const int bl = 63 - __builtin_clzll(here | 1);
+    const int b = min(base + bl, p.B - 1), n_tiles = max(__builtin_amdgcn_readlane(tiles, bl), 1);
     const Extent e = extent(p, __builtin_amdgcn_readlane(len, bl));
     const int rel = x - (before + __builtin_amdgcn_readlane(upto, bl) - n_tiles) * units;
-    const int unit = rel / n_tiles, off = rel - unit * n_tiles;
-    const int count = min(n_tiles - off, x_end - x);
+    const int unit = min(rel / n_tiles, units - 1), off = rel - unit * n_tiles;
+    const int count = max(min(n_tiles - off, x_end - x), 1);
     const int h = unit / p.head_tiles, head0 = (unit - h * p.head_tiles) * 16;
 
     // ---- its query heads: columns past the last one repeat it
