@@ -148,7 +148,7 @@ class Generator:
         self._paged_cache: Optional[PagedKVCache] = None
         self._paged_step = None
         # What ops.process_logits adds to the repetition penalty, over the same last tokens: a bias per token ({id: value} or [vocab]), and
-        # allowed_tokens(seen [B, T], lens [B]) -> which tokens may follow, bool [B, vocab] or bits (ops.pack_allowed), or None for all.
+        # allowed_tokens(seen [B, T], lens [B]) -> which tokens may follow, bool [B, vocab] or bits (ops.pack_allowed), or None for all; a row in which none may ends.
         self.presence_penalty, self.frequency_penalty = float(presence_penalty), float(frequency_penalty)
         self.allowed_tokens = allowed_tokens
         self.logit_bias = self._bias_row(logit_bias)
@@ -233,6 +233,13 @@ class Generator:
         return ops.process_logits(logits, seen, lens, repetition=strength, half_life=140.0, cap=3.0, presence=self.presence_penalty,
                                   frequency=self.frequency_penalty, lookback=_PENALTY_LOOKBACK, bias=self.logit_bias, allowed=allowed)
 
+    def _draw(self, scores: Tensor) -> Tensor:
+        """A token per row; the end of the sequence where the mask lets nothing follow."""
+        token = self.sample(scores, self.temperature, self.top_k, self.top_p)
+        if self.allowed_tokens is None:
+            return token
+        return torch.where(scores.amax(dim=-1) == _NEG_INF, self.eos_token_id.to(token.dtype), token)
+
     # -- model calls -----------------------------------------------------------------------
     def _prefill(self, prompt_ids: Tensor) -> Tensor:
         """Runs the prompt, stores its keys and values (the last ``W - 1`` positions fit) and
@@ -307,7 +314,7 @@ class Generator:
                 scores = self._adjusted(logits[-1:], self.history[None], seen)[0]
             else:
                 scores = self._penalised(logits[-1], self.history[-_PENALTY_LOOKBACK:])
-            token = self.sample(scores, self.temperature, self.top_k, self.top_p)
+            token = self._draw(scores)
             if token == self.eos_token_id:
                 break
             yield token.view(1)
@@ -359,7 +366,7 @@ class Generator:
                 scores = self._adjusted(scores, seen[:, :n_seen], torch.full((B,), n_seen, dtype=torch.int32, device=self.device))
             else:
                 scores = self._penalised(scores, seen[:, max(n_seen - _PENALTY_LOOKBACK, 0):n_seen])
-            token = self.sample(scores, self.temperature, self.top_k, self.top_p)
+            token = self._draw(scores)
             token = torch.where(done, eos, token)
             done |= token == eos
             seen[:, n_seen] = token
@@ -402,7 +409,7 @@ class Generator:
         done = torch.zeros(B, dtype=torch.bool, device=self.device)
         for produced in range(1, max_new_tokens + 1):
             scores = self._adjusted(self._trim(logits), seen, lens)
-            token = self.sample(scores, self.temperature, self.top_k, self.top_p)
+            token = self._draw(scores)
             token = torch.where(done, eos, token)
             done |= token == eos
             seen.scatter_(1, lens.long()[:, None], token[:, None])

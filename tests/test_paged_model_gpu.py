@@ -189,6 +189,17 @@ def test_presence_and_frequency_penalties_biases_and_masks_reach_every_loop():
         assert generator(model, allowed_tokens=lambda seen, lens: bits).generate_batch(both, 2).tolist() == [[33] * 2] * 2
         plain, none = generator(model, presence_penalty=0.0), generator(model, allowed_tokens=lambda seen, lens: None)
         assert torch.equal(none.generate_batch(both, 4), plain.generate_batch(both, 4))
+        # nothing may follow after the second token of the first row: it ends, the other goes on
+        def two(seen, lens):
+            keep = torch.ones(seen.size(0), 96, dtype=torch.bool, device=DEV)
+            keep[:, 1] = False
+            keep[:1] &= (lens[:1, None] < 11)
+            return keep
+        for temperature, top_p in ((0.0, None), (1.0, 0.9)):
+            gen = generator(model, allowed_tokens=two, temperature=temperature, top_p=top_p)
+            for out in (gen.generate_batch(both, 5), gen.generate_ragged(prompts, 5)):
+                assert (out[0] == 1).tolist() == [False, False, True, True, True] and not bool((out[1] == 1).any())
+            assert len([t for t in gen.generate(prompts[0], 5)]) == 2
     with pytest.raises(ValueError, match="token 96"):
         generator(model, logit_bias={96: 1.0})
     gen = generator(model, presence_penalty=1.0)
