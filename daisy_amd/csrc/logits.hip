@@ -5,9 +5,12 @@
 //   y = (x > 0 ? x / s : x s) - f n - p [n > 0] + bias[v],  and -inf where the mask's bit of v is clear.
 // Fp32 throughout, rounded once.  r, f and p are numbers or one per row.
 //
-// A workgroup takes a slice of one row's vocabulary, a word of 64 bits of the LDS for each of its tokens: it reads the history, adds one to
-// the count (17 bits) and the weight to the sum (17 + 30 bits) of every token of its slice in one integer atomic, so that the result
-// does not depend on the order, and then goes over the logits, which it has asked for before.
+// A workgroup takes a slice of one row's vocabulary, a word of the LDS for each of its tokens: it reads the history and counts the tokens of its
+// slice with integer atomics, whose order changes nothing: 32 bits of count, or with a half life 64 bits, count (17 bits) and sum of weights (17 + 30 bits)
+// in one addition.  Then it goes over the logits, which it has asked for before.
+//
+// Bound by HBM, each logit read and written once, for large batches: 256 rows of 131072 in bf16 after 4096 tokens, 281 MB, 57.6 us = 4.9 TB/s, a large
+// copy's rate; 64 of 50304 in fp32, with a mask, 27 MB, 7.6 us.  One row is a launch and two reads one behind the other: 3.5 us, where an empty launch takes 2.3.
 #include "common.h"
 
 #include <math.h>
@@ -17,7 +20,7 @@
 namespace daisy {
 
 enum LogitsType { kLogitsF32 = 0, kLogitsBf16 = 1, kLogitsF16 = 2 };
-constexpr int kWeightBits = 30, kCountShift = 47;      // a weight of one is 2^30; 2^17 - 1 of them stay below the count
+constexpr int kWeightBits = 30, kCountShift = 47;      // a weight of one is 2^30; 2^17 - 1 of them stay below the count, which has the 17 bits above
 constexpr int kMostHistory = (1 << 17) - 1;
 
 struct RowSetting { float value; const float* rows; };
@@ -34,7 +37,7 @@ struct LogitsParams {
   int V, slice;
 };
 
-// Four values of a row from element v on, where nothing but the elements' own alignment is known; `full`: all four are there.
+// Four values of a row from element v on, as many as `left` there are, where nothing but the elements' own alignment is known.
 typedef float f32x4_near __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint16_t u16x4_near __attribute__((ext_vector_type(4), aligned(2)));
 template <int E> __device__ __forceinline__ float widen(uint16_t u) {

@@ -59,7 +59,13 @@ struct AppendParams {
   int32_t* status;
 };
 
-// A row of D channels is shared by D / 16 lanes; lane c holds channels [8c, 8c + 8) and their partners of the rotation.
+// A row of D channels is shared by D / 16 lanes; lane c holds channels [8c, 8c + 8) and their partners of the rotation, so that a row is two
+// loads and two stores of 16 bytes a lane and the norm's sum stays among 4 to 16 lanes.
+//
+// Bound by HBM for prompts: 65536 tokens of 8 heads of 128 (32 of queries), 1.64 GB, 316 us = 5.2 TB/s, what a large copy reaches; 6001 tokens of 12 heads
+// of 64, 85 MB, 19 us.  A decode step is a launch and three reads one behind the other (position, table, tables of the rotation): 3.3 us for 1 sequence,
+// 3.6 for 64, where an empty launch takes 2.3.  Two, four or eight rows to a group of lanes: 3.3 -> 4.2, 5.7, 9.4 us for a step, against 5 % of a long prompt with
+// two; D / 8 lanes to a row: 317 -> 471 us; inputs or results past the caches: 19.2 -> 22.2 and 24.4 -> 26.1 us at 6001 tokens.
 template <int D, bool IN16, bool CACHE16>
 __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
   constexpr int LPR = D / 16, HALF = D / 2;
@@ -169,6 +175,12 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
 // the columns (one head uses one column of 16: the products are 1/16 of use then and still far from bounding anything), so that
 // a lane holds 4 + 4 keys of one head, and those are, as they are, the B operand of O^T = V^T P^T: rows 4c + r and 16 + 4c + r of a tile for
 // the lanes of group c.  V's rows arrive 16 bytes a lane, and v_perm pairs the keys of neighbouring rows.
+//
+// Bound by reading the cache, 4 H D bytes a position: 2 x 131072 positions, 16 heads of 128, 2.15 GB, 320 us = 6.7 TB/s; 32 sequences of up to 32768, 8 key
+// heads for 64, 123 us = 6.2; 64 of up to 4096 in a window, 69 us = 5.5.  Short work is bound by latencies: a launch that finds nothing to do takes
+// 2.5 us, the second kernel 3.2 more (with parts to join), and a wavefront comes to its first key by three reads (length, page, key).  1 sequence of 8192, 12 heads,
+// 50 MB: 12.1 + 3.2 us; 256 sequences of up to 300, 8 heads of 64: 13.6 + 3.2 us, of which a wavefront lives 7, half of it waiting for memory
+// and a quarter for its turn to issue.
 // What a wavefront's run leaves open: whether it begins inside a unit, whether that goes on beyond it, whether it ends inside another one; the
 // query heads of the two, and where the second one's results belong.
 enum { kBeginsInside = 1, kGoesThrough = 2, kEndsInside = 4 };
@@ -628,7 +640,8 @@ __device__ __forceinline__ void join_parts(const PagedParams& p, const SplitUnit
 }
 
 // Joins the partial sums of the units that lie in more than one workgroup's run.  The results of a unit are dealt to as many workgroups as there are
-// ends of runs in it: to those of the runs that it goes on beyond.
+// ends of runs in it: to those of the runs that it goes on beyond.  A launch and two reads one behind the other, 3.2 us, whatever there is to join; one
+// kernel would need a counter that somebody clears ahead of every call.
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
   constexpr int kFew = 8;
@@ -676,7 +689,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
   }
 }
 
-// How many workgroups share the work: one round of what the chip holds, less where there are fewer tiles.
+// How many workgroups share the work: what the chip holds at once, less where there are fewer tiles.  (Two and three times as many, in rounds: 16 heads to a key
+// head, whose queries every wavefront reads, are slower, the others level.)
 struct PagedSplit { int groups, heads, head_tiles; size_t lds; };
 static PagedSplit paged_split(int B, int H, int G, int D, int64_t capacity) {
   PagedSplit s;
