@@ -181,6 +181,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
 // 2.5 us, the second kernel 3.2 more (with parts to join), and a wavefront comes to its first key by three reads (length, page, key).  1 sequence of 8192, 12 heads,
 // 50 MB: 12.1 + 3.2 us; 256 sequences of up to 300, 8 heads of 64: 13.6 + 3.2 us, of which a wavefront lives 7, half of it waiting for memory
 // and a quarter for its turn to issue.
+
 // What a wavefront's run leaves open: whether it begins inside a unit, whether that goes on beyond it, whether it ends inside another one; the
 // query heads of the two, and where the second one's results belong.
 enum { kBeginsInside = 1, kGoesThrough = 2, kEndsInside = 4 };
