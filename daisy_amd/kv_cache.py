@@ -159,7 +159,8 @@ class PagedKVCache:
     skipped.  With ``window``, pages that no step can see any more go back to the pool.
 
     The host knows every length, so that ``admit`` and ``begin_step`` raise where the pool is empty; the device has the table, the next token's
-    ``positions`` (-1 for a free slot) and the ``lens`` with it, at fixed addresses, for steps recorded in a HIP graph.
+    ``positions`` (-1 for a free slot) and the ``lens`` with it, at fixed addresses, for steps recorded in a HIP graph.  Changes go to the
+    device on the current stream: admissions, releases and steps of one cache belong on the same one.
     """
 
     def __init__(self, L, sequences, H, D, pages, device, dtype, page_size: int = 64, max_len: int = 65536, window: Optional[int] = None):
