@@ -752,7 +752,7 @@ PyObject* py_paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (q_out && !(rows_half(*q_out, 3, dev) && (same_type(*q_out, kp) || same_type(*q_out, k)) && q_out->sizes() == q->sizes())) return none();
   for (const Tensor* t : {k_out, v_out})
     if (t && !(rows_half(*t, 3, dev) && same_type(*t, k) && t->sizes() == k.sizes())) return none();
-  if ((status && !one_of(*status, at::kInt, dev)) || needs_autograd({&k, &v, q, ve, gate})) return none();
+  if ((status && !one_of(*status, at::kInt, dev)) || needs_autograd({&k, &v, q, ve, gate, &kp, &vp})) return none();
   Unlocked unlocked;
   Tensor qo;
   if (q) qo = q_out ? *q_out : empty(q->sizes(), kp.scalar_type(), k);

@@ -236,7 +236,11 @@ __device__ __forceinline__ Extent extent(const PagedParams& p, int len) {
   e.tiles = e.hi > e.lo ? (e.hi + kTile - 1) / kTile - e.first : 0;
   return e;
 }
-__device__ __forceinline__ int len_of(const PagedParams& p, int b) { return b < p.B ? p.lens[b] : 0; }
+// (read in any case: a load under a condition is waited for by itself)
+__device__ __forceinline__ int len_of(const PagedParams& p, int b) {
+  const int len = p.lens[min(b, p.B - 1)];
+  return b < p.B ? len : 0;
+}
 
 constexpr int kCus = 256;
 __device__ __forceinline__ int wave_min(int x) {
@@ -290,9 +294,9 @@ __global__ __launch_bounds__(256, paged_groups_per_cu(D)) void paged_attn_kernel
   int own = 0, n4[4];
   for (int j = 0; j < per_lane; j += 4) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) n4[i] = j + i < per_lane ? len_of(p, lane * per_lane + j + i) : 0;
+    for (int i = 0; i < 4; ++i) n4[i] = len_of(p, lane * per_lane + min(j + i, per_lane - 1));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) own += extent(p, n4[i]).tiles;
+    for (int i = 0; i < 4; ++i) own += j + i < per_lane ? extent(p, n4[i]).tiles : 0;
   }
   const int own_upto = wave_scan(own);
   const int total = __builtin_amdgcn_readlane(own_upto, 63) * units;

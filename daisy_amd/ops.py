@@ -840,7 +840,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     if fast is not None:
         return fast if fast is not True else None
     dev = _lib.require_gpu(k, v, k_pages, v_pages, page_table, positions, rows, q, cos, sin, ve, gate, q_out, k_out, v_out, status)
-    _no_autograd("paged_append", k, v, q, ve, gate)
+    _no_autograd("paged_append", k, v, q, ve, gate, k_pages, v_pages)
     _check_status(status)
     P, H, size, D = _check_pages(k_pages, v_pages, page_table)
     _check_rows("k", k, 3, _HALF_TYPES)

@@ -562,7 +562,8 @@ def test_refusals_name_what_is_wrong():
                       (ValueError, dict(rows=pos.repeat(2))), (ValueError, dict(cos=cos)), (ValueError, dict(cos=cos, sin=sin[:40])), (ValueError, dict(cos=cos.bfloat16(), sin=sin.bfloat16())),
                       (ValueError, dict(eps=-1.0)), (ValueError, dict(ve=x)), (ValueError, dict(ve=x[..., :32], gate=cos[0, :1])), (ValueError, dict(q_out=x)), (TypeError, dict(q=x.float())),
                       (ValueError, dict(q=x[:, :0])), (ValueError, dict(q=x, q_out=x[:0])), (ValueError, dict(k_out=x[:0])), (TypeError, dict(v_out=x.half())),
-                      (ValueError, dict(table=table[:0])), (RuntimeError, dict(pos=pos.cpu())), (RuntimeError, dict(k=x.clone().requires_grad_()))]:
+                      (ValueError, dict(table=table[:0])), (RuntimeError, dict(pos=pos.cpu())), (RuntimeError, dict(k=x.clone().requires_grad_())),
+                      (RuntimeError, dict(k_pages=k.clone().requires_grad_()))]:
         with pytest.raises(error):
             call(**kw)
     with torch.no_grad():
