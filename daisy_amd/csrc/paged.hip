@@ -183,26 +183,30 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
 // and a quarter for its turn to issue.
 
 // What a wavefront's run leaves open: whether it begins inside a unit, whether that goes on beyond it, whether it ends inside another one; the
-// query heads of the two, and where the second one's results belong.
+// query heads of the two, and of the second one its sequence and its first head.
 enum { kBeginsInside = 1, kGoesThrough = 2, kEndsInside = 4 };
-struct OpenUnits { int flags, heads0, heads1; int64_t out; };
+struct OpenUnits { int flags, heads0, heads1, b, head; };
 // A unit that goes on beyond a workgroup's run: the workgroups that have a part of it (first, last; -1: there is no such unit), its sequence and
 // which one of the sequence's it is.
 struct SplitUnit { int first, last, b, unit; };
 
 struct PagedParams {
-  const uint16_t* q; int64_t q_sb, q_sh;
-  const uint16_t* k; int64_t k_sp, k_sh, k_ss;
-  const uint16_t* v; int64_t v_sp, v_sh, v_ss;
-  const int32_t* table; int64_t table_st; int max_pages, num_pages, blocks_per_page, capacity;
+  // (strides of q, k, v and o in pieces of 16 bytes: with 32 bits of them, an index's product is two scalar instructions)
+  const uint16_t* q; uint32_t q_sb, q_sh;
+  const uint16_t* k; uint32_t k_sp, k_sh, k_ss;
+  const uint16_t* v; uint32_t v_sp, v_sh, v_ss;
+  const int32_t* table; uint32_t table_st; int max_pages, num_pages, blocks_per_page, capacity;
   const int32_t* lens;
-  uint16_t* o; int64_t o_sb, o_sh; int o_f16;
+  uint16_t* o; uint32_t o_sb, o_sh; int o_f16;
   SplitUnit* split;               // [workgroups]
   float* part; float2* stat;      // [2 * workgroups][heads of a unit][D], [..][..]: unnormalised sums; reference and sum of exponentials
   int B, H, G, head_tiles, heads, window, groups;      // heads: of a unit, min(G, 16); groups: workgroups
   float scale_log2e;
   int32_t* status;
 };
+
+__device__ __forceinline__ uint64_t product(int i, uint32_t stride) { return (uint64_t)(uint32_t)i * stride; }
+__device__ __forceinline__ uint16_t* row_of_o(const PagedParams& p, int b, int head) { return p.o + 8 * (product(b, p.o_sb) + product(head, p.o_sh)); }
 
 // Four results in the type of o: bf16, or an fp16 cache's.
 template <bool F16> __device__ __forceinline__ u32x2 pack_out(const PagedParams& p, const f32x4& f) {
@@ -232,8 +236,8 @@ __device__ __forceinline__ Extent extent(const PagedParams& p, int len) {
   e.past = len > p.capacity;
   e.hi = min(max(len, 0), p.capacity);
   e.lo = p.window > 0 ? max(e.hi - p.window, 0) : 0;
-  e.first = e.lo / kTile;
-  e.tiles = e.hi > e.lo ? (e.hi + kTile - 1) / kTile - e.first : 0;
+  e.first = (unsigned)e.lo / kTile;
+  e.tiles = e.hi > e.lo ? (int)((unsigned)(e.hi + kTile - 1) / kTile) - e.first : 0;
   return e;
 }
 // (read in any case: a load under a condition is waited for by itself)
@@ -303,10 +307,10 @@ __global__ __launch_bounds__(256, paged_groups_per_cu(D)) void paged_attn_kernel
   const int share = share_of(p, total, lane);
   int x = (int)min((int64_t)wave * share, (int64_t)total);
   const int x_end = (int)min((int64_t)x + share, (int64_t)total);
-  OpenUnits mine = {0, 0, 0, 0};
+  OpenUnits mine = {0, 0, 0, 0, 0};
   SplitUnit beyond = {-1, 0, 0, 0};
 
-  const uint32_t k_row = (uint32_t)p.k_ss * 2, v_row = (uint32_t)p.v_ss * 2;      // bytes, fewer than 2^24
+  const uint32_t k_row = p.k_ss * 16, v_row = p.v_ss * 16;      // bytes, fewer than 2^24
   // 64 sequences from `base` on, one a lane; up to 64 are all there
   int base = 0, before = 0, len = n4[0], tiles = own, upto = own_upto, chunk = per_lane == 1 ? __builtin_amdgcn_readlane(own_upto, 63) : -1;
   if (per_lane > 1 && x < x_end) {
@@ -329,14 +333,14 @@ __global__ __launch_bounds__(256, paged_groups_per_cu(D)) void paged_attn_kernel
     const int b = min(base + bl, p.B - 1), n_tiles = max(__builtin_amdgcn_readlane(tiles, bl), 1);
     const Extent e = extent(p, __builtin_amdgcn_readlane(len, bl));
     const int rel = x - (before + __builtin_amdgcn_readlane(upto, bl) - n_tiles) * units;
-    const int unit = min(rel / n_tiles, units - 1), off = rel - unit * n_tiles;
+    const int unit = (int)min((unsigned)rel / (unsigned)n_tiles, (unsigned)units - 1), off = rel - unit * n_tiles;
     const int count = max(min(n_tiles - off, x_end - x), 1);
-    const int h = unit / p.head_tiles, head0 = (unit - h * p.head_tiles) * 16;
+    const int h = p.head_tiles == 1 ? unit : (int)((unsigned)unit / (unsigned)p.head_tiles), head0 = (unit - h * p.head_tiles) * 16;
 
     // ---- its query heads: columns past the last one repeat it
     u32x4 qf[KS];
     {
-      const uint16_t* src = p.q + b * p.q_sb + (int64_t)(h * p.G + min(head0 + n, p.G - 1)) * p.q_sh + 8 * c;
+      const uint16_t* src = p.q + 8 * (product(b, p.q_sb) + product(h * p.G + min(head0 + n, p.G - 1), p.q_sh) + c);
 #pragma unroll
       for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const u32x4*>(src + 32 * s);
     }
@@ -346,8 +350,8 @@ __global__ __launch_bounds__(256, paged_groups_per_cu(D)) void paged_attn_kernel
     float m = -FLT_MAX, l = 0.f;      // (finite: a key may score -inf, a whole tile of them too)
 
     // ---- pages: lane i has that of the run's block i, for 32 tiles at a time
-    const int32_t* row = p.table + b * p.table_st;
-    const int blk_lo = e.lo / kBlock, blk_hi = (e.hi - 1) / kBlock;
+    const int32_t* row = p.table + product(b, p.table_st);
+    const int blk_lo = (unsigned)e.lo / kBlock, blk_hi = max(e.hi - 1, 0) / kBlock;
     bool bad = e.past;
     int id = 0, in = 0;
     auto pages_from = [&](int block) {
@@ -359,16 +363,16 @@ __global__ __launch_bounds__(256, paged_groups_per_cu(D)) void paged_attn_kernel
       bad |= out;
       id = out ? 0 : id;
     };
-    const char* kh = reinterpret_cast<const char*>(p.k + h * p.k_sh);
-    const char* vh = reinterpret_cast<const char*>(p.v + h * p.v_sh);
+    const char* kh = reinterpret_cast<const char*>(p.k) + 16 * product(h, p.k_sh);
+    const char* vh = reinterpret_cast<const char*>(p.v) + 16 * product(h, p.v_sh);
     u32x4 kr[2][KS];
     uint32_t vr[8][VD];
     const int tile0 = e.first + off;
     auto at_edge = [&](int i) { return (tile0 + i) * kTile < e.lo || (tile0 + i + 1) * kTile > e.hi; };
     // Half `half` of tile i of the run: where its rows are, in the pages of `base`.
-    auto half_tile = [&](const char* base, int64_t sp, int64_t ss, int i, int half) {
-      const int64_t pg = __builtin_amdgcn_readlane(id, 2 * (i & 31) + half), slot = __builtin_amdgcn_readlane(in, 2 * (i & 31) + half) * kBlock;
-      return base + (pg * sp + slot * ss) * 2;
+    auto half_tile = [&](const char* base, uint32_t sp, uint32_t ss, int i, int half) {
+      const int pg = __builtin_amdgcn_readlane(id, 2 * (i & 31) + half), slot = __builtin_amdgcn_readlane(in, 2 * (i & 31) + half) * kBlock;
+      return base + 16 * (product(pg, sp) + product(slot, ss));
     };
     // A row of it, or where that is outside the range, another one that is read anyhow: nothing is fetched for the rows that a short sequence does not
     // have, and every tile is asked for by the same instructions in the same order, which the waits for them count.
@@ -496,7 +500,7 @@ __global__ __launch_bounds__(256, paged_groups_per_cu(D)) void paged_attn_kernel
     if (head < p.G) {
       if (off == 0 && count == n_tiles) {
         const float inv = 1.f / l;
-        uint16_t* dst = p.o + b * p.o_sb + (int64_t)(h * p.G + head) * p.o_sh + 4 * W * c;
+        uint16_t* dst = row_of_o(p, b, h * p.G + head) + 4 * W * c;
 #pragma unroll
         for (int t = 0; t < P; ++t)
 #pragma unroll
@@ -527,7 +531,8 @@ __global__ __launch_bounds__(256, paged_groups_per_cu(D)) void paged_attn_kernel
     } else if (count < n_tiles) {
       mine.flags |= kEndsInside;
       mine.heads1 = min(p.G - head0, 16);
-      mine.out = b * p.o_sb + (int64_t)(h * p.G + head0) * p.o_sh;
+      mine.b = b;
+      mine.head = h * p.G + head0;
     }
     if (off + count < n_tiles && wv == 3)
       beyond = SplitUnit{(x - off) / (4 * share), (x - off + n_tiles - 1) / (4 * share), b, unit};
@@ -541,7 +546,7 @@ __global__ __launch_bounds__(256, paged_groups_per_cu(D)) void paged_attn_kernel
   for (int b = blockIdx.x; b < p.B; b += p.groups) {
     if (extent(p, p.lens[b]).tiles > 0) continue;
     for (int i = threadIdx.x; i < p.H * p.G * (D / 8); i += 256)
-      *reinterpret_cast<u32x4*>(p.o + b * p.o_sb + (i / (D / 8)) * p.o_sh + i % (D / 8) * 8) = u32x4{0, 0, 0, 0};
+      *reinterpret_cast<u32x4*>(row_of_o(p, b, i / (D / 8)) + i % (D / 8) * 8) = u32x4{0, 0, 0, 0};
   }
   __syncthreads();
   for (int w = 0; w < 4; ++w) {
@@ -566,7 +571,7 @@ __global__ __launch_bounds__(256, paged_groups_per_cu(D)) void paged_attn_kernel
         }
         if (which == 1 && !on) {
           sum *= 1.f / st.y;
-          *reinterpret_cast<u32x2*>(p.o + open_units[w].out + g * p.o_sh + at) = pack_out<F16>(p, sum);
+          *reinterpret_cast<u32x2*>(row_of_o(p, open_units[w].b, open_units[w].head + g) + at) = pack_out<F16>(p, sum);
         } else {
           *reinterpret_cast<f32x4*>(p.part + (slot + g) * D + at) = sum;
           if (at == 0) p.stat[slot + g] = st;
@@ -583,7 +588,7 @@ __device__ __forceinline__ int64_t part_slot(const PagedParams& p, const SplitUn
 
 // A unit's parts, joined for some of its results: CH channels of a head at a time, CH / 4 lanes for them and 1024 / CH parts side by side.
 template <int D, bool F16, int CH>
-__device__ __forceinline__ void join_parts(const PagedParams& p, const SplitUnit& u, uint16_t* out, int heads, int parts, int helpers, int me, float4 (*sums)[16], float2* stats) {
+__device__ __forceinline__ void join_parts(const PagedParams& p, const SplitUnit& u, int first_head, int heads, int parts, int helpers, int me, float4 (*sums)[16], float2* stats) {
   constexpr int LPR = CH / 4, GROUPS = 256 / LPR, U = 4;      // (U parts asked for at once)
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = threadIdx.x / LPR, at = threadIdx.x % LPR * 4;
   for (int chunk = me; chunk < heads * (D / CH); chunk += helpers) {
@@ -639,7 +644,7 @@ __device__ __forceinline__ void join_parts(const PagedParams& p, const SplitUnit
         a += w * f32x4{t.x, t.y, t.z, t.w};
       }
       a *= 1.f / all;
-      *reinterpret_cast<u32x2*>(out + head * p.o_sh + d0 + at) = pack_out<F16>(p, a);
+      *reinterpret_cast<u32x2*>(row_of_o(p, u.b, first_head + head) + d0 + at) = pack_out<F16>(p, a);
     }
   }
 }
@@ -657,8 +662,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
   if (u.first < 0 || u.first > (int)blockIdx.x || u.last <= (int)blockIdx.x || u.last >= p.groups) return;
   if ((unsigned)u.b >= (unsigned)p.B || (unsigned)u.unit >= (unsigned)(p.H * p.head_tiles)) return;
   const int parts = u.last - u.first + 1, helpers = parts - 1, me = (int)blockIdx.x - u.first;
-  const int h = u.unit / p.head_tiles, head0 = (u.unit - h * p.head_tiles) * 16, heads = min(p.G - head0, 16);
-  uint16_t* out = p.o + u.b * p.o_sb + (int64_t)(h * p.G + head0) * p.o_sh;
+  const int h = u.unit / p.head_tiles, head0 = (u.unit - h * p.head_tiles) * 16, heads = min(p.G - head0, 16), first_head = h * p.G + head0;
   if (parts <= kFew) {
     // a thread per four channels, every part of which it asks for at once
     for (int col = me + helpers * (int)threadIdx.x; col < heads * (D / 4); col += helpers * 256) {
@@ -682,15 +686,15 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
         a = i < parts ? a + f * v[i] : a;
       }
       a *= 1.f / l;
-      *reinterpret_cast<u32x2*>(out + head * p.o_sh + at) = pack_out<F16>(p, a);
+      *reinterpret_cast<u32x2*>(row_of_o(p, u.b, first_head + head) + at) = pack_out<F16>(p, a);
     }
   // as narrow as there are workgroups for the pieces, and as parts ask for a pass of 256, 128, 64
   } else if (parts > 128 || heads * (D / 16) <= helpers) {
-    join_parts<D, F16, 16>(p, u, out, heads, parts, helpers, me, sums, stats);
+    join_parts<D, F16, 16>(p, u, first_head, heads, parts, helpers, me, sums, stats);
   } else if (parts > 64 || heads * (D / 32) <= helpers) {
-    join_parts<D, F16, 32>(p, u, out, heads, parts, helpers, me, sums, stats);
+    join_parts<D, F16, 32>(p, u, first_head, heads, parts, helpers, me, sums, stats);
   } else {
-    join_parts<D, F16, 64>(p, u, out, heads, parts, helpers, me, sums, stats);
+    join_parts<D, F16, 64>(p, u, first_head, heads, parts, helpers, me, sums, stats);
   }
 }
 
@@ -734,6 +738,11 @@ static bool step_of_16(int64_t stride, int n) { return n == 1 || (stride % 8 == 
 static bool rows_of_16(const int64_t* strides, int n0, int n1) { return step_of_16(strides[0], n0) && step_of_16(strides[1], n1); }
 // Rows that are written: two of them are not the same.
 static bool apart(const int64_t* strides, int n0, int n1) { return (n0 == 1 || strides[0] > 0) && (n1 == 1 || strides[1] > 0); }
+static uint32_t pieces_of_16(int64_t stride, int n) { return n == 1 ? 0 : (uint32_t)(stride / 8); }
+static int64_t max_stride(const int64_t* strides, int n0, int n1) {
+  const int64_t a = n0 == 1 ? 0 : strides[0], b = n1 == 1 ? 0 : strides[1];
+  return a > b ? a : b;
+}
 // A page's rows are reached with 24-bit products.
 static bool page_rows_fit(const int64_t* strides) { return step_of_16(strides[2], 16) && strides[2] < ((int64_t)1 << 23); }
 
@@ -860,6 +869,9 @@ extern "C" int daisy_paged_attn_fwd(const void* q, const int64_t* q_strides,
   DAISY_CHECK_ARG(paged_tiles_fit(B, Hq, H, capacity), "paged_attn: %d sequences of up to %lld positions, %d key heads, are too many", B, (long long)capacity, H);
   DAISY_CHECK_SUPPORTED(!o_is_f16 || cache_is_f16, "paged_attn: an fp16 o needs an fp16 cache");
   DAISY_CHECK_ARG(apart(o_strides, B, Hq), "paged_attn: rows of o must not overlap");
+  constexpr int64_t kWidest = (int64_t)1 << 35;
+  DAISY_CHECK_SUPPORTED(max_stride(q_strides, B, Hq) < kWidest && max_stride(o_strides, B, Hq) < kWidest && max_stride(k_pages_strides, num_pages, H) < kWidest &&
+                            max_stride(v_pages_strides, num_pages, H) < kWidest && (B == 1 || table_stride < (int64_t)1 << 32), "paged_attn: a stride is too long (2^35 elements, 2^32 of the table)");
   const PagedSplit sp = paged_split(B, H, Hq / H, D, capacity);
   const size_t need = daisy_paged_attn_workspace_bytes(B, Hq, H, D, max_pages, page_size);
   if (workspace == nullptr || workspace_bytes < need || !al16(workspace)) {
@@ -867,13 +879,15 @@ extern "C" int daisy_paged_attn_fwd(const void* q, const int64_t* q_strides,
     return DAISY_ERR_WORKSPACE;
   }
   PagedParams p = {};
-  p.q = (const uint16_t*)q; p.q_sb = q_strides[0]; p.q_sh = q_strides[1];
-  p.k = (const uint16_t*)k_pages; p.k_sp = k_pages_strides[0]; p.k_sh = k_pages_strides[1]; p.k_ss = k_pages_strides[2];
-  p.v = (const uint16_t*)v_pages; p.v_sp = v_pages_strides[0]; p.v_sh = v_pages_strides[1]; p.v_ss = v_pages_strides[2];
-  p.table = page_table; p.table_st = table_stride; p.max_pages = max_pages; p.num_pages = num_pages;
+  p.q = (const uint16_t*)q; p.q_sb = pieces_of_16(q_strides[0], B); p.q_sh = pieces_of_16(q_strides[1], Hq);
+  p.k = (const uint16_t*)k_pages; p.k_sp = pieces_of_16(k_pages_strides[0], num_pages); p.k_sh = pieces_of_16(k_pages_strides[1], H);
+  p.k_ss = pieces_of_16(k_pages_strides[2], page_size);
+  p.v = (const uint16_t*)v_pages; p.v_sp = pieces_of_16(v_pages_strides[0], num_pages); p.v_sh = pieces_of_16(v_pages_strides[1], H);
+  p.v_ss = pieces_of_16(v_pages_strides[2], page_size);
+  p.table = page_table; p.table_st = B == 1 ? 0 : (uint32_t)table_stride; p.max_pages = max_pages; p.num_pages = num_pages;
   p.blocks_per_page = page_size / kBlock; p.capacity = (int)capacity;
   p.lens = lens;
-  p.o = (uint16_t*)o; p.o_f16 = o_is_f16; p.o_sb = o_strides[0]; p.o_sh = o_strides[1];
+  p.o = (uint16_t*)o; p.o_f16 = o_is_f16; p.o_sb = pieces_of_16(o_strides[0], B); p.o_sh = pieces_of_16(o_strides[1], Hq);
   p.split = (SplitUnit*)workspace;
   p.part = (float*)(p.split + sp.groups);
   p.stat = (float2*)(p.part + (size_t)2 * sp.groups * sp.heads * D);

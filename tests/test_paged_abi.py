@@ -32,6 +32,8 @@ def append(q=P, k=P, v=P, table=P, stride=4, n_seq=1, max_pages=4, num_pages=8, 
     (dict(max_pages=1 << 27, page=16), -1, "too long"), (dict(max_pages=1 << 20, B=1 << 15), -1, "too many"),
     (dict(q=P + 2), -1, "aligned"), (dict(k=P + 8), -1, "aligned"), (dict(ks=(ctypes.c_int64 * 3)(4096, 2048, 129)), -1, "multiples of 8"),
     (dict(ks=(ctypes.c_int64 * 3)(4096, 2048, -128)), -1, "strides"), (dict(ks=(ctypes.c_int64 * 3)(4096, 2048, 1 << 23)), -1, "2^23"),
+    (dict(qs=(ctypes.c_int64 * 2)(256, 1 << 35)), -2, "too long"), (dict(os=(ctypes.c_int64 * 2)(1 << 35, 128), B=2), -2, "too long"),
+    (dict(ks=(ctypes.c_int64 * 3)(1 << 35, 2048, 128)), -2, "too long"), (dict(ks=(ctypes.c_int64 * 3)(4096, 1 << 36, 128)), -2, "too long"), (dict(stride=1 << 32, B=2), -2, "too long"),
     (dict(qs=(ctypes.c_int64 * 2)(128, 4)), -1, "multiples of 8"), (dict(os=(ctypes.c_int64 * 2)(256, 0)), -1, "overlap"), (dict(os=(ctypes.c_int64 * 2)(0, 128), B=2), -1, "overlap"),
     (dict(B=1 << 30, Hq=1 << 20, H=1 << 20, max_pages=1 << 20), -1, "too many"), (dict(ws=None), -3, "workspace"), (dict(ws_bytes=16), -3, "workspace"), (dict(ws=P + 4), -3, "workspace")])
 def test_attention_argument_errors(kw, rc, text):
