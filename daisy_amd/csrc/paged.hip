@@ -262,8 +262,10 @@ __device__ __forceinline__ int wave_min(int x) {
 // 2 x 131072 positions, 16 heads, 3049 runs of 43 tiles 319.6 us, 2048 of 64 329.9.
 __device__ __forceinline__ int share_of(const PagedParams& p, int total, int lane) {
   if (total <= 4 * kCus) return 1;
-  const int least = (total + 4 * p.groups - 1) / (4 * p.groups), more = min(lane, least);
-  const int share = least + more, groups = (total + 4 * share - 1) / (4 * share), load = (groups + kCus - 1) / kCus * share;
+  const int least = (int)((unsigned)(total + 4 * p.groups - 1) / (unsigned)(4 * p.groups)), more = min(lane, least), share = least + more;
+  // (in fp32: one more or less only makes another choice, the same one in every wavefront)
+  const float groups = ceilf((float)total * __builtin_amdgcn_rcpf((float)(4 * share)) - 0.001f);
+  const int load = (int)ceilf(groups * (1.f / kCus)) * share;
   return least + (wave_min((more == 0 ? load - load / 32 : load) * 64 + more) & 63);
 }
 
