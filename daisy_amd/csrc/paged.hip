@@ -196,6 +196,7 @@ struct PagedParams {
   const uint16_t* k; uint32_t k_sp, k_sh, k_ss;
   const uint16_t* v; uint32_t v_sp, v_sh, v_ss;
   const int32_t* table; uint32_t table_st; int max_pages, num_pages, blocks_per_page, capacity;
+  uint32_t per_block;             // 2^32 / blocks_per_page, a little less
   const int32_t* lens;
   uint16_t* o; uint32_t o_sb, o_sh; int o_f16;
   SplitUnit* split;               // [workgroups]
@@ -307,8 +308,8 @@ __global__ __launch_bounds__(256, paged_groups_per_cu(D)) void paged_attn_kernel
   const int own_upto = wave_scan(own);
   const int total = __builtin_amdgcn_readlane(own_upto, 63) * units;
   const int share = share_of(p, total, lane);
-  int x = (int)min((int64_t)wave * share, (int64_t)total);
-  const int x_end = (int)min((int64_t)x + share, (int64_t)total);
+  int x = (int)min((unsigned)wave * (unsigned)share, (unsigned)total);      // (the product is less than twice the total, 2^30 at most, and a share for each wavefront)
+  const int x_end = min(x + share, total);
   OpenUnits mine = {0, 0, 0, 0, 0};
   SplitUnit beyond = {-1, 0, 0, 0};
 
@@ -322,7 +323,7 @@ __global__ __launch_bounds__(256, paged_groups_per_cu(D)) void paged_attn_kernel
   }
   while (x < x_end) {
     // ---- the unit that x lies in.  (More than 64 lengths are read twice: somebody who changes them meanwhile gets wrong results, but every index below
-    // stays inside the call's tensors and x goes on.)
+    // stays inside the call's tensors and x goes on.  Divisors that few units need are read from a lane, which leaves what a division needs where it is.)
     while (chunk < 0 || (x >= (before + chunk) * units && base < p.B)) {
       if (chunk >= 0) { before += chunk; base += 64; }
       len = len_of(p, base + lane);
@@ -337,7 +338,7 @@ __global__ __launch_bounds__(256, paged_groups_per_cu(D)) void paged_attn_kernel
     const int rel = x - (before + __builtin_amdgcn_readlane(upto, bl) - n_tiles) * units;
     const int unit = (int)min((unsigned)rel / (unsigned)n_tiles, (unsigned)units - 1), off = rel - unit * n_tiles;
     const int count = max(min(n_tiles - off, x_end - x), 1);
-    const int h = p.head_tiles == 1 ? unit : (int)((unsigned)unit / (unsigned)p.head_tiles), head0 = (unit - h * p.head_tiles) * 16;
+    const int h = p.head_tiles == 1 ? unit : (int)((unsigned)unit / (unsigned)__builtin_amdgcn_readfirstlane(p.head_tiles)), head0 = (unit - h * p.head_tiles) * 16;
 
     // ---- its query heads: columns past the last one repeat it
     u32x4 qf[KS];
@@ -358,8 +359,11 @@ __global__ __launch_bounds__(256, paged_groups_per_cu(D)) void paged_attn_kernel
     int id = 0, in = 0;
     auto pages_from = [&](int block) {
       const int blk = min(max(block + lane, blk_lo), blk_hi);      // (blocks outside the range: read, but not used)
-      const int at = (unsigned)blk / (unsigned)p.blocks_per_page;
+      int at = (int)__umulhi((unsigned)blk, p.per_block);      // the page, or the one ahead of it: blocks are fewer than 2^27
       in = blk - at * p.blocks_per_page;
+      const bool next = in >= p.blocks_per_page;
+      at += next ? 1 : 0;
+      in -= next ? p.blocks_per_page : 0;
       id = row[at];
       const bool out = (unsigned)id >= (unsigned)p.num_pages;
       bad |= out;
@@ -536,8 +540,10 @@ __global__ __launch_bounds__(256, paged_groups_per_cu(D)) void paged_attn_kernel
       mine.b = b;
       mine.head = h * p.G + head0;
     }
-    if (off + count < n_tiles && wv == 3)
-      beyond = SplitUnit{(x - off) / (4 * share), (x - off + n_tiles - 1) / (4 * share), b, unit};
+    if (off + count < n_tiles && wv == 3) {
+      const unsigned run = (unsigned)__builtin_amdgcn_readfirstlane(4 * share);
+      beyond = SplitUnit{(int)((unsigned)(x - off) / run), (int)((unsigned)(x - off + n_tiles - 1) / run), b, unit};
+    }
     x += count;
   }
 
@@ -551,14 +557,15 @@ __global__ __launch_bounds__(256, paged_groups_per_cu(D)) void paged_attn_kernel
       *reinterpret_cast<u32x4*>(row_of_o(p, b, i / (D / 8)) + i % (D / 8) * 8) = u32x4{0, 0, 0, 0};
   }
   __syncthreads();
+  const int flags = open_units[lane & 3].flags;      // (bit w of each: wavefront w's)
+  const int begin = (int)__ballot(flags & kBeginsInside), through = (int)__ballot(flags & kGoesThrough), end = (int)__ballot(flags & kEndsInside);
   for (int w = 0; w < 4; ++w) {
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
-      const int flags = open_units[w].flags;
-      if (which == 0 ? w > 0 || !(flags & kBeginsInside) : !(flags & kEndsInside)) continue;
-      bool on = which == 1 || (flags & kGoesThrough);
+      if (which == 0 ? w > 0 || !(begin & 1) : !(end >> w & 1)) continue;
+      bool on = which == 1 || (through & 1);
       int last = w;
-      while (on && last < 3) on = open_units[++last].flags & kGoesThrough;
+      while (on && last < 3) on = through >> ++last & 1;
       const int heads = which == 0 ? open_units[w].heads0 : open_units[w].heads1;
       const int64_t slot = (int64_t)(2 * blockIdx.x + which) * p.heads;
       for (int i = threadIdx.x; i < heads * (D / 4); i += 256) {
@@ -887,7 +894,7 @@ extern "C" int daisy_paged_attn_fwd(const void* q, const int64_t* q_strides,
   p.v = (const uint16_t*)v_pages; p.v_sp = pieces_of_16(v_pages_strides[0], num_pages); p.v_sh = pieces_of_16(v_pages_strides[1], H);
   p.v_ss = pieces_of_16(v_pages_strides[2], page_size);
   p.table = page_table; p.table_st = B == 1 ? 0 : (uint32_t)table_stride; p.max_pages = max_pages; p.num_pages = num_pages;
-  p.blocks_per_page = page_size / kBlock; p.capacity = (int)capacity;
+  p.blocks_per_page = page_size / kBlock; p.per_block = 0xffffffffu / (uint32_t)p.blocks_per_page; p.capacity = (int)capacity;
   p.lens = lens;
   p.o = (uint16_t*)o; p.o_f16 = o_is_f16; p.o_sb = pieces_of_16(o_strides[0], B); p.o_sh = pieces_of_16(o_strides[1], Hq);
   p.split = (SplitUnit*)workspace;
