@@ -62,10 +62,11 @@ struct AppendParams {
 // A row of D channels is shared by D / 16 lanes; lane c holds channels [8c, 8c + 8) and their partners of the rotation, so that a row is two
 // loads and two stores of 16 bytes a lane and the norm's sum stays among 4 to 16 lanes.
 //
-// Bound by HBM for prompts: 65536 tokens of 8 heads of 128 (32 of queries), 1.64 GB, 316 us = 5.2 TB/s, what a large copy reaches; 6001 tokens of 12 heads
-// of 64, 85 MB, 19 us.  A decode step is a launch and three reads one behind the other (position, table, tables of the rotation): 3.3 us for 1 sequence,
-// 3.6 for 64, where an empty launch takes 2.3.  Two, four or eight rows to a group of lanes: 3.3 -> 4.2, 5.7, 9.4 us for a step, against 5 % of a long prompt with
-// two; D / 8 lanes to a row: 317 -> 471 us; inputs or results past the caches: 19.2 -> 22.2 and 24.4 -> 26.1 us at 6001 tokens.
+// Bound by HBM for prompts: 65536 tokens of 8 heads of 128 (32 of queries), 1.64 GB, 297 us = 5.5 TB/s, more than a large copy reaches; 6001 tokens of 12 heads
+// of 64, 85 MB, 18.4 us.  A decode step is a launch and reads one behind the other (position, then page and tables' rows): 3.3 us for 1 sequence, 3.4 for 64,
+// where an empty launch takes 2.3.  What a row is combined with is asked for ahead of what depends on it, in registers that tables and ve share: six wavefronts
+// a SIMD.  With separate ones, five: 297 -> 322 us; held to 72 registers, seven: 305.  Tried ahead of that order (317 us, steps 3.4): two, four or eight rows to a group of
+// lanes, 5 % of a long prompt with two, steps 4.2, 5.7, 9.4 us; D / 8 lanes to a row 471 us; inputs or results past the caches 15 and 7 % slower at 6001 tokens.
 template <int D, bool IN16, bool CACHE16>
 __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
   constexpr int LPR = D / 16, HALF = D / 2;
@@ -81,29 +82,28 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
   const u32x4 raw0 = *reinterpret_cast<const u32x4*>(src), raw1 = *reinterpret_cast<const u32x4*>(src + HALF);
   const int pos = p.positions[token];
   const int seq = p.rows != nullptr ? p.rows[token] : token;
+  // What is combined with the row: the tables' rows, which nothing but the position is waited for, or ve.
+  const bool rotated = kind < 2 && p.cos != nullptr, mixed = kind == 2 && p.ve != nullptr;
+  f32x4 with[4];
+  float g = 1.f;
+  if (mixed) {
+    const uint16_t* from = p.ve + token * p.e_st + h * p.e_sh + 8 * c;
+    with[0] = *reinterpret_cast<const f32x4*>(from);
+    with[1] = *reinterpret_cast<const f32x4*>(from + HALF);
+    g = gate_value(p.gate);
+  }
   // A negative position: no token.  Everything else that does not lead to a page of the pool is an error of the caller's that
   // only the device can see: nothing is written to the cache, q and the copies become NaN, the status word says so.
-  const bool skipped = pos < 0;
-  int bits = 0, page = 0, slot = 0;
-  if (!skipped) {
-    if (p.cos != nullptr && pos >= p.table_rows) bits |= DAISY_STATUS_POSITION_PAST_TABLES;
-    const int at = (int)((unsigned)pos / (unsigned)p.page_size);
-    slot = pos - at * p.page_size;
-    if (seq < 0 || seq >= p.seqs || at >= p.max_pages) {
-      bits |= DAISY_STATUS_LENGTH_PAST_PAGES;
-    } else {
-      page = p.table[seq * p.table_st + at];
-      if (page < 0 || page >= p.num_pages) bits |= DAISY_STATUS_PAGE_OUT_OF_RANGE;
-    }
-    if (bits && c == 0 && row == 0) raise_status(p.status, bits);
-  }
-  float cs[8], sn[8];
-  if (p.cos != nullptr && kind < 2) {
-    const int64_t off = (int64_t)(skipped || bits ? 0 : pos) * HALF + 8 * c;
-    const f32x4 c0 = *reinterpret_cast<const f32x4*>(p.cos + off), c1 = *reinterpret_cast<const f32x4*>(p.cos + off + 4);
-    const f32x4 s0 = *reinterpret_cast<const f32x4*>(p.sin + off), s1 = *reinterpret_cast<const f32x4*>(p.sin + off + 4);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) { cs[e] = c0[e]; cs[4 + e] = c1[e]; sn[e] = s0[e]; sn[4 + e] = s1[e]; }
+  const bool skipped = pos < 0, past = p.cos != nullptr && pos >= p.table_rows;
+  const int at = (int)((unsigned)max(pos, 0) / (unsigned)p.page_size), slot = pos - at * p.page_size;
+  const bool nowhere = seq < 0 || seq >= p.seqs || at >= p.max_pages;
+  const int page = skipped || nowhere ? 0 : p.table[seq * p.table_st + at];
+  if (rotated) {
+    const int64_t off = (int64_t)(skipped || past ? 0 : pos) * HALF + 8 * c;
+    with[0] = *reinterpret_cast<const f32x4*>(p.cos + off);
+    with[1] = *reinterpret_cast<const f32x4*>(p.cos + off + 4);
+    with[2] = *reinterpret_cast<const f32x4*>(p.sin + off);
+    with[3] = *reinterpret_cast<const f32x4*>(p.sin + off + 4);
   }
 
   float lo[8], hi[8];
@@ -118,22 +118,27 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) { lo[e] *= rstd; hi[e] *= rstd; }
   }
-  if (kind < 2 && p.cos != nullptr) {
+  if (rotated) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float x1 = lo[e], x2 = hi[e];
-      lo[e] = fmaf(x1, cs[e], x2 * sn[e]);
-      hi[e] = fmaf(x2, cs[e], -(x1 * sn[e]));
+      const float x1 = lo[e], x2 = hi[e], cs = with[e / 4][e % 4], sn = with[2 + e / 4][e % 4];
+      lo[e] = fmaf(x1, cs, x2 * sn);
+      hi[e] = fmaf(x2, cs, -(x1 * sn));
     }
   }
-  if (kind == 2 && p.ve != nullptr) {
-    const uint16_t* src = p.ve + token * p.e_st + h * p.e_sh + 8 * c;
+  if (mixed) {
     float el[8], eh[8];
-    unpack8_as<IN16>(*reinterpret_cast<const u32x4*>(src), el);
-    unpack8_as<IN16>(*reinterpret_cast<const u32x4*>(src + HALF), eh);
-    const float g = gate_value(p.gate), og = 1.f - g;
+    unpack8_as<IN16>(__builtin_bit_cast(u32x4, with[0]), el);
+    unpack8_as<IN16>(__builtin_bit_cast(u32x4, with[1]), eh);
+    const float og = 1.f - g;
 #pragma unroll
     for (int e = 0; e < 8; ++e) { lo[e] = fmaf(g, lo[e], og * el[e]); hi[e] = fmaf(g, hi[e], og * eh[e]); }
+  }
+  int bits = 0;
+  if (!skipped) {
+    bits = (past ? DAISY_STATUS_POSITION_PAST_TABLES : 0) |
+           (nowhere ? DAISY_STATUS_LENGTH_PAST_PAGES : (unsigned)page >= (unsigned)p.num_pages ? DAISY_STATUS_PAGE_OUT_OF_RANGE : 0);
+    if (bits && c == 0 && row == 0) raise_status(p.status, bits);
   }
   if (skipped || bits) {
     const float fill = skipped ? 0.f : __builtin_nanf("");
