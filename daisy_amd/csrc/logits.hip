@@ -9,8 +9,8 @@
 // slice with integer atomics, whose order changes nothing: 32 bits of count, or with a half life 64 bits, count (17 bits) and sum of weights (17 + 30 bits)
 // in one addition.  Then it goes over the logits, which it has asked for before.
 //
-// Bound by HBM, each logit read and written once, for large batches: 256 rows of 131072 in bf16 after 4096 tokens, 281 MB, 57.6 us = 4.9 TB/s, a large
-// copy's rate; 64 of 50304 in fp32, with a mask, 27 MB, 7.6 us.  One row is a launch and two reads one behind the other: 3.5 us, where an empty launch takes 2.3.
+// Bound by HBM, each logit read and written once, for large batches: 256 rows of 131072 in bf16 after 4096 tokens, 281 MB, 52.1 us = 5.4 TB/s, more than
+// a large copy's rate; 64 of 50304 in fp32, with a mask, 27 MB, 7.8 us.  One row is a launch and two reads one behind the other: 3.5 us, where an empty launch takes 2.3.
 #include "common.h"
 
 #include <math.h>
@@ -29,7 +29,7 @@ __device__ __forceinline__ float setting(const RowSetting& s, int b) { return s.
 struct LogitsParams {
   const void* x; int64_t x_st;
   void* y; int64_t y_st;
-  const void* history; int64_t h_st; const int32_t* lens; int T, lookback;
+  const void* history; int64_t h_st; const int32_t* lens; int T, lookback, tokens64;
   RowSetting repetition, presence, frequency;      // (the number `repetition` as its logarithm to base 2)
   float inv_half_life, cap;
   const float* bias; int64_t bias_st;
@@ -39,6 +39,7 @@ struct LogitsParams {
 
 // Four values of a row from element v on, as many as `left` there are, where nothing but the elements' own alignment is known.
 typedef float f32x4_near __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
 typedef uint16_t u16x4_near __attribute__((ext_vector_type(4), aligned(2)));
 template <int E> __device__ __forceinline__ float widen(uint16_t u) {
   if constexpr (E == kLogitsBf16) return bf16lo_to_f32(u);
@@ -48,23 +49,30 @@ template <int E> __device__ __forceinline__ uint16_t narrow(float f) {
   if constexpr (E == kLogitsBf16) return (uint16_t)(pack_bf16x2(f, 0.f) & 0xffffu);
   else return __builtin_bit_cast(uint16_t, (_Float16)f);
 }
-template <int E> __device__ __forceinline__ f32x4 load4(const void* row, int v, int left) {
-  f32x4 f = {0.f, 0.f, 0.f, 0.f};
+// (as they lie there: the 16-bit types take half the registers until they are needed)
+template <int E> struct Four { typedef u16x4 Raw; };
+template <> struct Four<kLogitsF32> { typedef f32x4 Raw; };
+template <int E> __device__ __forceinline__ typename Four<E>::Raw load4(const void* row, int v, int left) {
   if constexpr (E == kLogitsF32) {
     const float* at = (const float*)row + v;
     if (left >= 4) return __builtin_nontemporal_load((const f32x4_near*)at);
+    f32x4 f = {0.f, 0.f, 0.f, 0.f};
     for (int i = 0; i < left; ++i) f[i] = at[i];
+    return f;
   } else {
     const uint16_t* at = (const uint16_t*)row + v;
-    if (left >= 4) {
-      const u16x4_near u = __builtin_nontemporal_load((const u16x4_near*)at);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) f[i] = widen<E>(u[i]);
-      return f;
-    }
-    for (int i = 0; i < left; ++i) f[i] = widen<E>(at[i]);
+    if (left >= 4) return __builtin_nontemporal_load((const u16x4_near*)at);
+    u16x4 u = {0, 0, 0, 0};
+    for (int i = 0; i < left; ++i) u[i] = at[i];
+    return u;
   }
-  return f;
+}
+template <int E> __device__ __forceinline__ f32x4 widen4(const typename Four<E>::Raw& raw) {
+  if constexpr (E == kLogitsF32) {
+    return raw;
+  } else {
+    return f32x4{widen<E>(raw[0]), widen<E>(raw[1]), widen<E>(raw[2]), widen<E>(raw[3])};
+  }
 }
 template <int E> __device__ __forceinline__ void store4(void* row, int v, int left, const f32x4& f) {
   if constexpr (E == kLogitsF32) {
@@ -85,7 +93,10 @@ template <int E> __device__ __forceinline__ void store4(void* row, int v, int le
 }
 
 // COUNT: no history (void), a count per token (uint32_t), or a count and a sum of weights (uint64_t).  ROUNDS: times that a thread has four values of the slice.
-template <int E, typename COUNT, typename TOKEN, int ROUNDS>
+// BIAS: none, one row for all (through the caches), a row each (past them).  MASK: whether there is one.  Where the rows share a bias, past the caches costs 64 rows of
+// 50304 7.9 -> 10.2 us; where each has its own, through them 256 rows of 131072 in bf16 52.1 -> 55.  Branches for them in the loop over the rounds make each
+// round's loads wait for the round before: 58.2.
+template <int E, typename COUNT, int ROUNDS, int BIAS, bool MASK>
 __global__ __launch_bounds__(1024) void logits_kernel(LogitsParams p) {
   constexpr bool kHistory = !std::is_void<COUNT>::value, kDecay = std::is_same<COUNT, uint64_t>::value;
   typedef typename std::conditional<kHistory, COUNT, uint32_t>::type Word;
@@ -95,11 +106,11 @@ __global__ __launch_bounds__(1024) void logits_kernel(LogitsParams p) {
   const int v0 = blockIdx.x * p.slice, v1 = min(v0 + p.slice, p.V);
   const char* x_row = (const char*)p.x + b * p.x_st * (E == kLogitsF32 ? 4 : 2);
   char* y_row = (char*)p.y + b * p.y_st * (E == kLogitsF32 ? 4 : 2);
-  f32x4 x[ROUNDS];
+  typename Four<E>::Raw raw[ROUNDS];
 #pragma unroll
   for (int r = 0; r < ROUNDS; ++r) {
     const int v = v0 + 4 * (tid + r * threads);
-    x[r] = load4<E>(x_row, v, v1 - v);
+    raw[r] = load4<E>(x_row, v, v1 - v);
   }
   float lg = 0.f, presence = 0.f, frequency = 0.f;
   if constexpr (kHistory) {
@@ -109,31 +120,56 @@ __global__ __launch_bounds__(1024) void logits_kernel(LogitsParams p) {
     presence = lg != lg ? lg : setting(p.presence, b);      // (a row's number below zero or NaN: its seen tokens are NaN)
     frequency = setting(p.frequency, b);
     const int n = p.lens != nullptr ? min(max(p.lens[b], 0), p.T) : p.T;
-    const TOKEN* history = (const TOKEN*)p.history + b * p.h_st;
     __syncthreads();
     constexpr int U = 4;      // tokens that a thread asks for at once
     for (int j0 = max(n - p.lookback, 0) + tid; j0 < n; j0 += U * threads) {
-      TOKEN token[U];
+      int at[U];      // in the slice, or negative: another slice's, or no token at all
+      auto read = [&](auto* history) {
+        std::remove_cv_t<std::remove_pointer_t<decltype(history)>> token[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) token[u] = history[min(j0 + u * threads, n - 1)];
+        for (int u = 0; u < U; ++u) token[u] = history[b * p.h_st + min(j0 + u * threads, n - 1)];
+#pragma unroll
+        for (int u = 0; u < U; ++u) at[u] = j0 + u * threads < n && token[u] >= v0 && token[u] < v1 ? (int)token[u] - v0 : -1;
+      };
+      if (p.tokens64) read((const int64_t*)p.history);
+      else read((const int32_t*)p.history);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int j = j0 + u * threads;
-        if (j >= n || token[u] < (TOKEN)v0 || token[u] >= (TOKEN)v1) continue;      // another slice's, or no token at all
+        if (at[u] < 0) continue;
         Word add = 1;
         if constexpr (kDecay) {
           const float weight = fast_exp2((float)(j - n) * p.inv_half_life);
           add = ((uint64_t)1 << kCountShift) + (uint32_t)(weight * (float)(1u << kWeightBits) + 0.5f);
         }
-        __hip_atomic_fetch_add(&seen[(int)token[u] - v0], add, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        __hip_atomic_fetch_add(&seen[at[u]], add, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
       }
     }
-    __syncthreads();
   }
+  // bias and mask are on their way while the workgroup gathers
+  f32x4 bias[BIAS ? ROUNDS : 1];
+  uint32_t allowed[MASK ? ROUNDS : 1];
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r) {
+    const int v = v0 + 4 * (tid + r * threads), left = v1 - v;
+    if constexpr (BIAS) {
+      const float* at = p.bias + b * p.bias_st + v;
+      bias[r] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (left >= 4) {
+        if constexpr (BIAS == 2) bias[r] = __builtin_nontemporal_load((const f32x4_near*)at);
+        else bias[r] = *(const f32x4_near*)at;
+      } else {
+        for (int i = 0; i < left; ++i) bias[r][i] = at[i];
+      }
+    }
+    if constexpr (MASK) allowed[r] = left > 0 ? p.allowed[b * p.allowed_st + (v >> 5)] >> (v & 31) : 0;      // (v is a multiple of 4)
+  }
+  if constexpr (kHistory) __syncthreads();
 #pragma unroll
   for (int r = 0; r < ROUNDS; ++r) {
     const int v = v0 + 4 * (tid + r * threads), left = v1 - v;
     if (left <= 0) break;
+    f32x4 x = widen4<E>(raw[r]);
     if constexpr (kHistory) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -149,29 +185,24 @@ __global__ __launch_bounds__(1024) void logits_kernel(LogitsParams p) {
         // in two factors, each of them a normal number: what leaves fp32's range on either side leaves it by the product, and 0 stays 0, -inf
         // stays -inf (a token that came 400 times at 1.3 has a power of 151)
         float power = fminf(w, p.cap) * lg;
-        power = fminf(fmaxf(x[r][i] > 0.f ? -power : power, -252.f), 254.f);
+        power = fminf(fmaxf(x[i] > 0.f ? -power : power, -252.f), 254.f);
         const float half = rintf(0.5f * power);
-        x[r][i] = x[r][i] * fast_exp2(half) * fast_exp2(power - half);
-        x[r][i] -= fmaf(frequency, count, presence);
+        x[i] = x[i] * fast_exp2(half) * fast_exp2(power - half);
+        x[i] -= fmaf(frequency, count, presence);
       }
     }
-    if (p.bias != nullptr) {
-      const float* at = p.bias + b * p.bias_st + v;
-      if (left >= 4) x[r] += *(const f32x4_near*)at;
-      else for (int i = 0; i < left; ++i) x[r][i] += at[i];
-    }
-    if (p.allowed != nullptr) {
-      const uint32_t bits = p.allowed[b * p.allowed_st + (v >> 5)] >> (v & 31);      // (v is a multiple of 4)
+    if constexpr (BIAS) x += bias[r];
+    if constexpr (MASK) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[r][i] = (bits >> i) & 1 ? x[r][i] : -__builtin_inff();
+      for (int i = 0; i < 4; ++i) x[i] = (allowed[r] >> i) & 1 ? x[i] : -__builtin_inff();
     }
-    store4<E>(y_row, v, left, x[r]);
+    store4<E>(y_row, v, left, x);
   }
 }
 
 // A slice per workgroup: the largest one that leaves the chip enough workgroups, since every slice of a row reads its whole history.  A thread has
 // eight values of it, or fewer where a long history wants more threads.
-template <int E, typename COUNT, typename TOKEN> static void logits_launch(LogitsParams p, int B, int most, hipStream_t s) {
+template <int E, typename COUNT, int BIAS, bool MASK> static void logits_launch(LogitsParams p, int B, int most, hipStream_t s) {
   int slice = most;
   while (slice > 1024 && (int64_t)B * ((p.V + slice - 1) / slice) < 512) slice /= 2;
   p.slice = slice;
@@ -182,16 +213,20 @@ template <int E, typename COUNT, typename TOKEN> static void logits_launch(Logit
   const dim3 grid((unsigned)((p.V + slice - 1) / slice), (unsigned)B);
   const size_t lds = std::is_void<COUNT>::value ? 0 : (size_t)slice * (std::is_same<COUNT, uint64_t>::value ? 8 : 4);
   const int rounds = slice / 4 / threads;
-  if (rounds <= 1) hipLaunchKernelGGL((logits_kernel<E, COUNT, TOKEN, 1>), grid, dim3(threads), lds, s, p);
-  else if (rounds == 2) hipLaunchKernelGGL((logits_kernel<E, COUNT, TOKEN, 2>), grid, dim3(threads), lds, s, p);
-  else hipLaunchKernelGGL((logits_kernel<E, COUNT, TOKEN, 4>), grid, dim3(threads), lds, s, p);
+  if (rounds <= 1) hipLaunchKernelGGL((logits_kernel<E, COUNT, 1, BIAS, MASK>), grid, dim3(threads), lds, s, p);
+  else if (rounds == 2) hipLaunchKernelGGL((logits_kernel<E, COUNT, 2, BIAS, MASK>), grid, dim3(threads), lds, s, p);
+  else hipLaunchKernelGGL((logits_kernel<E, COUNT, 4, BIAS, MASK>), grid, dim3(threads), lds, s, p);
+}
+template <int E, typename COUNT> static void logits_launch(const LogitsParams& p, int B, int most, hipStream_t s) {
+  if (p.bias && p.bias_st != 0) p.allowed ? logits_launch<E, COUNT, 2, true>(p, B, most, s) : logits_launch<E, COUNT, 2, false>(p, B, most, s);
+  else if (p.bias) p.allowed ? logits_launch<E, COUNT, 1, true>(p, B, most, s) : logits_launch<E, COUNT, 1, false>(p, B, most, s);
+  else p.allowed ? logits_launch<E, COUNT, 0, true>(p, B, most, s) : logits_launch<E, COUNT, 0, false>(p, B, most, s);
 }
 // (256 rows of 131072 bf16 logits, 4096 tokens each: slices of 8192 65.0 us, of 16384 57.4; 128 of 151000 fp32: 29.7 and 32.2)
-template <int E> static void logits_launch(const LogitsParams& p, bool tokens64, int B, hipStream_t s) {
-  constexpr int kMost = E == kLogitsF32 ? 8192 : 16384;
-  if (!p.history) logits_launch<E, void, int32_t>(p, B, 8192, s);
-  else if (p.inv_half_life > 0.f) tokens64 ? logits_launch<E, uint64_t, int64_t>(p, B, 8192, s) : logits_launch<E, uint64_t, int32_t>(p, B, 8192, s);
-  else tokens64 ? logits_launch<E, uint32_t, int64_t>(p, B, kMost, s) : logits_launch<E, uint32_t, int32_t>(p, B, kMost, s);
+template <int E> static void logits_launch(const LogitsParams& p, int B, hipStream_t s) {
+  if (!p.history) logits_launch<E, void>(p, B, 8192, s);
+  else if (p.inv_half_life > 0.f) logits_launch<E, uint64_t>(p, B, 8192, s);
+  else logits_launch<E, uint32_t>(p, B, E == kLogitsF32 ? 8192 : 16384, s);
 }
 
 }  // namespace daisy
@@ -219,7 +254,7 @@ extern "C" int daisy_logits_process_fwd(const void* x, int64_t x_stride, void* y
                   "logits_process: tensors must be aligned to their elements");
   LogitsParams p = {};
   p.x = x; p.x_st = x_stride; p.y = y; p.y_st = y_stride;
-  p.history = history; p.h_st = history_stride; p.lens = history_lens; p.T = T; p.lookback = lookback;
+  p.history = history; p.h_st = history_stride; p.lens = history_lens; p.T = T; p.lookback = lookback; p.tokens64 = history_is_int64;
   // (from the caller's 64 bits: rounded to 32 first, a number near one is off by 2^-24 / (r - 1) of its logarithm, and that many times over
   // where nothing caps the power)
   p.repetition = {repetition_rows ? 0.f : (float)log2(repetition), repetition_rows}; p.presence = {presence, presence_rows}; p.frequency = {frequency, frequency_rows};
@@ -227,9 +262,9 @@ extern "C" int daisy_logits_process_fwd(const void* x, int64_t x_stride, void* y
   p.bias = bias; p.bias_st = bias_stride; p.allowed = (const uint32_t*)allowed; p.allowed_st = allowed_stride;
   p.V = V;
   hipStream_t s = (hipStream_t)stream;
-  if (type == kLogitsF32) logits_launch<kLogitsF32>(p, history_is_int64, B, s);
-  else if (type == kLogitsBf16) logits_launch<kLogitsBf16>(p, history_is_int64, B, s);
-  else logits_launch<kLogitsF16>(p, history_is_int64, B, s);
+  if (type == kLogitsF32) logits_launch<kLogitsF32>(p, B, s);
+  else if (type == kLogitsBf16) logits_launch<kLogitsBf16>(p, B, s);
+  else logits_launch<kLogitsF16>(p, B, s);
   DAISY_CHECK_LAUNCH("logits_kernel");
   return DAISY_OK;
 }
