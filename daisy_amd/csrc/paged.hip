@@ -40,6 +40,15 @@ __device__ __forceinline__ void raise_status(int32_t* status, int bit) {
   if (status != nullptr) __hip_atomic_fetch_or(status, bit, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
+// A number below 2^31 over a divisor that the host knows, as a product with a little less than its reciprocal, which is right or one too small.
+struct Divisor { uint32_t by, per; };
+static Divisor divisor(int by) { return Divisor{(uint32_t)by, 0xffffffffu / (uint32_t)by}; }
+struct Quotient { int of, rest; };
+__device__ __forceinline__ Quotient divide(uint32_t n, const Divisor& d) {
+  const uint32_t q = __umulhi(n, d.per), rest = n - q * d.by;
+  return rest >= d.by ? Quotient{(int)q + 1, (int)(rest - d.by)} : Quotient{(int)q, (int)rest};
+}
+
 // ---------------------------------------------------------------------------------------------------------------
 // Append
 // ---------------------------------------------------------------------------------------------------------------
@@ -51,7 +60,7 @@ struct AppendParams {
   const uint16_t* ve; int64_t e_st, e_sh; GateSource gate;
   const float* cos; const float* sin; int table_rows;
   uint16_t* pages[2]; int64_t sp[2], sh[2], ss[2];       // k, v [pages, H, page_size, D]
-  const int32_t* table; int64_t table_st; int seqs, max_pages, num_pages, page_size;
+  const int32_t* table; int64_t table_st; int seqs, max_pages, num_pages; Divisor page_size, rows_per_token;
   const int32_t* positions; const int32_t* rows;
   uint16_t* q_out; int64_t qo_st, qo_sh;
   uint16_t* copy[2]; int64_t c_st[2], c_sh[2];           // k, v [N, H, D] or null
@@ -70,10 +79,10 @@ struct AppendParams {
 template <int D, bool IN16, bool CACHE16>
 __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
   constexpr int LPR = D / 16, HALF = D / 2;
-  const int rows_per_token = p.Hq + 2 * p.H;
   const uint32_t item = blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
   const int c = threadIdx.x % LPR;
-  const int token = (int)(item / (uint32_t)rows_per_token), row = (int)(item - (uint32_t)token * (uint32_t)rows_per_token);
+  const Quotient of = divide(item, p.rows_per_token);
+  const int token = of.of, row = of.rest;
   if (token >= p.N) return;              // (whole groups of lanes: the sums below stay among lanes of one row)
   const int kind = row < p.Hq ? 0 : row < p.Hq + p.H ? 1 : 2, h = row - (kind == 0 ? 0 : kind == 1 ? p.Hq : p.Hq + p.H);
 
@@ -95,7 +104,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
   // A negative position: no token.  Everything else that does not lead to a page of the pool is an error of the caller's that
   // only the device can see: nothing is written to the cache, q and the copies become NaN, the status word says so.
   const bool skipped = pos < 0, past = p.cos != nullptr && pos >= p.table_rows;
-  const int at = (int)((unsigned)max(pos, 0) / (unsigned)p.page_size), slot = pos - at * p.page_size;
+  const Quotient place = divide((uint32_t)max(pos, 0), p.page_size);
+  const int at = place.of, slot = place.rest;
   const bool nowhere = seq < 0 || seq >= p.seqs || at >= p.max_pages;
   const int page = skipped || nowhere ? 0 : p.table[seq * p.table_st + at];
   if (rotated) {
@@ -200,8 +210,7 @@ struct PagedParams {
   const uint16_t* q; uint32_t q_sb, q_sh;
   const uint16_t* k; uint32_t k_sp, k_sh, k_ss;
   const uint16_t* v; uint32_t v_sp, v_sh, v_ss;
-  const int32_t* table; uint32_t table_st; int max_pages, num_pages, blocks_per_page, capacity;
-  uint32_t per_block;             // 2^32 / blocks_per_page, a little less
+  const int32_t* table; uint32_t table_st; int max_pages, num_pages, capacity; Divisor blocks_per_page;
   const int32_t* lens;
   uint16_t* o; uint32_t o_sb, o_sh; int o_f16;
   SplitUnit* split;               // [workgroups]
@@ -364,11 +373,9 @@ __global__ __launch_bounds__(256, paged_groups_per_cu(D)) void paged_attn_kernel
     int id = 0, in = 0;
     auto pages_from = [&](int block) {
       const int blk = min(max(block + lane, blk_lo), blk_hi);      // (blocks outside the range: read, but not used)
-      int at = (int)__umulhi((unsigned)blk, p.per_block);      // the page, or the one ahead of it: blocks are fewer than 2^27
-      in = blk - at * p.blocks_per_page;
-      const bool next = in >= p.blocks_per_page;
-      at += next ? 1 : 0;
-      in -= next ? p.blocks_per_page : 0;
+      const Quotient page = divide((uint32_t)blk, p.blocks_per_page);
+      const int at = page.of;
+      in = page.rest;
       id = row[at];
       const bool out = (unsigned)id >= (unsigned)p.num_pages;
       bad |= out;
@@ -824,7 +831,8 @@ int daisy::paged_append_launch(const void* q, const int64_t* q_strides, const vo
     p.sp[i] = page_strides[i][0]; p.sh[i] = page_strides[i][1]; p.ss[i] = page_strides[i][2];
     if (p.copy[i]) { p.c_st[i] = copy_strides[i][0]; p.c_sh[i] = copy_strides[i][1]; }
   }
-  p.table = page_table; p.table_st = table_stride; p.seqs = n_seq; p.max_pages = max_pages; p.num_pages = num_pages; p.page_size = page_size;
+  p.table = page_table; p.table_st = table_stride; p.seqs = n_seq; p.max_pages = max_pages; p.num_pages = num_pages;
+  p.page_size = divisor(page_size); p.rows_per_token = divisor(Hq + 2 * H);
   p.positions = positions; p.rows = rows;
   p.q_out = (uint16_t*)q_out;
   if (q_out) { p.qo_st = q_out_strides[0]; p.qo_sh = q_out_strides[1]; }
@@ -899,7 +907,7 @@ extern "C" int daisy_paged_attn_fwd(const void* q, const int64_t* q_strides,
   p.v = (const uint16_t*)v_pages; p.v_sp = pieces_of_16(v_pages_strides[0], num_pages); p.v_sh = pieces_of_16(v_pages_strides[1], H);
   p.v_ss = pieces_of_16(v_pages_strides[2], page_size);
   p.table = page_table; p.table_st = B == 1 ? 0 : (uint32_t)table_stride; p.max_pages = max_pages; p.num_pages = num_pages;
-  p.blocks_per_page = page_size / kBlock; p.per_block = 0xffffffffu / (uint32_t)p.blocks_per_page; p.capacity = (int)capacity;
+  p.blocks_per_page = divisor(page_size / kBlock); p.capacity = (int)capacity;
   p.lens = lens;
   p.o = (uint16_t*)o; p.o_f16 = o_is_f16; p.o_sb = pieces_of_16(o_strides[0], B); p.o_sh = pieces_of_16(o_strides[1], Hq);
   p.split = (SplitUnit*)workspace;
