@@ -191,10 +191,10 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
 // a lane holds 4 + 4 keys of one head, and those are, as they are, the B operand of O^T = V^T P^T: rows 4c + r and 16 + 4c + r of a tile for
 // the lanes of group c.  V's rows arrive 16 bytes a lane, and v_perm pairs the keys of neighbouring rows.
 //
-// Bound by reading the cache, 4 H D bytes a position: 2 x 131072 positions, 16 heads of 128, 2.15 GB, 320 us = 6.7 TB/s; 32 sequences of up to 32768, 8 key
-// heads for 64, 123 us = 6.2; 64 of up to 4096 in a window, 69 us = 5.5.  Short work is bound by latencies: a launch that finds nothing to do takes
-// 2.5 us, the second kernel 3.2 more (with parts to join), and a wavefront comes to its first key by three reads (length, page, key).  1 sequence of 8192, 12 heads,
-// 50 MB: 12.1 + 3.2 us; 256 sequences of up to 300, 8 heads of 64: 13.6 + 3.2 us, of which a wavefront lives 7, half of it waiting for memory
+// Bound by reading the cache, 4 H D bytes a position: 2 x 131072 positions, 16 heads of 128, 2.15 GB, 319 us = 6.7 TB/s; 32 sequences of up to 32768, 8 key
+// heads for 64, 122 us = 6.2; 64 of up to 4096 in a window, 68 us = 5.6.  Short work is bound by latencies and by the instructions ahead of the first key: a launch
+// that finds nothing to do takes 2.5 us, the second kernel 3.2 more (with parts to join), and a wavefront comes to its first key by three reads (length, page, key).
+// 1 sequence of 8192, 12 heads, 50 MB: 11.9 + 3.2 us; 256 sequences of up to 300, 8 heads of 64: 12.8 + 3.2 us, of which a wavefront lives 7, half of it waiting for memory
 // and a quarter for its turn to issue.
 
 // What a wavefront's run leaves open: whether it begins inside a unit, whether that goes on beyond it, whether it ends inside another one; the
