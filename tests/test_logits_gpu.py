@@ -2,7 +2,7 @@
 
 Tolerances.  A weight is one exp2 (2^-22 of it) and a rounding to 2^-31; their sum is exact, the power ``min(w, cap) log2 r`` is off by 2^-21 of itself and by
 2^-30 n, the exp2 of it by 2^-22: together 2^-21 (1 + |power|) of ``x s``.  Each of the three sums rounds to 2^-24 of its terms' magnitudes, the store to half a
-step of the value."""
+step of the value, or, below the type's normal numbers, to half of its smallest step: eps / 2 of the smallest normal number (fp16: 2^-25)."""
 import math
 
 import pytest
@@ -22,7 +22,7 @@ def gen(seed):
 
 def exact(x, history=None, lens=None, repetition=1.0, half_life=None, cap=None, presence=0.0, frequency=0.0, lookback=None, bias=None, allowed=None):
     """(y, tolerance) by loops over the tokens of the history, fp64 on the CPU."""
-    E = torch.finfo(x.dtype).eps / 2
+    E, least = torch.finfo(x.dtype).eps / 2, torch.finfo(x.dtype).smallest_normal
     x = x.double().cpu()
     B, V = x.shape
     of = lambda t, b: float(t[b]) if isinstance(t, torch.Tensor) else float(t)      # noqa: E731
@@ -51,7 +51,7 @@ def exact(x, history=None, lens=None, repetition=1.0, half_life=None, cap=None, 
             words = (allowed if allowed.dim() == 1 else allowed[b]).cpu().long()
             bits = (words[:, None] >> torch.arange(32)) & 1
             y[b, bits.flatten()[:V] == 0] = -math.inf
-    return y, tol + E * y.abs().nan_to_num(posinf=0.0, neginf=0.0) + 1e-30
+    return y, tol + E * y.abs().nan_to_num(posinf=0.0, neginf=0.0) + E * float(least) + 1e-30
 
 
 def check(got, x, *args, **kw):
