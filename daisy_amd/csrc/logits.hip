@@ -230,6 +230,16 @@ template <int E> static void logits_launch(const LogitsParams& p, int B, hipStre
   else logits_launch<E, uint32_t>(p, B, E == kLogitsF32 ? 8192 : 16384, s);
 }
 
+// Whether a row of y shares memory with another row of x, or with its own otherwise than by being it.
+static bool logits_overlap(const void* x, int64_t x_st, const void* y, int64_t y_st, int B, int V, int elem) {
+  const int64_t a = (int64_t)reinterpret_cast<uintptr_t>(x), b = (int64_t)reinterpret_cast<uintptr_t>(y), row = (int64_t)V * elem;
+  if (a == b) return B > 1 && x_st != y_st;
+  if (b >= a + (B - 1) * x_st * elem + row || a >= b + (B - 1) * y_st * elem + row) return false;
+  if (B == 1 || x_st != y_st) return true;
+  const int64_t st = x_st * elem, ahead = ((b - a) % st + st) % st;      // (halves of the rows of one buffer, say)
+  return ahead < row || st - ahead < row;
+}
+
 }  // namespace daisy
 
 using namespace daisy;
@@ -253,6 +263,7 @@ extern "C" int daisy_logits_process_fwd(const void* x, int64_t x_stride, void* y
   const int elem = type == kLogitsF32 ? 4 : 2;
   DAISY_CHECK_ARG((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) % elem == 0 && (reinterpret_cast<uintptr_t>(bias) & 3) == 0,
                   "logits_process: tensors must be aligned to their elements");
+  DAISY_CHECK_ARG(!logits_overlap(x, x_stride, y, y_stride, B, V, elem), "logits_process: y must be x or lie apart from it");
   LogitsParams p = {};
   p.x = x; p.x_st = x_stride; p.y = y; p.y_st = y_stride;
   p.history = history; p.h_st = history_stride; p.lens = history_lens; p.T = T; p.lookback = lookback; p.tokens64 = history_is_int64;

@@ -980,7 +980,7 @@ def process_logits(logits: torch.Tensor, history: Optional[torch.Tensor] = None,
     ``bias`` (fp32 ``[V]`` or ``[B, V]``) is added.  ``allowed`` (int32 ``[ceil(V / 32)]`` or ``[B, ceil(V / 32)]``, see ``pack_allowed``): tokens whose bit
     (``v % 32`` of word ``v // 32``) is clear become -inf, whatever they were; a row without a set bit is -inf throughout.
 
-    Returns a new tensor in the dtype of ``logits``, or ``out`` (which may be ``logits`` itself).  The result does not depend on any order of
+    Returns a new tensor in the dtype of ``logits``, or ``out`` (``logits`` itself, or memory of its own).  The result does not depend on any order of
     summation.
     """
     if lookback is not None and lookback < 0:

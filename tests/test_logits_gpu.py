@@ -203,6 +203,11 @@ def test_strides_and_in_place(dtype):
     assert torch.equal(ops.process_logits(x, h, **kw), want)
     one = bias[:1].expand(B, V)
     assert torch.equal(ops.process_logits(x, h, bias=one), ops.process_logits(x, h, bias=bias[0]))
+    half = room[:, 3 + V:]
+    assert torch.equal(ops.process_logits(x, h, out=half, **kw), want) and torch.equal(half, want)      # the other half of each row
+    for out in (room[:, 2:2 + V], room[:, 2 + V:2 + 2 * V]):
+        with pytest.raises(RuntimeError, match="apart"):
+            ops.process_logits(x, h, out=out, **kw)
     before = room.clone()
     got = ops.process_logits(x, h, out=x, **kw)
     assert got is x and torch.equal(x, want)

@@ -57,7 +57,9 @@ def process(x=P, y=P, xs=100, ys=100, kind=0, history=P, T=10, lookback=10, repe
 @pytest.mark.parametrize("kw,rc,text", [
     (dict(x=None), -1, "non-NULL"), (dict(B=0), -1, "B=0"), (dict(B=1 << 17), -1, "65535"), (dict(V=0), -1, "V=0"), (dict(kind=3), -2, "type 3"), (dict(ys=99), -1, "overlap"),
     (dict(T=-1), -1, "T=-1"), (dict(lookback=-1), -1, "lookback=-1"), (dict(half_life=-1.0), -1, "half_life"), (dict(cap=-1.0), -1, "cap"), (dict(repetition=0.0), -1, "repetition"),
-    (dict(repetition=float("nan")), -1, "repetition"), (dict(repetition=float("inf")), -1, "repetition"), (dict(T=1 << 30), -2, "too long"), (dict(T=1 << 20, lookback=1 << 17), -2, "131072"), (dict(x=P + 2), -1, "aligned")])
+    (dict(repetition=float("nan")), -1, "repetition"), (dict(repetition=float("inf")), -1, "repetition"), (dict(T=1 << 30), -2, "too long"), (dict(T=1 << 20, lookback=1 << 17), -2, "131072"), (dict(x=P + 2), -1, "aligned"),
+    (dict(y=P + 4), -1, "apart"), (dict(y=P + 4, B=1), -1, "apart"), (dict(ys=200), -1, "apart"), (dict(y=P + 400), -1, "apart"), (dict(xs=0), -1, "apart"),
+    (dict(x=P + 396, xs=200, ys=200), -1, "apart"), (dict(y=P + 404, xs=200, ys=200), -1, "apart")])
 def test_logits_argument_errors(kw, rc, text):
     assert process(**kw) == rc and text in error(), error()
 
