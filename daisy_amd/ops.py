@@ -828,7 +828,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     ``ve [N, H, D]`` and ``gate`` (one fp32): v becomes ``gate * v + (1 - gate) * ve``.  Fp32 throughout, one rounding.
 
     Returns the prepared queries in the cache's dtype, or ``q_out`` (the cache's dtype or k's); ``None`` without ``q``.  ``k_out``, ``v_out``: ``[N, H, D]`` in k's
-    dtype, receive k and v too (for the attention over a prompt).  A token at a negative position is skipped: the cache and rows of buffers
+    dtype, receive k and v too (for the attention over a prompt); they and ``q_out`` may be k, v and q themselves.  A token at a negative position is skipped: the cache and rows of buffers
     that the caller gave stay as they are, a query row of a tensor made here is zero.  Two tokens of one call must not share a place.
 
     The device reads positions, rows and table when the kernel runs.  One that leads to no page or past the rotary tables writes nothing to
@@ -912,7 +912,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     ``q [B, Hq, D]`` in the cache's dtype (bf16 or fp16), any batch and head strides; ``k_pages``, ``v_pages``, ``page_table`` as for ``paged_append``, row b of
     the table for sequence b; Hq a multiple of the cache's H, ``Hq // H`` query heads to a key head.  ``lens`` int32 ``[B]``: the number of
     positions of each sequence, the new token's among them; the last ``window`` of them are seen (``None``: all).  A sequence of length zero gives
-    zeros.  Returns ``o [B, Hq, D]`` in q's dtype, or ``out``, which may be bf16 with an fp16 cache.
+    zeros.  Returns ``o [B, Hq, D]`` in q's dtype, or ``out``, which may be bf16 with an fp16 cache, and q itself.
 
     Lengths and table are read when the kernels run, and the work is split over the lengths that are found there: nothing but shapes is fixed by a
     recording.  ``workspace``: at least ``paged_attention_workspace_bytes`` on the GPU, whatever it holds, for one call at a time (two that run at

@@ -527,6 +527,28 @@ def test_calls_on_two_streams_at_once():
         assert all(torch.equal(o, want[i]) for o in got[i])
 
 
+@pytest.mark.parametrize("lens", [[1, 40, 0, 7], [3000, 5, 900]])
+def test_results_in_the_place_of_the_inputs(lens):
+    g = gen(19)
+    B, H, G, D = len(lens), 2, 4, 128
+    k, v, table, _ = make_cache(lens, H, 32, D, BF16, g, junk=0.0)
+    cos, sin = tables(D, 4000, g)
+    pos = torch.tensor([n - 1 for n in lens], dtype=torch.int32, device=DEV)
+    seen = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    x = randn(g, B, H * G + 2 * H, D, dtype=BF16)
+    y, kc, vc = x.clone(), k.clone(), v.clone()
+    part = lambda t: (t[:, :H * G], t[:, H * G:H * G + H], t[:, H * G + H:])      # noqa: E731
+    (q, kk, vv), (q2, k2, v2) = part(x), part(y)
+    want = [torch.full_like(t, 0.0) for t in (q, kk, vv)]
+    for t, s in zip(want, (q, kk, vv)):
+        t.copy_(s)                                   # (skipped tokens stay as they are)
+    ops.paged_append(kk, vv, k, v, table, pos, q=q, cos=cos, sin=sin, eps=1e-6, q_out=want[0], k_out=want[1], v_out=want[2])
+    ops.paged_append(k2, v2, kc, vc, table, pos, q=q2, cos=cos, sin=sin, eps=1e-6, q_out=q2, k_out=k2, v_out=v2)
+    assert all(torch.equal(a, b) for a, b in zip(want, (q2, k2, v2))) and torch.equal(k, kc) and torch.equal(v, vc)
+    o = ops.paged_attention(want[0], k, v, table, seen)
+    assert torch.equal(ops.paged_attention(q2, k, v, table, seen, out=q2), o)
+
+
 def test_prefixes_shared_by_sequences():
     """Two sequences whose tables name the same first pages, as a shared prompt has them."""
     g = gen(12)
