@@ -229,6 +229,7 @@ template <bool F16> __device__ __forceinline__ u32x2 pack_out(const PagedParams&
 }
 
 constexpr int kTile = 32;       // positions
+constexpr int64_t kMostPositions = ((int64_t)1 << 31) - 1024;      // of a sequence: the end of a tile behind the last one fits 32 bits, too
 constexpr int kBlock = 16;      // positions: pages are multiples of it, so that half a tile lies in one page
 
 template <int CTRL, int ROWS> __device__ __forceinline__ int dpp_int(int x) {
@@ -779,7 +780,7 @@ using namespace daisy;
   DAISY_CHECK_ARG(num_pages > 0 && max_pages > 0 && table_stride >= 0, what ": num_pages=%d, max_pages=%d must be positive", num_pages,   \
                   max_pages);                                                                                                             \
   DAISY_CHECK_SUPPORTED(page_size > 0 && page_size % 16 == 0, what ": page_size %d not supported (a multiple of 16)", page_size);         \
-  DAISY_CHECK_ARG((int64_t)max_pages * page_size < ((int64_t)1 << 31), what ": a sequence of %lld positions is too long",                  \
+  DAISY_CHECK_ARG((int64_t)max_pages * page_size <= kMostPositions, what ": a sequence of %lld positions is too long",                  \
                   (long long)max_pages * page_size);                                                                                      \
   DAISY_CHECK_ARG(al16(k_pages) && al16(v_pages) && rows_of_16(k_pages_strides, num_pages, H) && rows_of_16(v_pages_strides, num_pages, H) && \
                       page_rows_fit(k_pages_strides) && page_rows_fit(v_pages_strides),                                                   \
@@ -867,7 +868,7 @@ static bool paged_tiles_fit(int B, int Hq, int H, int64_t capacity) {
 }
 static bool paged_shape_ok(int B, int Hq, int H, int D, int max_pages, int page_size) {
   return B > 0 && H > 0 && Hq > 0 && Hq % H == 0 && (D == 64 || D == 128 || D == 256) && max_pages > 0 && page_size > 0 &&
-         (int64_t)max_pages * page_size < ((int64_t)1 << 31) && paged_tiles_fit(B, Hq, H, (int64_t)max_pages * page_size);
+         (int64_t)max_pages * page_size <= kMostPositions && paged_tiles_fit(B, Hq, H, (int64_t)max_pages * page_size);
 }
 
 extern "C" size_t daisy_paged_attn_workspace_bytes(int B, int Hq, int H, int D, int max_pages, int page_size) {

@@ -29,7 +29,7 @@ def append(q=P, k=P, v=P, table=P, stride=4, n_seq=1, max_pages=4, num_pages=8, 
     (dict(q=None), -1, "non-NULL"), (dict(lens=None), -1, "non-NULL"), (dict(k=None), -1, "pages"), (dict(table=None), -1, "page table"), (dict(B=0), -1, "B=0"),
     (dict(Hq=3), -1, "Hq=3"), (dict(H=0), -1, "H=0"), (dict(D=96), -2, "head_dim 96"), (dict(D=512), -2, "head_dim"), (dict(page=8), -2, "page_size 8"),
     (dict(page=24), -2, "page_size"), (dict(page=0), -2, "page_size"), (dict(num_pages=0), -1, "num_pages"), (dict(max_pages=0), -1, "max_pages"),
-    (dict(max_pages=1 << 27, page=16), -1, "too long"), (dict(max_pages=1 << 20, B=1 << 15), -1, "too many"),
+    (dict(max_pages=1 << 27, page=16), -1, "too long"), (dict(max_pages=(1 << 27) - 63, page=16), -1, "too long"), (dict(max_pages=1 << 20, B=1 << 15), -1, "too many"),
     (dict(q=P + 2), -1, "aligned"), (dict(k=P + 8), -1, "aligned"), (dict(ks=(ctypes.c_int64 * 3)(4096, 2048, 129)), -1, "multiples of 8"),
     (dict(ks=(ctypes.c_int64 * 3)(4096, 2048, -128)), -1, "strides"), (dict(ks=(ctypes.c_int64 * 3)(4096, 2048, 1 << 23)), -1, "2^23"),
     (dict(qs=(ctypes.c_int64 * 2)(256, 1 << 35)), -2, "too long"), (dict(os=(ctypes.c_int64 * 2)(1 << 35, 128), B=2), -2, "too long"),
