@@ -124,6 +124,17 @@ def test_work_is_split_over_what_is_there(lens, H, G):
     check_attention(o, q, rows, ops.ATTN_SCALE, "split")
 
 
+@pytest.mark.parametrize("B", [256, 257, 1000, 4096, 4097, 9001])
+def test_many_sequences(B):
+    print(f"paged attention of {B} sequences", flush=True)
+    g = gen(B)
+    lens = [(7 * i) % 40 if i % 11 else 0 for i in range(B)]
+    lens[B // 2] = 3000
+    k, v, table, rows = make_cache(lens, 1, 16, 64, BF16, g)
+    q = randn(g, B, 2, 64, dtype=BF16)
+    check_attention(ops.paged_attention(q, k, v, table, torch.tensor(lens, dtype=torch.int32, device=DEV), scale=0.12), q, rows, 0.12, f"{B} sequences")
+
+
 @pytest.mark.parametrize("fill", [0, 0x01, 0x7f, 0xff])
 def test_what_a_workspace_held_before_means_nothing(fill):
     """One workspace for calls of different shapes, with anything in it."""
