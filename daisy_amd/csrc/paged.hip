@@ -194,7 +194,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
 // Bound by reading the cache, 4 H D bytes a position: 2 x 131072 positions, 16 heads of 128, 2.15 GB, 319 us = 6.7 TB/s; 32 sequences of up to 32768, 8 key
 // heads for 64, 122 us = 6.2; 64 of up to 4096 in a window, 68 us = 5.6.  Short work is bound by latencies and by the instructions ahead of the first key: a launch
 // that finds nothing to do takes 2.5 us, the second kernel 3.2 more (with parts to join), and a wavefront comes to its first key by three reads (length, page, key).
-// 1 sequence of 8192, 12 heads, 50 MB: 11.9 + 3.2 us; 256 sequences of up to 300, 8 heads of 64: 12.8 + 3.2 us, of which a wavefront lives 7, half of it waiting for memory
+// 1 sequence of 8192, 12 heads, 50 MB: 11.9 + 3.2 us; 256 sequences of up to 300, 8 heads of 64: 12.3 + 2.2 us, of which a wavefront lives 7, half of it waiting for memory
 // and a quarter for its turn to issue.
 
 // What a wavefront's run leaves open: whether it begins inside a unit, whether that goes on beyond it, whether it ends inside another one; the
@@ -695,20 +695,51 @@ __device__ __forceinline__ void join_parts(const PagedParams& p, const SplitUnit
 }
 
 // Joins the partial sums of the units that lie in more than one workgroup's run.  The results of a unit are dealt to as many workgroups as there are
-// ends of runs in it: to those of the runs that it goes on beyond.  A launch and two reads one behind the other, 3.2 us, whatever there is to join; one
+// ends of runs in it: to those of the runs that it goes on beyond.  A launch and two reads one behind the other, 3.2 us, whatever there is to join, or one read for units in two parts; one
 // kernel would need a counter that somebody clears ahead of every call.
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
   constexpr int kFew = 8;
   __shared__ float4 sums[4][16];
   __shared__ float2 stats[4];
+  // The two parts of a unit that lies in this workgroup's run and the next one's, as short units do, are asked for ahead of knowing that there is one (256 sequences
+  // of up to 300, 8 heads of 64 15.8 -> 14.5 us in all, 32 of 1024, 8 heads of 128 28.1 -> 27.0).  Few units are long and lie in many (2 of 3000 to 9000, 8 key heads for 64:
+  // asked for, 14.2 -> 14.7).
+  const int last_group = min((int)blockIdx.x + 1, p.groups - 1);
+  float2 st2[2];
+  f32x4 v2[2];
+  const bool ahead = (int64_t)8 * p.B * p.H * p.head_tiles >= p.groups;
+  if (ahead && (int)threadIdx.x < p.heads * (D / 4)) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int64_t s = (int64_t)(i == 0 ? 2 * (int)blockIdx.x + 1 : 2 * last_group) * p.heads + threadIdx.x / (D / 4);
+      st2[i] = p.stat[s];
+      v2[i] = *reinterpret_cast<const f32x4*>(p.part + s * D + threadIdx.x % (D / 4) * 4);
+    }
+  }
   const SplitUnit u = p.split[blockIdx.x];
   // No such unit; or, where another call has the same workspace at the same time, one that is not this call's: its results are lost, nothing else is.
   if (u.first < 0 || u.first > (int)blockIdx.x || u.last <= (int)blockIdx.x || u.last >= p.groups) return;
   if ((unsigned)u.b >= (unsigned)p.B || (unsigned)u.unit >= (unsigned)(p.H * p.head_tiles)) return;
   const int parts = u.last - u.first + 1, helpers = parts - 1, me = (int)blockIdx.x - u.first;
-  const int h = u.unit / p.head_tiles, head0 = (u.unit - h * p.head_tiles) * 16, heads = min(p.G - head0, 16), first_head = h * p.G + head0;
-  if (parts <= kFew) {
+  const int h = p.head_tiles == 1 ? u.unit : (int)((unsigned)u.unit / (unsigned)p.head_tiles), head0 = (u.unit - h * p.head_tiles) * 16;
+  const int heads = min(p.G - head0, 16), first_head = h * p.G + head0;
+  if (parts == 2) {
+    for (int col = threadIdx.x; col < heads * (D / 4); col += 256) {
+      const int head = col / (D / 4), at = col % (D / 4) * 4;
+      if (!ahead || col >= 256) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int64_t s = part_slot(p, u, i, head);
+          st2[i] = p.stat[s];
+          v2[i] = *reinterpret_cast<const f32x4*>(p.part + s * D + at);
+        }
+      }
+      const float top = fmaxf(st2[0].x, st2[1].x), f = fast_exp2(st2[0].x - top), e = fast_exp2(st2[1].x - top);
+      const f32x4 a = (f * v2[0] + e * v2[1]) * (1.f / fmaf(e, st2[1].y, f * st2[0].y));
+      *reinterpret_cast<u32x2*>(row_of_o(p, u.b, first_head + head) + at) = pack_out<F16>(p, a);
+    }
+  } else if (parts <= kFew) {
     // a thread per four channels, every part of which it asks for at once
     for (int col = me + helpers * (int)threadIdx.x; col < heads * (D / 4); col += helpers * 256) {
       const int head = col / (D / 4), at = col % (D / 4) * 4;
