@@ -27,7 +27,7 @@ import torch
 import torch.nn.functional as F
 from torch import Tensor
 
-from .attention import CausalSelfAttention, WindowMask, step_linear, build_window_mask
+from .attention import CausalSelfAttention, WindowMask, _held, build_window_mask, step_linear
 from .functional import norm
 from .kv_cache import KVCache, PagedKVCache
 
@@ -123,9 +123,8 @@ def admit(model, prompts: Sequence[Tensor], cache: PagedKVCache) -> Tuple[Tensor
     _check_paged(layers)
     if any(attn is not None and not attn._fused_prep_ok() for attn in layers):
         raise ValueError("a paged cache needs the fused kernels (bf16 weights, head dim 64 or 128)")
-    rotary = [attn.rotary.cos.shape[0] for attn in layers if attn is not None]
     lengths = [p.numel() for p in prompts]
-    torch._assert(max(lengths) <= min(rotary, default=max(lengths)), f"Rotary buffers too small {min(rotary, default=0)} < {max(lengths)}")
+    _check_positions(layers, max(lengths))
     slots = cache.admit(lengths)
     try:
         return _walk_prompts(model, prompts, lengths, slots, cache), slots
@@ -168,6 +167,15 @@ def _check_paged(layers) -> None:
             raise ValueError(f"a paged cache needs attention layers that take its pages, not {type(attn).__name__}")
 
 
+def _check_positions(layers, n: int) -> None:
+    """Raises where a layer's rotary tables have fewer than ``n`` rows."""
+    for attn in layers:
+        if attn is not None:
+            rotary = _held(attn._modules, attn, "rotary")
+            rows = _held(rotary._buffers, rotary, "cos").shape[0]
+            torch._assert(n <= rows, f"Rotary buffers too small {rows} < {n}")
+
+
 @torch.no_grad()
 def step(model, token_ids: Tensor, cache: Union[KVCache, PagedKVCache]) -> Tensor:
     """``DaisyCore.step`` (daisy_core.py:294-323) for one new token per sequence, ``token_ids [B]``
@@ -178,10 +186,13 @@ def step(model, token_ids: Tensor, cache: Union[KVCache, PagedKVCache]) -> Tenso
     Advances the cache; returns ``logits [B, V]``.
 
     With a ``PagedKVCache``, B is the number of its slots and every sequence is at a position of its own; the logits of free
-    slots mean nothing.  What only the device can see is reported by ``cache.check()``.
+    slots mean nothing.  A sequence at the end of the rotary tables raises and leaves the cache as it was; what only the device
+    can see is reported by ``cache.check()``.
     """
     if isinstance(cache, PagedKVCache):
-        _check_paged(getattr(blk, "attn", None) for blk in model.blocks)
+        layers = [getattr(blk, "attn", None) for blk in model.blocks]
+        _check_paged(layers)
+        _check_positions(layers, cache.longest + 1)
         cache.begin_step()
         logits = _walk_step(model, token_ids, cache, 0)
         cache.advance()
@@ -344,7 +355,8 @@ class GraphedPagedStep:
     """
 
     def __init__(self, model, cache: PagedKVCache):
-        _check_paged(getattr(blk, "attn", None) for blk in model.blocks)
+        self._layers = [getattr(blk, "attn", None) for blk in model.blocks]
+        _check_paged(self._layers)
         self.model, self.cache = model, cache
         self.tokens = torch.zeros(cache.sequences, dtype=torch.long, device=cache.k.device)
         self._graph: Optional[torch.cuda.CUDAGraph] = None
@@ -368,6 +380,7 @@ class GraphedPagedStep:
 
     @torch.no_grad()
     def __call__(self, token_ids: Tensor) -> Tensor:
+        _check_positions(self._layers, self.cache.longest + 1)
         self.cache.begin_step()
         self.tokens.copy_(token_ids.reshape(-1))
         if self._graph is None:

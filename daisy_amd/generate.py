@@ -387,6 +387,9 @@ class Generator:
         assert len(prompts) > 0 and all(p.ndim == 1 and p.numel() > 0 for p in prompts) and max_new_tokens > 0
         B, lengths = len(prompts), [p.numel() for p in prompts]
         longest = max(lengths) + max_new_tokens
+        layers = [getattr(blk, "attn", None) for blk in self.model.blocks]
+        core._check_paged(layers)
+        core._check_positions(layers, longest - 1)      # (the last token is not run through the model)
         cache, size = self._paged_cache, 64
         pages = sum(-(-(n + max_new_tokens) // size) for n in lengths)
         if cache is None or cache.sequences != B or cache.pages < pages or cache.max_len < longest:

@@ -195,6 +195,11 @@ class PagedKVCache:
         """Positions of a sequence, ``None`` for a free slot."""
         return self._length[slot]
 
+    @property
+    def longest(self) -> int:
+        """Positions of the longest sequence, 0 where there is none."""
+        return max((n for n in self._length if n is not None), default=0)
+
     def check(self) -> None:
         """Raises what the kernels reported (a position past the rotary tables, say).  Synchronises."""
         from . import ops
