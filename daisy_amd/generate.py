@@ -419,4 +419,5 @@ class Generator:
             lens += 1
             if produced < max_new_tokens:
                 logits = step(token)
+        cache.check()
         return seen.gather(1, first[:, None] + torch.arange(max_new_tokens, device=self.device))

@@ -201,9 +201,13 @@ class PagedKVCache:
         return max((n for n in self._length if n is not None), default=0)
 
     def check(self) -> None:
-        """Raises what the kernels reported (a position past the rotary tables, say).  Synchronises."""
+        """Raises what the kernels reported since the last time (a page that is none, say).  Synchronises."""
         from . import ops
-        ops.raise_for_status(self.status)
+        try:
+            ops.raise_for_status(self.status)
+        except RuntimeError:
+            self.status.zero_()
+            raise
 
     # -- slots and pages -----------------------------------------------------------------------
     def _take(self, wanted: Dict[int, range], left: Dict[int, List[int]]) -> None:

@@ -1,4 +1,5 @@
-"""Where the steps of a paged cache end: at the rows of the rotary tables, which the host knows, with the cache as it was."""
+"""Where the steps of a paged cache end: at the rows of the rotary tables, which the host knows, with the cache as it was; and what the cache's
+status word says once it has been read."""
 import types
 
 import pytest
@@ -27,6 +28,16 @@ def test_a_step_past_the_rotary_tables_is_refused_on_the_host(recorded):
         step(torch.zeros(3, dtype=torch.long))
     assert torch.equal(cache.page_table, before[0]) and cache.free_pages == before[1] and torch.equal(cache.positions, before[2])
     assert (cache.length(0), cache.length(1)) == (5, 32)
+
+
+def test_a_status_word_that_was_reported_is_clear():
+    cache = cpu_cache()
+    cache.check()
+    cache.status.fill_(1)
+    with pytest.raises(RuntimeError, match="rotary tables"):
+        cache.check()
+    cache.check()
+    assert cache.status.tolist() == [0]
 
 
 @pytest.mark.gpu
@@ -67,3 +78,25 @@ def test_the_generator_refuses_to_run_past_the_rotary_tables(record_steps):
     with pytest.raises(AssertionError, match="Rotary buffers too small 32 < 33"):
         gen.generate_ragged(prompts, 4, record_steps=record_steps)
     assert gen.generate_ragged(prompts[1:], 29, record_steps=record_steps).shape == (1, 29)
+
+
+@pytest.mark.gpu
+def test_the_generator_reads_the_status_word(monkeypatch):
+    """A page that is lost on the device while the ragged loop runs is an error of that call, and of no later one."""
+    from daisy_amd.generate import Generator
+    from test_core_gpu import DEV, _Core
+    model = _Core(window=48).to(DEV).eval()
+    gen = Generator(model, window=48, seed=3, device=DEV, dtype=torch.bfloat16, temperature=0.0)
+    prompts = [torch.arange(2, 2 + n, device=DEV) for n in (30, 4)]
+    want = gen.generate_ragged(prompts, 4)
+    real = core.step
+
+    def step(model, tokens, cache, **kw):
+        cache.page_table[1, 0] = -1
+        return real(model, tokens, cache, **kw)
+
+    with monkeypatch.context() as m:
+        m.setattr(core, "step", step)
+        with pytest.raises(RuntimeError, match="no page of the pool"):
+            gen.generate_ragged(prompts, 4)
+    assert torch.equal(gen.generate_ragged(prompts, 4), want)
