@@ -177,7 +177,7 @@ def _check_positions(layers, n: int) -> None:
 
 
 @torch.no_grad()
-def step(model, token_ids: Tensor, cache: Union[KVCache, PagedKVCache]) -> Tensor:
+def step(model, token_ids: Tensor, cache: Union[KVCache, PagedKVCache], window: Optional[int] = None) -> Tensor:
     """``DaisyCore.step`` (daisy_core.py:294-323) for one new token per sequence, ``token_ids [B]``
     (or a 0-dim tensor when B = 1), at position ``cache.t``.
 
@@ -187,14 +187,16 @@ def step(model, token_ids: Tensor, cache: Union[KVCache, PagedKVCache]) -> Tenso
 
     With a ``PagedKVCache``, B is the number of its slots and every sequence is at a position of its own; the logits of free
     slots mean nothing.  A sequence at the end of the rotary tables raises and leaves the cache as it was; what only the device
-    can see is reported by ``cache.check()``.
+    can see is reported by ``cache.check()``.  ``window`` (paged caches only; a ring has its own size): at most this many positions are
+    seen, the new one among them, where the model's ``attn_window_size`` is wider.
     """
+    _check_window(cache, window)
     if isinstance(cache, PagedKVCache):
         layers = [getattr(blk, "attn", None) for blk in model.blocks]
         _check_paged(layers)
         _check_positions(layers, cache.longest + 1)
         cache.begin_step()
-        logits = _walk_step(model, token_ids, cache, 0)
+        logits = _walk_step(model, token_ids, cache, 0, window=window)
         cache.advance()
         return logits
     logits = _walk_step(model, token_ids, cache, cache.t)
@@ -202,10 +204,17 @@ def step(model, token_ids: Tensor, cache: Union[KVCache, PagedKVCache]) -> Tenso
     return logits
 
 
-def _walk_step(model, token_ids: Tensor, cache: KVCache, pos, status: Optional[Tensor] = None) -> Tensor:
+def _check_window(cache, window: Optional[int]) -> None:
+    if window is not None and not isinstance(cache, PagedKVCache):
+        raise ValueError("a window of a call is for paged caches: a ring's size bounds what its steps see")
+    if window is not None and window <= 0:
+        raise ValueError(f"window must be positive or None, got {window}")
+
+
+def _walk_step(model, token_ids: Tensor, cache: KVCache, pos, status: Optional[Tensor] = None, window: Optional[int] = None) -> Tensor:
     """The layer walk of ``step`` at position ``pos`` (a host int, or a one-element int32 device
     tensor when the walk is being recorded for replay); leaves ``cache.advance()`` to the caller.
-    ``status``: the int32 word in which the attention kernels report a device position they cannot use."""
+    ``status``: the int32 word in which the attention kernels report a device position they cannot use.  ``window``: bounds the model's."""
     token_ids = token_ids.reshape(-1, 1)
     B = token_ids.size(0)
     paged = isinstance(cache, PagedKVCache)
@@ -214,7 +223,8 @@ def _walk_step(model, token_ids: Tensor, cache: KVCache, pos, status: Optional[T
     x = x0 = norm(model.embed(token_ids))
     skip_map, skip_weights = model.skip_map, model.skip_weights
     ve_map = _value_embeddings(model, token_ids)
-    window = getattr(model, "attn_window_size", cache.window if paged else cache.W)
+    own = getattr(model, "attn_window_size", cache.window if paged else cache.W)
+    window = own if window is None else window if own is None else min(window, own)
     in_place = cache.dtype in (torch.bfloat16, torch.float16)
     skip_connections = []
     # (A module's children and a list of modules are looked up by name on every access: four lookups of the attention and an index a
@@ -351,13 +361,14 @@ class GraphedStep:
 class GraphedPagedStep:
     """``step(model, tokens, cache)`` with a ``PagedKVCache`` recorded once as a HIP graph and replayed for every later step, while
     sequences grow, are admitted and released: the recorded launches read the table, positions and lengths from the cache's tensors, whose addresses
-    do not change.  The returned logits are a buffer that the next call overwrites.
+    do not change.  The returned logits are a buffer that the next call overwrites.  ``window``: as in ``step``, fixed with the recording.
     """
 
-    def __init__(self, model, cache: PagedKVCache):
+    def __init__(self, model, cache: PagedKVCache, window: Optional[int] = None):
+        _check_window(cache, window)
         self._layers = [getattr(blk, "attn", None) for blk in model.blocks]
         _check_paged(self._layers)
-        self.model, self.cache = model, cache
+        self.model, self.cache, self.window = model, cache, window
         self.tokens = torch.zeros(cache.sequences, dtype=torch.long, device=cache.k.device)
         self._graph: Optional[torch.cuda.CUDAGraph] = None
         self._logits: Optional[Tensor] = None
@@ -371,11 +382,11 @@ class GraphedPagedStep:
         side = torch.cuda.Stream(device=dev)
         side.wait_stream(torch.cuda.current_stream(dev))
         with torch.cuda.stream(side):
-            _walk_step(self.model, self.tokens, self.cache, 0)
+            _walk_step(self.model, self.tokens, self.cache, 0, window=self.window)
         torch.cuda.current_stream(dev).wait_stream(side)
         self._graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self._graph):
-            self._logits = _walk_step(self.model, self.tokens, self.cache, 0)
+            self._logits = _walk_step(self.model, self.tokens, self.cache, 0, window=self.window)
             self.cache.count_on_device()
 
     @torch.no_grad()

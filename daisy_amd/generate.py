@@ -98,6 +98,13 @@ def penalise_repeats(logits: Tensor, recent: Tensor, strength: Tensor, _one: Opt
 # ----------------------------------------------------------------------------------------------
 # generator
 # ----------------------------------------------------------------------------------------------
+def _ragged_pages(lengths: Sequence[int], new: int, window: int, size: int) -> int:
+    """Pages of ``size`` positions that sequences of these lengths need to grow by ``new``: those of the prompt or, later, those that
+    a step sees of ``window`` positions, which are its last page and as many as ``window - 1`` positions ahead of one take."""
+    pages = lambda n: -(-n // size)      # noqa: E731
+    return sum(min(pages(n + new), max(pages(n), pages(window - 1) + 1)) for n in lengths)
+
+
 class Generator:
     def __init__(self, model, window, seed, device=None, dtype=torch.float16, max_seq_len: int = 65536,
                  temperature=1.0, top_k=None, top_p=None, repetition_penalty=1.0, eos_token_id=None,
@@ -381,7 +388,8 @@ class Generator:
         ``generate``; a row that produces the end-of-sequence token keeps emitting it.
 
         The prompts run packed, without padding, into a bf16 paged cache (``core.admit``), every step runs all sequences at positions of their
-        own (``core.step``; ``record_steps``: recorded once as a HIP graph and replayed).  The model needs what ``generate_batch`` needs.
+        own (``core.step``; ``record_steps``: recorded once as a HIP graph and replayed).  The model needs what ``generate_batch`` needs.  A step
+        sees what it sees there: no more than the generator's window, whose pages go back to the pool.
         """
         from . import core
         assert len(prompts) > 0 and all(p.ndim == 1 and p.numel() > 0 for p in prompts) and max_new_tokens > 0
@@ -390,18 +398,21 @@ class Generator:
         layers = [getattr(blk, "attn", None) for blk in self.model.blocks]
         core._check_paged(layers)
         core._check_positions(layers, longest - 1)      # (the last token is not run through the model)
+        # (a ring of W rows is attended beside the new token where the model's window is wider than the ring)
+        own = getattr(self.model, "attn_window_size", self.cache.W)
+        window = self.cache.W + 1 if own is None else min(own, self.cache.W + 1)
         cache, size = self._paged_cache, 64
-        pages = sum(-(-(n + max_new_tokens) // size) for n in lengths)
-        if cache is None or cache.sequences != B or cache.pages < pages or cache.max_len < longest:
+        pages = _ragged_pages(lengths, max_new_tokens, window, size)
+        if cache is None or cache.sequences != B or cache.pages < pages or cache.max_len < longest or cache.window != window:
+            cache = self._paged_cache = self._paged_step = None      # (given up ahead of the new pool)
             cache = self._paged_cache = PagedKVCache(L=self.cache.L, sequences=B, H=self.cache.H, D=self.cache.D, pages=pages, device=self.device,
-                                                     dtype=torch.bfloat16, page_size=size, max_len=longest)
-            self._paged_step = None
+                                                     dtype=torch.bfloat16, page_size=size, max_len=longest, window=window)
         for slot in range(B):
             if cache.length(slot) is not None:
                 cache.release(slot)
         if record_steps and self._paged_step is None:
-            self._paged_step = core.GraphedPagedStep(self.model, cache)
-        step = self._paged_step if record_steps else lambda tokens: core.step(self.model, tokens, cache)
+            self._paged_step = core.GraphedPagedStep(self.model, cache, window=window)
+        step = self._paged_step if record_steps else lambda tokens: core.step(self.model, tokens, cache, window=window)
         logits, _ = core.admit(self.model, prompts, cache)      # (all slots are free: sequence i is in slot i)
         seen = torch.zeros(B, longest, dtype=torch.long, device=self.device)
         for row, prompt in zip(seen, prompts):
