@@ -812,8 +812,24 @@ static bool al16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 1
 // (the stride of a dim of one says nothing)
 static bool step_of_16(int64_t stride, int n) { return n == 1 || (stride % 8 == 0 && stride >= 0); }
 static bool rows_of_16(const int64_t* strides, int n0, int n1) { return step_of_16(strides[0], n0) && step_of_16(strides[1], n1); }
-// Rows that are written: two of them are not the same.
-static bool apart(const int64_t* strides, int n0, int n1) { return (n0 == 1 || strides[0] > 0) && (n1 == 1 || strides[1] > 0); }
+// Rows of D elements in up to three dims.
+struct Rows { int64_t n[3], st[3]; int D; };
+static Rows rows_of(const int64_t* strides, int n0, int n1, int D) { return Rows{{n0, n1, 1}, {strides[0], strides[1], 0}, D}; }
+static Rows rows_of(const int64_t* strides, int n0, int n1, int n2, int D) { return Rows{{n0, n1, n2}, {strides[0], strides[1], strides[2]}, D}; }
+// Rows that are written: no two of them share an element.  From the shortest stride to the longest, each steps over all that the shorter ones reach (what is no such
+// nest is refused, although its rows might miss each other).
+static bool apart(Rows r) {
+  __int128 reach = r.D;
+  for (;;) {
+    int next = -1;
+    for (int d = 0; d < 3; ++d)
+      if (r.n[d] > 1 && (next < 0 || r.st[d] < r.st[next])) next = d;
+    if (next < 0) return true;
+    if (r.st[next] < reach) return false;
+    reach += (__int128)(r.n[next] - 1) * r.st[next];
+    r.n[next] = 1;
+  }
+}
 static uint32_t pieces_of_16(int64_t stride, int n) { return n == 1 ? 0 : (uint32_t)(stride / 8); }
 static int64_t max_stride(const int64_t* strides, int n0, int n1) {
   const int64_t a = n0 == 1 ? 0 : strides[0], b = n1 == 1 ? 0 : strides[1];
@@ -865,10 +881,10 @@ int daisy::paged_append_launch(const void* q, const int64_t* q_strides, const vo
   DAISY_CHECK_ARG((!q || (rows_of_16(q_strides, N, Hq) && rows_of_16(q_out_strides, N, Hq))) && rows_of_16(k_strides, N, H) && rows_of_16(v_strides, N, H) &&
                       (!ve || rows_of_16(ve_strides, N, H)) && (!k_out || rows_of_16(k_out_strides, N, H)) && (!v_out || rows_of_16(v_out_strides, N, H)),
                   "paged_append: strides must be multiples of 8 elements");
-  DAISY_CHECK_ARG((!q || apart(q_out_strides, N, Hq)) && (!k_out || apart(k_out_strides, N, H)) && (!v_out || apart(v_out_strides, N, H)) &&
-                      apart(k_pages_strides, num_pages, H) && apart(v_pages_strides, num_pages, H) && k_pages_strides[2] > 0 && v_pages_strides[2] > 0,
-                  "paged_append: rows that are written must not overlap");
   DAISY_CHECK_ARG((int64_t)N * ((int64_t)Hq + 2 * (int64_t)H) < (int64_t)1 << 31, "paged_append: too many rows (%d tokens)", N);
+  DAISY_CHECK_ARG((!q || apart(rows_of(q_out_strides, N, Hq, D))) && (!k_out || apart(rows_of(k_out_strides, N, H, D))) && (!v_out || apart(rows_of(v_out_strides, N, H, D))) &&
+                      apart(rows_of(k_pages_strides, num_pages, H, page_size, D)) && apart(rows_of(v_pages_strides, num_pages, H, page_size, D)),
+                  "paged_append: rows that are written must not overlap");
   AppendParams p = {};
   const void* in[3] = {q, k, v};
   const int64_t* in_strides[3] = {q_strides, k_strides, v_strides};
@@ -945,10 +961,10 @@ extern "C" int daisy_paged_attn_fwd(const void* q, const int64_t* q_strides,
   const int64_t capacity = (int64_t)max_pages * page_size;
   DAISY_CHECK_ARG(paged_tiles_fit(B, Hq, H, capacity), "paged_attn: %d sequences of up to %lld positions, %d key heads, are too many", B, (long long)capacity, H);
   DAISY_CHECK_SUPPORTED(!o_is_f16 || cache_is_f16, "paged_attn: an fp16 o needs an fp16 cache");
-  DAISY_CHECK_ARG(apart(o_strides, B, Hq), "paged_attn: rows of o must not overlap");
   constexpr int64_t kWidest = (int64_t)1 << 35;
   DAISY_CHECK_SUPPORTED(max_stride(q_strides, B, Hq) < kWidest && max_stride(o_strides, B, Hq) < kWidest && max_stride(k_pages_strides, num_pages, H) < kWidest &&
                             max_stride(v_pages_strides, num_pages, H) < kWidest && (B == 1 || table_stride < (int64_t)1 << 32), "paged_attn: a stride is too long (2^35 elements, 2^32 of the table)");
+  DAISY_CHECK_ARG(apart(rows_of(o_strides, B, Hq, D)), "paged_attn: rows of o must not overlap");
   const PagedSplit sp = paged_split(B, H, Hq / H, D, capacity);
   const size_t need = daisy_paged_attn_workspace_bytes(B, Hq, H, D, max_pages, page_size);
   if (workspace == nullptr || workspace_bytes < need || !al16(workspace)) {
