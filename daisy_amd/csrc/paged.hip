@@ -830,6 +830,49 @@ static bool apart(Rows r) {
     r.n[next] = 1;
   }
 }
+// Whether rows at a and b are the same ones.
+static bool same_rows(const void* a, const Rows& x, const void* b, const Rows& y) {
+  if (a != b) return false;
+  for (int d = 0; d < 3; ++d)
+    if (x.n[d] != y.n[d] || (x.n[d] > 1 && x.st[d] != y.st[d])) return false;
+  return true;
+}
+// Whether a combination of strides from `d` on, up to less[i] times down and more[i] up each, leads from `off` to less than a row away.  The strides are a nest from the longest on, so
+// that each has two numbers at most that leave something for the shorter ones.
+static bool leads_here(__int128 off, const int64_t* st, const int64_t* less, const int64_t* more, int d, int D) {
+  if (d == 3) return off > -D && off < D;
+  if (st[d] == 0) return leads_here(off, st, less, more, d + 1, D);
+  const __int128 down = off >= 0 ? off / st[d] : -((-off + st[d] - 1) / st[d]);
+  for (__int128 i = down; i <= down + 1; ++i)
+    if (i <= less[d] && i >= -more[d] && leads_here(off - i * st[d], st, less, more, d + 1, D)) return true;
+  return false;
+}
+// Whether rows at a and b, 16-byte aligned, share memory.  Where each lies inside the other's range and their strides differ, they are taken to.
+static bool share(const void* a, const Rows& x, const void* b, const Rows& y) {
+  if (a == nullptr || b == nullptr) return false;
+  const __int128 off = ((__int128)(intptr_t)a - (__int128)(intptr_t)b) / 2;
+  __int128 end_x = off + x.D, end_y = y.D;
+  for (int d = 0; d < 3; ++d) { end_x += (__int128)(x.n[d] - 1) * x.st[d]; end_y += (__int128)(y.n[d] - 1) * y.st[d]; }
+  if (end_x <= 0 || end_y <= off) return false;
+  Rows both = {{1, 1, 1}, {0, 0, 0}, x.D};
+  for (int d = 0; d < 3; ++d) {
+    if (x.n[d] > 1 && y.n[d] > 1 && x.st[d] != y.st[d]) return true;
+    both.n[d] = x.n[d] > y.n[d] ? x.n[d] : y.n[d];
+    both.st[d] = x.n[d] > 1 ? x.st[d] : y.n[d] > 1 ? y.st[d] : 0;
+  }
+  if (!apart(both)) return true;
+  // (a row of x, i strides on from its first, is as far from a row of y, j on: off + (i - j) strides)
+  int64_t st[3], less[3], more[3];
+  bool taken[3] = {false, false, false};
+  for (int k = 0; k < 3; ++k) {
+    int next = -1;
+    for (int d = 0; d < 3; ++d)
+      if (!taken[d] && (next < 0 || both.st[d] > both.st[next])) next = d;
+    taken[next] = true;
+    st[k] = both.st[next]; less[k] = y.n[next] - 1; more[k] = x.n[next] - 1;
+  }
+  return leads_here(off, st, less, more, 0, x.D);
+}
 static uint32_t pieces_of_16(int64_t stride, int n) { return n == 1 ? 0 : (uint32_t)(stride / 8); }
 static int64_t max_stride(const int64_t* strides, int n0, int n1) {
   const int64_t a = n0 == 1 ? 0 : strides[0], b = n1 == 1 ? 0 : strides[1];
@@ -885,6 +928,21 @@ int daisy::paged_append_launch(const void* q, const int64_t* q_strides, const vo
   DAISY_CHECK_ARG((!q || apart(rows_of(q_out_strides, N, Hq, D))) && (!k_out || apart(rows_of(k_out_strides, N, H, D))) && (!v_out || apart(rows_of(v_out_strides, N, H, D))) &&
                       apart(rows_of(k_pages_strides, num_pages, H, page_size, D)) && apart(rows_of(v_pages_strides, num_pages, H, page_size, D)),
                   "paged_append: rows that are written must not overlap");
+  {
+    const Rows pages[2] = {rows_of(k_pages_strides, num_pages, H, page_size, D), rows_of(v_pages_strides, num_pages, H, page_size, D)};
+    const void* in[4] = {q, k, v, ve};
+    const Rows in_rows[4] = {q ? rows_of(q_strides, N, Hq, D) : Rows{}, rows_of(k_strides, N, H, D), rows_of(v_strides, N, H, D), ve ? rows_of(ve_strides, N, H, D) : Rows{}};
+    void* out[3] = {q_out, k_out, v_out};
+    const Rows out_rows[3] = {q ? rows_of(q_out_strides, N, Hq, D) : Rows{}, k_out ? rows_of(k_out_strides, N, H, D) : Rows{}, v_out ? rows_of(v_out_strides, N, H, D) : Rows{}};
+    bool clash = share(k_pages, pages[0], v_pages, pages[1]);
+    for (int i = 0; i < 3; ++i) {
+      if (out[i] == nullptr) continue;
+      for (int j = 0; j < 4; ++j) clash |= !(i == j && same_rows(out[i], out_rows[i], in[j], in_rows[j])) && share(out[i], out_rows[i], in[j], in_rows[j]);
+      for (int j = i + 1; j < 3; ++j) clash |= share(out[i], out_rows[i], out[j], out_rows[j]);
+      for (int j = 0; j < 2; ++j) clash |= share(out[i], out_rows[i], j ? v_pages : k_pages, pages[j]);
+    }
+    DAISY_CHECK_ARG(!clash, "paged_append: q_out, k_out and v_out must be q, k and v or share no memory with them, with ve, with each other or with the pages, nor the pages of k with those of v");
+  }
   AppendParams p = {};
   const void* in[3] = {q, k, v};
   const int64_t* in_strides[3] = {q_strides, k_strides, v_strides};

@@ -828,7 +828,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     ``ve [N, H, D]`` and ``gate`` (one fp32): v becomes ``gate * v + (1 - gate) * ve``.  Fp32 throughout, one rounding.
 
     Returns the prepared queries in the cache's dtype, or ``q_out`` (the cache's dtype or k's); ``None`` without ``q``.  ``k_out``, ``v_out``: ``[N, H, D]`` in k's
-    dtype, receive k and v too (for the attention over a prompt); they and ``q_out`` may be k, v and q themselves.  A token at a negative position is skipped: the cache and rows of buffers
+    dtype, receive k and v too (for the attention over a prompt); they and ``q_out`` may be k, v and q themselves, and share no memory with what else the
+    call reads or writes (rows beside each other in one buffer, with the same strides, are fine).  A token at a negative position is skipped: the cache and rows of buffers
     that the caller gave stay as they are, a query row of a tensor made here is zero.  Two tokens of one call must not share a place.
 
     The device reads positions, rows and table when the kernel runs.  One that leads to no page or past the rotary tables writes nothing to

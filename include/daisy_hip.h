@@ -481,8 +481,9 @@ int daisy_gated_rmsnorm_fwd(const void* x, const void* gate, const void* weight,
  * and v_out (the inputs' type) where those are given.  A token at a negative position is skipped: nothing of it
  * is written, except that its row of q_out becomes zero where zero_skipped is set.
  * q, k, v, ve: bf16 or fp16 (in_is_f16) [N, Hq], [N, H] heads of D with {token, head} strides; q and
- * q_out may be NULL (Hq = 0).  Two tokens of one call at the same place of the cache: either may be the one that
- * stays, or parts of both.
+ * q_out may be NULL (Hq = 0).  q_out, k_out and v_out may be q, k and v; otherwise they share no memory with these,
+ * with ve, with each other or with the pages, nor the pages of k with those of v (rows beside each other in one buffer, with the same
+ * strides, are fine).  Two tokens of one call at the same place of the cache: either may be the one that stays, or parts of both.
  */
 int daisy_paged_append_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
                            const void* v, const int64_t* v_strides, int in_is_f16,
