@@ -1029,6 +1029,12 @@ extern "C" int daisy_paged_attn_fwd(const void* q, const int64_t* q_strides,
     set_error("paged_attn: workspace of %zu bytes, %zu needed on a 16-byte boundary", workspace_bytes, need);
     return DAISY_ERR_WORKSPACE;
   }
+  {
+    const Rows q_rows = rows_of(q_strides, B, Hq, D), o_rows = rows_of(o_strides, B, Hq, D);
+    DAISY_CHECK_ARG((same_rows(o, o_rows, q, q_rows) || !share(o, o_rows, q, q_rows)) && !share(o, o_rows, k_pages, rows_of(k_pages_strides, num_pages, H, page_size, D)) &&
+                        !share(o, o_rows, v_pages, rows_of(v_pages_strides, num_pages, H, page_size, D)),
+                    "paged_attn: o must be q or share no memory with it or with the pages");
+  }
   PagedParams p = {};
   p.q = (const uint16_t*)q; p.q_sb = pieces_of_16(q_strides[0], B); p.q_sh = pieces_of_16(q_strides[1], Hq);
   p.k = (const uint16_t*)k_pages; p.k_sp = pieces_of_16(k_pages_strides[0], num_pages); p.k_sh = pieces_of_16(k_pages_strides[1], H);

@@ -913,7 +913,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     ``q [B, Hq, D]`` in the cache's dtype (bf16 or fp16), any batch and head strides; ``k_pages``, ``v_pages``, ``page_table`` as for ``paged_append``, row b of
     the table for sequence b; Hq a multiple of the cache's H, ``Hq // H`` query heads to a key head.  ``lens`` int32 ``[B]``: the number of
     positions of each sequence, the new token's among them; the last ``window`` of them are seen (``None``: all).  A sequence of length zero gives
-    zeros.  Returns ``o [B, Hq, D]`` in q's dtype, or ``out``, which may be bf16 with an fp16 cache, and q itself.
+    zeros.  Returns ``o [B, Hq, D]`` in q's dtype, or ``out``, which may be bf16 with an fp16 cache, and q itself, but share no
+    memory with q otherwise, or with the pages.
 
     Lengths and table are read when the kernels run, and the work is split over the lengths that are found there: nothing but shapes is fixed by a
     recording.  ``workspace``: at least ``paged_attention_workspace_bytes`` on the GPU, whatever it holds, for one call at a time (two that run at

@@ -501,8 +501,8 @@ int daisy_paged_append_fwd(const void* q, const int64_t* q_strides, const void* 
 /* daisy_paged_attn_fwd: the attention of one new token per sequence, whose key and value are in the cache already:
  *   o[b, h] = sum_t softmax_t(scale <q[b, h], k_t>) v_t,  max(0, lens[b] - window) <= t < lens[b]
  * (window <= 0: all positions), the key head of query head h being h / (Hq / H); a length of zero or less gives
- * zeros.  q: the cache's type, o: bf16, or fp16 (o_is_f16) with an fp16 cache, or q itself; [B, Hq, D] with {batch, head} strides.  The work is split over the lengths
- * as they are when the kernel runs.  workspace: daisy_paged_attn_workspace_bytes(...) bytes, 16-byte aligned,
+ * zeros.  q: the cache's type, o: bf16, or fp16 (o_is_f16) with an fp16 cache; [B, Hq, D] with {batch, head} strides.  o may be q, and shares no memory with it
+ * otherwise, or with the pages.  The work is split over the lengths as they are when the kernel runs.  workspace: daisy_paged_attn_workspace_bytes(...) bytes, 16-byte aligned,
  * of no other call that may run at the same time.
  */
 size_t daisy_paged_attn_workspace_bytes(int B, int Hq, int H, int D, int max_pages, int page_size);

@@ -107,3 +107,22 @@ def test_random_layouts_against_their_elements():
         elif norm(shape) == norm(other) or max(k) < min(out) or max(out) < min(k):
             assert rc == -4, (error(), N, H, a, b, shape, other)
     assert min(seen.values()) > 500, seen
+
+
+def attended(q=(0, 256, 128), o=(4096, 256, 128), k=8192, v=24576, B=3, Hq=2, num_pages=4):
+    """Everything in one buffer, at element offsets."""
+    return attend(q=P + 2 * q[0], qs=strides(*q[1:]), o=P + 2 * o[0], os=strides(*o[1:]), k=P + 2 * k, v=P + 2 * v, B=B, Hq=Hq, num_pages=num_pages, ws=P + 100000)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(o=(8, 256, 128)), dict(o=(128, 256, 128)), dict(o=(256, 256, 128)), dict(o=(0, 128, 384)), dict(q=(4096 + 760, 256, 128)), dict(o=(8192, 256, 128)), dict(o=(8192 + 16384 - 8, 256, 128)),
+    dict(o=(24576 + 16384 - 128, 256, 128)), dict(o=(8192 - 760, 256, 128)), dict(q=(0, 512, 128), o=(128, 512, 128)), dict(q=(0, 512, 128), o=(0, 512, 256))])
+def test_attention_over_what_it_reads(kw):
+    assert attended(**kw) == -1 and MEMORY in error(), error()
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(o=(0, 256, 128)), dict(q=(0, 512, 128), o=(256, 512, 128)), dict(q=(0, 128, 128), o=(0, 128, 128), B=1), dict(o=(8192 - 768, 256, 128)),
+                                dict(q=(0, 8, 128), o=(0, 16, 128), B=1), dict(v=8192)])
+def test_attention_beside_what_it_reads(kw):
+    """One pool for k and v is read only, and fine."""
+    assert attended(**kw) == -4 and "launch failed" in error(), error()

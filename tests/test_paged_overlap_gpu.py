@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from daisy_amd import ops
-from test_paged_gpu import BF16, DEV, gen, randn, tables
+from test_paged_gpu import BF16, DEV, gen, make_cache, randn, tables
 
 pytestmark = pytest.mark.gpu
 
@@ -44,3 +44,22 @@ def test_appends_over_what_others_read_are_refused():
         with pytest.raises(RuntimeError, match="share no memory"):
             ops.paged_append(k, v, kp, pages[1], table, pos, q=q, **kw)
     assert torch.equal(x, before[0]) and torch.equal(pages, before[1])
+
+
+@pytest.mark.parametrize("lens,G", [([40, 0, 7], 1), ([3000, 5, 900], 4)])
+def test_attention_into_the_buffer_of_its_queries(lens, G):
+    """Beside the queries, over them, and refused across them."""
+    g = gen(G)
+    H, D = 2, 128
+    k, v, table, _ = make_cache(lens, H, 32, D, BF16, g)
+    lt = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    room = randn(g, len(lens), 3 * H * G, D, dtype=BF16)
+    q = room[:, :H * G]
+    want = ops.paged_attention(q.clone(), k, v, table, lt)
+    assert torch.equal(ops.paged_attention(q, k, v, table, lt, out=room[:, H * G:2 * H * G]), want)
+    before = room.clone()
+    for out in (room[:, 1:1 + H * G], room.flatten(1)[:, 8:8 + H * G * D].unflatten(1, (H * G, D)), k[0, 0, :H * G].expand(len(lens), H * G, D), k.flatten()[:q.numel()].view(q.shape)):
+        with pytest.raises(RuntimeError, match="share no memory|must not overlap"):
+            ops.paged_attention(q, k, v, table, lt, out=out)
+    assert torch.equal(room, before)
+    assert torch.equal(ops.paged_attention(q, k, v, table, lt, out=q), want)
