@@ -230,14 +230,18 @@ template <int E> static void logits_launch(const LogitsParams& p, int B, hipStre
   else logits_launch<E, uint32_t>(p, B, E == kLogitsF32 ? 8192 : 16384, s);
 }
 
-// Whether a row of y shares memory with another row of x, or with its own otherwise than by being it.
-static bool logits_overlap(const void* x, int64_t x_st, const void* y, int64_t y_st, int B, int V, int elem) {
-  const int64_t a = (int64_t)reinterpret_cast<uintptr_t>(x), b = (int64_t)reinterpret_cast<uintptr_t>(y), row = (int64_t)V * elem;
-  if (a == b) return B > 1 && x_st != y_st;
-  if (b >= a + (B - 1) * x_st * elem + row || a >= b + (B - 1) * y_st * elem + row) return false;
-  if (B == 1 || x_st != y_st) return true;
-  const int64_t st = x_st * elem, ahead = ((b - a) % st + st) % st;      // (halves of the rows of one buffer, say)
-  return ahead < row || st - ahead < row;
+// n rows of `width` bytes, `stride` bytes apart.
+struct ByteRows { const void* p; int64_t n, stride, width; };
+// Whether two such sets share memory.  Where each lies inside the other's range and their strides differ, they are taken to.
+static bool share(const ByteRows& x, const ByteRows& y) {
+  if (x.p == nullptr || y.p == nullptr) return false;
+  const int64_t a = (int64_t)reinterpret_cast<uintptr_t>(x.p), b = (int64_t)reinterpret_cast<uintptr_t>(y.p);
+  if (b >= a + (x.n - 1) * x.stride + x.width || a >= b + (y.n - 1) * y.stride + y.width) return false;
+  if (x.n > 1 && y.n > 1 && x.stride != y.stride) return true;
+  const int64_t stride = x.n > 1 ? x.stride : y.stride;
+  if ((x.n == 1 && y.n == 1) || stride == 0) return true;
+  const int64_t ahead = ((b - a) % stride + stride) % stride;      // (halves of the rows of one buffer, say)
+  return ahead < x.width || ahead + y.width > stride;
 }
 
 }  // namespace daisy
@@ -263,7 +267,13 @@ extern "C" int daisy_logits_process_fwd(const void* x, int64_t x_stride, void* y
   const int elem = type == kLogitsF32 ? 4 : 2;
   DAISY_CHECK_ARG((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) % elem == 0 && (reinterpret_cast<uintptr_t>(bias) & 3) == 0,
                   "logits_process: tensors must be aligned to their elements");
-  DAISY_CHECK_ARG(!logits_overlap(x, x_stride, y, y_stride, B, V, elem), "logits_process: y must be x or lie apart from it");
+  const ByteRows to = {y, B, y_stride * elem, (int64_t)V * elem};
+  DAISY_CHECK_ARG((y == x && (B == 1 || x_stride == y_stride)) || !share({x, B, x_stride * elem, (int64_t)V * elem}, to), "logits_process: y must be x or lie apart from it");
+  const int id = history_is_int64 ? 8 : 4;
+  DAISY_CHECK_ARG(!share({history, B, history_stride * id, (int64_t)T * id}, to) && !share({history ? history_lens : nullptr, 1, 0, (int64_t)B * 4}, to) &&
+                      !share({bias, bias_stride ? B : 1, bias_stride * 4, (int64_t)V * 4}, to) && !share({allowed, allowed_stride ? B : 1, allowed_stride * 4, ((int64_t)V + 31) / 32 * 4}, to) &&
+                      !share({repetition_rows, 1, 0, (int64_t)B * 4}, to) && !share({presence_rows, 1, 0, (int64_t)B * 4}, to) && !share({frequency_rows, 1, 0, (int64_t)B * 4}, to),
+                  "logits_process: y must lie apart from the history, the settings, the bias and the mask");
   LogitsParams p = {};
   p.x = x; p.x_st = x_stride; p.y = y; p.y_st = y_stride;
   p.history = history; p.h_st = history_stride; p.lens = history_lens; p.T = T; p.lookback = lookback; p.tokens64 = history_is_int64;

@@ -523,7 +523,8 @@ int daisy_paged_attn_fwd(const void* q, const int64_t* q_strides,
  *   s = repetition^min(w, cap);  y = (x > 0 ? x / s : x * s) - frequency * n - presence * [n > 0]
  *   y += bias[v];  y = -inf where bit v % 32 of allowed[v / 32] is clear
  * in fp32, rounded once to the type of x.
- * x, y        : [B, V], type 0 = fp32, 1 = bf16, 2 = fp16, row strides; y may be x, and must not overlap it otherwise.
+ * x, y        : [B, V], type 0 = fp32, 1 = bf16, 2 = fp16, row strides; y may be x, and must not overlap it otherwise,
+ *               nor anything else that the call reads.
  * history     : int32 or int64 (history_is_int64) [B, T] with a row stride, or NULL; ids outside 0 .. V - 1 count
  *               for nothing.  At most 131071 tokens of a row are looked at (min(T, lookback)).
  * repetition, presence, frequency: a number, or, where the pointer before it is given, fp32 [B].
