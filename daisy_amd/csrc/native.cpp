@@ -23,6 +23,7 @@
 #include <algorithm>
 #include <array>
 #include <cmath>
+#include <limits>
 
 #include "internal.h"
 
@@ -914,7 +915,9 @@ PyObject* py_process_logits(PyObject*, PyObject* const* a, Py_ssize_t n) {
       number[i] = PyFloat_AsDouble(o);
     }
   }
-  const double half_life = PyFloat_AsDouble(a[4]), cap = PyFloat_AsDouble(a[5]);
+  double half_life = PyFloat_AsDouble(a[4]);
+  const double cap = PyFloat_AsDouble(a[5]);
+  if (half_life > 0.0) half_life = std::max<double>(half_life, std::numeric_limits<float>::min());      // (as fp32 zero would be none; either forgets everything)
   const long asked = PyLong_AsLong(a[8]);
   if (PyErr_Occurred()) { PyErr_Clear(); return none(); }
   const int64_t lookback = asked < 0 ? T : std::min<int64_t>(asked, T);

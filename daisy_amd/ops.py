@@ -977,7 +977,7 @@ def process_logits(logits: torch.Tensor, history: Optional[torch.Tensor] = None,
     ``MAX_HISTORY``), a token that was seen n times, at ages (1 = the newest) that add up to ``w = sum 2 ** (-age / half_life)`` (``None``: w = n),
     has its logit divided by ``repetition ** min(w, cap)`` where positive and multiplied by it otherwise; ``frequency * n`` and, for n > 0, ``presence``
     are subtracted.  ``cap=1`` without a half life is the usual penalty; ``half_life=140, cap=3, lookback=128`` is the generator's
-    (``penalise_repeats``).  Ids outside the vocabulary count for nothing.  ``repetition`` (positive), ``presence``, ``frequency``: a number, or fp32 ``[B]`` on the GPU.
+    (``penalise_repeats``).  Ids outside the vocabulary count for nothing.  ``repetition`` (positive and finite), ``presence``, ``frequency``: a number, or fp32 ``[B]`` on the GPU.
 
     ``bias`` (fp32 ``[V]`` or ``[B, V]``) is added.  ``allowed`` (int32 ``[ceil(V / 32)]`` or ``[B, ceil(V / 32)]``, see ``pack_allowed``): tokens whose bit
     (``v % 32`` of word ``v // 32``) is clear become -inf, whatever they were; a row without a set bit is -inf throughout.
@@ -1048,7 +1048,7 @@ def process_logits(logits: torch.Tensor, history: Optional[torch.Tensor] = None,
         rc = lib.daisy_logits_process_fwd(
             x.data_ptr(), x.stride(0), y.data_ptr(), y.stride(0), _LOGITS_TYPES[logits.dtype], _lib.ptr(history),
             0 if history is None else history.stride(0), 0 if history is None or history.dtype == torch.int32 else 1, _lib.ptr(history_lens),
-            T, lookback, *numbers, 0.0 if half_life is None else float(half_life), float("inf") if cap is None else float(cap),
+            T, lookback, *numbers, 0.0 if half_life is None else max(float(half_life), torch.finfo(torch.float32).tiny), float("inf") if cap is None else float(cap),
             _lib.ptr(bias), strides[0], _lib.ptr(allowed), strides[1], B, V, _lib.current_stream(dev))
     _lib.check(rc, "daisy_logits_process_fwd")
     return out
