@@ -753,7 +753,7 @@ PyObject* py_paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (q_out && !(rows_half(*q_out, 3, dev) && (same_type(*q_out, kp) || same_type(*q_out, k)) && q_out->sizes() == q->sizes())) return none();
   for (const Tensor* t : {k_out, v_out})
     if (t && !(rows_half(*t, 3, dev) && same_type(*t, k) && t->sizes() == k.sizes())) return none();
-  if ((status && !one_of(*status, at::kInt, dev)) || needs_autograd({&k, &v, q, ve, gate, &kp, &vp})) return none();
+  if ((status && !one_of(*status, at::kInt, dev)) || needs_autograd({&k, &v, q, ve, gate, &kp, &vp, q_out, k_out, v_out})) return none();
   Unlocked unlocked;
   Tensor qo;
   if (q) qo = q_out ? *q_out : empty(q->sizes(), kp.scalar_type(), k);
@@ -791,7 +791,7 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t B = q.size(0), Hq = q.size(1), H = kp.size(1), D = kp.size(3);
   if (B < 1 || B > INT32_MAX || Hq < 1 || Hq > INT32_MAX || Hq % H != 0 || q.size(2) != D || table.size(0) < B || !int32_row(lens, B, dev)) return none();
   if (out && !(rows_half(*out, 3, dev) && (same_type(*out, q) || bf16(*out)) && out->sizes() == q.sizes())) return none();
-  if ((status && !one_of(*status, at::kInt, dev)) || (ws && !(on_gpu(*ws, dev) && ws->is_contiguous())) || needs_autograd({&q, &kp, &vp})) return none();
+  if ((status && !one_of(*status, at::kInt, dev)) || (ws && !(on_gpu(*ws, dev) && ws->is_contiguous())) || needs_autograd({&q, &kp, &vp, out})) return none();
   const int max_pages = (int)std::min<int64_t>(table.size(1), INT32_MAX), size = (int)std::min<int64_t>(kp.size(2), INT32_MAX);
   const size_t need = daisy_paged_attn_workspace_bytes((int)B, (int)Hq, (int)H, (int)D, max_pages, size);
   if (need == 0) return none();
@@ -924,7 +924,7 @@ PyObject* py_process_logits(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (T > INT32_MAX || (bias && !(on_gpu(*bias, dev) && f32(*bias) && bias->size(-1) == V && last_dense(*bias) && (bias->dim() == 1 || (bias->dim() == 2 && bias->size(0) == B))))) return none();
   if (allowed && !(on_gpu(*allowed, dev) && allowed->scalar_type() == at::kInt && allowed->size(-1) == (V + 31) / 32 && last_dense(*allowed) &&
                    (allowed->dim() == 1 || (allowed->dim() == 2 && allowed->size(0) == B)))) return none();
-  if (needs_autograd({&x, bias, settings[0], settings[1], settings[2]})) return none();
+  if (needs_autograd({&x, bias, settings[0], settings[1], settings[2], out})) return none();
   Unlocked unlocked;
   Tensor y = out ? *out : empty(x.sizes(), type, x);
   const int rc = daisy_logits_process_fwd(ptr(x), row(x), ptr(y), row(y), type == at::kFloat ? 0 : type == at::kBFloat16 ? 1 : 2, ptr(history), history ? row(*history) : 0,

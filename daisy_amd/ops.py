@@ -841,7 +841,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     if fast is not None:
         return fast if fast is not True else None
     dev = _lib.require_gpu(k, v, k_pages, v_pages, page_table, positions, rows, q, cos, sin, ve, gate, q_out, k_out, v_out, status)
-    _no_autograd("paged_append", k, v, q, ve, gate, k_pages, v_pages)
+    _no_autograd("paged_append", k, v, q, ve, gate, k_pages, v_pages, q_out, k_out, v_out)
     _check_status(status)
     P, H, size, D = _check_pages(k_pages, v_pages, page_table)
     _check_rows("k", k, 3, _HALF_TYPES)
@@ -926,7 +926,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if fast is not None:
         return fast
     dev = _lib.require_gpu(q, k_pages, v_pages, page_table, lens, out, workspace, status)
-    _no_autograd("paged_attention", q, k_pages, v_pages)
+    _no_autograd("paged_attention", q, k_pages, v_pages, out)
     _check_status(status)
     P, H, size, D = _check_pages(k_pages, v_pages, page_table)
     _check_rows("q", q, 3, (k_pages.dtype,))
@@ -993,7 +993,7 @@ def process_logits(logits: torch.Tensor, history: Optional[torch.Tensor] = None,
         return fast
     settings = [t for t in (repetition, presence, frequency) if isinstance(t, torch.Tensor)]
     dev = _lib.require_gpu(logits, history, history_lens, bias, allowed, out, *settings)
-    _no_autograd("process_logits", logits, bias, *settings)
+    _no_autograd("process_logits", logits, bias, out, *settings)
     if logits.dtype not in _LOGITS_TYPES:
         raise TypeError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")
     if logits.dim() not in (1, 2) or logits.stride(-1) != 1 and logits.shape[-1] > 1:
