@@ -195,6 +195,7 @@ def step(model, token_ids: Tensor, cache: Union[KVCache, PagedKVCache], window: 
         layers = [getattr(blk, "attn", None) for blk in model.blocks]
         _check_paged(layers)
         _check_positions(layers, cache.longest + 1)
+        torch._assert(token_ids.numel() == cache.sequences, "token batch does not match the cache")      # (ahead of what a step takes)
         cache.begin_step()
         logits = _walk_step(model, token_ids, cache, 0, window=window)
         cache.advance()
@@ -392,6 +393,7 @@ class GraphedPagedStep:
     @torch.no_grad()
     def __call__(self, token_ids: Tensor) -> Tensor:
         _check_positions(self._layers, self.cache.longest + 1)
+        torch._assert(token_ids.numel() == self.cache.sequences, "token batch does not match the cache")      # (one would be copied to all)
         self.cache.begin_step()
         self.tokens.copy_(token_ids.reshape(-1))
         if self._graph is None:
