@@ -916,6 +916,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     zeros.  Returns ``o [B, Hq, D]`` in q's dtype, or ``out``, which may be bf16 with an fp16 cache, and q itself, but share no
     memory with q otherwise, or with the pages.
 
+    Rows of a page that are not visible may hold anything.  A visible value that is not finite makes its channel not finite for the heads that share it (an infinity may
+    give NaN: a probability's rounding is a term of its own in the sum).
+
     Lengths and table are read when the kernels run, and the work is split over the lengths that are found there: nothing but shapes is fixed by a
     recording.  ``workspace``: at least ``paged_attention_workspace_bytes`` on the GPU, whatever it holds, for one call at a time (two that run at
     once, recorded ones too, need one each); ``None``: a tensor made for the call.  A length beyond the table's room, or a page that is none, gives NaN for the heads of that sequence and raises a bit in ``status``.

@@ -502,7 +502,8 @@ int daisy_paged_append_fwd(const void* q, const int64_t* q_strides, const void* 
  *   o[b, h] = sum_t softmax_t(scale <q[b, h], k_t>) v_t,  max(0, lens[b] - window) <= t < lens[b]
  * (window <= 0: all positions), the key head of query head h being h / (Hq / H); a length of zero or less gives
  * zeros.  q: the cache's type, o: bf16, or fp16 (o_is_f16) with an fp16 cache; [B, Hq, D] with {batch, head} strides.  o may be q, and shares no memory with it
- * otherwise, or with the pages.  The work is split over the lengths as they are when the kernel runs.  workspace: daisy_paged_attn_workspace_bytes(...) bytes, 16-byte aligned,
+ * otherwise, or with the pages.  Rows of a page that are not visible may hold anything; a visible value that is not finite makes its own channel not finite (NaN, it may be,
+ * where the sum is an infinity: a probability's rounding is a term of its own).  The work is split over the lengths as they are when the kernel runs.  workspace: daisy_paged_attn_workspace_bytes(...) bytes, 16-byte aligned,
  * of no other call that may run at the same time.
  */
 size_t daisy_paged_attn_workspace_bytes(int B, int Hq, int H, int D, int max_pages, int page_size);

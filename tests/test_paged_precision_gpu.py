@@ -81,3 +81,21 @@ def test_every_form_of_the_join(dtype, lens, H, G, D):
     space = torch.full((ops.paged_attention_workspace_bytes(len(lens), H * G, H, D, table.shape[1], 32),), 0x7f, dtype=torch.uint8, device=DEV)
     for _ in range(3):
         assert torch.equal(ops.paged_attention(q, k, v, table, lt, scale=0.12, workspace=space), o)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+def test_a_value_that_is_not_finite_spoils_its_own_channel_only(dtype, value):
+    g = gen(21)
+    lens, H, G, D = [300, 2000, 9], 2, 2, 128
+    k, v, table, rows = make_cache(lens, H, 16, D, dtype, g)
+    q = randn(g, 3, H * G, D, dtype=dtype)
+    lt = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    want = ops.paged_attention(q, k, v, table, lt, scale=0.12)
+    for b, t, h, d in ((1, 700, 1, 77), (2, 8, 0, 0)):
+        v[int(table[b, t // 16]), h, t % 16, d] = value
+    got = ops.paged_attention(q, k, v, table, lt, scale=0.12)
+    spoiled = torch.zeros_like(got, dtype=torch.bool)
+    spoiled[1, G:, 77] = True
+    spoiled[2, :G, 0] = True
+    assert not bool(torch.isfinite(got[spoiled]).any()) and torch.equal(got[~spoiled], want[~spoiled])
