@@ -200,11 +200,13 @@ __global__ __launch_bounds__(1024) void logits_kernel(LogitsParams p) {
   }
 }
 
+// (256 rows of 131072 bf16 logits, 4096 tokens each: slices of 8192 65.0 us, of 16384 57.4; 128 of 151000 fp32: 29.7 and 32.2)
+template <int E, typename COUNT> constexpr int largest_slice() { return std::is_same<COUNT, uint32_t>::value && E != kLogitsF32 ? 16384 : 8192; }
 // A slice per workgroup: the largest one that leaves the chip enough workgroups, since every slice of a row reads its whole history.  A thread has
 // eight values of it, four of the smallest slice, which few rows take (1 row of 50304 3.64 -> 3.11 us; of larger slices 64 rows 5.8 -> 6.9), or fewer where a long
 // history wants more threads.
-template <int E, typename COUNT, int BIAS, bool MASK> static void logits_launch(LogitsParams p, int B, int most, hipStream_t s) {
-  int slice = most;
+template <int E, typename COUNT, int BIAS, bool MASK> static void logits_launch(LogitsParams p, int B, hipStream_t s) {
+  int slice = largest_slice<E, COUNT>();
   while (slice > 1024 && (int64_t)B * ((p.V + slice - 1) / slice) < 512) slice /= 2;
   p.slice = slice;
   const int tokens = p.history ? p.lookback : 0;
@@ -213,21 +215,20 @@ template <int E, typename COUNT, int BIAS, bool MASK> static void logits_launch(
   if (threads > 1024) threads = 1024;
   const dim3 grid((unsigned)((p.V + slice - 1) / slice), (unsigned)B);
   const size_t lds = std::is_void<COUNT>::value ? 0 : (size_t)slice * (std::is_same<COUNT, uint64_t>::value ? 8 : 4);
-  const int rounds = slice / 4 / threads;
+  const int rounds = slice / 4 / threads;      // (four of the largest slices only: 1024 threads do the others in two)
   if (rounds <= 1) hipLaunchKernelGGL((logits_kernel<E, COUNT, 1, BIAS, MASK>), grid, dim3(threads), lds, s, p);
   else if (rounds == 2) hipLaunchKernelGGL((logits_kernel<E, COUNT, 2, BIAS, MASK>), grid, dim3(threads), lds, s, p);
-  else hipLaunchKernelGGL((logits_kernel<E, COUNT, 4, BIAS, MASK>), grid, dim3(threads), lds, s, p);
+  else if constexpr (largest_slice<E, COUNT>() == 16384) hipLaunchKernelGGL((logits_kernel<E, COUNT, 4, BIAS, MASK>), grid, dim3(threads), lds, s, p);
 }
-template <int E, typename COUNT> static void logits_launch(const LogitsParams& p, int B, int most, hipStream_t s) {
-  if (p.bias && p.bias_st != 0) p.allowed ? logits_launch<E, COUNT, 2, true>(p, B, most, s) : logits_launch<E, COUNT, 2, false>(p, B, most, s);
-  else if (p.bias) p.allowed ? logits_launch<E, COUNT, 1, true>(p, B, most, s) : logits_launch<E, COUNT, 1, false>(p, B, most, s);
-  else p.allowed ? logits_launch<E, COUNT, 0, true>(p, B, most, s) : logits_launch<E, COUNT, 0, false>(p, B, most, s);
+template <int E, typename COUNT> static void logits_launch(const LogitsParams& p, int B, hipStream_t s) {
+  if (p.bias && p.bias_st != 0) p.allowed ? logits_launch<E, COUNT, 2, true>(p, B, s) : logits_launch<E, COUNT, 2, false>(p, B, s);
+  else if (p.bias) p.allowed ? logits_launch<E, COUNT, 1, true>(p, B, s) : logits_launch<E, COUNT, 1, false>(p, B, s);
+  else p.allowed ? logits_launch<E, COUNT, 0, true>(p, B, s) : logits_launch<E, COUNT, 0, false>(p, B, s);
 }
-// (256 rows of 131072 bf16 logits, 4096 tokens each: slices of 8192 65.0 us, of 16384 57.4; 128 of 151000 fp32: 29.7 and 32.2)
 template <int E> static void logits_launch(const LogitsParams& p, int B, hipStream_t s) {
-  if (!p.history) logits_launch<E, void>(p, B, 8192, s);
-  else if (p.inv_half_life > 0.f) logits_launch<E, uint64_t>(p, B, 8192, s);
-  else logits_launch<E, uint32_t>(p, B, E == kLogitsF32 ? 8192 : 16384, s);
+  if (!p.history) logits_launch<E, void>(p, B, s);
+  else if (p.inv_half_life > 0.f) logits_launch<E, uint64_t>(p, B, s);
+  else logits_launch<E, uint32_t>(p, B, s);
 }
 
 // n rows of `width` bytes, `stride` bytes apart.
