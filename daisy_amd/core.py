@@ -169,11 +169,19 @@ def _check_paged(layers) -> None:
 
 def _check_positions(layers, n: int) -> None:
     """Raises where a layer's rotary tables have fewer than ``n`` rows."""
+    rows = _rotary_rows(layers)
+    if rows is not None and n > rows:
+        torch._assert(False, f"Rotary buffers too small {rows} < {n}")
+
+
+def _rotary_rows(layers) -> Optional[int]:
+    """Rows of the shortest rotary tables, ``None`` without attention."""
+    rows = []
     for attn in layers:
         if attn is not None:
             rotary = _held(attn._modules, attn, "rotary")
-            rows = _held(rotary._buffers, rotary, "cos").shape[0]
-            torch._assert(n <= rows, f"Rotary buffers too small {rows} < {n}")
+            rows.append(_held(rotary._buffers, rotary, "cos").size(0))
+    return min(rows, default=None)
 
 
 @torch.no_grad()
@@ -197,7 +205,7 @@ def step(model, token_ids: Tensor, cache: Union[KVCache, PagedKVCache], window: 
         _check_positions(layers, cache.longest + 1)
         torch._assert(token_ids.numel() == cache.sequences, "token batch does not match the cache")      # (ahead of what a step takes)
         cache.begin_step()
-        logits = _walk_step(model, token_ids, cache, 0, window=window)
+        logits = _walk_step(model, token_ids, cache, 0, window=window, layers=layers)
         cache.advance()
         return logits
     logits = _walk_step(model, token_ids, cache, cache.t)
@@ -212,10 +220,12 @@ def _check_window(cache, window: Optional[int]) -> None:
         raise ValueError(f"window must be positive or None, got {window}")
 
 
-def _walk_step(model, token_ids: Tensor, cache: KVCache, pos, status: Optional[Tensor] = None, window: Optional[int] = None) -> Tensor:
+def _walk_step(model, token_ids: Tensor, cache: KVCache, pos, status: Optional[Tensor] = None, window: Optional[int] = None,
+               layers: Optional[list] = None) -> Tensor:
     """The layer walk of ``step`` at position ``pos`` (a host int, or a one-element int32 device
     tensor when the walk is being recorded for replay); leaves ``cache.advance()`` to the caller.
-    ``status``: the int32 word in which the attention kernels report a device position they cannot use.  ``window``: bounds the model's."""
+    ``status``: the int32 word in which the attention kernels report a device position they cannot use.  ``window``: bounds the model's.  ``layers``: the blocks'
+    attention, where the caller has looked it up."""
     token_ids = token_ids.reshape(-1, 1)
     B = token_ids.size(0)
     paged = isinstance(cache, PagedKVCache)
@@ -234,7 +244,7 @@ def _walk_step(model, token_ids: Tensor, cache: KVCache, pos, status: Optional[T
         if i in skip_map:
             gate = torch.sigmoid(skip_weights[skip_map[i]])
             x = x * gate + (1 - gate) * skip_connections[skip_map[i]]
-        attn = getattr(blk, "attn", None)
+        attn = getattr(blk, "attn", None) if layers is None else layers[i]
         if attn is None or not getattr(attn, "uses_kv_context", True):
             k_ctx = v_ctx = None        # no attention, or one that keeps its own state (KDA layers)
         elif paged:
@@ -362,13 +372,15 @@ class GraphedStep:
 class GraphedPagedStep:
     """``step(model, tokens, cache)`` with a ``PagedKVCache`` recorded once as a HIP graph and replayed for every later step, while
     sequences grow, are admitted and released: the recorded launches read the table, positions and lengths from the cache's tensors, whose addresses
-    do not change.  The returned logits are a buffer that the next call overwrites.  ``window``: as in ``step``, fixed with the recording.
+    do not change.  The returned logits are a buffer that the next call overwrites.  ``window``: as in ``step``, fixed with the recording; so are the rotary
+    tables: positions up to their row count can be replayed.
     """
 
     def __init__(self, model, cache: PagedKVCache, window: Optional[int] = None):
         _check_window(cache, window)
-        self._layers = [getattr(blk, "attn", None) for blk in model.blocks]
-        _check_paged(self._layers)
+        layers = [getattr(blk, "attn", None) for blk in model.blocks]
+        _check_paged(layers)
+        self.max_positions = _rotary_rows(layers)
         self.model, self.cache, self.window = model, cache, window
         self.tokens = torch.zeros(cache.sequences, dtype=torch.long, device=cache.k.device)
         self._graph: Optional[torch.cuda.CUDAGraph] = None
@@ -392,7 +404,9 @@ class GraphedPagedStep:
 
     @torch.no_grad()
     def __call__(self, token_ids: Tensor) -> Tensor:
-        _check_positions(self._layers, self.cache.longest + 1)
+        longest = self.cache.longest
+        if self.max_positions is not None and longest >= self.max_positions:
+            torch._assert(False, f"Rotary buffers too small {self.max_positions} < {longest + 1}")
         torch._assert(token_ids.numel() == self.cache.sequences, "token batch does not match the cache")      # (one would be copied to all)
         self.cache.begin_step()
         self.tokens.copy_(token_ids.reshape(-1))
