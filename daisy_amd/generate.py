@@ -17,7 +17,7 @@ What is arranged differently here:
 Sampling follows the reference's arithmetic (inference/generate.py:13-58): temperature, top-k,
 nucleus filter, Gumbel-max draw, and the distance-decayed repetition penalty over the last 128
 tokens; the random numbers are drawn with the same call, so a seed gives the same tokens.  Beyond it: presence and frequency
-penalties, biases and a mask of the tokens that may follow (a grammar's, say), in one launch with the repetition penalty, and
+penalties, biases and a mask of the tokens that may follow (a grammar's, say; as bits), in one launch with the repetition penalty, and
 prompts of unequal length (``generate_ragged``).
 """
 from __future__ import annotations
@@ -155,7 +155,8 @@ class Generator:
         self._paged_cache: Optional[PagedKVCache] = None
         self._paged_step = None
         # What ops.process_logits adds to the repetition penalty, over the same last tokens: a bias per token ({id: value} or [vocab]), and
-        # allowed_tokens(seen [B, T], lens [B]) -> which tokens may follow, bool [B, vocab] or bits (ops.pack_allowed), or None for all; a row in which none may ends.
+        # allowed_tokens(seen [B, T], lens [B]) -> which tokens may follow, bool [B, vocab] or bits (ops.pack_allowed, which is ten launches of its own a token), or None for
+        # all; a row in which none may ends.  All three penalties count the prompt's tokens, too.
         self.presence_penalty, self.frequency_penalty = float(presence_penalty), float(frequency_penalty)
         self.allowed_tokens = allowed_tokens
         self.logit_bias = self._bias_row(logit_bias)
@@ -388,7 +389,8 @@ class Generator:
         ``generate``; a row that produces the end-of-sequence token keeps emitting it.
 
         The prompts run packed, without padding, into a bf16 paged cache (``core.admit``), every step runs all sequences at positions of their
-        own (``core.step``; ``record_steps``: recorded once as a HIP graph and replayed).  The model needs what ``generate_batch`` needs.  A step
+        own (``core.step``; ``record_steps``: recorded once as a HIP graph and replayed).  The model needs what ``generate_batch`` needs, and
+        attention layers that take pages: a stack with a KDA layer is refused.  A step
         sees what it sees there: no more than the generator's window, whose pages go back to the pool.
         """
         from . import core

@@ -156,7 +156,8 @@ class PagedKVCache:
 
     Storage is a pool of ``pages`` pages, ``k, v [L, pages, H, page_size, D]`` (bf16 or fp16); each of the ``sequences`` slots owns the pages
     that its row of ``page_table`` names, for up to ``max_len`` positions.  A step runs all slots at once; free ones are
-    skipped.  With ``window``, pages that no step can see any more go back to the pool.
+    skipped.  With ``window``, pages that no step can see any more go back to the pool as a sequence crosses into another page; a prompt takes
+    pages for all of its positions, which its own attention sees, so a pool has to hold the longest prompts whole.
 
     The host knows every length, so that ``admit`` and ``begin_step`` raise where the pool is empty; the device has the table, the next token's
     ``positions`` (-1 for a free slot) and the ``lens`` with it, at fixed addresses, for steps recorded in a HIP graph.  Changes go to the
