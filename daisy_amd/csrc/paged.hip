@@ -196,7 +196,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
 // heads for 64, 122 us = 6.2; 64 of up to 4096 in a window, 68 us = 5.6.  Short work is bound by latencies and by the instructions ahead of the first key: a launch
 // that finds nothing to do takes 2.5 us, the second kernel 3.2 more (with parts to join), and a wavefront comes to its first key by three reads (length, page, key).
 // 1 sequence of 8192, 12 heads, 50 MB: 11.9 + 3.2 us; 256 sequences of up to 300, 8 heads of 64: 12.3 + 2.2 us, of which a wavefront lives 7, half of it waiting for memory
-// and a quarter for its turn to issue.
+// and a quarter for its turn to issue; 33 to 44 scalar registers spill to lanes in every instance, no vector registers.
 
 // What a wavefront's run leaves open: whether it begins inside a unit, whether that goes on beyond it, whether it ends inside another one; the
 // query heads of the two, and of the second one its sequence and its first head.
