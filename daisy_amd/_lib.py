@@ -21,6 +21,8 @@ LINEAR_MAX_ROWS = 8
 STATUS_POSITION_PAST_TABLES = 1
 STATUS_LENGTH_PAST_PAGES = 2
 STATUS_PAGE_OUT_OF_RANGE = 4
+STATUS_INDEX_OUT_OF_ORDER = 8
+MAX_TREE_NODES = 256
 DECODE_STATIC_SCRATCH_BYTES = 4 << 20
 
 _I64P = POINTER(c_int64)
@@ -163,6 +165,15 @@ SIGNATURES = {
         c_void_p, c_void_p,                                     # positions, rows
         c_void_p, _I64P, c_int, c_void_p, _I64P, c_void_p, _I64P, c_int,  # q_out (+ strides), is fp16, k_out, v_out (+ strides), zero_skipped
         c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p]),  # N, Hq, H, D, eps, status, stream
+    "daisy_paged_append_slots_fwd": (c_int, [
+        c_void_p, _I64P, c_void_p, _I64P, c_void_p, _I64P, c_int,  # q, k, v (+ strides), inputs are fp16
+        c_void_p, _I64P, c_void_p,                              # ve, ve strides, gate
+        c_void_p, c_void_p, c_int,                              # cos, sin, table_rows
+        c_void_p, _I64P, c_void_p, _I64P, c_int,                # k_pages, v_pages (+ strides), cache is fp16
+        c_void_p, c_int64, c_int, c_int, c_int, c_int,          # page_table (+ row stride), n_seq, max_pages, num_pages, page_size
+        c_void_p, c_void_p, c_void_p,                           # positions, rows, slots
+        c_void_p, _I64P, c_int, c_void_p, _I64P, c_void_p, _I64P, c_int,  # q_out (+ strides), is fp16, k_out, v_out (+ strides), zero_skipped
+        c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p]),  # N, Hq, H, D, eps, status, stream
     "daisy_paged_attn_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
     "daisy_paged_attn_fwd": (c_int, [
         c_void_p, _I64P, c_void_p, _I64P, c_void_p, _I64P, c_int,  # q, k_pages, v_pages (+ strides), cache is fp16
@@ -170,12 +181,36 @@ SIGNATURES = {
         c_void_p, _I64P, c_int,                                 # o (+ strides), is fp16
         c_int, c_int, c_int, c_int, c_int, c_float, c_void_p,   # B, Hq, H, D, window, scale, status
         c_void_p, c_size_t, c_void_p]),                         # workspace, bytes, stream
+    "daisy_draft_tree_fwd": (c_int, [
+        c_void_p, c_int64, c_void_p, c_void_p,                  # parents (+ row stride), lens, nodes
+        c_void_p, c_void_p, c_void_p, c_void_p,                 # mask, positions, slots, rows
+        c_int, c_int, c_void_p]),                               # B, T, stream
+    "daisy_paged_tree_attn_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
+    "daisy_paged_tree_attn_fwd": (c_int, [
+        c_void_p, _I64P, c_void_p, _I64P, c_void_p, _I64P, c_int,  # q, k_pages, v_pages (+ strides), cache is fp16
+        c_void_p, c_int64, c_int, c_int, c_int,                 # page_table (+ row stride), max_pages, num_pages, page_size
+        c_void_p, c_void_p, c_void_p, _I64P,                    # lens, nodes, mask (+ strides)
+        c_void_p, _I64P, c_int,                                 # o (+ strides), is fp16
+        c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p,  # B, T, Hq, H, D, window, scale, status
+        c_void_p, c_size_t, c_void_p]),                         # workspace, bytes, stream
+    "daisy_paged_move_fwd": (c_int, [
+        c_void_p, _I64P, c_void_p, _I64P,                       # k_pages, v_pages (+ strides)
+        c_void_p, c_int64, c_int, c_int, c_int, c_int,          # page_table (+ row stride), n_seq, max_pages, num_pages, page_size
+        c_void_p, c_void_p, c_void_p, c_int64, c_void_p,        # starts, counts, index (+ row stride), sources
+        c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p]),  # B, rows, L, H, D, status, stream
     "daisy_logits_process_fwd": (c_int, [
         c_void_p, c_int64, c_void_p, c_int64, c_int,            # x, y (+ row strides), type
         c_void_p, c_int64, c_int, c_void_p, c_int, c_int,       # history (+ row stride), is int64, history_lens, T, lookback
         c_void_p, c_double, c_void_p, c_float, c_void_p, c_float, c_float, c_float,  # repetition, presence, frequency (rows, number), half_life, cap
         c_void_p, c_int64, c_void_p, c_int64,                   # bias, allowed (+ row strides)
         c_int, c_int, c_void_p]),                               # B, V, stream
+    "daisy_verify_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "daisy_verify_fwd": (c_int, [
+        c_void_p, _I64P, c_int, c_void_p, c_int64, c_int,       # logits (+ strides), type, tokens (+ row stride), are int64
+        c_void_p, c_int64, c_void_p, c_void_p, c_float,         # parents (+ row stride), nodes, temperature (rows, number)
+        c_void_p, c_int64, c_void_p, c_int64, c_void_p, _I64P,  # accept, noise (+ row strides), draft (+ strides)
+        c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,      # path, counts, next, B, T, V
+        c_void_p, c_size_t, c_void_p]),                         # workspace, bytes, stream
 }
 
 

@@ -111,12 +111,12 @@ int prep_launch(const void* q, const int64_t* q_strides, const void* k, const in
                 void* q_out, const int64_t* q_out_strides, void* k_out, const int64_t* k_out_strides,
                 void* v_out, const int64_t* v_out_strides, int B, int T, int H, int D, float eps, void* stream);
 
-// daisy_paged_append_fwd with the gate as the layer holds it.
+// daisy_paged_append_slots_fwd with the gate as the layer holds it.
 int paged_append_launch(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
                         int in_is_f16, const void* ve, const int64_t* ve_strides, GateSource gate, const float* cos, const float* sin, int table_rows,
                         void* k_pages, const int64_t* k_pages_strides, void* v_pages, const int64_t* v_pages_strides, int cache_is_f16,
                         const int32_t* page_table, int64_t table_stride, int n_seq, int max_pages, int num_pages, int page_size,
-                        const int32_t* positions, const int32_t* rows, void* q_out, const int64_t* q_out_strides, int q_out_is_f16,
+                        const int32_t* positions, const int32_t* rows, const int32_t* slots, void* q_out, const int64_t* q_out_strides, int q_out_is_f16,
                         void* k_out, const int64_t* k_out_strides, void* v_out, const int64_t* v_out_strides, int zero_skipped,
                         int N, int Hq, int H, int D, float eps, int32_t* status, void* stream);
 

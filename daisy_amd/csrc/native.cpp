@@ -728,24 +728,24 @@ bool paged_cache(const Tensor& k, const Tensor& v, const Tensor& table, int dev)
 }
 bool int32_row(const Tensor& t, int64_t n, int dev) { return int32_vector(t, n, dev) && t.dim() == 1; }
 
-// paged_append(k, v, k_pages, v_pages, page_table, positions, rows, q, cos, sin, eps (< 0: none), ve, gate, q_out, k_out, v_out, status) -> q_out, or True without q
+// paged_append(k, v, k_pages, v_pages, page_table, positions, rows, q, cos, sin, eps (< 0: none), ve, gate, q_out, k_out, v_out, status, slots) -> q_out, or True without q
 PyObject* py_paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (intercepted() || n != 17) return none();
+  if (intercepted() || n != 18) return none();
   for (int i = 0; i < 6; ++i)
     if (!is_tensor(a[i])) return none();
-  for (int i : {6, 7, 8, 9, 11, 12, 13, 14, 15, 16})
+  for (int i : {6, 7, 8, 9, 11, 12, 13, 14, 15, 16, 17})
     if (!tensor_or_none(a[i])) return none();
   const Tensor &k = THPVariable_Unpack(a[0]), &v = THPVariable_Unpack(a[1]), &kp = THPVariable_Unpack(a[2]), &vp = THPVariable_Unpack(a[3]);
   const Tensor &table = THPVariable_Unpack(a[4]), &pos = THPVariable_Unpack(a[5]);
   const Tensor *rows = opt_tensor(a[6]), *q = opt_tensor(a[7]), *cos = opt_tensor(a[8]), *sin = opt_tensor(a[9]), *ve = opt_tensor(a[11]), *gate = opt_tensor(a[12]);
-  const Tensor *q_out = opt_tensor(a[13]), *k_out = opt_tensor(a[14]), *v_out = opt_tensor(a[15]), *status = opt_tensor(a[16]);
+  const Tensor *q_out = opt_tensor(a[13]), *k_out = opt_tensor(a[14]), *v_out = opt_tensor(a[15]), *status = opt_tensor(a[16]), *slots = opt_tensor(a[17]);
   const float eps = (float)PyFloat_AsDouble(a[10]);
   if (PyErr_Occurred()) { PyErr_Clear(); return none(); }
   const int dev = gpu_of(k);
   if (dev < 0 || !paged_cache(kp, vp, table, dev) || !rows_half(k, 3, dev) || !rows_half(v, 3, dev) || !same_type(k, v) || k.sizes() != v.sizes()) return none();
   const int64_t N = k.size(0), H = kp.size(1), D = kp.size(3);
-  if (N < 1 || N > INT32_MAX || k.size(1) != H || k.size(2) != D || !int32_row(pos, N, dev) || (rows && !int32_row(*rows, N, dev))) return none();
+  if (N < 1 || N > INT32_MAX || k.size(1) != H || k.size(2) != D || !int32_row(pos, N, dev) || (rows && !int32_row(*rows, N, dev)) || (slots && !int32_row(*slots, N, dev))) return none();
   if ((cos == nullptr) != (sin == nullptr) || (ve == nullptr) != (gate == nullptr) || (!q && q_out)) return none();
   if (cos && !(rotary_table(*cos, 1, D / 2, dev) && rotary_table(*sin, 1, D / 2, dev) && cos->size(0) == sin->size(0) && cos->size(0) <= INT32_MAX)) return none();
   if (ve && !(rows_half(*ve, 3, dev) && same_type(*ve, k) && ve->sizes() == k.sizes() && one_of(*gate, at::kFloat, dev))) return none();
@@ -760,10 +760,10 @@ PyObject* py_paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   auto st = [](const Tensor* t) { return t ? Strides2(*t) : Strides2(); };
   const Strides2 qs = st(q), ks(k), vs(v), es = st(ve), qos = qo.defined() ? Strides2(qo) : Strides2(), kos = st(k_out), vos = st(v_out);
   const Strides3 kps(kp), vps(vp);
-  const int rc = daisy_paged_append_fwd(ptr(q), qs.s, ptr(k), ks.s, ptr(v), vs.s, is_f16(k), ptr(ve), es.s, (const float*)ptr(gate), (const float*)ptr(cos),
+  const int rc = daisy_paged_append_slots_fwd(ptr(q), qs.s, ptr(k), ks.s, ptr(v), vs.s, is_f16(k), ptr(ve), es.s, (const float*)ptr(gate), (const float*)ptr(cos),
                                         (const float*)ptr(sin), cos ? (int)cos->size(0) : 0, ptr(kp), kps.s, ptr(vp), vps.s, is_f16(kp),
                                         (const int32_t*)ptr(table), table.stride(0), (int)table.size(0), (int)std::min<int64_t>(table.size(1), INT32_MAX),
-                                        (int)kp.size(0), (int)std::min<int64_t>(kp.size(2), INT32_MAX), (const int32_t*)ptr(pos), (const int32_t*)ptr(rows),
+                                        (int)kp.size(0), (int)std::min<int64_t>(kp.size(2), INT32_MAX), (const int32_t*)ptr(pos), (const int32_t*)ptr(rows), (const int32_t*)ptr(slots),
                                         q ? ptr(qo) : nullptr, qos.s, q ? is_f16(qo) : 0, ptr(k_out), kos.s, ptr(v_out), vos.s, q && !q_out,
                                         (int)N, q ? (int)q->size(1) : 0, (int)H, (int)D, eps, (int32_t*)ptr(status), stream_of(dev));
   if (rc != DAISY_OK) return none();
@@ -858,7 +858,7 @@ PyObject* py_paged_layer_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Tensor q = empty({B, dim}, kp.scalar_type(), x), o = empty({B, 1, dim}, at::kBFloat16, x), ws = empty({(int64_t)need}, at::kByte, x);
   if (daisy::paged_append_launch(base, rs, base + dim, rs, base + 2 * dim, rs, 0, ptr(ve), os, gate, (const float*)ptr(cos), (const float*)ptr(sin), (int)cos.size(0),
                                  ptr(kp), ks.s, ptr(vp), vs.s, is_f16(kp), (const int32_t*)ptr(table), table.stride(0), (int)table.size(0), max_pages, (int)kp.size(0), size,
-                                 (const int32_t*)ptr(pos), nullptr, ptr(q), os, is_f16(q), nullptr, nullptr, nullptr, nullptr, 1, (int)B, (int)H, (int)H, (int)D, eps,
+                                 (const int32_t*)ptr(pos), nullptr, nullptr, ptr(q), os, is_f16(q), nullptr, nullptr, nullptr, nullptr, 1, (int)B, (int)H, (int)H, (int)D, eps,
                                  (int32_t*)ptr(status), s) != DAISY_OK) return none();
   if (daisy_paged_attn_fwd(ptr(q), os, ptr(kp), ks.s, ptr(vp), vs.s, is_f16(kp), (const int32_t*)ptr(table), table.stride(0), max_pages, (int)kp.size(0), size,
                            (const int32_t*)ptr(lens), ptr(o), os, 0, (int)B, (int)H, (int)H, (int)D, (int)std::min<long>(window, INT32_MAX), scale, (int32_t*)ptr(status),

@@ -4,57 +4,20 @@
 // sequence, and row s of the page table names the pages of sequence s in order.  Sequences have lengths of their own, so
 // everything that depends on a length or a position is read from device memory when the kernels run: a launch can be recorded
 // once and replayed while sequences grow, come and go.
-#include "common.h"
+#include "paged.h"
 
 #include <float.h>
 
 #include <type_traits>
-#include <utility>
 
 namespace daisy {
-
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-
-template <bool F16> __device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if constexpr (F16) {
-    const f16x2 h = {(_Float16)a, (_Float16)b};
-    return __builtin_bit_cast(uint32_t, h);
-  } else {
-    return pack_bf16x2(a, b);
-  }
-}
-template <bool F16> __device__ __forceinline__ void unpack8_as(const u32x4& r, float* f) {
-  if constexpr (F16) {
-    const f16x8 h = __builtin_bit_cast(f16x8, r);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = (float)h[i];
-  } else {
-    unpack8(r, f);
-  }
-}
-template <bool F16> __device__ __forceinline__ u32x4 pack8_as(const float* f) {
-  return u32x4{pack2<F16>(f[0], f[1]), pack2<F16>(f[2], f[3]), pack2<F16>(f[4], f[5]), pack2<F16>(f[6], f[7])};
-}
-
-__device__ __forceinline__ void raise_status(int32_t* status, int bit) {
-  if (status != nullptr) __hip_atomic_fetch_or(status, bit, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-
-// A number below 2^31 over a divisor that the host knows, as a product with a little less than its reciprocal, which is right or one too small.
-struct Divisor { uint32_t by, per; };
-static Divisor divisor(int by) { return Divisor{(uint32_t)by, 0xffffffffu / (uint32_t)by}; }
-struct Quotient { int of, rest; };
-__device__ __forceinline__ Quotient divide(uint32_t n, const Divisor& d) {
-  const uint32_t q = __umulhi(n, d.per), rest = n - q * d.by;
-  return rest >= d.by ? Quotient{(int)q + 1, (int)(rest - d.by)} : Quotient{(int)q, (int)rest};
-}
 
 // ---------------------------------------------------------------------------------------------------------------
 // Append
 // ---------------------------------------------------------------------------------------------------------------
 // Per token and head:  x' = x rsqrt(mean(x^2) + eps) for q, k and v where a norm is wanted;
 //   q, k: y1 = x1 cos + x2 sin, y2 = x2 cos - x1 sin on the pairs (i, i + D/2), row `position` of the tables;  v = g v + (1 - g) ve.
+// The row goes to the place of `position` in the pages, or to that of `slot`: the nodes of a drafted tree share positions.
 // All of it in fp32, rounded once as it is stored: pages in the cache's type, copies in the inputs', q in either.
 struct AppendParams {
   const uint16_t* in[3]; int64_t in_st[3], in_sh[3];     // q, k, v [N, heads, D]
@@ -62,7 +25,7 @@ struct AppendParams {
   const float* cos; const float* sin; int table_rows;
   uint16_t* pages[2]; int64_t sp[2], sh[2], ss[2];       // k, v [pages, H, page_size, D]
   const int32_t* table; int64_t table_st; int seqs, max_pages, num_pages; Divisor page_size, rows_per_token;
-  const int32_t* positions; const int32_t* rows;
+  const int32_t* positions; const int32_t* rows; const int32_t* slots;
   uint16_t* q_out; int64_t qo_st, qo_sh;
   uint16_t* copy[2]; int64_t c_st[2], c_sh[2];           // k, v [N, H, D] or null
   int N, Hq, H, zero_skipped, q_f16; float eps;                 // eps < 0: no norm
@@ -92,6 +55,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
   const u32x4 raw0 = *reinterpret_cast<const u32x4*>(src), raw1 = *reinterpret_cast<const u32x4*>(src + HALF);
   const int pos = p.positions[token];
   const int seq = p.rows != nullptr ? p.rows[token] : token;
+  const int spot = p.slots != nullptr ? p.slots[token] : pos;
   // What is combined with the row: the tables' rows, which nothing but the position is waited for, or ve.
   const bool rotated = kind < 2 && p.cos != nullptr, mixed = kind == 2 && p.ve != nullptr;
   f32x4 with[4];
@@ -104,8 +68,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
   }
   // A negative position: no token.  Everything else that does not lead to a page of the pool is an error of the caller's that
   // only the device can see: nothing is written to the cache, q and the copies become NaN, the status word says so.
-  const bool skipped = pos < 0, past = p.cos != nullptr && pos >= p.table_rows;
-  const Quotient place = divide((uint32_t)max(pos, 0), p.page_size);
+  const bool skipped = (pos | spot) < 0, past = p.cos != nullptr && pos >= p.table_rows;
+  const Quotient place = divide((uint32_t)max(spot, 0), p.page_size);
   const int at = place.of, slot = place.rest;
   const bool nowhere = seq < 0 || seq >= p.seqs || at >= p.max_pages;
   const int page = skipped || nowhere ? 0 : p.table[seq * p.table_st + at];
@@ -221,7 +185,6 @@ struct PagedParams {
   int32_t* status;
 };
 
-__device__ __forceinline__ uint64_t product(int i, uint32_t stride) { return (uint64_t)(uint32_t)i * stride; }
 __device__ __forceinline__ uint16_t* row_of_o(const PagedParams& p, int b, int head) { return p.o + 8 * (product(b, p.o_sb) + product(head, p.o_sh)); }
 
 // Four results in the type of o: bf16, or an fp16 cache's.
@@ -229,23 +192,6 @@ template <bool F16> __device__ __forceinline__ u32x2 pack_out(const PagedParams&
   return F16 && p.o_f16 ? u32x2{pack2<F16>(f[0], f[1]), pack2<F16>(f[2], f[3])} : u32x2{pack2<false>(f[0], f[1]), pack2<false>(f[2], f[3])};
 }
 
-constexpr int kTile = 32;       // positions
-constexpr int64_t kMostPositions = ((int64_t)1 << 31) - 1024;      // of a sequence: the end of a tile behind the last one fits 32 bits, too
-constexpr int kBlock = 16;      // positions: pages are multiples of it, so that half a tile lies in one page
-
-template <int CTRL, int ROWS> __device__ __forceinline__ int dpp_int(int x) {
-  return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, true);
-}
-// Sums of the lanes up to each lane.
-__device__ __forceinline__ int wave_scan(int x) {
-  x += dpp_int<0x111, 0xf>(x);      // row_shr 1, 2, 4, 8
-  x += dpp_int<0x112, 0xf>(x);
-  x += dpp_int<0x114, 0xf>(x);
-  x += dpp_int<0x118, 0xf>(x);
-  x += dpp_int<0x142, 0xa>(x);      // row_bcast 15 into rows 1 and 3
-  x += dpp_int<0x143, 0xc>(x);      // row_bcast 31 into rows 2 and 3
-  return x;
-}
 // The positions that a sequence's new token sees, [lo, hi), and the tiles they lie in.
 struct Extent { int lo, hi, first, tiles; bool past; };
 __device__ __forceinline__ Extent extent(const PagedParams& p, int len) {
@@ -263,16 +209,6 @@ __device__ __forceinline__ int len_of(const PagedParams& p, int b) {
   return b < p.B ? len : 0;
 }
 
-constexpr int kCus = 256;
-__device__ __forceinline__ int wave_min(int x) {
-  x = min(x, __builtin_amdgcn_update_dpp(x, x, 0x111, 0xf, 0xf, false));      // row_shr 1, 2, 4, 8: lanes without a neighbour keep their own
-  x = min(x, __builtin_amdgcn_update_dpp(x, x, 0x112, 0xf, 0xf, false));
-  x = min(x, __builtin_amdgcn_update_dpp(x, x, 0x114, 0xf, 0xf, false));
-  x = min(x, __builtin_amdgcn_update_dpp(x, x, 0x118, 0xf, 0xf, false));
-  x = min(x, __builtin_amdgcn_update_dpp(x, x, 0x142, 0xa, 0xf, false));      // row_bcast 15, 31
-  x = min(x, __builtin_amdgcn_update_dpp(x, x, 0x143, 0xc, 0xf, false));
-  return __builtin_amdgcn_readlane(x, 63);
-}
 // How many tiles a wavefront takes: no fewer than the workgroups there are can do, and more (a lane tries each number up to twice as many) where that
 // takes a thirty-second or more off the most loaded of the compute units.  32 sequences of 1024, 8 heads: 683 workgroups of 4 x 3 tiles, three of them
 // on most compute units, 31.1 us; 512 of 4 x 4, two on each, 28.6.  With next to nothing to gain, more wavefronts are the better ones:
@@ -284,11 +220,6 @@ __device__ __forceinline__ int share_of(const PagedParams& p, int total, int lan
   const float groups = ceilf((float)total * __builtin_amdgcn_rcpf((float)(4 * share)) - 0.001f);
   const int load = (int)ceilf(groups * (1.f / kCus)) * share;
   return least + (wave_min((more == 0 ? load - load / 32 : load) * 64 + more) & 63);
-}
-
-template <bool F16> __device__ __forceinline__ f32x4 mfma(const u32x4& a, const u32x4& b, const f32x4& c) {
-  if constexpr (F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-  else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
 // Workgroups per compute unit, a wavefront of each per SIMD: what the registers of a head width leave room for.  (Heads of 256: one, whose tiles of 32 KB
@@ -809,103 +740,9 @@ template <int D> static void append_launch(const AppendParams& p, bool in16, boo
   else cache16 ? append_launch<D, false, true>(p, s) : append_launch<D, false, false>(p, s);
 }
 
-static bool al16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0; }
-// (the stride of a dim of one says nothing)
-static bool step_of_16(int64_t stride, int n) { return n == 1 || (stride % 8 == 0 && stride >= 0); }
-static bool rows_of_16(const int64_t* strides, int n0, int n1) { return step_of_16(strides[0], n0) && step_of_16(strides[1], n1); }
-// Rows of D elements in up to three dims, and the elements from the first to the end of the last (no more than 2^60, which nothing that was allocated reaches).
-struct Rows { int64_t n[3], st[3], reach; int D; };
-static int64_t stepped(int64_t reach, int64_t n, int64_t stride) {
-  constexpr int64_t kFar = (int64_t)1 << 60;
-  const __int128 r = (__int128)(n - 1) * stride + reach;
-  return r < kFar ? (int64_t)r : kFar;
-}
-static Rows rows_of(const int64_t* strides, int n0, int n1, int n2, int D) {
-  Rows r = {{n0, n1, n2}, {n0 > 1 ? strides[0] : 0, n1 > 1 ? strides[1] : 0, n2 > 1 ? strides[2] : 0}, D, D};
-  for (int d = 0; d < 3; ++d) r.reach = stepped(r.reach, r.n[d], r.st[d]);
-  return r;
-}
-static Rows rows_of(const int64_t* strides, int n0, int n1, int D) {
-  const int64_t st[3] = {strides[0], strides[1], 0};
-  return rows_of(st, n0, n1, 1, D);
-}
-// Rows that are written: no two of them share an element.  From the shortest stride to the longest, each steps over all that the shorter ones reach (what is no such
-// nest is refused, although its rows might miss each other).
-static bool apart(const Rows& rows) {
-  int64_t reach = rows.D;
-  bool taken[3] = {rows.n[0] == 1, rows.n[1] == 1, rows.n[2] == 1};
-  for (;;) {
-    int next = -1;
-    for (int d = 0; d < 3; ++d)
-      if (!taken[d] && (next < 0 || rows.st[d] < rows.st[next])) next = d;
-    if (next < 0) return true;
-    if (rows.st[next] < reach) return false;
-    reach = stepped(reach, rows.n[next], rows.st[next]);
-    taken[next] = true;
-  }
-}
-// Whether rows at a and b are the same ones.
-static bool same_rows(const void* a, const Rows& x, const void* b, const Rows& y) {
-  if (a != b) return false;
-  for (int d = 0; d < 3; ++d)
-    if (x.n[d] != y.n[d] || x.st[d] != y.st[d]) return false;
-  return true;
-}
-// Whether a combination of strides from `d` on, up to less[i] times down and more[i] up each, leads from `off` to less than a row away.  The strides are a nest from the longest on, so
-// that each has two numbers at most that leave something for the shorter ones.
-static bool leads_here(int64_t off, const int64_t* st, const int64_t* less, const int64_t* more, int d, int D) {
-  if (d == 3) return off > -D && off < D;
-  if (st[d] == 0) return leads_here(off, st, less, more, d + 1, D);
-  const int64_t down = off >= 0 ? off / st[d] : -((-off + st[d] - 1) / st[d]);
-  for (int64_t i = down; i <= down + 1; ++i)
-    if (i <= less[d] && i >= -more[d] && leads_here(off - i * st[d], st, less, more, d + 1, D)) return true;
-  return false;
-}
-// Whether rows at a and b, 16-byte aligned, share memory.  Where each lies inside the other's range and their strides differ, they are taken to.
-static bool share(const void* a, const Rows& x, const void* b, const Rows& y) {
-  if (a == nullptr || b == nullptr) return false;
-  const int64_t off = ((intptr_t)a - (intptr_t)b) / 2;
-  if (off + x.reach <= 0 || y.reach <= off) return false;
-  Rows both = {{1, 1, 1}, {0, 0, 0}, 0, x.D};
-  for (int d = 0; d < 3; ++d) {
-    if (x.n[d] > 1 && y.n[d] > 1 && x.st[d] != y.st[d]) return true;
-    both.n[d] = x.n[d] > y.n[d] ? x.n[d] : y.n[d];
-    both.st[d] = x.n[d] > 1 ? x.st[d] : y.st[d];
-  }
-  if (!apart(both)) return true;
-  // (a row of x, i strides on from its first, is as far from a row of y, j on: off + (i - j) strides)
-  int order[3] = {0, 1, 2};
-  for (int k : {0, 1, 0})
-    if (both.st[order[k]] < both.st[order[k + 1]]) std::swap(order[k], order[k + 1]);
-  int64_t st[3], less[3], more[3];
-  for (int k = 0; k < 3; ++k) { st[k] = both.st[order[k]]; less[k] = y.n[order[k]] - 1; more[k] = x.n[order[k]] - 1; }
-  return leads_here(off, st, less, more, 0, x.D);
-}
-static uint32_t pieces_of_16(int64_t stride, int n) { return n == 1 ? 0 : (uint32_t)(stride / 8); }
-static int64_t max_stride(const int64_t* strides, int n0, int n1) {
-  const int64_t a = n0 == 1 ? 0 : strides[0], b = n1 == 1 ? 0 : strides[1];
-  return a > b ? a : b;
-}
-// A page's rows are reached with 24-bit products.
-static bool page_rows_fit(const int64_t* strides) { return step_of_16(strides[2], 16) && strides[2] < ((int64_t)1 << 23); }
-
 }  // namespace daisy
 
 using namespace daisy;
-
-#define DAISY_CHECK_HEAD_DIM(what, D) \
-  DAISY_CHECK_SUPPORTED((D) == 64 || (D) == 128 || (D) == 256, what ": head_dim %d not supported (64, 128 or 256)", (D))
-#define DAISY_CHECK_PAGES(what)                                                                                                           \
-  DAISY_CHECK_ARG(k_pages && v_pages && k_pages_strides && v_pages_strides, what ": the pages and their strides must be non-NULL");       \
-  DAISY_CHECK_ARG(page_table, what ": the page table must be non-NULL");                                                                  \
-  DAISY_CHECK_ARG(num_pages > 0 && max_pages > 0 && table_stride >= 0, what ": num_pages=%d, max_pages=%d must be positive", num_pages,   \
-                  max_pages);                                                                                                             \
-  DAISY_CHECK_SUPPORTED(page_size > 0 && page_size % 16 == 0, what ": page_size %d not supported (a multiple of 16)", page_size);         \
-  DAISY_CHECK_ARG((int64_t)max_pages * page_size <= kMostPositions, what ": a sequence of %lld positions is too long",                  \
-                  (long long)max_pages * page_size);                                                                                      \
-  DAISY_CHECK_ARG(al16(k_pages) && al16(v_pages) && rows_of_16(k_pages_strides, num_pages, H) && rows_of_16(v_pages_strides, num_pages, H) && \
-                      page_rows_fit(k_pages_strides) && page_rows_fit(v_pages_strides),                                                   \
-                  what ": pages must be 16-byte aligned, their strides multiples of 8 elements, a row's less than 2^23")
 
 int daisy::paged_append_launch(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
                                       const void* v, const int64_t* v_strides, int in_is_f16,
@@ -913,7 +750,7 @@ int daisy::paged_append_launch(const void* q, const int64_t* q_strides, const vo
                                       const float* cos, const float* sin, int table_rows,
                                       void* k_pages, const int64_t* k_pages_strides, void* v_pages, const int64_t* v_pages_strides,
                                       int cache_is_f16, const int32_t* page_table, int64_t table_stride, int n_seq, int max_pages,
-                                      int num_pages, int page_size, const int32_t* positions, const int32_t* rows,
+                                      int num_pages, int page_size, const int32_t* positions, const int32_t* rows, const int32_t* slots,
                                       void* q_out, const int64_t* q_out_strides, int q_out_is_f16,
                                       void* k_out, const int64_t* k_out_strides, void* v_out, const int64_t* v_out_strides, int zero_skipped,
                                       int N, int Hq, int H, int D, float eps, int32_t* status, void* stream) {
@@ -970,7 +807,7 @@ int daisy::paged_append_launch(const void* q, const int64_t* q_strides, const vo
   }
   p.table = page_table; p.table_st = table_stride; p.seqs = n_seq; p.max_pages = max_pages; p.num_pages = num_pages;
   p.page_size = divisor(page_size); p.rows_per_token = divisor(Hq + 2 * H);
-  p.positions = positions; p.rows = rows;
+  p.positions = positions; p.rows = rows; p.slots = slots;
   p.q_out = (uint16_t*)q_out;
   if (q_out) { p.qo_st = q_out_strides[0]; p.qo_sh = q_out_strides[1]; }
   p.N = N; p.Hq = Hq; p.H = H; p.zero_skipped = zero_skipped; p.q_f16 = q_out_is_f16; p.eps = eps; p.status = status;
@@ -994,7 +831,23 @@ extern "C" int daisy_paged_append_fwd(const void* q, const int64_t* q_strides, c
                                       int N, int Hq, int H, int D, float eps, int32_t* status, void* stream) {
   return paged_append_launch(q, q_strides, k, k_strides, v, v_strides, in_is_f16, ve, ve_strides, GateSource{gate, GateSource::kValue}, cos, sin, table_rows,
                              k_pages, k_pages_strides, v_pages, v_pages_strides, cache_is_f16, page_table, table_stride, n_seq, max_pages, num_pages,
-                             page_size, positions, rows, q_out, q_out_strides, q_out_is_f16, k_out, k_out_strides, v_out, v_out_strides, zero_skipped,
+                             page_size, positions, rows, nullptr, q_out, q_out_strides, q_out_is_f16, k_out, k_out_strides, v_out, v_out_strides, zero_skipped,
+                             N, Hq, H, D, eps, status, stream);
+}
+
+extern "C" int daisy_paged_append_slots_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                                            const void* v, const int64_t* v_strides, int in_is_f16,
+                                            const void* ve, const int64_t* ve_strides, const float* gate,
+                                            const float* cos, const float* sin, int table_rows,
+                                            void* k_pages, const int64_t* k_pages_strides, void* v_pages, const int64_t* v_pages_strides,
+                                            int cache_is_f16, const int32_t* page_table, int64_t table_stride, int n_seq, int max_pages,
+                                            int num_pages, int page_size, const int32_t* positions, const int32_t* rows, const int32_t* slots,
+                                            void* q_out, const int64_t* q_out_strides, int q_out_is_f16,
+                                            void* k_out, const int64_t* k_out_strides, void* v_out, const int64_t* v_out_strides, int zero_skipped,
+                                            int N, int Hq, int H, int D, float eps, int32_t* status, void* stream) {
+  return paged_append_launch(q, q_strides, k, k_strides, v, v_strides, in_is_f16, ve, ve_strides, GateSource{gate, GateSource::kValue}, cos, sin, table_rows,
+                             k_pages, k_pages_strides, v_pages, v_pages_strides, cache_is_f16, page_table, table_stride, n_seq, max_pages, num_pages,
+                             page_size, positions, rows, slots, q_out, q_out_strides, q_out_is_f16, k_out, k_out_strides, v_out, v_out_strides, zero_skipped,
                              N, Hq, H, D, eps, status, stream);
 }
 

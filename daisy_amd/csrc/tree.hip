@@ -1,0 +1,836 @@
+// Trees of drafted tokens over a paged cache (gfx950): what their nodes see, and their attention.
+//
+// A tree's nodes are in an order in which each comes behind its parent; node i lies at place len + i of its sequence, behind the len positions of the
+// context that every node sees, and is the position len + depth of its own line.
+#include "paged.h"
+
+#include <float.h>
+
+#include <type_traits>
+
+namespace daisy {
+
+constexpr int kMostNodes = 256;
+
+// ---------------------------------------------------------------------------------------------------------------
+// What the nodes see
+// ---------------------------------------------------------------------------------------------------------------
+struct DraftTreeParams {
+  const int32_t* parents; int64_t parents_sb;      // [B, T], or one tree for all
+  const int32_t* lens; const int32_t* nodes;
+  uint32_t* mask; int32_t* positions; int32_t* slots; int32_t* rows;
+  int T, words;
+};
+
+// A workgroup per tree, a thread per node.  Lines double: a node's set and those of the node that its line goes on from are joined, and that node's
+// own next one becomes its next one; after log2 of the depth all lines have come to their roots.
+//
+// A launch and two reads one behind the other for small trees.
+template <int W>
+__global__ __launch_bounds__(kMostNodes) void draft_tree_kernel(DraftTreeParams p) {
+  __shared__ uint32_t sets[W][32 * W];
+  __shared__ int up[32 * W];
+  const int b = blockIdx.x, i = threadIdx.x;
+  const int len = p.lens[b];
+  const int n = len < 0 ? 0 : p.nodes != nullptr ? min(max(p.nodes[b], 0), p.T) : p.T;
+  int next = i < p.T ? p.parents[b * p.parents_sb + i] : -1;
+  if (next >= i) next = -1;
+  next = max(next, -1);
+  uint32_t set[W];
+#pragma unroll
+  for (int w = 0; w < W; ++w) set[w] = w == i >> 5 ? 1u << (i & 31) : 0;
+  // (every thread makes every round: there is nothing to gain from an end that has to be agreed on)
+#pragma unroll
+  for (int reach = 1; reach < 32 * W; reach *= 2) {
+    if (reach > 1) __syncthreads();
+#pragma unroll
+    for (int w = 0; w < W; ++w) sets[w][i] = set[w];
+    up[i] = next;
+    __syncthreads();
+    const int from = max(next, 0);
+#pragma unroll
+    for (int w = 0; w < W; ++w) set[w] |= next >= 0 ? sets[w][from] : 0;
+    next = next >= 0 ? up[from] : -1;
+  }
+  if (i >= p.T) return;
+  int depth = -1;
+#pragma unroll
+  for (int w = 0; w < W; ++w) depth += __popc(set[w]);
+  const int64_t at = (int64_t)b * p.T + i;
+  const bool there = i < n;
+#pragma unroll
+  for (int w = 0; w < W; ++w)
+    if (w < p.words) p.mask[at * p.words + w] = there ? set[w] : 0;
+  p.positions[at] = there ? len + depth : -1;
+  p.slots[at] = there ? len + i : -1;
+  p.rows[at] = b;
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Attention
+// ---------------------------------------------------------------------------------------------------------------
+// o[b, i, h] = sum_t softmax_t(scale q[b, i, h] . k_t) v_t over what node i of sequence b sees: the positions of the context, t < len, and the places len + j
+// of the nodes j whose bit its mask has, itself always; of these the last `window`.  G = Hq / H query heads to a key head.
+//
+// The queries of a key head, G of each node, are columns of the products; a unit is a (sequence, key head, block of up to 16 NC columns), and the tiles of 32 positions
+// of all units, one behind the other, are dealt to the wavefronts in equal runs, whatever the lengths.  A run that covers a whole unit writes the result; of the others
+// partial sums stay: the one that the run ends in the middle of in the wavefront's registers, the one that it begins in the middle of in the LDS, where the
+// wavefront ahead takes it from; what goes on beyond the workgroup a second kernel joins.
+//
+// Products: S^T = K Q^T, O^T = V^T P^T on 16x16x32 matrix instructions, NC of them for each piece of K and V that a wavefront has loaded: rows 4c + r and
+// 16 + 4c + r of a tile are, for the lanes of group c, both rows of S^T and rows of the second product's operand.  V's rows arrive 16 bytes a lane, v_perm pairs neighbours.
+//
+// A tile that all columns see whole needs no mask.  The others, those with nodes in them and those at a window's edge, make a word of 32 bits for each column, the tile's keys
+// that it sees.
+
+// What a wavefront's run leaves open: whether it begins inside a unit, whether that goes on beyond it, whether it ends inside another one; their columns.
+enum { kBeginsInside = 1, kGoesThrough = 2, kEndsInside = 4 };
+struct OpenUnits { int flags, cols0, cols1; };
+// A unit that goes on beyond a workgroup's run: the workgroups that have a part of it (first, last; -1: there is no such unit), its sequence, key head, first column and
+// number of columns.
+struct SplitUnit { int first, last, b, h, col0, cols; };
+
+struct TreeParams {
+  // (strides of q, k, v and o in pieces of 16 bytes)
+  const uint16_t* q; uint32_t q_sb, q_st, q_sh;
+  const uint16_t* k; uint32_t k_sp, k_sh, k_ss;
+  const uint16_t* v; uint32_t v_sp, v_sh, v_ss;
+  const int32_t* table; uint32_t table_st; int max_pages, num_pages, capacity; Divisor blocks_per_page;
+  const int32_t* lens; const int32_t* nodes;
+  const uint32_t* mask; int64_t mask_sb, mask_st; int words;
+  uint16_t* o; uint32_t o_sb, o_st, o_sh; int o_f16;
+  SplitUnit* split;               // [workgroups]
+  float* part; float2* stat;      // [2 * workgroups][columns of a unit][D], [..][..]: unnormalised sums; reference and sum of exponentials
+  int B, T, H, G, cols, window, groups; Divisor per_node;      // cols: of a unit at most; per_node: G
+  float scale_log2e;
+  int32_t* status;
+};
+
+// A column's query, in q or in o: node and head of it.
+struct Query { int node, head; };
+__device__ __forceinline__ Query query_of(const TreeParams& p, int h, int col) {
+  const Quotient of = divide((uint32_t)col, p.per_node);
+  return Query{of.of, h * p.G + of.rest};
+}
+__device__ __forceinline__ uint16_t* row_of_o(const TreeParams& p, int b, const Query& q) {
+  return p.o + 8 * (product(b, p.o_sb) + product(q.node, p.o_st) + product(q.head, p.o_sh));
+}
+template <bool F16> __device__ __forceinline__ u32x2 pack_out(const TreeParams& p, const f32x4& f) {
+  return F16 && p.o_f16 ? u32x2{pack2<F16>(f[0], f[1]), pack2<F16>(f[2], f[3])} : u32x2{pack2<false>(f[0], f[1]), pack2<false>(f[2], f[3])};
+}
+
+// A sequence: its context, its nodes, the places that some node sees, [lo, hi), the tiles that they lie in and the blocks of columns.
+struct Extent { int len, nodes, lo, hi, first, tiles, blocks; bool past; };
+template <int NC> __device__ __forceinline__ Extent extent(const TreeParams& p, int len, int nodes) {
+  Extent e;
+  e.nodes = len < 0 ? 0 : min(max(nodes, 0), p.T);
+  e.past = len > p.capacity - e.nodes;
+  e.len = min(max(len, 0), p.capacity);
+  e.hi = min(e.len + e.nodes, p.capacity);
+  e.lo = p.window > 0 ? max(e.len + 1 - p.window, 0) : 0;
+  e.lo = min(e.lo, max(e.hi - 1, 0));
+  e.first = (unsigned)e.lo / kTile;
+  e.tiles = e.nodes > 0 ? (int)((unsigned)(e.hi + kTile - 1) / kTile) - e.first : 0;
+  e.blocks = (int)((unsigned)(e.nodes * p.G + 16 * NC - 1) / (16 * NC));
+  return e;
+}
+struct Sequence { int len, nodes; };
+__device__ __forceinline__ Sequence sequence(const TreeParams& p, int b) {
+  const int at = min(b, p.B - 1);
+  const int len = p.lens[at], nodes = p.nodes != nullptr ? p.nodes[at] : p.T;
+  return Sequence{b < p.B ? len : -1, nodes};
+}
+template <int NC> __device__ __forceinline__ int weight_of(const TreeParams& p, const Sequence& s) {
+  const Extent e = extent<NC>(p, s.len, s.nodes);
+  return e.tiles * e.blocks;
+}
+
+// How many tiles a wavefront takes: no fewer than the workgroups there are can do, and more (a lane tries each number up to twice as many) where that
+// takes a thirty-second or more off the most loaded of the compute units.
+__device__ __forceinline__ int share_of(const TreeParams& p, int total, int lane) {
+  if (total <= 4 * kCus) return 1;
+  const int least = (int)((unsigned)(total + 4 * p.groups - 1) / (unsigned)(4 * p.groups)), more = min(lane, least), share = least + more;
+  // (in fp32: one more or less only makes another choice, the same one in every wavefront)
+  const float groups = ceilf((float)total * __builtin_amdgcn_rcpf((float)(4 * share)) - 0.001f);
+  const int load = (int)ceilf(groups * (1.f / kCus)) * share;
+  return least + (wave_min((more == 0 ? load - load / 32 : load) * 64 + more) & 63);
+}
+
+// Workgroups per compute unit, a wavefront of each per SIMD: what the registers leave room for.
+constexpr int tree_groups_per_cu(int D, int NC) { return D == 64 ? (NC == 1 ? 4 : NC == 2 ? 3 : 2) : D == 128 ? (NC == 1 ? 3 : NC == 2 ? 2 : 1) : 1; }
+constexpr int tree_row(int D) { return D + 4; }      // floats of a partial sum's row in the LDS
+
+// Bit i of a mask that begins `from` bits before its first word (or behind it), ones ahead of it: 32 of them.
+__device__ __forceinline__ uint32_t bits_from(const uint32_t* row, int words, int from) {
+  if (from <= -32) return ~0u;
+  const int at = from >> 5;      // (-1 for the tile that the context ends in)
+  const uint32_t a = row[min(max(at, 0), words - 1)], b = row[min(max(at + 1, 0), words - 1)];
+  const uint32_t lo = at < 0 ? ~0u : at < words ? a : 0, hi = at + 1 < words ? b : 0;
+  return __builtin_amdgcn_alignbit(hi, lo, from & 31);
+}
+
+template <int D, bool F16, int NC>
+__global__ __launch_bounds__(256, tree_groups_per_cu(D, NC)) void tree_attn_kernel(TreeParams p) {
+  constexpr int KS = D / 32;                     // steps of the first product
+  constexpr int J = D / 16;                      // 16-row pieces of the second product's result
+  constexpr int W = D == 64 ? 4 : 8;             // channels of a V row that a lane has beside each other
+  constexpr int P = D / 16 / W;                  // such pieces of a row
+  constexpr int VD = J / 2;                      // dwords of a V row that a lane holds
+  constexpr int ROW = tree_row(D);
+  // The reference of the exponentials stays kHead below the largest score that set it and moves when a score is kLimit above it, so that
+  // fp16 probabilities use the type's range on both sides of one.
+  constexpr float kHead = F16 ? 9.f : 0.f, kLimit = F16 ? 15.f : 8.f;
+
+  extern __shared__ float open_sums[];      // [4 wavefronts][cols][ROW]: of the unit that the run begins in the middle of
+  __shared__ float2 open_stats[4][16 * NC];
+  __shared__ OpenUnits open_units[4];
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = blockIdx.x, wave = group * 4 + wv;
+  const int n = lane & 15, c = lane >> 4;
+  // Tiles of the sequences (of one key head each): lane i has the sum of those from i * per_lane on, which gives the total and where a run begins.
+  int own = 0, per_lane = (p.B + 63) >> 6;
+  Sequence s4[4];
+  if (per_lane <= 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s4[i] = sequence(p, lane * per_lane + min(i, per_lane - 1));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) own += i < per_lane ? weight_of<NC>(p, s4[i]) : 0;
+  } else {
+    // 64 at a time, the wavefronts in turn: in a row, where lanes by themselves are a cache line or more apart
+    __shared__ int sums[64];
+    per_lane = (p.B + 4095) >> 12 << 6;
+    const int used = (int)((unsigned)(p.B + per_lane - 1) / (unsigned)per_lane);
+    for (int i = wv; i < used; i += 4) {
+      int tiles = 0;
+      for (int j = 0; j < per_lane; j += 64) tiles += weight_of<NC>(p, sequence(p, i * per_lane + j + lane));
+      const int sum = wave_scan(tiles);
+      if (lane == 63) sums[i] = sum;
+    }
+    __syncthreads();
+    own = lane < used ? sums[lane] : 0;
+    s4[0] = Sequence{-1, 0};
+  }
+  const int own_upto = wave_scan(own);
+  const int total = __builtin_amdgcn_readlane(own_upto, 63) * p.H;
+  const int share = share_of(p, total, lane);
+  int x = (int)min((unsigned)wave * (unsigned)share, (unsigned)total);      // (the product is less than twice the total, 2^30 at most, and a share for each wavefront)
+  const int x_end = min(x + share, total);
+  OpenUnits mine = {0, 0, 0};
+  SplitUnit beyond = {-1, 0, 0, 0, 0, 0};
+
+  const uint32_t k_row = p.k_ss * 16, v_row = p.v_ss * 16;      // bytes, fewer than 2^24
+  // 64 sequences from `base` on, one a lane; up to 64 are all there
+  int base = 0, before = 0, weight = own, upto = own_upto, chunk = per_lane == 1 ? __builtin_amdgcn_readlane(own_upto, 63) : -1;
+  Sequence seq = s4[0];
+  if (per_lane > 1 && x < x_end) {
+    const int first = 63 - __builtin_clzll(__ballot(own > 0 && (own_upto - own) * p.H <= x));
+    base = first * per_lane;
+    before = __builtin_amdgcn_readlane(own_upto - own, first);
+  }
+  f32x4 acc[NC][J];
+  float m[NC], l[NC];
+  int b = 0, h = 0, col0 = 0, cols = 0;      // the unit: sequence, key head, first column and number of columns
+  while (x < x_end) {
+    // ---- the unit that x lies in.  (More than 64 lengths are read twice: somebody who changes them meanwhile gets wrong results, but every index below
+    // stays inside the call's tensors and x goes on.)
+    while (chunk < 0 || (x >= (before + chunk) * p.H && base < p.B)) {
+      if (chunk >= 0) { before += chunk; base += 64; }
+      seq = sequence(p, base + lane);
+      weight = weight_of<NC>(p, seq);
+      upto = wave_scan(weight);
+      chunk = __builtin_amdgcn_readlane(upto, 63);
+    }
+    const uint64_t here = __ballot(weight > 0 && (before + upto - weight) * p.H <= x);
+    const int bl = 63 - __builtin_clzll(here | 1);
+    b = min(base + bl, p.B - 1);
+    const Extent e = extent<NC>(p, __builtin_amdgcn_readlane(seq.len, bl), __builtin_amdgcn_readlane(seq.nodes, bl));
+    const int n_tiles = max(e.tiles, 1), blocks = max(e.blocks, 1);
+    const int rel = x - (before + __builtin_amdgcn_readlane(upto - weight, bl)) * p.H;
+    const int unit = (int)min((unsigned)rel / (unsigned)n_tiles, (unsigned)(p.H * blocks - 1)), off = min(max(rel - unit * n_tiles, 0), n_tiles - 1);
+    const int count = max(min(n_tiles - off, x_end - x), 1);
+    h = (int)((unsigned)unit / (unsigned)blocks);
+    col0 = (unit - h * blocks) * 16 * NC;
+    const int all_cols = max(e.nodes * p.G, 1);
+    cols = min(all_cols - col0, 16 * NC);
+
+    // ---- its queries: columns past the last one repeat it
+    u32x4 qf[NC][KS];
+    int node[NC], lo[NC];      // of a column: its node, the first place that it may see
+#pragma unroll
+    for (int t = 0; t < NC; ++t) {
+      const Query of = query_of(p, h, min(col0 + 16 * t + n, all_cols - 1));
+      node[t] = of.node;
+      lo[t] = 0;
+      const uint16_t* src = p.q + 8 * (product(b, p.q_sb) + product(of.node, p.q_st) + product(of.head, p.q_sh) + c);
+#pragma unroll
+      for (int s = 0; s < KS; ++s) qf[t][s] = *reinterpret_cast<const u32x4*>(src + 32 * s);
+    }
+    const uint32_t* mask = p.mask + b * p.mask_sb;
+    if (p.window > 0) {
+      for (int t = 0; t < NC; ++t) {
+        auto word = [&](int w) {
+          uint32_t bits = mask[node[t] * p.mask_st + w];
+          bits |= node[t] >> 5 == w ? 1u << (node[t] & 31) : 0;
+          const int there = e.nodes - 32 * w;      // bits of nodes that there are
+          return there >= 32 ? bits : there <= 0 ? 0 : bits & ((1u << there) - 1);
+        };
+        int seen = 0;
+        for (int w = 0; w < p.words; ++w) seen += __popc(word(w));
+        const int drop = e.len + seen - p.window;
+        lo[t] = max(drop, 0);
+        if (drop > e.len) {      // nodes, too: as many of them as are too many behind the context
+          int left = drop - e.len, w = 0;
+          uint32_t bits = word(0);
+          while (w + 1 < p.words && left >= __popc(bits)) { left -= __popc(bits); bits = word(++w); }
+          for (; left > 0; --left) bits &= bits - 1;
+          lo[t] = e.len + 32 * w + (bits != 0 ? __builtin_ctz(bits) : 31);
+        }
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < NC; ++t) {
+#pragma unroll
+      for (int j = 0; j < J; ++j) acc[t][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      m[t] = -FLT_MAX;      // (finite: a key may score -inf, a whole tile of them too)
+      l[t] = 0.f;
+    }
+
+    // ---- pages: lane i has that of the run's block i, for 32 tiles at a time
+    const int32_t* row = p.table + product(b, p.table_st);
+    const int blk_lo = (unsigned)e.lo / kBlock, blk_hi = max(e.hi - 1, 0) / kBlock;
+    bool bad = e.past;
+    int id = 0, in = 0;
+    auto pages_from = [&](int block) {
+      const int blk = min(max(block + lane, blk_lo), blk_hi);      // (blocks outside the range: read, but not used)
+      const Quotient page = divide((uint32_t)blk, p.blocks_per_page);
+      in = page.rest;
+      id = row[page.of];
+      const bool out = (unsigned)id >= (unsigned)p.num_pages;
+      bad |= out;
+      id = out ? 0 : id;
+    };
+    const char* kh = reinterpret_cast<const char*>(p.k) + 16 * product(h, p.k_sh);
+    const char* vh = reinterpret_cast<const char*>(p.v) + 16 * product(h, p.v_sh);
+    u32x4 kr[2][KS];
+    uint32_t vr[8][VD];
+    const int tile0 = e.first + off;
+    const int lo_edge = p.window > 0 ? e.len - p.window + e.nodes : 0;      // no column's first place lies behind this one, or it is a node
+    auto at_edge = [&](int i) { return (tile0 + i) * kTile < lo_edge || (tile0 + i + 1) * kTile > e.len; };
+    // Half `half` of tile i of the run: where its rows are, in the pages of `base`.
+    auto half_tile = [&](const char* base, uint32_t sp, uint32_t ss, int i, int half) {
+      const int pg = __builtin_amdgcn_readlane(id, 2 * (i & 31) + half), slot = __builtin_amdgcn_readlane(in, 2 * (i & 31) + half) * kBlock;
+      return base + 16 * (product(pg, sp) + product(slot, ss));
+    };
+    // A row of it, or where that is outside the range, another one that is read anyhow: nothing is fetched for the rows that a short sequence does not
+    // have, and every tile is asked for by the same instructions in the same order, which the waits for them count.
+    auto row_of = [&](int row, int i, int half) {
+      const int first = (tile0 + i) * kTile + half * kBlock;
+      return min(max(row, min(max(e.lo - first, 0), kBlock - 1)), min(max(e.hi - 1 - first, 0), kBlock - 1));
+    };
+    // (past the caches, unless other blocks of columns read the same rows)
+    auto load16 = [&](const char* at) {
+      if constexpr (NC == 1) return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at));
+      else return *reinterpret_cast<const u32x4*>(at);
+    };
+    auto load_k = [&](int i) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const char* src = half_tile(kh, p.k_sp, p.k_ss, i, half) + (__umul24(row_of(n, i, half), k_row) + 16 * c);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) kr[half][s] = load16(src + 64 * s);
+      }
+    };
+    auto load_v = [&](int i) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const char* src = half_tile(vh, p.v_sp, p.v_ss, i, half);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const char* at = src + (__umul24(row_of(4 * c + r, i, half), v_row) + 2 * W * n);
+#pragma unroll
+          for (int t = 0; t < P; ++t) {
+            if constexpr (W == 8) {
+              const u32x4 d = load16(at + 256 * t);
+#pragma unroll
+              for (int i4 = 0; i4 < 4; ++i4) vr[4 * half + r][4 * t + i4] = d[i4];
+            } else {
+              const u32x2 d = *reinterpret_cast<const u32x2*>(at);
+              vr[4 * half + r][0] = d[0];
+              vr[4 * half + r][1] = d[1];
+            }
+          }
+        }
+      }
+    };
+
+    pages_from(2 * tile0);
+    load_k(0);
+    __builtin_amdgcn_sched_barrier(0);      // K ahead of V, as in the loop: what waits for a tile's keys does not wait for its values
+    load_v(0);
+    // (The last tile by itself: a wait counts what was asked for behind what it waits for, which no branch may leave open.)
+    auto step = [&](int i, auto more) {
+      const int tile = (tile0 + i) * kTile;
+      // ---- scores
+      f32x4 sc[NC][2];
+#pragma unroll
+      for (int t = 0; t < NC; ++t) sc[t][0] = sc[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int t = 0; t < NC; ++t) {
+          sc[t][0] = mfma<F16>(kr[0][s], qf[t][s], sc[t][0]);
+          sc[t][1] = mfma<F16>(kr[1][s], qf[t][s], sc[t][1]);
+        }
+      if constexpr (more.value) {
+        if (((i + 1) & 31) == 0) pages_from(2 * (tile0 + i + 1));
+        load_k(i + 1);
+      }
+      // ---- who sees what; rows that nobody sees may hold anything, and a number that is not finite belongs to those who see it
+      const bool edge = at_edge(i);
+      bool dirty = false;
+      uint32_t vis[NC];
+      if (edge) {
+        const int end = e.hi - tile;      // (at least one)
+#pragma unroll
+        for (int t = 0; t < NC; ++t) {
+          uint32_t bits = bits_from(mask + node[t] * p.mask_st, p.words, tile - e.len);
+          const int self = e.len + node[t] - tile, low = lo[t] - tile;
+          bits |= (unsigned)self < 32u ? 1u << self : 0;
+          bits &= end >= 32 ? ~0u : (1u << max(end, 0)) - 1;
+          vis[t] = low >= 32 ? 0 : low <= 0 ? bits : bits & (~0u << low);
+        }
+        uint32_t most = 0;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const int key = tile + 4 * c + (r & 3) + (r & 4) * 4;
+          const bool there = key >= e.lo && key < e.hi;
+#pragma unroll
+          for (int d = 0; d < VD; ++d) {
+            vr[r][d] = there ? vr[r][d] : 0;
+            typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+            most = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, most), __builtin_bit_cast(u16x2, vr[r][d] & 0x7fff7fffu)));
+          }
+        }
+        constexpr uint32_t kInf = F16 ? 0x7c00u : 0x7f80u;
+        dirty = __any((most & 0xffffu) >= kInf || (most >> 16) >= kInf);
+      }
+      // ---- probabilities, in two parts, the second what the rounding of the first has lost: the result is as if they had not been rounded
+      u32x4 pf[NC], pl[NC];
+#pragma unroll
+      for (int t = 0; t < NC; ++t) {
+        float s[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) s[r] = sc[t][r >> 2][r & 3] * p.scale_log2e;
+        if (edge) {
+#pragma unroll
+          for (int r = 0; r < 8; ++r) s[r] = vis[t] >> (4 * c + (r & 3) + (r & 4) * 4) & 1 ? s[r] : -__builtin_inff();
+        }
+        float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+        {
+          const LanePair r = row_pair(top);
+          const LanePair u = half_pair(fmaxf(r.x, r.y));
+          top = fmaxf(u.x, u.y);
+        }
+        if (__any(top > m[t] + kLimit)) {
+          const float moved = top > m[t] + kLimit ? top - kHead : m[t];
+          const float f = moved > m[t] ? fast_exp2(m[t] - moved) : 1.f;
+          m[t] = moved;
+          l[t] *= f;
+#pragma unroll
+          for (int j = 0; j < J; ++j) acc[t][j] *= f;
+        }
+#pragma unroll
+        for (int r = 0; r < 8; ++r) s[r] = fast_exp2(s[r] - m[t]);
+        l[t] += ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+        pf[t] = pack8_as<F16>(s);
+        float f[8];
+        unpack8_as<F16>(pf[t], f);
+#pragma unroll
+        for (int r = 0; r < 8; ++r) f[r] = s[r] - f[r];
+        pl[t] = pack8_as<F16>(f);
+      }
+      // ---- O^T += V^T P^T
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const int d = (j / W) * (W / 2) + (j % W) / 2;
+        u32x4 vf;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) vf[t] = __builtin_amdgcn_perm(vr[2 * t + 1][d], vr[2 * t][d], (j & 1) ? 0x07060302u : 0x05040100u);
+        if (dirty) {
+          // Values that are not finite leave the product; who sees one of a channel gets NaN there.
+          constexpr uint32_t kInf = F16 ? 0x7c00u : 0x7f80u, kOne = F16 ? 0x3c00u : 0x3f80u;
+          u32x4 odd;
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            const uint32_t low = (vf[t] & kInf) == kInf ? 0xffffu : 0, high = (vf[t] >> 16 & kInf) == kInf ? 0xffff0000u : 0;
+            odd[t] = (low | high) & (kOne | kOne << 16);
+            vf[t] &= ~(low | high);
+          }
+#pragma unroll
+          for (int t = 0; t < NC; ++t) {
+            u32x4 sees;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const uint32_t pair = vis[t] >> (4 * c + (2 * r & 3) + (2 * r & 4) * 4);
+              sees[r] = (pair & 1 ? kOne : 0) | (pair & 2 ? kOne << 16 : 0);
+            }
+            const f32x4 met = mfma<F16>(odd, sees, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+            for (int i4 = 0; i4 < 4; ++i4) acc[t][j][i4] = met[i4] > 0.f ? __builtin_nanf("") : acc[t][j][i4];
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < NC; ++t) {
+          acc[t][j] = mfma<F16>(vf, pf[t], acc[t][j]);
+          acc[t][j] = mfma<F16>(vf, pl[t], acc[t][j]);
+        }
+      }
+      if constexpr (more.value) load_v(i + 1);
+    };
+    for (int i = 0; i + 1 < count; ++i) step(i, std::true_type());
+    step(count - 1, std::false_type());
+
+    // ---- the four groups of lanes have summed their own keys
+    const bool spoiled = __any(bad);
+    if (spoiled && lane == 0) raise_status(p.status, e.past ? DAISY_STATUS_LENGTH_PAST_PAGES : DAISY_STATUS_PAGE_OUT_OF_RANGE);
+#pragma unroll
+    for (int t = 0; t < NC; ++t) {
+      const LanePair r = row_pair(l[t]);
+      const LanePair u = half_pair(r.x + r.y);
+      l[t] = spoiled ? __builtin_nanf("") : u.x + u.y;
+    }
+    if (off == 0 && count == n_tiles) {
+#pragma unroll
+      for (int t = 0; t < NC; ++t) {
+        if (16 * t + n >= cols) continue;
+        const float inv = 1.f / l[t];
+        uint16_t* dst = row_of_o(p, b, query_of(p, h, col0 + 16 * t + n)) + 4 * W * c;
+#pragma unroll
+        for (int u = 0; u < P; ++u)
+#pragma unroll
+          for (int i8 = 0; i8 < W / 2; ++i8) {
+            float f[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = acc[t][u * W + (8 * i8 + i) % W][(8 * i8 + i) / W] * inv;
+            *reinterpret_cast<u32x4*>(dst + 128 * u + 8 * i8) = F16 && p.o_f16 ? pack8_as<F16>(f) : pack8_as<false>(f);
+          }
+      }
+    } else if (off > 0) {
+      mine.flags |= off + count < n_tiles ? kBeginsInside | kGoesThrough : kBeginsInside;
+      mine.cols0 = cols;
+#pragma unroll
+      for (int t = 0; t < NC; ++t) {
+        if (16 * t + n >= cols) continue;
+        float* dst = open_sums + (wv * p.cols + 16 * t + n) * ROW + 4 * W * c;
+#pragma unroll
+        for (int u = 0; u < P; ++u)
+#pragma unroll
+          for (int i4 = 0; i4 < W; ++i4) {
+            f32x4 f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = acc[t][u * W + (4 * i4 + i) % W][(4 * i4 + i) / W];
+            *reinterpret_cast<f32x4*>(dst + 128 * u + 4 * i4) = f;
+          }
+        if (c == 0) open_stats[wv][16 * t + n] = float2{m[t], l[t]};
+      }
+    } else {
+      mine.flags |= kEndsInside;
+      mine.cols1 = cols;
+    }
+    if (off + count < n_tiles && wv == 3) {
+      const unsigned run = (unsigned)__builtin_amdgcn_readfirstlane(4 * share);
+      beyond = SplitUnit{(int)((unsigned)(x - off) / run), (int)((unsigned)(x - off + n_tiles - 1) / run), b, h, col0, cols};
+    }
+    x += count;
+  }
+
+  // ---- what the wavefronts have left open: chains of the same unit, from where one of them broke off (or the workgroup began) on
+  if (lane == 0) open_units[wv] = mine;
+  if (lane == 0 && wv == 3) p.split[group] = beyond;
+  // (nodes that there are not: sequences dealt out one by one)
+  for (int s = group; s < p.B; s += p.groups) {
+    const Extent e = extent<NC>(p, p.lens[s], p.nodes != nullptr ? p.nodes[s] : p.T);
+    const int per_node = p.H * p.G * (D / 8);
+    for (int i = threadIdx.x + e.nodes * per_node; i < p.T * per_node; i += 256) {
+      const int row = i / (D / 8);
+      *reinterpret_cast<u32x4*>(row_of_o(p, s, Query{row / (p.H * p.G), row % (p.H * p.G)}) + i % (D / 8) * 8) = u32x4{0, 0, 0, 0};
+    }
+  }
+  __syncthreads();
+  const int flags = open_units[lane & 3].flags;      // (bit w of each: wavefront w's)
+  const int through = (int)__ballot(flags & kGoesThrough);
+  if (mine.flags & kEndsInside) {
+    // this wavefront's last unit, and what those behind it have of it
+    bool on = true;
+    int last = wv;
+    while (on && last < 3) on = through >> ++last & 1;
+#pragma unroll
+    for (int t = 0; t < NC; ++t) {
+      if (16 * t + n >= cols) continue;
+      for (int y = wv + 1; y <= last; ++y) {
+        const float2 more = open_stats[y][16 * t + n];
+        const float top = fmaxf(m[t], more.x), f = fast_exp2(m[t] - top), g = fast_exp2(more.x - top);
+        const float* src = open_sums + (y * p.cols + 16 * t + n) * ROW + 4 * W * c;
+        l[t] = f * l[t] + g * more.y;
+        m[t] = top;
+#pragma unroll
+        for (int u = 0; u < P; ++u)
+#pragma unroll
+          for (int i4 = 0; i4 < W; ++i4) {
+            const f32x4 a = *reinterpret_cast<const f32x4*>(src + 128 * u + 4 * i4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              f32x4& to = acc[t][u * W + (4 * i4 + i) % W];
+              to[(4 * i4 + i) / W] = f * to[(4 * i4 + i) / W] + g * a[i];
+            }
+          }
+      }
+      const float inv = on ? 1.f : 1.f / l[t];
+      const int64_t slot = (int64_t)(2 * group + 1) * p.cols + 16 * t + n;
+      uint16_t* dst = row_of_o(p, b, query_of(p, h, col0 + 16 * t + n)) + 4 * W * c;
+#pragma unroll
+      for (int u = 0; u < P; ++u)
+#pragma unroll
+        for (int i4 = 0; i4 < W; ++i4) {
+          f32x4 f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) f[i] = acc[t][u * W + (4 * i4 + i) % W][(4 * i4 + i) / W] * inv;
+          if (on) *reinterpret_cast<f32x4*>(p.part + slot * D + 4 * W * c + 128 * u + 4 * i4) = f;
+          else *reinterpret_cast<u32x2*>(dst + 128 * u + 4 * i4) = pack_out<F16>(p, f);
+        }
+      if (on && c == 0) p.stat[slot] = float2{m[t], l[t]};
+    }
+  }
+  if (open_units[0].flags & kBeginsInside) {
+    // the unit that the workgroup begins inside of
+    int last = 0;
+    for (bool on = through & 1; on && last < 3;) on = through >> ++last & 1;
+    const int64_t slot = (int64_t)(2 * group) * p.cols;
+    for (int i = threadIdx.x; i < open_units[0].cols0 * (D / 4); i += 256) {
+      const int g = i / (D / 4), at = i % (D / 4) * 4;
+      float2 st = open_stats[0][g];
+      f32x4 sum = *reinterpret_cast<const f32x4*>(open_sums + g * ROW + at);
+      for (int y = 1; y <= last; ++y) {
+        const float2 more = open_stats[y][g];
+        const float top = fmaxf(st.x, more.x), f = fast_exp2(st.x - top), a = fast_exp2(more.x - top);
+        sum = f * sum + a * *reinterpret_cast<const f32x4*>(open_sums + (y * p.cols + g) * ROW + at);
+        st = float2{top, f * st.y + a * more.y};
+      }
+      *reinterpret_cast<f32x4*>(p.part + (slot + g) * D + at) = sum;
+      if (at == 0) p.stat[slot + g] = st;
+    }
+  }
+}
+
+// Where part i of a unit is: the workgroup that the unit begins in has it in its second slot, the others in their first.
+__device__ __forceinline__ int64_t part_slot(const TreeParams& p, const SplitUnit& u, int i, int col) {
+  return (int64_t)(2 * (u.first + i) + (i == 0 ? 1 : 0)) * p.cols + col;
+}
+
+// Joins the partial sums of the units that lie in more than one workgroup's run.  The results of a unit are dealt to as many workgroups as there are ends of runs in
+// it, LPR lanes to a piece of 4 LPR channels and 256 / LPR parts side by side, the lanes' sums joined in the LDS.
+template <int D, bool F16, int LPR>
+__device__ __forceinline__ void join_parts(const TreeParams& p, const SplitUnit& u, int parts, int helpers, int me, f32x4 (*sums)[256], float2* stats) {
+  constexpr int GROUPS = 256 / LPR, U = 4, CH = 4 * LPR;      // (U parts asked for at once)
+  const int r = threadIdx.x / LPR, at = threadIdx.x % LPR * 4;
+  for (int chunk = me; chunk < u.cols * (D / CH); chunk += helpers) {
+    const int col = chunk / (D / CH), d0 = chunk % (D / CH) * CH;
+    float m = -__builtin_inff(), l = 0.f;
+    f32x4 a = {0.f, 0.f, 0.f, 0.f};
+    for (int i0 = r; i0 < parts; i0 += GROUPS * U) {
+      float2 st[U];
+      f32x4 v[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const int64_t s = part_slot(p, u, min(i0 + GROUPS * i, parts - 1), col);
+        st[i] = p.stat[s];
+        v[i] = *reinterpret_cast<const f32x4*>(p.part + s * D + d0 + at);
+      }
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        if (i0 + GROUPS * i >= parts) break;
+        const float top = fmaxf(m, st[i].x), f = m > -__builtin_inff() ? fast_exp2(m - top) : 0.f, e = fast_exp2(st[i].x - top);
+        l = f * l + e * st[i].y;
+        a = f * a + e * v[i];
+        m = top;
+      }
+    }
+    __syncthreads();      // (the chunk before has been read)
+    (*sums)[threadIdx.x] = a;
+    if (at == 0) stats[r] = float2{m, l};
+    __syncthreads();
+    if (threadIdx.x < LPR) {
+      const int used = min(GROUPS, parts);
+      float best = stats[0].x, all = 0.f;
+      for (int i = 1; i < used; ++i) best = fmaxf(best, stats[i].x);
+      a = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < used; ++i) {
+        const float w = fast_exp2(stats[i].x - best);
+        all = fmaf(w, stats[i].y, all);
+        a += w * (*sums)[i * LPR + threadIdx.x];
+      }
+      a *= 1.f / all;
+      *reinterpret_cast<u32x2*>(row_of_o(p, u.b, query_of(p, u.h, u.col0 + col)) + d0 + at) = pack_out<F16>(p, a);
+    }
+  }
+}
+
+template <int D, bool F16>
+__global__ __launch_bounds__(256) void tree_join_kernel(TreeParams p) {
+  constexpr int kFew = 8;
+  __shared__ f32x4 sums[1][256];
+  __shared__ float2 stats[64];
+  const SplitUnit u = p.split[blockIdx.x];
+  // No such unit; or, where another call has the same workspace at the same time, one that is not this call's: its results are lost, nothing else is.
+  if (u.first < 0 || u.first > (int)blockIdx.x || u.last <= (int)blockIdx.x || u.last >= p.groups) return;
+  if ((unsigned)u.b >= (unsigned)p.B || (unsigned)u.h >= (unsigned)p.H || u.cols <= 0 || u.cols > p.cols || u.col0 < 0 || u.col0 > p.T * p.G - u.cols) return;
+  const int parts = u.last - u.first + 1, helpers = parts - 1, me = (int)blockIdx.x - u.first;
+  if (parts <= kFew) {
+    // a thread per four channels, every part of which it asks for at once
+    for (int i0 = me * 256 + (int)threadIdx.x; i0 < u.cols * (D / 4); i0 += helpers * 256) {
+      const int col = i0 / (D / 4), at = i0 % (D / 4) * 4;
+      float2 st[kFew];
+      f32x4 v[kFew];
+#pragma unroll
+      for (int i = 0; i < kFew; ++i) {
+        const int64_t s = part_slot(p, u, min(i, parts - 1), col);
+        st[i] = p.stat[s];
+        v[i] = *reinterpret_cast<const f32x4*>(p.part + s * D + at);
+      }
+      float top = st[0].x, l = 0.f;
+#pragma unroll
+      for (int i = 1; i < kFew; ++i) top = fmaxf(top, st[i].x);
+      f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < kFew; ++i) {
+        const float f = i < parts ? fast_exp2(st[i].x - top) : 0.f;
+        l = i < parts ? fmaf(f, st[i].y, l) : l;
+        a = i < parts ? a + f * v[i] : a;
+      }
+      a *= 1.f / l;
+      *reinterpret_cast<u32x2*>(row_of_o(p, u.b, query_of(p, u.h, u.col0 + col)) + at) = pack_out<F16>(p, a);
+    }
+  } else if (parts > 128) {
+    join_parts<D, F16, 4>(p, u, parts, helpers, me, sums, stats);
+  } else {
+    join_parts<D, F16, 16>(p, u, parts, helpers, me, sums, stats);
+  }
+}
+
+// How many workgroups share the work: what the chip holds at once, less where there are fewer tiles.
+struct TreeSplit { int groups, cols, blocks, NC; size_t lds; };
+static TreeSplit tree_split(int B, int T, int H, int G, int D, int64_t capacity) {
+  TreeSplit s;
+  const int all = T * G;
+  s.NC = all <= 16 ? 1 : all <= 32 || D == 256 ? 2 : 4;
+  s.cols = all < 16 * s.NC ? all : 16 * s.NC;
+  s.blocks = (all + 16 * s.NC - 1) / (16 * s.NC);
+  s.lds = (size_t)4 * s.cols * tree_row(D) * sizeof(float);
+  const int64_t tiles = ((capacity + kTile - 1) / kTile) * B * H * s.blocks;
+  const int64_t groups = (tiles + 3) / 4, most = kCus * tree_groups_per_cu(D, s.NC);
+  s.groups = (int)(groups < most ? groups : most);
+  return s;
+}
+// Tiles are counted in 32 bits, with room for a share's rounding.
+static bool tree_tiles_fit(int B, int T, int Hq, int H, int D, int64_t capacity) {
+  return ((double)capacity / kTile + 1) * B * H * tree_split(1, T, H, Hq / H, D, 1).blocks < (double)(1 << 30);
+}
+static bool tree_shape_ok(int B, int T, int Hq, int H, int D, int max_pages, int page_size) {
+  return B > 0 && T > 0 && T <= kMostNodes && H > 0 && Hq > 0 && Hq % H == 0 && Hq <= 65536 && (D == 64 || D == 128 || D == 256) && max_pages > 0 && page_size > 0 &&
+         (int64_t)max_pages * page_size <= kMostPositions && tree_tiles_fit(B, T, Hq, H, D, (int64_t)max_pages * page_size);
+}
+
+template <int D, bool F16, int NC> static int tree_launch(const TreeParams& p, size_t lds, hipStream_t s) {
+  hipLaunchKernelGGL((tree_attn_kernel<D, F16, NC>), dim3((unsigned)p.groups), dim3(256), lds, s, p);
+  hipLaunchKernelGGL((tree_join_kernel<D, F16>), dim3((unsigned)p.groups), dim3(256), 0, s, p);
+  DAISY_CHECK_LAUNCH("tree_attn_kernel");
+  return DAISY_OK;
+}
+template <int D, bool F16> static int tree_launch(const TreeParams& p, int NC, size_t lds, hipStream_t s) {
+  if (NC == 1) return tree_launch<D, F16, 1>(p, lds, s);
+  if (D == 256 || NC == 2) return tree_launch<D, F16, 2>(p, lds, s);
+  if constexpr (D < 256) return tree_launch<D, F16, 4>(p, lds, s);
+  return DAISY_ERR_UNSUPPORTED;
+}
+template <bool F16> static int tree_launch(const TreeParams& p, int D, int NC, size_t lds, hipStream_t s) {
+  return D == 64 ? tree_launch<64, F16>(p, NC, lds, s) : D == 128 ? tree_launch<128, F16>(p, NC, lds, s) : tree_launch<256, F16>(p, NC, lds, s);
+}
+
+}  // namespace daisy
+
+using namespace daisy;
+
+extern "C" int daisy_draft_tree_fwd(const int32_t* parents, int64_t parents_stride, const int32_t* lens, const int32_t* nodes,
+                                    int32_t* mask, int32_t* positions, int32_t* slots, int32_t* rows, int B, int T, void* stream) {
+  DAISY_CHECK_ARG(parents && lens && mask && positions && slots && rows, "draft_tree: the parents, the lengths and the results must be non-NULL");
+  DAISY_CHECK_ARG(B > 0 && T > 0 && parents_stride >= 0, "draft_tree: B=%d, T=%d must be positive", B, T);
+  DAISY_CHECK_SUPPORTED(T <= kMostNodes, "draft_tree: trees of %d nodes not supported (at most %d)", T, kMostNodes);
+  DraftTreeParams p = {parents, parents_stride, lens, nodes, (uint32_t*)mask, positions, slots, rows, T, (T + 31) / 32};
+  hipStream_t s = (hipStream_t)stream;
+  if (T <= 64) hipLaunchKernelGGL((draft_tree_kernel<2>), dim3((unsigned)B), dim3(64), 0, s, p);
+  else if (T <= 128) hipLaunchKernelGGL((draft_tree_kernel<4>), dim3((unsigned)B), dim3(128), 0, s, p);
+  else hipLaunchKernelGGL((draft_tree_kernel<8>), dim3((unsigned)B), dim3(256), 0, s, p);
+  DAISY_CHECK_LAUNCH("draft_tree_kernel");
+  return DAISY_OK;
+}
+
+extern "C" size_t daisy_paged_tree_attn_workspace_bytes(int B, int T, int Hq, int H, int D, int max_pages, int page_size) {
+  if (!tree_shape_ok(B, T, Hq, H, D, max_pages, page_size)) return 0;
+  const TreeSplit sp = tree_split(B, T, H, Hq / H, D, (int64_t)max_pages * page_size);
+  return (size_t)sp.groups * (32 + 2 * (size_t)sp.cols * (D + 2) * sizeof(float));
+}
+
+extern "C" int daisy_paged_tree_attn_fwd(const void* q, const int64_t* q_strides,
+                                         const void* k_pages, const int64_t* k_pages_strides, const void* v_pages, const int64_t* v_pages_strides,
+                                         int cache_is_f16, const int32_t* page_table, int64_t table_stride, int max_pages, int num_pages, int page_size,
+                                         const int32_t* lens, const int32_t* nodes, const int32_t* mask, const int64_t* mask_strides,
+                                         void* o, const int64_t* o_strides, int o_is_f16, int B, int T, int Hq, int H, int D, int window, float scale,
+                                         int32_t* status, void* workspace, size_t workspace_bytes, void* stream) {
+  DAISY_CHECK_ARG(q && q_strides && o && o_strides && lens && mask && mask_strides, "paged_tree_attn: q, o, the mask, their strides and the lengths must be non-NULL");
+  DAISY_CHECK_ARG(B > 0 && T > 0 && H > 0 && Hq > 0 && Hq % H == 0, "paged_tree_attn: B=%d, T=%d, H=%d must be positive, Hq=%d a multiple of H", B, T, H, Hq);
+  DAISY_CHECK_SUPPORTED(T <= kMostNodes, "paged_tree_attn: trees of %d nodes not supported (at most %d)", T, kMostNodes);
+  DAISY_CHECK_SUPPORTED(Hq <= 65536, "paged_tree_attn: %d query heads not supported (at most 65536)", Hq);
+  DAISY_CHECK_HEAD_DIM("paged_tree_attn", D);
+  DAISY_CHECK_PAGES("paged_tree_attn");
+  DAISY_CHECK_ARG(al16(q) && al16(o) && rows_of_16(q_strides, B, T) && step_of_16(q_strides[2], Hq) && rows_of_16(o_strides, B, T) && step_of_16(o_strides[2], Hq),
+                  "paged_tree_attn: q and o must be 16-byte aligned, their strides multiples of 8 elements");
+  DAISY_CHECK_ARG((B == 1 || mask_strides[0] >= 0) && (T == 1 || mask_strides[1] >= 0), "paged_tree_attn: strides of the mask must not be negative");
+  const int64_t capacity = (int64_t)max_pages * page_size;
+  DAISY_CHECK_ARG(tree_tiles_fit(B, T, Hq, H, D, capacity), "paged_tree_attn: %d sequences of up to %lld positions, %d key heads, are too many", B, (long long)capacity, H);
+  DAISY_CHECK_SUPPORTED(!o_is_f16 || cache_is_f16, "paged_tree_attn: an fp16 o needs an fp16 cache");
+  constexpr int64_t kWidest = (int64_t)1 << 35;
+  auto narrow = [](const int64_t* st, int n0, int n1, int n2) {
+    return (n0 == 1 || st[0] < kWidest) && (n1 == 1 || st[1] < kWidest) && (n2 == 1 || st[2] < kWidest);
+  };
+  DAISY_CHECK_SUPPORTED(narrow(q_strides, B, T, Hq) && narrow(o_strides, B, T, Hq) && max_stride(k_pages_strides, num_pages, H) < kWidest &&
+                            max_stride(v_pages_strides, num_pages, H) < kWidest && (B == 1 || table_stride < (int64_t)1 << 32),
+                        "paged_tree_attn: a stride is too long (2^35 elements, 2^32 of the table)");
+  const Rows q_rows = rows_of(q_strides, B, T, Hq, D), o_rows = rows_of(o_strides, B, T, Hq, D);
+  DAISY_CHECK_ARG(apart(o_rows), "paged_tree_attn: rows of o must not overlap");
+  const size_t need = daisy_paged_tree_attn_workspace_bytes(B, T, Hq, H, D, max_pages, page_size);
+  if (workspace == nullptr || workspace_bytes < need || !al16(workspace)) {
+    set_error("paged_tree_attn: workspace of %zu bytes, %zu needed on a 16-byte boundary", workspace_bytes, need);
+    return DAISY_ERR_WORKSPACE;
+  }
+  DAISY_CHECK_ARG((same_rows(o, o_rows, q, q_rows) || !share(o, o_rows, q, q_rows)) && !share(o, o_rows, k_pages, rows_of(k_pages_strides, num_pages, H, page_size, D)) &&
+                      !share(o, o_rows, v_pages, rows_of(v_pages_strides, num_pages, H, page_size, D)),
+                  "paged_tree_attn: o must be q or share no memory with it or with the pages");
+  const TreeSplit sp = tree_split(B, T, H, Hq / H, D, capacity);
+  TreeParams p = {};
+  p.q = (const uint16_t*)q; p.q_sb = pieces_of_16(q_strides[0], B); p.q_st = pieces_of_16(q_strides[1], T); p.q_sh = pieces_of_16(q_strides[2], Hq);
+  p.k = (const uint16_t*)k_pages; p.k_sp = pieces_of_16(k_pages_strides[0], num_pages); p.k_sh = pieces_of_16(k_pages_strides[1], H);
+  p.k_ss = pieces_of_16(k_pages_strides[2], page_size);
+  p.v = (const uint16_t*)v_pages; p.v_sp = pieces_of_16(v_pages_strides[0], num_pages); p.v_sh = pieces_of_16(v_pages_strides[1], H);
+  p.v_ss = pieces_of_16(v_pages_strides[2], page_size);
+  p.table = page_table; p.table_st = B == 1 ? 0 : (uint32_t)table_stride; p.max_pages = max_pages; p.num_pages = num_pages;
+  p.blocks_per_page = divisor(page_size / kBlock); p.capacity = (int)capacity;
+  p.lens = lens; p.nodes = nodes;
+  p.mask = (const uint32_t*)mask; p.mask_sb = B == 1 ? 0 : mask_strides[0]; p.mask_st = T == 1 ? 0 : mask_strides[1]; p.words = (T + 31) / 32;
+  p.o = (uint16_t*)o; p.o_f16 = o_is_f16;
+  p.o_sb = pieces_of_16(o_strides[0], B); p.o_st = pieces_of_16(o_strides[1], T); p.o_sh = pieces_of_16(o_strides[2], Hq);
+  p.split = (SplitUnit*)workspace;
+  p.part = (float*)((char*)workspace + (size_t)32 * sp.groups);
+  p.stat = (float2*)(p.part + (size_t)2 * sp.groups * sp.cols * D);
+  p.B = B; p.T = T; p.H = H; p.G = Hq / H; p.cols = sp.cols; p.window = window; p.groups = sp.groups; p.per_node = divisor(Hq / H);
+  p.scale_log2e = scale * kLog2e; p.status = status;
+  return cache_is_f16 ? tree_launch<true>(p, D, sp.NC, sp.lds, (hipStream_t)stream) : tree_launch<false>(p, D, sp.NC, sp.lds, (hipStream_t)stream);
+}

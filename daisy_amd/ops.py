@@ -5,7 +5,7 @@ validate, allocate outputs and pass raw pointers to ``libdaisy_hip.so``.
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple, Union
+from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
 
@@ -424,6 +424,8 @@ def raise_for_status(status: torch.Tensor) -> None:
         raise RuntimeError("a length or position of a paged call lies past what the page table has room for; its outputs are NaN")
     if bits & _lib.STATUS_PAGE_OUT_OF_RANGE:
         raise RuntimeError("a paged call needed a page table entry that names no page of the pool; its outputs are NaN")
+    if bits & _lib.STATUS_INDEX_OUT_OF_ORDER:
+        raise RuntimeError("an index of rows to be moved in a paged cache does not rise; its sequence is as it was")
 
 
 def kda_workspace_bytes(B: int, T: int, H: int, Dk: int, Dv: int, chunk: int = 64) -> int:
@@ -815,21 +817,22 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
                  cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None, eps: Optional[float] = None,
                  ve: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None,
                  k_out: Optional[torch.Tensor] = None, v_out: Optional[torch.Tensor] = None,
-                 status: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+                 status: Optional[torch.Tensor] = None, slots: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
     """Appends keys and values to a paged cache, preparing them (and the queries) on the way, in one launch.
 
     ``k``, ``v`` ``[N, H, D]`` and ``q [N, Hq, D]``: rows of the QKV projection for N tokens, bf16 or fp16, any token and head
     strides; ``positions`` int32 ``[N]``: each token's position in its sequence, ``rows`` int32 ``[N]``: its sequence, a row of
     ``page_table`` (``None``: token i belongs to sequence i, a decode step).  ``k_pages``, ``v_pages`` ``[pages, H, page_size, D]``, bf16 or fp16;
     position t of sequence s is row ``t % page_size`` of page ``page_table[s, t // page_size]`` (int32).  Page size: a multiple of 16;
-    D: 64, 128 or 256.
+    D: 64, 128 or 256.  ``slots`` int32 ``[N]``: the position whose place a token's rows take, where that is not the one it is rotated by (the nodes of a
+    drafted tree, see ``draft_tree``).
 
     ``eps``: RMS norm of q, k and v first (``None``: none).  ``cos``/``sin`` (fp32 ``[rows, D/2]``) rotate q and k at the token's position.
     ``ve [N, H, D]`` and ``gate`` (one fp32): v becomes ``gate * v + (1 - gate) * ve``.  Fp32 throughout, one rounding.
 
     Returns the prepared queries in the cache's dtype, or ``q_out`` (the cache's dtype or k's); ``None`` without ``q``.  ``k_out``, ``v_out``: ``[N, H, D]`` in k's
     dtype, receive k and v too (for the attention over a prompt); they and ``q_out`` may be k, v and q themselves, and share no memory with what else the
-    call reads or writes (rows beside each other in one buffer, with the same strides, are fine).  A token at a negative position is skipped: the cache and rows of buffers
+    call reads or writes (rows beside each other in one buffer, with the same strides, are fine).  A token at a negative position or slot is skipped: the cache and rows of buffers
     that the caller gave stay as they are, a query row of a tensor made here is zero.  Two tokens of one call must not share a place.
 
     The device reads positions, rows and table when the kernel runs.  One that leads to no page or past the rotary tables writes nothing to
@@ -837,10 +840,10 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     """
     if eps is not None and not eps >= 0.0:
         raise ValueError(f"eps must not be negative, got {eps}")
-    fast = _lib.native().paged_append(k, v, k_pages, v_pages, page_table, positions, rows, q, cos, sin, -1.0 if eps is None else eps, ve, gate, q_out, k_out, v_out, status)
+    fast = _lib.native().paged_append(k, v, k_pages, v_pages, page_table, positions, rows, q, cos, sin, -1.0 if eps is None else eps, ve, gate, q_out, k_out, v_out, status, slots)
     if fast is not None:
         return fast if fast is not True else None
-    dev = _lib.require_gpu(k, v, k_pages, v_pages, page_table, positions, rows, q, cos, sin, ve, gate, q_out, k_out, v_out, status)
+    dev = _lib.require_gpu(k, v, k_pages, v_pages, page_table, positions, rows, q, cos, sin, ve, gate, q_out, k_out, v_out, status, slots)
     _no_autograd("paged_append", k, v, q, ve, gate, k_pages, v_pages, q_out, k_out, v_out)
     _check_status(status)
     P, H, size, D = _check_pages(k_pages, v_pages, page_table)
@@ -854,6 +857,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
         _check_index("rows", rows, N)
     elif N > page_table.shape[0]:
         raise ValueError(f"without rows, token i belongs to sequence i: {N} tokens, {page_table.shape[0]} sequences")
+    if slots is not None:
+        _check_index("slots", slots, N)
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin must be given together")
     if cos is not None:
@@ -890,14 +895,14 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     st = lambda t: None if t is None else _lib.strides(t, d2)      # noqa: E731
     lib = _lib.load()
     with _lib.on_device(dev):
-        rc = lib.daisy_paged_append_fwd(
+        rc = lib.daisy_paged_append_slots_fwd(
             _lib.ptr(q), st(q), k.data_ptr(), st(k), v.data_ptr(), st(v), 1 if k.dtype == torch.float16 else 0, _lib.ptr(ve), st(ve), _lib.ptr(gate),
             _lib.ptr(cos), _lib.ptr(sin), 0 if cos is None else int(cos.shape[0]),
             k_pages.data_ptr(), _lib.strides(k_pages, d3), v_pages.data_ptr(), _lib.strides(v_pages, d3), 1 if k_pages.dtype == torch.float16 else 0,
-            page_table.data_ptr(), page_table.stride(0), page_table.shape[0], page_table.shape[1], P, size, positions.data_ptr(), _lib.ptr(rows),
+            page_table.data_ptr(), page_table.stride(0), page_table.shape[0], page_table.shape[1], P, size, positions.data_ptr(), _lib.ptr(rows), _lib.ptr(slots),
             _lib.ptr(q_out), st(q_out), 1 if q_out is not None and q_out.dtype == torch.float16 else 0, _lib.ptr(k_out), st(k_out), _lib.ptr(v_out), st(v_out), 1 if zero_skipped else 0,
             N, Hq, H, D, -1.0 if eps is None else float(eps), _lib.ptr(status), _lib.current_stream(dev))
-    _lib.check(rc, "daisy_paged_append_fwd")
+    _lib.check(rc, "daisy_paged_append_slots_fwd")
     return q_out
 
 
@@ -1067,3 +1072,246 @@ def pack_allowed(mask: torch.Tensor) -> torch.Tensor:
     bits = words.view(*mask.shape[:-1], -1, 32).to(torch.int64) << torch.arange(32, device=mask.device)
     total = bits.sum(dim=-1)
     return (total - ((total >> 31) << 32)).to(torch.int32)
+
+
+# ----------------------------------------------------------------------------------------------
+# several drafted tokens per sequence in one step over a paged cache
+# ----------------------------------------------------------------------------------------------
+MAX_TREE_NODES = _lib.MAX_TREE_NODES
+
+
+class DraftTree(NamedTuple):
+    """What a step over trees of drafted tokens needs to know of them (``draft_tree``)."""
+    mask: torch.Tensor           # int32 [B, T, ceil(T / 32)]: bit j % 32 of word j // 32 of node i: node i sees node j
+    positions: torch.Tensor      # int32 [B * T]: the position that each node is rotated by, -1 for nodes that there are not
+    slots: torch.Tensor          # int32 [B * T]: the position whose place in the cache it takes
+    rows: torch.Tensor           # int32 [B * T]: its sequence
+
+
+def _check_nodes(nodes: Optional[torch.Tensor], B: int, T: int) -> None:
+    if not 0 < T <= MAX_TREE_NODES:
+        raise ValueError(f"a tree must have 1 to {MAX_TREE_NODES} nodes, got {T}")
+    if nodes is not None:
+        _check_index("nodes", nodes, B)
+
+
+def _check_parents(parents: torch.Tensor, B: int, T: Optional[int] = None) -> int:
+    """Nodes of a tree."""
+    T = parents.shape[-1] if T is None and parents.dim() else T
+    if parents.dtype != torch.int32 or parents.shape not in ((T,), (B, T)) or (T > 1 and parents.stride(-1) != 1):
+        raise ValueError(f"parents must be int32 [T] or [{B}, T], contiguous in the last dim, got {tuple(parents.shape)} {parents.dtype}")
+    return T
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.dim() == 2 and t.shape[0] > 1 else 0
+
+
+def draft_tree(parents: torch.Tensor, lens: torch.Tensor, *, nodes: Optional[torch.Tensor] = None) -> DraftTree:
+    """What the nodes of trees of drafted tokens see, the positions that they are rotated by and the places that they take in a paged cache, in one launch.
+
+    ``parents`` int32 ``[B, T]`` (``[T]``: one tree for all; at most ``MAX_TREE_NODES``): the node that each comes from, ahead of it in the tree; anything else (-1, by
+    convention) for a root.  Node 0 is the root that the step's tokens follow (``verify_drafts``).  ``lens`` int32 ``[B]``: the positions of each sequence's context
+    (negative: a free slot, which has no nodes; ``PagedKVCache.positions``), ``nodes`` int32 ``[B]``: how many of its nodes there are (``None``: all).
+
+    Node i of sequence b takes the place of position ``lens[b] + i`` and is rotated as position ``lens[b]`` plus the number of its ancestors: what ``paged_append``
+    takes as ``slots`` and ``positions``, with ``rows``.  It sees the context, its ancestors and itself: ``mask``, for ``paged_tree_attention``.
+    """
+    if lens.dtype != torch.int32 or lens.dim() != 1 or not lens.is_contiguous():
+        raise ValueError(f"lens must be a contiguous int32 [B] tensor, got {tuple(lens.shape)} {lens.dtype}")
+    dev = _lib.require_gpu(parents, lens, nodes)
+    B = lens.shape[0]
+    T = _check_parents(parents, B)
+    _check_nodes(nodes, B, T)
+    W = (T + 31) // 32
+    room = torch.empty(B * T * (W + 3), dtype=torch.int32, device=dev)
+    mask, positions, slots, rows = room.split([B * T * W, B * T, B * T, B * T])
+    tree = DraftTree(mask.view(B, T, W), positions, slots, rows)
+    if B == 0:
+        return tree
+    lib = _lib.load()
+    with _lib.on_device(dev):
+        rc = lib.daisy_draft_tree_fwd(parents.data_ptr(), _row_stride(parents), lens.data_ptr(), _lib.ptr(nodes), mask.data_ptr(), positions.data_ptr(),
+                                      slots.data_ptr(), rows.data_ptr(), B, T, _lib.current_stream(dev))
+    _lib.check(rc, "daisy_draft_tree_fwd")
+    return tree
+
+
+def paged_tree_attention_workspace_bytes(B: int, T: int, Hq: int, H: int, D: int, max_pages: int, page_size: int) -> int:
+    return int(_lib.load().daisy_paged_tree_attn_workspace_bytes(B, T, Hq, H, D, max_pages, page_size))
+
+
+def paged_tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor, mask: torch.Tensor, *,
+                         nodes: Optional[torch.Tensor] = None, window: Optional[int] = None, scale: float = ATTN_SCALE, out: Optional[torch.Tensor] = None,
+                         workspace: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The attention of a tree of drafted tokens per sequence over a paged cache that holds their keys and values already (``paged_append`` with ``slots``).
+
+    ``q [B, T, Hq, D]`` in the cache's dtype (bf16 or fp16), any strides of the first three dims; pages and table as for ``paged_attention``.  ``lens`` int32 ``[B]``: the
+    positions of each context, ahead of its tree (negative: a free slot); node i lies at position ``lens[b] + i``.  Every node sees the context, itself and the nodes whose bits ``mask``
+    (int32 ``[B, T, ceil(T / 32)]``, see ``draft_tree``; any set of nodes) has; with ``window``, the last ``window`` of these, in the order of the cache.  ``nodes`` int32 ``[B]``: as for
+    ``draft_tree``; the rows of the others become zero.  Returns ``o [B, T, Hq, D]``, or ``out``, as ``paged_attention`` does.
+
+    Rows of a page that no node sees may hold anything.  A value that is not finite makes its channel NaN for the nodes that see it and the heads that share it; the others
+    do not feel it.
+
+    Lengths, nodes, mask and table are read when the kernels run.  ``workspace``: at least ``paged_tree_attention_workspace_bytes``, as for ``paged_attention``.  A tree that goes beyond the
+    table's room, or a page that is none, gives NaN for the heads of that sequence and raises a bit in ``status``.
+    """
+    if window is not None and window <= 0:
+        raise ValueError(f"window must be positive or None, got {window}")
+    dev = _lib.require_gpu(q, k_pages, v_pages, page_table, lens, mask, nodes, out, workspace, status)
+    _no_autograd("paged_tree_attention", q, k_pages, v_pages, out)
+    _check_status(status)
+    P, H, size, D = _check_pages(k_pages, v_pages, page_table)
+    _check_rows("q", q, 4, (k_pages.dtype,))
+    B, T, Hq = q.shape[:3]
+    if q.shape[3] != D or Hq == 0 or Hq % H != 0:
+        raise ValueError(f"q must be [B, T, a multiple of {H}, {D}] to fit the pages, got {tuple(q.shape)}")
+    if page_table.shape[0] < B:
+        raise ValueError(f"page_table has {page_table.shape[0]} rows for {B} sequences")
+    _check_index("lens", lens, B)
+    _check_nodes(nodes, B, T)
+    W = (T + 31) // 32
+    if mask.dtype != torch.int32 or mask.shape != (B, T, W) or (W > 1 and mask.stride(2) != 1):
+        raise ValueError(f"mask must be an int32 [{B}, {T}, {W}] tensor, contiguous in its last dim, got {tuple(mask.shape)} {mask.dtype}")
+    if out is None:
+        out = torch.empty((B, T, Hq, D), dtype=q.dtype, device=dev)
+    else:
+        _check_rows("out", out, 4, (torch.bfloat16,) if q.dtype == torch.bfloat16 else _HALF_TYPES)
+        if out.shape != q.shape:
+            raise ValueError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
+    if B == 0:
+        return out
+    lib = _lib.load()
+    max_pages, d3 = page_table.shape[1], (0, 1, 2)
+    need = int(lib.daisy_paged_tree_attn_workspace_bytes(B, T, Hq, H, D, max_pages, size))
+    if workspace is None or workspace.numel() * workspace.element_size() < need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    elif not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
+    with _lib.on_device(dev):
+        rc = lib.daisy_paged_tree_attn_fwd(
+            q.data_ptr(), _lib.strides(q, d3), k_pages.data_ptr(), _lib.strides(k_pages, d3), v_pages.data_ptr(), _lib.strides(v_pages, d3),
+            1 if q.dtype == torch.float16 else 0, page_table.data_ptr(), page_table.stride(0), max_pages, P, size, lens.data_ptr(), _lib.ptr(nodes),
+            mask.data_ptr(), _lib.strides(mask, (0, 1)), out.data_ptr(), _lib.strides(out, d3), 1 if out.dtype == torch.float16 else 0, B, T, Hq, H, D,
+            min(int(window), 2 ** 31 - 1) if window is not None else 0, float(scale), _lib.ptr(status),
+            workspace.data_ptr(), workspace.numel() * workspace.element_size(), _lib.current_stream(dev))
+    _lib.check(rc, "daisy_paged_tree_attn_fwd")
+    return out
+
+
+def verify_drafts_workspace_bytes(B: int, T: int, V: int) -> int:
+    return int(_lib.load().daisy_verify_workspace_bytes(B, T, V))
+
+
+def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, *, nodes: Optional[torch.Tensor] = None,
+                  temperature: Union[float, torch.Tensor] = 0.0, accept: Optional[torch.Tensor] = None, noise: Optional[torch.Tensor] = None,
+                  draft: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Which nodes of trees of drafted tokens the target's probabilities accept, and the token that follows them, in two launches that wait for nobody.
+
+    ``logits [B, T, V]`` (fp32, bf16 or fp16; any strides of the first two dims): row u says what may follow node u, ``p = softmax(logits[b, u] / temperature)``, -inf what may not (what
+    ``process_logits`` or a filter has left).  ``tokens`` int64 or int32 ``[B, T]``: the nodes' tokens, of which node 0's is taken; ``parents``, ``nodes``: as for ``draft_tree``.
+    ``temperature``: a number or fp32 ``[B]``; zero: the likeliest token alone is accepted, and follows (of equal ones the lowest).
+
+    From node 0 on, the children of the node are tried in their order.  Child c, with token y, is accepted where ``accept[b, c] * (1 - what rejected children took of p) < p(y)``; its p is
+    taken where it is rejected (a token that an earlier child had has none left).  Where none is accepted, the token that follows is drawn from what is left: the
+    largest ``log p(v) + noise[b, v]``.  With ``draft`` (fp32 ``[B, T, V]``: row u the probabilities q that the children of u were drawn from, independently) each rejection
+    makes p ``max(p - q, 0)``, normalised (p as it was at first where that leaves nothing), and a child is accepted where ``accept[b, c] * q(y) < p(y)``.  Either way tokens come out as if drawn
+    from p one by one.  ``accept`` fp32 ``[B, T]`` in [0, 1), ``noise`` fp32 ``[B, V]``, Gumbel (``generate.gumbel_noise``): the random numbers; not needed at temperature zero.
+
+    Returns ``path`` int32 ``[B, T]`` (the accepted nodes from node 0 on, -1 behind them: an ``index`` for ``paged_move``), ``counts`` int32 ``[B]`` (how many) and the tokens that follow, int64 ``[B]``;
+    -1 where nothing may: a row that is -inf throughout beside its children, a row with NaN or +inf, no nodes.  Sums are held in 64 bits and do not depend on any order of atomics.
+    ``workspace``: at least ``verify_drafts_workspace_bytes``, whatever it holds, for one call at a time; ``None``: a tensor made for the call.
+    """
+    rows = temperature if isinstance(temperature, torch.Tensor) else None
+    dev = _lib.require_gpu(logits, tokens, parents, nodes, rows, accept, noise, draft, workspace)
+    _no_autograd("verify_drafts", logits, rows, accept, noise, draft)
+    if logits.dtype not in _LOGITS_TYPES:
+        raise TypeError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")
+    if logits.dim() != 3 or logits.shape[2] == 0 or (logits.shape[2] > 1 and logits.stride(2) != 1):
+        raise ValueError(f"logits must be [B, T, V], contiguous in the last dim, got {tuple(logits.shape)}")
+    B, T, V = logits.shape
+    _check_nodes(nodes, B, T)
+    _check_parents(parents, B, T)
+    if tokens.dtype not in (torch.int64, torch.int32) or tokens.shape != (B, T) or (T > 1 and tokens.stride(1) != 1):
+        raise ValueError(f"tokens must be int64 or int32 [{B}, {T}], contiguous in the last dim, got {tuple(tokens.shape)} {tokens.dtype}")
+    if rows is not None:
+        if rows.dtype != torch.float32 or rows.shape != (B,) or not rows.is_contiguous():
+            raise ValueError(f"temperature must be a number or a contiguous fp32 [{B}] tensor, got {tuple(rows.shape)} {rows.dtype}")
+    elif not 0.0 <= temperature < float("inf"):
+        raise ValueError(f"temperature must not be negative, and finite, got {temperature}")
+    if (rows is not None or temperature > 0.0) and (accept is None or noise is None):
+        raise ValueError("a temperature needs accept and noise")
+    for name, t, shape in (("accept", accept, (B, T)), ("noise", noise, (B, V)), ("draft", draft, (B, T, V))):
+        if t is not None and (t.dtype != torch.float32 or t.shape != shape or (shape[-1] > 1 and t.stride(-1) != 1)):
+            raise ValueError(f"{name} must be fp32 {list(shape)}, contiguous in the last dim, got {tuple(t.shape)} {t.dtype}")
+    path = torch.empty(B, T, dtype=torch.int32, device=dev)
+    counts = torch.empty(B, dtype=torch.int32, device=dev)
+    following = torch.empty(B, dtype=torch.int64, device=dev)
+    if B == 0:
+        return path, counts, following
+    lib = _lib.load()
+    need = int(lib.daisy_verify_workspace_bytes(B, T, V))
+    if workspace is None or workspace.numel() * workspace.element_size() < need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    elif not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
+    with _lib.on_device(dev):
+        rc = lib.daisy_verify_fwd(
+            logits.data_ptr(), _lib.strides(logits, (0, 1)), _LOGITS_TYPES[logits.dtype], tokens.data_ptr(), tokens.stride(0), 1 if tokens.dtype == torch.int64 else 0,
+            parents.data_ptr(), _row_stride(parents), _lib.ptr(nodes), _lib.ptr(rows), 0.0 if rows is not None else float(temperature),
+            _lib.ptr(accept), 0 if accept is None else accept.stride(0), _lib.ptr(noise), 0 if noise is None else noise.stride(0),
+            _lib.ptr(draft), None if draft is None else _lib.strides(draft, (0, 1)), path.data_ptr(), counts.data_ptr(), following.data_ptr(), B, T, V,
+            workspace.data_ptr(), workspace.numel() * workspace.element_size(), _lib.current_stream(dev))
+    _lib.check(rc, "daisy_verify_fwd")
+    return path, counts, following
+
+
+def paged_move(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, starts: torch.Tensor, counts: torch.Tensor, *, rows: Optional[int] = None,
+               index: Optional[torch.Tensor] = None, sources: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> None:
+    """Rows of a paged cache to other places of it, in all layers, in one launch.
+
+    ``k_pages``, ``v_pages`` ``[L, pages, H, page_size, D]`` (``PagedKVCache.k``, ``.v``; or one layer without the first dim), ``page_table`` as for ``paged_append``.  For
+    sequence b, a row of the table, and ``i < counts[b]`` (int32 ``[B]``): position ``starts[b] + i`` (int32 ``[B]``; negative: nothing to do) becomes what position ``starts[b] + index[b, i]`` of
+    sequence ``sources[b]`` held.  ``index`` int32 ``[B, M]`` (at most M rows of a sequence; ``None``: i itself, at most ``rows`` of them), ``sources`` int32 ``[B]`` (``None``: b itself).
+
+    With ``index=path, counts=counts`` of ``verify_drafts`` and the context's lengths as ``starts``, the accepted nodes of a tree become the context's next positions.  With ``sources``
+    a sequence gets another one's rows into pages of its own (a fork's last page).
+
+    An index must rise from 0 or more on, so that a sequence can be closed up in place; what other sequences of the call read or write is the caller's to keep apart.  The device
+    reads all of it when the kernel runs: an index that does not rise leaves its sequence as it was, a row that leads to no page is left out, and either raises a bit in
+    ``status``.
+    """
+    dev = _lib.require_gpu(k_pages, v_pages, page_table, starts, counts, index, sources, status)
+    _no_autograd("paged_move", k_pages, v_pages)
+    _check_status(status)
+    if k_pages.dim() == 4 and v_pages.dim() == 4:
+        k_pages, v_pages = k_pages[None], v_pages[None]
+    if k_pages.dim() != 5 or v_pages.shape != k_pages.shape or 0 in k_pages.shape:
+        raise ValueError(f"k_pages, v_pages must be [L, pages, H, page_size, D] or [pages, H, page_size, D], got {tuple(k_pages.shape)}, {tuple(v_pages.shape)}")
+    P, H, size, D = _check_pages(k_pages[0], v_pages[0], page_table)
+    B = starts.shape[0] if starts.dim() else 0
+    _check_index("starts", starts, B)
+    _check_index("counts", counts, B)
+    if B > page_table.shape[0]:
+        raise ValueError(f"page_table has {page_table.shape[0]} rows for {B} sequences")
+    if sources is not None:
+        _check_index("sources", sources, B)
+    if index is not None:
+        if index.dtype != torch.int32 or index.dim() != 2 or index.shape[0] != B or (index.shape[1] > 1 and index.stride(1) != 1):
+            raise ValueError(f"index must be an int32 [{B}, M] tensor, contiguous in its last dim, got {tuple(index.shape)} {index.dtype}")
+        rows = index.shape[1]
+    elif sources is None:
+        raise ValueError("paged_move needs an index or sources: without them every row stays where it is")
+    elif rows is None or rows < 0:
+        raise ValueError(f"without an index, rows must say how many a sequence has at most, got {rows}")
+    if B == 0 or rows == 0:
+        return
+    d4 = (0, 1, 2, 3)
+    lib = _lib.load()
+    with _lib.on_device(dev):
+        rc = lib.daisy_paged_move_fwd(
+            k_pages.data_ptr(), _lib.strides(k_pages, d4), v_pages.data_ptr(), _lib.strides(v_pages, d4), page_table.data_ptr(), page_table.stride(0),
+            page_table.shape[0], page_table.shape[1], P, size, starts.data_ptr(), counts.data_ptr(), _lib.ptr(index), 0 if index is None else index.stride(0),
+            _lib.ptr(sources), B, rows, k_pages.shape[0], H, D, _lib.ptr(status), _lib.current_stream(dev))
+    _lib.check(rc, "daisy_paged_move_fwd")

@@ -38,6 +38,7 @@ extern "C" {
 #define DAISY_STATUS_POSITION_PAST_TABLES 1   /* a position read from device memory lies past the rotation tables */
 #define DAISY_STATUS_LENGTH_PAST_PAGES 2      /* a length or position lies past the pages that the page table has room for, or names a row it does not have */
 #define DAISY_STATUS_PAGE_OUT_OF_RANGE 4      /* a page table entry that was needed names no page of the pool */
+#define DAISY_STATUS_INDEX_OUT_OF_ORDER 8     /* an index of rows to be moved does not rise */
 
 /* Text of the last error raised on this thread ("" if none). */
 const char* daisy_last_error(void);
@@ -498,6 +499,23 @@ int daisy_paged_append_fwd(const void* q, const int64_t* q_strides, const void* 
                            void* k_out, const int64_t* k_out_strides, void* v_out, const int64_t* v_out_strides, int zero_skipped,
                            int N, int Hq, int H, int D, float eps, int32_t* status, void* stream);
 
+/* daisy_paged_append_slots_fwd: the same, except that token i's rows go to the place of position slots[i] of its sequence, while it is rotated
+ * by positions[i] (slots NULL: by its place): the nodes of a tree of drafted tokens lie behind one another and share positions.  A token
+ * whose slot is negative is skipped, too.
+ */
+int daisy_paged_append_slots_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                                 const void* v, const int64_t* v_strides, int in_is_f16,
+                                 const void* ve, const int64_t* ve_strides, const float* gate,
+                                 const float* cos, const float* sin, int table_rows,
+                                 void* k_pages, const int64_t* k_pages_strides,
+                                 void* v_pages, const int64_t* v_pages_strides, int cache_is_f16,
+                                 const int32_t* page_table, int64_t table_stride, int n_seq, int max_pages,
+                                 int num_pages, int page_size,
+                                 const int32_t* positions, const int32_t* rows, const int32_t* slots,
+                                 void* q_out, const int64_t* q_out_strides, int q_out_is_f16,
+                                 void* k_out, const int64_t* k_out_strides, void* v_out, const int64_t* v_out_strides, int zero_skipped,
+                                 int N, int Hq, int H, int D, float eps, int32_t* status, void* stream);
+
 /* daisy_paged_attn_fwd: the attention of one new token per sequence, whose key and value are in the cache already:
  *   o[b, h] = sum_t softmax_t(scale <q[b, h], k_t>) v_t,  max(0, lens[b] - window) <= t < lens[b]
  * (window <= 0: all positions), the key head of query head h being h / (Hq / H); a length of zero or less gives
@@ -514,6 +532,50 @@ int daisy_paged_attn_fwd(const void* q, const int64_t* q_strides,
                          const int32_t* lens, void* o, const int64_t* o_strides, int o_is_f16,
                          int B, int Hq, int H, int D, int window, float scale, int32_t* status,
                          void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Several drafted tokens per sequence in one step over a paged cache: a tree of up to 256 nodes for each, node 0 its root, every node behind
+ * its parent.  Node i of sequence b lies at place lens[b] + i of the cache, behind the lens[b] positions of the context, and
+ * is the position lens[b] + (number of its ancestors).  nodes: int32 [B] or NULL, the nodes of each tree (NULL: T); a sequence
+ * with a negative length has none.
+ *
+ * daisy_draft_tree_fwd: parents int32 [B, T] with a row stride (0: one tree for all); a parent that is not one of the nodes ahead of its node: a root.
+ *   mask [B, T, ceil(T / 32)]: bit j % 32 of word j / 32 of node i, whether node j is i or an ancestor of it;
+ *   positions, slots, rows [B * T]: what daisy_paged_append_slots_fwd takes; -1 (mask: 0) for nodes that there are not.
+ */
+int daisy_draft_tree_fwd(const int32_t* parents, int64_t parents_stride, const int32_t* lens, const int32_t* nodes,
+                         int32_t* mask, int32_t* positions, int32_t* slots, int32_t* rows, int B, int T, void* stream);
+
+/* daisy_paged_tree_attn_fwd: the attention of the nodes over the cache, which holds their keys and values already:
+ *   o[b, i, h] = sum_t softmax_t(scale <q[b, i, h], k_t>) v_t
+ * over the places t < lens[b] and lens[b] + j for the bits j of node i's mask (int32 [B, T, ceil(T / 32)], strides {batch, node}), i itself among
+ * them whatever its bit; with window > 0 the last `window` of these, in the order of the places.  q, o: [B, T, Hq, D] with {batch, node, head} strides; types, pages and table
+ * as for daisy_paged_attn_fwd.  Rows of o for nodes that there are not become zero.  Rows of a page that no node sees may hold anything; a value that is
+ * not finite makes its channel NaN for the nodes that see it, and for those alone.  workspace: daisy_paged_tree_attn_workspace_bytes(...) bytes, 16-byte aligned, of no
+ * other call that may run at the same time.
+ */
+size_t daisy_paged_tree_attn_workspace_bytes(int B, int T, int Hq, int H, int D, int max_pages, int page_size);
+int daisy_paged_tree_attn_fwd(const void* q, const int64_t* q_strides,
+                              const void* k_pages, const int64_t* k_pages_strides,
+                              const void* v_pages, const int64_t* v_pages_strides, int cache_is_f16,
+                              const int32_t* page_table, int64_t table_stride, int max_pages, int num_pages, int page_size,
+                              const int32_t* lens, const int32_t* nodes, const int32_t* mask, const int64_t* mask_strides,
+                              void* o, const int64_t* o_strides, int o_is_f16,
+                              int B, int T, int Hq, int H, int D, int window, float scale, int32_t* status,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
+/* daisy_paged_move_fwd: rows of the cache to other places, in L layers at once (k_pages, v_pages [L, num_pages, H, page_size, D], strides
+ * {layer, page, head, row}): for b < B and i < counts[b] (rows at most)
+ *   place starts[b] + i of sequence b = place starts[b] + index[b, i] of sequence sources[b],
+ * index int32 [B, rows] with a row stride (NULL: i itself), sources int32 [B] (NULL: b itself); one of the two is needed.  An index must
+ * rise, from 0 or more on: with that, a sequence can be closed up in place.  Otherwise nothing of its sequence moves and DAISY_STATUS_INDEX_OUT_OF_ORDER
+ * is raised.  No place is written that another sequence of the call reads or writes.  A negative start: nothing to move.  Rows that lead to no page are
+ * left out, with a bit in *status.
+ */
+int daisy_paged_move_fwd(void* k_pages, const int64_t* k_pages_strides, void* v_pages, const int64_t* v_pages_strides,
+                         const int32_t* page_table, int64_t table_stride, int n_seq, int max_pages, int num_pages, int page_size,
+                         const int32_t* starts, const int32_t* counts, const int32_t* index, int64_t index_stride, const int32_t* sources,
+                         int B, int rows, int L, int H, int D, int32_t* status, void* stream);
 
 /* ---------------------------------------------------------------------------
  * Penalties for repeated tokens, biases and grammar masks on the logits of a batch, in one pass: the
@@ -541,6 +603,38 @@ int daisy_logits_process_fwd(const void* x, int64_t x_stride, void* y, int64_t y
                              const float* frequency_rows, float frequency, float half_life, float cap,
                              const float* bias, int64_t bias_stride, const int32_t* allowed, int64_t allowed_stride,
                              int B, int V, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Which of the drafted tokens the target's probabilities accept, from given random numbers, and the token that follows them.  The reference's
+ * generator draws one token at a time (inference/generate.py:13-58); this is its draw for a tree of drafted tokens whose scores one step has given.
+ * Row u of a sequence's scores says what may follow node u: p_u = softmax(logits[b, u] / temperature).  From the root, node 0, on the children of a node u are
+ * tried in their order.  Without `draft` child c with token y is accepted where
+ *   accept[b, c] * r < e(y),  e = exp((logits[b, u] - max) / temperature),  r = the sum of e over the tokens that no child rejected before had;
+ * a token that an earlier child had is rejected.  Where all are rejected, or there are none, the token that follows is the largest
+ * logits[b, u, v] / temperature + noise[b, v] of the tokens v that no child has (Gumbel noise: a draw).  With `draft`, the probabilities q_u = draft[b, u] that the children of u
+ * were drawn from, independently of each other, p = p_u becomes max(p - q_u, 0) / sum with each rejection (p_u again where nothing is left of it), c is
+ * accepted where accept[b, c] * q_u(y) < p(y), and the token that follows is the largest log p(v) + noise[b, v].  temperature 0: a child is accepted where it has
+ * the largest score's token, which follows otherwise (of equal scores the lowest token's).
+ * logits     : [B, T, V], type 0 = fp32, 1 = bf16, 2 = fp16, strides {sequence, node}; -inf: a token that may not follow.
+ * tokens     : int32 or int64 (tokens_are_int64) [B, T] with a row stride; a token outside 0 .. V - 1 is no candidate.
+ * parents, nodes: as for daisy_draft_tree_fwd; a node that does not come from node 0 is never accepted.
+ * temperature: a number, or, where temperature_rows is given, fp32 [B] (zero or less: the largest score).
+ * accept     : fp32 [B, T] with a row stride, in [0, 1);  noise: fp32 [B, V] with a row stride, finite;  both may be NULL where temperature is the number 0.
+ * draft      : fp32 [B, T, V], strides {sequence, node}, or NULL.
+ * path       : int32 [B, T], the accepted nodes from node 0 on, -1 behind them;  counts: int32 [B], how many;  next: int64 [B], the token that follows, -1
+ *              where nothing may: no score above -inf beside the children's, a score that is NaN or +inf, no nodes.
+ * The results share no memory with what the call reads.  workspace: daisy_verify_workspace_bytes(...) bytes, 16-byte aligned, of no other call that may
+ * run at the same time.
+ */
+size_t daisy_verify_workspace_bytes(int B, int T, int V);
+int daisy_verify_fwd(const void* logits, const int64_t* logits_strides, int type,
+                     const void* tokens, int64_t tokens_stride, int tokens_are_int64,
+                     const int32_t* parents, int64_t parents_stride, const int32_t* nodes,
+                     const float* temperature_rows, float temperature,
+                     const float* accept, int64_t accept_stride, const float* noise, int64_t noise_stride,
+                     const float* draft, const int64_t* draft_strides,
+                     int32_t* path, int32_t* counts, int64_t* next, int B, int T, int V,
+                     void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
