@@ -937,6 +937,171 @@ PyObject* py_process_logits(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- several drafted tokens per sequence ------------------------------------------------------------------------------
+struct Strides4 {
+  int64_t s[4];
+  explicit Strides4(const Tensor& t) : s{t.stride(0), t.stride(1), t.stride(2), t.stride(3)} {}
+};
+bool last_dense(const Tensor& t) { return t.size(-1) <= 1 || t.stride(-1) == 1; }
+// int32 [B, T], or [T] for all
+bool tree_parents(const Tensor& t, int64_t B, int64_t T, int dev) {
+  return on_gpu(t, dev) && t.scalar_type() == at::kInt && (t.dim() == 1 || (t.dim() == 2 && t.size(0) == B)) && t.size(-1) == T && last_dense(t);
+}
+int64_t shared_stride(const Tensor& t) { return t.dim() == 2 && t.size(0) > 1 ? t.stride(0) : 0; }
+
+// draft_tree(parents, lens, nodes) -> mask, positions, slots, rows
+PyObject* py_draft_tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (intercepted() || n != 3 || !is_tensor(a[0]) || !is_tensor(a[1]) || !tensor_or_none(a[2])) return none();
+  const Tensor &parents = THPVariable_Unpack(a[0]), &lens = THPVariable_Unpack(a[1]);
+  const Tensor* nodes = opt_tensor(a[2]);
+  const int dev = gpu_of(lens);
+  if (dev < 0 || lens.dim() != 1 || parents.dim() < 1) return none();
+  const int64_t B = lens.size(0), T = parents.size(-1), W = (T + 31) / 32;
+  if (B < 1 || B > INT32_MAX || T < 1 || T > 256 || !int32_row(lens, B, dev) || !tree_parents(parents, B, T, dev) || (nodes && !int32_row(*nodes, B, dev))) return none();
+  Unlocked unlocked;
+  Tensor room = empty({B * T * (W + 3)}, at::kInt, lens);
+  int32_t* at = (int32_t*)ptr(room);
+  const int64_t rows = B * T;
+  if (daisy_draft_tree_fwd((const int32_t*)ptr(parents), shared_stride(parents), (const int32_t*)ptr(lens), (const int32_t*)ptr(nodes), at, at + rows * W, at + rows * (W + 1),
+                           at + rows * (W + 2), (int)B, (int)T, stream_of(dev)) != DAISY_OK) return none();
+  const Tensor parts[4] = {room.as_strided({B, T, W}, {T * W, W, 1}, 0), room.as_strided({rows}, {1}, rows * W), room.as_strided({rows}, {1}, rows * (W + 1)),
+                           room.as_strided({rows}, {1}, rows * (W + 2))};
+  unlocked.end();
+  PyObject* res = PyTuple_New(4);
+  for (int i = 0; i < 4; ++i) PyTuple_SET_ITEM(res, i, wrap(parts[i]));
+  return res;
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_tree_attention(q, k_pages, v_pages, page_table, lens, mask, nodes, window (0: all), scale, out, workspace, status) -> out
+PyObject* py_paged_tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (intercepted() || n != 12) return none();
+  for (int i = 0; i < 6; ++i)
+    if (!is_tensor(a[i])) return none();
+  for (int i : {6, 9, 10, 11})
+    if (!tensor_or_none(a[i])) return none();
+  const Tensor &q = THPVariable_Unpack(a[0]), &kp = THPVariable_Unpack(a[1]), &vp = THPVariable_Unpack(a[2]), &table = THPVariable_Unpack(a[3]), &lens = THPVariable_Unpack(a[4]);
+  const Tensor &mask = THPVariable_Unpack(a[5]);
+  const Tensor *nodes = opt_tensor(a[6]), *out = opt_tensor(a[9]), *ws = opt_tensor(a[10]), *status = opt_tensor(a[11]);
+  const long window = PyLong_AsLong(a[7]);
+  const float scale = (float)PyFloat_AsDouble(a[8]);
+  if (PyErr_Occurred()) { PyErr_Clear(); return none(); }
+  const int dev = gpu_of(q);
+  if (dev < 0 || window < 0 || !paged_cache(kp, vp, table, dev) || !rows_half(q, 4, dev) || !same_type(q, kp)) return none();
+  const int64_t B = q.size(0), T = q.size(1), Hq = q.size(2), H = kp.size(1), D = kp.size(3);
+  if (B < 1 || B > INT32_MAX || T < 1 || T > 256 || Hq < 1 || Hq > INT32_MAX || Hq % H != 0 || q.size(3) != D || table.size(0) < B || !int32_row(lens, B, dev)) return none();
+  if (!on_gpu(mask, dev) || mask.scalar_type() != at::kInt || mask.dim() != 3 || mask.size(0) != B || mask.size(1) != T || mask.size(2) != (T + 31) / 32 || !last_dense(mask)) return none();
+  if (nodes && !int32_row(*nodes, B, dev)) return none();
+  if (out && !(rows_half(*out, 4, dev) && (same_type(*out, q) || bf16(*out)) && out->sizes() == q.sizes())) return none();
+  if ((status && !one_of(*status, at::kInt, dev)) || (ws && !(on_gpu(*ws, dev) && ws->is_contiguous())) || needs_autograd({&q, &kp, &vp, out})) return none();
+  const int max_pages = (int)std::min<int64_t>(table.size(1), INT32_MAX), size = (int)std::min<int64_t>(kp.size(2), INT32_MAX);
+  const size_t need = daisy_paged_tree_attn_workspace_bytes((int)B, (int)T, (int)Hq, (int)H, (int)D, max_pages, size);
+  if (need == 0) return none();
+  Unlocked unlocked;
+  Tensor o = out ? *out : empty(q.sizes(), q.scalar_type(), q);
+  Tensor w = ws && (size_t)(ws->numel() * ws->element_size()) >= need ? *ws : empty({(int64_t)need}, at::kByte, q);
+  const Strides3 qs(q), os(o), ks(kp), vs(vp);
+  const Strides2 ms(mask);
+  const int rc = daisy_paged_tree_attn_fwd(ptr(q), qs.s, ptr(kp), ks.s, ptr(vp), vs.s, is_f16(kp), (const int32_t*)ptr(table), table.stride(0), max_pages, (int)kp.size(0), size,
+                                           (const int32_t*)ptr(lens), (const int32_t*)ptr(nodes), (const int32_t*)ptr(mask), ms.s, ptr(o), os.s, is_f16(o), (int)B, (int)T, (int)Hq,
+                                           (int)H, (int)D, (int)std::min<long>(window, INT32_MAX), scale, (int32_t*)ptr(status), ptr(w), (size_t)(w.numel() * w.element_size()),
+                                           stream_of(dev));
+  if (rc != DAISY_OK) return none();
+  unlocked.end();
+  return wrap(o);
+  END_HANDLE_TH_ERRORS
+}
+
+// verify_drafts(logits, tokens, parents, nodes, temperature (a float or a tensor), accept, noise, draft, workspace) -> path, counts, next
+PyObject* py_verify_drafts(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (intercepted() || n != 9) return none();
+  for (int i = 0; i < 3; ++i)
+    if (!is_tensor(a[i])) return none();
+  for (int i : {3, 5, 6, 7, 8})
+    if (!tensor_or_none(a[i])) return none();
+  const Tensor &x = THPVariable_Unpack(a[0]), &tokens = THPVariable_Unpack(a[1]), &parents = THPVariable_Unpack(a[2]);
+  const Tensor *nodes = opt_tensor(a[3]), *rows = nullptr, *accept = opt_tensor(a[5]), *noise = opt_tensor(a[6]), *draft = opt_tensor(a[7]), *ws = opt_tensor(a[8]);
+  double temperature = 0.0;
+  if (is_tensor(a[4])) rows = &THPVariable_Unpack(a[4]);
+  else temperature = PyFloat_AsDouble(a[4]);
+  if (PyErr_Occurred()) { PyErr_Clear(); return none(); }
+  const int dev = gpu_of(x);
+  const at::ScalarType type = x.scalar_type();
+  if (dev < 0 || x.dim() != 3 || x.numel() == 0 || !last_dense(x) || !(type == at::kFloat || type == at::kBFloat16 || type == at::kHalf)) return none();
+  const int64_t B = x.size(0), T = x.size(1), V = x.size(2);
+  if (B > INT32_MAX || T > 256 || V > INT32_MAX || !tree_parents(parents, B, T, dev) || (nodes && !int32_row(*nodes, B, dev))) return none();
+  if (!on_gpu(tokens, dev) || !(tokens.scalar_type() == at::kLong || tokens.scalar_type() == at::kInt) || tokens.dim() != 2 || tokens.size(0) != B || tokens.size(1) != T ||
+      !last_dense(tokens)) return none();
+  if (rows && !(on_gpu(*rows, dev) && f32(*rows) && rows->dim() == 1 && rows->size(0) == B && rows->is_contiguous())) return none();
+  auto numbers = [&](const Tensor* t, at::IntArrayRef shape) { return !t || (on_gpu(*t, dev) && f32(*t) && t->sizes() == shape && last_dense(*t)); };
+  if (!numbers(accept, {B, T}) || !numbers(noise, {B, V}) || !numbers(draft, {B, T, V})) return none();
+  if ((ws && !(on_gpu(*ws, dev) && ws->is_contiguous())) || needs_autograd({&x, rows, accept, noise, draft})) return none();
+  const size_t need = daisy_verify_workspace_bytes((int)B, (int)T, (int)V);
+  if (need == 0) return none();
+  Unlocked unlocked;
+  // (the three results and the workspace in one allocation; the results keep it as long as they live, so a large one is by itself)
+  const int64_t ints = B * (T + 1), result_bytes = (8 * B + 4 * ints + 15) / 16 * 16;
+  const bool own = !(ws && (size_t)(ws->numel() * ws->element_size()) >= need), small = own && need <= 64 * 1024;
+  Tensor room = empty({(result_bytes + (small ? (int64_t)need : 0)) / 8 + 1}, at::kLong, x);
+  Tensor w = own ? (small ? room : empty({(int64_t)need}, at::kByte, x)) : *ws;
+  char* base = (char*)ptr(room);
+  void* work = small ? base + result_bytes : ptr(w);
+  const size_t work_bytes = small ? need : (size_t)(w.numel() * w.element_size());
+  const Strides2 xs(x);
+  const Strides2 ds = draft ? Strides2(*draft) : Strides2();
+  int32_t* counts = (int32_t*)(base + 8 * B);
+  const int rc = daisy_verify_fwd(ptr(x), xs.s, type == at::kFloat ? 0 : type == at::kBFloat16 ? 1 : 2, ptr(tokens), tokens.stride(0), tokens.scalar_type() == at::kLong,
+                                  (const int32_t*)ptr(parents), shared_stride(parents), (const int32_t*)ptr(nodes), (const float*)ptr(rows), (float)temperature,
+                                  (const float*)ptr(accept), accept ? accept->stride(0) : 0, (const float*)ptr(noise), noise ? noise->stride(0) : 0, (const float*)ptr(draft),
+                                  draft ? ds.s : nullptr, counts + B, counts, (int64_t*)base, (int)B, (int)T, (int)V, work, work_bytes, stream_of(dev));
+  if (rc != DAISY_OK) return none();
+  const Tensor as_ints = room.view(at::kInt);
+  const Tensor parts[3] = {as_ints.as_strided({B, T}, {T, 1}, 3 * B), as_ints.as_strided({B}, {1}, 2 * B), room.as_strided({B}, {1}, 0)};
+  unlocked.end();
+  PyObject* res = PyTuple_New(3);
+  for (int i = 0; i < 3; ++i) PyTuple_SET_ITEM(res, i, wrap(parts[i]));
+  return res;
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_move(k_pages, v_pages, page_table, starts, counts, rows (-1: the index's), index, sources, status) -> True
+PyObject* py_paged_move(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (intercepted() || n != 9) return none();
+  for (int i = 0; i < 5; ++i)
+    if (!is_tensor(a[i])) return none();
+  for (int i : {6, 7, 8})
+    if (!tensor_or_none(a[i])) return none();
+  const Tensor &kp = THPVariable_Unpack(a[0]), &vp = THPVariable_Unpack(a[1]), &table = THPVariable_Unpack(a[2]), &starts = THPVariable_Unpack(a[3]), &counts = THPVariable_Unpack(a[4]);
+  const Tensor *index = opt_tensor(a[6]), *sources = opt_tensor(a[7]), *status = opt_tensor(a[8]);
+  const long asked = PyLong_AsLong(a[5]);
+  if (PyErr_Occurred()) { PyErr_Clear(); return none(); }
+  const int dev = gpu_of(kp);
+  if (dev < 0 || !rows_half(kp, 5, dev) || !rows_half(vp, 5, dev) || !same_type(kp, vp) || kp.sizes() != vp.sizes() || kp.numel() == 0) return none();
+  for (int d = 0; d < 3; ++d)
+    if (kp.size(d) > INT32_MAX) return none();
+  if (!on_gpu(table, dev) || table.scalar_type() != at::kInt || table.dim() != 2 || table.size(1) == 0 || table.stride(1) != 1 || table.size(0) > INT32_MAX) return none();
+  const int64_t B = starts.dim() == 1 ? starts.size(0) : 0;
+  if (B < 1 || B > table.size(0) || !int32_row(starts, B, dev) || !int32_row(counts, B, dev) || (sources && !int32_row(*sources, B, dev))) return none();
+  if (index && !(on_gpu(*index, dev) && index->scalar_type() == at::kInt && index->dim() == 2 && index->size(0) == B && last_dense(*index))) return none();
+  if (!index && (!sources || asked < 1)) return none();
+  const int64_t rows = index ? index->size(1) : asked;
+  if (rows < 1 || rows > INT32_MAX || (status && !one_of(*status, at::kInt, dev)) || needs_autograd({&kp, &vp})) return none();
+  Unlocked unlocked;
+  const Strides4 ks(kp), vs(vp);
+  const int rc = daisy_paged_move_fwd(ptr(kp), ks.s, ptr(vp), vs.s, (const int32_t*)ptr(table), table.stride(0), (int)table.size(0), (int)std::min<int64_t>(table.size(1), INT32_MAX),
+                                      (int)kp.size(1), (int)std::min<int64_t>(kp.size(3), INT32_MAX), (const int32_t*)ptr(starts), (const int32_t*)ptr(counts),
+                                      (const int32_t*)ptr(index), index ? index->stride(0) : 0, (const int32_t*)ptr(sources), (int)B, (int)rows, (int)kp.size(0), (int)kp.size(2),
+                                      (int)std::min<int64_t>(kp.size(4), INT32_MAX), (int32_t*)ptr(status), stream_of(dev));
+  if (rc != DAISY_OK) return none();
+  unlocked.end();
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
 template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
 PyObject* call(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   PyObject* r = F(self, a, n);
@@ -946,6 +1111,7 @@ PyObject* call(PyObject* self, PyObject* const* a, Py_ssize_t n) {
 #define FAST(name) {#name, (PyCFunction)(void (*)(void))call<py_##name>, METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {FAST(linear), FAST(norm), FAST(linears), FAST(prefill_attention), FAST(layer_prefill), FAST(layer_step), FAST(kda_chunk), FAST(kda_layer),
                           FAST(paged_append), FAST(paged_attention), FAST(paged_layer_step), FAST(process_logits),
+                          FAST(draft_tree), FAST(paged_tree_attention), FAST(verify_drafts), FAST(paged_move),
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

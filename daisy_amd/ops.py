@@ -1117,6 +1117,9 @@ def draft_tree(parents: torch.Tensor, lens: torch.Tensor, *, nodes: Optional[tor
     Node i of sequence b takes the place of position ``lens[b] + i`` and is rotated as position ``lens[b]`` plus the number of its ancestors: what ``paged_append``
     takes as ``slots`` and ``positions``, with ``rows``.  It sees the context, its ancestors and itself: ``mask``, for ``paged_tree_attention``.
     """
+    fast = _lib.native().draft_tree(parents, lens, nodes)
+    if fast is not None:
+        return DraftTree(*fast)
     if lens.dtype != torch.int32 or lens.dim() != 1 or not lens.is_contiguous():
         raise ValueError(f"lens must be a contiguous int32 [B] tensor, got {tuple(lens.shape)} {lens.dtype}")
     dev = _lib.require_gpu(parents, lens, nodes)
@@ -1159,6 +1162,9 @@ def paged_tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.
     """
     if window is not None and window <= 0:
         raise ValueError(f"window must be positive or None, got {window}")
+    fast = _lib.native().paged_tree_attention(q, k_pages, v_pages, page_table, lens, mask, nodes, 0 if window is None else window, scale, out, workspace, status)
+    if fast is not None:
+        return fast
     dev = _lib.require_gpu(q, k_pages, v_pages, page_table, lens, mask, nodes, out, workspace, status)
     _no_autograd("paged_tree_attention", q, k_pages, v_pages, out)
     _check_status(status)
@@ -1223,6 +1229,9 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Ten
     -1 where nothing may: a row that is -inf throughout beside its children, a row with NaN or +inf, no nodes.  Sums are held in 64 bits and do not depend on any order of atomics.
     ``workspace``: at least ``verify_drafts_workspace_bytes``, whatever it holds, for one call at a time; ``None``: a tensor made for the call.
     """
+    fast = _lib.native().verify_drafts(logits, tokens, parents, nodes, temperature, accept, noise, draft, workspace)
+    if fast is not None:
+        return fast
     rows = temperature if isinstance(temperature, torch.Tensor) else None
     dev = _lib.require_gpu(logits, tokens, parents, nodes, rows, accept, noise, draft, workspace)
     _no_autograd("verify_drafts", logits, rows, accept, noise, draft)
@@ -1282,6 +1291,8 @@ def paged_move(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.T
     reads all of it when the kernel runs: an index that does not rise leaves its sequence as it was, a row that leads to no page is left out, and either raises a bit in
     ``status``.
     """
+    if _lib.native().paged_move(k_pages, v_pages, page_table, starts, counts, -1 if rows is None else rows, index, sources, status) is not None:
+        return
     dev = _lib.require_gpu(k_pages, v_pages, page_table, starts, counts, index, sources, status)
     _no_autograd("paged_move", k_pages, v_pages)
     _check_status(status)
