@@ -121,7 +121,7 @@ template <bool F16> __device__ __forceinline__ u32x2 pack_out(const TreeParams& 
 
 // A sequence: its context, its nodes, the places that some node sees, [lo, hi), the tiles that they lie in and the blocks of columns.
 struct Extent { int len, nodes, lo, hi, first, tiles, blocks; bool past; };
-template <int NC> __device__ __forceinline__ Extent extent(const TreeParams& p, int len, int nodes) {
+template <int COLS> __device__ __forceinline__ Extent extent(const TreeParams& p, int len, int nodes) {
   Extent e;
   e.nodes = len < 0 ? 0 : min(max(nodes, 0), p.T);
   e.past = len > p.capacity - e.nodes;
@@ -131,7 +131,7 @@ template <int NC> __device__ __forceinline__ Extent extent(const TreeParams& p, 
   e.lo = min(e.lo, max(e.hi - 1, 0));
   e.first = (unsigned)e.lo / kTile;
   e.tiles = e.nodes > 0 ? (int)((unsigned)(e.hi + kTile - 1) / kTile) - e.first : 0;
-  e.blocks = (int)((unsigned)(e.nodes * p.G + 16 * NC - 1) / (16 * NC));
+  e.blocks = (int)((unsigned)(e.nodes * p.G + COLS - 1) / COLS);
   return e;
 }
 struct Sequence { int len, nodes; };
@@ -140,24 +140,112 @@ __device__ __forceinline__ Sequence sequence(const TreeParams& p, int b) {
   const int len = p.lens[at], nodes = p.nodes != nullptr ? p.nodes[at] : p.T;
   return Sequence{b < p.B ? len : -1, nodes};
 }
-template <int NC> __device__ __forceinline__ int weight_of(const TreeParams& p, const Sequence& s) {
-  const Extent e = extent<NC>(p, s.len, s.nodes);
+template <int COLS> __device__ __forceinline__ int weight_of(const TreeParams& p, const Sequence& s) {
+  const Extent e = extent<COLS>(p, s.len, s.nodes);
   return e.tiles * e.blocks;
+}
+
+// The tiles of all units one behind the other, blocks of COLS columns: which unit one of them belongs to.  Every wavefront has one of these and asks for rising numbers.
+struct Unit { Extent e; int b, h, col0, cols, off, count, n_tiles; };
+template <int COLS> struct Deal {
+  int own, own_upto, per_lane;      // lane i: the tiles (of a key head each) of sequences from i * per_lane on; with those ahead
+  // 64 sequences from `base` on, one a lane; up to 64 are all there
+  int base, before, weight, upto, chunk;
+  Sequence seq;
+  // All tiles.  (For every wavefront of a workgroup at once: many sequences are summed up together.)
+  __device__ __forceinline__ int begin(const TreeParams& p, int wv, int lane) {
+    own = 0;
+    per_lane = (p.B + 63) >> 6;
+    Sequence s4[4];
+    if (per_lane <= 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s4[i] = sequence(p, lane * per_lane + min(i, per_lane - 1));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) own += i < per_lane ? weight_of<COLS>(p, s4[i]) : 0;
+    } else {
+      // 64 at a time, the wavefronts in turn: in a row, where lanes by themselves are a cache line or more apart
+      __shared__ int sums[64];
+      per_lane = (p.B + 4095) >> 12 << 6;
+      const int used = (int)((unsigned)(p.B + per_lane - 1) / (unsigned)per_lane), waves = blockDim.x / 64;
+      for (int i = wv; i < used; i += waves) {
+        int tiles = 0;
+        for (int j = 0; j < per_lane; j += 64) tiles += weight_of<COLS>(p, sequence(p, i * per_lane + j + lane));
+        const int sum = wave_scan(tiles);
+        if (lane == 63) sums[i] = sum;
+      }
+      __syncthreads();
+      own = lane < used ? sums[lane] : 0;
+      s4[0] = Sequence{-1, 0};
+    }
+    own_upto = wave_scan(own);
+    base = before = 0;
+    weight = own;
+    upto = own_upto;
+    seq = s4[0];
+    const int all = __builtin_amdgcn_readlane(own_upto, 63);
+    chunk = per_lane == 1 ? all : -1;
+    return all * p.H;
+  }
+  // Straight to where tile x lies.
+  __device__ __forceinline__ void go_to(const TreeParams& p, int x) {
+    if (per_lane == 1) return;
+    const int first = 63 - __builtin_clzll(__ballot(own > 0 && (own_upto - own) * p.H <= x) | 1);
+    base = first * per_lane;
+    before = __builtin_amdgcn_readlane(own_upto - own, first);
+  }
+  // The unit of tile x, and how much of it comes ahead of x_end.  (More than 64 lengths are read twice: somebody who changes them meanwhile gets wrong results, but every index
+  // stays inside the call's tensors and x goes on.)
+  __device__ __forceinline__ Unit unit(const TreeParams& p, int x, int x_end, int lane) {
+    while (chunk < 0 || (x >= (before + chunk) * p.H && base < p.B)) {
+      if (chunk >= 0) { before += chunk; base += 64; }
+      seq = sequence(p, base + lane);
+      weight = weight_of<COLS>(p, seq);
+      upto = wave_scan(weight);
+      chunk = __builtin_amdgcn_readlane(upto, 63);
+    }
+    const uint64_t here = __ballot(weight > 0 && (before + upto - weight) * p.H <= x);
+    const int bl = 63 - __builtin_clzll(here | 1);
+    Unit u;
+    u.b = min(base + bl, p.B - 1);
+    u.e = extent<COLS>(p, __builtin_amdgcn_readlane(seq.len, bl), __builtin_amdgcn_readlane(seq.nodes, bl));
+    u.n_tiles = max(u.e.tiles, 1);
+    const int blocks = max(u.e.blocks, 1);
+    const int rel = x - (before + __builtin_amdgcn_readlane(upto - weight, bl)) * p.H;
+    const int unit = (int)min((unsigned)rel / (unsigned)u.n_tiles, (unsigned)(p.H * blocks - 1));
+    u.off = min(max(rel - unit * u.n_tiles, 0), u.n_tiles - 1);
+    u.count = max(min(u.n_tiles - u.off, x_end - x), 1);
+    u.h = (int)((unsigned)unit / (unsigned)blocks);
+    u.col0 = (unit - u.h * blocks) * COLS;
+    u.cols = min(max(u.e.nodes * p.G, 1) - u.col0, COLS);
+    return u;
+  }
+};
+
+// Rows of nodes that there are not, the sequences dealt out to the workgroups one by one.
+template <int D> __device__ __forceinline__ void zero_the_rest(const TreeParams& p, int group) {
+  for (int s = group; s < p.B; s += p.groups) {
+    const Extent e = extent<1>(p, p.lens[s], p.nodes != nullptr ? p.nodes[s] : p.T);
+    const int per_node = p.H * p.G * (D / 8);
+    for (int i = threadIdx.x + e.nodes * per_node; i < p.T * per_node; i += blockDim.x) {
+      const int row = i / (D / 8);
+      *reinterpret_cast<u32x4*>(row_of_o(p, s, Query{row / (p.H * p.G), row % (p.H * p.G)}) + i % (D / 8) * 8) = u32x4{0, 0, 0, 0};
+    }
+  }
 }
 
 // How many tiles a wavefront takes: no fewer than the workgroups there are can do, and more (a lane tries each number up to twice as many) where that
 // takes a thirty-second or more off the most loaded of the compute units.
-__device__ __forceinline__ int share_of(const TreeParams& p, int total, int lane) {
-  if (total <= 4 * kCus) return 1;
-  const int least = (int)((unsigned)(total + 4 * p.groups - 1) / (unsigned)(4 * p.groups)), more = min(lane, least), share = least + more;
+template <int RUNS> __device__ __forceinline__ int share_of(const TreeParams& p, int total, int lane) {      // RUNS: of a workgroup
+  if (total <= RUNS * kCus) return 1;
+  const int least = (int)((unsigned)(total + RUNS * p.groups - 1) / (unsigned)(RUNS * p.groups)), more = min(lane, least), share = least + more;
   // (in fp32: one more or less only makes another choice, the same one in every wavefront)
-  const float groups = ceilf((float)total * __builtin_amdgcn_rcpf((float)(4 * share)) - 0.001f);
+  const float groups = ceilf((float)total * __builtin_amdgcn_rcpf((float)(RUNS * share)) - 0.001f);
   const int load = (int)ceilf(groups * (1.f / kCus)) * share;
   return least + (wave_min((more == 0 ? load - load / 32 : load) * 64 + more) & 63);
 }
 
 // Workgroups per compute unit, a wavefront of each per SIMD: what the registers leave room for.
-constexpr int tree_groups_per_cu(int D, int NC) { return D == 64 ? (NC == 1 ? 4 : NC == 2 ? 3 : 2) : D == 128 ? (NC == 1 ? 3 : NC == 2 ? 2 : 1) : 1; }
+constexpr int tree_groups_per_cu(int D, int NC) { return D == 64 ? (NC == 1 ? 4 : 3) : D == 128 ? (NC == 1 ? 3 : 2) : 1; }
 constexpr int tree_row(int D) { return D + 4; }      // floats of a partial sum's row in the LDS
 
 // Bit i of a mask that begins `from` bits before its first word (or behind it), ones ahead of it: 32 of them.
@@ -168,6 +256,45 @@ __device__ __forceinline__ uint32_t bits_from(const uint32_t* row, int words, in
   const uint32_t lo = at < 0 ? ~0u : at < words ? a : 0, hi = at + 1 < words ? b : 0;
   return __builtin_amdgcn_alignbit(hi, lo, from & 31);
 }
+
+// The first place that node `node`, whose mask is `row`, sees in a window: the last `window` of the context and of its bits.
+__device__ __forceinline__ int first_place(const TreeParams& p, const Extent& e, const uint32_t* row, int node) {
+  auto word = [&](int w) {
+    const uint32_t bits = row[w] | (node >> 5 == w ? 1u << (node & 31) : 0);
+    const int there = e.nodes - 32 * w;      // bits of nodes that there are
+    return there >= 32 ? bits : there <= 0 ? 0 : bits & ((1u << there) - 1);
+  };
+  int seen = 0;
+  for (int w = 0; w < p.words; ++w) seen += __popc(word(w));
+  const int drop = e.len + seen - p.window;
+  if (drop <= e.len) return max(drop, 0);
+  // nodes, too: as many of them as are too many behind the context
+  int left = drop - e.len, w = 0;
+  uint32_t bits = word(0);
+  while (w + 1 < p.words && left >= __popc(bits)) { left -= __popc(bits); bits = word(++w); }
+  for (; left > 0; --left) bits &= bits - 1;
+  return e.len + 32 * w + (bits != 0 ? __builtin_ctz(bits) : 31);
+}
+// The keys of the tile at place `tile` that the node sees, lo its first place.
+__device__ __forceinline__ uint32_t visible(const TreeParams& p, const Extent& e, const uint32_t* row, int node, int lo, int tile) {
+  uint32_t bits = bits_from(row, p.words, tile - e.len);
+  const int self = e.len + node - tile, low = lo - tile, end = e.hi - tile;      // (end: at least one)
+  bits |= (unsigned)self < 32u ? 1u << self : 0;
+  bits &= end >= 32 ? ~0u : (1u << max(end, 0)) - 1;
+  return low >= 32 ? 0 : low <= 0 ? bits : bits & (~0u << low);
+}
+
+// Pairs of bf16 or fp16 numbers: all bits of those that are not finite; the larger magnitudes; ones; all bits of the halves whose bits 0 and 1 of `bits` are set.
+template <bool F16> __device__ __forceinline__ uint32_t not_finite(uint32_t pair) {
+  constexpr uint32_t kInf = F16 ? 0x7c00u : 0x7f80u;
+  return ((pair & kInf) == kInf ? 0xffffu : 0) | ((pair & kInf << 16) == kInf << 16 ? 0xffff0000u : 0);
+}
+__device__ __forceinline__ uint32_t larger_halves(uint32_t a, uint32_t b) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b & 0x7fff7fffu)));
+}
+template <bool F16> __device__ __forceinline__ uint32_t ones() { return F16 ? 0x3c003c00u : 0x3f803f80u; }
+__device__ __forceinline__ uint32_t halves(uint32_t bits) { return (bits & 1 ? 0xffffu : 0) | (bits & 2 ? 0xffff0000u : 0); }
 
 template <int D, bool F16, int NC>
 __global__ __launch_bounds__(256, tree_groups_per_cu(D, NC)) void tree_attn_kernel(TreeParams p) {
@@ -186,71 +313,23 @@ __global__ __launch_bounds__(256, tree_groups_per_cu(D, NC)) void tree_attn_kern
   __shared__ OpenUnits open_units[4];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = blockIdx.x, wave = group * 4 + wv;
   const int n = lane & 15, c = lane >> 4;
-  // Tiles of the sequences (of one key head each): lane i has the sum of those from i * per_lane on, which gives the total and where a run begins.
-  int own = 0, per_lane = (p.B + 63) >> 6;
-  Sequence s4[4];
-  if (per_lane <= 4) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s4[i] = sequence(p, lane * per_lane + min(i, per_lane - 1));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) own += i < per_lane ? weight_of<NC>(p, s4[i]) : 0;
-  } else {
-    // 64 at a time, the wavefronts in turn: in a row, where lanes by themselves are a cache line or more apart
-    __shared__ int sums[64];
-    per_lane = (p.B + 4095) >> 12 << 6;
-    const int used = (int)((unsigned)(p.B + per_lane - 1) / (unsigned)per_lane);
-    for (int i = wv; i < used; i += 4) {
-      int tiles = 0;
-      for (int j = 0; j < per_lane; j += 64) tiles += weight_of<NC>(p, sequence(p, i * per_lane + j + lane));
-      const int sum = wave_scan(tiles);
-      if (lane == 63) sums[i] = sum;
-    }
-    __syncthreads();
-    own = lane < used ? sums[lane] : 0;
-    s4[0] = Sequence{-1, 0};
-  }
-  const int own_upto = wave_scan(own);
-  const int total = __builtin_amdgcn_readlane(own_upto, 63) * p.H;
-  const int share = share_of(p, total, lane);
+  Deal<16 * NC> deal;
+  const int total = deal.begin(p, wv, lane), share = share_of<4>(p, total, lane);
   int x = (int)min((unsigned)wave * (unsigned)share, (unsigned)total);      // (the product is less than twice the total, 2^30 at most, and a share for each wavefront)
   const int x_end = min(x + share, total);
   OpenUnits mine = {0, 0, 0};
   SplitUnit beyond = {-1, 0, 0, 0, 0, 0};
+  if (x < x_end) deal.go_to(p, x);
 
   const uint32_t k_row = p.k_ss * 16, v_row = p.v_ss * 16;      // bytes, fewer than 2^24
-  // 64 sequences from `base` on, one a lane; up to 64 are all there
-  int base = 0, before = 0, weight = own, upto = own_upto, chunk = per_lane == 1 ? __builtin_amdgcn_readlane(own_upto, 63) : -1;
-  Sequence seq = s4[0];
-  if (per_lane > 1 && x < x_end) {
-    const int first = 63 - __builtin_clzll(__ballot(own > 0 && (own_upto - own) * p.H <= x));
-    base = first * per_lane;
-    before = __builtin_amdgcn_readlane(own_upto - own, first);
-  }
   f32x4 acc[NC][J];
   float m[NC], l[NC];
   int b = 0, h = 0, col0 = 0, cols = 0;      // the unit: sequence, key head, first column and number of columns
   while (x < x_end) {
-    // ---- the unit that x lies in.  (More than 64 lengths are read twice: somebody who changes them meanwhile gets wrong results, but every index below
-    // stays inside the call's tensors and x goes on.)
-    while (chunk < 0 || (x >= (before + chunk) * p.H && base < p.B)) {
-      if (chunk >= 0) { before += chunk; base += 64; }
-      seq = sequence(p, base + lane);
-      weight = weight_of<NC>(p, seq);
-      upto = wave_scan(weight);
-      chunk = __builtin_amdgcn_readlane(upto, 63);
-    }
-    const uint64_t here = __ballot(weight > 0 && (before + upto - weight) * p.H <= x);
-    const int bl = 63 - __builtin_clzll(here | 1);
-    b = min(base + bl, p.B - 1);
-    const Extent e = extent<NC>(p, __builtin_amdgcn_readlane(seq.len, bl), __builtin_amdgcn_readlane(seq.nodes, bl));
-    const int n_tiles = max(e.tiles, 1), blocks = max(e.blocks, 1);
-    const int rel = x - (before + __builtin_amdgcn_readlane(upto - weight, bl)) * p.H;
-    const int unit = (int)min((unsigned)rel / (unsigned)n_tiles, (unsigned)(p.H * blocks - 1)), off = min(max(rel - unit * n_tiles, 0), n_tiles - 1);
-    const int count = max(min(n_tiles - off, x_end - x), 1);
-    h = (int)((unsigned)unit / (unsigned)blocks);
-    col0 = (unit - h * blocks) * 16 * NC;
-    const int all_cols = max(e.nodes * p.G, 1);
-    cols = min(all_cols - col0, 16 * NC);
+    const Unit at = deal.unit(p, x, x_end, lane);
+    const Extent& e = at.e;
+    const int off = at.off, count = at.count, n_tiles = at.n_tiles, all_cols = max(e.nodes * p.G, 1);
+    b = at.b; h = at.h; col0 = at.col0; cols = at.cols;
 
     // ---- its queries: columns past the last one repeat it
     u32x4 qf[NC][KS];
@@ -266,25 +345,8 @@ __global__ __launch_bounds__(256, tree_groups_per_cu(D, NC)) void tree_attn_kern
     }
     const uint32_t* mask = p.mask + b * p.mask_sb;
     if (p.window > 0) {
-      for (int t = 0; t < NC; ++t) {
-        auto word = [&](int w) {
-          uint32_t bits = mask[node[t] * p.mask_st + w];
-          bits |= node[t] >> 5 == w ? 1u << (node[t] & 31) : 0;
-          const int there = e.nodes - 32 * w;      // bits of nodes that there are
-          return there >= 32 ? bits : there <= 0 ? 0 : bits & ((1u << there) - 1);
-        };
-        int seen = 0;
-        for (int w = 0; w < p.words; ++w) seen += __popc(word(w));
-        const int drop = e.len + seen - p.window;
-        lo[t] = max(drop, 0);
-        if (drop > e.len) {      // nodes, too: as many of them as are too many behind the context
-          int left = drop - e.len, w = 0;
-          uint32_t bits = word(0);
-          while (w + 1 < p.words && left >= __popc(bits)) { left -= __popc(bits); bits = word(++w); }
-          for (; left > 0; --left) bits &= bits - 1;
-          lo[t] = e.len + 32 * w + (bits != 0 ? __builtin_ctz(bits) : 31);
-        }
-      }
+#pragma unroll
+      for (int t = 0; t < NC; ++t) lo[t] = first_place(p, e, mask + node[t] * p.mask_st, node[t]);
     }
 #pragma unroll
     for (int t = 0; t < NC; ++t) {
@@ -389,15 +451,8 @@ __global__ __launch_bounds__(256, tree_groups_per_cu(D, NC)) void tree_attn_kern
       bool dirty = false;
       uint32_t vis[NC];
       if (edge) {
-        const int end = e.hi - tile;      // (at least one)
 #pragma unroll
-        for (int t = 0; t < NC; ++t) {
-          uint32_t bits = bits_from(mask + node[t] * p.mask_st, p.words, tile - e.len);
-          const int self = e.len + node[t] - tile, low = lo[t] - tile;
-          bits |= (unsigned)self < 32u ? 1u << self : 0;
-          bits &= end >= 32 ? ~0u : (1u << max(end, 0)) - 1;
-          vis[t] = low >= 32 ? 0 : low <= 0 ? bits : bits & (~0u << low);
-        }
+        for (int t = 0; t < NC; ++t) vis[t] = visible(p, e, mask + node[t] * p.mask_st, node[t], lo[t], tile);
         uint32_t most = 0;
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
@@ -406,12 +461,10 @@ __global__ __launch_bounds__(256, tree_groups_per_cu(D, NC)) void tree_attn_kern
 #pragma unroll
           for (int d = 0; d < VD; ++d) {
             vr[r][d] = there ? vr[r][d] : 0;
-            typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-            most = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, most), __builtin_bit_cast(u16x2, vr[r][d] & 0x7fff7fffu)));
+            most = larger_halves(most, vr[r][d]);
           }
         }
-        constexpr uint32_t kInf = F16 ? 0x7c00u : 0x7f80u;
-        dirty = __any((most & 0xffffu) >= kInf || (most >> 16) >= kInf);
+        dirty = __any(not_finite<F16>(most) != 0);
       }
       // ---- probabilities, in two parts, the second what the rounding of the first has lost: the result is as if they had not been rounded
       u32x4 pf[NC], pl[NC];
@@ -448,36 +501,39 @@ __global__ __launch_bounds__(256, tree_groups_per_cu(D, NC)) void tree_attn_kern
         for (int r = 0; r < 8; ++r) f[r] = s[r] - f[r];
         pl[t] = pack8_as<F16>(f);
       }
-      // ---- O^T += V^T P^T
-#pragma unroll
-      for (int j = 0; j < J; ++j) {
+      // ---- values that are not finite leave the product; who sees one of a channel gets NaN there
+      auto v_operand = [&](int j) {
         const int d = (j / W) * (W / 2) + (j % W) / 2;
         u32x4 vf;
 #pragma unroll
         for (int t = 0; t < 4; ++t) vf[t] = __builtin_amdgcn_perm(vr[2 * t + 1][d], vr[2 * t][d], (j & 1) ? 0x07060302u : 0x05040100u);
-        if (dirty) {
-          // Values that are not finite leave the product; who sees one of a channel gets NaN there.
-          constexpr uint32_t kInf = F16 ? 0x7c00u : 0x7f80u, kOne = F16 ? 0x3c00u : 0x3f80u;
-          u32x4 odd;
+        return vf;
+      };
+      if (dirty) {
 #pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            const uint32_t low = (vf[t] & kInf) == kInf ? 0xffffu : 0, high = (vf[t] >> 16 & kInf) == kInf ? 0xffff0000u : 0;
-            odd[t] = (low | high) & (kOne | kOne << 16);
-            vf[t] &= ~(low | high);
-          }
+        for (int j = 0; j < J; ++j) {
+          u32x4 odd = v_operand(j);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) odd[r] = not_finite<F16>(odd[r]) & ones<F16>();
 #pragma unroll
           for (int t = 0; t < NC; ++t) {
             u32x4 sees;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const uint32_t pair = vis[t] >> (4 * c + (2 * r & 3) + (2 * r & 4) * 4);
-              sees[r] = (pair & 1 ? kOne : 0) | (pair & 2 ? kOne << 16 : 0);
-            }
+            for (int r = 0; r < 4; ++r) sees[r] = halves(vis[t] >> (4 * c + (2 * r & 3) + (2 * r & 4) * 4)) & ones<F16>();
             const f32x4 met = mfma<F16>(odd, sees, f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
             for (int i4 = 0; i4 < 4; ++i4) acc[t][j][i4] = met[i4] > 0.f ? __builtin_nanf("") : acc[t][j][i4];
           }
         }
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+#pragma unroll
+          for (int d = 0; d < VD; ++d) vr[r][d] &= ~not_finite<F16>(vr[r][d]);
+      }
+      // ---- O^T += V^T P^T
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const u32x4 vf = v_operand(j);
 #pragma unroll
         for (int t = 0; t < NC; ++t) {
           acc[t][j] = mfma<F16>(vf, pf[t], acc[t][j]);
@@ -546,15 +602,7 @@ __global__ __launch_bounds__(256, tree_groups_per_cu(D, NC)) void tree_attn_kern
   // ---- what the wavefronts have left open: chains of the same unit, from where one of them broke off (or the workgroup began) on
   if (lane == 0) open_units[wv] = mine;
   if (lane == 0 && wv == 3) p.split[group] = beyond;
-  // (nodes that there are not: sequences dealt out one by one)
-  for (int s = group; s < p.B; s += p.groups) {
-    const Extent e = extent<NC>(p, p.lens[s], p.nodes != nullptr ? p.nodes[s] : p.T);
-    const int per_node = p.H * p.G * (D / 8);
-    for (int i = threadIdx.x + e.nodes * per_node; i < p.T * per_node; i += 256) {
-      const int row = i / (D / 8);
-      *reinterpret_cast<u32x4*>(row_of_o(p, s, Query{row / (p.H * p.G), row % (p.H * p.G)}) + i % (D / 8) * 8) = u32x4{0, 0, 0, 0};
-    }
-  }
+  zero_the_rest<D>(p, group);
   __syncthreads();
   const int flags = open_units[lane & 3].flags;      // (bit w of each: wavefront w's)
   const int through = (int)__ballot(flags & kGoesThrough);
@@ -621,19 +669,296 @@ __global__ __launch_bounds__(256, tree_groups_per_cu(D, NC)) void tree_attn_kern
   }
 }
 
+// The same for more columns than a wavefront takes: a workgroup of NW wavefronts, 32 columns each, one unit's tiles at a time.  K and V come into the LDS by copies of
+// 16 bytes a lane, the next tile's while this one is computed, and all wavefronts read them there: V's through transposing reads.  Products are 32x32x16: a lane
+// has a column and 16 of a tile's keys, 8 (r / 4) + 4 (lane / 32) + r % 4.  Partial sums of units that the run begins or ends in the middle of go to the second kernel.
+//
+// 16-byte pieces of a row are swizzled by the row, so that the reads of an operand fall into different banks: K's by all of the row, V's, of which a transposing read takes four
+// rows at once, by two bits.
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) const uint16_t* lds_u16_ptr;
+__device__ __forceinline__ u32x2 read_transposed(lds_u16_ptr at) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)at));
+}
+template <bool F16> __device__ __forceinline__ f32x16 mfma32(const u32x4& a, const u32x4& b, const f32x16& c) {
+  if constexpr (F16) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+constexpr int wide_waves_per_simd(int D) { return D == 256 ? 1 : 2; }
+constexpr int wide_stages(int D, int NW) { return NW == 2 ? 2 : D == 256 ? 3 : 4; }      // tiles in the LDS: the one that is computed and those on their way
+
+template <int D, bool F16, int NW>
+__global__ __launch_bounds__(64 * NW, wide_waves_per_simd(D)) void tree_wide_kernel(TreeParams p) {
+  constexpr int NS = D / 16, NDT = D / 32, CPR = D / 8;      // steps of the first product; 32-row pieces of the second one's result; pieces of a row
+  constexpr int RPL = 64 / CPR, COPIES = kTile / RPL;        // rows of a copy, copies of a tile
+  constexpr int TILE = kTile * D;                            // elements
+  constexpr int COLS = 32 * NW;
+  constexpr float kHead = F16 ? 9.f : 0.f, kLimit = F16 ? 15.f : 8.f;
+  auto swz_k = [](int r) { return D == 64 ? (r >> 1) & 7 : r & 15; };
+  auto swz_v = [](int r) { return D == 64 ? 4 * ((r >> 1) & 1) : 4 * (r & 3); };
+  constexpr int STAGES = wide_stages(D, NW);
+  extern __shared__ __attribute__((aligned(1024))) char staged[];      // [STAGES][K, V][TILE]
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // (neighbouring runs, which read the same keys, to one XCD: workgroups are dealt to the eight of them in turn)
+  const int group = (p.groups & 7) == 0 ? (int)((blockIdx.x & 7) * (p.groups >> 3) + (blockIdx.x >> 3)) : (int)blockIdx.x;
+  const int n = lane & 31, c = lane >> 5;
+  Deal<COLS> deal;
+  const int total = deal.begin(p, wv, lane), share = share_of<1>(p, total, lane);
+  int x = (int)min((unsigned)group * (unsigned)share, (unsigned)total);
+  const int x_end = min(x + share, total);
+  SplitUnit beyond = {-1, 0, 0, 0, 0, 0};
+  if (x < x_end) deal.go_to(p, x);
+
+  const int k_row = p.k_ss * 16, v_row = p.v_ss * 16;      // bytes
+  const int ld_row = lane / CPR, ld_pos = lane % CPR;
+  const uint32_t k_a0 = lds_address(staged) + 2 * (n * D + 8 * (c ^ swz_k(n)));
+  uint32_t v_a0;
+  {
+    // a block of 16 lanes takes 16 channels of four keys: lane i of it addresses key i / 4, channels 4 (i % 4) .. + 3
+    const int i16 = lane & 15, row = 4 * c + (i16 >> 2), piece = 2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1);
+    v_a0 = lds_address(staged) + 2 * TILE + 2 * (row * D + 8 * (piece ^ swz_v(row)) + 4 * (i16 & 1));
+  }
+  while (x < x_end) {
+    const Unit at = deal.unit(p, x, x_end, lane);
+    const Extent& e = at.e;
+    const int b = at.b, h = at.h, off = at.off, count = at.count, all_cols = max(e.nodes * p.G, 1);
+
+    // ---- copies
+    const int32_t* row = p.table + product(b, p.table_st);
+    const int blk_lo = (unsigned)e.lo / kBlock, blk_hi = max(e.hi - 1, 0) / kBlock;
+    bool bad = e.past;
+    int id = 0, in = 0;
+    auto pages_from = [&](int block) {
+      const int blk = min(max(block + lane, blk_lo), blk_hi);      // (blocks outside the range: read, but not used)
+      const Quotient page = divide((uint32_t)blk, p.blocks_per_page);
+      in = page.rest;
+      id = row[page.of];
+      const bool out = (unsigned)id >= (unsigned)p.num_pages;
+      bad |= out;
+      id = out ? 0 : id;
+    };
+    const char* kh = reinterpret_cast<const char*>(p.k) + 16 * product(h, p.k_sh);
+    const char* vh = reinterpret_cast<const char*>(p.v) + 16 * product(h, p.v_sh);
+    const int tile0 = e.first + off;
+    auto copy_tile = [&](int i, int buf) {
+      const int tile = (tile0 + i) * kTile;
+      const bool whole = tile >= e.lo && tile + kTile <= e.hi;
+#pragma unroll
+      for (int j0 = 0; j0 < COPIES; j0 += NW) {
+        const int j = j0 + wv;
+        if (COPIES % NW != 0 && j >= COPIES) break;
+        const int half = RPL * j >> 4, r = RPL * j + ld_row;
+        const int pg = __builtin_amdgcn_readlane(id, 2 * (i & 31) + half), slot = __builtin_amdgcn_readlane(in, 2 * (i & 31) + half) * kBlock;
+        // a row of the half, or where that is outside the range, another one that is
+        const int first = tile + half * kBlock, own = r & 15;
+        const int from = whole ? own : min(max(own, min(max(e.lo - first, 0), kBlock - 1)), min(max(e.hi - 1 - first, 0), kBlock - 1));
+        copy16_to_lds_async((const uint16_t*)(kh + 16 * (product(pg, p.k_sp) + product(slot, p.k_ss))), from * k_row + 16 * (ld_pos ^ swz_k(r)),
+                            lds_address(staged) + 4 * TILE * buf + 1024 * j);
+        copy16_to_lds_async((const uint16_t*)(vh + 16 * (product(pg, p.v_sp) + product(slot, p.v_ss))), from * v_row + 16 * (ld_pos ^ swz_v(r)),
+                            lds_address(staged) + 2 * TILE + 4 * TILE * buf + 1024 * j);
+      }
+    };
+    pages_from(2 * tile0);
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i)
+      if (i < count) copy_tile(i, i);
+
+    // ---- this lane's query: columns past the last one repeat it
+    const int col = 32 * wv + n;
+    const bool mine = col < at.cols;
+    const Query of = query_of(p, h, min(at.col0 + col, all_cols - 1));
+    const uint32_t* mask = p.mask + b * p.mask_sb + of.node * p.mask_st;
+    u32x4 qf[NS];
+    {
+      const uint16_t* src = p.q + 8 * (product(b, p.q_sb) + product(of.node, p.q_st) + product(of.head, p.q_sh) + c);
+#pragma unroll
+      for (int s = 0; s < NS; ++s) qf[s] = *reinterpret_cast<const u32x4*>(src + 16 * s);
+    }
+    const int lo = p.window > 0 ? first_place(p, e, mask, of.node) : 0;
+    const int lo_edge = p.window > 0 ? e.len - p.window + e.nodes : 0;
+    f32x16 acc[NDT];
+#pragma unroll
+    for (int t = 0; t < NDT; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[t][r] = 0.f;
+    float m = -FLT_MAX, l = 0.f;
+
+    int buf = 0;
+    for (int i = 0; i < count; ++i) {
+      // The tile's own copies have landed where no more are under way than those behind it (which count from the last one asked for; what else has been asked for since only makes the
+      // wait longer); at the end all of them.
+      constexpr int BEHIND = (STAGES - 2) * 2 * ((COPIES + NW - 1) / NW);
+      static_assert(COPIES % NW == 0 || STAGES == 2, "");
+      static_assert(BEHIND < 16, "");
+      if (i + STAGES - 1 <= count) __builtin_amdgcn_s_waitcnt(0x0F70 + BEHIND);
+      else __builtin_amdgcn_s_waitcnt(0x0F70);
+      asm volatile("" ::: "memory");
+      __syncthreads();
+      if (i + STAGES - 1 < count) {
+        if (((i + STAGES - 1) & 31) == 0) pages_from(2 * (tile0 + i + STAGES - 1));
+        copy_tile(i + STAGES - 1, buf == 0 ? STAGES - 1 : buf - 1);
+      }
+      const uint32_t k_at = k_a0 + 4 * TILE * buf, v_at = v_a0 + 4 * TILE * buf;
+      const int tile = (tile0 + i) * kTile;
+      // ---- scores
+      f32x16 sc;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sc[r] = 0.f;
+      {
+        u32x4 kf[NS];
+#pragma unroll
+        for (int s = 0; s < NS; ++s) kf[s] = *(const u32x4 __attribute__((address_space(3)))*)(size_t)(k_at ^ (32u * s));
+#pragma unroll
+        for (int s = 0; s < NS; ++s) sc = mfma32<F16>(kf[s], qf[s], sc);
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);          // four reads of the LDS ahead of the products
+#pragma unroll
+        for (int s = 0; s < NS - 4; ++s) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+      }
+      auto v_operand = [&](int half, int t) {
+        lds_u16_ptr vp = (lds_u16_ptr)(size_t)((v_at ^ (64u * t)) + 2 * (16 * half * D));
+        const u32x2 a0 = read_transposed(vp), a1 = read_transposed(vp + 8 * D);
+        return u32x4{a0.x, a0.y, a1.x, a1.y};
+      };
+      // ---- who sees what
+      float s[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = sc[r] * p.scale_log2e;
+      if (tile < lo_edge || tile + kTile > e.len) {
+        const uint32_t vis = visible(p, e, mask, of.node, lo, tile) >> (4 * c);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = vis >> (8 * (r >> 2) + (r & 3)) & 1 ? s[r] : -__builtin_inff();
+        // values that are not finite leave the tile; who sees one of a channel gets NaN there
+        uint32_t most = 0;
+        u32x4 __attribute__((address_space(3)))* vs = (u32x4 __attribute__((address_space(3)))*)(size_t)(lds_address(staged) + 2 * TILE + 4 * TILE * buf);
+#pragma unroll
+        for (int i8 = 0; i8 < TILE / 512; ++i8) {
+          const u32x4 v = vs[64 * i8 + lane];
+#pragma unroll
+          for (int d = 0; d < 4; ++d) most = larger_halves(most, v[d]);
+        }
+        if (__any(not_finite<F16>(most) != 0)) {      // (the same for all wavefronts)
+#pragma unroll
+          for (int t = 0; t < NDT; ++t) {
+            f32x16 met;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) met[r] = 0.f;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              u32x4 odd = v_operand(half, t), sees;
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                odd[r] = not_finite<F16>(odd[r]) & ones<F16>();
+                sees[r] = halves(vis >> (16 * half + 8 * (r >> 1) + 2 * (r & 1))) & ones<F16>();
+              }
+              met = mfma32<F16>(odd, sees, met);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[t][r] = met[r] > 0.f ? __builtin_nanf("") : acc[t][r];
+          }
+          __syncthreads();
+          for (int i8 = threadIdx.x; i8 < TILE / 8; i8 += 64 * NW) {
+            u32x4 v = vs[i8];
+#pragma unroll
+            for (int d = 0; d < 4; ++d) v[d] &= ~not_finite<F16>(v[d]);
+            vs[i8] = v;
+          }
+          __syncthreads();
+        }
+      }
+      // ---- probabilities, in two parts
+      float top = s[0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
+      {
+        const LanePair u = half_pair(top);
+        top = fmaxf(u.x, u.y);
+      }
+      if (__any(top > m + kLimit)) {
+        const float moved = top > m + kLimit ? top - kHead : m;
+        const float f = moved > m ? fast_exp2(m - moved) : 1.f;
+        m = moved;
+        l *= f;
+#pragma unroll
+        for (int t = 0; t < NDT; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[t][r] *= f;
+      }
+      u32x4 pf[2], pl[2];
+      float sum = 0.f;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float w[8], f[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) { w[r] = fast_exp2(s[8 * half + r] - m); sum += w[r]; }
+        pf[half] = pack8_as<F16>(w);
+        unpack8_as<F16>(pf[half], f);
+#pragma unroll
+        for (int r = 0; r < 8; ++r) f[r] = w[r] - f[r];
+        pl[half] = pack8_as<F16>(f);
+      }
+      l += sum;
+      // ---- O^T += V^T P^T
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int t = 0; t < NDT; ++t) {
+          const u32x4 vf = v_operand(half, t);
+          acc[t] = mfma32<F16>(vf, pf[half], acc[t]);
+          acc[t] = mfma32<F16>(vf, pl[half], acc[t]);
+        }
+      buf = buf + 1 == STAGES ? 0 : buf + 1;
+    }
+    __syncthreads();      // (the next unit's first copies go over the tile that others may still read)
+
+    {
+      const LanePair u = half_pair(l);
+      l = u.x + u.y;
+    }
+    if (__any(bad)) {
+      l = __builtin_nanf("");
+      if (threadIdx.x == 0) raise_status(p.status, e.past ? DAISY_STATUS_LENGTH_PAST_PAGES : DAISY_STATUS_PAGE_OUT_OF_RANGE);
+    }
+    if (mine) {
+      const bool done = off == 0 && count == at.n_tiles;
+      const float inv = done ? 1.f / l : 1.f;
+      const int64_t slot = (int64_t)(2 * group + (off == 0 ? 1 : 0)) * p.cols + col;
+      uint16_t* dst = row_of_o(p, b, of) + 4 * c;
+      float* part = p.part + slot * D + 4 * c;
+#pragma unroll
+      for (int t = 0; t < NDT; ++t)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const f32x4 f = {acc[t][4 * g] * inv, acc[t][4 * g + 1] * inv, acc[t][4 * g + 2] * inv, acc[t][4 * g + 3] * inv};
+          if (done) *reinterpret_cast<u32x2*>(dst + 32 * t + 8 * g) = pack_out<F16>(p, f);
+          else *reinterpret_cast<f32x4*>(part + 32 * t + 8 * g) = f;
+        }
+      if (!done && c == 0) p.stat[slot] = float2{m, l};
+    }
+    if (off + count < at.n_tiles)
+      beyond = SplitUnit{(int)((unsigned)(x - off) / (unsigned)share), (int)((unsigned)(x - off + at.n_tiles - 1) / (unsigned)share), b, h, at.col0, at.cols};
+    x += count;
+  }
+  if (threadIdx.x == 0) p.split[group] = beyond;
+  zero_the_rest<D>(p, group);
+}
+
 // Where part i of a unit is: the workgroup that the unit begins in has it in its second slot, the others in their first.
 __device__ __forceinline__ int64_t part_slot(const TreeParams& p, const SplitUnit& u, int i, int col) {
   return (int64_t)(2 * (u.first + i) + (i == 0 ? 1 : 0)) * p.cols + col;
 }
 
-// Joins the partial sums of the units that lie in more than one workgroup's run.  The results of a unit are dealt to as many workgroups as there are ends of runs in
-// it, LPR lanes to a piece of 4 LPR channels and 256 / LPR parts side by side, the lanes' sums joined in the LDS.
+// Joins the partial sums of the units that lie in more than one workgroup's run.  The results of up to 16 of a unit's columns are dealt to as many workgroups as there are ends
+// of runs in it.  Many parts: LPR lanes to a piece of 4 LPR channels and 256 / LPR parts side by side, the lanes' sums joined in the LDS.
 template <int D, bool F16, int LPR>
-__device__ __forceinline__ void join_parts(const TreeParams& p, const SplitUnit& u, int parts, int helpers, int me, f32x4 (*sums)[256], float2* stats) {
+__device__ __forceinline__ void join_many(const TreeParams& p, const SplitUnit& u, int col0, int cols, int parts, int helpers, int me, f32x4* sums, float2* stats) {
   constexpr int GROUPS = 256 / LPR, U = 4, CH = 4 * LPR;      // (U parts asked for at once)
   const int r = threadIdx.x / LPR, at = threadIdx.x % LPR * 4;
-  for (int chunk = me; chunk < u.cols * (D / CH); chunk += helpers) {
-    const int col = chunk / (D / CH), d0 = chunk % (D / CH) * CH;
+  for (int chunk = me; chunk < cols * (D / CH); chunk += helpers) {
+    const int col = col0 + chunk / (D / CH), d0 = chunk % (D / CH) * CH;
     float m = -__builtin_inff(), l = 0.f;
     f32x4 a = {0.f, 0.f, 0.f, 0.f};
     for (int i0 = r; i0 < parts; i0 += GROUPS * U) {
@@ -655,7 +980,7 @@ __device__ __forceinline__ void join_parts(const TreeParams& p, const SplitUnit&
       }
     }
     __syncthreads();      // (the chunk before has been read)
-    (*sums)[threadIdx.x] = a;
+    sums[threadIdx.x] = a;
     if (at == 0) stats[r] = float2{m, l};
     __syncthreads();
     if (threadIdx.x < LPR) {
@@ -666,67 +991,73 @@ __device__ __forceinline__ void join_parts(const TreeParams& p, const SplitUnit&
       for (int i = 0; i < used; ++i) {
         const float w = fast_exp2(stats[i].x - best);
         all = fmaf(w, stats[i].y, all);
-        a += w * (*sums)[i * LPR + threadIdx.x];
+        a += w * sums[i * LPR + threadIdx.x];
       }
       a *= 1.f / all;
       *reinterpret_cast<u32x2*>(row_of_o(p, u.b, query_of(p, u.h, u.col0 + col)) + d0 + at) = pack_out<F16>(p, a);
     }
   }
 }
+// Few parts: a thread per four channels, every part of which it asks for at once.
+template <int D, bool F16, int FEW>
+__device__ __forceinline__ void join_few(const TreeParams& p, const SplitUnit& u, int col0, int cols, int parts, int helpers, int me) {
+  for (int i0 = me * 256 + (int)threadIdx.x; i0 < cols * (D / 4); i0 += helpers * 256) {
+    const int col = col0 + i0 / (D / 4), at = i0 % (D / 4) * 4;
+    float2 st[FEW];
+    f32x4 v[FEW];
+#pragma unroll
+    for (int i = 0; i < FEW; ++i) {
+      const int64_t s = part_slot(p, u, min(i, parts - 1), col);
+      st[i] = p.stat[s];
+      v[i] = *reinterpret_cast<const f32x4*>(p.part + s * D + at);
+    }
+    float top = st[0].x, l = 0.f;
+#pragma unroll
+    for (int i = 1; i < FEW; ++i) top = fmaxf(top, st[i].x);
+    f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < FEW; ++i) {
+      const float f = i < parts ? fast_exp2(st[i].x - top) : 0.f;
+      l = i < parts ? fmaf(f, st[i].y, l) : l;
+      a = i < parts ? a + f * v[i] : a;
+    }
+    a *= 1.f / l;
+    *reinterpret_cast<u32x2*>(row_of_o(p, u.b, query_of(p, u.h, u.col0 + col)) + at) = pack_out<F16>(p, a);
+  }
+}
 
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void tree_join_kernel(TreeParams p) {
-  constexpr int kFew = 8;
-  __shared__ f32x4 sums[1][256];
+  __shared__ f32x4 sums[256];
   __shared__ float2 stats[64];
   const SplitUnit u = p.split[blockIdx.x];
   // No such unit; or, where another call has the same workspace at the same time, one that is not this call's: its results are lost, nothing else is.
   if (u.first < 0 || u.first > (int)blockIdx.x || u.last <= (int)blockIdx.x || u.last >= p.groups) return;
   if ((unsigned)u.b >= (unsigned)p.B || (unsigned)u.h >= (unsigned)p.H || u.cols <= 0 || u.cols > p.cols || u.col0 < 0 || u.col0 > p.T * p.G - u.cols) return;
   const int parts = u.last - u.first + 1, helpers = parts - 1, me = (int)blockIdx.x - u.first;
-  if (parts <= kFew) {
-    // a thread per four channels, every part of which it asks for at once
-    for (int i0 = me * 256 + (int)threadIdx.x; i0 < u.cols * (D / 4); i0 += helpers * 256) {
-      const int col = i0 / (D / 4), at = i0 % (D / 4) * 4;
-      float2 st[kFew];
-      f32x4 v[kFew];
-#pragma unroll
-      for (int i = 0; i < kFew; ++i) {
-        const int64_t s = part_slot(p, u, min(i, parts - 1), col);
-        st[i] = p.stat[s];
-        v[i] = *reinterpret_cast<const f32x4*>(p.part + s * D + at);
-      }
-      float top = st[0].x, l = 0.f;
-#pragma unroll
-      for (int i = 1; i < kFew; ++i) top = fmaxf(top, st[i].x);
-      f32x4 a = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < kFew; ++i) {
-        const float f = i < parts ? fast_exp2(st[i].x - top) : 0.f;
-        l = i < parts ? fmaf(f, st[i].y, l) : l;
-        a = i < parts ? a + f * v[i] : a;
-      }
-      a *= 1.f / l;
-      *reinterpret_cast<u32x2*>(row_of_o(p, u.b, query_of(p, u.h, u.col0 + col)) + at) = pack_out<F16>(p, a);
-    }
-  } else if (parts > 128) {
-    join_parts<D, F16, 4>(p, u, parts, helpers, me, sums, stats);
-  } else {
-    join_parts<D, F16, 16>(p, u, parts, helpers, me, sums, stats);
-  }
+  const int col0 = 16 * blockIdx.y, cols = min(u.cols - col0, 16);
+  if (cols <= 0) return;
+  if (parts == 2) join_few<D, F16, 2>(p, u, col0, cols, parts, helpers, me);
+  else if (parts <= 4) join_few<D, F16, 4>(p, u, col0, cols, parts, helpers, me);
+  else if (parts <= 8) join_few<D, F16, 8>(p, u, col0, cols, parts, helpers, me);
+  else if (parts > 128) join_many<D, F16, 4>(p, u, col0, cols, parts, helpers, me, sums, stats);
+  else join_many<D, F16, 16>(p, u, col0, cols, parts, helpers, me, sums, stats);
 }
 
-// How many workgroups share the work: what the chip holds at once, less where there are fewer tiles.
-struct TreeSplit { int groups, cols, blocks, NC; size_t lds; };
+// Up to 16 columns a wavefront by itself, up to 32 too where its registers hold them, else workgroups of 64 columns or of 128; as many workgroups as the chip holds at once, fewer
+// where there are fewer tiles.
+struct TreeSplit { int groups, cols, blocks, NC, NW; size_t lds; };      // NC: pieces of 16 columns of a wavefront, or 0 and NW: wavefronts of 32
 static TreeSplit tree_split(int B, int T, int H, int G, int D, int64_t capacity) {
-  TreeSplit s;
+  TreeSplit s = {};
   const int all = T * G;
-  s.NC = all <= 16 ? 1 : all <= 32 || D == 256 ? 2 : 4;
-  s.cols = all < 16 * s.NC ? all : 16 * s.NC;
-  s.blocks = (all + 16 * s.NC - 1) / (16 * s.NC);
-  s.lds = (size_t)4 * s.cols * tree_row(D) * sizeof(float);
+  s.NC = all <= 16 ? 1 : all <= 32 && D < 256 ? 2 : 0;
+  s.NW = s.NC ? 0 : all <= 64 ? 2 : 4;
+  const int most_cols = s.NC ? 16 * s.NC : 32 * s.NW;
+  s.cols = all < most_cols ? all : most_cols;
+  s.blocks = (all + most_cols - 1) / most_cols;
+  s.lds = s.NC ? (size_t)4 * s.cols * tree_row(D) * sizeof(float) : (size_t)wide_stages(D, s.NW) * 2 * kTile * D * 2;
   const int64_t tiles = ((capacity + kTile - 1) / kTile) * B * H * s.blocks;
-  const int64_t groups = (tiles + 3) / 4, most = kCus * tree_groups_per_cu(D, s.NC);
+  const int64_t groups = s.NC ? (tiles + 3) / 4 : tiles, most = (int64_t)kCus * (s.NC ? tree_groups_per_cu(D, s.NC) : 4 * wide_waves_per_simd(D) / s.NW);
   s.groups = (int)(groups < most ? groups : most);
   return s;
 }
@@ -739,20 +1070,18 @@ static bool tree_shape_ok(int B, int T, int Hq, int H, int D, int max_pages, int
          (int64_t)max_pages * page_size <= kMostPositions && tree_tiles_fit(B, T, Hq, H, D, (int64_t)max_pages * page_size);
 }
 
-template <int D, bool F16, int NC> static int tree_launch(const TreeParams& p, size_t lds, hipStream_t s) {
-  hipLaunchKernelGGL((tree_attn_kernel<D, F16, NC>), dim3((unsigned)p.groups), dim3(256), lds, s, p);
-  hipLaunchKernelGGL((tree_join_kernel<D, F16>), dim3((unsigned)p.groups), dim3(256), 0, s, p);
+template <int D, bool F16> static int tree_launch(const TreeParams& p, const TreeSplit& sp, hipStream_t s) {
+  const dim3 grid((unsigned)p.groups);
+  if (sp.NC == 1) hipLaunchKernelGGL((tree_attn_kernel<D, F16, 1>), grid, dim3(256), sp.lds, s, p);
+  else if (sp.NW == 2) hipLaunchKernelGGL((tree_wide_kernel<D, F16, 2>), grid, dim3(128), sp.lds, s, p);
+  else if (sp.NW == 4) hipLaunchKernelGGL((tree_wide_kernel<D, F16, 4>), grid, dim3(256), sp.lds, s, p);
+  else if constexpr (D < 256) hipLaunchKernelGGL((tree_attn_kernel<D, F16, 2>), grid, dim3(256), sp.lds, s, p);
+  hipLaunchKernelGGL((tree_join_kernel<D, F16>), dim3((unsigned)p.groups, (unsigned)((p.cols + 15) / 16)), dim3(256), 0, s, p);
   DAISY_CHECK_LAUNCH("tree_attn_kernel");
   return DAISY_OK;
 }
-template <int D, bool F16> static int tree_launch(const TreeParams& p, int NC, size_t lds, hipStream_t s) {
-  if (NC == 1) return tree_launch<D, F16, 1>(p, lds, s);
-  if (D == 256 || NC == 2) return tree_launch<D, F16, 2>(p, lds, s);
-  if constexpr (D < 256) return tree_launch<D, F16, 4>(p, lds, s);
-  return DAISY_ERR_UNSUPPORTED;
-}
-template <bool F16> static int tree_launch(const TreeParams& p, int D, int NC, size_t lds, hipStream_t s) {
-  return D == 64 ? tree_launch<64, F16>(p, NC, lds, s) : D == 128 ? tree_launch<128, F16>(p, NC, lds, s) : tree_launch<256, F16>(p, NC, lds, s);
+template <bool F16> static int tree_launch(const TreeParams& p, int D, const TreeSplit& sp, hipStream_t s) {
+  return D == 64 ? tree_launch<64, F16>(p, sp, s) : D == 128 ? tree_launch<128, F16>(p, sp, s) : tree_launch<256, F16>(p, sp, s);
 }
 
 }  // namespace daisy
@@ -832,5 +1161,5 @@ extern "C" int daisy_paged_tree_attn_fwd(const void* q, const int64_t* q_strides
   p.stat = (float2*)(p.part + (size_t)2 * sp.groups * sp.cols * D);
   p.B = B; p.T = T; p.H = H; p.G = Hq / H; p.cols = sp.cols; p.window = window; p.groups = sp.groups; p.per_node = divisor(Hq / H);
   p.scale_log2e = scale * kLog2e; p.status = status;
-  return cache_is_f16 ? tree_launch<true>(p, D, sp.NC, sp.lds, (hipStream_t)stream) : tree_launch<false>(p, D, sp.NC, sp.lds, (hipStream_t)stream);
+  return cache_is_f16 ? tree_launch<true>(p, D, sp, (hipStream_t)stream) : tree_launch<false>(p, D, sp, (hipStream_t)stream);
 }
