@@ -140,19 +140,23 @@ __device__ __forceinline__ Sequence sequence(const TreeParams& p, int b) {
   const int len = p.lens[at], nodes = p.nodes != nullptr ? p.nodes[at] : p.T;
   return Sequence{b < p.B ? len : -1, nodes};
 }
+// What coming to a unit costs a workgroup of many columns, in tiles: what it reads one behind the other on the way to the first key, and its masks.  (12 sequences of 100 to 24000, 256 columns: 0 tiles 209 us,
+// 4 162, 8 158, 12 156, 16 158.  Wavefronts that take a unit each hide it behind each other; there the way around a unit without tiles costs registers.)
+constexpr int unit_tiles(int cols) { return cols <= 32 ? 0 : 8; }
 template <int COLS> __device__ __forceinline__ int weight_of(const TreeParams& p, const Sequence& s) {
   const Extent e = extent<COLS>(p, s.len, s.nodes);
-  return e.tiles * e.blocks;
+  return e.tiles > 0 ? (e.tiles + unit_tiles(COLS)) * e.blocks : 0;
 }
 
-// The tiles of all units one behind the other, blocks of COLS columns: which unit one of them belongs to.  Every wavefront has one of these and asks for rising numbers.
-struct Unit { Extent e; int b, h, col0, cols, off, count, n_tiles; };
+// The tiles of all units one behind the other, blocks of COLS columns and unit_tiles ahead of each unit's own: which unit one of them belongs to.  Every wavefront has one of these and
+// asks for rising numbers.
+struct Unit { Extent e; int b, h, col0, cols, off, count, n_tiles, x, next; };      // count tiles from `off` on (there may be none); x: the unit's first one; next: behind those
 template <int COLS> struct Deal {
   int own, own_upto, per_lane;      // lane i: the tiles (of a key head each) of sequences from i * per_lane on; with those ahead
   // 64 sequences from `base` on, one a lane; up to 64 are all there
   int base, before, weight, upto, chunk;
   Sequence seq;
-  // All tiles.  (For every wavefront of a workgroup at once: many sequences are summed up together.)
+  // How many there are.  (For every wavefront of a workgroup at once: many sequences are summed up together.)
   __device__ __forceinline__ int begin(const TreeParams& p, int wv, int lane) {
     own = 0;
     per_lane = (p.B + 63) >> 6;
@@ -211,9 +215,13 @@ template <int COLS> struct Deal {
     u.n_tiles = max(u.e.tiles, 1);
     const int blocks = max(u.e.blocks, 1);
     const int rel = x - (before + __builtin_amdgcn_readlane(upto - weight, bl)) * p.H;
-    const int unit = (int)min((unsigned)rel / (unsigned)u.n_tiles, (unsigned)(p.H * blocks - 1));
-    u.off = min(max(rel - unit * u.n_tiles, 0), u.n_tiles - 1);
-    u.count = max(min(u.n_tiles - u.off, x_end - x), 1);
+    const int ahead = unit_tiles(COLS), all = u.n_tiles + ahead;
+    const int unit = (int)min((unsigned)rel / (unsigned)all, (unsigned)(p.H * blocks - 1));
+    const int from = min(max(rel - unit * all, 0), all - 1), upto = min(all, from + max(x_end - x, 1));
+    u.off = max(from - ahead, 0);
+    u.count = ahead == 0 ? max(upto - from, 1) : max(upto - ahead, 0) - u.off;
+    u.x = x - from + ahead;
+    u.next = x + upto - from;
     u.h = (int)((unsigned)unit / (unsigned)blocks);
     u.col0 = (unit - u.h * blocks) * COLS;
     u.cols = min(max(u.e.nodes * p.G, 1) - u.col0, COLS);
@@ -329,6 +337,8 @@ __global__ __launch_bounds__(256, tree_groups_per_cu(D, NC)) void tree_attn_kern
     const Unit at = deal.unit(p, x, x_end, lane);
     const Extent& e = at.e;
     const int off = at.off, count = at.count, n_tiles = at.n_tiles, all_cols = max(e.nodes * p.G, 1);
+    static_assert(unit_tiles(16 * NC) == 0, "");      // (so that there always is a tile)
+    x = at.next;
     b = at.b; h = at.h; col0 = at.col0; cols = at.cols;
 
     // ---- its queries: columns past the last one repeat it
@@ -594,9 +604,8 @@ __global__ __launch_bounds__(256, tree_groups_per_cu(D, NC)) void tree_attn_kern
     }
     if (off + count < n_tiles && wv == 3) {
       const unsigned run = (unsigned)__builtin_amdgcn_readfirstlane(4 * share);
-      beyond = SplitUnit{(int)((unsigned)(x - off) / run), (int)((unsigned)(x - off + n_tiles - 1) / run), b, h, col0, cols};
+      beyond = SplitUnit{(int)((unsigned)at.x / run), (int)((unsigned)(at.x + n_tiles - 1) / run), b, h, col0, cols};
     }
-    x += count;
   }
 
   // ---- what the wavefronts have left open: chains of the same unit, from where one of them broke off (or the workgroup began) on
@@ -722,6 +731,8 @@ __global__ __launch_bounds__(64 * NW, wide_waves_per_simd(D)) void tree_wide_ker
     const Unit at = deal.unit(p, x, x_end, lane);
     const Extent& e = at.e;
     const int b = at.b, h = at.h, off = at.off, count = at.count, all_cols = max(e.nodes * p.G, 1);
+    x = at.next;
+    if (count <= 0) continue;
 
     // ---- copies
     const int32_t* row = p.table + product(b, p.table_st);
@@ -740,29 +751,31 @@ __global__ __launch_bounds__(64 * NW, wide_waves_per_simd(D)) void tree_wide_ker
     const char* kh = reinterpret_cast<const char*>(p.k) + 16 * product(h, p.k_sh);
     const char* vh = reinterpret_cast<const char*>(p.v) + 16 * product(h, p.v_sh);
     const int tile0 = e.first + off;
-    auto copy_tile = [&](int i, int buf) {
+    auto copy_rows = [&](const char* from_pages, uint32_t sp, uint32_t ss, int row_bytes, auto swizzle, int i, uint32_t to) {
       const int tile = (tile0 + i) * kTile;
       const bool whole = tile >= e.lo && tile + kTile <= e.hi;
 #pragma unroll
       for (int j0 = 0; j0 < COPIES; j0 += NW) {
         const int j = j0 + wv;
-        if (COPIES % NW != 0 && j >= COPIES) break;
         const int half = RPL * j >> 4, r = RPL * j + ld_row;
         const int pg = __builtin_amdgcn_readlane(id, 2 * (i & 31) + half), slot = __builtin_amdgcn_readlane(in, 2 * (i & 31) + half) * kBlock;
         // a row of the half, or where that is outside the range, another one that is
         const int first = tile + half * kBlock, own = r & 15;
         const int from = whole ? own : min(max(own, min(max(e.lo - first, 0), kBlock - 1)), min(max(e.hi - 1 - first, 0), kBlock - 1));
-        copy16_to_lds_async((const uint16_t*)(kh + 16 * (product(pg, p.k_sp) + product(slot, p.k_ss))), from * k_row + 16 * (ld_pos ^ swz_k(r)),
-                            lds_address(staged) + 4 * TILE * buf + 1024 * j);
-        copy16_to_lds_async((const uint16_t*)(vh + 16 * (product(pg, p.v_sp) + product(slot, p.v_ss))), from * v_row + 16 * (ld_pos ^ swz_v(r)),
-                            lds_address(staged) + 2 * TILE + 4 * TILE * buf + 1024 * j);
+        copy16_to_lds_async((const uint16_t*)(from_pages + 16 * (product(pg, sp) + product(slot, ss))), from * row_bytes + 16 * (ld_pos ^ swizzle(r)), to + 1024 * j);
       }
     };
+    auto copy_k = [&](int i, int slot) { copy_rows(kh, p.k_sp, p.k_ss, k_row, swz_k, i, lds_address(staged) + 4 * TILE * slot); };
+    auto copy_v = [&](int i, int slot) { copy_rows(vh, p.v_sp, p.v_ss, v_row, swz_v, i, lds_address(staged) + 4 * TILE * slot + 2 * TILE); };
+    // Tile i is in slot i % STAGES.  Ahead of tile i's softmax K(i + 1) and V(i) have landed, and V(i + STAGES - 1) and K(i + STAGES) are asked for, whose slots the tile before and this one's
+    // scores have left.
     pages_from(2 * tile0);
+    copy_k(0, 0);
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i)
-      if (i < count) copy_tile(i, i);
-
+    for (int i = 0; i < STAGES - 1; ++i) {
+      if (i < count) copy_v(i, i);
+      if (i + 1 < count) copy_k(i + 1, i + 1);
+    }
     // ---- this lane's query: columns past the last one repeat it
     const int col = 32 * wv + n;
     const bool mine = col < at.cols;
@@ -783,41 +796,42 @@ __global__ __launch_bounds__(64 * NW, wide_waves_per_simd(D)) void tree_wide_ker
       for (int r = 0; r < 16; ++r) acc[t][r] = 0.f;
     float m = -FLT_MAX, l = 0.f;
 
-    int buf = 0;
-    for (int i = 0; i < count; ++i) {
-      // The tile's own copies have landed where no more are under way than those behind it (which count from the last one asked for; what else has been asked for since only makes the
-      // wait longer); at the end all of them.
-      constexpr int BEHIND = (STAGES - 2) * 2 * ((COPIES + NW - 1) / NW);
-      static_assert(COPIES % NW == 0 || STAGES == 2, "");
-      static_assert(BEHIND < 16, "");
-      if (i + STAGES - 1 <= count) __builtin_amdgcn_s_waitcnt(0x0F70 + BEHIND);
-      else __builtin_amdgcn_s_waitcnt(0x0F70);
+    // Waits for all copies but the `behind` last ones (what else has been asked for since only makes the wait longer), then for everybody.
+    auto landed = [&](auto behind) {
+      constexpr int n = decltype(behind)::value;
+      __builtin_amdgcn_s_waitcnt(0x0F70 | (n & 15) | n >> 4 << 14);
       asm volatile("" ::: "memory");
       __syncthreads();
-      if (i + STAGES - 1 < count) {
-        if (((i + STAGES - 1) & 31) == 0) pages_from(2 * (tile0 + i + STAGES - 1));
-        copy_tile(i + STAGES - 1, buf == 0 ? STAGES - 1 : buf - 1);
-      }
-      const uint32_t k_at = k_a0 + 4 * TILE * buf, v_at = v_a0 + 4 * TILE * buf;
-      const int tile = (tile0 + i) * kTile;
-      // ---- scores
-      f32x16 sc;
+    };
+    constexpr int PER = 2 * ((COPIES + NW - 1) / NW);      // copies of a tile and wavefront
+    static_assert(COPIES % NW == 0, "");
+    using All = std::integral_constant<int, 0>;
+    f32x16 sc;
+    auto scores = [&](int slot) {
+      const uint32_t k_at = k_a0 + 4 * TILE * slot;
+      u32x4 kf[NS];
 #pragma unroll
       for (int r = 0; r < 16; ++r) sc[r] = 0.f;
-      {
-        u32x4 kf[NS];
 #pragma unroll
-        for (int s = 0; s < NS; ++s) kf[s] = *(const u32x4 __attribute__((address_space(3)))*)(size_t)(k_at ^ (32u * s));
+      for (int s = 0; s < NS; ++s) kf[s] = *(const u32x4 __attribute__((address_space(3)))*)(size_t)(k_at ^ (32u * s));
 #pragma unroll
-        for (int s = 0; s < NS; ++s) sc = mfma32<F16>(kf[s], qf[s], sc);
-        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);          // four reads of the LDS ahead of the products
-#pragma unroll
-        for (int s = 0; s < NS - 4; ++s) {
-          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        }
-        __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+      for (int s = 0; s < NS; ++s) sc = mfma32<F16>(kf[s], qf[s], sc);
+    };
+    if (count >= STAGES) landed(std::integral_constant<int, (STAGES - 1) * PER>());
+    else landed(All());
+    scores(0);
+    int slot = 0;
+    auto step = [&](int i, auto more) {
+      if (i + STAGES - 1 < count) landed(std::integral_constant<int, (STAGES - 2) * PER>());
+      else landed(All());
+      const int next = slot + 1 == STAGES ? 0 : slot + 1;
+      if (i + STAGES - 1 < count) copy_v(i + STAGES - 1, slot == 0 ? STAGES - 1 : slot - 1);
+      if (i + STAGES < count) {
+        if (((i + STAGES) & 31) == 0) pages_from(2 * (tile0 + i + STAGES));
+        copy_k(i + STAGES, slot);
       }
+      const int tile = (tile0 + i) * kTile;
+      const uint32_t v_at = v_a0 + 4 * TILE * slot;
       auto v_operand = [&](int half, int t) {
         lds_u16_ptr vp = (lds_u16_ptr)(size_t)((v_at ^ (64u * t)) + 2 * (16 * half * D));
         const u32x2 a0 = read_transposed(vp), a1 = read_transposed(vp + 8 * D);
@@ -833,7 +847,7 @@ __global__ __launch_bounds__(64 * NW, wide_waves_per_simd(D)) void tree_wide_ker
         for (int r = 0; r < 16; ++r) s[r] = vis >> (8 * (r >> 2) + (r & 3)) & 1 ? s[r] : -__builtin_inff();
         // values that are not finite leave the tile; who sees one of a channel gets NaN there
         uint32_t most = 0;
-        u32x4 __attribute__((address_space(3)))* vs = (u32x4 __attribute__((address_space(3)))*)(size_t)(lds_address(staged) + 2 * TILE + 4 * TILE * buf);
+        u32x4 __attribute__((address_space(3)))* vs = (u32x4 __attribute__((address_space(3)))*)(size_t)(lds_address(staged) + 2 * TILE + 4 * TILE * slot);
 #pragma unroll
         for (int i8 = 0; i8 < TILE / 512; ++i8) {
           const u32x4 v = vs[64 * i8 + lane];
@@ -869,7 +883,6 @@ __global__ __launch_bounds__(64 * NW, wide_waves_per_simd(D)) void tree_wide_ker
           __syncthreads();
         }
       }
-      // ---- probabilities, in two parts
       float top = s[0];
 #pragma unroll
       for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
@@ -887,31 +900,49 @@ __global__ __launch_bounds__(64 * NW, wide_waves_per_simd(D)) void tree_wide_ker
 #pragma unroll
           for (int r = 0; r < 16; ++r) acc[t][r] *= f;
       }
+      // ---- the next tile's scores, and this one's probabilities meanwhile
+      if constexpr (more.value) scores(next);
       u32x4 pf[2], pl[2];
-      float sum = 0.f;
+      float w[16], sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int r = 0; r < 16; ++r) { w[r] = fast_exp2(s[r] - m); sum[r & 3] += w[r]; }
+      pf[0] = pack8_as<F16>(w);
+      pf[1] = pack8_as<F16>(w + 8);
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      if constexpr (more.value) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);          // reads of the LDS
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);        // a product
+          if (s < NS - 4) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x002, 80 / NS, 0);  // vector instructions
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      // ---- O^T += V^T P^T, in two parts: the second is what the rounding of the first has lost
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        float w[8], f[8];
-#pragma unroll
-        for (int r = 0; r < 8; ++r) { w[r] = fast_exp2(s[8 * half + r] - m); sum += w[r]; }
-        pf[half] = pack8_as<F16>(w);
+        float f[8];
         unpack8_as<F16>(pf[half], f);
 #pragma unroll
-        for (int r = 0; r < 8; ++r) f[r] = w[r] - f[r];
+        for (int r = 0; r < 8; ++r) f[r] = w[8 * half + r] - f[r];
         pl[half] = pack8_as<F16>(f);
       }
-      l += sum;
-      // ---- O^T += V^T P^T
 #pragma unroll
-      for (int half = 0; half < 2; ++half)
+      for (int half = 0; half < 2; ++half) {
+        u32x4 vf[NDT];
 #pragma unroll
         for (int t = 0; t < NDT; ++t) {
-          const u32x4 vf = v_operand(half, t);
-          acc[t] = mfma32<F16>(vf, pf[half], acc[t]);
-          acc[t] = mfma32<F16>(vf, pl[half], acc[t]);
+          vf[t] = v_operand(half, t);
+          acc[t] = mfma32<F16>(vf[t], pf[half], acc[t]);
         }
-      buf = buf + 1 == STAGES ? 0 : buf + 1;
-    }
+#pragma unroll
+        for (int t = 0; t < NDT; ++t) acc[t] = mfma32<F16>(vf[t], pl[half], acc[t]);
+      }
+      slot = next;
+    };
+    for (int i = 0; i + 1 < count; ++i) step(i, std::true_type());
+    step(count - 1, std::false_type());
     __syncthreads();      // (the next unit's first copies go over the tile that others may still read)
 
     {
@@ -939,8 +970,7 @@ __global__ __launch_bounds__(64 * NW, wide_waves_per_simd(D)) void tree_wide_ker
       if (!done && c == 0) p.stat[slot] = float2{m, l};
     }
     if (off + count < at.n_tiles)
-      beyond = SplitUnit{(int)((unsigned)(x - off) / (unsigned)share), (int)((unsigned)(x - off + at.n_tiles - 1) / (unsigned)share), b, h, at.col0, at.cols};
-    x += count;
+      beyond = SplitUnit{(int)((unsigned)at.x / (unsigned)share), (int)((unsigned)(at.x + at.n_tiles - 1) / (unsigned)share), b, h, at.col0, at.cols};
   }
   if (threadIdx.x == 0) p.split[group] = beyond;
   zero_the_rest<D>(p, group);
@@ -1056,14 +1086,14 @@ static TreeSplit tree_split(int B, int T, int H, int G, int D, int64_t capacity)
   s.cols = all < most_cols ? all : most_cols;
   s.blocks = (all + most_cols - 1) / most_cols;
   s.lds = s.NC ? (size_t)4 * s.cols * tree_row(D) * sizeof(float) : (size_t)wide_stages(D, s.NW) * 2 * kTile * D * 2;
-  const int64_t tiles = ((capacity + kTile - 1) / kTile) * B * H * s.blocks;
+  const int64_t tiles = ((capacity + kTile - 1) / kTile + unit_tiles(most_cols)) * B * H * s.blocks;
   const int64_t groups = s.NC ? (tiles + 3) / 4 : tiles, most = (int64_t)kCus * (s.NC ? tree_groups_per_cu(D, s.NC) : 4 * wide_waves_per_simd(D) / s.NW);
   s.groups = (int)(groups < most ? groups : most);
   return s;
 }
 // Tiles are counted in 32 bits, with room for a share's rounding.
 static bool tree_tiles_fit(int B, int T, int Hq, int H, int D, int64_t capacity) {
-  return ((double)capacity / kTile + 1) * B * H * tree_split(1, T, H, Hq / H, D, 1).blocks < (double)(1 << 30);
+  return ((double)capacity / kTile + 8) * B * H * tree_split(1, T, H, Hq / H, D, 1).blocks < (double)(1 << 30);
 }
 static bool tree_shape_ok(int B, int T, int Hq, int H, int D, int max_pages, int page_size) {
   return B > 0 && T > 0 && T <= kMostNodes && H > 0 && Hq > 0 && Hq % H == 0 && Hq <= 65536 && (D == 64 || D == 128 || D == 256) && max_pages > 0 && page_size > 0 &&
