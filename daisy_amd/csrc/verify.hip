@@ -10,16 +10,22 @@
 // max(a p - b q, 0), with two numbers a and b; c is accepted where a_c q(y) < max(a p(y) - b q(y), 0).  Where nothing is left p_u itself is taken again.
 //
 // One pass over all scores leaves, of every row and slice of the vocabulary, its largest score, its sum and what would follow: which tokens are children's is known ahead of the walk.  A second
-// kernel joins the slices and walks.
+// kernel joins the slices and walks; where children were drawn, two more draw from what the walk has left of the last row.
+//
+// Sums of exponentials are fp32 in a slice and 64 bits beyond it, the children's e and all that decides about them 64 bits.  What follows is looked for in fp32, with the second best beside it: where
+// the two are nearer than fp32 tells apart, the row is gone over again in 64 bits.
 #include "common.h"
 
 #include <math.h>
+
+#include <type_traits>
 
 namespace daisy {
 
 enum ScoreType { kScoreF32 = 0, kScoreBf16 = 1, kScoreF16 = 2 };
 enum VerifyMode { kGreedy = 0, kChosen = 1, kDrawn = 2 };
 constexpr int kMostNodes = 256, kThreads = 256;
+constexpr int kPieceRounds = 4, kPiece = 4 * kThreads * kPieceRounds;      // of a row that is drawn from: a workgroup's
 
 struct VerifyParams {
   const void* x; int64_t x_sb, x_st;                        // [B, T, V]
@@ -31,13 +37,16 @@ struct VerifyParams {
   const float* noise; int64_t noise_sb;                     // [B, V]
   const float* q; int64_t q_sb, q_st;                       // [B, T, V]
   int32_t* path; int32_t* counts; int64_t* next;
-  struct RowSlice* part;                                    // [B, T, slices]
-  int B, T, V, slices, slice, rows;                         // rows: of a workgroup
+  f32x4* part; int32_t* part_token;                         // [B, T, slices]: sum, top, best, second (RowPart) and the best one's token
+  struct Left* left;                                        // [B]: what is to be drawn from
+  float2* drawn; int32_t* drawn_token; int pieces;          // [B, pieces]: best and second, and the best one's token
+  int B, T, V, slices, slice, rows;                         // slice: of a wavefront; rows: of a workgroup
 };
 
-// Of a slice of a row beside the children's tokens: the largest score, the sum of e relative to that, the best of x / t + noise, relative to it, too (a noise added to a mask of
-// the type's lowest value would be lost), and its token (INT32_MAX: none).  Where there is no noise the best is x itself.
-struct RowSlice { double sum, best; float top; int token; };
+// Of some of a row beside its children's tokens: the largest score, the sum of e relative to that; the two best of x / t + noise, relative to it, too (a noise added to a mask of the type's lowest
+// value would be lost), and the best one's token (INT32_MAX: none).
+template <typename SUM> struct RowPart { SUM sum; float top, best, second; int token; };
+struct Left { double scale, less; int at; float top; };     // max(scale e - less q, 0) of row `at`, whose largest score is `top`; at < 0: nothing to be drawn
 
 // 1 / t, 0 where the likeliest token is wanted
 __device__ __forceinline__ double inverse_temperature(const VerifyParams& p, int b) {
@@ -70,16 +79,19 @@ typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
 typedef uint16_t u16x4_near __attribute__((ext_vector_type(4), aligned(2)));
 template <int E> struct Four { typedef u16x4 Raw; };
 template <> struct Four<kScoreF32> { typedef f32x4 Raw; };
+template <int E> __device__ __forceinline__ typename Four<E>::Raw load4_whole(const void* row, int v) {
+  if constexpr (E == kScoreF32) return __builtin_nontemporal_load((const f32x4_near*)((const float*)row + v));
+  else return __builtin_nontemporal_load((const u16x4_near*)((const uint16_t*)row + v));
+}
 template <int E> __device__ __forceinline__ typename Four<E>::Raw load4(const void* row, int v, int left) {
+  if (left >= 4) return load4_whole<E>(row, v);
   if constexpr (E == kScoreF32) {
     const float* at = (const float*)row + v;
-    if (left >= 4) return __builtin_nontemporal_load((const f32x4_near*)at);
     f32x4 f = {-__builtin_inff(), -__builtin_inff(), -__builtin_inff(), -__builtin_inff()};
     for (int i = 0; i < left; ++i) f[i] = at[i];
     return f;
   } else {
     const uint16_t* at = (const uint16_t*)row + v;
-    if (left >= 4) return __builtin_nontemporal_load((const u16x4_near*)at);
     constexpr uint16_t kNone = E == kScoreBf16 ? 0xff80 : 0xfc00;
     u16x4 u = {kNone, kNone, kNone, kNone};
     for (int i = 0; i < left; ++i) u[i] = at[i];
@@ -104,73 +116,145 @@ __device__ __forceinline__ f32x4 load4_f32(const float* row, int v, int left) {
   return f;
 }
 
-__device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-  for (int d = 32; d > 0; d /= 2) x = fmaxf(x, __shfl_xor(x, d));
+// A value and its neighbour's, 1, 2, 4 (mirrored), 8, 16 and 32 lanes away: step by step over groups of 2 to 64 lanes, whose lanes then all have the result.
+template <int STEP> __device__ __forceinline__ LanePair neighbours(float x) {
+  if constexpr (STEP == 0) return LanePair{x, dpp_move<0xB1>(x)};
+  else if constexpr (STEP == 1) return LanePair{x, dpp_move<0x4E>(x)};
+  else if constexpr (STEP == 2) return LanePair{x, dpp_move<0x141>(x)};
+  else if constexpr (STEP == 3) return LanePair{x, dpp_move<0x128>(x)};
+  else if constexpr (STEP == 4) return row_pair(x);
+  else return half_pair(x);
+}
+struct IntPair { int x, y; };
+template <int STEP> __device__ __forceinline__ IntPair neighbours(int x) {
+  const LanePair r = neighbours<STEP>(__int_as_float(x));
+  return IntPair{__float_as_int(r.x), __float_as_int(r.y)};
+}
+struct DoublePair { double x, y; };
+template <int STEP> __device__ __forceinline__ DoublePair neighbours(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const IntPair lo = neighbours<STEP>((int)(uint32_t)u), hi = neighbours<STEP>((int)(uint32_t)(u >> 32));
+  return DoublePair{__builtin_bit_cast(double, (uint64_t)(uint32_t)hi.x << 32 | (uint32_t)lo.x), __builtin_bit_cast(double, (uint64_t)(uint32_t)hi.y << 32 | (uint32_t)lo.y)};
+}
+template <typename F> __device__ __forceinline__ void steps(int group, F f) {
+  if (group > 1) f(std::integral_constant<int, 0>());
+  if (group > 2) f(std::integral_constant<int, 1>());
+  if (group > 4) f(std::integral_constant<int, 2>());
+  if (group > 8) f(std::integral_constant<int, 3>());
+  if (group > 16) f(std::integral_constant<int, 4>());
+  if (group > 32) f(std::integral_constant<int, 5>());
+}
+__device__ __forceinline__ float wave_max(float x, int group = 64) {
+  steps(group, [&](auto s) { const LanePair r = neighbours<decltype(s)::value>(x); x = fmaxf(r.x, r.y); });
   return x;
 }
-// The larger score, of equal ones the lower token.
+__device__ __forceinline__ double wave_sum64(double x, int group = 64) {
+  steps(group, [&](auto s) { const DoublePair r = neighbours<decltype(s)::value>(x); x = r.x + r.y; });
+  return x;
+}
+// The two best, of equal ones the lower token.
+struct Two { float best, second; int token; };
+__device__ __forceinline__ Two both(Two a, Two b) {
+  const bool other = b.best > a.best || (b.best == a.best && b.token < a.token);
+  return Two{other ? b.best : a.best, fmaxf(fmaxf(a.second, b.second), other ? a.best : b.best), other ? b.token : a.token};
+}
+__device__ __forceinline__ Two wave_two(Two x, int group = 64) {
+  steps(group, [&](auto s) {
+    constexpr int S = decltype(s)::value;
+    const LanePair b = neighbours<S>(x.best), n = neighbours<S>(x.second);
+    const IntPair t = neighbours<S>(x.token);
+    x = both(Two{b.x, n.x, t.x}, Two{b.y, n.y, t.y});
+  });
+  return x;
+}
+// The same for a whole wavefront, most of which has next to nothing to say: the largest, whose lane it is, and the largest of what is not that.
+__device__ __forceinline__ Two two_of_wave(Two x) {
+  const float best = wave_max(x.best);
+  if (!(best > -__builtin_inff())) return Two{best, best, INT32_MAX};
+  const uint64_t at = __ballot(x.best == best);
+  int lane = __builtin_ctzll(at), token = __builtin_amdgcn_readlane(x.token, lane);
+  for (uint64_t more = at & (at - 1); more; more &= more - 1) token = min(token, __builtin_amdgcn_readlane(x.token, __builtin_ctzll(more)));
+  const float second = wave_max((int)(threadIdx.x & 63) == lane ? x.second : x.best);
+  return Two{best, second, token};
+}
+// The larger score in 64 bits, of equal ones the lower token.
 struct Best { double score; int token; };
-__device__ __forceinline__ Best better(const Best& a, const Best& b) {
-  return b.score > a.score || (b.score == a.score && b.token < a.token) ? b : a;
+// (By value: of references the compiler chooses between addresses, in the LDS and on a stack.)
+__device__ __forceinline__ Best better(Best a, Best b) {
+  const bool other = b.score > a.score || (b.score == a.score && b.token < a.token);
+  return Best{other ? b.score : a.score, other ? b.token : a.token};
 }
 __device__ __forceinline__ Best wave_best(Best x) {
-#pragma unroll
-  for (int d = 32; d > 0; d /= 2) x = better(x, Best{__shfl_xor(x.score, d), __shfl_xor(x.token, d)});
+  steps(64, [&](auto s) {
+    constexpr int S = decltype(s)::value;
+    const DoublePair b = neighbours<S>(x.score);
+    const IntPair t = neighbours<S>(x.token);
+    x = better(Best{b.x, t.x}, Best{b.y, t.y});
+  });
   return x;
 }
-__device__ __forceinline__ double wave_sum64(double x) {
-#pragma unroll
-  for (int d = 32; d > 0; d /= 2) x += __shfl_xor(x, d);
-  return x;
-}
+// Whether fp32 tells the two apart: a score is off by 2^-23 of its two terms, of which one is the noise, and 2^-24 of itself.
+__device__ __forceinline__ bool too_near(float best, float second) { return best - second <= 0x1p-20f * (fabsf(best) + 64.f); }
 
-// A best score, relative to `top`, relative to `to`.
-template <int MODE> __device__ __forceinline__ Best shifted(const Best& x, float top, float to, double by) {
-  return MODE == kChosen && x.token != INT32_MAX ? Best{x.score + ((double)top - (double)to) * by, x.token} : x;
-}
-
-// A workgroup takes a slice of the vocabulary for up to `rows` rows of a sequence, whose noise it holds, the next row on its way.  Scores with noise are compared in 64 bits: nothing
-// but equal numbers is a tie.
+// A wavefront takes a slice of the vocabulary for up to `rows` rows of a sequence, whose noise it holds, the next row on its way.
 template <int E, int MODE, int ROUNDS>
 __global__ __launch_bounds__(kThreads) void verify_rows_kernel(VerifyParams p) {
-  __shared__ int2 away[kMostNodes];      // a row, and a token of the slice that one of its children has
+  __shared__ int2 away[kMostNodes];      // a row, and a token of the workgroup's slices that one of its children has
   __shared__ int n_away;
-  __shared__ RowSlice waves[kThreads / 64];
-  const int b = blockIdx.z, tid = threadIdx.x, lane = tid & 63;
-  const int u0 = blockIdx.y * p.rows, u1 = min(u0 + p.rows, nodes_of(p, b));
+  const int b = blockIdx.z, lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int slice = blockIdx.x * (kThreads / 64) + wv;
+  const int v0 = min(slice * p.slice, p.V), v1 = min(v0 + p.slice, p.V);
+  const bool whole = v1 - v0 == p.slice;      // (the same for the wavefront: its loads are not each under a condition of their own)
+  // (all that depends on nothing is asked for at once)
+  f32x4 noise[ROUNDS];
+  int of = 0;
+  int64_t token = 0;
+  if constexpr (MODE == kChosen) {
+    const int j = min((int)threadIdx.x, p.T - 1);
+    of = p.parents[b * p.parents_sb + j];
+    token = p.tokens64 ? ((const int64_t*)p.tokens)[b * p.tokens_sb + j] : ((const int32_t*)p.tokens)[b * p.tokens_sb + j];
+    const float* row = p.noise + b * p.noise_sb;
+    if (whole) {
+#pragma unroll
+      for (int r = 0; r < ROUNDS; ++r) noise[r] = *(const f32x4_near*)(row + v0 + 4 * (lane + 64 * r));
+    } else {
+#pragma unroll
+      for (int r = 0; r < ROUNDS; ++r) {
+        const int v = v0 + 4 * (lane + 64 * r);
+        noise[r] = load4_f32(row, v, v1 - v);
+      }
+    }
+    if (threadIdx.x == 0) n_away = 0;
+  }
+  const int n = nodes_of(p, b), u0 = blockIdx.y * p.rows, u1 = min(u0 + p.rows, n);
   if (u0 >= u1) return;
-  const int v0 = blockIdx.x * p.slice, v1 = min(v0 + p.slice, p.V);
   typename Four<E>::Raw raw[ROUNDS];
   auto load = [&](int u) {
     const void* row = row_of_x<E>(p, b, u);
+    if (whole) {
 #pragma unroll
-    for (int r = 0; r < ROUNDS; ++r) {
-      const int v = v0 + 4 * (tid + r * kThreads);
-      raw[r] = load4<E>(row, v, v1 - v);
+      for (int r = 0; r < ROUNDS; ++r) raw[r] = load4_whole<E>(row, v0 + 4 * (lane + 64 * r));
+    } else {
+#pragma unroll
+      for (int r = 0; r < ROUNDS; ++r) {
+        const int v = v0 + 4 * (lane + 64 * r);
+        raw[r] = load4<E>(row, v, v1 - v);
+      }
     }
   };
   load(u0);
   const double inv_t = MODE == kGreedy ? 0.0 : inverse_temperature(p, b);
   const bool greedy = inv_t == 0.0;
-  f32x4 noise[ROUNDS];
-  if (MODE == kChosen) {
-#pragma unroll
-    for (int r = 0; r < ROUNDS; ++r) {
-      const int v = v0 + 4 * (tid + r * kThreads);
-      noise[r] = greedy ? f32x4{0.f, 0.f, 0.f, 0.f} : load4_f32(p.noise + b * p.noise_sb, v, v1 - v);
-    }
-    if (tid == 0) n_away = 0;
+  if constexpr (MODE == kChosen) {
+    const int first = blockIdx.x * (kThreads / 64) * p.slice;
     __syncthreads();
-    if (!greedy && tid < nodes_of(p, b)) {
-      const int u = parent_of(p, b, tid), y = token_of(p, b, tid);
-      if (u >= u0 && u < u1 && y >= v0 && y < v1) away[atomicAdd(&n_away, 1)] = int2{u, y};
-    }
+    if (!greedy && (int)threadIdx.x < n && of >= u0 && of < u1 && of < (int)threadIdx.x && token >= first && token < min(first + kThreads / 64 * p.slice, p.V))
+      away[atomicAdd(&n_away, 1)] = int2{of, (int)token};
     __syncthreads();
   }
+  if (slice >= p.slices) return;
   const int known = MODE == kChosen ? n_away : 0;
-  const double by = greedy ? 1.0 : inv_t;
-  const float c = (float)fmin(by * 1.4426950408889634, 1e30);
+  const float by = greedy ? 1.f : (float)fmin(inv_t, 1e30), c = greedy ? kLog2e : (float)fmin(inv_t * 1.4426950408889634, 1e30);
   for (int u = u0; u < u1; ++u) {
     f32x4 x[ROUNDS];
 #pragma unroll
@@ -179,12 +263,12 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(VerifyParams p) {
     for (int i = 0; i < known; ++i) {
       const int2 a = away[i];
       const int at = a.y - v0;
-      if (a.x != u || (at >> 2) % kThreads != tid) continue;
+      if (a.x != u || at < 0 || at >= p.slice) continue;
 #pragma unroll
       for (int r = 0; r < ROUNDS; ++r)
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          if (4 * (tid + r * kThreads) + k == at) x[r][k] = -__builtin_inff();
+          if (4 * (lane + 64 * r) + k == at) x[r][k] = -__builtin_inff();
     }
     float top = -__builtin_inff();
     bool odd = false;
@@ -198,63 +282,94 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(VerifyParams p) {
     top = wave_max(top);
     const float ref = top > -__builtin_inff() ? top : 0.f;
     float sum = 0.f;
-    Best best = {-__builtin_inf(), INT32_MAX};
+    Two two = {-__builtin_inff(), -__builtin_inff(), INT32_MAX};
+    auto look = [&](float score, int at) {
+      two.second = __builtin_amdgcn_fmed3f(score, two.best, two.second);
+      two.token = score > two.best ? at : two.token;
+      two.best = fmaxf(two.best, score);
+    };
 #pragma unroll
     for (int r = 0; r < ROUNDS; ++r)
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        if (MODE != kGreedy) sum += fast_exp2((x[r][k] - ref) * c);
-        const double score = MODE == kChosen ? fma((double)x[r][k] - (double)ref, by, (double)noise[r][k]) : (double)x[r][k];
-        if (score > best.score) best = Best{score, v0 + 4 * (tid + r * kThreads) + k};
+        const float d = x[r][k] - ref;
+        if (MODE != kGreedy) sum += fast_exp2(d * c);
+        if (MODE != kDrawn) look(MODE != kChosen ? d : fmaf(d, by, greedy ? 0.f : noise[r][k]), v0 + 4 * (lane + 64 * r) + k);
       }
-    best = wave_best(best);
-    sum = MODE == kGreedy ? (__any(odd) ? __builtin_nanf("") : 0.f) : wave_sum(sum);
-    if (lane == 0) waves[tid / 64] = RowSlice{(double)sum, best.score, top, best.token};
-    __syncthreads();
-    if (tid == 0) {
-      RowSlice all = waves[0];
+    if (MODE == kDrawn && greedy) {
 #pragma unroll
-      for (int w = 1; w < kThreads / 64; ++w) {
-        const RowSlice more = waves[w];
-        const float t = fmaxf(all.top, more.top);
-        if (MODE != kGreedy && t > -__builtin_inff()) {
-          all.sum = all.sum * (double)fast_exp2((all.top - t) * c) + more.sum * (double)fast_exp2((more.top - t) * c);
-        } else {
-          all.sum += more.sum;
-        }
-        const Best better_one = better(shifted<MODE>(Best{all.best, all.token}, all.top, t, by), shifted<MODE>(Best{more.best, more.token}, more.top, t, by));
-        all.top = t;
-        all.best = better_one.score;
-        all.token = better_one.token;
-      }
-      p.part[((int64_t)b * p.T + u) * p.slices + blockIdx.x] = all;
+      for (int r = 0; r < ROUNDS; ++r)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) look(x[r][k] - ref, v0 + 4 * (lane + 64 * r) + k);
     }
-    __syncthreads();
+    if (MODE != kDrawn || greedy) {
+      two = two_of_wave(two);
+    }
+    sum = MODE == kGreedy ? (__any(odd) ? __builtin_nanf("") : 0.f) : wave_sum(sum);
+    if (lane == 0) {
+      const int64_t at = ((int64_t)b * p.T + u) * p.slices + slice;
+      p.part[at] = f32x4{sum, top, two.best, two.second};
+      p.part_token[at] = two.token;
+    }
   }
 }
 
-// A row's slices as one: every lane has the result.
-template <int MODE> __device__ __forceinline__ RowSlice join_row(const VerifyParams& p, int b, int u, double by, int lane) {
-  const RowSlice* part = p.part + ((int64_t)b * p.T + u) * p.slices;
+// The parts of a row as one, `group` lanes for it, all of which have the result.
+template <int MODE> __device__ __forceinline__ RowPart<double> join_row(const VerifyParams& p, int b, int u, double by, int lane, int group) {
+  constexpr int U = 4;      // parts that a lane asks for at once
+  const int64_t first = ((int64_t)b * p.T + u) * p.slices;
+  const float c = (float)fmin(by * 1.4426950408889634, 1e30);
   float top = -__builtin_inff();
   double sum = 0.0;
-  Best best = {-__builtin_inf(), INT32_MAX};
-  for (int i = lane; i < p.slices; i += 64) {
-    const RowSlice s = part[i];
-    const float t = fmaxf(top, s.top);
-    if (MODE == kGreedy || !(t > -__builtin_inff())) sum += s.sum;
-    else sum = sum * exp(((double)top - t) * by) + s.sum * exp(((double)s.top - t) * by);
-    best = better(shifted<MODE>(best, top, t, by), shifted<MODE>(Best{s.best, s.token}, s.top, t, by));
-    top = t;
+  Two two = {-__builtin_inff(), -__builtin_inff(), INT32_MAX};
+  auto towards = [&](Two x, float from, float to) {      // (relative to `to`)
+    const float d = to > from ? (float)(((double)from - (double)to) * by) : 0.f;
+    return Two{x.best + d, x.second + d, x.token};
+  };
+  auto scaled = [&](double s, float from, float to) { return MODE == kGreedy || !(to > from) ? s : s * (double)fast_exp2((from - to) * c); };
+  for (int i0 = lane; i0 < p.slices; i0 += U * group) {
+    f32x4 s[U];
+    int token[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int64_t at = first + min(i0 + i * group, p.slices - 1);
+      s[i] = p.part[at];
+      token[i] = p.part_token[at];
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      if (i0 + i * group >= p.slices) break;
+      const float t = fmaxf(top, s[i][1]);
+      sum = scaled(sum, top, t) + scaled((double)s[i][0], s[i][1], t);
+      two = both(towards(two, top, t), towards(Two{s[i][2], s[i][3], token[i]}, s[i][1], t));
+      top = t;
+    }
   }
-  const float t = wave_max(top);
-  if (MODE != kGreedy && t > -__builtin_inff()) sum *= exp(((double)top - t) * by);
-  sum = wave_sum64(sum);
-  best = wave_best(shifted<MODE>(best, top, t, by));
-  return RowSlice{sum, best.score, t, best.token};
+  const float t = wave_max(top, group);
+  sum = wave_sum64(scaled(sum, top, t), group);
+  two = wave_two(towards(two, top, t), group);
+  return RowPart<double>{sum, t, two.best, two.second, two.token};
+}
+// All rows of a tree, by the wavefronts of a workgroup.
+template <int MODE> __device__ __forceinline__ void join_rows(const VerifyParams& p, int b, int n, double by, RowPart<double>* rows) {
+  int group = 1;
+  while (group < 64 && group < p.slices) group *= 2;
+  const int per_wave = 64 / group, lane = threadIdx.x & 63, sub = lane / group;
+  for (int u0 = (threadIdx.x >> 6) * per_wave; u0 < n; u0 += blockDim.x / 64 * per_wave) {
+    const int u = min(u0 + sub, n - 1);
+    const RowPart<double> row = join_row<MODE>(p, b, u, by, lane % group, group);
+    if (lane % group == 0) rows[u] = row;
+  }
 }
 
-// The nodes of a tree, four to a lane of a wavefront, and the walk's results.
+// exp(d), d <= 0, to what fp32's exponential leaves, 2^-23: the argument is held in 64 bits.
+__device__ __forceinline__ double exp_of(double d) {
+  const double y = fmax(d * 1.4426950408889634, -1000.0);
+  const float h = (float)y;
+  return (double)fast_exp2(h) * (1.0 + (y - (double)h) * 0.6931471805599453);
+}
+
+// The nodes of a tree, four to a lane of a wavefront.
 struct Tree { int n; int parent[4], token[4]; };
 __device__ __forceinline__ Tree tree_of(const VerifyParams& p, int b, int lane) {
   Tree t;
@@ -267,161 +382,205 @@ __device__ __forceinline__ Tree tree_of(const VerifyParams& p, int b, int lane) 
   }
   return t;
 }
+__device__ __forceinline__ double lane_of(double x, int lane) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)u, lane), hi = __builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ float lane_of(float x, int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane)); }
 
 // A workgroup per sequence: its wavefronts join the slices of the rows, one of them walks.
+constexpr int kWalkThreads = 512;
 template <int E, int MODE>
-__global__ __launch_bounds__(kThreads) void verify_walk_kernel(VerifyParams p) {
-  __shared__ RowSlice rows[kMostNodes];
+__global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams p) {
+  __shared__ RowPart<double> rows[kMostNodes];
   __shared__ int path[kMostNodes];
+  __shared__ Best bests[kWalkThreads / 64];
+  __shared__ int unsure;                  // the row whose best token fp32 does not tell
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   const double inv_t = MODE == kGreedy ? 0.0 : inverse_temperature(p, b);
   const bool greedy = inv_t == 0.0;
   const double by = greedy ? 1.0 : inv_t;
-  const int n = nodes_of(p, b);
-  Tree t;
-  float x[4], a[4];
+  const int n = nodes_of(p, b), groups = (n + 63) / 64;
+  Tree t = {};
+  float x[4], a[4];      // the nodes' scores in their parents' rows, and their numbers
   if (wv == 0) {
     t = tree_of(p, b, lane);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const bool child = t.parent[k] >= 0 && t.token[k] >= 0;
-      x[k] = child ? score_at<E>(row_of_x<E>(p, b, t.parent[k]), t.token[k]) : -__builtin_inff();
+      x[k] = child && MODE != kGreedy ? score_at<E>(row_of_x<E>(p, b, t.parent[k]), t.token[k]) : -__builtin_inff();
       a[k] = child && !greedy ? p.accept[b * p.accept_sb + 64 * k + lane] : 0.f;
     }
   }
-  for (int u = wv; u < n; u += kThreads / 64) {
-    const RowSlice row = join_row<MODE>(p, b, u, by, lane);
-    if (lane == 0) rows[u] = row;
-  }
   if (tid < p.T) path[tid] = -1;
+  if (tid == 0) unsure = -1;
+  join_rows<MODE>(p, b, n, by, rows);
   __syncthreads();
+  int at = n > 0 ? 0 : -1, count = 0, token = -1;
   if (wv == 0) {
-    int at = n > 0 ? 0 : -1, count = 0, token = -1;
     while (at >= 0) {
       if (lane == 0) path[count] = at;
       ++count;
-      const RowSlice row = rows[at];
-      uint64_t kids[4];
-      float ref = row.top;
+      const RowPart<double> row = rows[at];
+      uint64_t kids[4], any = 0;
+      bool several = false;      // more than one child
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const bool kid = t.parent[k] == at && t.token[k] >= 0;
-        kids[k] = __ballot(kid);
-        if (!greedy) ref = fmaxf(ref, wave_max(kid ? x[k] : -__builtin_inff()));
+        kids[k] = k < groups ? __ballot(t.parent[k] == at && t.token[k] >= 0) : 0;
+        several |= any != 0 && kids[k] != 0;
+        any |= kids[k];
       }
       int accepted = -1;
       if (greedy) {
         if (row.sum == row.sum) {      // (NaN: a score that is none)
 #pragma unroll
           for (int k = 3; k >= 0; --k) {
-            const uint64_t same = kids[k] & __ballot(t.token[k] == row.token);
+            const uint64_t same = kids[k] != 0 ? kids[k] & __ballot(t.token[k] == row.token) : 0;
             if (same) accepted = 64 * k + __builtin_ctzll(same);
           }
-          token = row.token == INT32_MAX ? -1 : row.token;
+          if (accepted < 0 && row.token != INT32_MAX) token = row.token;
         }
       } else {
-        // the children's e, each token once, and the sum of all that may follow
-        double e[4], left = ref > -__builtin_inff() && row.top > -__builtin_inff() ? row.sum * exp(((double)row.top - ref) * by) : row.sum;
-        double of_kids = 0.0;
+        double left = row.sum;
+        const auto possible = [](double sum) { return sum > 0.0 && sum < __builtin_inf(); };      // (not NaN either)
+        if (any && !several && !(any & (any - 1))) {
+          // one child, as in chains: no sums over lanes
+          const int from = __builtin_ctzll(any);
+          float x_c = 0.f, a_c = 0.f;
+          int c = 0;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          e[k] = 0.0;
-          if (kids[k] == 0) continue;
-          const bool kid = kids[k] >> lane & 1;
-          bool again = false;
-          for (int g = 0; g <= k; ++g) {
-            for (uint64_t rest = kids[g]; rest; rest &= rest - 1) {
-              const int from = __builtin_ctzll(rest);
-              const int y = g == 0 ? __builtin_amdgcn_readlane(t.token[0], from) : g == 1 ? __builtin_amdgcn_readlane(t.token[1], from)
-                          : g == 2 ? __builtin_amdgcn_readlane(t.token[2], from) : __builtin_amdgcn_readlane(t.token[3], from);
-              again |= y == t.token[k] && 64 * g + from < 64 * k + lane;
-            }
-          }
-          if (kid && !again) e[k] = x[k] > -__builtin_inff() ? exp(((double)x[k] - ref) * by) : x[k] == x[k] ? 0.0 : (double)x[k];
-          of_kids += e[k];
-        }
-        left += wave_sum64(of_kids);
-        if (left > 0.0 && left < __builtin_inf()) {
+          for (int k = 0; k < 4; ++k)
+            if (kids[k]) { x_c = lane_of(x[k], from); a_c = lane_of(a[k], from); c = 64 * k + from; }
+          const float ref = fmaxf(row.top, x_c);
+          if (ref > row.top && row.top > -__builtin_inff()) left *= exp_of(((double)row.top - ref) * by);
+          const double w = x_c > -__builtin_inff() ? exp_of(((double)x_c - ref) * by) : x_c == x_c ? 0.0 : (double)x_c;
+          left += w;
+          if (possible(left) && (double)a_c * left < w) accepted = c;
+        } else if (any) {
+          // the children's e, each token once, and the sum of all that may follow
+          float ref = row.top;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (kids[k]) ref = fmaxf(ref, wave_max(kids[k] >> lane & 1 ? x[k] : -__builtin_inff()));
+          if (ref > row.top && row.top > -__builtin_inff()) left *= exp_of(((double)row.top - ref) * by);
+          double e[4], of_kids = 0.0;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            for (uint64_t rest = kids[k]; rest && accepted < 0; rest &= rest - 1) {
-              const int from = __builtin_ctzll(rest);
-              const double w = __shfl(e[k], from);
-              if ((double)__shfl(a[k], from) * left < w) accepted = 64 * k + from;
-              left -= w;
+            e[k] = 0.0;
+            if (kids[k] == 0) continue;
+            bool twice = false;
+            if (several || (any & (any - 1))) {
+#pragma unroll
+              for (int g = 0; g <= k; ++g)
+                for (uint64_t todo = kids[g]; todo; todo &= todo - 1) {
+                  const int from = __builtin_ctzll(todo);
+                  twice |= __builtin_amdgcn_readlane(t.token[g], from) == t.token[k] && 64 * g + from < 64 * k + lane;
+                }
+            }
+            if ((kids[k] >> lane & 1) && !twice) e[k] = x[k] > -__builtin_inff() ? exp_of(((double)x[k] - ref) * by) : x[k] == x[k] ? 0.0 : (double)x[k];
+            of_kids += e[k];
+          }
+          left += wave_sum64(of_kids);
+          if (possible(left)) {
+            double rest = left;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              for (uint64_t todo = kids[k]; todo && accepted < 0; todo &= todo - 1) {
+                const int from = __builtin_ctzll(todo);
+                const double w = lane_of(e[k], from);
+                if ((double)lane_of(a[k], from) * rest < w) accepted = 64 * k + from;
+                rest -= w;
+              }
             }
           }
+        }
+        if (accepted < 0 && possible(left)) {
           token = row.token == INT32_MAX ? -1 : row.token;
+          if (token >= 0 && too_near(row.best, row.second) && lane == 0) unsure = at;
         }
       }
       at = accepted;
-      if (at >= 0) token = -1;
-    }
-    if (lane == 0) {
-      p.counts[b] = count;
-      p.next[b] = token;
     }
   }
   __syncthreads();
+  if (MODE != kGreedy && unsure >= 0) {
+    // in 64 bits, by everybody
+    const void* row = row_of_x<E>(p, b, unsure);
+    const float* noise = p.noise + b * p.noise_sb;
+    const double top = (double)rows[unsure].top;
+    Best best = {-__builtin_inf(), INT32_MAX};
+    for (int v = tid; v < p.V; v += kWalkThreads) {
+      const double score = ((double)score_at<E>(row, v) - top) * by + (double)noise[v];
+      if (!(score >= best.score)) continue;
+      bool taken = false;
+      for (int i = unsure + 1; i < n; ++i) taken |= parent_of(p, b, i) == unsure && token_of(p, b, i) == v;
+      if (!taken) best = better(best, Best{score, v});
+    }
+    best = wave_best(best);
+    if (lane == 0) bests[wv] = best;
+    __syncthreads();
+    if (tid == 0) {
+#pragma unroll
+      for (int w = 1; w < kWalkThreads / 64; ++w) best = better(best, bests[w]);
+      token = best.score > -__builtin_inf() ? best.token : -1;
+    }
+  }
+  if (tid == 0) {
+    p.counts[b] = count;
+    p.next[b] = token;
+  }
   if (tid < p.T) p.path[(int64_t)b * p.T + tid] = path[tid];
 }
 
-// Drawn children: a workgroup per sequence goes over a whole row where a rejection has to be taken out of it for the child behind, and once at the end.  The first
-// wavefront walks and tells the others what to do: nobody decides by numbers that it has read by itself.
+// Drawn children: a workgroup per sequence goes over a whole row where a rejection has to be taken out of it for the child behind.  The first wavefront walks and tells the others what
+// to do: nobody decides by numbers that it has read by itself.
 constexpr int kDrawThreads = 1024;
-enum PassKind { kEnd, kSum, kSample };
-struct Pass { PassKind kind; int at; double scale, less; };
 template <int E>
 __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyParams p) {
-  __shared__ RowSlice rows[kMostNodes];
+  __shared__ RowPart<double> rows[kMostNodes];
   __shared__ int path[kMostNodes];
-  __shared__ Pass todo;
+  __shared__ Left todo;
   __shared__ double sums[kDrawThreads / 64];
-  __shared__ Best bests[kDrawThreads / 64];
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   const double inv_t = inverse_temperature(p, b);
   const bool greedy = inv_t == 0.0;
   const double by = greedy ? 1.0 : inv_t;
   const float c = (float)fmin(by * 1.4426950408889634, 1e30);
   const int n = nodes_of(p, b);
-  for (int u = wv; u < n; u += kDrawThreads / 64) {
-    const RowSlice row = join_row<kDrawn>(p, b, u, by, lane);
-    if (lane == 0) rows[u] = row;
-  }
-  if (tid < p.T) path[tid] = -1;
   Tree t = {};
   if (wv == 0) t = tree_of(p, b, lane);
+  // (what the children are tried with, for all of them at once: numbers, probabilities and scores)
+  float a[4], q[4], x[4];
+  if (wv == 0) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const bool child = t.parent[k] >= 0 && t.token[k] >= 0 && !greedy;
+      a[k] = child ? p.accept[b * p.accept_sb + 64 * k + lane] : 0.f;
+      q[k] = child ? p.q[b * p.q_sb + t.parent[k] * p.q_st + t.token[k]] : 0.f;
+      x[k] = child ? score_at<E>(row_of_x<E>(p, b, t.parent[k]), t.token[k]) : 0.f;
+    }
+  }
+  join_rows<kDrawn>(p, b, n, by, rows);
+  if (tid < p.T) path[tid] = -1;
   __syncthreads();
-  // the first wavefront's: where it is, the child that it has looked at last, what is left of the row, max(scale e - less q, 0)
+  // the first wavefront's: where it is, the child that it has looked at last, what is left of the row
   int at = n > 0 ? 0 : -1, last = 0, count = 0;
   double scale = 0.0, less = 0.0;
-  bool fresh = true, rejected = false, again = false;      // rejected: the last child, and it is not taken out yet; again: nothing was left
-  PassKind asked = kEnd;
+  bool fresh = true, rejected = false, summed = false;      // rejected: the last child, and it is not taken out yet; summed: the row's sum without it is there
   int64_t token = -1;
+  Left sample = {0.0, 0.0, -1, 0.f};
   for (;;) {
     if (wv == 0) {
-      Pass next = {kEnd, 0, 0.0, 0.0};
-      bool summed = asked == kSum;      // (the row's sum is there: the child that it was asked for can be looked at)
+      Left next = {0.0, 0.0, -1, 0.f};
       if (summed) {
-        double z = lane < kDrawThreads / 64 ? sums[lane] : 0.0;
-        z = wave_sum64(z);
+        const double z = wave_sum64(lane < kDrawThreads / 64 ? sums[lane] : 0.0);
         scale = z > 0.0 ? scale / z : 1.0 / rows[at].sum;
         less = z > 0.0 ? less / z : 0.0;
       }
       bool walking = at >= 0;
-      if (asked == kSample) {
-        const Best best = wave_best(lane < kDrawThreads / 64 ? bests[lane] : Best{0.0, INT32_MAX});
-        if (best.token == INT32_MAX && !again) {
-          again = true;
-          next = Pass{kSample, at, 1.0 / rows[at].sum, 0.0};
-        } else {
-          token = best.token == INT32_MAX ? -1 : best.token;
-        }
-        walking = false;
-      }
-      asked = kEnd;
       while (walking) {
-        const RowSlice row = rows[at];
+        const RowPart<double> row = rows[at];
         if (fresh) {
           if (lane == 0) path[count] = at;
           ++count;
@@ -431,7 +590,8 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyParams 
           rejected = fresh = false;
         }
         // the next child
-        int j = -1, y = 0;
+        int j = -1;
+        double q_j = 0.0, a_j = 0.0, x_j = 0.0;
 #pragma unroll
         for (int k = 3; k >= 0; --k) {
           bool kid = t.parent[k] == at && t.token[k] >= 0 && 64 * k + lane > last;
@@ -440,7 +600,9 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyParams 
           if (kids) {
             const int from = __builtin_ctzll(kids);
             j = 64 * k + from;
-            y = __builtin_amdgcn_readlane(t.token[k], from);
+            q_j = lane_of(q[k], from);
+            a_j = lane_of(a[k], from);
+            x_j = lane_of(x[k], from);
           }
         }
         if (!(greedy ? row.sum == row.sum : row.sum > 0.0 && row.sum < __builtin_inf())) {
@@ -451,17 +613,16 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyParams 
           fresh = true;
           if (j >= 0) at = j;
         } else if (j < 0) {
-          next = Pass{kSample, at, scale, rejected ? less + 1.0 : less};
+          sample = Left{scale, rejected ? less + 1.0 : less, at, row.top};
           walking = false;
         } else if (rejected && !summed) {
           less += 1.0;
-          next = Pass{kSum, at, scale, less};
+          next = Left{scale, less, at, row.top};
           walking = false;
         } else {
           summed = false;
-          const double q = p.q[b * p.q_sb + at * p.q_st + y];
-          const double left = fmax(scale * exp(((double)score_at<E>(row_of_x<E>(p, b, at), y) - row.top) * by) - less * q, 0.0);
-          if ((double)p.accept[b * p.accept_sb + j] * q < left) {
+          const double left = fmax(scale * exp_of((x_j - (double)row.top) * by) - less * q_j, 0.0);
+          if (a_j * q_j < left) {
             at = j;
             fresh = true;
           } else {
@@ -470,74 +631,161 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyParams 
           }
         }
       }
-      asked = next.kind;
+      summed = next.at >= 0;
       if (lane == 0) todo = next;
     }
     __syncthreads();
-    const Pass pass = todo;
-    if (pass.kind == kEnd) break;
+    const Left pass = todo;
+    if (pass.at < 0) break;
     const void* x_row = row_of_x<E>(p, b, pass.at);
     const float* q_row = p.q + b * p.q_sb + pass.at * p.q_st;
-    const float* g_row = p.noise + b * p.noise_sb;
-    const float top = rows[pass.at].top, s32 = (float)pass.scale, l32 = (float)pass.less;
-    const bool sample = pass.kind == kSample;
+    const float top = pass.top, s32 = (float)pass.scale, l32 = (float)pass.less;
     double total = 0.0;
-    Best mine = {0.0, INT32_MAX};
     for (int v = 4 * tid; v < p.V; v += 4 * kDrawThreads) {
-      const f32x4 x = widen4<E>(load4<E>(x_row, v, p.V - v)), q = load4_f32(q_row, v, p.V - v);
-      const f32x4 g = sample ? load4_f32(g_row, v, p.V - v) : f32x4{0.f, 0.f, 0.f, 0.f};
+      const f32x4 xs = widen4<E>(load4<E>(x_row, v, p.V - v)), qs = load4_f32(q_row, v, p.V - v);
       float sum = 0.f;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float r = fmaxf(fmaf(s32, fast_exp2((x[k] - top) * c), -l32 * q[k]), 0.f);
-        sum += r;
-        const double key = (double)r * (double)fast_exp2(g[k] * kLog2e);
-        if (sample && key > mine.score) mine = Best{key, v + k};
-      }
+      for (int k = 0; k < 4; ++k) sum += fmaxf(fmaf(s32, fast_exp2((xs[k] - top) * c), -l32 * qs[k]), 0.f);
       total += (double)sum;
     }
     total = wave_sum64(total);
-    mine = wave_best(mine);
-    if (lane == 0) { sums[wv] = total; bests[wv] = mine; }
+    if (lane == 0) sums[wv] = total;
     __syncthreads();
   }
   if (tid == 0) {
     p.counts[b] = count;
     p.next[b] = token;
+    p.left[b] = sample;
   }
   if (tid < p.T) p.path[(int64_t)b * p.T + tid] = path[tid];
 }
 
-// The slices: as long as leaves the chip enough workgroups, and then as many rows to a workgroup, which share the noise.
-struct VerifySplit { int rounds, slice, slices, rows; };
+// What is left of the last row with its noise, the largest of it: max(scale e - less q, 0) exp(noise).  A workgroup takes a piece of the row.
+template <int E>
+__global__ __launch_bounds__(kThreads) void verify_sample_kernel(VerifyParams p) {
+  __shared__ Two twos[kThreads / 64];
+  const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  const Left left = p.left[b];
+  if (left.at < 0) return;
+  const double by = inverse_temperature(p, b);
+  const float c = (float)fmin(by * 1.4426950408889634, 1e30), s32 = (float)left.scale, l32 = (float)left.less, top = left.top;
+  const void* x_row = row_of_x<E>(p, b, left.at);
+  const float *q_row = p.q + b * p.q_sb + left.at * p.q_st, *g_row = p.noise + b * p.noise_sb;
+  Two two = {0.f, 0.f, INT32_MAX};
+  constexpr int R = kPieceRounds;
+  typename Four<E>::Raw raw[R];
+  f32x4 q[R], g[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int v = blockIdx.x * kPiece + 4 * (tid + r * kThreads);
+    raw[r] = load4<E>(x_row, v, p.V - v);
+    q[r] = load4_f32(q_row, v, p.V - v);
+    g[r] = load4_f32(g_row, v, p.V - v);
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const f32x4 x = widen4<E>(raw[r]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float key = fmaxf(fmaf(s32, fast_exp2((x[k] - top) * c), -l32 * q[r][k]), 0.f) * fast_exp2(g[r][k] * kLog2e);
+      two.second = __builtin_amdgcn_fmed3f(key, two.best, two.second);
+      two.token = key > two.best ? (int)(blockIdx.x * kPiece) + 4 * (tid + r * kThreads) + k : two.token;
+      two.best = fmaxf(two.best, key);
+    }
+  }
+  two = wave_two(two);
+  if (lane == 0) twos[wv] = two;
+  __syncthreads();
+  if (tid == 0) {
+#pragma unroll
+    for (int w = 1; w < kThreads / 64; ++w) two = both(two, twos[w]);
+    const int64_t at = (int64_t)b * p.pieces + blockIdx.x;
+    p.drawn[at] = float2{two.best, two.second};
+    p.drawn_token[at] = two.token;
+  }
+}
+
+// The pieces as one.  (Not by the last workgroup of a sequence's to come in the kernel above: its fences write back the L2s, 147 us for 64 rows of 131072 where the draw itself takes 17.)
+template <int E>
+__global__ __launch_bounds__(kThreads) void verify_last_kernel(VerifyParams p) {
+  __shared__ Two twos[kThreads / 64];
+  __shared__ Best bests[kThreads / 64];
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  Two two = Two{0.f, 0.f, INT32_MAX};
+  for (int i = tid; i < p.pieces; i += kThreads) {
+    const float2 f = p.drawn[(int64_t)b * p.pieces + i];
+    two = both(two, Two{f.x, f.y, p.drawn_token[(int64_t)b * p.pieces + i]});
+  }
+  const Left left = p.left[b];
+  if (left.at < 0) return;
+  two = wave_two(two);
+  if (lane == 0) twos[wv] = two;
+  __syncthreads();
+  two = twos[0];
+#pragma unroll
+  for (int w = 1; w < kThreads / 64; ++w) two = both(two, twos[w]);
+  // (NaN and nothing at all look alike: nothing has been larger than zero)
+  if (two.token != INT32_MAX && two.best - two.second > 0x1p-16f * two.best) {
+    if (tid == 0) p.next[b] = two.token;
+    return;
+  }
+  const double by = inverse_temperature(p, b);
+  const float top = left.top;
+  const void* x_row = row_of_x<E>(p, b, left.at);
+  const float *q_row = p.q + b * p.q_sb + left.at * p.q_st, *g_row = p.noise + b * p.noise_sb;
+  // Too near to be told apart, or nothing that fp32 holds: in 64 bits, and where nothing is left, from the row as it was.
+  for (int whole = 0; whole < 2; ++whole) {
+    const double scale = whole ? 1.0 : left.scale, less = whole ? 0.0 : left.less;      // (a factor of all of them decides nothing)
+    Best best = {-__builtin_inf(), INT32_MAX};
+    for (int v = tid; v < p.V; v += kThreads) {
+      const double rest = scale * exp(((double)score_at<E>(x_row, v) - (double)top) * by) - less * (double)q_row[v];
+      if (rest > 0.0) best = better(best, Best{log(rest) + (double)g_row[v], v});
+    }
+    best = wave_best(best);
+    __syncthreads();
+    if (lane == 0) bests[wv] = best;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; ++w) best = better(best, bests[w]);
+    if (best.token != INT32_MAX || whole) {
+      if (tid == 0) p.next[b] = best.token == INT32_MAX ? -1 : best.token;
+      return;
+    }
+  }
+}
+
+// The slices: as long as leaves the chip enough wavefronts, and then as many rows to a workgroup, which share the noise.
+struct VerifySplit { int rounds, slice, slices, rows, pieces; };
 static VerifySplit verify_split(int B, int T, int V) {
   VerifySplit s;
-  for (s.rounds = 8; s.rounds > 1; s.rounds /= 2)
+  for (s.rounds = 4; s.rounds > 1; s.rounds /= 2)
     if ((int64_t)B * T * ((V + 1024 * s.rounds - 1) / (1024 * s.rounds)) >= 1024) break;
-  s.slice = 4 * kThreads * s.rounds;
+  s.slice = 256 * s.rounds;
   s.slices = (V + s.slice - 1) / s.slice;
   s.rows = 1;
-  while (s.rows < T && (int64_t)B * ((T + 2 * s.rows - 1) / (2 * s.rows)) * s.slices >= 1024) s.rows *= 2;
+  while (s.rows < T && (int64_t)B * ((T + 2 * s.rows - 1) / (2 * s.rows)) * s.slices >= 16384) s.rows *= 2;
+  s.pieces = (V + kPiece - 1) / kPiece;
   return s;
 }
 
 template <int E, int MODE> static void rows_launch(const VerifyParams& p, int rounds, hipStream_t s) {
-  const dim3 grid((unsigned)p.slices, (unsigned)((p.T + p.rows - 1) / p.rows), (unsigned)p.B);
+  const dim3 grid((unsigned)((p.slices + kThreads / 64 - 1) / (kThreads / 64)), (unsigned)((p.T + p.rows - 1) / p.rows), (unsigned)p.B);
   if (rounds == 1) hipLaunchKernelGGL((verify_rows_kernel<E, MODE, 1>), grid, dim3(kThreads), 0, s, p);
   else if (rounds == 2) hipLaunchKernelGGL((verify_rows_kernel<E, MODE, 2>), grid, dim3(kThreads), 0, s, p);
-  else if (rounds == 4) hipLaunchKernelGGL((verify_rows_kernel<E, MODE, 4>), grid, dim3(kThreads), 0, s, p);
-  else hipLaunchKernelGGL((verify_rows_kernel<E, MODE, 8>), grid, dim3(kThreads), 0, s, p);
+  else hipLaunchKernelGGL((verify_rows_kernel<E, MODE, 4>), grid, dim3(kThreads), 0, s, p);
 }
 template <int E> static void verify_launch(const VerifyParams& p, int rounds, hipStream_t s) {
   if (p.q != nullptr) {
     rows_launch<E, kDrawn>(p, rounds, s);
     hipLaunchKernelGGL((verify_draw_kernel<E>), dim3((unsigned)p.B), dim3(kDrawThreads), 0, s, p);
+    hipLaunchKernelGGL((verify_sample_kernel<E>), dim3((unsigned)p.pieces, (unsigned)p.B), dim3(kThreads), 0, s, p);
+    hipLaunchKernelGGL((verify_last_kernel<E>), dim3((unsigned)p.B), dim3(kThreads), 0, s, p);
   } else if (p.noise != nullptr) {
     rows_launch<E, kChosen>(p, rounds, s);
-    hipLaunchKernelGGL((verify_walk_kernel<E, kChosen>), dim3((unsigned)p.B), dim3(kThreads), 0, s, p);
+    hipLaunchKernelGGL((verify_walk_kernel<E, kChosen>), dim3((unsigned)p.B), dim3(kWalkThreads), 0, s, p);
   } else {
     rows_launch<E, kGreedy>(p, rounds, s);
-    hipLaunchKernelGGL((verify_walk_kernel<E, kGreedy>), dim3((unsigned)p.B), dim3(kThreads), 0, s, p);
+    hipLaunchKernelGGL((verify_walk_kernel<E, kGreedy>), dim3((unsigned)p.B), dim3(kWalkThreads), 0, s, p);
   }
 }
 
@@ -549,7 +797,9 @@ static bool verify_shape_ok(int B, int T, int V) { return B > 0 && B <= 65535 &&
 
 extern "C" size_t daisy_verify_workspace_bytes(int B, int T, int V) {
   if (!verify_shape_ok(B, T, V)) return 0;
-  return (size_t)B * T * verify_split(B, T, V).slices * sizeof(RowSlice);
+  const VerifySplit s = verify_split(B, T, V);
+  const size_t parts = (size_t)B * T * s.slices * (sizeof(f32x4) + sizeof(int32_t));      // (then each sequence's, a multiple of 8)
+  return (parts + 15) / 16 * 16 + (size_t)B * sizeof(Left) + (size_t)B * s.pieces * (sizeof(float2) + sizeof(int32_t));
 }
 
 extern "C" int daisy_verify_fwd(const void* logits, const int64_t* logits_strides, int type, const void* tokens, int64_t tokens_stride, int tokens_are_int64,
@@ -583,8 +833,13 @@ extern "C" int daisy_verify_fwd(const void* logits, const int64_t* logits_stride
     if (draft) { p.q = draft; p.q_sb = draft_strides[0]; p.q_st = draft_strides[1]; }
   }
   p.path = path; p.counts = counts; p.next = next;
-  p.part = (RowSlice*)workspace;
-  p.B = B; p.T = T; p.V = V; p.slices = sp.slices; p.slice = sp.slice; p.rows = sp.rows;
+  const size_t parts = (size_t)B * T * sp.slices;
+  p.part = (f32x4*)workspace;
+  p.part_token = (int32_t*)(p.part + parts);
+  p.left = (Left*)((char*)workspace + (parts * (sizeof(f32x4) + sizeof(int32_t)) + 15) / 16 * 16);
+  p.drawn = (float2*)(p.left + B);
+  p.drawn_token = (int32_t*)(p.drawn + (size_t)B * sp.pieces);
+  p.B = B; p.T = T; p.V = V; p.slices = sp.slices; p.slice = sp.slice; p.rows = sp.rows; p.pieces = sp.pieces;
   hipStream_t s = (hipStream_t)stream;
   if (type == kScoreF32) verify_launch<kScoreF32>(p, sp.rounds, s);
   else if (type == kScoreBf16) verify_launch<kScoreBf16>(p, sp.rounds, s);
