@@ -14,7 +14,7 @@ struct MoveParams {
   int32_t* status;
 };
 
-constexpr int kMoveRows = 64;      // rows whose places a workgroup looks up at once
+constexpr int kOrderedRows = 64, kMoveRows = 16;  // rows whose places a workgroup looks up at once
 
 // Where a place lies: element offsets of its row in the pages of k and of v (-1: nowhere).
 struct Place { int page, slot; };
@@ -35,14 +35,20 @@ __device__ __forceinline__ Place place_of(const MoveParams& p, int seq, int pos,
 // A thread has 16 bytes of a head of a layer, of k or of v, and moves them for one row after the other, U at once.  With an index that only rises no row is
 // read behind being written: row i goes to a place no later than its own, and those behind it come from later ones.  ORDERED: with an index, one workgroup
 // has all rows of a sequence; otherwise a workgroup has kMoveRows of them (rows keep their places, in another sequence's pages).
+//
+// Bound by memory: each row is read and written once.  Stores go past the caches, since the next reader of a row is a layer's attention, long behind the call:
+// 19.9 us against 22.9 for the paths of 64 sequences (4 rows of 16 layers, 8 heads of 128: 100 MB in all).  Loads of copied pages do too, since no row is read
+// twice, with 16 rows a workgroup: 96 copies of up to 127 rows (316 MB read, as many written, of which the caches hold one part) take 130 to 145 us, against
+// 155 to 159 with 64 rows a workgroup and cached accesses, 150 with 32 rows and 217 with 8.  Rows just drafted are read from the caches, so an index's loads
+// stay ordinary ones (21.0 us otherwise).
 template <bool ORDERED>
 __global__ __launch_bounds__(256) void paged_move_kernel(MoveParams p) {
-  constexpr int U = 8;
-  __shared__ int4 places[kMoveRows];      // page and slot from, page and slot to; page -1: not to be moved
+  constexpr int U = 8, ROWS = ORDERED ? kOrderedRows : kMoveRows;
+  __shared__ int4 places[ROWS];      // page and slot from, page and slot to; page -1: not to be moved
   const int b = blockIdx.z;
   const int start = p.starts[b], count = start < 0 ? 0 : min(p.counts[b], p.rows);
   const int source = p.sources != nullptr ? p.sources[b] : b;
-  int row0 = ORDERED ? 0 : (int)blockIdx.y * kMoveRows;
+  int row0 = ORDERED ? 0 : (int)blockIdx.y * ROWS;
   if (row0 >= count) return;
   const int32_t* index = ORDERED ? p.index + b * p.index_st : nullptr;
   if (ORDERED) {
@@ -60,8 +66,8 @@ __global__ __launch_bounds__(256) void paged_move_kernel(MoveParams p) {
   const bool mine = piece.of < p.combos;
   uint16_t* base = p.pages[w] + (mine ? head.of * p.sl[w] + head.rest * p.sh[w] + 8 * piece.rest : 0);
   const int64_t sp = p.sp[w], ss = p.ss[w];
-  for (;; row0 += kMoveRows) {
-    const int n = min(count - row0, kMoveRows);
+  for (;; row0 += ROWS) {
+    const int n = min(count - row0, ROWS);
     if (ORDERED && row0 > 0) __syncthreads();
     if ((int)threadIdx.x < n) {
       const int i = row0 + threadIdx.x;
@@ -80,16 +86,19 @@ __global__ __launch_bounds__(256) void paged_move_kernel(MoveParams p) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const int4 at = places[min(i0 + u, n - 1)];
-          if (i0 + u < n && at.x >= 0) held[u] = *reinterpret_cast<const u32x4*>(base + at.x * sp + at.y * ss);
+          if (i0 + u < n && at.x >= 0) {
+            const u32x4* from = reinterpret_cast<const u32x4*>(base + at.x * sp + at.y * ss);
+            held[u] = ORDERED ? *from : __builtin_nontemporal_load(from);
+          }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const int4 at = places[min(i0 + u, n - 1)];
-          if (i0 + u < n && at.x >= 0) *reinterpret_cast<u32x4*>(base + at.z * sp + at.w * ss) = held[u];
+          if (i0 + u < n && at.x >= 0) __builtin_nontemporal_store(held[u], reinterpret_cast<u32x4*>(base + at.z * sp + at.w * ss));
         }
       }
     }
-    if (!ORDERED || row0 + kMoveRows >= count) return;
+    if (!ORDERED || row0 + ROWS >= count) return;
   }
 }
 
