@@ -499,7 +499,7 @@ class CausalSelfAttention(nn.Module):
         out = torch.empty(3, N, H, D, dtype=torch.bfloat16, device=x.device) if prompt else (None, None, None)
         q = ops.paged_append(qkv[:, H:2 * H], qkv[:, 2 * H:], ctx.k_pages, ctx.v_pages, ctx.page_table, ctx.positions, rows=ctx.rows, q=qkv[:, :H],
                              cos=self.rotary.cos, sin=self.rotary.sin, eps=NORM_EPS_BF16, ve=ve, gate=gate, q_out=out[0], k_out=out[1], v_out=out[2],
-                             status=ctx.status)
+                             status=ctx.status, slots=None if ctx.tree is None else ctx.tree.slots)
         return (q, out[1], out[2]) if prompt else q
 
     def _attend_paged(self, x: Tensor, ve: Optional[Tensor], mask: WindowMask, window: Optional[int]):
@@ -511,9 +511,11 @@ class CausalSelfAttention(nn.Module):
         return y, q[None], k[None].transpose(1, 2), v[None].transpose(1, 2)
 
     def _step_paged(self, x: Tensor, ctx: PagedContext, ve: Optional[Tensor], window: Optional[int]):
-        """One token of every sequence of a paged cache, at the positions that the device holds."""
+        """One token of every sequence of a paged cache, at the positions that the device holds; or the nodes of a tree of every sequence, behind one another in ``x``."""
         if ctx.window is not None and (window is None or window > ctx.window):
             raise ValueError(f"the paged cache keeps {ctx.window} positions, a window of {window} was asked for")
+        if ctx.tree is not None:
+            return self._step_tree(x, ctx, ve, window), None, None
         if self._fused_prep_ok():
             rot = _held(self._modules, self, "rotary")
             x, ve = _as_bf16(x), _as_bf16(ve) if self.receives_ve else None
@@ -529,6 +531,14 @@ class CausalSelfAttention(nn.Module):
                                 out=torch.empty(q.shape, dtype=torch.bfloat16, device=q.device), status=ctx.status)
         y = step_linear(o.view(B, 1, self.m_dim), self.qkvo_w[3])
         return y, None, None
+
+    def _step_tree(self, x: Tensor, ctx: PagedContext, ve: Optional[Tensor], window: Optional[int]) -> Tensor:
+        B, T = ctx.tree.mask.shape[:2]
+        torch._assert(x.size(0) == B * T, "the tokens of a tree are its nodes")
+        q = self._append_paged(x[:, 0], ve, ctx, False).view(B, T, self.num_heads, self.head_dim)
+        o = ops.paged_tree_attention(q, ctx.k_pages, ctx.v_pages, ctx.page_table, ctx.lens, ctx.tree.mask, nodes=ctx.nodes, window=window, scale=self.attn_scale,
+                                     out=torch.empty(q.shape, dtype=torch.bfloat16, device=q.device), status=ctx.status)
+        return step_linear(o.view(B * T, 1, self.m_dim), self.qkvo_w[3])
 
     # -- reference interface -----------------------------------------------
     def forward(self, x: Tensor, ve: Optional[Tensor], block_mask=None, attn_mask: MaskLike = None):
@@ -570,7 +580,7 @@ class CausalSelfAttention(nn.Module):
         replayed while the tensor counts up.
 
         With the ``PagedContext`` of a ``PagedKVCache`` layer every sequence is at a position of its own: ``pos`` is not looked at, the new rows
-        go into the pages, and ``None, None`` is returned for them.
+        go into the pages, and ``None, None`` is returned for them.  Where the context has a tree, B is the number of all sequences' nodes.
         """
         B = x.size(0)
         torch._assert(x.size(1) == 1, "step() requires single position only")

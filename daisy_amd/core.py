@@ -27,6 +27,7 @@ import torch
 import torch.nn.functional as F
 from torch import Tensor
 
+from . import ops
 from .attention import CausalSelfAttention, WindowMask, _held, build_window_mask, step_linear
 from .functional import norm
 from .kv_cache import KVCache, PagedKVCache
@@ -213,6 +214,49 @@ def step(model, token_ids: Tensor, cache: Union[KVCache, PagedKVCache], window: 
     return logits
 
 
+@torch.no_grad()
+def draft_step(model, tokens: Tensor, parents: Tensor, cache: PagedKVCache, nodes: Optional[Sequence[int]] = None, window: Optional[int] = None) -> Tensor:
+    """A step over a tree of drafted tokens per sequence of a paged cache: the logits behind every node, ``[B, T, V]``.
+
+    ``tokens [B, T]``, B the cache's slots: node 0 is the token that follows the sequence, the others are drafts.  ``parents`` int32 ``[B, T]`` or ``[T]``: the
+    node that each follows (``ops.draft_tree``).  ``nodes``: how many of its nodes each slot has (``None``: all; 0: the sequence waits).  ``window``: as in ``step``; a node sees
+    the last positions of the path that leads to it.
+
+    The nodes' keys and values lie behind the contexts until ``cache.accept(path, counts)`` keeps those of the path that ``ops.verify_drafts`` has accepted;
+    the token that follows it is the next step's node 0.
+    """
+    layers, counts = _check_draft(model, tokens, parents, cache, nodes, window)
+    B, T = tokens.shape
+    on_device = None if nodes is None else torch.tensor(counts, dtype=torch.int32).to(cache.k.device)
+    cache.begin_draft(counts)
+    try:
+        tree = ops.draft_tree(parents, cache.positions, nodes=on_device)
+        return _walk_step(model, tokens, cache, 0, window=window, layers=layers, tree=tree, nodes=on_device).view(B, T, -1)
+    except BaseException:
+        cache.forget_draft()
+        raise
+
+
+def _check_draft(model, tokens: Tensor, parents: Tensor, cache: PagedKVCache, nodes: Optional[Sequence[int]], window: Optional[int]) -> Tuple[list, List[int]]:
+    """What a draft has to fulfil ahead of what it takes: the layers' attention, and the nodes of each slot."""
+    torch._assert(isinstance(cache, PagedKVCache), "drafts need a paged cache")
+    _check_window(cache, window)
+    layers = [getattr(blk, "attn", None) for blk in model.blocks]
+    _check_paged(layers)
+    torch._assert(tokens.dim() == 2 and tokens.size(0) == cache.sequences, "token batch does not match the cache")
+    B, T = tokens.shape
+    if not 0 < T <= ops.MAX_TREE_NODES:
+        raise ValueError(f"a tree must have 1 to {ops.MAX_TREE_NODES} nodes, got {T}")
+    if parents.dtype != torch.int32 or parents.shape not in ((T,), (B, T)):
+        raise ValueError(f"parents must be int32 [{T}] or [{B}, {T}], got {tuple(parents.shape)} {parents.dtype}")
+    counts = [T] * B if nodes is None else [int(n) for n in nodes]
+    if len(counts) != B or not all(0 <= n <= T for n in counts):
+        raise ValueError(f"nodes must be 0 to {T} for each of the {B} slots, got {counts}")
+    # (a node is rotated as the position behind its ancestors: T - 1 of them at most)
+    _check_positions(layers, max((cache.length(slot) + n for slot, n in enumerate(counts) if cache.length(slot) is not None), default=0))
+    return layers, counts
+
+
 def _check_window(cache, window: Optional[int]) -> None:
     if window is not None and not isinstance(cache, PagedKVCache):
         raise ValueError("a window of a call is for paged caches: a ring's size bounds what its steps see")
@@ -221,15 +265,16 @@ def _check_window(cache, window: Optional[int]) -> None:
 
 
 def _walk_step(model, token_ids: Tensor, cache: KVCache, pos, status: Optional[Tensor] = None, window: Optional[int] = None,
-               layers: Optional[list] = None) -> Tensor:
+               layers: Optional[list] = None, tree: Optional[ops.DraftTree] = None, nodes: Optional[Tensor] = None) -> Tensor:
     """The layer walk of ``step`` at position ``pos`` (a host int, or a one-element int32 device
     tensor when the walk is being recorded for replay); leaves ``cache.advance()`` to the caller.
     ``status``: the int32 word in which the attention kernels report a device position they cannot use.  ``window``: bounds the model's.  ``layers``: the blocks'
-    attention, where the caller has looked it up."""
+    attention, where the caller has looked it up.  ``tree``, ``nodes``: the tokens are those of a tree per sequence of a paged cache, which the layers see as so
+    many sequences of one token."""
     token_ids = token_ids.reshape(-1, 1)
     B = token_ids.size(0)
     paged = isinstance(cache, PagedKVCache)
-    torch._assert(B == (cache.sequences if paged else cache.B), "token batch does not match the cache")
+    torch._assert(B == ((cache.sequences if tree is None else tree.rows.size(0)) if paged else cache.B), "token batch does not match the cache")
     on_device = isinstance(pos, Tensor)
     x = x0 = norm(model.embed(token_ids))
     skip_map, skip_weights = model.skip_map, model.skip_weights
@@ -248,7 +293,7 @@ def _walk_step(model, token_ids: Tensor, cache: KVCache, pos, status: Optional[T
         if attn is None or not getattr(attn, "uses_kv_context", True):
             k_ctx = v_ctx = None        # no attention, or one that keeps its own state (KDA layers)
         elif paged:
-            k_ctx = v_ctx = cache.context(i)
+            k_ctx = v_ctx = cache.context(i, tree=tree, nodes=nodes)
         elif in_place and getattr(attn, "accepts_ring_context", False):
             k_ctx = v_ctx = cache.ring(i)
             k_ctx.status = status
@@ -414,6 +459,64 @@ class GraphedPagedStep:
             self._record()
         self._graph.replay()
         self.cache.advance(on_device=False)
+        return self._logits
+
+
+class GraphedDraftStep:
+    """``draft_step`` over trees of ``T`` nodes recorded once as a HIP graph and replayed for every later draft, whatever its trees: tokens, parents and how many nodes
+    there are lie in buffers of the recording.  Logits, window and rotary tables as in ``GraphedPagedStep``.
+    """
+
+    def __init__(self, model, cache: PagedKVCache, T: int, window: Optional[int] = None):
+        _check_window(cache, window)
+        _check_paged([getattr(blk, "attn", None) for blk in model.blocks])
+        if not 0 < T <= ops.MAX_TREE_NODES:
+            raise ValueError(f"a tree must have 1 to {ops.MAX_TREE_NODES} nodes, got {T}")
+        self.model, self.cache, self.T, self.window = model, cache, T, window
+        dev, B = cache.k.device, cache.sequences
+        self.tokens = torch.zeros(B, T, dtype=torch.long, device=dev)
+        self.parents = torch.full((B, T), -1, dtype=torch.int32, device=dev)
+        self.nodes = torch.zeros(B, dtype=torch.int32, device=dev)
+        self._graph: Optional[torch.cuda.CUDAGraph] = None
+        self._logits: Optional[Tensor] = None
+
+    def check(self) -> None:
+        self.cache.check()
+
+    def _body(self) -> Tensor:
+        tree = ops.draft_tree(self.parents, self.cache.positions, nodes=self.nodes)
+        logits = _walk_step(self.model, self.tokens, self.cache, 0, window=self.window, tree=tree, nodes=self.nodes)
+        return logits.view(self.cache.sequences, self.T, -1)
+
+    def _record(self) -> None:
+        dev = self.cache.k.device
+        # One eager pass on a side stream first; it writes the rows that the first replay writes again.
+        side = torch.cuda.Stream(device=dev)
+        side.wait_stream(torch.cuda.current_stream(dev))
+        with torch.cuda.stream(side):
+            self._body()
+        torch.cuda.current_stream(dev).wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            self._logits = self._body()
+        self._graph = graph
+
+    @torch.no_grad()
+    def __call__(self, tokens: Tensor, parents: Tensor, nodes: Optional[Sequence[int]] = None) -> Tensor:
+        if tokens.dim() != 2 or tokens.size(1) != self.T:
+            raise ValueError(f"the recording is of trees of {self.T} nodes, got tokens {tuple(tokens.shape)}")
+        _, counts = _check_draft(self.model, tokens, parents, self.cache, nodes, self.window)
+        self.cache.begin_draft(counts)
+        try:
+            self.tokens.copy_(tokens)
+            self.parents.copy_(parents)
+            self.nodes.copy_(torch.tensor(counts, dtype=torch.int32))
+            if self._graph is None:
+                self._record()
+            self._graph.replay()
+        except BaseException:
+            self.cache.forget_draft()
+            raise
         return self._logits
 
 

@@ -26,6 +26,7 @@ import time
 from typing import Callable, Dict, Iterator, List, Optional, Sequence, Tuple, Union
 
 import torch
+import torch.nn.functional as F
 from torch import Tensor
 
 from . import ops
@@ -154,6 +155,7 @@ class Generator:
         # generate_ragged: the paged cache of the last call and its recorded step
         self._paged_cache: Optional[PagedKVCache] = None
         self._paged_step = None
+        self._draft_step = None
         # What ops.process_logits adds to the repetition penalty, over the same last tokens: a bias per token ({id: value} or [vocab]), and
         # allowed_tokens(seen [B, T], lens [B]) -> which tokens may follow, bool [B, vocab] or bits (ops.pack_allowed, which is ten launches of its own a token), or None for
         # all; a row in which none may ends.  All three penalties count the prompt's tokens, too.
@@ -384,7 +386,8 @@ class Generator:
         return seen[:, ids.size(1):n_seen].clone()
 
     @torch.inference_mode()
-    def generate_ragged(self, prompts: Sequence[Tensor], max_new_tokens: int, record_steps: bool = False) -> Tensor:
+    def generate_ragged(self, prompts: Sequence[Tensor], max_new_tokens: int, record_steps: bool = False,
+                        drafts: Optional[Callable[[Tensor, Tensor], Tuple[Tensor, Tensor]]] = None) -> Tensor:
         """Prompts of unequal length (1-D token tensors) -> ``[B, max_new_tokens]`` ids, with the same sampling settings as
         ``generate``; a row that produces the end-of-sequence token keeps emitting it.
 
@@ -392,6 +395,12 @@ class Generator:
         own (``core.step``; ``record_steps``: recorded once as a HIP graph and replayed).  The model needs what ``generate_batch`` needs, and
         attention layers that take pages: a stack with a KDA layer is refused.  A step
         sees what it sees there: no more than the generator's window, whose pages go back to the pool.
+
+        ``drafts(seen [B, N], lens [B]) -> (tokens [B, M], parents int32 [B, M] or [M])``: tokens that may follow each row's first ``lens[b]`` tokens, as a tree: the draft that
+        each one follows, -1 for the last token seen.  One step (``core.draft_step``) then runs all of them, and those that the model's own choice agrees with
+        (``ops.verify_drafts``) are kept, with a token that follows them: greedily the tokens are those without drafts (but for near ties: a product over more rows rounds
+        otherwise), drawn ones have the distribution that they have without.  Penalties and masks depend on the tokens ahead of each draft and are refused.
+        ``record_steps`` records for each M anew: a tree of one size is recorded once.
         """
         from . import core
         assert len(prompts) > 0 and all(p.ndim == 1 and p.numel() > 0 for p in prompts) and max_new_tokens > 0
@@ -403,16 +412,21 @@ class Generator:
         # (a ring of W rows is attended beside the new token where the model's window is wider than the ring)
         own = getattr(self.model, "attn_window_size", self.cache.W)
         window = self.cache.W + 1 if own is None else min(own, self.cache.W + 1)
+        if drafts is not None and (self._rep_p_host != 1.0 or self.presence_penalty != 0.0 or self.frequency_penalty != 0.0 or self.allowed_tokens is not None
+                                   or self.sample is not sample_token or self.apply_repetition_penalty is not penalise_repeats):
+            raise ValueError("drafts do not combine with penalties, masks or routines of the caller's")
         cache, size = self._paged_cache, 64
-        pages = _ragged_pages(lengths, max_new_tokens, window, size)
+        # (a tree's nodes lie behind a context of which the first of them sees all of the window)
+        pages = _ragged_pages(lengths, max_new_tokens, window + (ops.MAX_TREE_NODES if drafts is not None else 0), size)
         if cache is None or cache.sequences != B or cache.pages < pages or cache.max_len < longest or cache.window != window:
-            cache = self._paged_cache = self._paged_step = None      # (given up ahead of the new pool)
+            cache = self._paged_cache = self._paged_step = self._draft_step = None      # (given up ahead of the new pool)
             cache = self._paged_cache = PagedKVCache(L=self.cache.L, sequences=B, H=self.cache.H, D=self.cache.D, pages=pages, device=self.device,
                                                      dtype=torch.bfloat16, page_size=size, max_len=longest, window=window)
+        cache.forget_draft()      # (of a call that ended in an error)
         for slot in range(B):
             if cache.length(slot) is not None:
                 cache.release(slot)
-        if record_steps and self._paged_step is None:
+        if record_steps and drafts is None and self._paged_step is None:
             self._paged_step = core.GraphedPagedStep(self.model, cache, window=window)
         step = self._paged_step if record_steps else lambda tokens: core.step(self.model, tokens, cache, window=window)
         logits, _ = core.admit(self.model, prompts, cache)      # (all slots are free: sequence i is in slot i)
@@ -423,6 +437,9 @@ class Generator:
         first = lens.long()
         eos = self.eos_token_id.to(torch.long)
         done = torch.zeros(B, dtype=torch.bool, device=self.device)
+        if drafts is not None:
+            self._follow_drafts(cache, logits, seen, lens, lengths, max_new_tokens, window, drafts, record_steps)
+            return seen.gather(1, first[:, None] + torch.arange(max_new_tokens, device=self.device))
         for produced in range(1, max_new_tokens + 1):
             scores = self._adjusted(self._trim(logits), seen, lens)
             token = self._draw(scores)
@@ -434,3 +451,59 @@ class Generator:
                 logits = step(token)
         cache.check()
         return seen.gather(1, first[:, None] + torch.arange(max_new_tokens, device=self.device))
+
+    def _follow_drafts(self, cache: PagedKVCache, logits: Tensor, seen: Tensor, lens: Tensor, lengths: List[int], new: int, window: Optional[int], drafts, record_steps: bool) -> None:
+        """The loop of ``generate_ragged`` with drafts: fills ``seen`` behind the prompts from their ``logits`` on."""
+        from . import core
+        B, eos, dev = len(lengths), self.eos_token_id.to(torch.long), self.device
+        end = int(eos)
+        last = self._draw(self._biased(self._trim(logits)))
+        seen.scatter_(1, lens.long()[:, None], last[:, None])
+        lens += 1
+        left = [new - 1] * B      # tokens that each row still takes
+        for row, token in enumerate(last.tolist()):
+            if token == end:
+                seen[row, lengths[row]:lengths[row] + new], left[row] = eos, 0
+        while any(left):
+            tokens, parents = drafts(seen, lens)
+            if tokens.dim() != 2 or tokens.size(0) != B or parents.shape not in (tokens.shape, tokens.shape[1:]) or tokens.size(1) >= ops.MAX_TREE_NODES:
+                raise ValueError(f"drafts must be tokens [{B}, up to {ops.MAX_TREE_NODES - 1}] and parents of that shape or one row, got {tuple(tokens.shape)} and {tuple(parents.shape)}")
+            if tokens.numel() and not 0 <= int(tokens.min()) <= int(tokens.max()) < self.vocab_size:
+                raise ValueError(f"drafts must be tokens of a vocabulary of {self.vocab_size}")
+            T = tokens.size(1) + 1
+            tokens = torch.cat([last[:, None], tokens.to(device=dev, dtype=torch.long)], dim=1)
+            parents = F.pad(parents.to(device=dev, dtype=torch.int32) + 1, (1, 0), value=-1).contiguous()
+            # (node 0 of the call is the last token seen; a row that takes n more tokens has no use for a path of more than n nodes)
+            nodes = [min(T, n) for n in left]
+            if record_steps:
+                if self._draft_step is None or self._draft_step.T != T or self._draft_step.cache is not cache:
+                    self._draft_step = core.GraphedDraftStep(self.model, cache, T, window=window)
+                logits = self._draft_step(tokens, parents, nodes)
+            else:
+                logits = core.draft_step(self.model, tokens, parents, cache, nodes, window=window)
+            scores = self._biased(self._trim(logits).reshape(B * T, -1)).view(B, T, -1)
+            kw = {}
+            if self.temperature != 0.0:
+                scores = keep_nucleus(keep_top_k(scores / max(self.temperature, 1e-6), self.top_k), self.top_p)
+                like = torch.empty(B, scores.size(2), device=dev)
+                kw = dict(temperature=1.0, accept=torch.rand(B, T, device=dev), noise=gumbel_noise(like))
+            path, counts, following = ops.verify_drafts(scores, tokens, parents, nodes=torch.tensor(nodes, dtype=torch.int32).to(dev), **kw)
+            taken = cache.accept(path, counts)
+            # the accepted drafts and the token behind them
+            chosen = tokens.gather(1, path.clamp_min(0).long())
+            following = torch.where(following < 0, eos, following)
+            chosen = torch.cat([chosen[:, 1:], chosen[:, :1]], dim=1).scatter(1, (counts.long() - 1).clamp_min(0)[:, None], following[:, None])
+            step = torch.arange(T, device=dev)
+            keep = step < counts[:, None]
+            seen[keep.nonzero()[:, 0], (lens[:, None] + step)[keep]] = chosen[keep]
+            for row, (n, row_tokens) in enumerate(zip(taken, chosen.tolist())):
+                left[row] -= n
+                if end in row_tokens[:n]:
+                    at = lengths[row] + new - left[row] - n + row_tokens.index(end)
+                    seen[row, at:lengths[row] + new], left[row] = eos, 0
+            last = torch.where(counts > 0, following, last)
+            lens += counts
+        cache.check()
+
+    def _biased(self, rows: Tensor) -> Tensor:
+        return rows if self.logit_bias is None else ops.process_logits(rows, bias=self.logit_bias)

@@ -11,10 +11,13 @@ writes the new row itself, and no chronological copy is ever made.
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Dict, List, Optional, Tuple
+from typing import TYPE_CHECKING, Dict, List, Optional, Tuple
 
 import torch
 from torch import Tensor
+
+if TYPE_CHECKING:
+    from .ops import DraftTree
 
 
 @dataclass
@@ -139,7 +142,8 @@ class KVCache:
 class PagedContext:
     """Handle to one layer of a ``PagedKVCache`` for one call: ``k_pages``/``v_pages`` ``[pages, H, page_size, D]`` (views), the
     cache's ``page_table``, the ``positions`` of the call's tokens and, for a prompt, the sequences (``rows``) that they belong to;
-    for a step the sequences' lengths with the new token (``lens``)."""
+    for a step the sequences' lengths with the new token (``lens``); for a step over trees of drafted tokens the ``tree``, whose positions and rows those of the call
+    are, how many ``nodes`` of it there are, and the lengths of the contexts (``lens``)."""
     k_pages: Tensor
     v_pages: Tensor
     page_table: Tensor
@@ -148,6 +152,8 @@ class PagedContext:
     rows: Optional[Tensor]
     status: Optional[Tensor]
     window: Optional[int]
+    tree: Optional["DraftTree"] = None
+    nodes: Optional[Tensor] = None
 
 
 class PagedKVCache:
@@ -158,6 +164,9 @@ class PagedKVCache:
     that its row of ``page_table`` names, for up to ``max_len`` positions.  A step runs all slots at once; free ones are
     skipped.  With ``window``, pages that no step can see any more go back to the pool as a sequence crosses into another page; a prompt takes
     pages for all of its positions, which its own attention sees, so a pool has to hold the longest prompts whole.
+
+    A step may run a tree of drafted tokens per sequence instead of one token: ``begin_draft`` makes room behind each context, ``accept`` keeps the nodes of the accepted
+    path (``core.draft_step``).  ``fork`` gives a sequence's positions to others that go on from there: they share its full pages, which nobody writes again.
 
     The host knows every length, so that ``admit`` and ``begin_step`` raise where the pool is empty; the device has the table, the next token's
     ``positions`` (-1 for a free slot) and the ``lens`` with it, at fixed addresses, for steps recorded in a HIP graph.  Changes go to the
@@ -184,7 +193,9 @@ class PagedKVCache:
         self._free = list(range(pages - 1, -1, -1))
         self._length: List[Optional[int]] = [None] * sequences               # None: a free slot
         self._owned: List[Dict[int, int]] = [{} for _ in range(sequences)]    # entry of the table -> page
+        self._users: List[int] = [0] * pages                                 # slots that own each page
         self._reach: List[int] = [0] * sequences                             # entries that each slot has taken so far
+        self._drafted: Optional[List[int]] = None                            # nodes of each slot's tree that accept() has not had yet
         self._changes: Dict[int, int] = {}                                   # flat entry -> page, not on the device yet
 
     # -- what there is -----------------------------------------------------------------------
@@ -213,7 +224,12 @@ class PagedKVCache:
     # -- slots and pages -----------------------------------------------------------------------
     def _take(self, wanted: Dict[int, range], left: Dict[int, List[int]]) -> None:
         """Gives every slot the entries that it wants and takes those that it has left behind, or raises and changes nothing."""
-        count, back = sum(len(e) for e in wanted.values()), sum(len(e) for e in left.values())
+        dropped: Dict[int, int] = {}
+        for slot, entries in left.items():
+            for entry in entries:
+                page = self._owned[slot][entry]
+                dropped[page] = dropped.get(page, 0) + 1
+        count, back = sum(len(e) for e in wanted.values()), sum(n == self._users[page] for page, n in dropped.items())
         if count > len(self._free) + back:
             raise RuntimeError(f"the paged cache is full: {count} pages wanted, {len(self._free) + back} of {self.pages} free")
         for slot, entries in left.items():
@@ -226,9 +242,13 @@ class PagedKVCache:
 
     def _set(self, slot: int, entry: int, page: int) -> None:
         if page < 0:
-            self._free.append(self._owned[slot].pop(entry))
+            old = self._owned[slot].pop(entry)
+            self._users[old] -= 1
+            if self._users[old] == 0:
+                self._free.append(old)
         else:
             self._owned[slot][entry] = page
+            self._users[page] += 1
         self._changes[slot * self.page_table.shape[1] + entry] = page
 
     def _upload(self) -> None:
@@ -252,13 +272,46 @@ class PagedKVCache:
             if not 0 < n <= self.max_len:
                 raise ValueError(f"a sequence must have 1 to {self.max_len} positions, got {n}")
         self._take({s: range(-(-n // self.page_size)) for s, n in zip(slots, lengths)}, {})
+        self._upload()
+        self._open(slots, lengths)
+        return slots
+
+    def _open(self, slots: List[int], lengths: List[int]) -> None:
         for s, n in zip(slots, lengths):
             self._length[s] = n
-        self._upload()
         at = torch.tensor(slots, device=self.page_table.device)
         self.positions[at] = torch.tensor(lengths, dtype=torch.int32, device=self.page_table.device)
         self.lens[at] = self.positions[at] + 1
         self._live[at] = 1
+
+    def fork(self, slot: int, count: int = 1) -> List[int]:
+        """Free slots for ``count`` sequences that begin with the positions of the one in ``slot``: the slots, in order.  Full pages are shared from then on; of the last
+        one, where it is not full, each gets a copy."""
+        from . import ops
+        n = self._length[slot]
+        if n is None:
+            raise ValueError(f"slot {slot} has no sequence")
+        if count <= 0:
+            raise ValueError(f"a sequence forks into one more or several, not {count}")
+        if self._drafted is not None:
+            raise RuntimeError("accept() has not had the last draft's path yet")
+        slots = [s for s, m in enumerate(self._length) if m is None][:count]
+        if len(slots) < count:
+            raise RuntimeError(f"the paged cache has {len(slots)} free slots for {count} sequences")
+        full, rest = divmod(n, self.page_size)
+        self._take({s: range(full, full + (rest > 0)) for s in slots}, {})
+        for s in slots:
+            for entry, page in self._owned[slot].items():
+                if entry < full:
+                    self._set(s, entry, page)
+        self._upload()
+        if rest:
+            copied = torch.zeros((3, self.sequences), dtype=torch.int32)
+            copied[2] = slot
+            copied[0, slots], copied[1, slots] = full * self.page_size, rest
+            starts, counts, sources = copied.to(self.page_table.device)
+            ops.paged_move(self.k, self.v, self.page_table, starts, counts, rows=self.page_size, sources=sources, status=self.status)
+        self._open(slots, [n] * count)
         return slots
 
     def release(self, slot: int) -> None:
@@ -268,24 +321,65 @@ class PagedKVCache:
         for entry in list(self._owned[slot]):
             self._set(slot, entry, -1)
         self._length[slot], self._reach[slot] = None, 0
+        if self._drafted is not None:
+            self._drafted[slot] = 0
         self._upload()
         self.positions[slot], self.lens[slot], self._live[slot] = -1, 0, 0
 
     def begin_step(self) -> None:
         """Makes room for one more position of every sequence, from the pages that a window has left behind and the pool."""
+        self._make_room([1] * self.sequences)
+
+    def begin_draft(self, nodes: List[int]) -> None:
+        """Makes room for a tree of ``nodes[slot]`` drafted tokens behind every sequence (free slots have none), as ``begin_step`` for one token.  ``accept`` ends
+        the draft."""
+        if len(nodes) != self.sequences or min(nodes) < 0:
+            raise ValueError(f"a draft needs how many nodes each of the {self.sequences} slots has, got {nodes}")
+        self._make_room(nodes)
+        self._drafted = [0 if n is None else m for n, m in zip(self._length, nodes)]
+
+    def _make_room(self, more: List[int]) -> None:
+        if self._drafted is not None:
+            raise RuntimeError("accept() has not had the last draft's path yet")
         wanted, left = {}, {}
-        for slot, n in enumerate(self._length):
-            if n is None:
+        for slot, (n, m) in enumerate(zip(self._length, more)):
+            if n is None or m == 0:
                 continue
-            if n >= self.max_len:
-                raise RuntimeError(f"the sequence in slot {slot} has reached {self.max_len} positions")
-            if n >= self._reach[slot] * self.page_size:
-                wanted[slot] = range(self._reach[slot], n // self.page_size + 1)
+            if n + m > self.max_len:
+                raise RuntimeError(f"the sequence in slot {slot} has reached {n} of {self.max_len} positions, {m} more are wanted")
+            if n + m > self._reach[slot] * self.page_size:
+                wanted[slot] = range(self._reach[slot], (n + m - 1) // self.page_size + 1)
                 if self.window is not None:
                     left[slot] = [e for e in self._owned[slot] if (e + 1) * self.page_size <= n + 1 - self.window]
         if wanted:
             self._take(wanted, left)
             self._upload()
+
+    def accept(self, path: Tensor, counts: Tensor) -> List[int]:
+        """Ends a draft: the first ``counts[slot]`` nodes of ``path[slot]`` (``ops.verify_drafts``; [sequences, M] and [sequences], int32, on the device) become the next positions of each
+        sequence, in all layers; the other nodes are forgotten.  Returns the counts, for which the host waits (0 for
+        free slots, whatever theirs say).  (A row of ``path`` that does not rise leaves its positions as
+        they were and is reported by ``check``.)"""
+        from . import ops
+        if self._drafted is None:
+            raise RuntimeError("there is no draft: begin_draft() comes first")
+        if path.dim() != 2 or path.shape[0] != self.sequences or counts.shape != (self.sequences,):
+            raise ValueError(f"path and counts must be [{self.sequences}, M] and [{self.sequences}], got {tuple(path.shape)} and {tuple(counts.shape)}")
+        taken = [0 if n is None else c for c, n in zip(counts.tolist(), self._length)]
+        for slot, (n, m) in enumerate(zip(taken, self._drafted)):
+            if not 0 <= n <= min(m, path.shape[1]):
+                raise ValueError(f"{n} of the {min(m, path.shape[1])} nodes of slot {slot} cannot be accepted")
+        ops.paged_move(self.k, self.v, self.page_table, self.positions, counts, index=path, status=self.status)
+        counts = counts * self._live
+        self.positions.add_(counts)
+        self.lens.add_(counts)
+        self._length = [None if n is None else n + more for n, more in zip(self._length, taken)]
+        self._drafted = None
+        return taken
+
+    def forget_draft(self) -> None:
+        """Ends a draft of which nothing is accepted."""
+        self._drafted = None
 
     def advance(self, on_device: bool = True) -> None:
         """Every sequence has one position more.  ``on_device=False``: the device has counted already (a recorded step)."""
@@ -298,8 +392,11 @@ class PagedKVCache:
         self.lens.add_(self._live)
 
     # -- handles --------------------------------------------------------------------------------
-    def context(self, layer: int, positions: Optional[Tensor] = None, rows: Optional[Tensor] = None) -> PagedContext:
-        """The layer for a step of all slots, or for a prompt's tokens at ``positions`` of sequences ``rows``."""
+    def context(self, layer: int, positions: Optional[Tensor] = None, rows: Optional[Tensor] = None, tree: Optional["DraftTree"] = None,
+                nodes: Optional[Tensor] = None) -> PagedContext:
+        """The layer for a step of all slots, for a prompt's tokens at ``positions`` of sequences ``rows``, or for a step over a ``tree`` (``ops.draft_tree``)."""
+        if tree is not None:
+            return PagedContext(self.k[layer], self.v[layer], self.page_table, tree.positions, self.positions, tree.rows, self.status, self.window, tree, nodes)
         if positions is None:
             return PagedContext(self.k[layer], self.v[layer], self.page_table, self.positions, self.lens, None, self.status, self.window)
         return PagedContext(self.k[layer], self.v[layer], self.page_table, positions, None, rows, self.status, self.window)
