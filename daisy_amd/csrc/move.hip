@@ -102,27 +102,6 @@ __global__ __launch_bounds__(256) void paged_move_kernel(MoveParams p) {
   }
 }
 
-// Layers of pages: no two rows of one tensor share memory, the layers one behind the other.
-static bool layers_apart(const int64_t* st, int L, int P, int H, int S, int D) {
-  const Rows r = rows_of(st + 1, P, H, S, D);
-  return apart(r) && (L == 1 || st[0] >= r.reach);
-}
-// Whether the layers of two tensors of pages share memory (where their layers' strides differ and one lies in the other's range, they are taken to).
-static bool layers_share(const void* k, const int64_t* ks, const void* v, const int64_t* vs, int L, int P, int H, int S, int D) {
-  const Rows x = rows_of(ks + 1, P, H, S, D), y = rows_of(vs + 1, P, H, S, D);
-  const int64_t sk = L > 1 ? ks[0] : 0, sv = L > 1 ? vs[0] : 0, off = ((intptr_t)k - (intptr_t)v) / 2;
-  if (off + (L - 1) * sk + x.reach <= 0 || (L - 1) * sv + y.reach <= off) return false;
-  if (sk != sv) return true;
-  if (sk == 0) return share(k, x, v, y);
-  // layer i of k against layer j of v: off + (i - j) strides apart
-  const int64_t down = off >= 0 ? off / sk : -((-off + sk - 1) / sk);
-  for (int64_t i = down - 1; i <= down + 2; ++i) {
-    if (i >= L || i <= -L) continue;
-    if (share((const uint16_t*)v + (off - i * sk), x, v, y)) return true;
-  }
-  return false;
-}
-
 }  // namespace daisy
 
 using namespace daisy;
@@ -138,12 +117,13 @@ extern "C" int daisy_paged_move_fwd(void* k_pages, const int64_t* k_pages_stride
   DAISY_CHECK_HEAD_DIM("paged_move", D);
   DAISY_CHECK_ARG(k_pages && v_pages && k_pages_strides && v_pages_strides, "paged_move: the pages and their strides must be non-NULL");
   {
-    const int64_t *k5 = k_pages_strides, *v5 = v_pages_strides;
-    const int64_t *k_pages_strides = k5 + 1, *v_pages_strides = v5 + 1;      // (of a layer)
+    const int64_t *k4 = k_pages_strides, *v4 = v_pages_strides;
+    const int64_t *k_pages_strides = k4 + 1, *v_pages_strides = v4 + 1;      // (of a layer)
     DAISY_CHECK_PAGES("paged_move");
-    DAISY_CHECK_ARG(step_of_16(k5[0], L) && step_of_16(v5[0], L), "paged_move: strides must be multiples of 8 elements");
-    DAISY_CHECK_ARG(layers_apart(k5, L, num_pages, H, page_size, D) && layers_apart(v5, L, num_pages, H, page_size, D), "paged_move: rows of the pages must not overlap");
-    DAISY_CHECK_ARG(!layers_share(k_pages, k5, v_pages, v5, L, num_pages, H, page_size, D), "paged_move: the pages of k and v must share no memory");
+    DAISY_CHECK_ARG(step_of_16(k4[0], L) && step_of_16(v4[0], L), "paged_move: strides must be multiples of 8 elements");
+    const Rows k = rows_of(k4, L, num_pages, H, page_size, D), v = rows_of(v4, L, num_pages, H, page_size, D);
+    DAISY_CHECK_ARG(apart(k) && apart(v), "paged_move: rows of the pages must not overlap");
+    DAISY_CHECK_ARG(!share(k_pages, k, v_pages, v), "paged_move: the pages of k and v must share no memory");
   }
   const int64_t items = (int64_t)2 * L * H * (D / 8);
   DAISY_CHECK_ARG(items < (int64_t)1 << 31, "paged_move: %d layers of %d heads are too many", L, H);

@@ -82,30 +82,35 @@ static bool al16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 1
 // (the stride of a dim of one says nothing)
 static bool step_of_16(int64_t stride, int n) { return n == 1 || (stride % 8 == 0 && stride >= 0); }
 static bool rows_of_16(const int64_t* strides, int n0, int n1) { return step_of_16(strides[0], n0) && step_of_16(strides[1], n1); }
-// Rows of D elements in up to three dims, and the elements from the first to the end of the last (no more than 2^60, which nothing that was allocated reaches).
-struct Rows { int64_t n[3], st[3], reach; int D; };
+// Rows of D elements in up to four dims, and the elements from the first to the end of the last (no more than 2^60, which nothing that was allocated reaches).
+constexpr int kRowDims = 4;
+struct Rows { int64_t n[kRowDims], st[kRowDims], reach; int D; };
 static int64_t stepped(int64_t reach, int64_t n, int64_t stride) {
   constexpr int64_t kFar = (int64_t)1 << 60;
   const __int128 r = (__int128)(n - 1) * stride + reach;
   return r < kFar ? (int64_t)r : kFar;
 }
-static Rows rows_of(const int64_t* strides, int n0, int n1, int n2, int D) {
-  Rows r = {{n0, n1, n2}, {n0 > 1 ? strides[0] : 0, n1 > 1 ? strides[1] : 0, n2 > 1 ? strides[2] : 0}, D, D};
-  for (int d = 0; d < 3; ++d) r.reach = stepped(r.reach, r.n[d], r.st[d]);
+static Rows rows_of(const int64_t* strides, int n0, int n1, int n2, int n3, int D) {
+  Rows r = {{n0, n1, n2, n3}, {n0 > 1 ? strides[0] : 0, n1 > 1 ? strides[1] : 0, n2 > 1 ? strides[2] : 0, n3 > 1 ? strides[3] : 0}, D, D};
+  for (int d = 0; d < kRowDims; ++d) r.reach = stepped(r.reach, r.n[d], r.st[d]);
   return r;
 }
+static Rows rows_of(const int64_t* strides, int n0, int n1, int n2, int D) {
+  const int64_t st[kRowDims] = {strides[0], strides[1], strides[2], 0};
+  return rows_of(st, n0, n1, n2, 1, D);
+}
 static Rows rows_of(const int64_t* strides, int n0, int n1, int D) {
-  const int64_t st[3] = {strides[0], strides[1], 0};
-  return rows_of(st, n0, n1, 1, D);
+  const int64_t st[kRowDims] = {strides[0], strides[1], 0, 0};
+  return rows_of(st, n0, n1, 1, 1, D);
 }
 // Rows that are written: no two of them share an element.  From the shortest stride to the longest, each steps over all that the shorter ones reach (what is no such
 // nest is refused, although its rows might miss each other).
 static bool apart(const Rows& rows) {
   int64_t reach = rows.D;
-  bool taken[3] = {rows.n[0] == 1, rows.n[1] == 1, rows.n[2] == 1};
+  bool taken[kRowDims] = {rows.n[0] == 1, rows.n[1] == 1, rows.n[2] == 1, rows.n[3] == 1};
   for (;;) {
     int next = -1;
-    for (int d = 0; d < 3; ++d)
+    for (int d = 0; d < kRowDims; ++d)
       if (!taken[d] && (next < 0 || rows.st[d] < rows.st[next])) next = d;
     if (next < 0) return true;
     if (rows.st[next] < reach) return false;
@@ -116,14 +121,14 @@ static bool apart(const Rows& rows) {
 // Whether rows at a and b are the same ones.
 static bool same_rows(const void* a, const Rows& x, const void* b, const Rows& y) {
   if (a != b) return false;
-  for (int d = 0; d < 3; ++d)
+  for (int d = 0; d < kRowDims; ++d)
     if (x.n[d] != y.n[d] || x.st[d] != y.st[d]) return false;
   return true;
 }
 // Whether a combination of strides from `d` on, up to less[i] times down and more[i] up each, leads from `off` to less than a row away.  The strides are a nest from the longest on, so
 // that each has two numbers at most that leave something for the shorter ones.
 static bool leads_here(int64_t off, const int64_t* st, const int64_t* less, const int64_t* more, int d, int D) {
-  if (d == 3) return off > -D && off < D;
+  if (d == kRowDims) return off > -D && off < D;
   if (st[d] == 0) return leads_here(off, st, less, more, d + 1, D);
   const int64_t down = off >= 0 ? off / st[d] : -((-off + st[d] - 1) / st[d]);
   for (int64_t i = down; i <= down + 1; ++i)
@@ -135,19 +140,19 @@ static bool share(const void* a, const Rows& x, const void* b, const Rows& y) {
   if (a == nullptr || b == nullptr) return false;
   const int64_t off = ((intptr_t)a - (intptr_t)b) / 2;
   if (off + x.reach <= 0 || y.reach <= off) return false;
-  Rows both = {{1, 1, 1}, {0, 0, 0}, 0, x.D};
-  for (int d = 0; d < 3; ++d) {
+  Rows both = {{1, 1, 1, 1}, {0, 0, 0, 0}, 0, x.D};
+  for (int d = 0; d < kRowDims; ++d) {
     if (x.n[d] > 1 && y.n[d] > 1 && x.st[d] != y.st[d]) return true;
     both.n[d] = x.n[d] > y.n[d] ? x.n[d] : y.n[d];
     both.st[d] = x.n[d] > 1 ? x.st[d] : y.st[d];
   }
   if (!apart(both)) return true;
   // (a row of x, i strides on from its first, is as far from a row of y, j on: off + (i - j) strides)
-  int order[3] = {0, 1, 2};
-  for (int k : {0, 1, 0})
+  int order[kRowDims] = {0, 1, 2, 3};
+  for (int k : {0, 1, 2, 0, 1, 0})
     if (both.st[order[k]] < both.st[order[k + 1]]) std::swap(order[k], order[k + 1]);
-  int64_t st[3], less[3], more[3];
-  for (int k = 0; k < 3; ++k) { st[k] = both.st[order[k]]; less[k] = y.n[order[k]] - 1; more[k] = x.n[order[k]] - 1; }
+  int64_t st[kRowDims], less[kRowDims], more[kRowDims];
+  for (int k = 0; k < kRowDims; ++k) { st[k] = both.st[order[k]]; less[k] = y.n[order[k]] - 1; more[k] = x.n[order[k]] - 1; }
   return leads_here(off, st, less, more, 0, x.D);
 }
 static uint32_t pieces_of_16(int64_t stride, int n) { return n == 1 ? 0 : (uint32_t)(stride / 8); }
