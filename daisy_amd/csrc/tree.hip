@@ -751,12 +751,13 @@ __global__ __launch_bounds__(64 * NW, wide_waves_per_simd(D)) void tree_wide_ker
     const char* kh = reinterpret_cast<const char*>(p.k) + 16 * product(h, p.k_sh);
     const char* vh = reinterpret_cast<const char*>(p.v) + 16 * product(h, p.v_sh);
     const int tile0 = e.first + off;
-    auto copy_rows = [&](const char* from_pages, uint32_t sp, uint32_t ss, int row_bytes, auto swizzle, int i, uint32_t to) {
+    auto copy_rows = [&](const char* from_pages, uint32_t sp, uint32_t ss, int row_bytes, auto swizzle, int i, uint32_t to, int first_wave) {
       const int tile = (tile0 + i) * kTile;
       const bool whole = tile >= e.lo && tile + kTile <= e.hi;
 #pragma unroll
       for (int j0 = 0; j0 < COPIES; j0 += NW) {
-        const int j = j0 + wv;
+        const int j = j0 + wv - first_wave;
+        if (COPIES < NW && (unsigned)j >= (unsigned)COPIES) break;
         const int half = RPL * j >> 4, r = RPL * j + ld_row;
         const int pg = __builtin_amdgcn_readlane(id, 2 * (i & 31) + half), slot = __builtin_amdgcn_readlane(in, 2 * (i & 31) + half) * kBlock;
         // a row of the half, or where that is outside the range, another one that is
@@ -765,8 +766,8 @@ __global__ __launch_bounds__(64 * NW, wide_waves_per_simd(D)) void tree_wide_ker
         copy16_to_lds_async((const uint16_t*)(from_pages + 16 * (product(pg, sp) + product(slot, ss))), from * row_bytes + 16 * (ld_pos ^ swizzle(r)), to + 1024 * j);
       }
     };
-    auto copy_k = [&](int i, int slot) { copy_rows(kh, p.k_sp, p.k_ss, k_row, swz_k, i, lds_address(staged) + 4 * TILE * slot); };
-    auto copy_v = [&](int i, int slot) { copy_rows(vh, p.v_sp, p.v_ss, v_row, swz_v, i, lds_address(staged) + 4 * TILE * slot + 2 * TILE); };
+    auto copy_k = [&](int i, int slot) { copy_rows(kh, p.k_sp, p.k_ss, k_row, swz_k, i, lds_address(staged) + 4 * TILE * slot, 0); };
+    auto copy_v = [&](int i, int slot) { copy_rows(vh, p.v_sp, p.v_ss, v_row, swz_v, i, lds_address(staged) + 4 * TILE * slot + 2 * TILE, COPIES < NW ? COPIES : 0); };
     // Tile i is in slot i % STAGES.  Ahead of tile i's softmax K(i + 1) and V(i) have landed, and V(i + STAGES - 1) and K(i + STAGES) are asked for, whose slots the tile before and this one's
     // scores have left.
     pages_from(2 * tile0);
@@ -803,8 +804,9 @@ __global__ __launch_bounds__(64 * NW, wide_waves_per_simd(D)) void tree_wide_ker
       asm volatile("" ::: "memory");
       __syncthreads();
     };
-    constexpr int PER = 2 * ((COPIES + NW - 1) / NW);      // copies of a tile and wavefront
-    static_assert(COPIES % NW == 0, "");
+    // copies of a tile's keys and values a wavefront; or of either, by half of the wavefronts each
+    constexpr int PER = COPIES < NW ? 1 : 2 * (COPIES / NW);
+    static_assert(COPIES % NW == 0 || 2 * COPIES == NW, "");
     using All = std::integral_constant<int, 0>;
     f32x16 sc;
     auto scores = [&](int slot) {
@@ -1074,14 +1076,16 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeParams p) {
   else join_many<D, F16, 16>(p, u, col0, cols, parts, helpers, me, sums, stats);
 }
 
-// Up to 16 columns a wavefront by itself, up to 32 too where its registers hold them, else workgroups of 64 columns or of 128; as many workgroups as the chip holds at once, fewer
-// where there are fewer tiles.
+// Up to 16 columns a wavefront by itself, up to 32 too where its registers hold them (D < 256), else workgroups of 64 columns, of 128 or of 256; as many workgroups as the chip holds
+// at once, fewer where there are fewer tiles.  A workgroup of 256 reads a tile once for what two of 128 read it twice: 150 us against 162 (12 sequences of 100 to 24000, 8 key
+// heads of 8 query heads, 32 nodes, D = 128), 305 against 332 (32 of 8000, 4 query heads, 64 nodes, D = 64).  D = 256 leaves room for one wavefront a SIMD: four, although half of them have
+// no column, take 332 us for what two take 446 for (16 of 8000, 64 columns), because twice as many copies are on their way.
 struct TreeSplit { int groups, cols, blocks, NC, NW; size_t lds; };      // NC: pieces of 16 columns of a wavefront, or 0 and NW: wavefronts of 32
 static TreeSplit tree_split(int B, int T, int H, int G, int D, int64_t capacity) {
   TreeSplit s = {};
   const int all = T * G;
   s.NC = all <= 16 ? 1 : all <= 32 && D < 256 ? 2 : 0;
-  s.NW = s.NC ? 0 : all <= 64 ? 2 : 4;
+  s.NW = s.NC ? 0 : all <= 64 && D < 256 ? 2 : all <= 128 || D == 256 ? 4 : 8;
   const int most_cols = s.NC ? 16 * s.NC : 32 * s.NW;
   s.cols = all < most_cols ? all : most_cols;
   s.blocks = (all + most_cols - 1) / most_cols;
@@ -1103,9 +1107,12 @@ static bool tree_shape_ok(int B, int T, int Hq, int H, int D, int max_pages, int
 template <int D, bool F16> static int tree_launch(const TreeParams& p, const TreeSplit& sp, hipStream_t s) {
   const dim3 grid((unsigned)p.groups);
   if (sp.NC == 1) hipLaunchKernelGGL((tree_attn_kernel<D, F16, 1>), grid, dim3(256), sp.lds, s, p);
-  else if (sp.NW == 2) hipLaunchKernelGGL((tree_wide_kernel<D, F16, 2>), grid, dim3(128), sp.lds, s, p);
   else if (sp.NW == 4) hipLaunchKernelGGL((tree_wide_kernel<D, F16, 4>), grid, dim3(256), sp.lds, s, p);
-  else if constexpr (D < 256) hipLaunchKernelGGL((tree_attn_kernel<D, F16, 2>), grid, dim3(256), sp.lds, s, p);
+  else if constexpr (D < 256) {
+    if (sp.NW == 2) hipLaunchKernelGGL((tree_wide_kernel<D, F16, 2>), grid, dim3(128), sp.lds, s, p);
+    else if (sp.NW == 8) hipLaunchKernelGGL((tree_wide_kernel<D, F16, 8>), grid, dim3(512), sp.lds, s, p);
+    else hipLaunchKernelGGL((tree_attn_kernel<D, F16, 2>), grid, dim3(256), sp.lds, s, p);
+  }
   hipLaunchKernelGGL((tree_join_kernel<D, F16>), dim3((unsigned)p.groups, (unsigned)((p.cols + 15) / 16)), dim3(256), 0, s, p);
   DAISY_CHECK_LAUNCH("tree_attn_kernel");
   return DAISY_OK;

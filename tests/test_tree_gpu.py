@@ -143,7 +143,7 @@ def trees(T, B, rng, shape="random"):
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("D,H,G,T,page", [(64, 2, 1, 1, 16), (64, 1, 3, 5, 48), (128, 2, 1, 8, 16), (128, 3, 2, 8, 32), (128, 1, 1, 17, 64), (128, 2, 4, 8, 16), (128, 1, 8, 33, 32),
                                           (64, 2, 1, 33, 16), (64, 1, 4, 40, 64), (256, 2, 1, 5, 16), (256, 1, 2, 12, 96), (256, 1, 8, 9, 32), (64, 1, 1, 100, 256), (128, 1, 1, 256, 32),
-                                          (128, 2, 16, 3, 16)])
+                                          (128, 2, 16, 3, 16), (128, 1, 8, 12, 48), (64, 2, 4, 24, 16), (256, 1, 4, 70, 16)])
 def test_attention_over_every_edge_of_blocks_tiles_and_pages(dtype, D, H, G, T, page):
     print(f"tree attention {dtype} D{D} H{H} G{G} T{T} page {page}", flush=True)
     g, rng = gen(D + H + G + T + page), random.Random(T)
