@@ -45,7 +45,7 @@ struct VerifyParams {
 
 // Of some of a row beside its children's tokens: the largest score, the sum of e relative to that; the two best of x / t + noise, relative to it, too (a noise added to a mask of the type's lowest
 // value would be lost), and the best one's token (INT32_MAX: none).
-template <typename SUM> struct RowPart { SUM sum; float top, best, second; int token; };
+struct RowPart { double sum; float top, best, second; int token; };
 struct Left { double scale, less; int at; float top; };     // max(scale e - less q, 0) of row `at`, whose largest score is `top`; at < 0: nothing to be drawn
 
 // 1 / t, 0 where the likeliest token is wanted
@@ -315,7 +315,7 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(VerifyParams p) {
 }
 
 // The parts of a row as one, `group` lanes for it, all of which have the result.
-template <int MODE> __device__ __forceinline__ RowPart<double> join_row(const VerifyParams& p, int b, int u, double by, int lane, int group) {
+template <int MODE> __device__ __forceinline__ RowPart join_row(const VerifyParams& p, int b, int u, double by, int lane, int group) {
   constexpr int U = 4;      // parts that a lane asks for at once
   const int64_t first = ((int64_t)b * p.T + u) * p.slices;
   const float c = (float)fmin(by * 1.4426950408889634, 1e30);
@@ -348,16 +348,16 @@ template <int MODE> __device__ __forceinline__ RowPart<double> join_row(const Ve
   const float t = wave_max(top, group);
   sum = wave_sum64(scaled(sum, top, t), group);
   two = wave_two(towards(two, top, t), group);
-  return RowPart<double>{sum, t, two.best, two.second, two.token};
+  return RowPart{sum, t, two.best, two.second, two.token};
 }
 // All rows of a tree, by the wavefronts of a workgroup.
-template <int MODE> __device__ __forceinline__ void join_rows(const VerifyParams& p, int b, int n, double by, RowPart<double>* rows) {
+template <int MODE> __device__ __forceinline__ void join_rows(const VerifyParams& p, int b, int n, double by, RowPart* rows) {
   int group = 1;
   while (group < 64 && group < p.slices) group *= 2;
   const int per_wave = 64 / group, lane = threadIdx.x & 63, sub = lane / group;
   for (int u0 = (threadIdx.x >> 6) * per_wave; u0 < n; u0 += blockDim.x / 64 * per_wave) {
     const int u = min(u0 + sub, n - 1);
-    const RowPart<double> row = join_row<MODE>(p, b, u, by, lane % group, group);
+    const RowPart row = join_row<MODE>(p, b, u, by, lane % group, group);
     if (lane % group == 0) rows[u] = row;
   }
 }
@@ -393,7 +393,7 @@ __device__ __forceinline__ float lane_of(float x, int lane) { return __int_as_fl
 constexpr int kWalkThreads = 512;
 template <int E, int MODE>
 __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams p) {
-  __shared__ RowPart<double> rows[kMostNodes];
+  __shared__ RowPart rows[kMostNodes];
   __shared__ int path[kMostNodes];
   __shared__ Best bests[kWalkThreads / 64];
   __shared__ int unsure;                  // the row whose best token fp32 does not tell
@@ -422,7 +422,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams 
     while (at >= 0) {
       if (lane == 0) path[count] = at;
       ++count;
-      const RowPart<double> row = rows[at];
+      const RowPart row = rows[at];
       uint64_t kids[4], any = 0;
       bool several = false;      // more than one child
 #pragma unroll
@@ -538,7 +538,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams 
 constexpr int kDrawThreads = 1024;
 template <int E>
 __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyParams p) {
-  __shared__ RowPart<double> rows[kMostNodes];
+  __shared__ RowPart rows[kMostNodes];
   __shared__ int path[kMostNodes];
   __shared__ Left todo;
   __shared__ double sums[kDrawThreads / 64];
@@ -580,7 +580,7 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyParams 
       }
       bool walking = at >= 0;
       while (walking) {
-        const RowPart<double> row = rows[at];
+        const RowPart row = rows[at];
         if (fresh) {
           if (lane == 0) path[count] = at;
           ++count;
@@ -763,7 +763,7 @@ static VerifySplit verify_split(int B, int T, int V) {
   s.slice = 256 * s.rounds;
   s.slices = (V + s.slice - 1) / s.slice;
   s.rows = 1;
-  while (s.rows < T && (int64_t)B * ((T + 2 * s.rows - 1) / (2 * s.rows)) * s.slices >= 16384) s.rows *= 2;
+  while (s.rows < T && (int64_t)B * ((T + 2 * s.rows - 1) / (2 * s.rows)) * s.slices >= 4096) s.rows *= 2;
   s.pieces = (V + kPiece - 1) / kPiece;
   return s;
 }
