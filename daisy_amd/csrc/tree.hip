@@ -462,12 +462,12 @@ __global__ __launch_bounds__(256, tree_groups_per_cu(D, NC)) void tree_attn_kern
       uint32_t vis[NC];
       if (edge) {
 #pragma unroll
-        for (int t = 0; t < NC; ++t) vis[t] = visible(p, e, mask + node[t] * p.mask_st, node[t], lo[t], tile);
+        for (int t = 0; t < NC; ++t) vis[t] = visible(p, e, mask + node[t] * p.mask_st, node[t], lo[t], tile) >> (4 * c);      // (rows 4c + r and 16 + 4c + r: bits r and 16 + r)
         uint32_t most = 0;
+        const int first = tile + 4 * c - e.lo;
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
-          const int key = tile + 4 * c + (r & 3) + (r & 4) * 4;
-          const bool there = key >= e.lo && key < e.hi;
+          const bool there = (unsigned)(first + (r & 3) + (r & 4) * 4) < (unsigned)(e.hi - e.lo);
 #pragma unroll
           for (int d = 0; d < VD; ++d) {
             vr[r][d] = there ? vr[r][d] : 0;
@@ -485,7 +485,7 @@ __global__ __launch_bounds__(256, tree_groups_per_cu(D, NC)) void tree_attn_kern
         for (int r = 0; r < 8; ++r) s[r] = sc[t][r >> 2][r & 3] * p.scale_log2e;
         if (edge) {
 #pragma unroll
-          for (int r = 0; r < 8; ++r) s[r] = vis[t] >> (4 * c + (r & 3) + (r & 4) * 4) & 1 ? s[r] : -__builtin_inff();
+          for (int r = 0; r < 8; ++r) s[r] = vis[t] >> ((r & 3) + (r & 4) * 4) & 1 ? s[r] : -__builtin_inff();
         }
         float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
         {
@@ -529,7 +529,7 @@ __global__ __launch_bounds__(256, tree_groups_per_cu(D, NC)) void tree_attn_kern
           for (int t = 0; t < NC; ++t) {
             u32x4 sees;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) sees[r] = halves(vis[t] >> (4 * c + (2 * r & 3) + (2 * r & 4) * 4)) & ones<F16>();
+            for (int r = 0; r < 4; ++r) sees[r] = halves(vis[t] >> ((2 * r & 3) + (2 * r & 4) * 4)) & ones<F16>();
             const f32x4 met = mfma<F16>(odd, sees, f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
             for (int i4 = 0; i4 < 4; ++i4) acc[t][j][i4] = met[i4] > 0.f ? __builtin_nanf("") : acc[t][j][i4];
