@@ -80,6 +80,9 @@ __global__ __launch_bounds__(kMostNodes) void draft_tree_kernel(DraftTreeParams 
 // Products: S^T = K Q^T, O^T = V^T P^T on 16x16x32 matrix instructions, NC of them for each piece of K and V that a wavefront has loaded: rows 4c + r and
 // 16 + 4c + r of a tile are, for the lanes of group c, both rows of S^T and rows of the second product's operand.  V's rows arrive 16 bytes a lane, v_perm pairs neighbours.
 //
+// One wavefront a SIMD, a workgroup a compute unit: fewer runs begin and end inside units, and registers hold all that a run needs.  One sequence of 8000, 12 heads of 128, 8 nodes: 17.0 us, with three workgroups a
+// compute unit (and 12 registers spilled) 21.6; two of 131000, 16 heads, 5 nodes 317 (6.8 TB/s) against 358; 24 of up to 8300, window 4096, 16 nodes 39.6 (4.8 TB/s) against 53.7.
+//
 // A tile that all columns see whole needs no mask.  The others, those with nodes in them and those at a window's edge, make a word of 32 bits for each column, the tile's keys
 // that it sees.
 
@@ -140,18 +143,19 @@ __device__ __forceinline__ Sequence sequence(const TreeParams& p, int b) {
   const int len = p.lens[at], nodes = p.nodes != nullptr ? p.nodes[at] : p.T;
   return Sequence{b < p.B ? len : -1, nodes};
 }
-// What coming to a unit costs a workgroup of many columns, in tiles: what it reads one behind the other on the way to the first key, and its masks.  (12 sequences of 100 to 24000, 256 columns: 0 tiles 209 us,
-// 4 162, 8 158, 12 156, 16 158.  Wavefronts that take a unit each hide it behind each other; there the way around a unit without tiles costs registers.)
-constexpr int unit_tiles(int cols) { return cols <= 32 ? 0 : 8; }
-template <int COLS> __device__ __forceinline__ int weight_of(const TreeParams& p, const Sequence& s) {
+// What coming to a unit costs, in tiles: what is read one behind the other on the way to the first key, and its masks.  Workgroups of many columns (12 sequences of 100 to 24000, 256 columns): 0 tiles
+// 209 us, 4 162, 8 158, 12 156, 16 158.  Wavefronts by themselves (24 sequences of up to 8300, window 4096, 16 columns): 0 tiles 58 us, 1 40.8, 2 40.2, 3 39.6, 4 39.4; one sequence of 8000 18.0, 17.7, 17.2, 17.0, 17.1.
+// With D = 256 the way around a unit without tiles spills registers (54.8 us against 64.2, 32000 positions).
+constexpr int unit_tiles(int D, int cols) { return cols > 32 ? 8 : D == 256 ? 0 : 3; }
+template <int COLS, int AHEAD> __device__ __forceinline__ int weight_of(const TreeParams& p, const Sequence& s) {
   const Extent e = extent<COLS>(p, s.len, s.nodes);
-  return e.tiles > 0 ? (e.tiles + unit_tiles(COLS)) * e.blocks : 0;
+  return e.tiles > 0 ? (e.tiles + AHEAD) * e.blocks : 0;
 }
 
-// The tiles of all units one behind the other, blocks of COLS columns and unit_tiles ahead of each unit's own: which unit one of them belongs to.  Every wavefront has one of these and
+// The tiles of all units one behind the other, blocks of COLS columns and AHEAD tiles ahead of each unit's own: which unit one of them belongs to.  Every wavefront has one of these and
 // asks for rising numbers.
 struct Unit { Extent e; int b, h, col0, cols, off, count, n_tiles, x, next; };      // count tiles from `off` on (there may be none); x: the unit's first one; next: behind those
-template <int COLS> struct Deal {
+template <int COLS, int AHEAD> struct Deal {
   int own, own_upto, per_lane;      // lane i: the tiles (of a key head each) of sequences from i * per_lane on; with those ahead
   // 64 sequences from `base` on, one a lane; up to 64 are all there
   int base, before, weight, upto, chunk;
@@ -165,7 +169,7 @@ template <int COLS> struct Deal {
 #pragma unroll
       for (int i = 0; i < 4; ++i) s4[i] = sequence(p, lane * per_lane + min(i, per_lane - 1));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) own += i < per_lane ? weight_of<COLS>(p, s4[i]) : 0;
+      for (int i = 0; i < 4; ++i) own += i < per_lane ? weight_of<COLS, AHEAD>(p, s4[i]) : 0;
     } else {
       // 64 at a time, the wavefronts in turn: in a row, where lanes by themselves are a cache line or more apart
       __shared__ int sums[64];
@@ -173,7 +177,7 @@ template <int COLS> struct Deal {
       const int used = (int)((unsigned)(p.B + per_lane - 1) / (unsigned)per_lane), waves = blockDim.x / 64;
       for (int i = wv; i < used; i += waves) {
         int tiles = 0;
-        for (int j = 0; j < per_lane; j += 64) tiles += weight_of<COLS>(p, sequence(p, i * per_lane + j + lane));
+        for (int j = 0; j < per_lane; j += 64) tiles += weight_of<COLS, AHEAD>(p, sequence(p, i * per_lane + j + lane));
         const int sum = wave_scan(tiles);
         if (lane == 63) sums[i] = sum;
       }
@@ -203,7 +207,7 @@ template <int COLS> struct Deal {
     while (chunk < 0 || (x >= (before + chunk) * p.H && base < p.B)) {
       if (chunk >= 0) { before += chunk; base += 64; }
       seq = sequence(p, base + lane);
-      weight = weight_of<COLS>(p, seq);
+      weight = weight_of<COLS, AHEAD>(p, seq);
       upto = wave_scan(weight);
       chunk = __builtin_amdgcn_readlane(upto, 63);
     }
@@ -215,12 +219,12 @@ template <int COLS> struct Deal {
     u.n_tiles = max(u.e.tiles, 1);
     const int blocks = max(u.e.blocks, 1);
     const int rel = x - (before + __builtin_amdgcn_readlane(upto - weight, bl)) * p.H;
-    const int ahead = unit_tiles(COLS), all = u.n_tiles + ahead;
+    const int all = u.n_tiles + AHEAD;
     const int unit = (int)min((unsigned)rel / (unsigned)all, (unsigned)(p.H * blocks - 1));
     const int from = min(max(rel - unit * all, 0), all - 1), upto = min(all, from + max(x_end - x, 1));
-    u.off = max(from - ahead, 0);
-    u.count = ahead == 0 ? max(upto - from, 1) : max(upto - ahead, 0) - u.off;
-    u.x = x - from + ahead;
+    u.off = max(from - AHEAD, 0);
+    u.count = AHEAD == 0 ? max(upto - from, 1) : max(upto - AHEAD, 0) - u.off;
+    u.x = x - from + AHEAD;
     u.next = x + upto - from;
     u.h = (int)((unsigned)unit / (unsigned)blocks);
     u.col0 = (unit - u.h * blocks) * COLS;
@@ -252,8 +256,6 @@ template <int RUNS> __device__ __forceinline__ int share_of(const TreeParams& p,
   return least + (wave_min((more == 0 ? load - load / 32 : load) * 64 + more) & 63);
 }
 
-// Workgroups per compute unit, a wavefront of each per SIMD: what the registers leave room for.
-constexpr int tree_groups_per_cu(int D, int NC) { return D == 64 ? (NC == 1 ? 4 : 3) : D == 128 ? (NC == 1 ? 3 : 2) : 1; }
 constexpr int tree_row(int D) { return D + 4; }      // floats of a partial sum's row in the LDS
 
 // Bit i of a mask that begins `from` bits before its first word (or behind it), ones ahead of it: 32 of them.
@@ -305,7 +307,7 @@ template <bool F16> __device__ __forceinline__ uint32_t ones() { return F16 ? 0x
 __device__ __forceinline__ uint32_t halves(uint32_t bits) { return (bits & 1 ? 0xffffu : 0) | (bits & 2 ? 0xffff0000u : 0); }
 
 template <int D, bool F16, int NC>
-__global__ __launch_bounds__(256, tree_groups_per_cu(D, NC)) void tree_attn_kernel(TreeParams p) {
+__global__ __launch_bounds__(256, 1) void tree_attn_kernel(TreeParams p) {
   constexpr int KS = D / 32;                     // steps of the first product
   constexpr int J = D / 16;                      // 16-row pieces of the second product's result
   constexpr int W = D == 64 ? 4 : 8;             // channels of a V row that a lane has beside each other
@@ -321,7 +323,7 @@ __global__ __launch_bounds__(256, tree_groups_per_cu(D, NC)) void tree_attn_kern
   __shared__ OpenUnits open_units[4];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = blockIdx.x, wave = group * 4 + wv;
   const int n = lane & 15, c = lane >> 4;
-  Deal<16 * NC> deal;
+  Deal<16 * NC, unit_tiles(D, 16 * NC)> deal;
   const int total = deal.begin(p, wv, lane), share = share_of<4>(p, total, lane);
   int x = (int)min((unsigned)wave * (unsigned)share, (unsigned)total);      // (the product is less than twice the total, 2^30 at most, and a share for each wavefront)
   const int x_end = min(x + share, total);
@@ -337,8 +339,8 @@ __global__ __launch_bounds__(256, tree_groups_per_cu(D, NC)) void tree_attn_kern
     const Unit at = deal.unit(p, x, x_end, lane);
     const Extent& e = at.e;
     const int off = at.off, count = at.count, n_tiles = at.n_tiles, all_cols = max(e.nodes * p.G, 1);
-    static_assert(unit_tiles(16 * NC) == 0, "");      // (so that there always is a tile)
     x = at.next;
+    if (unit_tiles(D, 16 * NC) > 0 && count <= 0) continue;      // (only what goes ahead of it)
     b = at.b; h = at.h; col0 = at.col0; cols = at.cols;
 
     // ---- its queries: columns past the last one repeat it
@@ -711,7 +713,7 @@ __global__ __launch_bounds__(64 * NW, wide_waves_per_simd(D)) void tree_wide_ker
   // (neighbouring runs, which read the same keys, to one XCD: workgroups are dealt to the eight of them in turn)
   const int group = (p.groups & 7) == 0 ? (int)((blockIdx.x & 7) * (p.groups >> 3) + (blockIdx.x >> 3)) : (int)blockIdx.x;
   const int n = lane & 31, c = lane >> 5;
-  Deal<COLS> deal;
+  Deal<COLS, unit_tiles(D, COLS)> deal;
   const int total = deal.begin(p, wv, lane), share = share_of<1>(p, total, lane);
   int x = (int)min((unsigned)group * (unsigned)share, (unsigned)total);
   const int x_end = min(x + share, total);
@@ -1090,8 +1092,8 @@ static TreeSplit tree_split(int B, int T, int H, int G, int D, int64_t capacity)
   s.cols = all < most_cols ? all : most_cols;
   s.blocks = (all + most_cols - 1) / most_cols;
   s.lds = s.NC ? (size_t)4 * s.cols * tree_row(D) * sizeof(float) : (size_t)wide_stages(D, s.NW) * 2 * kTile * D * 2;
-  const int64_t tiles = ((capacity + kTile - 1) / kTile + unit_tiles(most_cols)) * B * H * s.blocks;
-  const int64_t groups = s.NC ? (tiles + 3) / 4 : tiles, most = (int64_t)kCus * (s.NC ? tree_groups_per_cu(D, s.NC) : 4 * wide_waves_per_simd(D) / s.NW);
+  const int64_t tiles = ((capacity + kTile - 1) / kTile + unit_tiles(D, most_cols)) * B * H * s.blocks;
+  const int64_t groups = s.NC ? (tiles + 3) / 4 : tiles, most = (int64_t)kCus * (s.NC ? 1 : 4 * wide_waves_per_simd(D) / s.NW);
   s.groups = (int)(groups < most ? groups : most);
   return s;
 }

@@ -100,9 +100,9 @@ def test_workspaces():
     assert 0 < size(1, 1, 1) <= size(1, 1, 50000) <= size(64, 8, 50000) <= size(65535, 256, 50000)
     size = ops.paged_tree_attention_workspace_bytes
     assert size(0, 1, 1, 1, 128, 1, 16) == size(1, 257, 1, 1, 128, 1, 16) == size(1, 1, 3, 2, 128, 1, 16) == size(1, 1, 1, 1, 80, 1, 16) == size(1, 1, 1, 1, 128, 1 << 27, 16) == 0
-    # two partial results of D + 2 floats for every column of a workgroup, and 32 bytes: columns are the queries of a key head, 128 of them at most
+    # two partial results of D + 2 floats for every column of a workgroup, and 32 bytes: columns are the queries of a key head, 256 of them at most
     assert size(1, 1, 1, 1, 128, 1, 16) % (32 + 2 * 130 * 4) == 0
-    assert size(1, 64, 8, 1, 128, 4096, 64) % (32 + 2 * 128 * 130 * 4) == 0
+    assert size(1, 64, 8, 1, 128, 4096, 64) % (32 + 2 * 256 * 130 * 4) == 0
     assert size(1000, 64, 64, 8, 128, 4096, 64) < 1 << 28      # (bounded by what the chip holds)
 
 
