@@ -714,7 +714,7 @@ __global__ __launch_bounds__(64 * NW, wide_waves_per_simd(D)) void tree_wide_ker
   const int group = (p.groups & 7) == 0 ? (int)((blockIdx.x & 7) * (p.groups >> 3) + (blockIdx.x >> 3)) : (int)blockIdx.x;
   const int n = lane & 31, c = lane >> 5;
   Deal<COLS, unit_tiles(D, COLS)> deal;
-  const int total = deal.begin(p, wv, lane), share = share_of<1>(p, total, lane);
+  const int total = deal.begin(p, wv, lane), share = max(share_of<1>(p, total, lane), 4);      // (fewer than 4: 300 positions, 8 key heads, 256 columns 32.6 us, with 4 22.1)
   int x = (int)min((unsigned)group * (unsigned)share, (unsigned)total);
   const int x_end = min(x + share, total);
   SplitUnit beyond = {-1, 0, 0, 0, 0, 0};
