@@ -1213,7 +1213,7 @@ def verify_drafts_workspace_bytes(B: int, T: int, V: int) -> int:
 def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, *, nodes: Optional[torch.Tensor] = None,
                   temperature: Union[float, torch.Tensor] = 0.0, accept: Optional[torch.Tensor] = None, noise: Optional[torch.Tensor] = None,
                   draft: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """Which nodes of trees of drafted tokens the target's probabilities accept, and the token that follows them, in two launches that wait for nobody.
+    """Which nodes of trees of drafted tokens the target's probabilities accept, and the token that follows them, in two launches (four with ``draft``) that the host does not wait for.
 
     ``logits [B, T, V]`` (fp32, bf16 or fp16; any strides of the first two dims): row u says what may follow node u, ``p = softmax(logits[b, u] / temperature)``, -inf what may not (what
     ``process_logits`` or a filter has left).  ``tokens`` int64 or int32 ``[B, T]``: the nodes' tokens, of which node 0's is taken; ``parents``, ``nodes``: as for ``draft_tree``.
