@@ -227,7 +227,7 @@ def draft_step(model, tokens: Tensor, parents: Tensor, cache: PagedKVCache, node
     """
     layers, counts = _check_draft(model, tokens, parents, cache, nodes, window)
     B, T = tokens.shape
-    on_device = None if nodes is None else torch.tensor(counts, dtype=torch.int32).to(cache.k.device)
+    on_device = None if nodes is None else ints_on(cache.k.device, counts)
     cache.begin_draft(counts)
     try:
         tree = ops.draft_tree(parents, cache.positions, nodes=on_device)
@@ -235,6 +235,12 @@ def draft_step(model, tokens: Tensor, parents: Tensor, cache: PagedKVCache, node
     except BaseException:
         cache.forget_draft()
         raise
+
+
+def ints_on(device, values: Sequence[int]) -> Tensor:
+    """int32 numbers on their way to a device; the host does not wait for them."""
+    device = torch.device(device)
+    return torch.tensor(values, dtype=torch.int32, pin_memory=device.type == "cuda").to(device, non_blocking=True)
 
 
 def _check_draft(model, tokens: Tensor, parents: Tensor, cache: PagedKVCache, nodes: Optional[Sequence[int]], window: Optional[int]) -> Tuple[list, List[int]]:
@@ -510,7 +516,7 @@ class GraphedDraftStep:
         try:
             self.tokens.copy_(tokens)
             self.parents.copy_(parents)
-            self.nodes.copy_(torch.tensor(counts, dtype=torch.int32))
+            self.nodes.copy_(ints_on(self.nodes.device, counts))
             if self._graph is None:
                 self._record()
             self._graph.replay()

@@ -37,10 +37,9 @@ __device__ __forceinline__ Place place_of(const MoveParams& p, int seq, int pos,
 // has all rows of a sequence; otherwise a workgroup has kMoveRows of them (rows keep their places, in another sequence's pages).
 //
 // Bound by memory: each row is read and written once.  Stores go past the caches, since the next reader of a row is a layer's attention, long behind the call:
-// 19.9 us against 22.9 for the paths of 64 sequences (4 rows of 16 layers, 8 heads of 128: 100 MB in all).  Loads of copied pages do too, since no row is read
-// twice, with 16 rows a workgroup: 96 copies of up to 127 rows (316 MB read, as many written, of which the caches hold one part) take 130 to 145 us, against
-// 155 to 159 with 64 rows a workgroup and cached accesses, 150 with 32 rows and 217 with 8.  Rows just drafted are read from the caches, so an index's loads
-// stay ordinary ones (21.0 us otherwise).
+// 19.9 us against 22.9 for the paths of 64 sequences (up to 9 rows of 32 layers, 8 heads of 128: 50 MB read, as many written).  Loads of copied pages do too, since no row is
+// read twice, with 16 rows a workgroup: 96 copies of up to 63 rows (12 layers, 16 heads of 128: 316 MB read, as many written) take 130 to 145 us, against 155 to 159 with 64
+// rows a workgroup and cached accesses, 150 with 32 rows and 217 with 8.  Rows just drafted lie in the caches: an index's loads are ordinary ones.
 template <bool ORDERED>
 __global__ __launch_bounds__(256) void paged_move_kernel(MoveParams p) {
   constexpr int U = 8, ROWS = ORDERED ? kOrderedRows : kMoveRows;
@@ -66,9 +65,10 @@ __global__ __launch_bounds__(256) void paged_move_kernel(MoveParams p) {
   const bool mine = piece.of < p.combos;
   uint16_t* base = p.pages[w] + (mine ? head.of * p.sl[w] + head.rest * p.sh[w] + 8 * piece.rest : 0);
   const int64_t sp = p.sp[w], ss = p.ss[w];
-  for (;; row0 += ROWS) {
+  const int ahead = ORDERED ? ROWS : (int)gridDim.y * ROWS;
+  for (bool again = false;; again = true) {
     const int n = min(count - row0, ROWS);
-    if (ORDERED && row0 > 0) __syncthreads();
+    if (again) __syncthreads();
     if ((int)threadIdx.x < n) {
       const int i = row0 + threadIdx.x;
       int bits = 0;
@@ -98,7 +98,8 @@ __global__ __launch_bounds__(256) void paged_move_kernel(MoveParams p) {
         }
       }
     }
-    if (!ORDERED || row0 + ROWS >= count) return;
+    if (count - row0 <= ahead) return;
+    row0 += ahead;
   }
 }
 
@@ -112,7 +113,7 @@ extern "C" int daisy_paged_move_fwd(void* k_pages, const int64_t* k_pages_stride
                                     int B, int rows, int L, int H, int D, int32_t* status, void* stream) {
   DAISY_CHECK_ARG(starts && counts && (index || sources), "paged_move: starts and counts, and an index or sources, must be non-NULL");
   DAISY_CHECK_ARG(B > 0 && rows > 0 && L > 0 && H > 0 && n_seq >= B, "paged_move: B=%d (at most the table's %d), rows=%d, L=%d, H=%d must be positive", B, n_seq, rows, L, H);
-  DAISY_CHECK_SUPPORTED(B <= 65535 && rows <= 64 * 65535, "paged_move: %d sequences of %d rows are too many (65535, 64 times as many rows)", B, rows);
+  DAISY_CHECK_SUPPORTED(B <= 65535, "paged_move: %d sequences are too many (65535)", B);
   DAISY_CHECK_ARG(index_stride >= 0, "paged_move: the index's stride must not be negative");
   DAISY_CHECK_HEAD_DIM("paged_move", D);
   DAISY_CHECK_ARG(k_pages && v_pages && k_pages_strides && v_pages_strides, "paged_move: the pages and their strides must be non-NULL");
@@ -135,7 +136,8 @@ extern "C" int daisy_paged_move_fwd(void* k_pages, const int64_t* k_pages_stride
   p.starts = starts; p.counts = counts; p.index = index; p.index_st = index_stride; p.sources = sources;
   p.rows = rows; p.combos = 2 * L * H; p.by_pieces = divisor(D / 8); p.by_heads = divisor(H);
   p.status = status;
-  const dim3 grid((unsigned)((items + 255) / 256), index ? 1 : (unsigned)((rows + kMoveRows - 1) / kMoveRows), (unsigned)B);
+  const int groups = rows / kMoveRows + (rows % kMoveRows != 0);
+  const dim3 grid((unsigned)((items + 255) / 256), index ? 1 : (unsigned)(groups < 65535 ? groups : 65535), (unsigned)B);
   if (index) hipLaunchKernelGGL((paged_move_kernel<true>), grid, dim3(256), 0, (hipStream_t)stream, p);
   else hipLaunchKernelGGL((paged_move_kernel<false>), grid, dim3(256), 0, (hipStream_t)stream, p);
   DAISY_CHECK_LAUNCH("paged_move_kernel");

@@ -487,7 +487,7 @@ class Generator:
                 scores = keep_nucleus(keep_top_k(scores / max(self.temperature, 1e-6), self.top_k), self.top_p)
                 like = torch.empty(B, scores.size(2), device=dev)
                 kw = dict(temperature=1.0, accept=torch.rand(B, T, device=dev), noise=gumbel_noise(like))
-            path, counts, following = ops.verify_drafts(scores, tokens, parents, nodes=torch.tensor(nodes, dtype=torch.int32).to(dev), **kw)
+            path, counts, following = ops.verify_drafts(scores, tokens, parents, nodes=core.ints_on(dev, nodes), **kw)
             taken = cache.accept(path, counts)
             # the accepted drafts and the token behind them
             chosen = tokens.gather(1, path.clamp_min(0).long())

@@ -74,7 +74,7 @@ def test_verification_argument_errors(kw, rc, text):
 @pytest.mark.parametrize("kw,rc,text", [
     (dict(starts=None), -1, "non-NULL"), (dict(counts=None), -1, "non-NULL"), (dict(index=None), -1, "an index or sources"), (dict(k=None), -1, "non-NULL"), (dict(vs=None), -1, "non-NULL"),
     (dict(table=None), -1, "page table"), (dict(B=0), -1, "B=0"), (dict(B=3), -1, "at most the table's 2"), (dict(rows=0), -1, "rows=0"), (dict(L=0), -1, "L=0"), (dict(H=0), -1, "H=0"),
-    (dict(B=65536, n_seq=65536), -2, "65535"), (dict(index=None, sources=P, rows=1 << 23), -2, "as many rows"), (dict(index_stride=-1), -1, "stride"), (dict(D=96), -2, "head_dim 96"), (dict(page=20), -2, "page_size"),
+    (dict(B=65536, n_seq=65536), -2, "65535"), (dict(index_stride=-1), -1, "stride"), (dict(D=96), -2, "head_dim 96"), (dict(page=20), -2, "page_size"),
     (dict(num_pages=0), -1, "num_pages"), (dict(max_pages=1 << 27), -1, "too long"), (dict(k=P + 2), -1, "aligned"), (dict(ks=strides(1 << 16, 4096, 2048, 130)), -1, "multiples of 8"),
     (dict(ks=strides((1 << 16) + 4, 4096, 2048, 128)), -1, "multiples of 8"), (dict(ks=strides(1 << 16, 4096, 2048, 64)), -1, "overlap"), (dict(ks=strides(1 << 14, 4096, 2048, 128)), -1, "overlap"),
     (dict(v=P + 256), -1, "share no memory"), (dict(v=P), -1, "share no memory"), (dict(v=P + (1 << 17)), -1, "share no memory"), (dict(v=P + (1 << 17) + (1 << 16) - 256), -1, "share no memory"),

@@ -135,6 +135,18 @@ def test_replays_and_streams():
         assert torch.equal(k, mirror[0]) and torch.equal(v, mirror[1]), n
 
 
+def test_more_rows_than_a_grid_has_workgroups_for():
+    rows, page = 16 * 65535 + 40, 4096
+    pages = -(-rows // page)
+    g = gen(9)
+    k, v = (randn(g, 1, 2 * pages, 1, page, 64, dtype=BF16) for _ in range(2))
+    table = torch.randperm(2 * pages, generator=g, device=DEV).int().view(2, pages)
+    ops.paged_move(k, v, table, ints([0, 3]), ints([0, rows - 3]), rows=rows, sources=ints([0, 0]))
+    for x in (k, v):
+        from_rows, to_rows = (x[0, table[i].long(), 0].reshape(-1, 64)[:rows] for i in (0, 1))
+        assert torch.equal(from_rows[3:], to_rows[3:]) and not torch.equal(from_rows[:3], to_rows[:3])
+
+
 def test_offsets_past_32_bits():
     L, H, page, D = 2, 2, 16, 64
     pages = 2 ** 31 // (H * page * D) // L + 9

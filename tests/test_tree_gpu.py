@@ -191,7 +191,7 @@ def test_any_set_of_nodes_and_always_itself():
 
 @pytest.mark.parametrize("lens,H,G,T", [([5000], 1, 1, 4), ([5000], 1, 1, 64), ([1, 20001, 3], 2, 1, 20), ([9000] + [7] * 70, 1, 4, 8), ([33] * 200, 3, 1, 6), ([4096] * 3, 4, 8, 16),
                                         ([0], 1, 1, 1), ([-1] * 100 + [700] + [-1] * 100, 2, 2, 10), ([50] * 300 + [4000] + [11] * 100, 2, 1, 3), ([17] * 4200 + [900], 1, 1, 2),
-                                        ([30000], 2, 8, 32)])
+                                        ([30000], 2, 8, 32), ([17] * 300 + [900], 1, 8, 20), ([17] * 300 + [900, -1], 1, 2, 20), ([6000, 5, 0], 1, 8, 10)])
 def test_work_is_split_over_what_is_there(lens, H, G, T):
     """One long row, long ones among many short, more sequences than a wavefront or a workgroup has lanes, free slots all around."""
     print(f"tree attention of {len(lens)} sequences, the longest {max(lens)}, H{H} G{G} T{T}", flush=True)
