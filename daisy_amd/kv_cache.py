@@ -300,17 +300,25 @@ class PagedKVCache:
             raise RuntimeError(f"the paged cache has {len(slots)} free slots for {count} sequences")
         full, rest = divmod(n, self.page_size)
         self._take({s: range(full, full + (rest > 0)) for s in slots}, {})
-        for s in slots:
-            for entry, page in self._owned[slot].items():
-                if entry < full:
-                    self._set(s, entry, page)
-        self._upload()
-        if rest:
-            copied = torch.zeros((3, self.sequences), dtype=torch.int32)
-            copied[2] = slot
-            copied[0, slots], copied[1, slots] = full * self.page_size, rest
-            starts, counts, sources = copied.to(self.page_table.device)
-            ops.paged_move(self.k, self.v, self.page_table, starts, counts, rows=self.page_size, sources=sources, status=self.status)
+        try:
+            for s in slots:
+                for entry, page in self._owned[slot].items():
+                    if entry < full:
+                        self._set(s, entry, page)
+            self._upload()
+            if rest:
+                copied = torch.zeros((3, self.sequences), dtype=torch.int32)
+                copied[2] = slot
+                copied[0, slots], copied[1, slots] = full * self.page_size, rest
+                starts, counts, sources = copied.to(self.page_table.device)
+                ops.paged_move(self.k, self.v, self.page_table, starts, counts, rows=self.page_size, sources=sources, status=self.status)
+        except BaseException:
+            for s in slots:
+                for entry in list(self._owned[s]):
+                    self._set(s, entry, -1)
+                self._reach[s] = 0
+            self._upload()
+            raise
         self._open(slots, [n] * count)
         return slots
 

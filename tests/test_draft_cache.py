@@ -139,6 +139,17 @@ def test_a_fork_that_does_not_fit_leaves_the_cache_as_it_was(moves):
         assert state(c) == before and not moves
 
 
+def test_a_fork_whose_copy_fails_leaves_the_cache_as_it_was():
+    c = cpu_cache()
+    c.admit([5, 37])
+    before = state(c)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        c.fork(1, 2)
+    after = state(c)
+    assert after[0] == before[0] and after[2:] == before[2:] and after[1] == before[1]
+    consistent(c)
+
+
 def test_pages_that_a_window_leaves_go_back_when_the_last_fork_leaves_them(moves):
     c = cpu_cache(sequences=2, pages=6, window=16)
     c.admit([31])
