@@ -393,7 +393,7 @@ __device__ __forceinline__ double lane_of(double x, int lane) {
 __device__ __forceinline__ float lane_of(float x, int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane)); }
 
 // A workgroup per sequence: its wavefronts join the slices of the rows, one of them walks.  Latency: 5 us for a tree of 8 nodes, 8 to 9 for 32 of 16.
-constexpr int kWalkThreads = 512;
+constexpr int kWalkThreads = 1024;      // at most: a row of the tree for each wavefront, where there are so many (32 trees of 16 nodes 25.8 us, with 512 27.0; one of 8 9.5, with 1024 9.8)
 template <int E, int MODE>
 __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams p) {
   __shared__ RowPart rows[kMostNodes];
@@ -513,7 +513,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams 
     const float* noise = p.noise + b * p.noise_sb;
     const double top = (double)rows[unsure].top;
     Best best = {-__builtin_inf(), INT32_MAX};
-    for (int v = tid; v < p.V; v += kWalkThreads) {
+    for (int v = tid; v < p.V; v += (int)blockDim.x) {
       const double score = ((double)score_at<E>(row, v) - top) * by + (double)noise[v];
       if (!(score >= best.score)) continue;
       bool taken = false;
@@ -524,8 +524,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams 
     if (lane == 0) bests[wv] = best;
     __syncthreads();
     if (tid == 0) {
-#pragma unroll
-      for (int w = 1; w < kWalkThreads / 64; ++w) best = better(best, bests[w]);
+      for (int w = 1; w < (int)blockDim.x / 64; ++w) best = better(best, bests[w]);
       token = best.score > -__builtin_inf() ? best.token : -1;
     }
   }
@@ -778,6 +777,7 @@ template <int E, int MODE> static void rows_launch(const VerifyParams& p, int ro
   else hipLaunchKernelGGL((verify_rows_kernel<E, MODE, 4>), grid, dim3(kThreads), 0, s, p);
 }
 template <int E> static void verify_launch(const VerifyParams& p, int rounds, hipStream_t s) {
+  const dim3 walkers(p.T > 8 ? kWalkThreads : kWalkThreads / 2);
   if (p.q != nullptr) {
     rows_launch<E, kDrawn>(p, rounds, s);
     hipLaunchKernelGGL((verify_draw_kernel<E>), dim3((unsigned)p.B), dim3(kDrawThreads), 0, s, p);
@@ -785,10 +785,10 @@ template <int E> static void verify_launch(const VerifyParams& p, int rounds, hi
     hipLaunchKernelGGL((verify_last_kernel<E>), dim3((unsigned)p.B), dim3(kThreads), 0, s, p);
   } else if (p.noise != nullptr) {
     rows_launch<E, kChosen>(p, rounds, s);
-    hipLaunchKernelGGL((verify_walk_kernel<E, kChosen>), dim3((unsigned)p.B), dim3(kWalkThreads), 0, s, p);
+    hipLaunchKernelGGL((verify_walk_kernel<E, kChosen>), dim3((unsigned)p.B), walkers, 0, s, p);
   } else {
     rows_launch<E, kGreedy>(p, rounds, s);
-    hipLaunchKernelGGL((verify_walk_kernel<E, kGreedy>), dim3((unsigned)p.B), dim3(kWalkThreads), 0, s, p);
+    hipLaunchKernelGGL((verify_walk_kernel<E, kGreedy>), dim3((unsigned)p.B), walkers, 0, s, p);
   }
 }
 
