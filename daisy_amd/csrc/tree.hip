@@ -723,8 +723,19 @@ __global__ __launch_bounds__(64 * NW, wide_waves_per_simd(D)) void tree_wide_ker
   SplitUnit beyond = {-1, 0, 0, 0, 0, 0};
   if (x < x_end) deal.go_to(p, x);
 
-  const int k_row = p.k_ss * 16, v_row = p.v_ss * 16;      // bytes
+  // this lane's part of a copy: its row's place behind the half tile's first one, in bytes, the row's piece swizzled
+  constexpr int EACH = COPIES < NW ? 1 : COPIES / NW;      // copies of a tile's keys, or of its values, a wavefront (or of either, by half of the wavefronts each)
+  static_assert(COPIES % NW == 0 || 2 * COPIES == NW, "");
   const int ld_row = lane / CPR, ld_pos = lane % CPR;
+  auto copy_of = [&](int e) { return COPIES < NW ? wv % COPIES : e * NW + wv; };
+  auto piece_of = [&](auto swizzle, int e) { return 16 * (ld_pos ^ swizzle(RPL * copy_of(e) + ld_row)); };
+  auto row_of = [&](int e) { return (RPL * copy_of(e) + ld_row) & 15; };
+  int k_off[EACH], v_off[EACH];
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    k_off[e] = row_of(e) * (int)(p.k_ss * 16) + piece_of(swz_k, e);
+    v_off[e] = row_of(e) * (int)(p.v_ss * 16) + piece_of(swz_v, e);
+  }
   const uint32_t k_a0 = lds_address(staged) + 2 * (n * D + 8 * (c ^ swz_k(n)));
   uint32_t v_a0;
   {
@@ -743,36 +754,38 @@ __global__ __launch_bounds__(64 * NW, wide_waves_per_simd(D)) void tree_wide_ker
     const int32_t* row = p.table + product(b, p.table_st);
     const int blk_lo = (unsigned)e.lo / kBlock, blk_hi = max(e.hi - 1, 0) / kBlock;
     bool bad = e.past;
-    int id = 0, in = 0;
+    // lane i has where the run's block i lies, its first row of the unit's key head, in k and in v, for 32 tiles at a time
+    uint64_t k_at = 0, v_at = 0;
     auto pages_from = [&](int block) {
       const int blk = min(max(block + lane, blk_lo), blk_hi);      // (blocks outside the range: read, but not used)
       const Quotient page = divide((uint32_t)blk, p.blocks_per_page);
-      in = page.rest;
-      id = row[page.of];
+      const int id = row[page.of];
       const bool out = (unsigned)id >= (unsigned)p.num_pages;
       bad |= out;
-      id = out ? 0 : id;
+      const int there = out ? 0 : id, in = page.rest * kBlock;
+      k_at = (uint64_t)p.k + 16 * (product(h, p.k_sh) + product(there, p.k_sp) + product(in, p.k_ss));
+      v_at = (uint64_t)p.v + 16 * (product(h, p.v_sh) + product(there, p.v_sp) + product(in, p.v_ss));
     };
-    const char* kh = reinterpret_cast<const char*>(p.k) + 16 * product(h, p.k_sh);
-    const char* vh = reinterpret_cast<const char*>(p.v) + 16 * product(h, p.v_sh);
     const int tile0 = e.first + off;
-    auto copy_rows = [&](const char* from_pages, uint32_t sp, uint32_t ss, int row_bytes, auto swizzle, int i, uint32_t to, int first_wave) {
+    auto copy_rows = [&](uint64_t at, const int* offsets, uint32_t ss, auto swizzle, int i, uint32_t to, bool mine) {
+      if (COPIES < NW && !mine) return;
       const int tile = (tile0 + i) * kTile;
       const bool whole = tile >= e.lo && tile + kTile <= e.hi;
 #pragma unroll
-      for (int j0 = 0; j0 < COPIES; j0 += NW) {
-        const int j = j0 + wv - first_wave;
-        if (COPIES < NW && (unsigned)j >= (unsigned)COPIES) break;
-        const int half = RPL * j >> 4, r = RPL * j + ld_row;
-        const int pg = __builtin_amdgcn_readlane(id, 2 * (i & 31) + half), slot = __builtin_amdgcn_readlane(in, 2 * (i & 31) + half) * kBlock;
-        // a row of the half, or where that is outside the range, another one that is
-        const int first = tile + half * kBlock, own = r & 15;
-        const int from = whole ? own : min(max(own, min(max(e.lo - first, 0), kBlock - 1)), min(max(e.hi - 1 - first, 0), kBlock - 1));
-        copy16_to_lds_async((const uint16_t*)(from_pages + 16 * (product(pg, sp) + product(slot, ss))), from * row_bytes + 16 * (ld_pos ^ swizzle(r)), to + 1024 * j);
+      for (int c = 0; c < EACH; ++c) {
+        const int j = copy_of(c), half = RPL * j >> 4, from = 2 * (i & 31) + half;
+        const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)at, from), hi = __builtin_amdgcn_readlane((int)(uint32_t)(at >> 32), from);
+        int offset = offsets[c];
+        if (!whole || D == 256) {      // (whose registers are all taken)
+          // a row of the half, or where that is outside the range, another one that is
+          const int first = tile + half * kBlock;
+          offset = min(max(row_of(c), min(max(e.lo - first, 0), kBlock - 1)), min(max(e.hi - 1 - first, 0), kBlock - 1)) * (int)(ss * 16) + piece_of(swizzle, c);
+        }
+        copy16_to_lds_async((const uint16_t*)((uint64_t)hi << 32 | lo), offset, to + 1024 * j);
       }
     };
-    auto copy_k = [&](int i, int slot) { copy_rows(kh, p.k_sp, p.k_ss, k_row, swz_k, i, lds_address(staged) + 4 * TILE * slot, 0); };
-    auto copy_v = [&](int i, int slot) { copy_rows(vh, p.v_sp, p.v_ss, v_row, swz_v, i, lds_address(staged) + 4 * TILE * slot + 2 * TILE, COPIES < NW ? COPIES : 0); };
+    auto copy_k = [&](int i, int slot) { copy_rows(k_at, k_off, p.k_ss, swz_k, i, lds_address(staged) + 4 * TILE * slot, wv < COPIES); };
+    auto copy_v = [&](int i, int slot) { copy_rows(v_at, v_off, p.v_ss, swz_v, i, lds_address(staged) + 4 * TILE * slot + 2 * TILE, wv >= COPIES); };
     // Tile i is in slot i % STAGES.  Ahead of tile i's softmax K(i + 1) and V(i) have landed, and V(i + STAGES - 1) and K(i + STAGES) are asked for, whose slots the tile before and this one's
     // scores have left.
     pages_from(2 * tile0);
@@ -809,9 +822,7 @@ __global__ __launch_bounds__(64 * NW, wide_waves_per_simd(D)) void tree_wide_ker
       asm volatile("" ::: "memory");
       __syncthreads();
     };
-    // copies of a tile's keys and values a wavefront; or of either, by half of the wavefronts each
-    constexpr int PER = COPIES < NW ? 1 : 2 * (COPIES / NW);
-    static_assert(COPIES % NW == 0 || 2 * COPIES == NW, "");
+    constexpr int PER = COPIES < NW ? 1 : 2 * EACH;      // copies of a tile a wavefront
     using All = std::integral_constant<int, 0>;
     f32x16 sc;
     auto scores = [&](int slot) {
