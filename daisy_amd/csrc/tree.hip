@@ -684,8 +684,8 @@ __global__ __launch_bounds__(256, 1) void tree_attn_kernel(TreeParams p) {
 // 16 bytes a lane, the next tile's while this one is computed, and all wavefronts read them there: V's through transposing reads.  Products are 32x32x16: a lane
 // has a column and 16 of a tile's keys, 8 (r / 4) + 4 (lane / 32) + r % 4.  Partial sums of units that the run begins or ends in the middle of go to the second kernel.
 //
-// Bound by the matrix cores, whose work the probabilities' second part makes half as much again, by the exponentials, and by the clock that is left beside both: 12 sequences of 100 to 24000, 8 key heads of 8 query heads, 32 nodes, D = 128 (76 GFLOP, 307 MB): 130 us, 580 TFLOP/s
-// of the formula's products.  A long run of it takes 72 % of its time without copies and exponentials.
+// Bound by the matrix cores, whose work the probabilities' second part makes half as much again, by the exponentials, and by the clock that is left beside both: 12 sequences of 100 to 24000, 8 key heads of 8 query heads, 32 nodes, D = 128 (76 GFLOP, 307 MB): 128 us, 590 TFLOP/s
+// of the formula's products.  A tile takes some 2700 cycles, 770 of them the products', with two wavefronts a SIMD; a long run 72 % of its time without copies and exponentials.
 //
 // 16-byte pieces of a row are swizzled by the row, so that the reads of an operand fall into different banks: K's by all of the row, V's, of which a transposing read takes four
 // rows at once, by two bits.
@@ -999,7 +999,7 @@ __device__ __forceinline__ int64_t part_slot(const TreeParams& p, const SplitUni
   return (int64_t)(2 * (u.first + i) + (i == 0 ? 1 : 0)) * p.cols + col;
 }
 
-// Joins the partial sums of the units that lie in more than one workgroup's run (3 to 5 us for few columns; 256 columns, 43 MB of sums: 17).  The results of up to 16 of a unit's columns are dealt to as many workgroups as there are ends
+// Joins the partial sums of the units that lie in more than one workgroup's run (3 to 5 us for few columns; 256 columns, 43 MB of sums: 10).  The results of up to 16 of a unit's columns are dealt to as many workgroups as there are ends
 // of runs in it.  Many parts: LPR lanes to a piece of 4 LPR channels and 256 / LPR parts side by side, the lanes' sums joined in the LDS.
 template <int D, bool F16, int LPR>
 __device__ __forceinline__ void join_many(const TreeParams& p, const SplitUnit& u, int col0, int cols, int parts, int helpers, int me, f32x4* sums, float2* stats) {
@@ -1095,7 +1095,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeParams p) {
 }
 
 // Up to 16 columns a wavefront by itself, up to 32 too where its registers hold them (D < 256), else workgroups of 64 columns, of 128 or of 256; as many workgroups as the chip holds
-// at once, fewer where there are fewer tiles.  A workgroup of 256 reads a tile once for what two of 128 read it twice: 150 us against 162 (12 sequences of 100 to 24000, 8 key
+// at once, fewer where there are fewer tiles.  A workgroup of 256 reads a tile once for what two of 128 read it twice: 150 us against 162 when it was tried (12 sequences of 100 to 24000, 8 key
 // heads of 8 query heads, 32 nodes, D = 128), 305 against 332 (32 of 8000, 4 query heads, 64 nodes, D = 64).  D = 256 leaves room for one wavefront a SIMD: four, although half of them have
 // no column, take 332 us for what two take 446 for (16 of 8000, 64 columns), because twice as many copies are on their way.
 struct TreeSplit { int groups, cols, blocks, NC, NW; size_t lds; };      // NC: pieces of 16 columns of a wavefront, or 0 and NW: wavefronts of 32
