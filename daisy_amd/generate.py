@@ -484,7 +484,8 @@ class Generator:
             scores = self._biased(self._trim(logits).reshape(B * T, -1)).view(B, T, -1)
             kw = {}
             if self.temperature != 0.0:
-                scores = keep_nucleus(keep_top_k(scores / max(self.temperature, 1e-6), self.top_k), self.top_p)
+                # (in fp32: a quotient past fp16's range would be a row that nothing can follow)
+                scores = keep_nucleus(keep_top_k(scores.float() / max(self.temperature, 1e-6), self.top_k), self.top_p)
                 like = torch.empty(B, scores.size(2), device=dev)
                 kw = dict(temperature=1.0, accept=torch.rand(B, T, device=dev), noise=gumbel_noise(like))
             path, counts, following = ops.verify_drafts(scores, tokens, parents, nodes=core.ints_on(dev, nodes), **kw)

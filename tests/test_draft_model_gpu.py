@@ -214,6 +214,9 @@ def test_drafts_with_a_bias_a_temperature_and_an_end():
         gen = generator(model, logit_bias={17: 1000.0}, **kw)
         right = oracle_drafts([[17] * 9] * 2, firsts, 6, 0.2)
         assert gen.generate_ragged(prompts, 9, drafts=right).tolist() == [[17] * 9] * 2
+    # scores over a temperature beyond fp16's range (the first token is drawn as ever, in the generator's dtype, where several of them are infinite)
+    gen = generator(model, dtype=torch.float16, temperature=1e-5, logit_bias={17: 50.0})
+    assert gen.generate_ragged(prompts, 9, drafts=oracle_drafts([[17] * 9] * 2, firsts, 4, 0.2))[:, 1:].tolist() == [[17] * 8] * 2
     # the end of the sequence inside an accepted path, and as the first token
     gen = generator(model, logit_bias={1: 1000.0})
     assert gen.generate_ragged(prompts, 5, drafts=oracle_drafts([[1] * 5] * 2, firsts, 3, 0.0)).tolist() == [[1] * 5] * 2
