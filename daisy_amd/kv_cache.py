@@ -336,6 +336,13 @@ class PagedKVCache:
 
     def begin_step(self) -> None:
         """Makes room for one more position of every sequence, from the pages that a window has left behind and the pool."""
+        if self._drafted is None:
+            size, most = self.page_size, self.max_len
+            for slot, n in enumerate(self._length):
+                if n is not None and (n >= self._reach[slot] * size or n >= most):
+                    break
+            else:
+                return      # (as in most steps)
         self._make_room([1] * self.sequences)
 
     def begin_draft(self, nodes: List[int]) -> None:
