@@ -16,7 +16,7 @@ import torch
 _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "csrc", "libdaisy_hip.so")
 _lib: Optional[ctypes.CDLL] = None
 
-ABI_VERSION = 6
+ABI_VERSION = 7
 LINEAR_MAX_ROWS = 8
 STATUS_POSITION_PAST_TABLES = 1
 STATUS_LENGTH_PAST_PAGES = 2
@@ -207,7 +207,7 @@ SIGNATURES = {
     "daisy_verify_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
     "daisy_verify_fwd": (c_int, [
         c_void_p, _I64P, c_int, c_void_p, c_int64, c_int,       # logits (+ strides), type, tokens (+ row stride), are int64
-        c_void_p, c_int64, c_void_p, c_void_p, c_float,         # parents (+ row stride), nodes, temperature (rows, number)
+        c_void_p, c_int64, c_void_p, c_void_p, c_double,        # parents (+ row stride), nodes, temperature (rows, number)
         c_void_p, c_int64, c_void_p, c_int64, c_void_p, _I64P,  # accept, noise (+ row strides), draft (+ strides)
         c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,      # path, counts, next, B, T, V
         c_void_p, c_size_t, c_void_p]),                         # workspace, bytes, stream

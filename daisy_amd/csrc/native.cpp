@@ -1054,7 +1054,7 @@ PyObject* py_verify_drafts(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const Strides2 ds = draft ? Strides2(*draft) : Strides2();
   int32_t* counts = (int32_t*)(base + 8 * B);
   const int rc = daisy_verify_fwd(ptr(x), xs.s, type == at::kFloat ? 0 : type == at::kBFloat16 ? 1 : 2, ptr(tokens), tokens.stride(0), tokens.scalar_type() == at::kLong,
-                                  (const int32_t*)ptr(parents), shared_stride(parents), (const int32_t*)ptr(nodes), (const float*)ptr(rows), (float)temperature,
+                                  (const int32_t*)ptr(parents), shared_stride(parents), (const int32_t*)ptr(nodes), (const float*)ptr(rows), temperature,
                                   (const float*)ptr(accept), accept ? accept->stride(0) : 0, (const float*)ptr(noise), noise ? noise->stride(0) : 0, (const float*)ptr(draft),
                                   draft ? ds.s : nullptr, counts + B, counts, (int64_t*)base, (int)B, (int)T, (int)V, work, work_bytes, stream_of(dev));
   if (rc != DAISY_OK) return none();

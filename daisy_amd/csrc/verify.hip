@@ -16,6 +16,7 @@
 // the two are nearer than fp32 tells apart, the row is gone over again in 64 bits.
 #include "common.h"
 
+#include <float.h>
 #include <math.h>
 
 #include <type_traits>
@@ -32,7 +33,7 @@ struct VerifyParams {
   const void* tokens; int64_t tokens_sb; int tokens64;      // [B, T]
   const int32_t* parents; int64_t parents_sb;               // [B, T]
   const int32_t* nodes;
-  float temperature; const float* temperatures;
+  double temperature; const float* temperatures;
   const float* accept; int64_t accept_sb;                   // [B, T]
   const float* noise; int64_t noise_sb;                     // [B, V]
   const float* q; int64_t q_sb, q_st;                       // [B, T, V]
@@ -50,8 +51,8 @@ struct Left { double scale, less; int at; float top; };     // max(scale e - les
 
 // 1 / t, 0 where the likeliest token is wanted
 __device__ __forceinline__ double inverse_temperature(const VerifyParams& p, int b) {
-  const float t = p.temperatures != nullptr ? p.temperatures[b] : p.temperature;
-  return t > 0.f ? 1.0 / (double)t : 0.0;
+  const double t = p.temperatures != nullptr ? (double)p.temperatures[b] : p.temperature;
+  return t > 0.0 ? fmin(1.0 / t, 1e300) : 0.0;
 }
 __device__ __forceinline__ int nodes_of(const VerifyParams& p, int b) { return p.nodes != nullptr ? min(max(p.nodes[b], 0), p.T) : p.T; }
 // The token of node j (-1: none that the vocabulary has).
@@ -806,7 +807,7 @@ extern "C" size_t daisy_verify_workspace_bytes(int B, int T, int V) {
 }
 
 extern "C" int daisy_verify_fwd(const void* logits, const int64_t* logits_strides, int type, const void* tokens, int64_t tokens_stride, int tokens_are_int64,
-                                const int32_t* parents, int64_t parents_stride, const int32_t* nodes, const float* temperature_rows, float temperature,
+                                const int32_t* parents, int64_t parents_stride, const int32_t* nodes, const float* temperature_rows, double temperature,
                                 const float* accept, int64_t accept_stride, const float* noise, int64_t noise_stride, const float* draft, const int64_t* draft_strides,
                                 int32_t* path, int32_t* counts, int64_t* next, int B, int T, int V, void* workspace, size_t workspace_bytes, void* stream) {
   DAISY_CHECK_ARG(logits && logits_strides && tokens && parents && path && counts && next, "verify: the scores, the tokens, the parents and the results must be non-NULL");
@@ -815,8 +816,8 @@ extern "C" int daisy_verify_fwd(const void* logits, const int64_t* logits_stride
   DAISY_CHECK_SUPPORTED(type >= 0 && type <= 2, "verify: type %d not supported (0 fp32, 1 bf16, 2 fp16)", type);
   DAISY_CHECK_ARG(logits_strides[0] >= 0 && logits_strides[1] >= 0 && tokens_stride >= 0 && parents_stride >= 0 && accept_stride >= 0 && noise_stride >= 0,
                   "verify: strides must not be negative");
-  DAISY_CHECK_ARG(temperature_rows || (temperature >= 0.f && isfinite(temperature)), "verify: the temperature must not be negative, and finite");
-  const bool greedy = !temperature_rows && temperature == 0.f;
+  DAISY_CHECK_ARG(temperature_rows || (temperature >= 0.0 && temperature <= (double)FLT_MAX), "verify: the temperature must not be negative, and finite in fp32");
+  const bool greedy = !temperature_rows && temperature == 0.0;
   DAISY_CHECK_ARG(greedy || (accept && noise), "verify: a temperature needs the numbers of the acceptance and the noise");
   DAISY_CHECK_ARG(!draft || (draft_strides && draft_strides[0] >= 0 && draft_strides[1] >= 0), "verify: the draft's probabilities need strides that are not negative");
   DAISY_CHECK_ARG(reinterpret_cast<uintptr_t>(logits) % (type == kScoreF32 ? 4 : 2) == 0, "verify: tensors must be aligned to their elements");

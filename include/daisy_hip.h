@@ -618,7 +618,7 @@ int daisy_logits_process_fwd(const void* x, int64_t x_stride, void* y, int64_t y
  * logits     : [B, T, V], type 0 = fp32, 1 = bf16, 2 = fp16, strides {sequence, node}; -inf: a token that may not follow.
  * tokens     : int32 or int64 (tokens_are_int64) [B, T] with a row stride; a token outside 0 .. V - 1 is no candidate.
  * parents, nodes: as for daisy_draft_tree_fwd; a node that does not come from node 0 is never accepted.
- * temperature: a number, or, where temperature_rows is given, fp32 [B] (zero or less: the largest score).
+ * temperature: a number, no larger than the largest of fp32, or, where temperature_rows is given, fp32 [B] (zero or less: the largest score).
  * accept     : fp32 [B, T] with a row stride, in [0, 1);  noise: fp32 [B, V] with a row stride, finite;  both may be NULL where temperature is the number 0.
  * draft      : fp32 [B, T, V], strides {sequence, node}, or NULL.
  * path       : int32 [B, T], the accepted nodes from node 0 on, -1 behind them;  counts: int32 [B], how many;  next: int64 [B], the token that follows, -1
@@ -630,7 +630,7 @@ size_t daisy_verify_workspace_bytes(int B, int T, int V);
 int daisy_verify_fwd(const void* logits, const int64_t* logits_strides, int type,
                      const void* tokens, int64_t tokens_stride, int tokens_are_int64,
                      const int32_t* parents, int64_t parents_stride, const int32_t* nodes,
-                     const float* temperature_rows, float temperature,
+                     const float* temperature_rows, double temperature,
                      const float* accept, int64_t accept_stride, const float* noise, int64_t noise_stride,
                      const float* draft, const int64_t* draft_strides,
                      int32_t* path, int32_t* counts, int64_t* next, int B, int T, int V,
