@@ -12,8 +12,9 @@
 // One pass over all scores leaves, of every row and slice of the vocabulary, its largest score, its sum and what would follow: which tokens are children's is known ahead of the walk.  A second
 // kernel joins the slices and walks; where children were drawn, two more draw from what the walk has left of the last row.
 //
-// Sums of exponentials are fp32 in a slice and 64 bits beyond it, the children's e and all that decides about them 64 bits.  What follows is looked for in fp32, with the second best beside it: where
-// the two are nearer than fp32 tells apart, the row is gone over again in 64 bits.
+// Sums of exponentials are fp32 in a slice and 64 bits beyond it (within 2^-17 of themselves, see kSumOff), the children's e fp32 exponentials of 64-bit arguments: that is how near the numbers of an acceptance are where
+// nothing has been subtracted.  What a rejected draft leaves, max(a p - b q, 0), may be any small part of p: its sum, the row's own sum in it and the children's share of it are 64 bits throughout.  What follows is looked for in fp32, with
+// bounds of what its keys are off by: where these do not tell the best one, the row is gone over again in 64 bits.
 #include "common.h"
 
 #include <float.h>
@@ -28,6 +29,9 @@ enum VerifyMode { kGreedy = 0, kChosen = 1, kDrawn = 2 };
 constexpr int kMostNodes = 256, kThreads = 256;
 constexpr int kPieceRounds = 4, kPiece = 4 * kThreads * kPieceRounds;      // of a row that is drawn from: a workgroup's
 
+// What the sum of a row's slices is off by at most, and an fp32 exponential for each unit of its argument to the base 2 (derived at verify_sample_kernel).
+constexpr float kSumOff = 0x1p-16f, kExpOff = 0x1p-22f;
+
 struct VerifyParams {
   const void* x; int64_t x_sb, x_st;                        // [B, T, V]
   const void* tokens; int64_t tokens_sb; int tokens64;      // [B, T]
@@ -40,14 +44,17 @@ struct VerifyParams {
   int32_t* path; int32_t* counts; int64_t* next;
   f32x4* part; int32_t* part_token;                         // [B, T, slices]: sum, top, best, second (RowPart) and the best one's token
   struct Left* left;                                        // [B]: what is to be drawn from
-  float2* drawn; int32_t* drawn_token; int pieces;          // [B, pieces]: best and second, and the best one's token
+  f32x4* drawn; int pieces;                                 // [B, pieces]: Key
   int B, T, V, slices, slice, rows;                         // slice: of a wavefront; rows: of a workgroup
 };
 
 // Of some of a row beside its children's tokens: the largest score, the sum of e relative to that; the two best of x / t + noise, relative to it, too (a noise added to a mask of the type's lowest
 // value would be lost), and the best one's token (INT32_MAX: none).
 struct RowPart { double sum; float top, best, second; int token; };
-struct Left { double scale, less; int at; float top; };     // max(scale e - less q, 0) of row `at`, whose largest score is `top`; at < 0: nothing to be drawn
+// max(scale e - less q, 0) of row `at`, whose largest score is `top`; at < 0: nothing to be drawn; exact: `scale` comes from a sum of the row in 64 bits, not from that of its slices
+struct Left { double scale, less; int at; float top; int exact, unused; };
+// Of some of a row: the largest of what the keys may be at most, what that one is at least, the largest of the others', and the token.
+struct Key { float most, least, others; int token; };
 
 // 1 / t, 0 where the likeliest token is wanted
 __device__ __forceinline__ double inverse_temperature(const VerifyParams& p, int b) {
@@ -165,6 +172,19 @@ __device__ __forceinline__ Two wave_two(Two x, int group = 64) {
     const LanePair b = neighbours<S>(x.best), n = neighbours<S>(x.second);
     const IntPair t = neighbours<S>(x.token);
     x = both(Two{b.x, n.x, t.x}, Two{b.y, n.y, t.y});
+  });
+  return x;
+}
+__device__ __forceinline__ Key both(Key a, Key b) {
+  const bool other = b.most > a.most || (b.most == a.most && b.token < a.token);
+  return Key{other ? b.most : a.most, other ? b.least : a.least, fmaxf(fmaxf(a.others, b.others), other ? a.most : b.most), other ? b.token : a.token};
+}
+__device__ __forceinline__ Key wave_key(Key x) {
+  steps(64, [&](auto s) {
+    constexpr int S = decltype(s)::value;
+    const LanePair m = neighbours<S>(x.most), l = neighbours<S>(x.least), o = neighbours<S>(x.others);
+    const IntPair t = neighbours<S>(x.token);
+    x = both(Key{m.x, l.x, o.x, t.x}, Key{m.y, l.y, o.y, t.y});
   });
   return x;
 }
@@ -536,20 +556,34 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams 
   if (tid < p.T) p.path[(int64_t)b * p.T + tid] = path[tid];
 }
 
+// 2^(y / 32), y <= 0, to 2^-47 of itself (and 2^-53 of y): the nearest 32nd of a power from a table, and five terms of the series for what is left of the exponent, whose sixth is below (ln2 / 64)^6 / 6! = 2^-48.
+constexpr int kPowers = 32;
+__device__ __forceinline__ double power_of(const double* powers, double y) {
+  constexpr double c = 0.6931471805599453 / kPowers;
+  y = fmax(y, -1100.0 * kPowers);
+  const double whole = rint(y), g = y - whole;
+  const int i = (int)whole;
+  const double series = fma(g, fma(g, fma(g, fma(g, fma(g, c * c * c * c * c / 120, c * c * c * c / 24), c * c * c / 6), c * c / 2), c), 1.0);
+  return ldexp(powers[i & (kPowers - 1)] * series, i >> 5);
+}
+
 // Drawn children: a workgroup per sequence goes over a whole row where a rejection has to be taken out of it for the child behind.  The first wavefront walks and tells the others what
 // to do: nobody decides by numbers that it has read by itself.
+//
+// All that is left of a row after a rejection is in 64 bits, exponentials too, and so is the row's own sum, which the first such pass takes beside the subtraction: a draft next to the target leaves less than fp32 has
+// bits for.  Bound by these exponentials, on one compute unit a sequence: trees of 16 nodes with several children to a node over 50257 tokens 34 us for one sequence, 90 to 156 for 32 (all four kernels; with fp32, which
+// took other tokens where the draft is within 1e-4, 27 and 70 to 115; with a pass of its own for the row's sum and the library's exponentials 43 and 120 to 189).
 constexpr int kDrawThreads = 1024;
 template <int E>
 __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyParams p) {
   __shared__ RowPart rows[kMostNodes];
   __shared__ int path[kMostNodes];
   __shared__ Left todo;
-  __shared__ double sums[kDrawThreads / 64];
+  __shared__ double powers[kPowers], sums[kDrawThreads / 64], row_sums[4][kDrawThreads / 64];
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   const double inv_t = inverse_temperature(p, b);
   const bool greedy = inv_t == 0.0;
   const double by = greedy ? 1.0 : inv_t;
-  const float c = (float)fmin(by * 1.4426950408889634, 1e30);
   const int n = nodes_of(p, b);
   Tree t = {};
   if (wv == 0) t = tree_of(p, b, lane);
@@ -566,19 +600,26 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyParams 
   }
   join_rows<kDrawn>(p, b, n, by, rows);
   if (tid < p.T) path[tid] = -1;
+  if (tid < kPowers) powers[tid] = exp2((double)tid / kPowers);
+  const double per = by * (1.4426950408889634 * kPowers);
   __syncthreads();
   // the first wavefront's: where it is, the child that it has looked at last, what is left of the row
   int at = n > 0 ? 0 : -1, last = 0, count = 0;
   double scale = 0.0, less = 0.0;
   bool fresh = true, rejected = false, summed = false;      // rejected: the last child, and it is not taken out yet; summed: the row's sum without it is there
+  bool exact = false;      // `whole`, the row's sum in 64 bits, is there, and `scale` comes from it
+  double whole = 0.0, left_sum = 0.0;
   int64_t token = -1;
-  Left sample = {0.0, 0.0, -1, 0.f};
+  Left sample = {0.0, 0.0, -1, 0.f, 0, 0};
+  const auto wave_total = [&](const double* of) { return wave_sum64(lane < kDrawThreads / 64 ? of[lane] : 0.0); };
   for (;;) {
     if (wv == 0) {
-      Left next = {0.0, 0.0, -1, 0.f};
+      Left next = {0.0, 0.0, -1, 0.f, 0, 0};
       if (summed) {
-        const double z = wave_sum64(lane < kDrawThreads / 64 ? sums[lane] : 0.0);
-        scale = z > 0.0 ? scale / z : 1.0 / rows[at].sum;
+        const double z = left_sum;
+        if (!exact) scale = 1.0 / whole;
+        exact = true;
+        scale = z > 0.0 ? scale / z : 1.0 / whole;
         less = z > 0.0 ? less / z : 0.0;
       }
       bool walking = at >= 0;
@@ -590,7 +631,7 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyParams 
           last = at;
           scale = 1.0 / row.sum;
           less = 0.0;
-          rejected = fresh = false;
+          rejected = fresh = exact = false;
         }
         // the next child
         int j = -1;
@@ -616,15 +657,17 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyParams 
           fresh = true;
           if (j >= 0) at = j;
         } else if (j < 0) {
-          sample = Left{scale, rejected ? less + 1.0 : less, at, row.top};
+          if (rejected) less += 1.0;
+          const double unit = exact ? fmax(scale, less) : 1.0;      // (a factor of all that is left decides nothing, and with this one fp32 holds both)
+          sample = Left{scale / unit, less / unit, at, row.top, exact, 0};
           walking = false;
         } else if (rejected && !summed) {
           less += 1.0;
-          next = Left{scale, less, at, row.top};
+          next = Left{scale, less, at, row.top, exact, 0};
           walking = false;
         } else {
           summed = false;
-          const double left = fmax(scale * exp_of((x_j - (double)row.top) * by) - less * q_j, 0.0);
+          const double left = fmax(scale * exp((x_j - (double)row.top) * by) - less * q_j, 0.0);
           if (a_j * q_j < left) {
             at = j;
             fresh = true;
@@ -642,18 +685,54 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyParams 
     if (pass.at < 0) break;
     const void* x_row = row_of_x<E>(p, b, pass.at);
     const float* q_row = p.q + b * p.q_sb + pass.at * p.q_st;
-    const float top = pass.top, s32 = (float)pass.scale, l32 = (float)pass.less;
-    double total = 0.0;
-    for (int v = 4 * tid; v < p.V; v += 4 * kDrawThreads) {
-      const f32x4 xs = widen4<E>(load4<E>(x_row, v, p.V - v)), qs = load4_f32(q_row, v, p.V - v);
-      float sum = 0.f;
+    const double top = (double)pass.top;
+    // (four of each a thread, the next ones on their way)
+    const auto over_row = [&](auto each) {
+      auto raw = load4<E>(x_row, 4 * tid, p.V - 4 * tid);
+      f32x4 qs = load4_f32(q_row, 4 * tid, p.V - 4 * tid);
+      for (int v = 4 * tid; v < p.V; v += 4 * kDrawThreads) {
+        const f32x4 x4 = widen4<E>(raw), q4 = qs;
+        raw = load4<E>(x_row, v + 4 * kDrawThreads, p.V - v - 4 * kDrawThreads);
+        qs = load4_f32(q_row, v + 4 * kDrawThreads, p.V - v - 4 * kDrawThreads);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) sum += fmaxf(fmaf(s32, fast_exp2((xs[k] - top) * c), -l32 * qs[k]), 0.f);
-      total += (double)sum;
+        for (int k = 0; k < 4; ++k) each(power_of(powers, ((double)x4[k] - top) * per), (double)q4[k]);
+      }
+    };
+    double mul = pass.scale;
+    bool known = false;
+    if (!pass.exact) {
+      // The first rejection at this row, less = 1.  With the slices' sum for the row's own what is left would be sum(max(d, 0)); with its own it is that and sum(e, d > 0) times what the reciprocals differ by, but for
+      // those d whose sign the difference changes, off by no more than it.  Where that matters, or all that is left is below fp32's numbers, the row is gone over again.
+      double sum = 0.0, left = 0.0;
+      float above = 0.f, near = 0.f;      // (times the difference alone: fp32, 2^-16 of them)
+      const float near_by = (float)mul * kSumOff;
+      over_row([&](double e, double q_v) {
+        const double d = fma(mul, e, -q_v);
+        const float e32 = (float)e, d32 = (float)d;
+        sum += e;
+        left += fmax(d, 0.0);
+        above += d32 > 0.f ? e32 : 0.f;
+        near += fabsf(d32) <= near_by * e32 ? e32 : 0.f;
+      });
+      sum = wave_sum64(sum);
+      left = wave_sum64(left);
+      const double above64 = wave_sum64((double)above), near64 = wave_sum64((double)near);
+      if (lane == 0) { row_sums[0][wv] = sum; row_sums[1][wv] = left; row_sums[2][wv] = above64; row_sums[3][wv] = near64; }
+      __syncthreads();
+      whole = wave_total(row_sums[0]);
+      const double off = 1.0 / whole - mul, all_above = wave_total(row_sums[2]);
+      left_sum = wave_total(row_sums[1]) + all_above * off;
+      known = all_above > 0x1p-100 && fabs(off) <= mul * (kSumOff / 2) && fabs(off) * (wave_total(row_sums[3]) + 0x1p-16 * all_above) <= 0x1p-26 * left_sum;
+      mul = 1.0 / whole;
     }
-    total = wave_sum64(total);
-    if (lane == 0) sums[wv] = total;
-    __syncthreads();
+    if (!known) {
+      double total = 0.0;
+      over_row([&](double e, double q_v) { total += fmax(fma(mul, e, -pass.less * q_v), 0.0); });
+      total = wave_sum64(total);
+      if (lane == 0) sums[wv] = total;
+      __syncthreads();
+      left_sum = wave_total(sums);
+    }
   }
   if (tid == 0) {
     p.counts[b] = count;
@@ -664,9 +743,12 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyParams 
 }
 
 // What is left of the last row with its noise, the largest of it: max(scale e - less q, 0) exp(noise).  A workgroup takes a piece of the row (64 rows of 131072, 84 MB of scores, probabilities and noise: 15 us, 5.6 TB/s).
+//
+// In fp32, with what that may be off by.  Of scale e: the slices' sum 2^-17 (21 additions of exponentials that are off by 2^-23 (1 + |log2 e|) each, whose mean |log2 e| is below log2 V <= 30), scale's own rounding 2^-24, e's argument and e itself
+// 2^-23 (1 + 1.04 |log2 e|).  Of less q: two roundings, 2^-23.  Of the noise's exponential, up to 64: 2^-17.  All of it is below kSumOff + kExpOff |log2 e| of scale e + less q, however little their difference is.
 template <int E>
 __global__ __launch_bounds__(kThreads) void verify_sample_kernel(VerifyParams p) {
-  __shared__ Two twos[kThreads / 64];
+  __shared__ Key keys[kThreads / 64];
   const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   const Left left = p.left[b];
   if (left.at < 0) return;
@@ -674,7 +756,7 @@ __global__ __launch_bounds__(kThreads) void verify_sample_kernel(VerifyParams p)
   const float c = (float)fmin(by * 1.4426950408889634, 1e30), s32 = (float)left.scale, l32 = (float)left.less, top = left.top;
   const void* x_row = row_of_x<E>(p, b, left.at);
   const float *q_row = p.q + b * p.q_sb + left.at * p.q_st, *g_row = p.noise + b * p.noise_sb;
-  Two two = {0.f, 0.f, INT32_MAX};
+  Key key = {0.f, 0.f, 0.f, INT32_MAX};
   constexpr int R = kPieceRounds;
   typename Four<E>::Raw raw[R];
   f32x4 q[R], g[R];
@@ -690,55 +772,66 @@ __global__ __launch_bounds__(kThreads) void verify_sample_kernel(VerifyParams p)
     const f32x4 x = widen4<E>(raw[r]);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const float key = fmaxf(fmaf(s32, fast_exp2((x[k] - top) * c), -l32 * q[r][k]), 0.f) * fast_exp2(g[r][k] * kLog2e);
-      two.second = __builtin_amdgcn_fmed3f(key, two.best, two.second);
-      two.token = key > two.best ? (int)(blockIdx.x * kPiece) + 4 * (tid + r * kThreads) + k : two.token;
-      two.best = fmaxf(two.best, key);
+      const float y = fmaxf((x[k] - top) * c, -1000.f), e = fast_exp2(y), weight = fast_exp2(g[r][k] * kLog2e), lost = l32 * q[r][k];
+      const float rest = fmaf(s32, e, -lost), off = fmaf(s32, e, lost) * fmaf(-y, kExpOff, kSumOff);
+      const float most = fmaxf(rest + off, 0.f) * weight;
+      key.others = __builtin_amdgcn_fmed3f(most, key.most, key.others);
+      key.least = most > key.most ? (rest - off) * weight : key.least;
+      key.token = most > key.most ? (int)(blockIdx.x * kPiece) + 4 * (tid + r * kThreads) + k : key.token;
+      key.most = fmaxf(key.most, most);
     }
   }
-  two = wave_two(two);
-  if (lane == 0) twos[wv] = two;
+  key = wave_key(key);
+  if (lane == 0) keys[wv] = key;
   __syncthreads();
   if (tid == 0) {
 #pragma unroll
-    for (int w = 1; w < kThreads / 64; ++w) two = both(two, twos[w]);
-    const int64_t at = (int64_t)b * p.pieces + blockIdx.x;
-    p.drawn[at] = float2{two.best, two.second};
-    p.drawn_token[at] = two.token;
+    for (int w = 1; w < kThreads / 64; ++w) key = both(key, keys[w]);
+    p.drawn[(int64_t)b * p.pieces + blockIdx.x] = f32x4{key.most, key.least, key.others, __int_as_float(key.token)};
   }
 }
 
 // The pieces as one.  (Not by the last workgroup of a sequence's to come in the kernel above: its fences write back the L2s, 147 us for 64 rows of 131072 where the draw itself takes 17.)
 template <int E>
 __global__ __launch_bounds__(kThreads) void verify_last_kernel(VerifyParams p) {
-  __shared__ Two twos[kThreads / 64];
+  __shared__ Key keys[kThreads / 64];
   __shared__ Best bests[kThreads / 64];
+  __shared__ double sums[kThreads / 64];
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-  Two two = Two{0.f, 0.f, INT32_MAX};
+  Key key = {0.f, 0.f, 0.f, INT32_MAX};
   for (int i = tid; i < p.pieces; i += kThreads) {
-    const float2 f = p.drawn[(int64_t)b * p.pieces + i];
-    two = both(two, Two{f.x, f.y, p.drawn_token[(int64_t)b * p.pieces + i]});
+    const f32x4 f = p.drawn[(int64_t)b * p.pieces + i];
+    key = both(key, Key{f[0], f[1], f[2], __float_as_int(f[3])});
   }
   const Left left = p.left[b];
   if (left.at < 0) return;
-  two = wave_two(two);
-  if (lane == 0) twos[wv] = two;
+  key = wave_key(key);
+  if (lane == 0) keys[wv] = key;
   __syncthreads();
-  two = twos[0];
+  key = keys[0];
 #pragma unroll
-  for (int w = 1; w < kThreads / 64; ++w) two = both(two, twos[w]);
-  // (NaN and nothing at all look alike: nothing has been larger than zero)
-  if (two.token != INT32_MAX && two.best - two.second > 0x1p-16f * two.best) {
-    if (tid == 0) p.next[b] = two.token;
+  for (int w = 1; w < kThreads / 64; ++w) key = both(key, keys[w]);
+  // (NaN and nothing at all look alike: nothing has been larger than zero.  Exponentials below fp32's numbers, 2^-126, have counted for nothing: with noise of up to 40 they stay below 2^-68.)
+  if (key.token != INT32_MAX && key.least > key.others && key.least > (float)left.scale * 0x1p-64f) {
+    if (tid == 0) p.next[b] = key.token;
     return;
   }
   const double by = inverse_temperature(p, b);
   const float top = left.top;
   const void* x_row = row_of_x<E>(p, b, left.at);
   const float *q_row = p.q + b * p.q_sb + left.at * p.q_st, *g_row = p.noise + b * p.noise_sb;
-  // Too near to be told apart, or nothing that fp32 holds: in 64 bits, and where nothing is left, from the row as it was.
+  // Too near to be told apart, or nothing that fp32 holds: in 64 bits, with a sum of the row that is, and where nothing is left, from the row as it was.
+  double first = left.scale;
+  if (!left.exact && left.less > 0.0) {
+    double sum = 0.0;
+    for (int v = tid; v < p.V; v += kThreads) sum += exp(((double)score_at<E>(x_row, v) - (double)top) * by);
+    sum = wave_sum64(sum);
+    if (lane == 0) sums[wv] = sum;
+    __syncthreads();
+    first = 1.0 / ((sums[0] + sums[1]) + (sums[2] + sums[3]));
+  }
   for (int whole = 0; whole < 2; ++whole) {
-    const double scale = whole ? 1.0 : left.scale, less = whole ? 0.0 : left.less;      // (a factor of all of them decides nothing)
+    const double scale = whole ? 1.0 : first, less = whole ? 0.0 : left.less;      // (a factor of all of them decides nothing)
     Best best = {-__builtin_inf(), INT32_MAX};
     for (int v = tid; v < p.V; v += kThreads) {
       const double rest = scale * exp(((double)score_at<E>(x_row, v) - (double)top) * by) - less * (double)q_row[v];
@@ -797,13 +890,14 @@ template <int E> static void verify_launch(const VerifyParams& p, int rounds, hi
 
 using namespace daisy;
 
+static_assert(sizeof(Left) % 16 == 0, "the pieces behind them are read 16 bytes at a time");
 static bool verify_shape_ok(int B, int T, int V) { return B > 0 && B <= 65535 && T > 0 && T <= kMostNodes && V > 0 && V < (1 << 30); }
 
 extern "C" size_t daisy_verify_workspace_bytes(int B, int T, int V) {
   if (!verify_shape_ok(B, T, V)) return 0;
   const VerifySplit s = verify_split(B, T, V);
-  const size_t parts = (size_t)B * T * s.slices * (sizeof(f32x4) + sizeof(int32_t));      // (then each sequence's, a multiple of 8)
-  return (parts + 15) / 16 * 16 + (size_t)B * sizeof(Left) + (size_t)B * s.pieces * (sizeof(float2) + sizeof(int32_t));
+  const size_t parts = (size_t)B * T * s.slices * (sizeof(f32x4) + sizeof(int32_t));      // (then each sequence's, a multiple of 16)
+  return (parts + 15) / 16 * 16 + (size_t)B * sizeof(Left) + (size_t)B * s.pieces * sizeof(f32x4);
 }
 
 extern "C" int daisy_verify_fwd(const void* logits, const int64_t* logits_strides, int type, const void* tokens, int64_t tokens_stride, int tokens_are_int64,
@@ -841,8 +935,7 @@ extern "C" int daisy_verify_fwd(const void* logits, const int64_t* logits_stride
   p.part = (f32x4*)workspace;
   p.part_token = (int32_t*)(p.part + parts);
   p.left = (Left*)((char*)workspace + (parts * (sizeof(f32x4) + sizeof(int32_t)) + 15) / 16 * 16);
-  p.drawn = (float2*)(p.left + B);
-  p.drawn_token = (int32_t*)(p.drawn + (size_t)B * sp.pieces);
+  p.drawn = (f32x4*)(p.left + B);
   p.B = B; p.T = T; p.V = V; p.slices = sp.slices; p.slice = sp.slice; p.rows = sp.rows; p.pieces = sp.pieces;
   hipStream_t s = (hipStream_t)stream;
   if (type == kScoreF32) verify_launch<kScoreF32>(p, sp.rounds, s);
