@@ -56,10 +56,10 @@ struct Left { double scale, less; int at; float top; int exact, unused; };
 // Of some of a row: the largest of what the keys may be at most, what that one is at least, the largest of the others', and the token.
 struct Key { float most, least, others; int token; };
 
-// 1 / t, 0 where the likeliest token is wanted
+// 1 / t; 0 where the likeliest token is wanted, NaN where nothing can follow: a row's temperature that is not finite
 __device__ __forceinline__ double inverse_temperature(const VerifyParams& p, int b) {
   const double t = p.temperatures != nullptr ? (double)p.temperatures[b] : p.temperature;
-  return t > 0.0 ? fmin(1.0 / t, 1e300) : 0.0;
+  return t <= 0.0 ? 0.0 : t <= (double)FLT_MAX ? fmin(1.0 / t, 1e300) : __builtin_nan("");
 }
 __device__ __forceinline__ int nodes_of(const VerifyParams& p, int b) { return p.nodes != nullptr ? min(max(p.nodes[b], 0), p.T) : p.T; }
 // The token of node j (-1: none that the vocabulary has).
@@ -467,7 +467,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams 
         }
       } else {
         double left = row.sum;
-        const auto possible = [](double sum) { return sum > 0.0 && sum < __builtin_inf(); };      // (not NaN either)
+        const auto possible = [&](double sum) { return sum > 0.0 && sum < __builtin_inf() && by == by; };      // (not NaN either)
         if (any && !several && !(any & (any - 1))) {
           // one child, as in chains: no sums over lanes
           const int from = __builtin_ctzll(any);
@@ -649,8 +649,8 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyParams 
             x_j = lane_of(x[k], from);
           }
         }
-        if (!(greedy ? row.sum == row.sum : row.sum > 0.0 && row.sum < __builtin_inf())) {
-          walking = false;      // a row of scores that are none, or of nothing
+        if (!(greedy ? row.sum == row.sum : row.sum > 0.0 && row.sum < __builtin_inf() && by == by)) {
+          walking = false;      // a row of scores that are none, or of nothing; a temperature that is none
         } else if (greedy) {
           if (j < 0) token = row.token == INT32_MAX ? -1 : row.token;
           walking = j >= 0;

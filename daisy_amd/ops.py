@@ -1217,7 +1217,7 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Ten
 
     ``logits [B, T, V]`` (fp32, bf16 or fp16; any strides of the first two dims): row u says what may follow node u, ``p = softmax(logits[b, u] / temperature)``, -inf what may not (what
     ``process_logits`` or a filter has left).  ``tokens`` int64 or int32 ``[B, T]``: the nodes' tokens, of which node 0's is taken; ``parents``, ``nodes``: as for ``draft_tree``.
-    ``temperature``: a number or fp32 ``[B]``; zero: the likeliest token alone is accepted, and follows (of equal ones the lowest).
+    ``temperature``: a number or fp32 ``[B]``; zero (in rows, less too): the likeliest token alone is accepted, and follows (of equal ones the lowest).
 
     From node 0 on, the children of the node are tried in their order.  Child c, with token y, is accepted where ``accept[b, c] * (1 - what rejected children took of p) < p(y)``; its p is
     taken where it is rejected (a token that an earlier child had has none left).  Where none is accepted, the token that follows is drawn from what is left: the
@@ -1226,7 +1226,7 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Ten
     from p one by one.  ``accept`` fp32 ``[B, T]`` in [0, 1), ``noise`` fp32 ``[B, V]``, Gumbel (``generate.gumbel_noise``): the random numbers; not needed at temperature zero.
 
     Returns ``path`` int32 ``[B, T]`` (the accepted nodes from node 0 on, -1 behind them: an ``index`` for ``paged_move``), ``counts`` int32 ``[B]`` (how many) and the tokens that follow, int64 ``[B]``;
-    -1 where nothing may: a row that is -inf throughout beside its children, a row with NaN or +inf, no nodes.  Sums are held in 64 bits and do not depend on any order of atomics.
+    -1 where nothing may: a row that is -inf throughout beside its children, a row with NaN or +inf, a row's temperature that is NaN or +inf, no nodes.  Sums are held in 64 bits and do not depend on any order of atomics.
     ``workspace``: at least ``verify_drafts_workspace_bytes``, whatever it holds, for one call at a time; ``None``: a tensor made for the call.
     """
     fast = _lib.native().verify_drafts(logits, tokens, parents, nodes, temperature, accept, noise, draft, workspace)

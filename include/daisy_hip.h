@@ -618,11 +618,11 @@ int daisy_logits_process_fwd(const void* x, int64_t x_stride, void* y, int64_t y
  * logits     : [B, T, V], type 0 = fp32, 1 = bf16, 2 = fp16, strides {sequence, node}; -inf: a token that may not follow.
  * tokens     : int32 or int64 (tokens_are_int64) [B, T] with a row stride; a token outside 0 .. V - 1 is no candidate.
  * parents, nodes: as for daisy_draft_tree_fwd; a node that does not come from node 0 is never accepted.
- * temperature: a number, no larger than the largest of fp32, or, where temperature_rows is given, fp32 [B] (zero or less: the largest score).
+ * temperature: a number, no larger than the largest of fp32, or, where temperature_rows is given, fp32 [B] (zero or less: the largest score; NaN or +inf: nothing follows).
  * accept     : fp32 [B, T] with a row stride, in [0, 1);  noise: fp32 [B, V] with a row stride, finite;  both may be NULL where temperature is the number 0.
  * draft      : fp32 [B, T, V], strides {sequence, node}, or NULL.
  * path       : int32 [B, T], the accepted nodes from node 0 on, -1 behind them;  counts: int32 [B], how many;  next: int64 [B], the token that follows, -1
- *              where nothing may: no score above -inf beside the children's, a score that is NaN or +inf, no nodes.
+ *              where nothing may: no score above -inf beside the children's, a score or a row's temperature that is NaN or +inf, no nodes.
  * The results share no memory with what the call reads.  workspace: daisy_verify_workspace_bytes(...) bytes, 16-byte aligned, of no other call that may
  * run at the same time.
  */
