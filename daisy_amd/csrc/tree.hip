@@ -513,7 +513,7 @@ __global__ __launch_bounds__(256, 1) void tree_attn_kernel(TreeParams p) {
         for (int r = 0; r < 8; ++r) f[r] = s[r] - f[r];
         pl[t] = pack8_as<F16>(f);
       }
-      // ---- values that are not finite leave the product; who sees one of a channel gets NaN there
+      // ---- values that are not finite leave the product; who sees one of a channel gets NaN there (in a tile that all see whole they stay in it, and the channel becomes not finite for all)
       auto v_operand = [&](int j) {
         const int d = (j / W) * (W / 2) + (j % W) / 2;
         u32x4 vf;
@@ -863,7 +863,7 @@ __global__ __launch_bounds__(64 * NW, wide_waves_per_simd(D)) void tree_wide_ker
         const uint32_t vis = visible(p, e, mask, of.node, lo, tile) >> (4 * c);
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = vis >> (8 * (r >> 2) + (r & 3)) & 1 ? s[r] : -__builtin_inff();
-        // values that are not finite leave the tile; who sees one of a channel gets NaN there
+        // values that are not finite leave the tile; who sees one of a channel gets NaN there (in a tile that all see whole they stay, and the channel becomes not finite for all)
         uint32_t most = 0;
         u32x4 __attribute__((address_space(3)))* vs = (u32x4 __attribute__((address_space(3)))*)(size_t)(lds_address(staged) + 2 * TILE + 4 * TILE * slot);
 #pragma unroll

@@ -1154,8 +1154,8 @@ def paged_tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.
     (int32 ``[B, T, ceil(T / 32)]``, see ``draft_tree``; any set of nodes) has; with ``window``, the last ``window`` of these, in the order of the cache.  ``nodes`` int32 ``[B]``: as for
     ``draft_tree``; the rows of the others become zero.  Returns ``o [B, T, Hq, D]``, or ``out``, as ``paged_attention`` does.
 
-    Rows of a page that no node sees may hold anything.  A value that is not finite makes its channel NaN for the nodes that see it and the heads that share it; the others
-    do not feel it.
+    Rows of a page that no node sees may hold anything.  A value that is not finite makes its channel not finite for the nodes that see it and the heads that share it (an infinity may
+    come out as NaN); the others do not feel it.
 
     Lengths, nodes, mask and table are read when the kernels run.  ``workspace``: at least ``paged_tree_attention_workspace_bytes``, as for ``paged_attention``.  A tree that goes beyond the
     table's room, or a page that is none, gives NaN for the heads of that sequence and raises a bit in ``status``.

@@ -551,7 +551,7 @@ int daisy_draft_tree_fwd(const int32_t* parents, int64_t parents_stride, const i
  * over the places t < lens[b] and lens[b] + j for the bits j of node i's mask (int32 [B, T, ceil(T / 32)], strides {batch, node}), i itself among
  * them whatever its bit; with window > 0 the last `window` of these, in the order of the places.  q, o: [B, T, Hq, D] with {batch, node, head} strides; types, pages and table
  * as for daisy_paged_attn_fwd.  Rows of o for nodes that there are not become zero.  Rows of a page that no node sees may hold anything; a value that is
- * not finite makes its channel NaN for the nodes that see it, and for those alone.  workspace: daisy_paged_tree_attn_workspace_bytes(...) bytes, 16-byte aligned, of no
+ * not finite makes its channel not finite (NaN, it may be) for the nodes that see it, and for those alone.  workspace: daisy_paged_tree_attn_workspace_bytes(...) bytes, 16-byte aligned, of no
  * other call that may run at the same time.
  */
 size_t daisy_paged_tree_attn_workspace_bytes(int B, int T, int Hq, int H, int D, int max_pages, int page_size);
