@@ -400,7 +400,7 @@ class Generator:
         each one follows, -1 for the last token seen.  One step (``core.draft_step``) then runs all of them, and those that the model's own choice agrees with
         (``ops.verify_drafts``) are kept, with a token that follows them: greedily the tokens are those without drafts (but for near ties: a product over more rows rounds
         otherwise), drawn ones have the distribution that they have without.  Penalties and masks depend on the tokens ahead of each draft and are refused.
-        ``record_steps`` records for each M anew: a tree of one size is recorded once.
+        ``record_steps`` records for each M anew: a tree of one size is recorded once.  A row that takes n more tokens looks at the first n - 1 of its drafts alone, so the best ones come first.
         """
         from . import core
         assert len(prompts) > 0 and all(p.ndim == 1 and p.numel() > 0 for p in prompts) and max_new_tokens > 0
