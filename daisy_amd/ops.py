@@ -1226,7 +1226,11 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Ten
     from p one by one.  ``accept`` fp32 ``[B, T]`` in [0, 1), ``noise`` fp32 ``[B, V]``, Gumbel (``generate.gumbel_noise``): the random numbers; not needed at temperature zero.
 
     Returns ``path`` int32 ``[B, T]`` (the accepted nodes from node 0 on, -1 behind them: an ``index`` for ``paged_move``), ``counts`` int32 ``[B]`` (how many) and the tokens that follow, int64 ``[B]``;
-    -1 where nothing may: a row that is -inf throughout beside its children, a row with NaN or +inf, a row's temperature that is NaN or +inf, no nodes.  Sums are held in 64 bits and do not depend on any order of atomics.
+    -1 where nothing may: a row that is -inf throughout beside its children, a row with NaN or +inf, a row's temperature that is NaN or +inf, no nodes.
+
+    Temperature zero compares the scores as they are.  Otherwise sums of exponentials are fp32 within up to 1024 tokens and 64 bits beyond them, within 2^-17 of themselves: so near are the probabilities that a child is accepted
+    with.  What rejections of drawn children leave is held in 64 bits, however little it is, and the token that follows is looked for in 64 bits where fp32 does not tell it.  The same call gives the same results.
+
     ``workspace``: at least ``verify_drafts_workspace_bytes``, whatever it holds, for one call at a time; ``None``: a tensor made for the call.
     """
     fast = _lib.native().verify_drafts(logits, tokens, parents, nodes, temperature, accept, noise, draft, workspace)
