@@ -494,14 +494,12 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams 
             e[k] = 0.0;
             if (kids[k] == 0) continue;
             bool twice = false;
-            if (several || (any & (any - 1))) {
 #pragma unroll
-              for (int g = 0; g <= k; ++g)
-                for (uint64_t todo = kids[g]; todo; todo &= todo - 1) {
-                  const int from = __builtin_ctzll(todo);
-                  twice |= __builtin_amdgcn_readlane(t.token[g], from) == t.token[k] && 64 * g + from < 64 * k + lane;
-                }
-            }
+            for (int g = 0; g <= k; ++g)
+              for (uint64_t todo = kids[g]; todo; todo &= todo - 1) {
+                const int from = __builtin_ctzll(todo);
+                twice |= __builtin_amdgcn_readlane(t.token[g], from) == t.token[k] && 64 * g + from < 64 * k + lane;
+              }
             if ((kids[k] >> lane & 1) && !twice) e[k] = x[k] > -__builtin_inff() ? exp_of(((double)x[k] - ref) * by) : x[k] == x[k] ? 0.0 : (double)x[k];
             of_kids += e[k];
           }
