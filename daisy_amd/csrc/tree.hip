@@ -1096,8 +1096,8 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeParams p) {
 
 // Up to 16 columns a wavefront by itself, up to 32 too where its registers hold them (D < 256), else workgroups of 64 columns, of 128 or of 256; as many workgroups as the chip holds
 // at once, fewer where there are fewer tiles.  A workgroup of 256 reads a tile once for what two of 128 read it twice: 150 us against 162 when it was tried (12 sequences of 100 to 24000, 8 key
-// heads of 8 query heads, 32 nodes, D = 128), 305 against 332 (32 of 8000, 4 query heads, 64 nodes, D = 64).  D = 256 leaves room for one wavefront a SIMD: four, although half of them have
-// no column, take 332 us for what two take 446 for (16 of 8000, 64 columns), because twice as many copies are on their way.
+// heads of 8 query heads, 32 nodes, D = 128), 305 against 332 (32 of 8000, 4 query heads, 64 nodes, D = 64; with the later steps 278).  D = 256 leaves room for one wavefront a SIMD: four, although half of them have
+// no column, take 332 us for what two take 446 for (16 of 8000, 64 columns; with the later steps 301), because twice as many copies are on their way.
 struct TreeSplit { int groups, cols, blocks, NC, NW; size_t lds; };      // NC: pieces of 16 columns of a wavefront, or 0 and NW: wavefronts of 32
 static TreeSplit tree_split(int B, int T, int H, int G, int D, int64_t capacity) {
   TreeSplit s = {};

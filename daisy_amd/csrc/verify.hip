@@ -414,7 +414,7 @@ __device__ __forceinline__ double lane_of(double x, int lane) {
 __device__ __forceinline__ float lane_of(float x, int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane)); }
 
 // A workgroup per sequence: its wavefronts join the slices of the rows, one of them walks.  Latency: 5 us for a tree of 8 nodes, 8 to 9 for 32 of 16.
-constexpr int kWalkThreads = 1024;      // at most: a row of the tree for each wavefront, where there are so many (32 trees of 16 nodes 25.8 us, with 512 27.0; one of 8 9.5, with 1024 9.8)
+constexpr int kWalkThreads = 1024;      // at most: a row of the tree for each wavefront, where there are so many (both kernels, over 50257 tokens, 512 and 1024 threads: one tree of 9 nodes 10.2 and 9.1 us, of 16 11.0 and 10.0, of 64 22.3 and 18.3, 32 of 9 26.2 and 25.1, of 16 35.2 and 34.2; of 8 and fewer, and over 5000 tokens, level or better)
 template <int E, int MODE>
 __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams p) {
   __shared__ RowPart rows[kMostNodes];
@@ -848,7 +848,9 @@ __global__ __launch_bounds__(kThreads) void verify_last_kernel(VerifyParams p) {
   }
 }
 
-// The slices: as long as leaves the chip enough wavefronts, and then as many rows to a workgroup, which share the noise, as leave it 4096 (32 trees of 16 nodes over 50257 tokens: 27.3 us; 16384 28.7, 8192 29.1, 2048 28.7).
+// The slices: as long as leaves the chip enough wavefronts, and then as many rows to a workgroup, which share the noise, as leave it 4096.  Chosen drafts with 2048, 4096, 8192 and 16384 wavefronts, in us: 32 trees of 16 nodes over 50257 tokens 35.4, 34.2, 35.2, 36.4;
+// 16 of 64 nodes 62.9, 58.5, 55.3, 56.2; 8 of 32 over 131072 (bf16) 41.1, 33.2, 32.3, 33.7; 128 of 5 over 32000 26.0, 26.0, 30.6, 27.6; 128 of 16 over 8000 (bf16) 30.4, 25.6, 24.5, 26.1.  Fewer lose up to a quarter, more up to a sixth, and 8192 is better by
+// 6 % at most; drawn ones are level.
 struct VerifySplit { int rounds, slice, slices, rows, pieces; };
 static VerifySplit verify_split(int B, int T, int V) {
   VerifySplit s;
